@@ -362,6 +362,119 @@ int popkv_dense_attention(const void* queries, int32_t dtype,
                           int64_t q_heads, int64_t kv_heads, int64_t tokens, void* output,
                           void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- paged 4-bit K/V cache ------------------------------------------------
+ * No counterpart in the reference, whose caches are one sequence's 16- or
+ * 32-bit rows (popkv.py:105-111).
+ *
+ * The pool of a model, head_dim 128:
+ *   codes   uint8 [layers, pages, KVH, P, 2, 64]: a token's K row, then its V
+ *           row; byte j holds dims 2j (low nibble) and 2j + 1.
+ *   scales  fp16 [layers, pages, KVH, P, 2, R, 2]: (low, delta) of each of the
+ *           R = 128 / G dimension groups (G 16, 32 or 64).
+ * A value is low + code * delta.  low = fp16(min of the group), delta =
+ * fp16((max - low) / 15), code = (x - low) / delta rounded to the nearest
+ * integer in 0 .. 15, ties to even (0 where delta is 0); the extrema are held
+ * in +-57344, and a group with a NaN or an infinity reads back as NaN.
+ * P = page_tokens is 32, 64, 128 or 256.
+ *
+ * The page table of a batch, shared by the layers:
+ *   table   int32 [batch, width]: the page of every P tokens; an entry outside
+ *           [0, pages) is no page, its tokens are not there.
+ *   counts  int64 [batch] IN DEVICE MEMORY: cached tokens (held in [0, width *
+ *           P] by every call).
+ *   refs    int32 [pages]: how often a page is held; 0 is free.  A program may
+ *           hold pages of its own accord (a kept prefix) by adding to refs.
+ * A page that a sequence still fills belongs to it alone; full pages may be
+ * shared.  `status` (device int32, may be NULL) collects bits: 1 a sequence
+ * has no table entry left, 4 the pool has no page left or a token's page is
+ * missing, 8 a parent outside the batch. */
+
+/* Quantises rows k / v [batch, KVH, rows, 128] (strides in elements, rows of
+ * 128 contiguous; 16-byte aligned) of one layer into the pages: row t of
+ * sequence b at position counts[b] + t, for t < tokens[b] (device, NULL: every
+ * row).  codes / scales: that layer's.  The pages must be there
+ * (popkv_page_reserve); a row without one writes nothing and sets status. */
+int popkv_paged_write(const void* k, const void* v, int32_t dtype, int64_t k_batch_stride, int64_t k_head_stride,
+                      int64_t k_token_stride, int64_t v_batch_stride, int64_t v_head_stride, int64_t v_token_stride,
+                      int64_t rows, const int64_t* tokens, void* codes, void* scales, int64_t pages, int64_t kv_heads,
+                      int32_t page_tokens, int32_t dim_group_size, const int32_t* table, int64_t width,
+                      const int64_t* counts, int64_t batch, int32_t* status, void* stream);
+
+/* The inverse: rows [0, min(rows, counts[b])) of one layer's sequences as
+ * contiguous k / v [batch, KVH, rows, 128].  Rows past a count are zeroed with
+ * fill, else left as they are; a cached row whose page is missing is zero. */
+int popkv_paged_read(void* k, void* v, int32_t dtype, int64_t rows, int32_t fill, const void* codes, const void* scales,
+                     int64_t pages, int64_t kv_heads, int32_t page_tokens, int32_t dim_group_size,
+                     const int32_t* table, int64_t width, const int64_t* counts, int64_t batch, void* stream);
+
+/* Dense attention of one decode step of one layer: output[b, i] = softmax(q .
+ * [K; k] / sqrt(128)) . [V; v] over sequence b's cached tokens and its current
+ * token (current_k / current_v [batch, KVH, 128], not cached yet); queries,
+ * output [batch, QH, 128], query head i on KV head i / (QH / KVH), 1 to 16
+ * query heads per KV head.  max_tokens (host) bounds every count and sizes the
+ * launch; a larger count is taken as max_tokens.  Tokens without a page are
+ * left out.  Workspace: popkv_paged_attention_workspace_bytes() bytes, 16-byte
+ * aligned, whose first batch * KVH * 4 bytes (the merge tickets) are zero on
+ * entry and left zero.  One launch. */
+size_t popkv_paged_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t max_tokens);
+int popkv_paged_attention(const void* queries, int32_t dtype, const void* codes, const void* scales, int64_t pages,
+                          int64_t kv_heads, int32_t page_tokens, int32_t dim_group_size, const int32_t* table,
+                          int64_t width, const int64_t* counts, int64_t batch, int64_t max_tokens,
+                          const void* current_k, const void* current_v, int64_t q_heads, void* output, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* The same over a selection: indices [batch, QH, selected] int64 or int32.  An
+ * index equal to counts[b] is the current token; one outside [0, counts[b]]
+ * (-1 pads a short row) or with valid_mask 0 is left out, one named twice
+ * counts twice, and a row with nothing left is zero.  head_to_kv [QH] int64
+ * (entries are clamped to [0, KVH)).  Workspace as above, its first batch * QH
+ * * 4 bytes zero. */
+size_t popkv_paged_indexed_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t selected);
+int popkv_paged_indexed_attention(const void* queries, int32_t dtype, const void* codes, const void* scales,
+                                  int64_t pages, int64_t kv_heads, int32_t page_tokens, int32_t dim_group_size,
+                                  const int32_t* table, int64_t width, const int64_t* counts, int64_t batch,
+                                  const void* current_k, const void* current_v, const void* indices,
+                                  int32_t index_dtype, const uint8_t* valid_mask, const int64_t* head_to_kv,
+                                  int64_t q_heads, int64_t selected, void* output, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
+/* Page bookkeeping.  Each call reads a page table (table_in, counts_in,
+ * refs_in) and writes another, or the same one (all three outputs the inputs,
+ * or none of them).  Pages are taken lowest first.  The workspace's content
+ * does not matter.
+ *
+ * reserve: every sequence gets the pages that tokens[b] (device; NULL: `each`)
+ * more tokens need, sequences in order; one whose share the pool or the table
+ * does not hold gets none and sets status.  counts are as they were. */
+size_t popkv_page_reserve_workspace_bytes(int64_t batch, int64_t pages);
+int popkv_page_reserve(const int32_t* table_in, const int64_t* counts_in, const int32_t* refs_in, int32_t* table,
+                       int64_t* counts, int32_t* refs, int64_t width, int64_t batch, int64_t pages,
+                       int32_t page_tokens, const int64_t* tokens, int64_t each, int32_t* status, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* fork: sequence b becomes a copy of sequence parents[b] (int64 [batch],
+ * device; all at once, from the old table), or empty for -1 (its pages are
+ * given back; any other value outside the batch empties it too and sets
+ * status).  Full pages are shared.  The open page, and pages reserved behind
+ * it, stay with the parent's lowest child; every other child gets a copy of
+ * the open page in all `layers` (codes / scales: the whole pool).  A child for
+ * whose copy the pool has no page is left empty and sets status. */
+size_t popkv_page_fork_workspace_bytes(int64_t batch, int64_t width);
+int popkv_page_fork(void* codes, void* scales, int64_t layers, int64_t pages, int64_t kv_heads, int32_t page_tokens,
+                    int32_t dim_group_size, const int32_t* table_in, const int64_t* counts_in, const int32_t* refs_in,
+                    int32_t* table, int64_t* counts, int32_t* refs, int64_t width, int64_t batch,
+                    const int64_t* parents, int32_t* status, void* workspace, size_t workspace_bytes, void* stream);
+
+/* compact: the n pages with refs > 0 end in places 0 .. n - 1: those at n or
+ * later move, in order, to the free places before n, in order, in all layers.
+ * page_map int32 [pages]: the place of every such page, -1 for free ones (for
+ * whoever holds pages outside this table). */
+size_t popkv_page_compact_workspace_bytes(int64_t pages);
+int popkv_page_compact(void* codes, void* scales, int64_t layers, int64_t pages, int64_t kv_heads, int32_t page_tokens,
+                       int32_t dim_group_size, const int32_t* table_in, const int64_t* counts_in,
+                       const int32_t* refs_in, int32_t* table, int64_t* counts, int32_t* refs, int64_t width,
+                       int64_t batch, int32_t* page_map, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

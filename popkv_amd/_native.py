@@ -73,6 +73,26 @@ _SIGNATURES = {
     "popkv_dense_attention_workspace_bytes": (_c_size, [_c_i64, _c_i64]),
     "popkv_dense_attention": (ctypes.c_int, [_vp, _c_i32, _vp, _vp, _c_i64, _c_i64, _vp, _vp, _c_i64, _c_i64,
                                              _c_i64, _vp, _vp, _c_size, _vp]),
+    "popkv_paged_write": (ctypes.c_int, [_vp, _vp, _c_i32, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp,
+                                         _vp, _vp, _c_i64, _c_i64, _c_i32, _c_i32, _vp, _c_i64, _vp, _c_i64, _vp, _vp]),
+    "popkv_paged_read": (ctypes.c_int, [_vp, _vp, _c_i32, _c_i64, _c_i32, _vp, _vp, _c_i64, _c_i64, _c_i32, _c_i32, _vp,
+                                        _c_i64, _vp, _c_i64, _vp]),
+    "popkv_paged_attention_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64, _c_i64]),
+    "popkv_paged_attention": (ctypes.c_int, [_vp, _c_i32, _vp, _vp, _c_i64, _c_i64, _c_i32, _c_i32, _vp, _c_i64, _vp,
+                                             _c_i64, _c_i64, _vp, _vp, _c_i64, _vp, _vp, _c_size, _vp]),
+    "popkv_paged_indexed_attention_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64]),
+    "popkv_paged_indexed_attention": (ctypes.c_int, [_vp, _c_i32, _vp, _vp, _c_i64, _c_i64, _c_i32, _c_i32, _vp, _c_i64,
+                                                     _vp, _c_i64, _vp, _vp, _vp, _c_i32, _vp, _vp, _c_i64, _c_i64, _vp,
+                                                     _vp, _c_size, _vp]),
+    "popkv_page_reserve_workspace_bytes": (_c_size, [_c_i64, _c_i64]),
+    "popkv_page_reserve": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i32, _vp, _c_i64, _vp,
+                                          _vp, _c_size, _vp]),
+    "popkv_page_fork_workspace_bytes": (_c_size, [_c_i64, _c_i64]),
+    "popkv_page_fork": (ctypes.c_int, [_vp, _vp, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _vp, _vp, _vp, _vp, _vp, _vp,
+                                       _c_i64, _c_i64, _vp, _vp, _vp, _c_size, _vp]),
+    "popkv_page_compact_workspace_bytes": (_c_size, [_c_i64]),
+    "popkv_page_compact": (ctypes.c_int, [_vp, _vp, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _vp, _vp, _vp, _vp, _vp, _vp,
+                                          _c_i64, _c_i64, _vp, _vp, _c_size, _vp]),
 }
 
 

@@ -832,3 +832,319 @@ int popkv_dense_attention(const void* queries, int32_t dtype, const void* prefix
 }
 
 }  // extern "C"
+
+// ---- paged 4-bit K/V cache -------------------------------------------------
+
+namespace {
+
+constexpr int64_t kMaxPages = int64_t{1} << 30;
+
+bool valid_page_tokens(int32_t p) { return p == 32 || p == 64 || p == 128 || p == 256; }
+int log2_of(int32_t p) { return __builtin_ctz(static_cast<unsigned>(p)); }
+
+int check_pool(const void* codes, const void* scales, int64_t pages, int64_t kv_heads, int32_t page_tokens,
+               int32_t dim_group_size) {
+    if (!codes || !scales) return fail(POPKV_ERR_INVALID, "null pointer");
+    if (pages <= 0 || pages > kMaxPages || kv_heads <= 0 || kv_heads > 65535)
+        return fail(POPKV_ERR_INVALID, "bad page or KV head count");
+    if (!valid_page_tokens(page_tokens)) return fail(POPKV_ERR_INVALID, "page_tokens must be 32, 64, 128 or 256");
+    if (!valid_group(dim_group_size)) return fail(POPKV_ERR_INVALID, "dim_group_size must be 16, 32, or 64");
+    if (!aligned16(codes) || !aligned16(scales)) return fail(POPKV_ERR_UNSUPPORTED, "the pool needs 16-byte alignment");
+    return POPKV_OK;
+}
+
+int check_table(const void* table, const void* counts, int64_t width, int64_t batch) {
+    if (!table || !counts) return fail(POPKV_ERR_INVALID, "null pointer");
+    if (batch <= 0 || batch > 65535 || width <= 0 || width > (int64_t{1} << 24) || batch * width > (int64_t{1} << 30))
+        return fail(POPKV_ERR_INVALID, "bad batch or page table width");
+    return POPKV_OK;
+}
+
+popkv::PagedView paged_view(void* codes, void* scales, int64_t pages, int64_t kv_heads, int32_t page_tokens,
+                            const int32_t* table, int64_t width, const int64_t* counts, int64_t batch) {
+    return {static_cast<char*>(codes), static_cast<uint32_t*>(scales), table, counts, pages, width,
+            static_cast<int>(batch), static_cast<int>(kv_heads), log2_of(page_tokens)};
+}
+
+popkv::PageMoves page_moves(void* codes, void* scales, int64_t layers, int64_t pages, int64_t kv_heads,
+                            int32_t page_tokens, int32_t dim_group_size) {
+    popkv::PageMoves m{};
+    m.codes = static_cast<char*>(codes);
+    m.scales = static_cast<char*>(scales);
+    m.layers = layers;
+    m.pages = pages;
+    m.code_bytes = kv_heads * page_tokens * 128;
+    m.scale_bytes = kv_heads * page_tokens * 8 * (128 / dim_group_size);
+    m.code_parts = ceil_div(m.code_bytes, popkv::kMoveBytes);
+    m.parts = m.code_parts + ceil_div(m.scale_bytes, popkv::kMoveBytes);
+    return m;
+}
+
+// Carves 256-byte aligned pieces out of a workspace (sizes only when null).
+struct Carve {
+    char* base;
+    size_t off = 0;
+    template <typename T>
+    T* take(int64_t n) {
+        T* p = base ? reinterpret_cast<T*>(base + off) : nullptr;
+        off = align_up(off + static_cast<size_t>(n) * sizeof(T));
+        return p;
+    }
+};
+
+void carve_reserve(Carve& c, popkv::PageReserve& a) {
+    a.need = c.take<int32_t>(a.batch + 1);
+    a.list = c.take<int32_t>(a.pages);
+}
+void carve_fork(Carve& c, popkv::PageFork& a) {
+    a.rows = c.take<int32_t>(a.batch * a.width);
+    a.new_counts = c.take<int64_t>(a.batch);
+    a.need = c.take<int32_t>(a.batch + 1);
+    a.source = c.take<int32_t>(a.batch);
+    a.list = c.take<int32_t>(a.batch);
+    a.pairs = c.take<int2>(a.batch);
+    a.moves = c.take<int32_t>(1);
+}
+void carve_compact(Carve& c, popkv::PageCompact& a) {
+    a.pairs = c.take<int2>(a.pages / 2 + 1);
+    a.moves = c.take<int32_t>(1);
+}
+
+size_t attend_tickets(int64_t rows) { return align_up(static_cast<size_t>(rows) * 4); }
+
+}  // namespace
+
+extern "C" {
+
+int popkv_paged_write(const void* k, const void* v, int32_t dtype, int64_t k_batch_stride, int64_t k_head_stride,
+                      int64_t k_token_stride, int64_t v_batch_stride, int64_t v_head_stride, int64_t v_token_stride,
+                      int64_t rows, const int64_t* tokens, void* codes, void* scales, int64_t pages, int64_t kv_heads,
+                      int32_t page_tokens, int32_t dim_group_size, const int32_t* table, int64_t width,
+                      const int64_t* counts, int64_t batch, int32_t* status, void* stream) {
+    int st = check_pool(codes, scales, pages, kv_heads, page_tokens, dim_group_size);
+    if (st) return st;
+    if ((st = check_table(table, counts, width, batch))) return st;
+    if (!k || !v) return fail(POPKV_ERR_INVALID, "null pointer");
+    if (!valid_dtype(dtype)) return fail(POPKV_ERR_INVALID, "keys and values must be fp32/fp16/bf16");
+    if (rows < 0 || rows > (int64_t{1} << 30)) return fail(POPKV_ERR_INVALID, "bad row count");
+    if (rows == 0) return POPKV_OK;
+    const int64_t es = static_cast<int64_t>(elem_size(dtype));
+    const int64_t strides[] = {k_batch_stride, k_head_stride, k_token_stride, v_batch_stride, v_head_stride,
+                               v_token_stride};
+    for (int64_t x : strides)
+        if (x < 0 || (x * es) % 16) return fail(POPKV_ERR_UNSUPPORTED, "rows written to pages need 16-byte alignment");
+    if (!aligned16(k) || !aligned16(v)) return fail(POPKV_ERR_UNSUPPORTED, "rows written to pages need 16-byte alignment");
+    const popkv::PagedWrite a{k,             v,    k_batch_stride, k_head_stride, k_token_stride, v_batch_stride,
+                              v_head_stride, v_token_stride, rows, tokens,        status};
+    return launched(popkv::launch_paged_write(a, paged_view(codes, scales, pages, kv_heads, page_tokens, table, width,
+                                                            counts, batch),
+                                              dtype, dim_group_size, as_stream(stream)),
+                    "popkv_paged_write");
+}
+
+int popkv_paged_read(void* k, void* v, int32_t dtype, int64_t rows, int32_t fill, const void* codes, const void* scales,
+                     int64_t pages, int64_t kv_heads, int32_t page_tokens, int32_t dim_group_size,
+                     const int32_t* table, int64_t width, const int64_t* counts, int64_t batch, void* stream) {
+    int st = check_pool(codes, scales, pages, kv_heads, page_tokens, dim_group_size);
+    if (st) return st;
+    if ((st = check_table(table, counts, width, batch))) return st;
+    if (!k || !v) return fail(POPKV_ERR_INVALID, "null pointer");
+    if (!valid_dtype(dtype)) return fail(POPKV_ERR_INVALID, "keys and values must be fp32/fp16/bf16");
+    if (rows < 0 || rows > (int64_t{1} << 30)) return fail(POPKV_ERR_INVALID, "bad row count");
+    if (!aligned16(k) || !aligned16(v)) return fail(POPKV_ERR_UNSUPPORTED, "rows read from pages need 16-byte alignment");
+    if (rows == 0) return POPKV_OK;
+    const popkv::PagedRead a{k, v, rows, fill};
+    return launched(popkv::launch_paged_read(a, paged_view(const_cast<void*>(codes), const_cast<void*>(scales), pages,
+                                                           kv_heads, page_tokens, table, width, counts, batch),
+                                             dtype, dim_group_size, as_stream(stream)),
+                    "popkv_paged_read");
+}
+
+size_t popkv_paged_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t max_tokens) {
+    if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || max_tokens < 0) return 0;
+    return attend_tickets(batch * kv_heads) +
+           align_up(static_cast<size_t>(popkv::paged_dense_items(batch, kv_heads, max_tokens) * q_heads * (128 + 2)) * 4);
+}
+
+int popkv_paged_attention(const void* queries, int32_t dtype, const void* codes, const void* scales, int64_t pages,
+                          int64_t kv_heads, int32_t page_tokens, int32_t dim_group_size, const int32_t* table,
+                          int64_t width, const int64_t* counts, int64_t batch, int64_t max_tokens,
+                          const void* current_k, const void* current_v, int64_t q_heads, void* output, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+    int st = check_pool(codes, scales, pages, kv_heads, page_tokens, dim_group_size);
+    if (st) return st;
+    if ((st = check_table(table, counts, width, batch))) return st;
+    if (!queries || !current_k || !current_v || !output || !workspace) return fail(POPKV_ERR_INVALID, "null pointer");
+    if (!valid_dtype(dtype)) return fail(POPKV_ERR_INVALID, "tensors must be fp32/fp16/bf16");
+    if (q_heads <= 0 || q_heads > 65535 || q_heads % kv_heads != 0 || q_heads / kv_heads > 16)
+        return fail(POPKV_ERR_UNSUPPORTED, "paged attention supports 1 to 16 query heads per KV head");
+    if (max_tokens < 0 || max_tokens > (int64_t{1} << 30)) return fail(POPKV_ERR_TOKENS, "invalid token count");
+    if (workspace_bytes < popkv_paged_attention_workspace_bytes(batch, q_heads, kv_heads, max_tokens))
+        return fail(POPKV_ERR_WORKSPACE, "paged attention needs %zu workspace bytes",
+                    popkv_paged_attention_workspace_bytes(batch, q_heads, kv_heads, max_tokens));
+    if (!aligned16(workspace) || !aligned16(queries) || !aligned16(current_k) || !aligned16(current_v) || !aligned16(output))
+        return fail(POPKV_ERR_UNSUPPORTED, "paged attention tensors need 16-byte alignment");
+    char* ws = static_cast<char*>(workspace);
+    const popkv::PagedAttend a{queries, current_k, current_v, output, static_cast<int>(q_heads),
+                               reinterpret_cast<float*>(ws + attend_tickets(batch * kv_heads)),
+                               reinterpret_cast<uint32_t*>(ws)};
+    return launched(popkv::launch_paged_dense(a, paged_view(const_cast<void*>(codes), const_cast<void*>(scales), pages,
+                                                            kv_heads, page_tokens, table, width, counts, batch),
+                                              max_tokens, dtype, dim_group_size, as_stream(stream)),
+                    "popkv_paged_attention");
+}
+
+size_t popkv_paged_indexed_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t selected) {
+    if (batch <= 0 || q_heads <= 0 || selected <= 0) return 0;
+    const int64_t rows = batch * q_heads;
+    return attend_tickets(rows) +
+           align_up(static_cast<size_t>(rows * popkv::paged_indexed_splits(rows, selected) * (128 + 3)) * 4);
+}
+
+int popkv_paged_indexed_attention(const void* queries, int32_t dtype, const void* codes, const void* scales,
+                                  int64_t pages, int64_t kv_heads, int32_t page_tokens, int32_t dim_group_size,
+                                  const int32_t* table, int64_t width, const int64_t* counts, int64_t batch,
+                                  const void* current_k, const void* current_v, const void* indices,
+                                  int32_t index_dtype, const uint8_t* valid_mask, const int64_t* head_to_kv,
+                                  int64_t q_heads, int64_t selected, void* output, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+    int st = check_pool(codes, scales, pages, kv_heads, page_tokens, dim_group_size);
+    if (st) return st;
+    if ((st = check_table(table, counts, width, batch))) return st;
+    if (!queries || !current_k || !current_v || !indices || !head_to_kv || !output || !workspace)
+        return fail(POPKV_ERR_INVALID, "null pointer");
+    if (!valid_dtype(dtype)) return fail(POPKV_ERR_INVALID, "tensors must be fp32/fp16/bf16");
+    if (index_dtype != POPKV_INDEX_I64 && index_dtype != POPKV_INDEX_I32)
+        return fail(POPKV_ERR_INVALID, "indices must be int64 or int32");
+    if (q_heads <= 0 || q_heads > 65535) return fail(POPKV_ERR_INVALID, "empty or too many heads");
+    if (selected <= 0 || selected > (int64_t{1} << 30)) return fail(POPKV_ERR_INVALID, "bad selection size");
+    if (workspace_bytes < popkv_paged_indexed_attention_workspace_bytes(batch, q_heads, selected))
+        return fail(POPKV_ERR_WORKSPACE, "paged indexed attention needs %zu workspace bytes",
+                    popkv_paged_indexed_attention_workspace_bytes(batch, q_heads, selected));
+    if (!aligned16(workspace) || !aligned16(queries) || !aligned16(current_k) || !aligned16(current_v) || !aligned16(output))
+        return fail(POPKV_ERR_UNSUPPORTED, "paged attention tensors need 16-byte alignment");
+    char* ws = static_cast<char*>(workspace);
+    const popkv::PagedAttend a{queries, current_k, current_v, output, static_cast<int>(q_heads),
+                               reinterpret_cast<float*>(ws + attend_tickets(batch * q_heads)),
+                               reinterpret_cast<uint32_t*>(ws)};
+    const popkv::PagedIndexed ix{indices, index_dtype, valid_mask, head_to_kv, selected};
+    return launched(popkv::launch_paged_indexed(a, ix, paged_view(const_cast<void*>(codes), const_cast<void*>(scales),
+                                                                  pages, kv_heads, page_tokens, table, width, counts,
+                                                                  batch),
+                                                dtype, dim_group_size, as_stream(stream)),
+                    "popkv_paged_indexed_attention");
+}
+
+size_t popkv_page_reserve_workspace_bytes(int64_t batch, int64_t pages) {
+    if (batch <= 0 || pages <= 0) return 0;
+    Carve c{nullptr};
+    popkv::PageReserve a{};
+    a.batch = batch;
+    a.pages = pages;
+    carve_reserve(c, a);
+    return c.off;
+}
+
+int popkv_page_reserve(const int32_t* table_in, const int64_t* counts_in, const int32_t* refs_in, int32_t* table,
+                       int64_t* counts, int32_t* refs, int64_t width, int64_t batch, int64_t pages,
+                       int32_t page_tokens, const int64_t* tokens, int64_t each, int32_t* status, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+    int st = check_table(table_in, counts_in, width, batch);
+    if (st) return st;
+    if (!refs_in || !table || !counts || !refs || !workspace) return fail(POPKV_ERR_INVALID, "null pointer");
+    if (pages <= 0 || pages > kMaxPages) return fail(POPKV_ERR_INVALID, "bad page count");
+    if (!valid_page_tokens(page_tokens)) return fail(POPKV_ERR_INVALID, "page_tokens must be 32, 64, 128 or 256");
+    if (!tokens && each < 0) return fail(POPKV_ERR_INVALID, "bad token count");
+    if ((table == table_in) != (counts == counts_in) || (table == table_in) != (refs == refs_in))
+        return fail(POPKV_ERR_INVALID, "the outputs are the inputs or none of them");
+    if (workspace_bytes < popkv_page_reserve_workspace_bytes(batch, pages))
+        return fail(POPKV_ERR_WORKSPACE, "page reserve needs %zu workspace bytes",
+                    popkv_page_reserve_workspace_bytes(batch, pages));
+    if (!aligned16(workspace)) return fail(POPKV_ERR_UNSUPPORTED, "the workspace needs 16-byte alignment");
+    popkv::PageReserve a{table_in, counts_in, table, counts, refs, batch, width, pages, log2_of(page_tokens), tokens,
+                         each, status, nullptr, nullptr};
+    Carve c{static_cast<char*>(workspace)};
+    carve_reserve(c, a);
+    return launched(popkv::launch_page_reserve(a, refs_in, as_stream(stream)), "popkv_page_reserve");
+}
+
+size_t popkv_page_fork_workspace_bytes(int64_t batch, int64_t width) {
+    if (batch <= 0 || width <= 0) return 0;
+    Carve c{nullptr};
+    popkv::PageFork a{};
+    a.batch = batch;
+    a.width = width;
+    carve_fork(c, a);
+    return c.off;
+}
+
+int popkv_page_fork(void* codes, void* scales, int64_t layers, int64_t pages, int64_t kv_heads, int32_t page_tokens,
+                    int32_t dim_group_size, const int32_t* table_in, const int64_t* counts_in, const int32_t* refs_in,
+                    int32_t* table, int64_t* counts, int32_t* refs, int64_t width, int64_t batch,
+                    const int64_t* parents, int32_t* status, void* workspace, size_t workspace_bytes, void* stream) {
+    int st = check_pool(codes, scales, pages, kv_heads, page_tokens, dim_group_size);
+    if (st) return st;
+    if ((st = check_table(table_in, counts_in, width, batch))) return st;
+    if (!refs_in || !table || !counts || !refs || !parents || !workspace) return fail(POPKV_ERR_INVALID, "null pointer");
+    if (layers <= 0 || layers > 65535) return fail(POPKV_ERR_INVALID, "bad layer count");
+    if ((table == table_in) != (counts == counts_in) || (table == table_in) != (refs == refs_in))
+        return fail(POPKV_ERR_INVALID, "the outputs are the inputs or none of them");
+    if (workspace_bytes < popkv_page_fork_workspace_bytes(batch, width))
+        return fail(POPKV_ERR_WORKSPACE, "page fork needs %zu workspace bytes", popkv_page_fork_workspace_bytes(batch, width));
+    if (!aligned16(workspace)) return fail(POPKV_ERR_UNSUPPORTED, "the workspace needs 16-byte alignment");
+    popkv::PageFork a{table_in, counts_in, parents, refs, batch, width, pages, log2_of(page_tokens), status,
+                      nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
+    Carve c{static_cast<char*>(workspace)};
+    carve_fork(c, a);
+    popkv::PageMoves m = page_moves(codes, scales, layers, pages, kv_heads, page_tokens, dim_group_size);
+    m.moves = a.moves;
+    m.pairs = a.pairs;
+    m.table_in = a.rows;
+    m.table = table;
+    m.entries = batch * width;
+    m.counts_in = a.new_counts;
+    m.counts = counts;
+    m.batch = batch;
+    return launched(popkv::launch_page_fork(a, refs_in, m, as_stream(stream)), "popkv_page_fork");
+}
+
+size_t popkv_page_compact_workspace_bytes(int64_t pages) {
+    if (pages <= 0) return 0;
+    Carve c{nullptr};
+    popkv::PageCompact a{};
+    a.pages = pages;
+    carve_compact(c, a);
+    return c.off;
+}
+
+int popkv_page_compact(void* codes, void* scales, int64_t layers, int64_t pages, int64_t kv_heads, int32_t page_tokens,
+                       int32_t dim_group_size, const int32_t* table_in, const int64_t* counts_in,
+                       const int32_t* refs_in, int32_t* table, int64_t* counts, int32_t* refs, int64_t width,
+                       int64_t batch, int32_t* page_map, void* workspace, size_t workspace_bytes, void* stream) {
+    int st = check_pool(codes, scales, pages, kv_heads, page_tokens, dim_group_size);
+    if (st) return st;
+    if ((st = check_table(table_in, counts_in, width, batch))) return st;
+    if (!refs_in || !table || !counts || !refs || !page_map || !workspace) return fail(POPKV_ERR_INVALID, "null pointer");
+    if (layers <= 0 || layers > 65535) return fail(POPKV_ERR_INVALID, "bad layer count");
+    if ((table == table_in) != (counts == counts_in) || (table == table_in) != (refs == refs_in))
+        return fail(POPKV_ERR_INVALID, "the outputs are the inputs or none of them");
+    if (workspace_bytes < popkv_page_compact_workspace_bytes(pages))
+        return fail(POPKV_ERR_WORKSPACE, "page compact needs %zu workspace bytes", popkv_page_compact_workspace_bytes(pages));
+    if (!aligned16(workspace)) return fail(POPKV_ERR_UNSUPPORTED, "the workspace needs 16-byte alignment");
+    popkv::PageCompact a{refs_in, refs, page_map, pages, nullptr, nullptr};
+    Carve c{static_cast<char*>(workspace)};
+    carve_compact(c, a);
+    popkv::PageMoves m = page_moves(codes, scales, layers, pages, kv_heads, page_tokens, dim_group_size);
+    m.moves = a.moves;
+    m.pairs = a.pairs;
+    m.table_in = table_in;
+    m.map = page_map;
+    m.table = table;
+    m.entries = batch * width;
+    m.counts_in = counts_in;
+    m.counts = counts == counts_in ? nullptr : counts;
+    m.batch = batch;
+    return launched(popkv::launch_page_compact(a, m, as_stream(stream)), "popkv_page_compact");
+}
+
+}  // extern "C"

@@ -251,4 +251,125 @@ hipError_t launch_attention_dense(const void* queries, int dtype, const void* pr
                                   int kv_heads, float* partials, uint32_t* tickets, const void* current_k,
                                   const void* current_v, void* output, hipStream_t stream);
 
+// ---- paged 4-bit K/V cache (pages.hip, paged_attention.hip) ----------------
+// One layer of the pool and the batch's page table: codes [pages, KVH, P, 2,
+// 64] bytes, scales [pages, KVH, P, 2, R] (low, delta) fp16 pairs, table
+// [batch, width] (page of every P = 2^page_log2 tokens; outside [0, pages):
+// none), counts [batch] cached tokens.
+struct PagedView {
+    char* codes;
+    uint32_t* scales;
+    const int32_t* table;
+    const int64_t* counts;
+    int64_t pages, width;
+    int batch, kv_heads, page_log2;
+};
+// Bits of the status word of the page calls.
+constexpr int32_t kStatusFull = 1;       // a sequence has no table entry left for its tokens
+constexpr int32_t kStatusNoPage = 4;     // the pool has no page left (or a token's page is missing)
+constexpr int32_t kStatusBadParent = 8;  // a fork's parent is no sequence of the table
+
+// Rows [0, tokens[b]) (all `rows` without tokens) of k / v, strides in
+// elements, to positions counts[b] + t; a row without a page writes nothing.
+struct PagedWrite {
+    const void *k, *v;
+    int64_t k_bs, k_hs, k_ts, v_bs, v_hs, v_ts, rows;
+    const int64_t* tokens;
+    int32_t* status;
+};
+hipError_t launch_paged_write(const PagedWrite& a, const PagedView& c, int dtype, int dim_group, hipStream_t stream);
+// The cached rows as k / v [batch, KVH, rows, 128]; rows past a count are
+// cleared with `fill`, else left.
+struct PagedRead {
+    void *k, *v;
+    int64_t rows;
+    int fill;
+};
+hipError_t launch_paged_read(const PagedRead& a, const PagedView& c, int dtype, int dim_group, hipStream_t stream);
+
+// Pages for tokens[b] (or `each`) more tokens a sequence.  Outputs may be the
+// inputs.  Workspace: need batch + 1, list pages.
+struct PageReserve {
+    const int32_t* table_in;
+    const int64_t* counts_in;
+    int32_t* table;
+    int64_t* counts;
+    int32_t* refs;
+    int64_t batch, width, pages;
+    int page_log2;
+    const int64_t* tokens;
+    int64_t each;
+    int32_t *status, *need, *list;
+};
+hipError_t launch_page_reserve(const PageReserve& a, const int32_t* refs_in, hipStream_t stream);
+
+// The pages of a plan copied in every layer (moves of (source, target)), and
+// the plan's table and counts laid down.
+constexpr int64_t kMoveBytes = 16384;
+struct PageMoves {
+    const int32_t* moves;
+    const int2* pairs;
+    char *codes, *scales;
+    int64_t layers, pages, code_bytes, scale_bytes, parts, code_parts;
+    const int32_t *table_in, *map;  // map: page -> page, or null
+    int32_t* table;
+    int64_t entries;
+    const int64_t* counts_in;
+    int64_t* counts;  // null: as they are
+    int64_t batch;
+};
+// new[b] = old[parents[b]].  Workspace: rows batch * width, new_counts batch,
+// need batch + 1, source batch, list batch, pairs batch, moves 1.
+struct PageFork {
+    const int32_t* table_in;
+    const int64_t *counts_in, *parents;
+    int32_t* refs;
+    int64_t batch, width, pages;
+    int page_log2;
+    int32_t *status, *rows;
+    int64_t* new_counts;
+    int32_t *need, *source, *list;
+    int2* pairs;
+    int32_t* moves;
+};
+hipError_t launch_page_fork(const PageFork& a, const int32_t* refs_in, const PageMoves& m, hipStream_t stream);
+// Live pages to the front.  map [pages]: where a live page went, -1 for free
+// ones.  Workspace: pairs pages / 2 + 1, moves 1.
+struct PageCompact {
+    const int32_t* refs_in;
+    int32_t *refs, *map;
+    int64_t pages;
+    int2* pairs;
+    int32_t* moves;
+};
+hipError_t launch_page_compact(const PageCompact& a, const PageMoves& m, hipStream_t stream);
+
+// Decode attention over the pages (head_dim 128): q, out [batch, QH, 128],
+// current k / v [batch, KVH, 128].  tickets (batch * KVH, or batch * QH
+// indexed): zero on entry, left zero.
+struct PagedAttend {
+    const void *q, *cur_k, *cur_v;
+    void* out;
+    int q_heads;
+    float* partials;
+    uint32_t* tickets;
+};
+// Every cached token and the current one; query head i reads KV head
+// i / (QH / KVH).  partials: paged_dense_items(...) * QH states of 130 floats.
+int64_t paged_dense_items(int64_t batch, int64_t kv_heads, int64_t max_tokens);
+hipError_t launch_paged_dense(const PagedAttend& a, const PagedView& c, int64_t max_tokens, int dtype, int dim_group,
+                              hipStream_t stream);
+// The tokens of indices [batch, QH, selected] (counts[b]: the current token;
+// others outside [0, counts[b]] and masked ones: none).
+struct PagedIndexed {
+    const void* indices;
+    int index_dtype;
+    const uint8_t* valid;
+    const int64_t* head_to_kv;
+    int64_t selected;
+};
+int64_t paged_indexed_splits(int64_t rows, int64_t selected);
+hipError_t launch_paged_indexed(const PagedAttend& a, const PagedIndexed& ix, const PagedView& c, int dtype,
+                                int dim_group, hipStream_t stream);
+
 }  // namespace popkv

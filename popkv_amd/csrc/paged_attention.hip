@@ -1,0 +1,599 @@
+// Decode attention over the paged 4-bit K/V cache: every cached token
+// (dense) or a selection of them (indexed), with the current token's K/V, not
+// cached yet, folded into the merge at full precision.
+//
+// Both split a row's tokens among workgroups that each leave an online-softmax
+// state (m, l, acc[128]), base-2 exponents; the last workgroup of a row merges
+// them in the same launch (the hand-off rule stands in attention_common.h).
+#include "attention_common.h"
+#include "paged.h"
+
+namespace popkv {
+namespace {
+
+constexpr int kState = 128 + 2;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The factor that takes a state (m, l) to the maximum mx.  A state that folded
+// nothing has l = 0; one whose logits were all NaN keeps its NaN.
+__device__ __forceinline__ float state_weight(float m, float l, float mx) {
+    return m == -INFINITY && l == 0.0f ? 0.0f : exp2_fast(m - mx);
+}
+
+// ---- the VALU fold ----------------------------------------------------------
+
+// Eight lanes a token, sixteen dims each (one scale group at G = 16, 32, 64).
+struct Row4 {
+    uint2 k, v;
+    uint32_t ks, vs;
+};
+
+template <int QC>
+struct FoldState {
+    float m[QC], l[QC], low[QC], acc[QC][16];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int j = 0; j < QC; ++j) {
+            m[j] = -INFINITY;
+            l[j] = low[j] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < 16; ++d) acc[j][d] = 0.0f;
+        }
+    }
+};
+
+__device__ __forceinline__ void codes16(uint2 w, float (&c)[16]) {
+    codes8(w.x, c);
+    codes8(w.y, c + 8);
+}
+
+// Folds four tokens into the lane octet's state: s = delta sum(q c) + low
+// sum(q), acc += (p delta) c, and p low apart, all in fp32.  Dead tokens have
+// zero scales and weight 0.
+template <int QC>
+__device__ __forceinline__ void fold4(FoldState<QC>& st, const float (&q)[QC][16], const float (&qsum)[QC],
+                                      const Row4 (&r)[4], const bool (&live)[4], float scale) {
+    float s[QC][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        float c[16];
+        codes16(r[t].k, c);
+        const float low = f16_lo(r[t].ks), delta = f16_hi(r[t].ks);
+#pragma unroll
+        for (int j = 0; j < QC; ++j) {
+            float dot = 0.0f;
+#pragma unroll
+            for (int d = 0; d < 16; ++d) dot = fmaf(q[j][d], c[d], dot);
+            const float x = row_sum<8>(fmaf(delta, dot, low * qsum[j])) * scale;
+            s[j][t] = live[t] ? x : -INFINITY;
+        }
+    }
+    bool moved = false;
+    float alpha[QC];
+#pragma unroll
+    for (int j = 0; j < QC; ++j) {
+        const float mn = fmaxf(fmaxf(fmaxf(s[j][0], s[j][1]), fmaxf(s[j][2], s[j][3])), st.m[j]);
+        alpha[j] = mn == -INFINITY ? 1.0f : exp2_fast(st.m[j] - mn);
+        moved = moved || mn != st.m[j];
+        st.m[j] = mn;
+    }
+    if (__ballot(moved) != 0) {
+#pragma unroll
+        for (int j = 0; j < QC; ++j) {
+            st.l[j] *= alpha[j];
+            st.low[j] *= alpha[j];
+#pragma unroll
+            for (int d = 0; d < 16; ++d) st.acc[j][d] *= alpha[j];
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        float c[16];
+        codes16(r[t].v, c);
+        const float low = f16_lo(r[t].vs), delta = f16_hi(r[t].vs);
+#pragma unroll
+        for (int j = 0; j < QC; ++j) {
+            const float p = s[j][t] == -INFINITY ? 0.0f : exp2_fast(s[j][t] - st.m[j]);
+            st.l[j] += p;
+            st.low[j] = fmaf(p, low, st.low[j]);
+            const float pd = p * delta;
+#pragma unroll
+            for (int d = 0; d < 16; ++d) st.acc[j][d] = fmaf(pd, c[d], st.acc[j][d]);
+        }
+    }
+}
+
+// The eight octets' states of a wave become one, in every octet.
+template <int QC>
+__device__ __forceinline__ void join_octets(FoldState<QC>& st) {
+#pragma unroll
+    for (int j = 0; j < QC; ++j) {
+        float mx = st.m[j];
+        mx = fmaxf(mx, lane_xor<8>(mx));
+        mx = fmaxf(mx, lane_xor<16>(mx));
+        mx = fmaxf(mx, lane_xor<32>(mx));
+        const float f = state_weight(st.m[j], st.l[j], mx);
+        auto sum = [](float v) {
+            v += lane_xor<8>(v);
+            v += lane_xor<16>(v);
+            return v + lane_xor<32>(v);
+        };
+        st.l[j] = sum(st.l[j] * f);
+#pragma unroll
+        for (int d = 0; d < 16; ++d) st.acc[j][d] = sum((st.acc[j][d] + st.low[j]) * f);
+        st.m[j] = mx;
+    }
+}
+
+// ---- the merge --------------------------------------------------------------
+
+// Whether this workgroup is the last of `n` to come here (the states before it
+// are acknowledged; the ticket goes back to zero).
+__device__ __forceinline__ bool last_of(uint32_t* ticket, uint32_t n, uint32_t* s_last) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const uint32_t old = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *s_last = old + 1u == n ? 1u : 0u;
+        if (*s_last != 0u) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    return *s_last != 0u;
+}
+
+// Adds `n` states, `stride` floats apart, to a wave's running (m, l, a0, a1);
+// a lane owns dims lane and lane + 64.
+__device__ __forceinline__ void fold_states(const float* ps, int64_t stride, int n, float& m, float& l, float& a0,
+                                            float& a1) {
+    constexpr int NF = 16;
+    const int lane = threadIdx.x & (kWave - 1);
+    for (int s0 = 0; s0 < n; s0 += NF) {
+        float ms = -INFINITY, ls = 0.0f, x0[NF], x1[NF];
+        const int k = min(NF, n - s0);
+        if (lane < k) {
+            ms = ld_f32<true>(ps + (s0 + lane) * stride);
+            ls = ld_f32<true>(ps + (s0 + lane) * stride + 1);
+        }
+#pragma unroll
+        for (int j = 0; j < NF; ++j) {
+            const float* p = ps + (s0 + min(j, k - 1)) * stride + 2;
+            x0[j] = ld_f32<true>(p + lane);
+            x1[j] = ld_f32<true>(p + lane + 64);
+        }
+        const float mx = fmaxf(m, wave_max(ms));
+        const float w = state_weight(ms, ls, mx);
+        const float f = state_weight(m, l, mx);
+        l = fmaf(l, f, wave_sum(ls * w));
+        a0 *= f;
+        a1 *= f;
+#pragma unroll
+        for (int j = 0; j < NF; ++j) {
+            if (j < k) {
+                const float wj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), j));
+                a0 = fmaf(wj, x0[j], a0);
+                a1 = fmaf(wj, x1[j], a1);
+            }
+        }
+        m = mx;
+    }
+}
+
+// A row's output from its merged state and `hits` times the current token (NaN
+// logits stay; nothing at all gives zeros).
+template <typename T>
+__device__ __forceinline__ void finish_row(float m, float l, float a0, float a1, float hits, const T* q, const T* ck,
+                                           const T* cv, float scale, T* out) {
+    const int lane = threadIdx.x & (kWave - 1);
+    if (hits > 0.0f) {
+        const float q0 = Elem<T>::load(q, lane), q1 = Elem<T>::load(q, lane + 64);
+        const float k0 = Elem<T>::load(ck, lane), k1 = Elem<T>::load(ck, lane + 64);
+        const float v0 = Elem<T>::load(cv, lane), v1 = Elem<T>::load(cv, lane + 64);
+        const float s = wave_sum(fmaf(q0, k0, q1 * k1)) * scale;
+        const float mx = fmaxf(m, s);
+        const float f = state_weight(m, l, mx), w = s == -INFINITY && mx != -INFINITY ? 0.0f : hits * exp2_fast(s - mx);
+        l = fmaf(l, f, w);
+        a0 = fmaf(a0, f, w * v0);
+        a1 = fmaf(a1, f, w * v1);
+    }
+    const bool empty = l == 0.0f;
+    Elem<T>::store(out, lane, empty ? 0.0f : a0 / l);
+    Elem<T>::store(out, lane + 64, empty ? 0.0f : a1 / l);
+}
+
+// ---- dense ------------------------------------------------------------------
+
+constexpr int kDenseWaves = 8;
+constexpr int kDenseThreads = kDenseWaves * kWave;
+// Tokens of a split: at least a tile for every wave.
+constexpr int kDenseLeast = kDenseWaves * kPageTile;
+constexpr int kDenseBlocks = 256;
+
+int64_t dense_target(int64_t kv_heads) { return kDenseBlocks / kv_heads < 1 ? 1 : kDenseBlocks / kv_heads; }
+
+// A workgroup's share: tokens [t0, t1) of sequence b, split `s` of `n`, the
+// sequence's first item.
+struct DenseShare {
+    int b, s, n, first;
+    int64_t t0, t1;
+};
+
+// The splits follow the real lengths, read on the device: every split holds at
+// most total / target tokens (at least kDenseLeast), so a batch of short and
+// long sequences is shared out evenly, in at most target + batch items.  Each
+// wave works it out by itself from the counts.
+__device__ __forceinline__ bool dense_share(const PagedView& c, int64_t max_tokens, int target, int item,
+                                            DenseShare& out) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const int64_t most = min(c.width << c.page_log2, max_tokens);
+    int64_t total = 0;
+    for (int b0 = 0; b0 < c.batch; b0 += kWave) {
+        int64_t n = b0 + lane < c.batch ? clamp_count(c.counts[b0 + lane], most) : 0;
+        for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o);
+        total += n;
+    }
+    int64_t per = ((total + target - 1) / target + kDenseLeast - 1) / kDenseLeast * kDenseLeast;
+    if (per < kDenseLeast) per = kDenseLeast;
+    int base = 0;
+    for (int b0 = 0; b0 < c.batch; b0 += kWave) {
+        const int64_t count = b0 + lane < c.batch ? clamp_count(c.counts[b0 + lane], most) : 0;
+        const int splits = b0 + lane < c.batch ? max(1, static_cast<int>((count + per - 1) / per)) : 0;
+        const int incl = static_cast<int>(wave_incl_scan(static_cast<uint32_t>(splits), lane));
+        const int excl = base + incl - splits;
+        const uint64_t mine = __ballot(item >= excl && item < excl + splits);
+        if (mine) {
+            const int src = __ffsll(static_cast<unsigned long long>(mine)) - 1;
+            out.b = b0 + src;
+            out.first = __builtin_amdgcn_readlane(excl, src);
+            out.n = __builtin_amdgcn_readlane(splits, src);
+            out.s = item - out.first;
+            out.t0 = out.s * per;
+            const int64_t n = __shfl(count, src);
+            out.t1 = min(n, out.t0 + per);
+            return true;
+        }
+        base += __builtin_amdgcn_readlane(incl, kWave - 1);
+    }
+    return false;
+}
+
+// The workgroup's waves hold `rows` states each in LDS (row-major: s_m, s_l
+// [W][rows], s_acc [W][rows][128]); rows r0 .. of the item's group go to the
+// partials as one state each.
+template <int ROWS>
+__device__ __forceinline__ void store_states(const float (*s_m)[ROWS], const float (*s_l)[ROWS],
+                                             const float (*s_acc)[ROWS][128], int rows, float* dst) {
+    for (int i = threadIdx.x; i < rows * 128; i += kDenseThreads) {
+        const int j = i / 128, d = i % 128;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kDenseWaves; ++w) mx = fmaxf(mx, s_m[w][j]);
+        float a = 0.0f, l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kDenseWaves; ++w) {
+            const float f = state_weight(s_m[w][j], s_l[w][j], mx);
+            a = fmaf(f, s_acc[w][j][d], a);
+            l = fmaf(f, s_l[w][j], l);
+        }
+        float* p = dst + static_cast<int64_t>(j) * kState;
+        st_f32<true>(p + 2 + d, a);
+        if (d == 0) {
+            st_f32<true>(p, mx);
+            st_f32<true>(p + 1, l);
+        }
+    }
+}
+
+// The last workgroup of a (sequence, KV head) merges the group's rows: a row
+// takes a wave, or up to eight waves' shares of its splits where the group has
+// fewer rows than the workgroup waves.
+template <typename T>
+__device__ __forceinline__ void dense_merge(const PagedAttend& a, const PagedView& c, const DenseShare& sh, int h,
+                                            int group, float scale) {
+    __shared__ uint32_t s_last;
+    __shared__ float s_part[kDenseWaves][kState];
+    if (!last_of(a.tickets + sh.b * c.kv_heads + h, sh.n, &s_last)) return;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    int share = 1;  // waves a row
+    while (share * 2 * group <= kDenseWaves && share * 2 <= sh.n) share *= 2;
+    const int at_once = kDenseWaves / share;
+    const int64_t stride = static_cast<int64_t>(c.kv_heads) * group * kState;
+    for (int r0 = 0; r0 < group; r0 += at_once) {
+        const int r = r0 + wave / share, part = wave % share;
+        float m = -INFINITY, l = 0.0f, a0 = 0.0f, a1 = 0.0f;
+        if (r < group) {
+            const int s0 = sh.n * part / share, s1 = sh.n * (part + 1) / share;
+            const float* ps = a.partials + (static_cast<int64_t>(sh.first + s0) * c.kv_heads + h) * group * kState +
+                              static_cast<int64_t>(r) * kState;
+            fold_states(ps, stride, s1 - s0, m, l, a0, a1);
+        }
+        if (share > 1) {
+            __syncthreads();
+            if (lane == 0) {
+                s_part[wave][0] = m;
+                s_part[wave][1] = l;
+            }
+            s_part[wave][2 + lane] = a0;
+            s_part[wave][66 + lane] = a1;
+            __syncthreads();
+            if (part == 0 && r < group) {
+                for (int w = 1; w < share; ++w) {
+                    const float m2 = s_part[wave + w][0], l2 = s_part[wave + w][1], mx = fmaxf(m, m2);
+                    const float f = state_weight(m, l, mx), g = state_weight(m2, l2, mx);
+                    l = fmaf(l, f, l2 * g);
+                    a0 = fmaf(a0, f, s_part[wave + w][2 + lane] * g);
+                    a1 = fmaf(a1, f, s_part[wave + w][66 + lane] * g);
+                    m = mx;
+                }
+            }
+        }
+        if (part == 0 && r < group) {
+            const int64_t row = static_cast<int64_t>(sh.b) * a.q_heads + static_cast<int64_t>(h) * group + r;
+            const int64_t kv = (static_cast<int64_t>(sh.b) * c.kv_heads + h) * 128;
+            finish_row<T>(m, l, a0, a1, 1.0f, static_cast<const T*>(a.q) + row * 128,
+                          static_cast<const T*>(a.cur_k) + kv, static_cast<const T*>(a.cur_v) + kv, scale,
+                          static_cast<T*>(a.out) + row * 128);
+        }
+    }
+}
+
+// One workgroup a (share, KV head); QC query heads of the group at a time.  A
+// tile of 32 tokens lies in one page: its table entry is one scalar.
+template <typename T, int G, int QC>
+__global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend a, PagedView c, int64_t max_tokens,
+                                                                    int target, float scale) {
+    constexpr int R = 128 / G;
+    const int h = blockIdx.x % c.kv_heads, item = blockIdx.x / c.kv_heads;
+    DenseShare sh;
+    if (!dense_share(c, max_tokens, target, item, sh)) return;
+    const int group = a.q_heads / c.kv_heads;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int oct = lane / 8, d0 = (lane % 8) * 16;
+    __shared__ float s_m[kDenseWaves][QC], s_l[kDenseWaves][QC];
+    __shared__ float s_acc[kDenseWaves][QC][128];
+    const int64_t per_page = static_cast<int64_t>(c.kv_heads) << c.page_log2;
+    const int64_t head_row = static_cast<int64_t>(h) << c.page_log2;
+    for (int j0 = 0; j0 < group; j0 += QC) {
+        const int rows = min(QC, group - j0);
+        float q[QC][16], qsum[QC];
+#pragma unroll
+        for (int j = 0; j < QC; ++j) {
+            const int64_t row = static_cast<int64_t>(sh.b) * a.q_heads + static_cast<int64_t>(h) * group + j0 + min(j, rows - 1);
+            load8<T>(static_cast<const T*>(a.q) + row * 128 + d0, q[j]);
+            load8<T>(static_cast<const T*>(a.q) + row * 128 + d0 + 8, q[j] + 8);
+            qsum[j] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < 16; ++d) qsum[j] += q[j][d];
+        }
+        FoldState<QC> st;
+        st.clear();
+        for (int64_t t = sh.t0 + wave * kPageTile; t < sh.t1; t += kDenseLeast) {
+            const int32_t page = c.table[sh.b * c.width + (t >> c.page_log2)];
+            if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(c.pages)) continue;  // uniform
+            const int64_t row0 = page * per_page + head_row + (t & ((1 << c.page_log2) - 1));
+            const int left = static_cast<int>(min<int64_t>(kPageTile, sh.t1 - t));
+            Row4 r[4];
+            bool live[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int tok = oct + 8 * i;
+                live[i] = tok < left;
+                const char* code = c.codes + (row0 + tok) * kCodeRow + d0 / 2;
+                const uint32_t* sc = c.scales + (row0 + tok) * (2 * R) + d0 / G;
+                r[i].k = *reinterpret_cast<const uint2*>(code);
+                r[i].v = *reinterpret_cast<const uint2*>(code + 64);
+                r[i].ks = sc[0];
+                r[i].vs = live[i] ? sc[R] : 0u;  // what lies behind the last token may be anything
+            }
+            fold4<QC>(st, q, qsum, r, live, scale);
+        }
+        join_octets<QC>(st);
+        if (lane < 8) {
+#pragma unroll
+            for (int j = 0; j < QC; ++j) {
+#pragma unroll
+                for (int d = 0; d < 16; ++d) s_acc[wave][j][d0 + d] = st.acc[j][d];
+                if (lane == 0) {
+                    s_m[wave][j] = st.m[j];
+                    s_l[wave][j] = st.l[j];
+                }
+            }
+        }
+        __syncthreads();
+        store_states<QC>(s_m, s_l, s_acc, rows,
+                         a.partials + ((static_cast<int64_t>(item) * c.kv_heads + h) * group + j0) * kState);
+        __syncthreads();
+    }
+    dense_merge<T>(a, c, sh, h, group, scale);
+}
+
+// ---- indexed ----------------------------------------------------------------
+
+constexpr int kPickWaves = 4;
+constexpr int kPickThreads = kPickWaves * kWave;
+constexpr int kPickLeast = kPickWaves * kPageTile;
+constexpr int kPickBlocks = 1024;
+
+// One workgroup a (split of the selection, query head, sequence): every query
+// head gathers its own tokens.  The current token is counted, not read: the
+// merge folds it in as often as it was selected.
+template <typename T, int G, typename I>
+__global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend a, PagedIndexed ix, PagedView c,
+                                                                     int splits, int per, float scale) {
+    constexpr int R = 128 / G, STATE = kState + 1;  // (m, l, acc[128], hits of the current token)
+    const int s = blockIdx.x, qh = blockIdx.y, b = blockIdx.z;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int oct = lane / 8, d0 = (lane % 8) * 16;
+    const int64_t row = static_cast<int64_t>(b) * a.q_heads + qh;
+    const int64_t kvh = ix.head_to_kv[qh];
+    const int h = static_cast<int>(kvh < 0 ? 0 : kvh >= c.kv_heads ? c.kv_heads - 1 : kvh);
+    const int64_t count = clamp_count(c.counts[b], c.width << c.page_log2);
+    float q[1][16], qsum[1] = {0.0f};
+    load8<T>(static_cast<const T*>(a.q) + row * 128 + d0, q[0]);
+    load8<T>(static_cast<const T*>(a.q) + row * 128 + d0 + 8, q[0] + 8);
+#pragma unroll
+    for (int d = 0; d < 16; ++d) qsum[0] += q[0][d];
+    const I* idx = static_cast<const I*>(ix.indices) + row * ix.selected;
+    const uint8_t* valid = ix.valid ? ix.valid + row * ix.selected : nullptr;
+    const int64_t e0 = static_cast<int64_t>(s) * per, e1 = min<int64_t>(e0 + per, ix.selected);
+    FoldState<1> st;
+    st.clear();
+    int hits = 0;
+    for (int64_t e = e0 + wave * kPageTile; e < e1; e += kPickLeast) {
+        Row4 r[4];
+        bool live[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t at = e + oct + 8 * i;
+            const bool in = at < e1 && (!valid || valid[at] != 0);
+            const int64_t tok = in ? static_cast<int64_t>(idx[at]) : -1;
+            hits += tok == count ? 1 : 0;
+            const bool cached = tok >= 0 && tok < count;
+            const int32_t page = cached ? c.table[b * c.width + (tok >> c.page_log2)] : -1;
+            live[i] = static_cast<uint32_t>(page) < static_cast<uint32_t>(c.pages);
+            r[i].k = r[i].v = make_uint2(0u, 0u);
+            r[i].ks = r[i].vs = 0u;
+            if (live[i]) {
+                const int64_t at_row = ((static_cast<int64_t>(page) * c.kv_heads + h) << c.page_log2) +
+                                       (tok & ((1 << c.page_log2) - 1));
+                const char* code = c.codes + at_row * kCodeRow + d0 / 2;
+                const uint32_t* sc = c.scales + at_row * (2 * R) + d0 / G;
+                r[i].k = *reinterpret_cast<const uint2*>(code);
+                r[i].v = *reinterpret_cast<const uint2*>(code + 64);
+                r[i].ks = sc[0];
+                r[i].vs = sc[R];
+            }
+        }
+        fold4<1>(st, q, qsum, r, live, scale);
+    }
+    join_octets<1>(st);
+    const float wave_hits = wave_sum(static_cast<float>(hits)) * 0.125f;  // the eight lanes of an octet count alike
+    __shared__ float s_m[kPickWaves], s_l[kPickWaves], s_hits[kPickWaves], s_acc[kPickWaves][128];
+    if (lane < 8) {
+#pragma unroll
+        for (int d = 0; d < 16; ++d) s_acc[wave][d0 + d] = st.acc[0][d];
+        if (lane == 0) {
+            s_m[wave] = st.m[0];
+            s_l[wave] = st.l[0];
+            s_hits[wave] = wave_hits;
+        }
+    }
+    __syncthreads();
+    float* mine = a.partials + (row * splits + s) * STATE;
+    if (threadIdx.x < 128) {
+        float mx = -INFINITY, l = 0.0f, x = 0.0f, n = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kPickWaves; ++w) mx = fmaxf(mx, s_m[w]);
+#pragma unroll
+        for (int w = 0; w < kPickWaves; ++w) {
+            const float f = state_weight(s_m[w], s_l[w], mx);
+            x = fmaf(f, s_acc[w][threadIdx.x], x);
+            l = fmaf(f, s_l[w], l);
+            n += s_hits[w];
+        }
+        st_f32<true>(mine + 2 + threadIdx.x, x);
+        if (threadIdx.x == 0) {
+            st_f32<true>(mine, mx);
+            st_f32<true>(mine + 1, l);
+            st_f32<true>(mine + kState, n);
+        }
+    }
+    __shared__ uint32_t s_last;
+    if (!last_of(a.tickets + row, splits, &s_last)) return;
+    if (wave != 0) return;
+    const float* ps = a.partials + row * splits * STATE;
+    float n = 0.0f;
+    for (int i = lane; i < splits; i += kWave) n += ld_f32<true>(ps + static_cast<int64_t>(i) * STATE + kState);
+    n = wave_sum(n);
+    float m = -INFINITY, l = 0.0f, a0 = 0.0f, a1 = 0.0f;
+    fold_states(ps, STATE, splits, m, l, a0, a1);
+    const int64_t kv = (static_cast<int64_t>(b) * c.kv_heads + h) * 128;
+    finish_row<T>(m, l, a0, a1, n, static_cast<const T*>(a.q) + row * 128, static_cast<const T*>(a.cur_k) + kv,
+                  static_cast<const T*>(a.cur_v) + kv, scale, static_cast<T*>(a.out) + row * 128);
+}
+
+struct PickPlan {
+    int splits, per;
+};
+PickPlan pick_plan(int64_t rows, int64_t selected) {
+    int64_t want = kPickBlocks / rows;
+    const int64_t most = (selected + kPickLeast - 1) / kPickLeast;
+    if (want > most) want = most;
+    if (want < 1) want = 1;
+    const int64_t per = ((selected + want - 1) / want + kPickLeast - 1) / kPickLeast * kPickLeast;
+    return {static_cast<int>((selected + per - 1) / per), static_cast<int>(per)};
+}
+
+template <typename T, int G>
+hipError_t launch_dense_t(const PagedAttend& a, const PagedView& c, int64_t max_tokens, hipStream_t stream) {
+    const float scale = static_cast<float>(1.0 / sqrt(128.0)) * kLog2e;
+    const int group = a.q_heads / c.kv_heads;
+    const dim3 grid(static_cast<unsigned>(paged_dense_items(c.batch, c.kv_heads, max_tokens) * c.kv_heads));
+    const int target = static_cast<int>(dense_target(c.kv_heads));
+#define POPKV_DENSE(QC)                                                                                            \
+    hipLaunchKernelGGL((paged_dense_kernel<T, G, QC>), grid, dim3(kDenseThreads), 0, stream, a, c, max_tokens, target, \
+                       scale)
+    if (group == 1) POPKV_DENSE(1);
+    else if (group == 2) POPKV_DENSE(2);
+    else POPKV_DENSE(4);
+#undef POPKV_DENSE
+    return hipGetLastError();
+}
+
+template <typename T, int G>
+hipError_t launch_indexed_t(const PagedAttend& a, const PagedIndexed& ix, const PagedView& c, hipStream_t stream) {
+    const float scale = static_cast<float>(1.0 / sqrt(128.0)) * kLog2e;
+    const PickPlan p = pick_plan(static_cast<int64_t>(c.batch) * a.q_heads, ix.selected);
+    const dim3 grid(static_cast<unsigned>(p.splits), static_cast<unsigned>(a.q_heads), static_cast<unsigned>(c.batch));
+    if (ix.index_dtype == POPKV_INDEX_I32)
+        hipLaunchKernelGGL((paged_indexed_kernel<T, G, int32_t>), grid, dim3(kPickThreads), 0, stream, a, ix, c, p.splits,
+                           p.per, scale);
+    else
+        hipLaunchKernelGGL((paged_indexed_kernel<T, G, int64_t>), grid, dim3(kPickThreads), 0, stream, a, ix, c, p.splits,
+                           p.per, scale);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t paged_dense_items(int64_t batch, int64_t kv_heads, int64_t max_tokens) {
+    const int64_t target = dense_target(kv_heads);
+    const int64_t per_sequence = max_tokens < 1 ? 1 : (max_tokens + kDenseLeast - 1) / kDenseLeast;
+    const int64_t all = batch * per_sequence;
+    return all < target + batch ? all : target + batch;
+}
+
+int64_t paged_indexed_splits(int64_t rows, int64_t selected) { return pick_plan(rows, selected).splits; }
+
+#define POPKV_PAGED_G(CALL, T)                  \
+    switch (dim_group) {                        \
+        case 16: return CALL(T, 16);            \
+        case 32: return CALL(T, 32);            \
+        default: return CALL(T, 64);            \
+    }
+#define POPKV_PAGED_T(CALL)                              \
+    switch (dtype) {                                     \
+        case POPKV_DTYPE_F32: POPKV_PAGED_G(CALL, float) \
+        case POPKV_DTYPE_F16: POPKV_PAGED_G(CALL, f16_t) \
+        default: POPKV_PAGED_G(CALL, bf16_t)             \
+    }
+
+hipError_t launch_paged_dense(const PagedAttend& a, const PagedView& c, int64_t max_tokens, int dtype, int dim_group,
+                              hipStream_t stream) {
+#define POPKV_CALL(T, G) launch_dense_t<T, G>(a, c, max_tokens, stream)
+    POPKV_PAGED_T(POPKV_CALL)
+#undef POPKV_CALL
+}
+
+hipError_t launch_paged_indexed(const PagedAttend& a, const PagedIndexed& ix, const PagedView& c, int dtype,
+                                int dim_group, hipStream_t stream) {
+#define POPKV_CALL(T, G) launch_indexed_t<T, G>(a, ix, c, stream)
+    POPKV_PAGED_T(POPKV_CALL)
+#undef POPKV_CALL
+}
+
+}  // namespace popkv
