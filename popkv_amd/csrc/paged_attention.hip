@@ -261,9 +261,9 @@ __device__ __forceinline__ bool dense_share(const PagedView& c, int64_t max_toke
 // The workgroup's waves hold `rows` states each in LDS (row-major: s_m, s_l
 // [W][rows], s_acc [W][rows][128]); rows r0 .. of the item's group go to the
 // partials as one state each.
-template <int ROWS>
+template <int ROWS, int PITCH>
 __device__ __forceinline__ void store_states(const float (*s_m)[ROWS], const float (*s_l)[ROWS],
-                                             const float (*s_acc)[ROWS][128], int rows, float* dst) {
+                                             const float (*s_acc)[ROWS][PITCH], int rows, float* dst) {
     for (int i = threadIdx.x; i < rows * 128; i += kDenseThreads) {
         const int j = i / 128, d = i % 128;
         float mx = -INFINITY;
@@ -339,8 +339,250 @@ __device__ __forceinline__ void dense_merge(const PagedAttend& a, const PagedVie
     }
 }
 
-// One workgroup a (share, KV head); QC query heads of the group at a time.  A
-// tile of 32 tokens lies in one page: its table entry is one scalar.
+// Matrix-core form (16-bit types), one workgroup a (share, KV head) for the
+// whole group: its query heads are the 16 columns of the products (those past
+// the group zero), so any group of 1 to 16 costs the same.  A wave takes tiles
+// of 32 tokens, two 16 x 16 x 32 products of K rows and queries each,
+//   S^T[token, head] = K . q^T      (A: lane l holds token l % 16, dims 32 (l /
+//                                    16) .. + 31 in four steps of eight)
+//   O^T[dim, head]  += V^T . P^T    (A: lane l holds dims 8 (l % 16) .. + 7 of
+//                                    tokens 4 (l / 16) .. + 3 and 16 + those)
+// S^T leaves lane l with head l % 16 and just those eight tokens, which is how
+// the second product wants P: weights go from one to the other in registers.
+// A code becomes fp16 by its bits (0x6400 | c is 1024 + c), then low + c delta
+// in one packed fma, rounded to fp16: 13 instructions for eight values.
+// Queries are scaled by a power of two per head (bf16 reaches past fp16), and
+// the weights are kept around 2^8, where fp16 is exact to 2^-11.
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ half2_t as_half2(uint32_t x) { return __builtin_bit_cast(half2_t, x); }
+__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) {  // a.lo, b.lo
+    return __builtin_amdgcn_perm(b, a, 0x05040100u);
+}
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {
+    return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+
+// The nibble pairs (i, i + 4), i = 0 .. 3, of w as low + c * delta.
+__device__ __forceinline__ void dequantise_pairs(uint32_t w, half2_t delta, half2_t low, uint32_t (&out)[4]) {
+    const half2_t k1024 = {1024.0f16, 1024.0f16}, k16th = {0.0625f16, 0.0625f16}, k64 = {-64.0f16, -64.0f16};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t x = i ? w >> 8 : w;
+        const half2_t even = as_half2((x & 0x000f000fu) | 0x64006400u) - k1024;
+        const half2_t odd = __builtin_elementwise_fma(as_half2((x & 0x00f000f0u) | 0x64006400u), k16th, k64);
+        out[2 * i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(even, delta, low));
+        out[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(odd, delta, low));
+    }
+}
+
+__device__ __forceinline__ f32x4_t mfma_f16(const uint32_t (&a)[4], const uint32_t (&b)[4], f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, make_uint4(a[0], a[1], a[2], a[3])),
+                                                  __builtin_bit_cast(half8_t, make_uint4(b[0], b[1], b[2], b[3])), c, 0, 0, 0);
+}
+
+template <typename T, int G>
+__global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAttend a, PagedView c, int64_t max_tokens,
+                                                                         int target, float scale) {
+    constexpr int R = 128 / G, KS = R == 8 ? 2 : 1;  // scale pairs of a lane's 32 dims of K
+    constexpr float kBase = 8.0f, kTop = 15.0f;      // weights start at 2^8 and may grow to 2^15
+    const int h = blockIdx.x % c.kv_heads, item = blockIdx.x / c.kv_heads;
+    DenseShare sh;
+    if (!dense_share(c, max_tokens, target, item, sh)) return;
+    const int group = a.q_heads / c.kv_heads;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int col = lane & 15, grp = lane >> 4;
+
+    // the queries as fp16, largest magnitude of a head in [2^10, 2^11)
+    uint32_t qb[4][4];
+    float factor;
+    {
+        float q[32], top = 0.0f;
+        const int64_t row = static_cast<int64_t>(sh.b) * a.q_heads + static_cast<int64_t>(h) * group + min(col, group - 1);
+        const T* src = static_cast<const T*>(a.q) + row * 128 + 32 * grp;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load8<T>(src + 8 * i, q + 8 * i);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            if (col >= group) q[i] = 0.0f;
+            top = fmaxf(top, fabsf(q[i]));
+        }
+        top = fmaxf(top, lane_xor<16>(top));
+        top = fmaxf(top, lane_xor<32>(top));
+        const int e = static_cast<int>((__float_as_uint(top) >> 23) & 0xffu) - 127;
+        factor = ldexpf(scale, e - 10);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const half2_t x = {static_cast<_Float16>(ldexpf(q[8 * i + j], 10 - e)),
+                                   static_cast<_Float16>(ldexpf(q[8 * i + j + 4], 10 - e))};
+                qb[i][j] = __builtin_bit_cast(uint32_t, x);
+            }
+    }
+
+    struct Tile {
+        uint4 k[2];
+        uint32_t ks[2][KS], v[8], vs[8];
+        int left;  // live tokens
+    };
+    const int64_t per_page = static_cast<int64_t>(c.kv_heads) << c.page_log2, head_row = static_cast<int64_t>(h) << c.page_log2;
+    const int in_page = (1 << c.page_log2) - 1;
+    const int64_t first = sh.t0 + wave * kPageTile;
+    const int tiles = first < sh.t1 ? static_cast<int>((sh.t1 - first + kDenseLeast - 1) / kDenseLeast) : 0;
+    const uint32_t ko = col * kCodeRow + 16 * grp, vo = 4 * grp * kCodeRow + 64 + 4 * col;
+    const uint32_t kso = col * (8 * R) + 4 * (32 * grp / G), vso = 4 * grp * (8 * R) + 4 * (R + 8 * col / G);
+    int32_t entries = -1;  // lane i: the page of this wave's tile i of a block of 64
+    auto load_entries = [&](int i0) {
+        const int64_t t = first + static_cast<int64_t>(i0 + lane) * kDenseLeast;
+        entries = t < sh.t1 ? c.table[sh.b * c.width + (t >> c.page_log2)] : -1;
+    };
+    auto load_tile = [&](int i, Tile& x) {
+        const int64_t t = first + static_cast<int64_t>(i) * kDenseLeast;
+        const int32_t e = __builtin_amdgcn_readlane(entries, i & (kWave - 1));
+        const bool there = static_cast<uint32_t>(e) < static_cast<uint32_t>(c.pages);
+        x.left = there ? static_cast<int>(min<int64_t>(kPageTile, sh.t1 - t)) : 0;
+        const int64_t row = (there ? e : 0) * per_page + head_row + (t & in_page);
+        const char* code = c.codes + row * kCodeRow;
+        const char* sc = reinterpret_cast<const char*>(c.scales) + row * (8 * R);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            x.k[s] = *reinterpret_cast<const uint4*>(code + ko + 16 * s * kCodeRow);
+#pragma unroll
+            for (int i2 = 0; i2 < KS; ++i2)
+                x.ks[s][i2] = *reinterpret_cast<const uint32_t*>(sc + kso + 16 * s * (8 * R) + 4 * i2);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int tok = (j & 3) + 16 * (j >> 2);
+            x.v[j] = *reinterpret_cast<const uint32_t*>(code + vo + tok * kCodeRow);
+            x.vs[j] = *reinterpret_cast<const uint32_t*>(sc + vso + tok * (8 * R));
+        }
+    };
+
+    f32x4_t acc[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    float ref = -INFINITY, l = 0.0f;  // weights are 2^(logit - ref)
+    auto fold = [&](Tile& x) {
+        const bool whole = x.left == kPageTile;  // uniform
+        f32x4_t s[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            s[u] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            const uint32_t w[4] = {x.k[u].x, x.k[u].y, x.k[u].z, x.k[u].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t sc = x.ks[u][KS == 2 ? i / 2 : 0];
+                uint32_t kf[4];
+                dequantise_pairs(w[i], as_half2(high_halves(sc, sc)), as_half2(low_halves(sc, sc)), kf);
+                s[u] = mfma_f16(kf, qb[i], s[u]);
+            }
+        }
+        float t[8];
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = s[j >> 2][j & 3] * factor;
+        if (!whole) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool live = 4 * grp + (j & 3) + 16 * (j >> 2) < x.left;
+                t[j] = live ? t[j] : -INFINITY;
+                x.vs[j] = live ? x.vs[j] : 0u;  // what lies behind the last token may be anything
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, t[j]);
+        if (__ballot(top > ref + kTop) != 0) {  // some weight would pass 2^15
+            top = fmaxf(top, lane_xor<16>(top));
+            top = fmaxf(top, lane_xor<32>(top));
+            if (top > ref + kBase) {
+                const float to = top - kBase;
+                const float f = exp2_fast(ref - to);  // 0 at first
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[i][r] *= f;
+                ref = to;
+            }
+        }
+        uint32_t pb[4];
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const float p0 = t[j] == -INFINITY ? 0.0f : exp2_fast(t[j] - ref);
+            const float p1 = t[j + 1] == -INFINITY ? 0.0f : exp2_fast(t[j + 1] - ref);
+            l += p0 + p1;
+            const half2_t p = {static_cast<_Float16>(p0), static_cast<_Float16>(p1)};
+            pb[j / 2] = __builtin_bit_cast(uint32_t, p);
+        }
+        // eight dims of V: dims i and i + ... come from the low (0 .. 3) and the
+        // high (4 .. 7) halves of the tokens' dwords, a pair of tokens at a time
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            uint32_t vf[4][4];  // [dim][token pair]
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t v0 = x.v[2 * j], v1 = x.v[2 * j + 1];
+                const uint32_t pair = half ? high_halves(v0, v1) : low_halves(v0, v1);
+                uint32_t d[4];
+                dequantise_pairs(pair, as_half2(high_halves(x.vs[2 * j], x.vs[2 * j + 1])),
+                                 as_half2(low_halves(x.vs[2 * j], x.vs[2 * j + 1])), d);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) vf[i][j] = d[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[4 * half + i] = mfma_f16(vf[i], pb, acc[4 * half + i]);
+        }
+    };
+    Tile x, y;
+    for (int i0 = 0; i0 < tiles; i0 += kWave) {
+        const int n = min(kWave, tiles - i0);
+        load_entries(i0);
+        load_tile(i0, x);
+        for (int i = 0; i < n; i += 2) {
+            if (i + 1 < n) load_tile(i0 + i + 1, y);
+            fold(x);
+            if (i + 1 >= n) break;
+            if (i + 2 < n) load_tile(i0 + i + 2, x);
+            fold(y);
+        }
+    }
+
+    // the waves' states meet in LDS, eight heads at a time
+    constexpr int ROWS = 8, PITCH = 132;
+    __shared__ float s_m[kDenseWaves][ROWS], s_l[kDenseWaves][ROWS];
+    __shared__ __align__(16) float s_acc[kDenseWaves][ROWS][PITCH];
+    l += lane_xor<16>(l);
+    l += lane_xor<32>(l);
+    for (int r0 = 0; r0 < group; r0 += ROWS) {
+        if (col >= r0 && col < r0 + ROWS) {
+            const int r = col - r0;
+            if (grp == 0) {
+                s_m[wave][r] = ref;
+                s_l[wave][r] = l;
+            }
+            // this lane's dims: 8 (4 grp + i) + d of acc[d][i]
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float4* dst = reinterpret_cast<float4*>(&s_acc[wave][r][32 * grp + 8 * i]);
+                dst[0] = make_float4(acc[0][i], acc[1][i], acc[2][i], acc[3][i]);
+                dst[1] = make_float4(acc[4][i], acc[5][i], acc[6][i], acc[7][i]);
+            }
+        }
+        __syncthreads();
+        store_states<ROWS, PITCH>(s_m, s_l, s_acc, min(ROWS, group - r0),
+                                  a.partials + ((static_cast<int64_t>(item) * c.kv_heads + h) * group + r0) * kState);
+        __syncthreads();
+    }
+    dense_merge<T>(a, c, sh, h, group, scale);
+}
+
+// VALU form (fp32), QC query heads of the group at a time.  A tile of 32
+// tokens lies in one page: its table entry is one scalar.
 template <typename T, int G, int QC>
 __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend a, PagedView c, int64_t max_tokens,
                                                                     int target, float scale) {
@@ -403,7 +645,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
             }
         }
         __syncthreads();
-        store_states<QC>(s_m, s_l, s_acc, rows,
+        store_states<QC, 128>(s_m, s_l, s_acc, rows,
                          a.partials + ((static_cast<int64_t>(item) * c.kv_heads + h) * group + j0) * kState);
         __syncthreads();
     }
@@ -537,9 +779,14 @@ hipError_t launch_dense_t(const PagedAttend& a, const PagedView& c, int64_t max_
 #define POPKV_DENSE(QC)                                                                                            \
     hipLaunchKernelGGL((paged_dense_kernel<T, G, QC>), grid, dim3(kDenseThreads), 0, stream, a, c, max_tokens, target, \
                        scale)
-    if (group == 1) POPKV_DENSE(1);
-    else if (group == 2) POPKV_DENSE(2);
-    else POPKV_DENSE(4);
+    if constexpr (sizeof(T) == 2) {
+        hipLaunchKernelGGL((paged_dense_mfma_kernel<T, G>), grid, dim3(kDenseThreads), 0, stream, a, c, max_tokens, target,
+                           scale);
+    } else {
+        if (group == 1) POPKV_DENSE(1);
+        else if (group == 2) POPKV_DENSE(2);
+        else POPKV_DENSE(4);
+    }
 #undef POPKV_DENSE
     return hipGetLastError();
 }
