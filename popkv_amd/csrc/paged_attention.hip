@@ -12,7 +12,12 @@ namespace popkv {
 namespace {
 
 constexpr int kState = 128 + 2;
-constexpr float kLog2e = 1.4426950408889634f;
+// log2(e) / sqrt(128) as a float and what it leaves: logits reach tens, and
+// one float's rounding of the factor would show in fp32 outputs
+constexpr double kScale = 1.4426950408889634 * 0.08838834764831845;
+constexpr float kScaleHigh = static_cast<float>(kScale);
+constexpr float kScaleLow = static_cast<float>(kScale - static_cast<double>(kScaleHigh));
+__device__ __forceinline__ float scaled_logit(float dot) { return fmaf(dot, kScaleHigh, dot * kScaleLow); }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -32,41 +37,45 @@ struct Row4 {
 
 template <int QC>
 struct FoldState {
-    float m[QC], l[QC], low[QC], acc[QC][16];
+    float m[QC], l[QC], acc[QC][16];
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int j = 0; j < QC; ++j) {
             m[j] = -INFINITY;
-            l[j] = low[j] = 0.0f;
+            l[j] = 0.0f;
 #pragma unroll
             for (int d = 0; d < 16; ++d) acc[j][d] = 0.0f;
         }
     }
 };
 
-__device__ __forceinline__ void codes16(uint2 w, float (&c)[16]) {
-    codes8(w.x, c);
-    codes8(w.y, c + 8);
+// This lane's sixteen values low + c * delta, rounded once to fp32.  (Sums of
+// codes with the scales applied after save an fma a value, but delta sum(q c)
+// and low sum(q) cancel: fp32 results were twice as far off.)
+__device__ __forceinline__ void values16(uint2 w, uint32_t scale, float (&x)[16]) {
+    codes8(w.x, x);
+    codes8(w.y, x + 8);
+    const float low = f16_lo(scale), delta = f16_hi(scale);
+#pragma unroll
+    for (int d = 0; d < 16; ++d) x[d] = fmaf(x[d], delta, low);
 }
 
-// Folds four tokens into the lane octet's state: s = delta sum(q c) + low
-// sum(q), acc += (p delta) c, and p low apart, all in fp32.  Dead tokens have
-// zero scales and weight 0.
+// Folds four tokens into the lane octet's state, in fp32.  Dead tokens have
+// zero scales (their values count with weight 0, so they must be finite).
 template <int QC>
-__device__ __forceinline__ void fold4(FoldState<QC>& st, const float (&q)[QC][16], const float (&qsum)[QC],
-                                      const Row4 (&r)[4], const bool (&live)[4], float scale) {
+__device__ __forceinline__ void fold4(FoldState<QC>& st, const float (&q)[QC][16], const Row4 (&r)[4],
+                                      const bool (&live)[4]) {
     float s[QC][4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-        float c[16];
-        codes16(r[t].k, c);
-        const float low = f16_lo(r[t].ks), delta = f16_hi(r[t].ks);
+        float k[16];
+        values16(r[t].k, r[t].ks, k);
 #pragma unroll
         for (int j = 0; j < QC; ++j) {
             float dot = 0.0f;
 #pragma unroll
-            for (int d = 0; d < 16; ++d) dot = fmaf(q[j][d], c[d], dot);
-            const float x = row_sum<8>(fmaf(delta, dot, low * qsum[j])) * scale;
+            for (int d = 0; d < 16; ++d) dot = fmaf(q[j][d], k[d], dot);
+            const float x = scaled_logit(row_sum<8>(dot));
             s[j][t] = live[t] ? x : -INFINITY;
         }
     }
@@ -83,24 +92,20 @@ __device__ __forceinline__ void fold4(FoldState<QC>& st, const float (&q)[QC][16
 #pragma unroll
         for (int j = 0; j < QC; ++j) {
             st.l[j] *= alpha[j];
-            st.low[j] *= alpha[j];
 #pragma unroll
             for (int d = 0; d < 16; ++d) st.acc[j][d] *= alpha[j];
         }
     }
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-        float c[16];
-        codes16(r[t].v, c);
-        const float low = f16_lo(r[t].vs), delta = f16_hi(r[t].vs);
+        float v[16];
+        values16(r[t].v, r[t].vs, v);
 #pragma unroll
         for (int j = 0; j < QC; ++j) {
             const float p = s[j][t] == -INFINITY ? 0.0f : exp2_fast(s[j][t] - st.m[j]);
             st.l[j] += p;
-            st.low[j] = fmaf(p, low, st.low[j]);
-            const float pd = p * delta;
 #pragma unroll
-            for (int d = 0; d < 16; ++d) st.acc[j][d] = fmaf(pd, c[d], st.acc[j][d]);
+            for (int d = 0; d < 16; ++d) st.acc[j][d] = fmaf(p, v[d], st.acc[j][d]);
         }
     }
 }
@@ -122,7 +127,7 @@ __device__ __forceinline__ void join_octets(FoldState<QC>& st) {
         };
         st.l[j] = sum(st.l[j] * f);
 #pragma unroll
-        for (int d = 0; d < 16; ++d) st.acc[j][d] = sum((st.acc[j][d] + st.low[j]) * f);
+        for (int d = 0; d < 16; ++d) st.acc[j][d] = sum(st.acc[j][d] * f);
         st.m[j] = mx;
     }
 }
@@ -184,13 +189,13 @@ __device__ __forceinline__ void fold_states(const float* ps, int64_t stride, int
 // logits stay; nothing at all gives zeros).
 template <typename T>
 __device__ __forceinline__ void finish_row(float m, float l, float a0, float a1, float hits, const T* q, const T* ck,
-                                           const T* cv, float scale, T* out) {
+                                           const T* cv, T* out) {
     const int lane = threadIdx.x & (kWave - 1);
     if (hits > 0.0f) {
         const float q0 = Elem<T>::load(q, lane), q1 = Elem<T>::load(q, lane + 64);
         const float k0 = Elem<T>::load(ck, lane), k1 = Elem<T>::load(ck, lane + 64);
         const float v0 = Elem<T>::load(cv, lane), v1 = Elem<T>::load(cv, lane + 64);
-        const float s = wave_sum(fmaf(q0, k0, q1 * k1)) * scale;
+        const float s = scaled_logit(wave_sum(fmaf(q0, k0, q1 * k1)));
         const float mx = fmaxf(m, s);
         const float f = state_weight(m, l, mx), w = s == -INFINITY && mx != -INFINITY ? 0.0f : hits * exp2_fast(s - mx);
         l = fmaf(l, f, w);
@@ -290,7 +295,7 @@ __device__ __forceinline__ void store_states(const float (*s_m)[ROWS], const flo
 // fewer rows than the workgroup waves.
 template <typename T>
 __device__ __forceinline__ void dense_merge(const PagedAttend& a, const PagedView& c, const DenseShare& sh, int h,
-                                            int group, float scale) {
+                                            int group) {
     __shared__ uint32_t s_last;
     __shared__ float s_part[kDenseWaves][kState];
     if (!last_of(a.tickets + sh.b * c.kv_heads + h, sh.n, &s_last)) return;
@@ -333,31 +338,42 @@ __device__ __forceinline__ void dense_merge(const PagedAttend& a, const PagedVie
             const int64_t row = static_cast<int64_t>(sh.b) * a.q_heads + static_cast<int64_t>(h) * group + r;
             const int64_t kv = (static_cast<int64_t>(sh.b) * c.kv_heads + h) * 128;
             finish_row<T>(m, l, a0, a1, 1.0f, static_cast<const T*>(a.q) + row * 128,
-                          static_cast<const T*>(a.cur_k) + kv, static_cast<const T*>(a.cur_v) + kv, scale,
+                          static_cast<const T*>(a.cur_k) + kv, static_cast<const T*>(a.cur_v) + kv,
                           static_cast<T*>(a.out) + row * 128);
         }
     }
 }
 
 // Matrix-core form (16-bit types), one workgroup a (share, KV head) for the
-// whole group: its query heads are the 16 columns of the products (those past
-// the group zero), so any group of 1 to 16 costs the same.  A wave takes tiles
-// of 32 tokens, two 16 x 16 x 32 products of K rows and queries each,
-//   S^T[token, head] = K . q^T      (A: lane l holds token l % 16, dims 32 (l /
-//                                    16) .. + 31 in four steps of eight)
-//   O^T[dim, head]  += V^T . P^T    (A: lane l holds dims 8 (l % 16) .. + 7 of
-//                                    tokens 4 (l / 16) .. + 3 and 16 + those)
-// S^T leaves lane l with head l % 16 and just those eight tokens, which is how
-// the second product wants P: weights go from one to the other in registers.
-// A code becomes fp16 by its bits (0x6400 | c is 1024 + c), then low + c delta
-// in one packed fma, rounded to fp16: 13 instructions for eight values.
-// Queries are scaled by a power of two per head (bf16 reaches past fp16), and
-// the weights are kept around 2^8, where fp16 is exact to 2^-11.
+// whole group: its query heads are the 16 rows of the products (those past the
+// group zero), so any group of 1 to 16 costs the same.  A wave takes tiles of
+// 32 tokens, two of 16 for the logits:
+//   dot_g[head, token] = q . c       one 16 x 16 x 32 step per 32 dims, codes as
+//                                    they are, each scale group by itself
+//   S = sum_g delta_g dot_g + sum_g low_g qsum_g   in fp32, the second sum by
+//                                    one more product (qsum in two fp16 terms)
+//   O[head, dim] += P . V            V as low + c delta in fp16
+// so keys enter the logits exactly: with the outlier channels that keys have,
+// their rounding to fp16 was four times fp16's own in the result.  (C layout:
+// lane l holds rows 4 (l / 16) .. + 3 of column l % 16; A and B: lane l holds
+// k-elements 8 (l / 16) .. + 7 of row / column l % 16.)
+// A code becomes fp16 by its bits: 0x6400 | c is 1024 + c, and 0x6400 | 16 c
+// is 1024 + 16 c.  For the keys the queries of odd dims are divided by 16, and
+// what codes of zero would give, times delta, is taken off in that same extra
+// product, so a dword of eight costs five instructions; for the values a packed
+// subtraction and a packed fma follow (13).  A token's 16-byte quarters are exchanged among the four
+// lane groups (lane swaps), so that a step's 32 dims are one group's.
+// Queries are scaled by a power of two per head (bf16 reaches past fp16, and
+// 1024 times a group's sum must not), and the weights are kept around 2^8, where fp16 keeps
+// 11 bits; fp16 outputs take a second term for the rest of each weight.
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ half2_t as_half2(uint32_t x) { return __builtin_bit_cast(half2_t, x); }
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+    return __builtin_bit_cast(uint32_t, half2_t{static_cast<_Float16>(a), static_cast<_Float16>(b)});
+}
 __device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) {  // a.lo, b.lo
     return __builtin_amdgcn_perm(b, a, 0x05040100u);
 }
@@ -365,16 +381,25 @@ __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {
     return __builtin_amdgcn_perm(b, a, 0x07060302u);
 }
 
-// The nibble pairs (i, i + 4), i = 0 .. 3, of w as low + c * delta.
+// Nibble pairs (0, 4), (1, 5), (2, 6), (3, 7) of w as fp16 1024 + c (first and
+// third) and 1024 + 16 c.
+__device__ __forceinline__ void biased_pairs(uint32_t w, uint32_t (&out)[4]) {
+    const uint32_t x = w >> 8;
+    out[0] = (w & 0x000f000fu) | 0x64006400u;
+    out[1] = (w & 0x00f000f0u) | 0x64006400u;
+    out[2] = (x & 0x000f000fu) | 0x64006400u;
+    out[3] = (x & 0x00f000f0u) | 0x64006400u;
+}
+
+// The same pairs as low + c * delta.
 __device__ __forceinline__ void dequantise_pairs(uint32_t w, half2_t delta, half2_t low, uint32_t (&out)[4]) {
     const half2_t k1024 = {1024.0f16, 1024.0f16}, k16th = {0.0625f16, 0.0625f16}, k64 = {-64.0f16, -64.0f16};
+    uint32_t b[4];
+    biased_pairs(w, b);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const uint32_t x = i ? w >> 8 : w;
-        const half2_t even = as_half2((x & 0x000f000fu) | 0x64006400u) - k1024;
-        const half2_t odd = __builtin_elementwise_fma(as_half2((x & 0x00f000f0u) | 0x64006400u), k16th, k64);
-        out[2 * i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(even, delta, low));
-        out[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(odd, delta, low));
+    for (int i = 0; i < 4; ++i) {
+        const half2_t c = i & 1 ? __builtin_elementwise_fma(as_half2(b[i]), k16th, k64) : as_half2(b[i]) - k1024;
+        out[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c, delta, low));
     }
 }
 
@@ -383,11 +408,27 @@ __device__ __forceinline__ f32x4_t mfma_f16(const uint32_t (&a)[4], const uint32
                                                   __builtin_bit_cast(half8_t, make_uint4(b[0], b[1], b[2], b[3])), c, 0, 0, 0);
 }
 
+// d[s] of lane group g becomes d[g] of lane group s.
+__device__ __forceinline__ void exchange_quarters(uint32_t (&d)[4]) {
+    const auto a = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
+    const auto x = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+    const auto y = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+    d[0] = x[0];
+    d[1] = x[1];
+    d[2] = y[0];
+    d[3] = y[1];
+}
+
 template <typename T, int G>
 __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAttend a, PagedView c, int64_t max_tokens,
-                                                                         int target, float scale) {
-    constexpr int R = 128 / G, KS = R == 8 ? 2 : 1;  // scale pairs of a lane's 32 dims of K
-    constexpr float kBase = 8.0f, kTop = 15.0f;      // weights start at 2^8 and may grow to 2^15
+                                                                         int target) {
+    constexpr int R = 128 / G;
+    constexpr int HALVES = R == 8 ? 2 : 1;        // groups of a 32-dim step
+    constexpr int LOWS = R == 8 ? 2 : 1;          // products for the low terms (four groups each)
+    constexpr int TERMS = std::is_same_v<T, f16_t> ? 2 : 1;
+    constexpr float kBase = 8.0f, kTop = 15.0f;   // weights start at 2^8 and may grow to 2^15
+    constexpr float kNone = -3e38f;               // no weight yet
     const int h = blockIdx.x % c.kv_heads, item = blockIdx.x / c.kv_heads;
     DenseShare sh;
     if (!dense_share(c, max_tokens, target, item, sh)) return;
@@ -396,37 +437,88 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int col = lane & 15, grp = lane >> 4;
 
-    // the queries as fp16, largest magnitude of a head in [2^10, 2^11)
-    uint32_t qb[4][4];
-    float factor;
+    // the queries: row `col`, dims 32 s + 8 grp .. + 7 in step s, largest
+    // magnitude of a head in [1/2, 1)
+    uint32_t qa[HALVES][4][4], ql[LOWS][4];
+    float factor[4];  // of rows 4 grp + i
     {
-        float q[32], top = 0.0f;
+        float q[4][8], top = 0.0f;
         const int64_t row = static_cast<int64_t>(sh.b) * a.q_heads + static_cast<int64_t>(h) * group + min(col, group - 1);
-        const T* src = static_cast<const T*>(a.q) + row * 128 + 32 * grp;
+        const T* src = static_cast<const T*>(a.q) + row * 128 + 8 * grp;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) load8<T>(src + 8 * i, q + 8 * i);
+        for (int s = 0; s < 4; ++s) load8<T>(src + 32 * s, q[s]);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            if (col >= group) q[i] = 0.0f;
-            top = fmaxf(top, fabsf(q[i]));
-        }
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (col >= group) q[s][i] = 0.0f;
+                top = fmaxf(top, fabsf(q[s][i]));
+            }
         top = fmaxf(top, lane_xor<16>(top));
         top = fmaxf(top, lane_xor<32>(top));
         const int e = static_cast<int>((__float_as_uint(top) >> 23) & 0xffu) - 127;
-        factor = ldexpf(scale, e - 10);
+        const float mine = ldexpf(kScaleHigh, e + 1);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) factor[i] = __shfl(mine, 4 * grp + i);
+        float sum[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            sum[s] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                q[s][i] = ldexpf(q[s][i], -1 - e);
+                sum[s] += q[s][i];
+                if (i & 1) q[s][i] *= 0.0625f;
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const half2_t x = {static_cast<_Float16>(ldexpf(q[8 * i + j], 10 - e)),
-                                   static_cast<_Float16>(ldexpf(q[8 * i + j + 4], 10 - e))};
-                qb[i][j] = __builtin_bit_cast(uint32_t, x);
+                const uint32_t x = pack_half2(q[s][j], q[s][j + 4]);
+                if constexpr (HALVES == 2) {
+                    qa[0][s][j] = grp < 2 ? x : 0u;
+                    qa[1][s][j] = grp < 2 ? 0u : x;
+                } else {
+                    qa[0][s][j] = x;
+                }
             }
+            sum[s] += lane_xor<16>(sum[s]);
+        }
+        // the low terms' product: lane group 0 holds the groups' sums of queries
+        // for low, lane group 1 minus their products with codes of zero for
+        // delta, each as (high, rest)
+        float qs[R];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const float other = lane_xor<32>(sum[s]);
+            if constexpr (R == 8) {
+                qs[2 * s] = grp < 2 ? sum[s] : other;
+                qs[2 * s + 1] = grp < 2 ? other : sum[s];
+            } else if constexpr (R == 4) {
+                qs[s] = sum[s] + other;
+            } else {
+                qs[s / 2] = s & 1 ? qs[s / 2] + (sum[s] + other) : sum[s] + other;
+            }
+        }
+        const uint32_t none[4] = {0x64006400u, 0x64006400u, 0x64006400u, 0x64006400u};
+#pragma unroll
+        for (int g = 0; g < 4 * LOWS; ++g) {
+            uint32_t x = 0;
+            if (g < R) {
+                f32x4_t z = {0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (R == 2) z = mfma_f16(none, qa[0][2 * g % 4 + 1], mfma_f16(none, qa[0][2 * g % 4], z));
+                else z = mfma_f16(none, qa[g % HALVES][g / HALVES % 4], z);
+                // (rows of codes times columns of queries: every element of column `col` is head `col`'s)
+                const float term = grp == 0 ? qs[g % R] : -z[0];
+                const float high = static_cast<float>(static_cast<_Float16>(term));
+                x = pack_half2(high, term - high);
+            }
+            ql[g / 4][g % 4] = grp < 2 ? x : 0u;
+        }
     }
+    const uint32_t low_or_delta = grp == 1 ? 0x03020302u : 0x01000100u;  // byte picks of a scale pair
 
     struct Tile {
         uint4 k[2];
-        uint32_t ks[2][KS], v[8], vs[8];
+        uint32_t ks[2][R], v[8], vs[8];
         int left;  // live tokens
     };
     const int64_t per_page = static_cast<int64_t>(c.kv_heads) << c.page_log2, head_row = static_cast<int64_t>(h) << c.page_log2;
@@ -434,7 +526,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
     const int64_t first = sh.t0 + wave * kPageTile;
     const int tiles = first < sh.t1 ? static_cast<int>((sh.t1 - first + kDenseLeast - 1) / kDenseLeast) : 0;
     const uint32_t ko = col * kCodeRow + 16 * grp, vo = 4 * grp * kCodeRow + 64 + 4 * col;
-    const uint32_t kso = col * (8 * R) + 4 * (32 * grp / G), vso = 4 * grp * (8 * R) + 4 * (R + 8 * col / G);
+    const uint32_t kso = col * (8 * R), vso = 4 * grp * (8 * R) + 4 * (R + 8 * col / G);
     int32_t entries = -1;  // lane i: the page of this wave's tile i of a block of 64
     auto load_entries = [&](int i0) {
         const int64_t t = first + static_cast<int64_t>(i0 + lane) * kDenseLeast;
@@ -449,94 +541,161 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
         const char* code = c.codes + row * kCodeRow;
         const char* sc = reinterpret_cast<const char*>(c.scales) + row * (8 * R);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            x.k[s] = *reinterpret_cast<const uint4*>(code + ko + 16 * s * kCodeRow);
+        for (int u = 0; u < 2; ++u) {
+            x.k[u] = *reinterpret_cast<const uint4*>(code + ko + 16 * u * kCodeRow);
+            const char* p = sc + kso + 16 * u * (8 * R);
+            if constexpr (R == 2) {
+                const uint2 w = *reinterpret_cast<const uint2*>(p);
+                x.ks[u][0] = w.x;
+                x.ks[u][1] = w.y;
+            } else {
 #pragma unroll
-            for (int i2 = 0; i2 < KS; ++i2)
-                x.ks[s][i2] = *reinterpret_cast<const uint32_t*>(sc + kso + 16 * s * (8 * R) + 4 * i2);
+                for (int g = 0; g < R; g += 4) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(p + 4 * g);
+                    x.ks[u][g] = w.x;
+                    x.ks[u][g + 1] = w.y;
+                    x.ks[u][g + 2] = w.z;
+                    x.ks[u][g + 3] = w.w;
+                }
+            }
         }
+        // v[2 j], v[2 j + 1]: tokens 4 grp + j and 16 + 4 grp + j
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int tok = (j & 3) + 16 * (j >> 2);
+            const int tok = (j >> 1) + 16 * (j & 1);
             x.v[j] = *reinterpret_cast<const uint32_t*>(code + vo + tok * kCodeRow);
             x.vs[j] = *reinterpret_cast<const uint32_t*>(sc + vso + tok * (8 * R));
         }
     };
 
+    // a wave's weights on their way from the logits' lanes to the product's:
+    // [term][head][token pair (n, 16 + n)]
+    __shared__ __align__(16) uint32_t s_p[kDenseWaves][TERMS][16][16];
     f32x4_t acc[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    float ref = -INFINITY, l = 0.0f;  // weights are 2^(logit - ref)
+    float ref[4], l[4];  // rows 4 grp + i: weights are 2^(logit - ref)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        ref[i] = kNone;
+        l[i] = 0.0f;
+    }
     auto fold = [&](Tile& x) {
-        const bool whole = x.left == kPageTile;  // uniform
         f32x4_t s[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
+            uint32_t w[4] = {x.k[u].x, x.k[u].y, x.k[u].z, x.k[u].w};
+            exchange_quarters(w);
             s[u] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            const uint32_t w[4] = {x.k[u].x, x.k[u].y, x.k[u].z, x.k[u].w};
+#pragma unroll
+            for (int n = 0; n < LOWS; ++n) {
+                uint32_t lows[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int g = 0; g < 4 && g < R; ++g)
+                    lows[g] = __builtin_amdgcn_perm(x.ks[u][4 * n + g], x.ks[u][4 * n + g], low_or_delta);
+                s[u] = mfma_f16(ql[n], lows, s[u]);
+            }
+            f32x4_t dot[R];
+#pragma unroll
+            for (int st = 0; st < 4; ++st) {
+                uint32_t cb[4];
+                biased_pairs(w[st], cb);
+                if constexpr (R == 2) {
+                    dot[st / 2] = mfma_f16(qa[0][st], cb, st & 1 ? dot[st / 2] : f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
+                } else {
+#pragma unroll
+                    for (int n = 0; n < HALVES; ++n)
+                        dot[HALVES * st + n] = mfma_f16(qa[n][st], cb, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < R; ++g) {
+                const float delta = static_cast<float>(as_half2(x.ks[u][g])[1]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[u][i] = fmaf(delta, dot[g][i], s[u][i]);
+            }
+        }
+        bool live[2] = {true, true};
+        if (x.left != kPageTile) {  // uniform
+#pragma unroll
+            for (int u = 0; u < 2; ++u) live[u] = col + 16 * u < x.left;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (4 * grp + (j >> 1) + 16 * (j & 1) >= x.left) x.vs[j] = 0u;  // what lies behind the last token may be anything
+        }
+        float e[4][2], top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                e[i][u] = live[u] ? fmaf(s[u][i], factor[i], -ref[i]) : -INFINITY;
+                top = fmaxf(top, e[i][u]);
+            }
+        if (__ballot(top > kTop) != 0) {  // some weight would pass 2^15
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t sc = x.ks[u][KS == 2 ? i / 2 : 0];
-                uint32_t kf[4];
-                dequantise_pairs(w[i], as_half2(high_halves(sc, sc)), as_half2(low_halves(sc, sc)), kf);
-                s[u] = mfma_f16(kf, qb[i], s[u]);
-            }
-        }
-        float t[8];
-        float top = -INFINITY;
+                float mx = fmaxf(live[0] ? s[0][i] * factor[i] : -INFINITY, live[1] ? s[1][i] * factor[i] : -INFINITY);
+                mx = fmaxf(mx, dpp_mov<0xB1>(mx));
+                mx = fmaxf(mx, dpp_mov<0x4E>(mx));
+                mx = fmaxf(mx, dpp_mov<0x141>(mx));
+                mx = fmaxf(mx, dpp_mov<0x140>(mx));
+                const float to = fmaxf(mx - kBase, ref[i]);
+                const float f = exp2_fast(ref[i] - to);
+                l[i] *= f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) t[j] = s[j >> 2][j & 3] * factor;
-        if (!whole) {
+                for (int d = 0; d < 8; ++d) acc[d][i] *= f;
+                ref[i] = to;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const bool live = 4 * grp + (j & 3) + 16 * (j >> 2) < x.left;
-                t[j] = live ? t[j] : -INFINITY;
-                x.vs[j] = live ? x.vs[j] : 0u;  // what lies behind the last token may be anything
+                for (int u = 0; u < 2; ++u) e[i][u] = live[u] ? fmaf(s[u][i], factor[i], -to) : -INFINITY;
             }
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, t[j]);
-        if (__ballot(top > ref + kTop) != 0) {  // some weight would pass 2^15
-            top = fmaxf(top, lane_xor<16>(top));
-            top = fmaxf(top, lane_xor<32>(top));
-            if (top > ref + kBase) {
-                const float to = top - kBase;
-                const float f = exp2_fast(ref - to);  // 0 at first
-                l *= f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[i][r] *= f;
-                ref = to;
-            }
+        for (int i = 0; i < 4; ++i) {
+            const float p0 = exp2_fast(e[i][0]), p1 = exp2_fast(e[i][1]);
+            l[i] += p0 + p1;
+            const uint32_t p = pack_half2(p0, p1);
+            s_p[wave][0][4 * grp + i][col] = p;
+            if constexpr (TERMS == 2)
+                s_p[wave][1][4 * grp + i][col] = pack_half2(p0 - static_cast<float>(as_half2(p)[0]),
+                                                            p1 - static_cast<float>(as_half2(p)[1]));
         }
-        uint32_t pb[4];
+        // the wave reads its own weights next: one wave's LDS operations complete in order
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        uint32_t pa[TERMS][4];
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            const float p0 = t[j] == -INFINITY ? 0.0f : exp2_fast(t[j] - ref);
-            const float p1 = t[j + 1] == -INFINITY ? 0.0f : exp2_fast(t[j + 1] - ref);
-            l += p0 + p1;
-            const half2_t p = {static_cast<_Float16>(p0), static_cast<_Float16>(p1)};
-            pb[j / 2] = __builtin_bit_cast(uint32_t, p);
+        for (int n = 0; n < TERMS; ++n) {
+            const uint4 w = *reinterpret_cast<const uint4*>(&s_p[wave][n][col][4 * grp]);
+            pa[n][0] = w.x;
+            pa[n][1] = w.y;
+            pa[n][2] = w.z;
+            pa[n][3] = w.w;
         }
-        // eight dims of V: dims i and i + ... come from the low (0 .. 3) and the
-        // high (4 .. 7) halves of the tokens' dwords, a pair of tokens at a time
+        // a lane's eight dims 8 col .. + 7 of V: the low halves of the tokens'
+        // dwords hold dims 0 .. 3, the high ones 4 .. 7
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             uint32_t vf[4][4];  // [dim][token pair]
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const uint32_t v0 = x.v[2 * j], v1 = x.v[2 * j + 1];
-                const uint32_t pair = half ? high_halves(v0, v1) : low_halves(v0, v1);
                 uint32_t d[4];
-                dequantise_pairs(pair, as_half2(high_halves(x.vs[2 * j], x.vs[2 * j + 1])),
+                dequantise_pairs(half ? high_halves(v0, v1) : low_halves(v0, v1),
+                                 as_half2(high_halves(x.vs[2 * j], x.vs[2 * j + 1])),
                                  as_half2(low_halves(x.vs[2 * j], x.vs[2 * j + 1])), d);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) vf[i][j] = d[i];
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[4 * half + i] = mfma_f16(vf[i], pb, acc[4 * half + i]);
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int n = 0; n < TERMS; ++n) acc[4 * half + i] = mfma_f16(pa[n], vf[i], acc[4 * half + i]);
         }
+        // the next tile's weights overwrite s_p only after every lane has read
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     };
     Tile x, y;
     for (int i0 = 0; i0 < tiles; i0 += kWave) {
@@ -556,19 +715,18 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
     constexpr int ROWS = 8, PITCH = 132;
     __shared__ float s_m[kDenseWaves][ROWS], s_l[kDenseWaves][ROWS];
     __shared__ __align__(16) float s_acc[kDenseWaves][ROWS][PITCH];
-    l += lane_xor<16>(l);
-    l += lane_xor<32>(l);
-    for (int r0 = 0; r0 < group; r0 += ROWS) {
-        if (col >= r0 && col < r0 + ROWS) {
-            const int r = col - r0;
-            if (grp == 0) {
-                s_m[wave][r] = ref;
-                s_l[wave][r] = l;
-            }
-            // this lane's dims: 8 (4 grp + i) + d of acc[d][i]
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float4* dst = reinterpret_cast<float4*>(&s_acc[wave][r][32 * grp + 8 * i]);
+    for (int i = 0; i < 4; ++i) l[i] = row_sum<16>(l[i]);
+    for (int r0 = 0; r0 < group; r0 += ROWS) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = 4 * grp + i - r0;
+            if (r >= 0 && r < ROWS) {
+                if (col == 0) {
+                    s_m[wave][r] = l[i] == 0.0f ? -INFINITY : ref[i];
+                    s_l[wave][r] = l[i];
+                }
+                float4* dst = reinterpret_cast<float4*>(&s_acc[wave][r][8 * col]);
                 dst[0] = make_float4(acc[0][i], acc[1][i], acc[2][i], acc[3][i]);
                 dst[1] = make_float4(acc[4][i], acc[5][i], acc[6][i], acc[7][i]);
             }
@@ -578,14 +736,14 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
                                   a.partials + ((static_cast<int64_t>(item) * c.kv_heads + h) * group + r0) * kState);
         __syncthreads();
     }
-    dense_merge<T>(a, c, sh, h, group, scale);
+    dense_merge<T>(a, c, sh, h, group);
 }
 
 // VALU form (fp32), QC query heads of the group at a time.  A tile of 32
 // tokens lies in one page: its table entry is one scalar.
 template <typename T, int G, int QC>
 __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend a, PagedView c, int64_t max_tokens,
-                                                                    int target, float scale) {
+                                                                    int target) {
     constexpr int R = 128 / G;
     const int h = blockIdx.x % c.kv_heads, item = blockIdx.x / c.kv_heads;
     DenseShare sh;
@@ -600,15 +758,12 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
     const int64_t head_row = static_cast<int64_t>(h) << c.page_log2;
     for (int j0 = 0; j0 < group; j0 += QC) {
         const int rows = min(QC, group - j0);
-        float q[QC][16], qsum[QC];
+        float q[QC][16];
 #pragma unroll
         for (int j = 0; j < QC; ++j) {
             const int64_t row = static_cast<int64_t>(sh.b) * a.q_heads + static_cast<int64_t>(h) * group + j0 + min(j, rows - 1);
             load8<T>(static_cast<const T*>(a.q) + row * 128 + d0, q[j]);
             load8<T>(static_cast<const T*>(a.q) + row * 128 + d0 + 8, q[j] + 8);
-            qsum[j] = 0.0f;
-#pragma unroll
-            for (int d = 0; d < 16; ++d) qsum[j] += q[j][d];
         }
         FoldState<QC> st;
         st.clear();
@@ -630,7 +785,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
                 r[i].ks = sc[0];
                 r[i].vs = live[i] ? sc[R] : 0u;  // what lies behind the last token may be anything
             }
-            fold4<QC>(st, q, qsum, r, live, scale);
+            fold4<QC>(st, q, r, live);
         }
         join_octets<QC>(st);
         if (lane < 8) {
@@ -649,7 +804,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
                          a.partials + ((static_cast<int64_t>(item) * c.kv_heads + h) * group + j0) * kState);
         __syncthreads();
     }
-    dense_merge<T>(a, c, sh, h, group, scale);
+    dense_merge<T>(a, c, sh, h, group);
 }
 
 // ---- indexed ----------------------------------------------------------------
@@ -664,7 +819,7 @@ constexpr int kPickBlocks = 1024;
 // merge folds it in as often as it was selected.
 template <typename T, int G, typename I>
 __global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend a, PagedIndexed ix, PagedView c,
-                                                                     int splits, int per, float scale) {
+                                                                     int splits, int per) {
     constexpr int R = 128 / G, STATE = kState + 1;  // (m, l, acc[128], hits of the current token)
     const int s = blockIdx.x, qh = blockIdx.y, b = blockIdx.z;
     const int lane = threadIdx.x & (kWave - 1);
@@ -674,11 +829,9 @@ __global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend
     const int64_t kvh = ix.head_to_kv[qh];
     const int h = static_cast<int>(kvh < 0 ? 0 : kvh >= c.kv_heads ? c.kv_heads - 1 : kvh);
     const int64_t count = clamp_count(c.counts[b], c.width << c.page_log2);
-    float q[1][16], qsum[1] = {0.0f};
+    float q[1][16];
     load8<T>(static_cast<const T*>(a.q) + row * 128 + d0, q[0]);
     load8<T>(static_cast<const T*>(a.q) + row * 128 + d0 + 8, q[0] + 8);
-#pragma unroll
-    for (int d = 0; d < 16; ++d) qsum[0] += q[0][d];
     const I* idx = static_cast<const I*>(ix.indices) + row * ix.selected;
     const uint8_t* valid = ix.valid ? ix.valid + row * ix.selected : nullptr;
     const int64_t e0 = static_cast<int64_t>(s) * per, e1 = min<int64_t>(e0 + per, ix.selected);
@@ -710,7 +863,7 @@ __global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend
                 r[i].vs = sc[R];
             }
         }
-        fold4<1>(st, q, qsum, r, live, scale);
+        fold4<1>(st, q, r, live);
     }
     join_octets<1>(st);
     const float wave_hits = wave_sum(static_cast<float>(hits)) * 0.125f;  // the eight lanes of an octet count alike
@@ -755,7 +908,7 @@ __global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend
     fold_states(ps, STATE, splits, m, l, a0, a1);
     const int64_t kv = (static_cast<int64_t>(b) * c.kv_heads + h) * 128;
     finish_row<T>(m, l, a0, a1, n, static_cast<const T*>(a.q) + row * 128, static_cast<const T*>(a.cur_k) + kv,
-                  static_cast<const T*>(a.cur_v) + kv, scale, static_cast<T*>(a.out) + row * 128);
+                  static_cast<const T*>(a.cur_v) + kv, static_cast<T*>(a.out) + row * 128);
 }
 
 struct PickPlan {
@@ -772,16 +925,13 @@ PickPlan pick_plan(int64_t rows, int64_t selected) {
 
 template <typename T, int G>
 hipError_t launch_dense_t(const PagedAttend& a, const PagedView& c, int64_t max_tokens, hipStream_t stream) {
-    const float scale = static_cast<float>(1.0 / sqrt(128.0)) * kLog2e;
     const int group = a.q_heads / c.kv_heads;
     const dim3 grid(static_cast<unsigned>(paged_dense_items(c.batch, c.kv_heads, max_tokens) * c.kv_heads));
     const int target = static_cast<int>(dense_target(c.kv_heads));
 #define POPKV_DENSE(QC)                                                                                            \
-    hipLaunchKernelGGL((paged_dense_kernel<T, G, QC>), grid, dim3(kDenseThreads), 0, stream, a, c, max_tokens, target, \
-                       scale)
+    hipLaunchKernelGGL((paged_dense_kernel<T, G, QC>), grid, dim3(kDenseThreads), 0, stream, a, c, max_tokens, target)
     if constexpr (sizeof(T) == 2) {
-        hipLaunchKernelGGL((paged_dense_mfma_kernel<T, G>), grid, dim3(kDenseThreads), 0, stream, a, c, max_tokens, target,
-                           scale);
+        hipLaunchKernelGGL((paged_dense_mfma_kernel<T, G>), grid, dim3(kDenseThreads), 0, stream, a, c, max_tokens, target);
     } else {
         if (group == 1) POPKV_DENSE(1);
         else if (group == 2) POPKV_DENSE(2);
@@ -793,15 +943,14 @@ hipError_t launch_dense_t(const PagedAttend& a, const PagedView& c, int64_t max_
 
 template <typename T, int G>
 hipError_t launch_indexed_t(const PagedAttend& a, const PagedIndexed& ix, const PagedView& c, hipStream_t stream) {
-    const float scale = static_cast<float>(1.0 / sqrt(128.0)) * kLog2e;
     const PickPlan p = pick_plan(static_cast<int64_t>(c.batch) * a.q_heads, ix.selected);
     const dim3 grid(static_cast<unsigned>(p.splits), static_cast<unsigned>(a.q_heads), static_cast<unsigned>(c.batch));
     if (ix.index_dtype == POPKV_INDEX_I32)
         hipLaunchKernelGGL((paged_indexed_kernel<T, G, int32_t>), grid, dim3(kPickThreads), 0, stream, a, ix, c, p.splits,
-                           p.per, scale);
+                           p.per);
     else
         hipLaunchKernelGGL((paged_indexed_kernel<T, G, int64_t>), grid, dim3(kPickThreads), 0, stream, a, ix, c, p.splits,
-                           p.per, scale);
+                           p.per);
     return hipGetLastError();
 }
 
