@@ -1061,11 +1061,11 @@ int popkv_page_reserve(const int32_t* table_in, const int64_t* counts_in, const 
         return fail(POPKV_ERR_WORKSPACE, "page reserve needs %zu workspace bytes",
                     popkv_page_reserve_workspace_bytes(batch, pages));
     if (!aligned16(workspace)) return fail(POPKV_ERR_UNSUPPORTED, "the workspace needs 16-byte alignment");
-    popkv::PageReserve a{table_in, counts_in, table, counts, refs, batch, width, pages, log2_of(page_tokens), tokens,
+    popkv::PageReserve a{table_in, counts_in, refs_in, table, counts, refs, batch, width, pages, log2_of(page_tokens), tokens,
                          each, status, nullptr, nullptr};
     Carve c{static_cast<char*>(workspace)};
     carve_reserve(c, a);
-    return launched(popkv::launch_page_reserve(a, refs_in, as_stream(stream)), "popkv_page_reserve");
+    return launched(popkv::launch_page_reserve(a, as_stream(stream)), "popkv_page_reserve");
 }
 
 size_t popkv_page_fork_workspace_bytes(int64_t batch, int64_t width) {
@@ -1092,7 +1092,7 @@ int popkv_page_fork(void* codes, void* scales, int64_t layers, int64_t pages, in
     if (workspace_bytes < popkv_page_fork_workspace_bytes(batch, width))
         return fail(POPKV_ERR_WORKSPACE, "page fork needs %zu workspace bytes", popkv_page_fork_workspace_bytes(batch, width));
     if (!aligned16(workspace)) return fail(POPKV_ERR_UNSUPPORTED, "the workspace needs 16-byte alignment");
-    popkv::PageFork a{table_in, counts_in, parents, refs, batch, width, pages, log2_of(page_tokens), status,
+    popkv::PageFork a{table_in, counts_in, parents, refs_in, refs, batch, width, pages, log2_of(page_tokens), status,
                       nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
     Carve c{static_cast<char*>(workspace)};
     carve_fork(c, a);
@@ -1105,7 +1105,7 @@ int popkv_page_fork(void* codes, void* scales, int64_t layers, int64_t pages, in
     m.counts_in = a.new_counts;
     m.counts = counts;
     m.batch = batch;
-    return launched(popkv::launch_page_fork(a, refs_in, m, as_stream(stream)), "popkv_page_fork");
+    return launched(popkv::launch_page_fork(a, m, as_stream(stream)), "popkv_page_fork");
 }
 
 size_t popkv_page_compact_workspace_bytes(int64_t pages) {

@@ -292,6 +292,7 @@ hipError_t launch_paged_read(const PagedRead& a, const PagedView& c, int dtype, 
 struct PageReserve {
     const int32_t* table_in;
     const int64_t* counts_in;
+    const int32_t* refs_in;
     int32_t* table;
     int64_t* counts;
     int32_t* refs;
@@ -301,7 +302,7 @@ struct PageReserve {
     int64_t each;
     int32_t *status, *need, *list;
 };
-hipError_t launch_page_reserve(const PageReserve& a, const int32_t* refs_in, hipStream_t stream);
+hipError_t launch_page_reserve(const PageReserve& a, hipStream_t stream);
 
 // The pages of a plan copied in every layer (moves of (source, target)), and
 // the plan's table and counts laid down.
@@ -323,6 +324,7 @@ struct PageMoves {
 struct PageFork {
     const int32_t* table_in;
     const int64_t *counts_in, *parents;
+    const int32_t* refs_in;
     int32_t* refs;
     int64_t batch, width, pages;
     int page_log2;
@@ -332,7 +334,7 @@ struct PageFork {
     int2* pairs;
     int32_t* moves;
 };
-hipError_t launch_page_fork(const PageFork& a, const int32_t* refs_in, const PageMoves& m, hipStream_t stream);
+hipError_t launch_page_fork(const PageFork& a, const PageMoves& m, hipStream_t stream);
 // Live pages to the front.  map [pages]: where a live page went, -1 for free
 // ones.  Workspace: pairs pages / 2 + 1, moves 1.
 struct PageCompact {

@@ -159,12 +159,10 @@ __device__ __forceinline__ void reserve_range(const PageReserve& a, int64_t b, i
     hi = fits ? (n + more + (int64_t{1} << a.page_log2) - 1) >> a.page_log2 : lo;
 }
 
-// One wave a sequence: its row and count to the output, its missing entries
+// Sequence b by one wave: its row and count to the output, its missing entries
 // counted.
-__global__ __launch_bounds__(256) void reserve_count_kernel(PageReserve a) {
+__device__ __forceinline__ void reserve_row(const PageReserve& a, int64_t b) {
     const int lane = threadIdx.x & (kWave - 1);
-    const int64_t b = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
-    if (b >= a.batch) return;
     int64_t lo, hi;
     bool fits;
     reserve_range(a, b, lo, hi, fits);
@@ -180,6 +178,11 @@ __global__ __launch_bounds__(256) void reserve_count_kernel(PageReserve a) {
         for (int64_t i = lane; i < a.width; i += kWave) a.table[b * a.width + i] = row[i];
         if (lane == 0) a.counts[b] = a.counts_in[b];
     }
+}
+
+__global__ __launch_bounds__(256) void reserve_rows_kernel(PageReserve a) {
+    const int64_t b = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
+    if (b < a.batch) reserve_row(a, b);
 }
 
 constexpr int kPlanThreads = 1024;
@@ -211,17 +214,24 @@ __device__ __forceinline__ int32_t plan_prefix(int32_t v, int32_t* sh, int32_t& 
 
 // The lowest `want` pages without a reference, ascending, to list; returns how
 // many there are in all.  Every thread of the block calls it.
+// COH: this workgroup's own atomics changed them in this launch, so the loads
+// read past the cache that may still hold what was there before.
+template <bool COH>
 __device__ __forceinline__ int32_t list_free(const int32_t* refs, int64_t pages, int32_t want, int32_t* list, int32_t* sh) {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    auto is_free = [&](int64_t i, int64_t end) {
+        if (i >= end) return false;
+        if constexpr (COH) return __hip_atomic_load(refs + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0;
+        else return refs[i] == 0;
+    };
     int64_t first, last;
     plan_segment(pages, wave, first, last);
     int32_t mine = 0;
-    for (int64_t i = first; i < last; i += kWave)
-        mine += __popcll(__ballot(i + lane < last && refs[i + lane] == 0));
+    for (int64_t i = first; i < last; i += kWave) mine += __popcll(__ballot(is_free(i + lane, last)));
     int32_t total;
     int32_t at = plan_prefix(mine, sh, total);
     for (int64_t i = first; i < last && at < want; i += kWave) {
-        const bool free = i + lane < last && refs[i + lane] == 0;
+        const bool free = is_free(i + lane, last);
         const uint64_t mask = __ballot(free);
         const int32_t r = at + __popcll(mask & ((uint64_t{1} << lane) - 1));
         if (free && r < want) list[r] = static_cast<int32_t>(i + lane);
@@ -249,15 +259,32 @@ __device__ __forceinline__ int32_t scan_needs(int32_t* need, int64_t batch, int3
     return base;
 }
 
+// Tables and pools up to which one workgroup does the whole plan: a launch
+// saved is worth more than the other CUs.  Reserve and fork, out of place, one
+// launch against two or three (us):
+constexpr int64_t kPlanAlone = 16384;
+
+bool plan_alone(int64_t batch, int64_t width, int64_t pages) {
+    return batch * width <= kPlanAlone && pages <= kPlanAlone;
+}
+
 // One workgroup: the missing entries of the sequences, in order, take the
-// lowest free pages; a sequence whose share does not fit gets none.
+// lowest free pages; a sequence whose share does not fit gets none.  ALONE:
+// the rows and references are its work too.
+template <bool ALONE>
 __global__ __launch_bounds__(kPlanThreads) void reserve_plan_kernel(PageReserve a) {
     __shared__ int32_t sh[kPlanWaves];
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    if constexpr (ALONE) {
+        for (int64_t b = wave; b < a.batch; b += kPlanWaves) reserve_row(a, b);
+        if (a.refs != a.refs_in)
+            for (int64_t i = threadIdx.x; i < a.pages; i += kPlanThreads) a.refs[i] = a.refs_in[i];
+        __syncthreads();
+    }
     const int32_t total = scan_needs(a.need, a.batch, sh);
     if (total == 0) return;
     const int32_t want = static_cast<int32_t>(min<int64_t>(total, a.pages));
-    const int32_t found = list_free(a.refs, a.pages, want, a.list, sh);
+    const int32_t found = list_free<false>(a.refs, a.pages, want, a.list, sh);
     __syncthreads();  // the list is this workgroup's own: the barrier orders it
     for (int64_t b = wave; b < a.batch; b += kPlanWaves) {
         const int32_t at = a.need[b], end = a.need[b + 1];
@@ -291,22 +318,17 @@ __device__ __forceinline__ int64_t parent_of(const PageFork& a, int64_t b) {
     return p >= 0 && p < a.batch ? p : -1;
 }
 
-// One workgroup a sequence: its new row (in the workspace: another sequence
-// may still read the old one) and the reference counts' changes.  The lowest
-// child of a parent keeps its whole row; the others share the full pages and
-// get an open page of their own (need = 1), whose place holds the parent's
-// until then.
-__global__ __launch_bounds__(256) void fork_rows_kernel(PageFork a) {
-    const int64_t b = blockIdx.x;
+// Sequence b by one wave: its new row (in the workspace: another sequence may
+// still read the old one) and the reference counts' changes.  The lowest child
+// of a parent keeps its whole row; the others share the full pages and get an
+// open page of their own (need = 1).
+__device__ __forceinline__ void fork_row(const PageFork& a, int64_t b) {
+    const int lane = threadIdx.x & (kWave - 1);
     const int64_t p = parent_of(a, b);
-    __shared__ int32_t s_earlier;
-    if (threadIdx.x == 0) s_earlier = 0;
-    __syncthreads();
+    bool earlier = false;
     if (p >= 0)
-        for (int64_t i = threadIdx.x; i < b; i += 256)
-            if (a.parents[i] == p) s_earlier = 1;
-    __syncthreads();
-    const bool first = s_earlier == 0;
+        for (int64_t i = lane; i < b; i += kWave) earlier = earlier || a.parents[i] == p;
+    const bool first = __ballot(earlier) == 0;
     const int64_t count = p >= 0 ? clamp_count(a.counts_in[p], a.width << a.page_log2) : 0;
     const int64_t full = count >> a.page_log2;
     const bool open = (count & ((int64_t{1} << a.page_log2) - 1)) != 0;
@@ -314,7 +336,7 @@ __global__ __launch_bounds__(256) void fork_rows_kernel(PageFork a) {
     const int32_t* old = a.table_in + b * a.width;
     int32_t* to = a.rows + b * a.width;
     const int64_t kept = p < 0 ? 0 : first ? a.width : full;
-    for (int64_t i = threadIdx.x; i < a.width; i += 256) {
+    for (int64_t i = lane; i < a.width; i += kWave) {
         const int32_t was = old[i];
         const int32_t now = i < kept ? from[i] : -1;
         to[i] = now;
@@ -323,7 +345,7 @@ __global__ __launch_bounds__(256) void fork_rows_kernel(PageFork a) {
             if (static_cast<uint32_t>(now) < static_cast<uint32_t>(a.pages)) atomicAdd(a.refs + now, 1);
         }
     }
-    if (threadIdx.x == 0) {
+    if (lane == 0) {
         const int32_t source = p >= 0 && !first && open ? from[full] : -1;
         const bool need = static_cast<uint32_t>(source) < static_cast<uint32_t>(a.pages);
         a.need[b] = need ? 1 : 0;
@@ -333,15 +355,30 @@ __global__ __launch_bounds__(256) void fork_rows_kernel(PageFork a) {
     }
 }
 
+__global__ __launch_bounds__(256) void fork_rows_kernel(PageFork a) {
+    const int64_t b = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
+    if (b < a.batch) fork_row(a, b);
+}
+
 // One workgroup: the open pages wanted take the lowest free pages; a sequence
-// that finds none is left empty.
+// that finds none is left empty.  ALONE: the rows and references are its work
+// too.
+template <bool ALONE>
 __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(PageFork a) {
     __shared__ int32_t sh[kPlanWaves];
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    if constexpr (ALONE) {
+        if (a.refs != a.refs_in) {
+            for (int64_t i = threadIdx.x; i < a.pages; i += kPlanThreads) a.refs[i] = a.refs_in[i];
+            __syncthreads();
+        }
+        for (int64_t b = wave; b < a.batch; b += kPlanWaves) fork_row(a, b);
+        __syncthreads();
+    }
     const int32_t total = scan_needs(a.need, a.batch, sh);
     if (threadIdx.x == 0) *a.moves = total;
     if (total == 0) return;
-    const int32_t found = list_free(a.refs, a.pages, static_cast<int32_t>(min<int64_t>(total, a.pages)), a.list, sh);
+    const int32_t found = list_free<ALONE>(a.refs, a.pages, static_cast<int32_t>(min<int64_t>(total, a.pages)), a.list, sh);
     if (threadIdx.x == 0 && found < total) *a.moves = found;
     __syncthreads();
     for (int64_t b = wave; b < a.batch; b += kPlanWaves) {
@@ -489,23 +526,31 @@ hipError_t launch_paged_read(const PagedRead& a, const PagedView& c, int dtype, 
 #undef POPKV_PAGED_T
 #undef POPKV_PAGED_G
 
-hipError_t launch_page_reserve(const PageReserve& a, const int32_t* refs_in, hipStream_t s) {
-    if (a.refs != refs_in) {
-        const hipError_t e = copy_words(refs_in, a.refs, a.pages, s);
+hipError_t launch_page_reserve(const PageReserve& a, hipStream_t s) {
+    if (plan_alone(a.batch, a.width, a.pages)) {
+        hipLaunchKernelGGL(reserve_plan_kernel<true>, dim3(1), dim3(kPlanThreads), 0, s, a);
+        return hipGetLastError();
+    }
+    if (a.refs != a.refs_in) {
+        const hipError_t e = copy_words(a.refs_in, a.refs, a.pages, s);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(reserve_count_kernel, dim3(static_cast<unsigned>((a.batch + 3) / 4)), dim3(256), 0, s, a);
-    hipLaunchKernelGGL(reserve_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
+    hipLaunchKernelGGL(reserve_rows_kernel, dim3(static_cast<unsigned>((a.batch + 3) / 4)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(reserve_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, s, a);
     return hipGetLastError();
 }
 
-hipError_t launch_page_fork(const PageFork& a, const int32_t* refs_in, const PageMoves& m, hipStream_t s) {
-    if (a.refs != refs_in) {
-        const hipError_t e = copy_words(refs_in, a.refs, a.pages, s);
-        if (e != hipSuccess) return e;
+hipError_t launch_page_fork(const PageFork& a, const PageMoves& m, hipStream_t s) {
+    if (plan_alone(a.batch, a.width, a.pages)) {
+        hipLaunchKernelGGL(fork_plan_kernel<true>, dim3(1), dim3(kPlanThreads), 0, s, a);
+    } else {
+        if (a.refs != a.refs_in) {
+            const hipError_t e = copy_words(a.refs_in, a.refs, a.pages, s);
+            if (e != hipSuccess) return e;
+        }
+        hipLaunchKernelGGL(fork_rows_kernel, dim3(static_cast<unsigned>((a.batch + 3) / 4)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(fork_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, s, a);
     }
-    hipLaunchKernelGGL(fork_rows_kernel, dim3(static_cast<unsigned>(a.batch)), dim3(256), 0, s, a);
-    hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
     hipLaunchKernelGGL(move_pages_kernel, dim3(blocks_for(a.batch * m.layers * m.parts, 1, 2048)), dim3(256), 0, s, m);
     return hipGetLastError();
 }

@@ -140,44 +140,47 @@ def allocate_paged_cache(layers: int, pages: int, kv_heads: int, *, page_tokens:
                         dim_group_size)
 
 
-def _check_pool(cache: PagedKVCache) -> None:
-    g = cache.dim_group_size
-    if g not in (16, 32, 64):
-        raise ValueError("dim_group_size must be one of 16, 32, 64")
-    codes, scales = cache.codes, cache.scales
-    if codes.ndim != 6 or codes.dtype != torch.uint8 or tuple(codes.shape[4:]) != (2, 64) or not codes.is_contiguous():
-        raise ValueError("codes must be a contiguous uint8 [layers, pages, KV heads, page tokens, 2, 64]")
-    if tuple(scales.shape) != (*codes.shape[:5], 128 // g, 2) or scales.dtype != torch.float16 \
-            or not scales.is_contiguous():
-        raise ValueError(f"scales must be a contiguous float16 {[*codes.shape[:5], 128 // g, 2]}")
-    if cache.page_tokens not in PAGE_TOKENS:
-        raise ValueError(f"page_tokens must be one of {PAGE_TOKENS}")
+# (The checks below run at every call of a decode loop, which the host can
+# bound: each reads a shape once.)
 
-
-def _check_table(pages: PageTable, what: str = "page table") -> None:
-    t = pages.table
-    if t.ndim != 2 or t.dtype != torch.int32 or not t.is_contiguous() or t.numel() == 0:
+def _check_table(pages: PageTable, what: str = "page table") -> tuple[int, int, int]:
+    """Shapes and types of a page table (ValueError): (batch, width, pages)."""
+    table, counts, refs = pages.table, pages.counts, pages.refs
+    shape, held = table.shape, refs.shape
+    if len(shape) != 2 or table.dtype is not torch.int32 or not table.is_contiguous() or not shape[0] or not shape[1]:
         raise ValueError(f"{what}: table must be a contiguous int32 [batch, width]")
-    if tuple(pages.counts.shape) != (int(t.shape[0]),) or pages.counts.dtype != torch.int64 \
-            or not pages.counts.is_contiguous():
+    if counts.shape != shape[:1] or counts.dtype is not torch.int64 or not counts.is_contiguous():
         raise ValueError(f"{what}: counts must be a contiguous int64 [batch]")
-    if pages.refs.ndim != 1 or pages.refs.dtype != torch.int32 or not pages.refs.is_contiguous() \
-            or pages.refs.numel() == 0:
+    if len(held) != 1 or refs.dtype is not torch.int32 or not refs.is_contiguous() or not held[0]:
         raise ValueError(f"{what}: refs must be a contiguous int32 [pages]")
     if pages.page_tokens not in PAGE_TOKENS:
         raise ValueError(f"page_tokens must be one of {PAGE_TOKENS}")
+    return shape[0], shape[1], held[0]
 
 
-def _check_cache(cache: PagedKVCache, pages: PageTable) -> None:
-    _check_pool(cache)
-    _check_table(pages)
-    if pages.page_tokens != cache.page_tokens or int(pages.refs.numel()) != cache.pages:
+def _check_cache(cache: PagedKVCache, pages: PageTable, layer: int = 0) -> tuple[tuple[int, int, int], tuple]:
+    """Shapes and types of a pool and its page table (ValueError):
+    (batch, width, KV heads), and the C entries' arguments for a layer, from
+    the codes to the batch."""
+    batch, width, count = _check_table(pages)
+    codes, scales, g = cache.codes, cache.scales, cache.dim_group_size
+    if g != 16 and g != 32 and g != 64:
+        raise ValueError("dim_group_size must be one of 16, 32, 64")
+    shape = codes.shape
+    if len(shape) != 6 or codes.dtype is not torch.uint8 or shape[4] != 2 or shape[5] != 64 or not codes.is_contiguous():
+        raise ValueError("codes must be a contiguous uint8 [layers, pages, KV heads, page tokens, 2, 64]")
+    layers, held, kv_heads, page_tokens = shape[:4]
+    want = (layers, held, kv_heads, page_tokens, 2, 128 // g, 2)
+    if scales.shape != want or scales.dtype is not torch.float16 or not scales.is_contiguous():
+        raise ValueError(f"scales must be a contiguous float16 {list(want)}")
+    if pages.page_tokens != page_tokens or count != held:
         raise ValueError("the page table belongs to a pool of another page size or page count")
-
-
-def _check_layer(cache: PagedKVCache, layer: int) -> None:
-    if not 0 <= layer < cache.layers:
-        raise ValueError(f"layer must be in [0, {cache.layers})")
+    if not 0 <= layer < layers:
+        raise ValueError(f"layer must be in [0, {layers})")
+    rows = layer * held * kv_heads * page_tokens
+    return (batch, width, kv_heads), (codes.data_ptr() + rows * 128, scales.data_ptr() + rows * (1024 // g), held,
+                                      kv_heads, page_tokens, g, pages.table.data_ptr(), width, pages.counts.data_ptr(),
+                                      batch)
 
 
 def _check_status(status: torch.Tensor | None) -> None:
@@ -189,7 +192,7 @@ def _on_device(first: torch.Tensor, *tensors: torch.Tensor | None) -> torch.devi
     """Every operand on the first one's CUDA device (RuntimeError, as
     elsewhere in the package)."""
     dev = first.device
-    if dev.type != "cuda":
+    if not first.is_cuda:
         raise RuntimeError("the paged cache must be on a CUDA device")
     for t in tensors:
         if t is not None and t.device != dev:
@@ -198,16 +201,9 @@ def _on_device(first: torch.Tensor, *tensors: torch.Tensor | None) -> torch.devi
 
 
 def _tokens(tokens: torch.Tensor, batch: int) -> torch.Tensor:
-    if tuple(tokens.shape) != (batch,) or tokens.dtype != torch.int64:
+    if tokens.shape != (batch,) or tokens.dtype is not torch.int64:
         raise ValueError(f"tokens must be an int64 [{batch}] tensor")
     return tokens.contiguous()
-
-
-def _pool_args(cache: PagedKVCache, layer: int, pages: PageTable) -> tuple:
-    return (cache.codes.data_ptr() + layer * cache.codes.stride(0),
-            cache.scales.data_ptr() + layer * cache.scales.stride(0) * 2, cache.pages, cache.kv_heads,
-            cache.page_tokens, cache.dim_group_size, pages.table.data_ptr(), int(pages.table.shape[1]),
-            pages.counts.data_ptr(), pages.batch)
 
 
 def _rows4(x: torch.Tensor, batch: int, kv_heads: int, what: str) -> torch.Tensor:
@@ -215,31 +211,35 @@ def _rows4(x: torch.Tensor, batch: int, kv_heads: int, what: str) -> torch.Tenso
     rows; a [B, KVH, 128] is one row."""
     if x.ndim == 3:
         x = x.unsqueeze(2)
-    if x.ndim != 4 or int(x.shape[0]) != batch or int(x.shape[1]) != kv_heads or int(x.shape[3]) != 128:
+    shape = x.shape
+    if len(shape) != 4 or shape[0] != batch or shape[1] != kv_heads or shape[3] != 128:
         raise ValueError(f"{what} must be [{batch}, {kv_heads}, rows, 128] or [{batch}, {kv_heads}, 128]")
     if x.dtype not in _FLOATS:
         raise RuntimeError(f"{x.dtype} is not supported; expected fp32/fp16/bf16")
-    size = x.element_size()
-    if x.stride(3) != 1 or x.data_ptr() % 16 or any(s * size % 16 or s < 0 for s in x.stride()[:3]):
-        x = x.contiguous()
+    if x.data_ptr() % 16 or not x.is_contiguous():
+        unit = 16 // x.element_size()
+        strides = x.stride()
+        if strides[3] != 1 or x.data_ptr() % 16 or any(s % unit for s in strides[:3]):
+            x = _aligned(x)
     return x
 
 
 def _new_table(pages: PageTable, out: PageTable | None) -> PageTable:
     """The table a call writes: `out`, or a new one."""
+    if out is pages:
+        return pages
     if out is None:
         return PageTable(torch.empty_like(pages.table), torch.empty_like(pages.counts), torch.empty_like(pages.refs),
                          pages.page_tokens, pages.bound)
-    if out is not pages:
-        _check_table(out, "out")
-        if out.table.shape != pages.table.shape or out.refs.shape != pages.refs.shape \
-                or out.page_tokens != pages.page_tokens:
-            raise ValueError("out must have the page table's shape")
-        same = [a.data_ptr() == b.data_ptr() for a, b in ((out.table, pages.table), (out.counts, pages.counts),
-                                                          (out.refs, pages.refs))]
-        if any(same) and not all(same):
-            raise ValueError("out shares some of the page table's tensors: share all of them or none")
-        out.bound = pages.bound
+    _check_table(out, "out")
+    if out.table.shape != pages.table.shape or out.refs.shape != pages.refs.shape \
+            or out.page_tokens != pages.page_tokens:
+        raise ValueError("out must have the page table's shape")
+    same = [a.data_ptr() == b.data_ptr() for a, b in ((out.table, pages.table), (out.counts, pages.counts),
+                                                      (out.refs, pages.refs))]
+    if any(same) and not all(same):
+        raise ValueError("out shares some of the page table's tensors: share all of them or none")
+    out.bound = pages.bound
     return out
 
 
@@ -252,26 +252,25 @@ def reserve_pages(pages: PageTable, tokens: int | torch.Tensor = 1, *, bound: in
     once the rows are written.  Returns a new page table, or writes ``out``
     (which may be ``pages``: in place).  ``bound``: the most tokens a sequence
     will hold, checked against the table's width."""
-    _check_table(pages)
+    batch, width, count = _check_table(pages)
     _check_status(status)
     if bound is not None and bound > pages.capacity:
         raise RuntimeError("the page table has no entries left")
     each = 0
     if isinstance(tokens, torch.Tensor):
-        tokens = _tokens(tokens, pages.batch)
+        tokens = _tokens(tokens, batch)
     else:
         each, tokens = int(tokens), None
         if each < 0:
             raise ValueError("tokens must not be negative")
     new = _new_table(pages, out)
     dev = _on_device(pages.table, pages.counts, pages.refs, tokens, status, new.table, new.counts, new.refs)
-    nbytes = int(nat.lib().popkv_page_reserve_workspace_bytes(pages.batch, int(pages.refs.numel())))
+    nbytes = nat.lib().popkv_page_reserve_workspace_bytes(batch, count)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with nat.on_device(dev):
         nat.call("popkv_page_reserve", pages.table.data_ptr(), pages.counts.data_ptr(), pages.refs.data_ptr(),
-                 new.table.data_ptr(), new.counts.data_ptr(), new.refs.data_ptr(), int(pages.table.shape[1]),
-                 pages.batch, int(pages.refs.numel()), pages.page_tokens, nat.ptr(tokens), each, nat.ptr(status),
-                 ws.data_ptr(), nbytes, nat.stream_of(dev))
+                 new.table.data_ptr(), new.counts.data_ptr(), new.refs.data_ptr(), width, batch, count,
+                 pages.page_tokens, nat.ptr(tokens), each, nat.ptr(status), ws.data_ptr(), nbytes, nat.stream_of(dev))
     return new
 
 
@@ -283,20 +282,18 @@ def write_tokens(cache: PagedKVCache, layer: int, pages: PageTable, k: torch.Ten
     ``tokens[b]`` (int64 [B] on the device; None: all rows).  The pages come
     from ``reserve_pages``; a row without one is not written and sets
     ``status`` (bit 4, or bit 1 past the table's end)."""
-    _check_cache(cache, pages)
-    _check_layer(cache, layer)
+    (batch, _, kv_heads), pool = _check_cache(cache, pages, layer)
     _check_status(status)
-    k = _rows4(k, pages.batch, cache.kv_heads, "new keys")
-    v = _rows4(v, pages.batch, cache.kv_heads, "new values")
+    k = _rows4(k, batch, kv_heads, "new keys")
+    v = _rows4(v, batch, kv_heads, "new values")
     if k.shape != v.shape or k.dtype != v.dtype:
         raise ValueError("new keys and values must share shape and dtype")
     if tokens is not None:
-        tokens = _tokens(tokens, pages.batch)
+        tokens = _tokens(tokens, batch)
     dev = _on_device(cache.codes, cache.scales, pages.table, pages.counts, k, v, tokens, status)
     with nat.on_device(dev):
         nat.call("popkv_paged_write", k.data_ptr(), v.data_ptr(), nat.dtype_code(k), *k.stride()[:3], *v.stride()[:3],
-                 int(k.shape[2]), nat.ptr(tokens), *_pool_args(cache, layer, pages), nat.ptr(status),
-                 nat.stream_of(dev))
+                 k.shape[2], nat.ptr(tokens), *pool, nat.ptr(status), nat.stream_of(dev))
 
 
 def read_tokens(cache: PagedKVCache, layer: int, pages: PageTable, *, dtype: torch.dtype = torch.bfloat16,
@@ -305,50 +302,53 @@ def read_tokens(cache: PagedKVCache, layer: int, pages: PageTable, *, dtype: tor
     """One layer's cached rows as K, V [B, KVH, rows, 128] (``rows``: default
     ``pages.bound``).  Rows past a sequence's count are zero in new tensors and
     left as they are in ``out``."""
-    _check_cache(cache, pages)
-    _check_layer(cache, layer)
+    (batch, _, kv_heads), pool = _check_cache(cache, pages, layer)
     if out is None:
         rows = pages.bound if rows is None else int(rows)
         if rows < 0:
             raise ValueError("rows must not be negative")
         if dtype not in _FLOATS:
             raise RuntimeError(f"{dtype} is not supported; expected fp32/fp16/bf16")
-        shape = (pages.batch, cache.kv_heads, rows, 128)
-        k, v = (torch.empty(shape, dtype=dtype, device=cache.codes.device) for _ in range(2))
+        k = torch.empty((batch, kv_heads, rows, 128), dtype=dtype, device=cache.codes.device)
+        v = torch.empty_like(k)
     else:
         k, v = out
-        if k.ndim != 4 or tuple(k.shape) != (pages.batch, cache.kv_heads, int(k.shape[2]), 128) \
-                or v.shape != k.shape or v.dtype != k.dtype or not k.is_contiguous() or not v.is_contiguous():
-            raise ValueError(f"out must be two contiguous [{pages.batch}, {cache.kv_heads}, rows, 128] tensors")
+        if k.ndim != 4 or tuple(k.shape) != (batch, kv_heads, int(k.shape[2]), 128) != k.shape \
+                or v.dtype != k.dtype or not k.is_contiguous() or not v.is_contiguous():
+            raise ValueError(f"out must be two contiguous [{batch}, {kv_heads}, rows, 128] tensors")
         if rows is not None and rows != int(k.shape[2]):
             raise ValueError("rows must be out's row count")
     dev = _on_device(cache.codes, cache.scales, pages.table, pages.counts, k, v)
     with nat.on_device(dev):
-        nat.call("popkv_paged_read", k.data_ptr(), v.data_ptr(), nat.dtype_code(k), int(k.shape[2]),
-                 1 if out is None else 0, *_pool_args(cache, layer, pages), nat.stream_of(dev))
+        nat.call("popkv_paged_read", k.data_ptr(), v.data_ptr(), nat.dtype_code(k), k.shape[2],
+                 1 if out is None else 0, *pool, nat.stream_of(dev))
     return k, v
 
 
-def _step_operands(q: torch.Tensor, cache: PagedKVCache, pages: PageTable, k: torch.Tensor, v: torch.Tensor,
-                   out: torch.Tensor | None) -> int:
-    batch, kv_heads = pages.batch, cache.kv_heads
-    if q.ndim != 3 or int(q.shape[0]) != batch or int(q.shape[2]) != 128:
+def _step_operands(q: torch.Tensor, batch: int, kv_heads: int, k: torch.Tensor, v: torch.Tensor,
+                   out: torch.Tensor | None) -> tuple[int, int]:
+    """Shapes and types of a step's operands: (query heads, dtype code)."""
+    shape = q.shape
+    if len(shape) != 3 or shape[0] != batch or shape[2] != 128:
         raise ValueError(f"q must be [{batch}, query heads, 128]")
-    q_heads = int(q.shape[1])
+    q_heads = shape[1]
     if q_heads <= 0 or q_heads % kv_heads != 0:
         raise ValueError("query heads must be a positive multiple of the KV heads")
-    for t, what in ((k, "current k"), (v, "current v")):
-        if tuple(t.shape) != (batch, kv_heads, 128):
-            raise ValueError(f"{what} must be [{batch}, {kv_heads}, 128]")
-    if out is not None and (tuple(out.shape) != tuple(q.shape) or not out.is_contiguous()):
+    want = (batch, kv_heads, 128)
+    if k.shape != want:
+        raise ValueError(f"current k must be [{batch}, {kv_heads}, 128]")
+    if v.shape != want:
+        raise ValueError(f"current v must be [{batch}, {kv_heads}, 128]")
+    dtype = q.dtype
+    if out is not None and (out.shape != shape or not out.is_contiguous()):
         raise ValueError("out must be a contiguous tensor shaped like q")
-    if any(t.dtype != q.dtype for t in (k, v, out) if t is not None):
+    if k.dtype != dtype or v.dtype != dtype or (out is not None and out.dtype != dtype):
         raise RuntimeError("queries, current K/V and out must share a dtype")
-    nat.dtype_code(q)
-    return q_heads
+    return q_heads, nat.dtype_code(q)
 
 
 def _aligned(x: torch.Tensor) -> torch.Tensor:
+    """x contiguous and 16-byte aligned."""
     x = x.contiguous()
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
@@ -364,24 +364,22 @@ def paged_attention_step(q: torch.Tensor, cache: PagedKVCache, layer: int, pages
     for the launch -- give the largest count a captured graph will see.  The
     workspace holds merge tickets and split states: do not share it with
     ``popkv_layer_step``."""
-    _check_cache(cache, pages)
-    _check_layer(cache, layer)
-    q_heads = _step_operands(q, cache, pages, k, v, out)
-    if q_heads // cache.kv_heads > 16:
+    (batch, width, kv_heads), pool = _check_cache(cache, pages, layer)
+    q_heads, dtype = _step_operands(q, batch, kv_heads, k, v, out)
+    if q_heads > 16 * kv_heads:
         raise ValueError("paged attention supports 1 to 16 query heads per KV head")
     most = pages.bound if max_tokens is None else int(max_tokens)
     if most < pages.bound:
         raise ValueError("max_tokens must cover the page table's bound")
-    most = min(most, pages.capacity)
+    most = min(most, width * pages.page_tokens)
     dev = _on_device(cache.codes, cache.scales, pages.table, pages.counts, q, k, v, out)
     qc, kc, vc = _aligned(q), _aligned(k), _aligned(v)
     output = torch.empty_like(qc) if out is None else out
-    nbytes = int(nat.lib().popkv_paged_attention_workspace_bytes(pages.batch, q_heads, cache.kv_heads, most))
-    ws = (workspace or LayerStepWorkspace()).get(nbytes, dev, pages.batch * cache.kv_heads)
+    nbytes = nat.lib().popkv_paged_attention_workspace_bytes(batch, q_heads, kv_heads, most)
+    ws = (workspace or LayerStepWorkspace()).get(nbytes, dev, batch * kv_heads)
     with nat.on_device(dev):
-        nat.call("popkv_paged_attention", qc.data_ptr(), nat.dtype_code(qc), *_pool_args(cache, layer, pages), most,
-                 kc.data_ptr(), vc.data_ptr(), q_heads, output.data_ptr(), ws.data_ptr(), ws.numel(),
-                 nat.stream_of(dev))
+        nat.call("popkv_paged_attention", qc.data_ptr(), dtype, *pool, most, kc.data_ptr(), vc.data_ptr(), q_heads,
+                 output.data_ptr(), ws.data_ptr(), ws.numel(), nat.stream_of(dev))
     return output
 
 
@@ -397,14 +395,14 @@ def paged_indexed_attention(q: torch.Tensor, cache: PagedKVCache, layer: int, pa
     ``valid_mask`` is False are left out, an index named twice counts twice,
     and a row with nothing left is zero.  head_to_kv: [QH] KV head indices.
     The workspace as for ``paged_attention_step``."""
-    _check_cache(cache, pages)
-    _check_layer(cache, layer)
-    q_heads = _step_operands(q, cache, pages, k, v, out)
-    if indices.ndim != 3 or tuple(indices.shape[:2]) != (pages.batch, q_heads) or int(indices.shape[2]) < 1:
-        raise ValueError(f"indices must be [{pages.batch}, {q_heads}, selected tokens]")
-    if valid_mask is not None and valid_mask.shape != indices.shape:
+    (batch, _, kv_heads), pool = _check_cache(cache, pages, layer)
+    q_heads, dtype = _step_operands(q, batch, kv_heads, k, v, out)
+    shape = indices.shape
+    if len(shape) != 3 or shape[0] != batch or shape[1] != q_heads or shape[2] < 1:
+        raise ValueError(f"indices must be [{batch}, {q_heads}, selected tokens]")
+    if valid_mask is not None and valid_mask.shape != shape:
         raise ValueError("valid mask must match indices")
-    if head_to_kv.ndim != 1 or int(head_to_kv.numel()) != q_heads:
+    if head_to_kv.ndim != 1 or head_to_kv.shape[0] != q_heads:
         raise ValueError(f"head_to_kv must be a vector of {q_heads} KV head indices")
     dev = _on_device(cache.codes, cache.scales, pages.table, pages.counts, q, k, v, out, indices, valid_mask)
     qc, kc, vc = _aligned(q), _aligned(k), _aligned(v)
@@ -412,14 +410,13 @@ def paged_indexed_attention(q: torch.Tensor, cache: PagedKVCache, layer: int, pa
     mask = None if valid_mask is None else valid_mask.to(torch.bool).contiguous().view(torch.uint8)
     mapping = head_to_kv.to(device=dev, dtype=torch.int64).contiguous()
     output = torch.empty_like(qc) if out is None else out
-    selected = int(idx.shape[2])
-    nbytes = int(nat.lib().popkv_paged_indexed_attention_workspace_bytes(pages.batch, q_heads, selected))
-    ws = (workspace or LayerStepWorkspace()).get(nbytes, dev, pages.batch * q_heads)
+    selected = shape[2]
+    nbytes = nat.lib().popkv_paged_indexed_attention_workspace_bytes(batch, q_heads, selected)
+    ws = (workspace or LayerStepWorkspace()).get(nbytes, dev, batch * q_heads)
     with nat.on_device(dev):
-        nat.call("popkv_paged_indexed_attention", qc.data_ptr(), nat.dtype_code(qc),
-                 *_pool_args(cache, layer, pages), kc.data_ptr(), vc.data_ptr(), idx.data_ptr(),
-                 _INDEX_CODES[idx.dtype], nat.ptr(mask), mapping.data_ptr(), q_heads, selected, output.data_ptr(),
-                 ws.data_ptr(), ws.numel(), nat.stream_of(dev))
+        nat.call("popkv_paged_indexed_attention", qc.data_ptr(), dtype, *pool, kc.data_ptr(), vc.data_ptr(),
+                 idx.data_ptr(), _INDEX_CODES[idx.dtype], nat.ptr(mask), mapping.data_ptr(), q_heads, selected,
+                 output.data_ptr(), ws.data_ptr(), ws.numel(), nat.stream_of(dev))
     return output
 
 
@@ -434,23 +431,20 @@ def fork_sequences(cache: PagedKVCache, pages: PageTable, parents: torch.Tensor,
     sets ``status`` bit 4; a parent outside the batch empties the sequence and
     sets bit 8.  Returns a new page table, or writes ``out`` (which may be
     ``pages``); the old one must not be written through any more."""
-    _check_cache(cache, pages)
+    (batch, width, kv_heads), pool = _check_cache(cache, pages)
     _check_status(status)
-    if tuple(parents.shape) != (pages.batch,) or parents.dtype != torch.int64:
-        raise ValueError(f"parents must be an int64 [{pages.batch}] tensor")
+    if parents.shape != (batch,) or parents.dtype is not torch.int64:
+        raise ValueError(f"parents must be an int64 [{batch}] tensor")
     new = _new_table(pages, out)
     dev = _on_device(cache.codes, cache.scales, pages.table, pages.counts, pages.refs, parents, status, new.table,
                      new.counts, new.refs)
     parents = parents.contiguous()
-    width = int(pages.table.shape[1])
-    nbytes = int(nat.lib().popkv_page_fork_workspace_bytes(pages.batch, width))
+    nbytes = nat.lib().popkv_page_fork_workspace_bytes(batch, width)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with nat.on_device(dev):
-        nat.call("popkv_page_fork", cache.codes.data_ptr(), cache.scales.data_ptr(), cache.layers, cache.pages,
-                 cache.kv_heads, cache.page_tokens, cache.dim_group_size, pages.table.data_ptr(),
-                 pages.counts.data_ptr(), pages.refs.data_ptr(), new.table.data_ptr(), new.counts.data_ptr(),
-                 new.refs.data_ptr(), width, pages.batch, parents.data_ptr(), nat.ptr(status), ws.data_ptr(), nbytes,
-                 nat.stream_of(dev))
+        nat.call("popkv_page_fork", pool[0], pool[1], cache.codes.shape[0], pool[2], kv_heads, pool[4], pool[5], pool[6],
+                 pool[8], pages.refs.data_ptr(), new.table.data_ptr(), new.counts.data_ptr(), new.refs.data_ptr(), width,
+                 batch, parents.data_ptr(), nat.ptr(status), ws.data_ptr(), nbytes, nat.stream_of(dev))
     return new
 
 
@@ -461,16 +455,14 @@ def compact_pages(cache: PagedKVCache, pages: PageTable, *, out: PageTable | Non
     Returns the new page table (or ``out``, which may be ``pages``) and the
     int32 [pages] map of where each live page is now (-1: it was free), for
     whoever holds pages outside this table."""
-    _check_cache(cache, pages)
+    (batch, width, kv_heads), pool = _check_cache(cache, pages)
     new = _new_table(pages, out)
     dev = _on_device(cache.codes, cache.scales, pages.table, pages.counts, pages.refs, new.table, new.counts, new.refs)
     page_map = torch.empty_like(pages.refs)
-    nbytes = int(nat.lib().popkv_page_compact_workspace_bytes(cache.pages))
+    nbytes = nat.lib().popkv_page_compact_workspace_bytes(pool[2])
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with nat.on_device(dev):
-        nat.call("popkv_page_compact", cache.codes.data_ptr(), cache.scales.data_ptr(), cache.layers, cache.pages,
-                 cache.kv_heads, cache.page_tokens, cache.dim_group_size, pages.table.data_ptr(),
-                 pages.counts.data_ptr(), pages.refs.data_ptr(), new.table.data_ptr(), new.counts.data_ptr(),
-                 new.refs.data_ptr(), int(pages.table.shape[1]), pages.batch, page_map.data_ptr(), ws.data_ptr(),
-                 nbytes, nat.stream_of(dev))
+        nat.call("popkv_page_compact", pool[0], pool[1], cache.codes.shape[0], pool[2], kv_heads, pool[4], pool[5],
+                 pool[6], pool[8], pages.refs.data_ptr(), new.table.data_ptr(), new.counts.data_ptr(),
+                 new.refs.data_ptr(), width, batch, page_map.data_ptr(), ws.data_ptr(), nbytes, nat.stream_of(dev))
     return new, page_map
