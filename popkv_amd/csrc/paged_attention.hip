@@ -46,12 +46,22 @@ __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {
 
 // Nibble pairs (0, 4), (1, 5), (2, 6), (3, 7) of w as fp16 1024 + c (first and
 // third) and 1024 + 16 c.
-__device__ __forceinline__ void biased_pairs(uint32_t w, uint32_t (&out)[4]) {
+// The constants sit in registers (an instruction takes one literal here, and
+// with two the compiler makes an "and" and an "or" of it).
+struct CodeBits {
+    uint32_t even = 0x000f000fu, odd = 0x00f000f0u, bias = 0x64006400u;
+    __device__ __forceinline__ CodeBits() {
+        asm("" : "+s"(even));
+        asm("" : "+s"(odd));
+        asm("" : "+v"(bias));
+    }
+};
+__device__ __forceinline__ void biased_pairs(const CodeBits& k, uint32_t w, uint32_t (&out)[4]) {
     const uint32_t x = w >> 8;
-    out[0] = (w & 0x000f000fu) | 0x64006400u;
-    out[1] = (w & 0x00f000f0u) | 0x64006400u;
-    out[2] = (x & 0x000f000fu) | 0x64006400u;
-    out[3] = (x & 0x00f000f0u) | 0x64006400u;
+    out[0] = (w & k.even) | k.bias;
+    out[1] = (w & k.odd) | k.bias;
+    out[2] = (x & k.even) | k.bias;
+    out[3] = (x & k.odd) | k.bias;
 }
 
 // ---- the VALU fold ----------------------------------------------------------
@@ -244,6 +254,13 @@ constexpr int kDenseBlocks = 256;
 
 int64_t dense_target(int64_t kv_heads) { return kDenseBlocks / kv_heads < 1 ? 1 : kDenseBlocks / kv_heads; }
 
+// A wave-uniform 64-bit value as one the compiler knows to be uniform.
+__device__ __forceinline__ int64_t uniform64(int64_t v, int src = 0) {
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), src);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(static_cast<uint64_t>(v) >> 32), src);
+    return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+}
+
 // A workgroup's share: tokens [t0, t1) of sequence b, split `s` of `n`, the
 // sequence's first item.
 struct DenseShare {
@@ -265,6 +282,7 @@ __device__ __forceinline__ bool dense_share(const PagedView& c, int64_t max_toke
         for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o);
         total += n;
     }
+    total = uniform64(total);
     int64_t per = ((total + target - 1) / target + kDenseLeast - 1) / kDenseLeast * kDenseLeast;
     if (per < kDenseLeast) per = kDenseLeast;
     int base = 0;
@@ -281,7 +299,7 @@ __device__ __forceinline__ bool dense_share(const PagedView& c, int64_t max_toke
             out.n = __builtin_amdgcn_readlane(splits, src);
             out.s = item - out.first;
             out.t0 = out.s * per;
-            const int64_t n = __shfl(count, src);
+            const int64_t n = uniform64(count, src);
             out.t1 = min(n, out.t0 + per);
             return true;
         }
@@ -394,10 +412,10 @@ __device__ __forceinline__ void dense_merge(const PagedAttend& a, const PagedVie
 // 1024 times a group's sum must not), and the weights are kept around 2^8, where fp16 keeps
 // 11 bits; fp16 outputs take a second term for the rest of each weight.
 // The same pairs as low + c * delta.
-__device__ __forceinline__ void dequantise_pairs(uint32_t w, half2_t delta, half2_t low, uint32_t (&out)[4]) {
+__device__ __forceinline__ void dequantise_pairs(const CodeBits& k, uint32_t w, half2_t delta, half2_t low, uint32_t (&out)[4]) {
     const half2_t k1024 = {1024.0f16, 1024.0f16}, k16th = {0.0625f16, 0.0625f16}, k64 = {-64.0f16, -64.0f16};
     uint32_t b[4];
-    biased_pairs(w, b);
+    biased_pairs(k, w, b);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const half2_t c = i & 1 ? __builtin_elementwise_fma(as_half2(b[i]), k16th, k64) : as_half2(b[i]) - k1024;
@@ -516,6 +534,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
             ql[g / 4][g % 4] = grp < 2 ? x : 0u;
         }
     }
+    const CodeBits bits;
     const uint32_t low_or_delta = grp == 1 ? 0x03020302u : 0x01000100u;  // byte picks of a scale pair
 
     struct Tile {
@@ -601,7 +620,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
 #pragma unroll
             for (int st = 0; st < 4; ++st) {
                 uint32_t cb[4];
-                biased_pairs(w[st], cb);
+                biased_pairs(bits, w[st], cb);
                 if constexpr (R == 2) {
                     dot[st / 2] = mfma_f16(qa[0][st], cb, st & 1 ? dot[st / 2] : f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
                 } else {
@@ -617,8 +636,10 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
                 for (int i = 0; i < 4; ++i) s[u][i] = fmaf(delta, dot[g][i], s[u][i]);
             }
         }
+        const bool whole = x.left == kPageTile;  // uniform; the branches stay branches
         bool live[2] = {true, true};
-        if (x.left != kPageTile) {  // uniform
+        if (!whole) {
+            asm volatile("");
 #pragma unroll
             for (int u = 0; u < 2; ++u) live[u] = col + 16 * u < x.left;
 #pragma unroll
@@ -626,13 +647,22 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
                 if (4 * grp + (j >> 1) + 16 * (j & 1) >= x.left) x.vs[j] = 0u;  // what lies behind the last token may be anything
         }
         float e[4][2], top = -INFINITY;
+        auto exponents = [&] {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                e[i][u] = live[u] ? fmaf(s[u][i], factor[i], -ref[i]) : -INFINITY;
-                top = fmaxf(top, e[i][u]);
+                for (int u = 0; u < 2; ++u) e[i][u] = fmaf(s[u][i], factor[i], -ref[i]);
+            if (!whole) {
+                asm volatile("");
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) e[i][u] = live[u] ? e[i][u] : -INFINITY;
             }
+        };
+        exponents();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(e[i][0], e[i][1]));
         if (__ballot(top > kTop) != 0) {  // some weight would pass 2^15
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -647,9 +677,8 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
 #pragma unroll
                 for (int d = 0; d < 8; ++d) acc[d][i] *= f;
                 ref[i] = to;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) e[i][u] = live[u] ? fmaf(s[u][i], factor[i], -to) : -INFINITY;
             }
+            exponents();
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -683,7 +712,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
             for (int j = 0; j < 4; ++j) {
                 const uint32_t v0 = x.v[2 * j], v1 = x.v[2 * j + 1];
                 uint32_t d[4];
-                dequantise_pairs(half ? high_halves(v0, v1) : low_halves(v0, v1),
+                dequantise_pairs(bits, half ? high_halves(v0, v1) : low_halves(v0, v1),
                                  as_half2(high_halves(x.vs[2 * j], x.vs[2 * j + 1])),
                                  as_half2(low_halves(x.vs[2 * j], x.vs[2 * j + 1])), d);
 #pragma unroll
@@ -820,6 +849,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
 template <typename T>
 struct PickFold {
     FoldState<1> st;
+    CodeBits bits;
     uint32_t qh[8];
     float qsum, factor, mid;
     __device__ __forceinline__ void start(const T* src) {
@@ -847,10 +877,10 @@ struct PickFold {
 #pragma unroll
             for (int j = 0; j < 4; ++j) qh[4 * w + j] = pack_half2(q[8 * w + j], q[8 * w + j + 4]);
     }
-    static __device__ __forceinline__ void centred(uint32_t w, half2_t (&out)[4]) {
+    static __device__ __forceinline__ void centred(const CodeBits& k, uint32_t w, half2_t (&out)[4]) {
         const half2_t k1032 = {1032.0f16, 1032.0f16}, k16th = {0.0625f16, 0.0625f16}, k72 = {-72.0f16, -72.0f16};
         uint32_t b[4];
-        biased_pairs(w, b);
+        biased_pairs(k, w, b);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             out[j] = j & 1 ? __builtin_elementwise_fma(as_half2(b[j]), k16th, k72) : as_half2(b[j]) - k1032;
@@ -863,7 +893,7 @@ struct PickFold {
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 half2_t c[4];
-                centred(w ? r[t].k.y : r[t].k.x, c);
+                centred(bits, w ? r[t].k.y : r[t].k.x, c);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) dot = __builtin_amdgcn_fdot2(as_half2(qh[4 * w + j]), c[j], dot, false);
             }
@@ -890,7 +920,7 @@ struct PickFold {
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 half2_t c[4];
-                centred(w ? r[t].v.y : r[t].v.x, c);
+                centred(bits, w ? r[t].v.y : r[t].v.x, c);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     st.acc[0][8 * w + j] = fmaf(static_cast<float>(c[j][0]), pd, st.acc[0][8 * w + j]);
