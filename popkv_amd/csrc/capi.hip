@@ -910,7 +910,10 @@ void carve_compact(Carve& c, popkv::PageCompact& a) {
     a.moves = c.take<int32_t>(1);
 }
 
-size_t attend_tickets(int64_t rows) { return align_up(static_cast<size_t>(rows) * 4); }
+// The merge tickets at the start of the attention workspaces: the same size for
+// both calls, so that one workspace serves both (rows: batch * KVH, or batch *
+// QH indexed).
+size_t attend_tickets(int64_t rows) { return align_up(static_cast<size_t>(rows) * popkv::kPagedTickets * 4); }
 
 }  // namespace
 
@@ -979,6 +982,8 @@ int popkv_paged_attention(const void* queries, int32_t dtype, const void* codes,
     if (q_heads <= 0 || q_heads > 65535 || q_heads % kv_heads != 0 || q_heads / kv_heads > 16)
         return fail(POPKV_ERR_UNSUPPORTED, "paged attention supports 1 to 16 query heads per KV head");
     if (max_tokens < 0 || max_tokens > (int64_t{1} << 30)) return fail(POPKV_ERR_TOKENS, "invalid token count");
+    if (batch * ceil_div(max_tokens, 32) > 0x7fffffff)
+        return fail(POPKV_ERR_UNSUPPORTED, "batch * max_tokens must stay below 2^36 tokens");
     if (workspace_bytes < popkv_paged_attention_workspace_bytes(batch, q_heads, kv_heads, max_tokens))
         return fail(POPKV_ERR_WORKSPACE, "paged attention needs %zu workspace bytes",
                     popkv_paged_attention_workspace_bytes(batch, q_heads, kv_heads, max_tokens));

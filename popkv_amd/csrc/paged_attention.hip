@@ -189,7 +189,7 @@ __device__ __forceinline__ bool last_of(uint32_t* ticket, uint32_t n, uint32_t* 
 // a lane owns dims lane and lane + 64.
 __device__ __forceinline__ void fold_states(const float* ps, int64_t stride, int n, float& m, float& l, float& a0,
                                             float& a1) {
-    constexpr int NF = 16;
+    constexpr int NF = 32;
     const int lane = threadIdx.x & (kWave - 1);
     for (int s0 = 0; s0 < n; s0 += NF) {
         float ms = -INFINITY, ls = 0.0f, x0[NF], x1[NF];
@@ -246,118 +246,156 @@ __device__ __forceinline__ void finish_row(float m, float l, float a0, float a1,
 
 // ---- dense ------------------------------------------------------------------
 
+// Workgroups of eight waves, one a CU.  (Four waves three times a CU, with as
+// many bytes again on their way, were slower, 137 against 116 us at 8 x 64K and
+// 43 against 35 at 131071 tokens: three times as many states to merge, and more
+// places of memory read at once.)
 constexpr int kDenseWaves = 8;
 constexpr int kDenseThreads = kDenseWaves * kWave;
-// Tokens of a split: at least a tile for every wave.
-constexpr int kDenseLeast = kDenseWaves * kPageTile;
 constexpr int kDenseBlocks = 256;
 
-int64_t dense_target(int64_t kv_heads) { return kDenseBlocks / kv_heads < 1 ? 1 : kDenseBlocks / kv_heads; }
-
-// A wave-uniform 64-bit value as one the compiler knows to be uniform.
-__device__ __forceinline__ int64_t uniform64(int64_t v, int src = 0) {
-    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), src);
-    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(static_cast<uint64_t>(v) >> 32), src);
-    return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+// Workgroups of a KV head: one a CU in all, with a tile for each wave.
+int dense_workgroups(int64_t batch, int64_t kv_heads, int64_t max_tokens) {
+    const int64_t target = kDenseBlocks / kv_heads < 1 ? 1 : kDenseBlocks / kv_heads;
+    const int64_t tiles = batch * ((max_tokens + kPageTile - 1) / kPageTile);
+    const int64_t most = (tiles + kDenseWaves - 1) / kDenseWaves;
+    return static_cast<int>(most < 1 ? 1 : most < target ? most : target);
 }
 
-// A workgroup's share: tokens [t0, t1) of sequence b, split `s` of `n`, the
-// sequence's first item.
+// A workgroup's part of a sequence: tokens [t0, t1) of sequence b, part s of n;
+// its state goes to place first + s.
 struct DenseShare {
-    int b, s, n, first;
-    int64_t t0, t1;
+    int b, s, n, first, t0, t1;
 };
 
-// The splits follow the real lengths, read on the device: every split holds at
-// most total / target tokens (at least kDenseLeast), so a batch of short and
-// long sequences is shared out evenly, in at most target + batch items.  Each
-// wave works it out by itself from the counts.
-__device__ __forceinline__ bool dense_share(const PagedView& c, int64_t max_tokens, int target, int item,
-                                            DenseShare& out) {
+// The work of one KV head is the batch's tiles of 32 tokens laid end to end,
+// cut among the grid's workgroups by the real lengths, which are read on the
+// device: every workgroup takes as many tiles (at least one a wave), whether they
+// are part of one long sequence or several short ones, and calls f for each of
+// the sequences that it has some of.  (Splits of each sequence by itself left a
+// few workgroups more than fit at once, a second round: a ragged batch of five up
+// to 20001, 64 query heads over 8 KV heads fp16 35 us.)  An empty sequence
+// belongs to the workgroup at whose tiles it lies.  Workgroup w's state for
+// sequence b has place w + b: one of the two grows from a part to the next, so
+// places differ.  Each wave works this out by itself from the counts.  (The
+// entry refuses batches of 2^31 tiles and more.)
+template <typename F>
+__device__ __forceinline__ void dense_walk(const PagedView& c, int64_t max_tokens, int groups, F&& f) {
     const int lane = threadIdx.x & (kWave - 1);
+    const int w = div_nonneg(blockIdx.x, c.kv_heads);
     const int64_t most = min(c.width << c.page_log2, max_tokens);
-    int64_t total = 0;
-    for (int b0 = 0; b0 < c.batch; b0 += kWave) {
-        int64_t n = b0 + lane < c.batch ? clamp_count(c.counts[b0 + lane], most) : 0;
-        for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o);
-        total += n;
-    }
-    total = uniform64(total);
-    int64_t per = ((total + target - 1) / target + kDenseLeast - 1) / kDenseLeast * kDenseLeast;
-    if (per < kDenseLeast) per = kDenseLeast;
+    auto count_of = [&](int b) { return b < c.batch ? static_cast<int>(clamp_count(c.counts[b], most)) : 0; };
+    auto tiles_of = [](int count) { return (count + kPageTile - 1) / kPageTile; };
+    auto scan = [&](int v) { return static_cast<int>(wave_incl_scan(static_cast<uint32_t>(v), lane)); };
+    const int count0 = count_of(lane), incl0 = scan(tiles_of(count0));
+    int total = __builtin_amdgcn_readlane(incl0, kWave - 1);
+    for (int b0 = kWave; b0 < c.batch; b0 += kWave)
+        total += __builtin_amdgcn_readlane(scan(tiles_of(count_of(b0 + lane))), kWave - 1);
+    const int per = max(div_nonneg(total + groups - 1, groups), kDenseWaves);
+    // (w * per may pass 2^31 only past the last tile)
+    const int r0 = static_cast<int>(min<int64_t>(static_cast<int64_t>(w) * per, total)), r1 = min(r0 + per, total);
+    if (w > 0 && r0 >= total) return;
+    const bool last = r1 >= total;
     int base = 0;
-    for (int b0 = 0; b0 < c.batch; b0 += kWave) {
-        const int64_t count = b0 + lane < c.batch ? clamp_count(c.counts[b0 + lane], most) : 0;
-        const int splits = b0 + lane < c.batch ? max(1, static_cast<int>((count + per - 1) / per)) : 0;
-        const int incl = static_cast<int>(wave_incl_scan(static_cast<uint32_t>(splits), lane));
-        const int excl = base + incl - splits;
-        const uint64_t mine = __ballot(item >= excl && item < excl + splits);
-        if (mine) {
-            const int src = __ffsll(static_cast<unsigned long long>(mine)) - 1;
-            out.b = b0 + src;
-            out.first = __builtin_amdgcn_readlane(excl, src);
-            out.n = __builtin_amdgcn_readlane(splits, src);
-            out.s = item - out.first;
-            out.t0 = out.s * per;
-            const int64_t n = uniform64(count, src);
-            out.t1 = min(n, out.t0 + per);
-            return true;
+    for (int b0 = 0; b0 < c.batch && (last || base < r1); b0 += kWave) {
+        const int count = b0 == 0 ? count0 : count_of(b0 + lane);
+        const int tiles = tiles_of(count), incl = b0 == 0 ? incl0 : scan(tiles);
+        const int start = base + incl - tiles;
+        const bool here =
+            b0 + lane < c.batch && (tiles ? start < r1 && start + tiles > r0 : start >= r0 && (last || start < r1));
+        for (uint64_t mask = __ballot(here); mask; mask &= mask - 1) {
+            const int src = __ffsll(static_cast<unsigned long long>(mask)) - 1;
+            const int from = __builtin_amdgcn_readlane(start, src), to = from + __builtin_amdgcn_readlane(tiles, src);
+            DenseShare sh;
+            sh.b = b0 + src;
+            const int w0 = from >= r0 ? w : from / per, w1 = to <= r1 ? w : (to - 1) / per;
+            sh.s = w - w0;
+            sh.n = w1 - w0 + 1;
+            sh.first = w0 + sh.b;
+            sh.t0 = (max(from, r0) - from) * kPageTile;
+            sh.t1 = min(__builtin_amdgcn_readlane(count, src), (min(to, r1) - from) * kPageTile);
+            f(sh);
         }
         base += __builtin_amdgcn_readlane(incl, kWave - 1);
     }
-    return false;
 }
 
-// The workgroup's waves hold `rows` states each in LDS (row-major: s_m, s_l
-// [W][rows], s_acc [W][rows][128]); rows r0 .. of the item's group go to the
-// partials as one state each.
-template <int ROWS, int PITCH>
-__device__ __forceinline__ void store_states(const float (*s_m)[ROWS], const float (*s_l)[ROWS],
-                                             const float (*s_acc)[ROWS][PITCH], int rows, float* dst) {
-    for (int i = threadIdx.x; i < rows * 128; i += kDenseThreads) {
+// A row's logit with the current token, by one wave.
+template <typename T>
+__device__ __forceinline__ float current_logit(const T* q, const T* ck) {
+    const int lane = threadIdx.x & (kWave - 1);
+    return scaled_logit(wave_sum(fmaf(Elem<T>::load(q, lane), Elem<T>::load(ck, lane),
+                                      Elem<T>::load(q, lane + 64) * Elem<T>::load(ck, lane + 64))));
+}
+
+// The workgroup's waves hold the states of rows r0 .. r0 + rows - 1 of the
+// group in LDS (s_m, s_l [W][ROWS], s_acc [W][ROWS][PITCH]): one state each to the partials, or, where the part is the whole
+// sequence, the rows' outputs.
+template <typename T, int ROWS, int PITCH>
+__device__ __forceinline__ void emit_rows(const PagedAttend& a, const PagedView& c, const DenseShare& sh, int h,
+                                          int group, int r0, const float (*s_m)[ROWS], const float (*s_l)[ROWS],
+                                          const float (*s_acc)[ROWS][PITCH]) {
+    constexpr int W = kDenseWaves;
+    __shared__ float s_cur[ROWS];
+    const int rows = min(ROWS, group - r0);
+    const int64_t kv = (static_cast<int64_t>(sh.b) * c.kv_heads + h) * 128;
+    const int64_t row0 = static_cast<int64_t>(sh.b) * a.q_heads + static_cast<int64_t>(h) * group + r0;
+    if (sh.n == 1) {
+        for (int r = threadIdx.x / kWave; r < rows; r += W) {
+            const float x = current_logit(static_cast<const T*>(a.q) + (row0 + r) * 128,
+                                          static_cast<const T*>(a.cur_k) + kv);
+            if ((threadIdx.x & (kWave - 1)) == 0) s_cur[r] = x;
+        }
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < rows * 128; i += W * kWave) {
         const int j = i / 128, d = i % 128;
         float mx = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kDenseWaves; ++w) mx = fmaxf(mx, s_m[w][j]);
-        float a = 0.0f, l = 0.0f;
+        for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_m[w][j]);
+        if (sh.n == 1) mx = fmaxf(mx, s_cur[j]);
+        float x = 0.0f, l = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kDenseWaves; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float f = state_weight(s_m[w][j], s_l[w][j], mx);
-            a = fmaf(f, s_acc[w][j][d], a);
+            x = fmaf(f, s_acc[w][j][d], x);
             l = fmaf(f, s_l[w][j], l);
         }
-        float* p = dst + static_cast<int64_t>(j) * kState;
-        st_f32<true>(p + 2 + d, a);
-        if (d == 0) {
-            st_f32<true>(p, mx);
-            st_f32<true>(p + 1, l);
+        if (sh.n == 1) {
+            const float s = s_cur[j], f = s == -INFINITY && mx != -INFINITY ? 0.0f : exp2_fast(s - mx);
+            x = fmaf(f, Elem<T>::load(static_cast<const T*>(a.cur_v) + kv, d), x);
+            Elem<T>::store(static_cast<T*>(a.out) + (row0 + j) * 128, d, x / (l + f));
+        } else {
+            float* p = a.partials +
+                       ((static_cast<int64_t>(sh.first + sh.s) * c.kv_heads + h) * group + r0 + j) * kState;
+            st_f32<true>(p + 2 + d, x);
+            if (d == 0) {
+                st_f32<true>(p, mx);
+                st_f32<true>(p + 1, l);
+            }
         }
     }
 }
 
-// The last workgroup of a (sequence, KV head) merges the group's rows: a row
-// takes a wave, or up to eight waves' shares of its splits where the group has
-// fewer rows than the workgroup waves.
-template <typename T>
-__device__ __forceinline__ void dense_merge(const PagedAttend& a, const PagedView& c, const DenseShare& sh, int h,
-                                            int group) {
-    __shared__ uint32_t s_last;
-    __shared__ float s_part[kDenseWaves][kState];
-    if (!last_of(a.tickets + sh.b * c.kv_heads + h, sh.n, &s_last)) return;
+// Merges `n` states of each of the group's rows, `stride` floats apart: a row
+// takes a wave, or several waves' shares of its states where the group has fewer
+// rows than the workgroup waves.  done(r, m, l, a0, a1) by the wave that has row
+// r's state.
+template <typename F>
+__device__ __forceinline__ void merge_rows(const float* ps, int64_t stride, int n, int group, F&& done) {
+    constexpr int W = kDenseWaves;
+    __shared__ float s_part[W][kState];
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     int share = 1;  // waves a row
-    while (share * 2 * group <= kDenseWaves && share * 2 <= sh.n) share *= 2;
-    const int at_once = kDenseWaves / share;
-    const int64_t stride = static_cast<int64_t>(c.kv_heads) * group * kState;
+    while (share * 2 * group <= W && share * 2 <= n) share *= 2;
+    const int at_once = W / share;
     for (int r0 = 0; r0 < group; r0 += at_once) {
         const int r = r0 + wave / share, part = wave % share;
         float m = -INFINITY, l = 0.0f, a0 = 0.0f, a1 = 0.0f;
         if (r < group) {
-            const int s0 = sh.n * part / share, s1 = sh.n * (part + 1) / share;
-            const float* ps = a.partials + (static_cast<int64_t>(sh.first + s0) * c.kv_heads + h) * group * kState +
-                              static_cast<int64_t>(r) * kState;
-            fold_states(ps, stride, s1 - s0, m, l, a0, a1);
+            const int s0 = n * part / share, s1 = n * (part + 1) / share;
+            fold_states(ps + s0 * stride + static_cast<int64_t>(r) * kState, stride, s1 - s0, m, l, a0, a1);
         }
         if (share > 1) {
             __syncthreads();
@@ -379,14 +417,51 @@ __device__ __forceinline__ void dense_merge(const PagedAttend& a, const PagedVie
                 }
             }
         }
-        if (part == 0 && r < group) {
-            const int64_t row = static_cast<int64_t>(sh.b) * a.q_heads + static_cast<int64_t>(h) * group + r;
-            const int64_t kv = (static_cast<int64_t>(sh.b) * c.kv_heads + h) * 128;
-            finish_row<T>(m, l, a0, a1, 1.0f, static_cast<const T*>(a.q) + row * 128,
-                          static_cast<const T*>(a.cur_k) + kv, static_cast<const T*>(a.cur_v) + kv,
-                          static_cast<T*>(a.out) + row * 128);
-        }
+        if (part == 0 && r < group) done(r, m, l, a0, a1);
     }
+}
+
+// The last workgroup of a (sequence, KV head) in several parts merges them.
+// More than kOneLevel merge in two levels, as one workgroup's reading of them is
+// what takes the time: the last workgroup of every kSet leaves the set's state
+// in the place of its first, and the last of those merges the sets'.  Tickets of
+// a (sequence, KV head): kTickets, the sets' from 1 on.
+constexpr int kOneLevel = 32, kSet = 16;
+static_assert(kDenseBlocks / kSet + 1 <= kPagedTickets);
+
+template <typename T>
+__device__ __forceinline__ void dense_merge(const PagedAttend& a, const PagedView& c, const DenseShare& sh, int h,
+                                            int group) {
+    __shared__ uint32_t s_last;
+    if (sh.n == 1) return;
+    const int lane = threadIdx.x & (kWave - 1);
+    uint32_t* tickets = a.tickets + (static_cast<int64_t>(sh.b) * c.kv_heads + h) * kPagedTickets;
+    const int64_t stride = static_cast<int64_t>(c.kv_heads) * group * kState;
+    float* ps = a.partials + (static_cast<int64_t>(sh.first) * c.kv_heads + h) * group * kState;
+    int n = sh.n, step = 1;
+    if (n > kOneLevel) {
+        const int set = sh.s / kSet, in_set = min(kSet, n - set * kSet);
+        float* dst = ps + set * kSet * stride;
+        if (!last_of(tickets + 1 + set, in_set, &s_last)) return;
+        merge_rows(dst, stride, in_set, group, [&](int r, float m, float l, float a0, float a1) {
+            float* p = dst + static_cast<int64_t>(r) * kState;
+            if (lane == 0) {
+                st_f32<true>(p, m);
+                st_f32<true>(p + 1, l);
+            }
+            st_f32<true>(p + 2 + lane, a0);
+            st_f32<true>(p + 66 + lane, a1);
+        });
+        n = (n + kSet - 1) / kSet;
+        step = kSet;
+    }
+    if (!last_of(tickets, n, &s_last)) return;
+    merge_rows(ps, step * stride, n, group, [&](int r, float m, float l, float a0, float a1) {
+        const int64_t row = static_cast<int64_t>(sh.b) * a.q_heads + static_cast<int64_t>(h) * group + r;
+        const int64_t kv = (static_cast<int64_t>(sh.b) * c.kv_heads + h) * 128;
+        finish_row<T>(m, l, a0, a1, 1.0f, static_cast<const T*>(a.q) + row * 128, static_cast<const T*>(a.cur_k) + kv,
+                      static_cast<const T*>(a.cur_v) + kv, static_cast<T*>(a.out) + row * 128);
+    });
 }
 
 // Matrix-core form (16-bit types), one workgroup a (share, KV head) for the
@@ -442,21 +517,31 @@ __device__ __forceinline__ void exchange_quarters(uint32_t (&d)[4]) {
 
 template <typename T, int G>
 __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAttend a, PagedView c, int64_t max_tokens,
-                                                                         int target) {
+                                                                         int groups) {
     constexpr int R = 128 / G;
     constexpr int HALVES = R == 8 ? 2 : 1;        // groups of a 32-dim step
     constexpr int LOWS = R == 8 ? 2 : 1;          // products for the low terms (four groups each)
     constexpr int TERMS = std::is_same_v<T, f16_t> ? 2 : 1;
     constexpr float kBase = 8.0f, kTop = 15.0f;   // weights start at 2^8 and may grow to 2^15
     constexpr float kNone = -3e38f;               // no weight yet
-    const int h = blockIdx.x % c.kv_heads, item = blockIdx.x / c.kv_heads;
-    DenseShare sh;
-    if (!dense_share(c, max_tokens, target, item, sh)) return;
+    constexpr int W = kDenseWaves, ROWS = 8, PITCH = 132;
+    constexpr int ROWB = 8 * R;                                     // bytes of a token's scales
+    constexpr int SLOADS = R == 8 ? 2 : 1, LOADS = 4 + SLOADS;      // 1 KB loads of a tile's scales, of a tile
+    constexpr int STAGE = LOADS * 1024, STAGES = 2, PP = 20;
+    constexpr int WAVE_BYTES = STAGES * STAGE + TERMS * 16 * PP * 4;
+    // a wave's two stages, then its weights on their way from the logits' lanes
+    // to the product's: [term][head][token pair (t, 16 + t) at 4 (t % 4) + t / 4]
+    // (20 words a head: writes and reads meet different banks); once the tiles are done the waves' states meet in the same place
+    __shared__ __align__(16) unsigned char s_mem[W * WAVE_BYTES];
+    __shared__ float s_m[W][ROWS], s_l[W][ROWS];
+    static_assert(W * ROWS * PITCH * 4 <= W * WAVE_BYTES);
+    float (*s_acc)[ROWS][PITCH] = reinterpret_cast<float (*)[ROWS][PITCH]>(s_mem);
+    const int h = blockIdx.x - div_nonneg(blockIdx.x, c.kv_heads) * c.kv_heads;
     const int group = a.q_heads / c.kv_heads;
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int col = lane & 15, grp = lane >> 4;
-
+    dense_walk(c, max_tokens, groups, [&](const DenseShare& sh) __attribute__((always_inline)) {
     // the queries: row `col`, dims 32 s + 8 grp .. + 7 in step s, largest
     // magnitude of a head in [1/2, 1)
     uint32_t qa[HALVES][4][4], ql[LOWS][4];
@@ -537,42 +622,76 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
     const CodeBits bits;
     const uint32_t low_or_delta = grp == 1 ? 0x03020302u : 0x01000100u;  // byte picks of a scale pair
 
+    // A tile's codes and scales go from memory to LDS without passing through
+    // registers, 1 KB an instruction, two tiles ahead of the one in work: lane
+    // l's 16 bytes of load i are quarter (l % 8) ^ swz(token) of token 8 i + l /
+    // 8, so that the reads below (16 tokens' equal quarters; four tokens' 64
+    // bytes of V) meet 64 different banks.  swz(t) = 4 (t / 2 % 2) + t / 4 % 4.
     struct Tile {
         uint4 k[2];
         uint32_t ks[2][R], v[8], vs[8];
-        int left;  // live tokens
     };
     const int64_t per_page = static_cast<int64_t>(c.kv_heads) << c.page_log2, head_row = static_cast<int64_t>(h) << c.page_log2;
     const int in_page = (1 << c.page_log2) - 1;
-    const int64_t first = sh.t0 + wave * kPageTile;
-    const int tiles = first < sh.t1 ? static_cast<int>((sh.t1 - first + kDenseLeast - 1) / kDenseLeast) : 0;
-    const uint32_t ko = col * kCodeRow + 16 * grp, vo = 4 * grp * kCodeRow + 64 + 4 * col;
-    const uint32_t kso = col * (8 * R), vso = 4 * grp * (8 * R) + 4 * (R + 8 * col / G);
+    const int first = sh.t0 + wave * kPageTile;
+    const int tiles = first < sh.t1 ? (sh.t1 - first + W * kPageTile - 1) / (W * kPageTile) : 0;
+    unsigned char* const mine = s_mem + wave * WAVE_BYTES;
+    const uint32_t lds = __builtin_amdgcn_readfirstlane(
+        static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)mine)));
+    const int t8 = lane / 8, swz = 4 * ((t8 >> 1) & 1) + ((t8 >> 2) & 1);
+    const uint32_t even = t8 * kCodeRow + 16 * ((lane % 8) ^ swz), odd = even ^ 32u;
+    const uint32_t flat = R == 2 ? (lane & 31) * 16 : lane * 16;  // (R = 2: 512 bytes, twice)
     int32_t entries = -1;  // lane i: the page of this wave's tile i of a block of 64
-    auto load_entries = [&](int i0) {
-        const int64_t t = first + static_cast<int64_t>(i0 + lane) * kDenseLeast;
-        entries = t < sh.t1 ? c.table[sh.b * c.width + (t >> c.page_log2)] : -1;
-    };
-    auto load_tile = [&](int i, Tile& x) {
-        const int64_t t = first + static_cast<int64_t>(i) * kDenseLeast;
+    // starts tile i's loads into a stage; returns its live tokens
+    auto issue = [&](int i, int stage) {
+        if ((i & (kWave - 1)) == 0) {
+            const int t = first + (i + lane) * (W * kPageTile);
+            entries = t < sh.t1 && t >= 0 ? c.table[sh.b * c.width + (t >> c.page_log2)] : -1;
+        }
+        const int t = first + i * (W * kPageTile);
         const int32_t e = __builtin_amdgcn_readlane(entries, i & (kWave - 1));
         const bool there = static_cast<uint32_t>(e) < static_cast<uint32_t>(c.pages);
-        x.left = there ? static_cast<int>(min<int64_t>(kPageTile, sh.t1 - t)) : 0;
         const int64_t row = (there ? e : 0) * per_page + head_row + (t & in_page);
         const char* code = c.codes + row * kCodeRow;
-        const char* sc = reinterpret_cast<const char*>(c.scales) + row * (8 * R);
+        const char* sc = reinterpret_cast<const char*>(c.scales) + row * ROWB;
+        // (the wave has read what the stage held; the loads write LDS behind the compiler's back)
+        asm volatile(
+            "s_waitcnt lgkmcnt(0)\n\t"
+            "s_mov_b32 m0, %0\n\t"
+            "s_nop 1\n\t"
+            "global_load_lds_dwordx4 %1, %3\n\t"
+            "global_load_lds_dwordx4 %2, %3 offset:1024\n\t"
+            "global_load_lds_dwordx4 %1, %3 offset:2048\n\t"
+            "global_load_lds_dwordx4 %2, %3 offset:3072\n\t"
+            "s_mov_b32 m0, %4\n\t"
+            "s_nop 1\n\t"
+            "global_load_lds_dwordx4 %5, %6"
+            :
+            : "s"(lds + stage * STAGE), "v"(even), "v"(odd), "s"(code), "s"(lds + stage * STAGE + 4096), "v"(flat), "s"(sc)
+            : "memory");
+        if constexpr (SLOADS == 2)
+            asm volatile("global_load_lds_dwordx4 %0, %1 offset:1024" : : "v"(flat), "s"(sc) : "memory");
+        return there ? min(kPageTile, sh.t1 - t) : 0;
+    };
+    // lane addresses in a stage: K of token col (+ 16), V dword col of tokens
+    // grp + 4 j (+ 16), and their scales
+    const int kswz = 4 * ((col >> 1) & 1) + ((col >> 2) & 3);
+    const int ka = col * kCodeRow + 16 * (grp ^ kswz);
+    const int va = grp * kCodeRow + 16 * ((4 ^ (4 * (grp >> 1))) + (col >> 2)) + 4 * (col & 3);
+    const int ksa = 4096 + col * ROWB, vsa = 4096 + grp * ROWB + 4 * (R + 8 * col / G);
+    auto read_tile = [&](int stage, Tile& x) {
+        const unsigned char* p = mine + stage * STAGE;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            x.k[u] = *reinterpret_cast<const uint4*>(code + ko + 16 * u * kCodeRow);
-            const char* p = sc + kso + 16 * u * (8 * R);
+            x.k[u] = *reinterpret_cast<const uint4*>(p + ka + 16 * u * kCodeRow);
             if constexpr (R == 2) {
-                const uint2 w = *reinterpret_cast<const uint2*>(p);
+                const uint2 w = *reinterpret_cast<const uint2*>(p + ksa + 16 * u * ROWB);
                 x.ks[u][0] = w.x;
                 x.ks[u][1] = w.y;
             } else {
 #pragma unroll
                 for (int g = 0; g < R; g += 4) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(p + 4 * g);
+                    const uint4 w = *reinterpret_cast<const uint4*>(p + ksa + 16 * u * ROWB + 4 * g);
                     x.ks[u][g] = w.x;
                     x.ks[u][g + 1] = w.y;
                     x.ks[u][g + 2] = w.z;
@@ -580,18 +699,17 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
                 }
             }
         }
-        // v[2 j], v[2 j + 1]: tokens 4 grp + j and 16 + 4 grp + j
+        // v[2 j], v[2 j + 1]: tokens grp + 4 j and 16 + grp + 4 j
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int tok = (j >> 1) + 16 * (j & 1);
-            x.v[j] = *reinterpret_cast<const uint32_t*>(code + vo + tok * kCodeRow);
-            x.vs[j] = *reinterpret_cast<const uint32_t*>(sc + vso + tok * (8 * R));
+            const int tok = 4 * (j >> 1) + 16 * (j & 1);
+            x.v[j] = *reinterpret_cast<const uint32_t*>(p + (va ^ (16 * (j >> 1))) + tok * kCodeRow);
+            x.vs[j] = *reinterpret_cast<const uint32_t*>(p + vsa + tok * ROWB);
         }
     };
+    uint32_t* const s_p = reinterpret_cast<uint32_t*>(mine + STAGES * STAGE);
+    const int pair = 4 * (col & 3) + (col >> 2);  // where the weights of tokens col and 16 + col go
 
-    // a wave's weights on their way from the logits' lanes to the product's:
-    // [term][head][token pair (n, 16 + n)]
-    __shared__ __align__(16) uint32_t s_p[kDenseWaves][TERMS][16][16];
     f32x4_t acc[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -601,7 +719,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
         ref[i] = kNone;
         l[i] = 0.0f;
     }
-    auto fold = [&](Tile& x) {
+    auto fold = [&](Tile& x, int left) {
         f32x4_t s[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -636,15 +754,14 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
                 for (int i = 0; i < 4; ++i) s[u][i] = fmaf(delta, dot[g][i], s[u][i]);
             }
         }
-        const bool whole = x.left == kPageTile;  // uniform; the branches stay branches
-        bool live[2] = {true, true};
+        const bool whole = left == kPageTile;  // uniform; the branches stay branches
+        const bool live[2] = {col < left, col + 16 < left};
         if (!whole) {
-            asm volatile("");
 #pragma unroll
-            for (int u = 0; u < 2; ++u) live[u] = col + 16 * u < x.left;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (4 * grp + (j >> 1) + 16 * (j & 1) >= x.left) x.vs[j] = 0u;  // what lies behind the last token may be anything
+            for (int j = 0; j < 8; ++j) {
+                if (grp + 4 * (j >> 1) + 16 * (j & 1) >= left) x.vs[j] = 0u;  // what lies behind the last token may be anything
+                asm volatile("" : "+v"(x.vs[j]));
+            }
         }
         float e[4][2], top = -INFINITY;
         auto exponents = [&] {
@@ -653,11 +770,13 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
 #pragma unroll
                 for (int u = 0; u < 2; ++u) e[i][u] = fmaf(s[u][i], factor[i], -ref[i]);
             if (!whole) {
-                asm volatile("");
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) e[i][u] = live[u] ? e[i][u] : -INFINITY;
+                    for (int u = 0; u < 2; ++u) {
+                        e[i][u] = live[u] ? e[i][u] : -INFINITY;
+                        asm volatile("" : "+v"(e[i][u]));
+                    }
             }
         };
         exponents();
@@ -685,9 +804,9 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
             const float p0 = exp2_fast(e[i][0]), p1 = exp2_fast(e[i][1]);
             l[i] += p0 + p1;
             const uint32_t p = pack_half2(p0, p1);
-            s_p[wave][0][4 * grp + i][col] = p;
+            s_p[PP * (4 * grp + i) + pair] = p;
             if constexpr (TERMS == 2)
-                s_p[wave][1][4 * grp + i][col] = pack_half2(p0 - static_cast<float>(as_half2(p)[0]),
+                s_p[PP * (16 + 4 * grp + i) + pair] = pack_half2(p0 - static_cast<float>(as_half2(p)[0]),
                                                             p1 - static_cast<float>(as_half2(p)[1]));
         }
         // the wave reads its own weights next: one wave's LDS operations complete in order
@@ -697,7 +816,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
         uint32_t pa[TERMS][4];
 #pragma unroll
         for (int n = 0; n < TERMS; ++n) {
-            const uint4 w = *reinterpret_cast<const uint4*>(&s_p[wave][n][col][4 * grp]);
+            const uint4 w = *reinterpret_cast<const uint4*>(s_p + PP * (16 * n + col) + 4 * grp);
             pa[n][0] = w.x;
             pa[n][1] = w.y;
             pa[n][2] = w.z;
@@ -728,24 +847,25 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     };
-    Tile x, y;
-    for (int i0 = 0; i0 < tiles; i0 += kWave) {
-        const int n = min(kWave, tiles - i0);
-        load_entries(i0);
-        load_tile(i0, x);
-        for (int i = 0; i < n; i += 2) {
-            if (i + 1 < n) load_tile(i0 + i + 1, y);
-            fold(x);
-            if (i + 1 >= n) break;
-            if (i + 2 < n) load_tile(i0 + i + 2, x);
-            fold(y);
-        }
+    // tile i is whole once at most the next one's loads are outstanding
+    auto arrived = [&](bool next) {
+        if (next) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LOADS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    };
+    int left = tiles > 0 ? issue(0, 0) : 0, next = tiles > 1 ? issue(1, 1) : 0;
+#pragma unroll 1
+    for (int i = 0; i < tiles; ++i) {
+        Tile x;
+        arrived(i + 1 < tiles);
+        read_tile(i & 1, x);
+        const int after = i + 2 < tiles ? issue(i + 2, i & 1) : 0;
+        fold(x, left);
+        left = next;
+        next = after;
     }
 
+    __syncthreads();  // every wave is done with its stages
     // the waves' states meet in LDS, eight heads at a time
-    constexpr int ROWS = 8, PITCH = 132;
-    __shared__ float s_m[kDenseWaves][ROWS], s_l[kDenseWaves][ROWS];
-    __shared__ __align__(16) float s_acc[kDenseWaves][ROWS][PITCH];
 #pragma unroll
     for (int i = 0; i < 4; ++i) l[i] = row_sum<16>(l[i]);
     for (int r0 = 0; r0 < group; r0 += ROWS) {
@@ -763,30 +883,29 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
             }
         }
         __syncthreads();
-        store_states<ROWS, PITCH>(s_m, s_l, s_acc, min(ROWS, group - r0),
-                                  a.partials + ((static_cast<int64_t>(item) * c.kv_heads + h) * group + r0) * kState);
+        emit_rows<T, ROWS, PITCH>(a, c, sh, h, group, r0, s_m, s_l, s_acc);
         __syncthreads();
     }
     dense_merge<T>(a, c, sh, h, group);
+    });
 }
 
 // VALU form (fp32), QC query heads of the group at a time.  A tile of 32
 // tokens lies in one page: its table entry is one scalar.
 template <typename T, int G, int QC>
 __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend a, PagedView c, int64_t max_tokens,
-                                                                    int target) {
-    constexpr int R = 128 / G;
-    const int h = blockIdx.x % c.kv_heads, item = blockIdx.x / c.kv_heads;
-    DenseShare sh;
-    if (!dense_share(c, max_tokens, target, item, sh)) return;
+                                                                    int groups) {
+    constexpr int R = 128 / G, W = kDenseWaves;
+    const int h = blockIdx.x - div_nonneg(blockIdx.x, c.kv_heads) * c.kv_heads;
     const int group = a.q_heads / c.kv_heads;
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int oct = lane / 8, d0 = (lane % 8) * 16;
-    __shared__ float s_m[kDenseWaves][QC], s_l[kDenseWaves][QC];
-    __shared__ float s_acc[kDenseWaves][QC][128];
+    __shared__ float s_m[W][QC], s_l[W][QC];
+    __shared__ float s_acc[W][QC][128];
     const int64_t per_page = static_cast<int64_t>(c.kv_heads) << c.page_log2;
     const int64_t head_row = static_cast<int64_t>(h) << c.page_log2;
+    dense_walk(c, max_tokens, groups, [&](const DenseShare& sh) __attribute__((always_inline)) {
     for (int j0 = 0; j0 < group; j0 += QC) {
         const int rows = min(QC, group - j0);
         float q[QC][16];
@@ -798,7 +917,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
         }
         FoldState<QC> st;
         st.clear();
-        for (int64_t t = sh.t0 + wave * kPageTile; t < sh.t1; t += kDenseLeast) {
+        for (int64_t t = sh.t0 + wave * kPageTile; t < sh.t1; t += W * kPageTile) {
             const int32_t page = c.table[sh.b * c.width + (t >> c.page_log2)];
             if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(c.pages)) continue;  // uniform
             const int64_t row0 = page * per_page + head_row + (t & ((1 << c.page_log2) - 1));
@@ -831,11 +950,11 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
             }
         }
         __syncthreads();
-        store_states<QC, 128>(s_m, s_l, s_acc, rows,
-                         a.partials + ((static_cast<int64_t>(item) * c.kv_heads + h) * group + j0) * kState);
+        emit_rows<T, QC, 128>(a, c, sh, h, group, j0, s_m, s_l, s_acc);
         __syncthreads();
     }
     dense_merge<T>(a, c, sh, h, group);
+    });
 }
 
 // ---- indexed ----------------------------------------------------------------
@@ -1129,16 +1248,16 @@ PickPlan pick_plan(int64_t rows, int64_t selected) {
 template <typename T, int G>
 hipError_t launch_dense_t(const PagedAttend& a, const PagedView& c, int64_t max_tokens, hipStream_t stream) {
     const int group = a.q_heads / c.kv_heads;
-    const dim3 grid(static_cast<unsigned>(paged_dense_items(c.batch, c.kv_heads, max_tokens) * c.kv_heads));
-    const int target = static_cast<int>(dense_target(c.kv_heads));
-#define POPKV_DENSE(QC)                                                                                            \
-    hipLaunchKernelGGL((paged_dense_kernel<T, G, QC>), grid, dim3(kDenseThreads), 0, stream, a, c, max_tokens, target)
+    const int per_head = dense_workgroups(c.batch, c.kv_heads, max_tokens);
+    const dim3 grid(static_cast<unsigned>(per_head * c.kv_heads));
+#define POPKV_DENSE(...) \
+    hipLaunchKernelGGL((__VA_ARGS__), grid, dim3(kDenseThreads), 0, stream, a, c, max_tokens, per_head)
     if constexpr (sizeof(T) == 2) {
-        hipLaunchKernelGGL((paged_dense_mfma_kernel<T, G>), grid, dim3(kDenseThreads), 0, stream, a, c, max_tokens, target);
+        POPKV_DENSE(paged_dense_mfma_kernel<T, G>);
     } else {
-        if (group == 1) POPKV_DENSE(1);
-        else if (group == 2) POPKV_DENSE(2);
-        else POPKV_DENSE(4);
+        if (group == 1) POPKV_DENSE(paged_dense_kernel<T, G, 1>);
+        else if (group == 2) POPKV_DENSE(paged_dense_kernel<T, G, 2>);
+        else POPKV_DENSE(paged_dense_kernel<T, G, 4>);
     }
 #undef POPKV_DENSE
     return hipGetLastError();
@@ -1160,10 +1279,7 @@ hipError_t launch_indexed_t(const PagedAttend& a, const PagedIndexed& ix, const 
 }  // namespace
 
 int64_t paged_dense_items(int64_t batch, int64_t kv_heads, int64_t max_tokens) {
-    const int64_t target = dense_target(kv_heads);
-    const int64_t per_sequence = max_tokens < 1 ? 1 : (max_tokens + kDenseLeast - 1) / kDenseLeast;
-    const int64_t all = batch * per_sequence;
-    return all < target + batch ? all : target + batch;
+    return dense_workgroups(batch, kv_heads, max_tokens) + batch;
 }
 
 int64_t paged_indexed_splits(int64_t rows, int64_t selected) { return pick_plan(rows, selected).splits; }

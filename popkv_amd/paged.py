@@ -362,8 +362,8 @@ def paged_attention_step(q: torch.Tensor, cache: PagedKVCache, layer: int, pages
     query head h reading KV head h // (QH / KVH); 1 to 16 query heads per KV
     head.  ``max_tokens`` (default ``pages.bound``) bounds the device counts
     for the launch -- give the largest count a captured graph will see.  The
-    workspace holds merge tickets and split states: do not share it with
-    ``popkv_layer_step``."""
+    workspace holds merge tickets and split states: share it only with this
+    module's attention calls, ordered on one stream."""
     (batch, width, kv_heads), pool = _check_cache(cache, pages, layer)
     q_heads, dtype = _step_operands(q, batch, kv_heads, k, v, out)
     if q_heads > 16 * kv_heads:

@@ -443,6 +443,54 @@ def test_indexed_attention_skips_missing_pages_and_keeps_nan():
     assert got[0, 1].isnan().all()
 
 
+@pytest.mark.parametrize("group", (1, 4))
+def test_one_workspace_for_both_attentions(group):
+    """Dense and indexed calls of different sizes in turn on one workspace, the
+    counts of their rows equal (one query head per KV head) or not."""
+    gen = torch.Generator().manual_seed(20 + group)
+    ws = popkv.LayerStepWorkspace()
+    work = []
+    for lengths in ([9000], [700, 40], [3, 0], [20000]):
+        kv_heads, batch = 4 // len(lengths), len(lengths)  # batch * KVH is the same
+        cache, table = make(lengths, kv_heads, max_tokens=max(lengths) + 1)
+        k, v = fill(cache, table, 0, lengths, gen)
+        table.advance(torch.tensor(lengths, device=DEV), bound=max(lengths))
+        q = torch.randn(batch, kv_heads * group, 128, generator=gen).to(DEV)
+        ck, cv = (torch.randn(batch, kv_heads, 128, generator=gen).to(DEV) for _ in range(2))
+        idx = torch.arange(max(lengths) + 1, device=DEV).expand(batch, kv_heads * group, -1).contiguous()
+        work.append((q, cache, table, ck, cv, idx, torch.arange(kv_heads * group, device=DEV) // group,
+                     attend(q, k, v, ck, cv, lengths)))
+    for _ in range(3):
+        for q, cache, table, ck, cv, idx, mapping, want in work:
+            for got in (paged.paged_attention_step(q, cache, 0, table, ck, cv, workspace=ws),
+                        paged.paged_indexed_attention(q, cache, 0, table, ck, cv, idx, mapping, workspace=ws),
+                        paged.paged_attention_step(q.half(), cache, 0, table, ck.half(), cv.half(), workspace=ws)):
+                scale = 1 if got.dtype == torch.float32 else 200  # fp16 inputs: 2^-11 of queries, keys and values
+                assert ((got.cpu().double() - want).abs() <= scale * FP32).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kv_heads,group,lengths", [(1, 16, [8200]), (1, 8, [66000]), (2, 3, [33000]), (4, 1, [20000, 9000]),
+                                                    (1, 4, [256 * 8 * 32 - 1]), (1, 1, [256 * 8 * 32 + 33])])
+def test_dense_attention_merge_levels(dtype, kv_heads, group, lengths):
+    """33 and more parts merge in two levels (sets of 16, the last one short),
+    up to the 256 of one KV head; equal bits from the same workspace again,
+    tickets back at zero."""
+    gen = torch.Generator().manual_seed(group)
+    cache, table = make(lengths, kv_heads, page=128)
+    k, v = fill(cache, table, 0, lengths, gen)
+    table.advance(torch.tensor(lengths, device=DEV), bound=max(lengths))
+    batch = len(lengths)
+    q = (torch.randn(batch, kv_heads * group, 128, generator=gen) * 2).to(dtype).to(DEV)
+    ck, cv = (torch.randn(batch, kv_heads, 128, generator=gen).to(dtype).to(DEV) for _ in range(2))
+    ws = popkv.LayerStepWorkspace()
+    got = paged.paged_attention_step(q, cache, 0, table, ck, cv, workspace=ws)
+    want = attend(q, k, v, ck, cv, lengths)
+    assert ((got.cpu().double() - want).abs() <= allowed(want, dtype, q, k, v, ck, cv)).all()
+    assert torch.equal(paged.paged_attention_step(q, cache, 0, table, ck, cv, workspace=ws), got)
+    assert not ws.buffer[:batch * kv_heads * 128].any()
+
+
 # ---------------------------------------------------------------- pages
 
 class Book:
