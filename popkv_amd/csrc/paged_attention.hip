@@ -348,34 +348,46 @@ __device__ __forceinline__ void emit_rows(const PagedAttend& a, const PagedView&
         }
         __syncthreads();
     }
+    // a row's maximum and the factors of its waves, once
+    __shared__ float s_f[ROWS][W + 3];  // factors, maximum, sum, the current token's weight
+    if (threadIdx.x < rows * W) {
+        const int j = threadIdx.x / W, w = threadIdx.x % W;
+        float mx = s_m[w][j];
+        mx = fmaxf(mx, dpp_mov<0xB1>(mx));
+        mx = fmaxf(mx, dpp_mov<0x4E>(mx));
+        mx = fmaxf(mx, dpp_mov<0x141>(mx));
+        if (sh.n == 1) mx = fmaxf(mx, s_cur[j]);
+        const float f = state_weight(s_m[w][j], s_l[w][j], mx), l = row_sum<8>(f * s_l[w][j]);
+        s_f[j][w] = f;
+        if (w == 0) {
+            float cur = 0.0f;
+            if (sh.n == 1) cur = s_cur[j] == -INFINITY && mx != -INFINITY ? 0.0f : exp2_fast(s_cur[j] - mx);
+            s_f[j][W] = mx;
+            s_f[j][W + 1] = l + cur;
+            s_f[j][W + 2] = cur;
+        }
+    }
+    __syncthreads();
     for (int i = threadIdx.x; i < rows * 128; i += W * kWave) {
         const int j = i / 128, d = i % 128;
-        float mx = -INFINITY;
+        float x = 0.0f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_m[w][j]);
-        if (sh.n == 1) mx = fmaxf(mx, s_cur[j]);
-        float x = 0.0f, l = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float f = state_weight(s_m[w][j], s_l[w][j], mx);
-            x = fmaf(f, s_acc[w][j][d], x);
-            l = fmaf(f, s_l[w][j], l);
-        }
+        for (int w = 0; w < W; ++w) x = fmaf(s_f[j][w], s_acc[w][j][d], x);
         if (sh.n == 1) {
-            const float s = s_cur[j], f = s == -INFINITY && mx != -INFINITY ? 0.0f : exp2_fast(s - mx);
-            x = fmaf(f, Elem<T>::load(static_cast<const T*>(a.cur_v) + kv, d), x);
-            Elem<T>::store(static_cast<T*>(a.out) + (row0 + j) * 128, d, x / (l + f));
+            x = fmaf(s_f[j][W + 2], Elem<T>::load(static_cast<const T*>(a.cur_v) + kv, d), x);
+            Elem<T>::store(static_cast<T*>(a.out) + (row0 + j) * 128, d, x / s_f[j][W + 1]);
         } else {
             float* p = a.partials +
                        ((static_cast<int64_t>(sh.first + sh.s) * c.kv_heads + h) * group + r0 + j) * kState;
             st_f32<true>(p + 2 + d, x);
             if (d == 0) {
-                st_f32<true>(p, mx);
-                st_f32<true>(p + 1, l);
+                st_f32<true>(p, s_f[j][W]);
+                st_f32<true>(p + 1, s_f[j][W + 1]);
             }
         }
     }
 }
+static_assert(kDenseWaves == 8, "a row's waves are eight neighbouring lanes");
 
 // Merges `n` states of each of the group's rows, `stride` floats apart: a row
 // takes a wave, or several waves' shares of its states where the group has fewer
@@ -855,6 +867,10 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
     int left = tiles > 0 ? issue(0, 0) : 0, next = tiles > 1 ? issue(1, 1) : 0;
 #pragma unroll 1
     for (int i = 0; i < tiles; ++i) {
+        // the two waves of a SIMD go first in turn: left to itself the older one
+        // ends early and leaves the other alone (131071 tokens: 20 and 28 us)
+        if (((i ^ (wave >> 2)) & 1) != 0) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
         Tile x;
         arrived(i + 1 < tiles);
         read_tile(i & 1, x);
@@ -864,6 +880,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
         next = after;
     }
 
+    __builtin_amdgcn_s_setprio(0);
     __syncthreads();  // every wave is done with its stages
     // the waves' states meet in LDS, eight heads at a time
 #pragma unroll
