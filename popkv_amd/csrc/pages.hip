@@ -16,23 +16,46 @@ constexpr float kScaleLimit = 57344.0f;
 
 // ---- write ----------------------------------------------------------------
 
+// Eight neighbouring elements as loaded, and what the encode asks of them.
+template <typename T>
+struct Eight {
+    Raw8<T> raw;
+    // the largest magnitude's bits: at least kNotFinite for infinity and NaN
+    static constexpr uint32_t kNotFinite = Elem<T>::kDtype == POPKV_DTYPE_F32 ? 0x7f800000u
+                                           : Elem<T>::kDtype == POPKV_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
+    __device__ __forceinline__ uint32_t top() const {
+        if constexpr (sizeof(T) == 4) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(raw.get(i)) & 0x7fffffffu);
+            return m;
+        } else {
+            typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+            const uint32_t w[4] = {raw.u.x, raw.u.y, raw.u.z, raw.u.w};
+            u16x2 m = __builtin_bit_cast(u16x2, w[0] & 0x7fff7fffu);
+#pragma unroll
+            for (int i = 1; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+            return max(m[0], m[1]);
+        }
+    }
+};
+
 // low = fp16(min), delta = fp16((max - low) / 15), code = round((x - low) /
 // delta) in 0 .. 15, ties to even, of this lane's eight values; the LPG lanes
-// of a group hold its G = 8 * LPG values.  The quotient for delta is taken in
-// fp64 (max - low need not fit fp32) and rounded to fp32, then fp16.  A group
-// with a NaN or an infinity gets low = NaN: it reads back as NaN.
+// of a group hold its G = 8 * LPG values.  A group with a NaN or an infinity
+// gets low = NaN: it reads back as NaN.
 template <typename T, int LPG>
-__device__ __forceinline__ void quantise8(const T* src, uint32_t& code, uint32_t& scale) {
+__device__ __forceinline__ void quantise8(const Eight<T>& in, uint32_t& code, uint32_t& scale) {
     float x[8];
-    load8<T>(src, x);
-    float lo = x[0], hi = x[0];
-    uint32_t top = 0;  // largest magnitude's bits: infinity and NaN lie above every number
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 8; ++i) x[i] = in.raw.get(i);
+    float lo = x[0], hi = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
         lo = fminf(lo, x[i]);
         hi = fmaxf(hi, x[i]);
-        top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
     }
+    uint32_t top = in.top();
     auto fold = [&](auto ctrl) {
         constexpr int C = decltype(ctrl)::value;
         lo = fminf(lo, dpp_mov<C>(lo));
@@ -42,66 +65,100 @@ __device__ __forceinline__ void quantise8(const T* src, uint32_t& code, uint32_t
     fold(std::integral_constant<int, 0xB1>{});
     if constexpr (LPG >= 4) fold(std::integral_constant<int, 0x4E>{});
     if constexpr (LPG >= 8) fold(std::integral_constant<int, 0x141>{});
-    if (top >= 0x7f800000u) {
-        code = 0;
-        scale = 0x7e00u;  // low = NaN, delta = 0
-        return;
-    }
     lo = fminf(fmaxf(lo, -kScaleLimit), kScaleLimit);
     hi = fminf(fmaxf(hi, -kScaleLimit), kScaleLimit);
     const uint32_t lob = f16_rne(lo);
     const float low = bits_f16(lob);
-    const uint32_t deb = f16_rne(static_cast<float>((static_cast<double>(hi) - static_cast<double>(low)) / 15.0));
+    // (max - low) / 15 in fp64, as max - low need not fit fp32: the product with
+    // 1 / 15 and one correction by its exact remainder is the division's result
+    // (Markstein), in three instructions
+    const double t = static_cast<double>(hi) - static_cast<double>(low), fifteenth = 1.0 / 15.0;
+    double d15 = t * fifteenth;
+    d15 = fma(fma(-15.0, d15, t), fifteenth, d15);
+    const uint32_t deb = f16_rne(static_cast<float>(d15));
     const float delta = bits_f16(deb);
-    scale = lob | (deb << 16);
-    code = 0;
-    if (delta == 0.0f) return;
-    // fp32 quotients are off by less than 2^-18 (three roundings of at most
-    // 2^-24 of a quotient below 16); a value that near a border between two
-    // codes is decided in fp64
-    const float inv = 1.0f / delta;
+    const bool bad = top >= Eight<T>::kNotFinite, flat = bad || delta == 0.0f;
+    scale = bad ? 0x7e00u : lob | (deb << 16);
+    // fp32 quotients are off by less than 2^-18 (a reciprocal within 2^-23 and two
+    // roundings of 2^-24, of a quotient below 16); a value that near a border
+    // between two codes is decided in fp64.  Adding 2^23 rounds to an integer.
+    const float inv = flat ? 0.0f : __builtin_amdgcn_rcpf(delta);
+    constexpr float kMagic = 8388608.0f;
+    float r[8], off = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float q = fminf(fmaxf((x[i] - low) * inv, 0.0f), 15.0f);
-        float r = rintf(q);
-        if (fabsf(q - r) > 0.5f - 0x1p-16f)
-            r = static_cast<float>(
-                rint(fmin(fmax((static_cast<double>(x[i]) - static_cast<double>(low)) / static_cast<double>(delta), 0.0), 15.0)));
-        code |= static_cast<uint32_t>(r) << (4 * i);
+        r[i] = (q + kMagic) - kMagic;
+        off = fmaxf(off, fabsf(q - r[i]));
     }
+    if (__ballot(off > 0.5f - 0x1p-16f) != 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float q = fminf(fmaxf((x[i] - low) * inv, 0.0f), 15.0f);
+            if (fabsf(q - r[i]) > 0.5f - 0x1p-16f && !flat) {
+                const double e = (static_cast<double>(x[i]) - static_cast<double>(low)) / static_cast<double>(delta);
+                r[i] = static_cast<float>(rint(fmin(fmax(e, 0.0), 15.0)));
+            }
+        }
+    }
+    // four codes at a time as one number of 16 bits
+    const float even = fmaf(fmaf(fmaf(r[3], 16.0f, r[2]), 16.0f, r[1]), 16.0f, r[0]);
+    const float odd = fmaf(fmaf(fmaf(r[7], 16.0f, r[6]), 16.0f, r[5]), 16.0f, r[4]);
+    code = bad ? 0u : static_cast<uint32_t>(even) | (static_cast<uint32_t>(odd) << 16);
 }
 
-// Sixteen lanes a row (eight dims each), four tokens a wave: the K and the V
-// row of a token make one 128-byte line of codes.  Bound by the stream of the
-// rows: 2 * 128 * sizeof(T) bytes read, 128 + 8R written per token and head.
+// Sixteen lanes a row (eight dims each), NT rows of K and V a lane, all loaded
+// before the first is encoded: the K and the V row of a token make one 128-byte
+// line of codes.  Bound by the stream of the rows, 2 * 128 * sizeof(T) bytes
+// read and 128 + 8R written per token and head: 32767 tokens of 8 heads bf16,
+// 64-dim groups, 172 MB in 33.5 us (5.1 TB/s); with one row a lane and the codes
+// by way of fp64 divisions and fp32 reciprocals by division 41.1, four rows 34.6,
+// eight 40.6.
+template <typename T>
+constexpr int kWriteRows = sizeof(T) == 4 ? 1 : 2;
 template <typename T, int G>
 __global__ __launch_bounds__(256) void paged_write_kernel(PagedWrite a, PagedView c) {
-    constexpr int R = 128 / G;
-    const int lane = threadIdx.x & (kWave - 1);
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16;
+    constexpr int R = 128 / G, NT = kWriteRows<T>;
+    const int lane16 = threadIdx.x & 15;
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (16 * NT) + threadIdx.x / 16;
     const int h = blockIdx.y, b = blockIdx.z;
     const int64_t most = a.tokens ? clamp_count(a.tokens[b], a.rows) : a.rows;
-    if (t >= most) return;  // whole 16-lane rows leave
+    if (static_cast<int64_t>(blockIdx.x) * (16 * NT) >= most) return;
     const int64_t limit = c.width << c.page_log2;
-    const int64_t pos = clamp_count(c.counts[b], limit) + t;
-    const int64_t entry = pos >> c.page_log2;
-    const int32_t page = pos < limit ? c.table[b * c.width + entry] : -1;
-    if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(c.pages)) {
-        if (a.status && (lane & 15) == 0 && h == 0) atomicOr(a.status, pos < limit ? kStatusNoPage : kStatusFull);
-        return;
-    }
-    const int d = (lane & 15) * 8;
-    const int64_t row = ((static_cast<int64_t>(page) * c.kv_heads + h) << c.page_log2) + (pos & ((1 << c.page_log2) - 1));
-    uint32_t* codes = reinterpret_cast<uint32_t*>(c.codes + row * kCodeRow);
-    uint32_t* scales = c.scales + row * (2 * R);
-    const T* src[2] = {static_cast<const T*>(a.k) + b * a.k_bs + h * a.k_hs + t * a.k_ts + d,
-                       static_cast<const T*>(a.v) + b * a.v_bs + h * a.v_hs + t * a.v_ts + d};
+    const int64_t count = clamp_count(c.counts[b], limit);
+    const int d = lane16 * 8;
+    const T* k = static_cast<const T*>(a.k) + b * a.k_bs + h * a.k_hs + d;
+    const T* v = static_cast<const T*>(a.v) + b * a.v_bs + h * a.v_hs + d;
+    Eight<T> x[NT][2];
+    int32_t page[NT];
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-        uint32_t code, scale;
-        quantise8<T, G / 8>(src[w], code, scale);
-        codes[16 * w + (lane & 15)] = code;
-        if (d % G == 0) scales[R * w + d / G] = scale;
+    for (int i = 0; i < NT; ++i) {
+        const int64_t t = min(t0 + 16 * i, most - 1), pos = count + t;  // (rows past the last repeat it)
+        x[i][0].raw.load(k + t * a.k_ts);
+        x[i][1].raw.load(v + t * a.v_ts);
+        page[i] = pos < limit ? c.table[b * c.width + (pos >> c.page_log2)] : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const int64_t t = t0 + 16 * i, pos = count + t;
+        const bool live = t < most, there = static_cast<uint32_t>(page[i]) < static_cast<uint32_t>(c.pages);
+        uint32_t code[2], scale[2];
+        quantise8<T, G / 8>(x[i][0], code[0], scale[0]);
+        quantise8<T, G / 8>(x[i][1], code[1], scale[1]);
+        if (live && there) {
+            const int64_t row =
+                ((static_cast<int64_t>(page[i]) * c.kv_heads + h) << c.page_log2) + (pos & ((1 << c.page_log2) - 1));
+            uint32_t* codes = reinterpret_cast<uint32_t*>(c.codes + row * kCodeRow);
+            uint32_t* scales = c.scales + row * (2 * R);
+            codes[lane16] = code[0];
+            codes[16 + lane16] = code[1];
+            if (d % G == 0) {
+                scales[d / G] = scale[0];
+                scales[R + d / G] = scale[1];
+            }
+        } else if (live && a.status && lane16 == 0 && h == 0) {
+            atomicOr(a.status, pos < limit ? kStatusNoPage : kStatusFull);
+        }
     }
 }
 
@@ -188,13 +245,6 @@ __global__ __launch_bounds__(256) void reserve_rows_kernel(PageReserve a) {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / kWave;
 
-// The pages [0, n) cut among the plan's waves, a whole number of 64 each.
-__device__ __forceinline__ void plan_segment(int64_t n, int wave, int64_t& first, int64_t& last) {
-    const int64_t per = ((n + kPlanWaves - 1) / kPlanWaves + kWave - 1) / kWave * kWave;
-    first = min(per * wave, n);
-    last = min(first + per, n);
-}
-
 // Exclusive prefix over the block of one value a wave (lane-uniform), and the
 // total; sh holds kPlanWaves words and is free again on return.
 __device__ __forceinline__ int32_t plan_prefix(int32_t v, int32_t* sh, int32_t& total) {
@@ -212,32 +262,68 @@ __device__ __forceinline__ int32_t plan_prefix(int32_t v, int32_t* sh, int32_t& 
     return base;
 }
 
+// The used pages of a part of the pool as bits in LDS, with how many lie before
+// each word: any page's rank among the used or the free ones is a popcount
+// away.  A pool of more than kMapPages goes through it part by part.
+constexpr int kMapPages = 65536, kMapWords = kMapPages / 64;
+static_assert(kMapWords == kPlanThreads);
+struct PageMap {
+    uint64_t words[kMapWords];
+    int32_t before[kMapWords];
+    int32_t sh[kPlanWaves];
+};
+// Builds the map of pages [first, first + kMapPages) of a pool; returns the used
+// pages there.  Every thread of the block calls it.
+template <typename F>
+__device__ __forceinline__ int32_t map_pages(PageMap& m, int64_t first, int64_t pages, F&& used) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const int n = static_cast<int>(min<int64_t>(kMapPages, pages - first));
+    __syncthreads();  // nothing reads the last part's any more
+    constexpr int AHEAD = 8;  // loads on their way at once
+    static_assert(kMapPages % (AHEAD * kPlanThreads) == 0);
+    for (int i0 = 0; i0 < n; i0 += AHEAD * kPlanThreads) {
+        bool u[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int i = i0 + j * kPlanThreads + threadIdx.x;
+            u[j] = i < n && used(first + i);
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const uint64_t bits = __ballot(u[j]);
+            if (lane == 0) m.words[(i0 + j * kPlanThreads + threadIdx.x) / 64] = bits;
+        }
+    }
+    __syncthreads();
+    const int32_t v = static_cast<int>(threadIdx.x) * 64 < n ? __popcll(m.words[threadIdx.x]) : 0;
+    const int32_t incl = static_cast<int32_t>(wave_incl_scan(static_cast<uint32_t>(v), lane));
+    int32_t total;
+    const int32_t base = plan_prefix(__builtin_amdgcn_readlane(incl, kWave - 1), m.sh, total);
+    m.before[threadIdx.x] = base + incl - v;
+    __syncthreads();
+    return total;
+}
+// Used pages of the mapped part before page i of it.
+__device__ __forceinline__ int32_t used_before(const PageMap& m, int i) {
+    return m.before[i / 64] + __popcll(m.words[i / 64] & ((uint64_t{1} << (i & 63)) - 1));
+}
+
 // The lowest `want` pages without a reference, ascending, to list; returns how
 // many there are in all.  Every thread of the block calls it.
-// COH: this workgroup's own atomics changed them in this launch, so the loads
-// read past the cache that may still hold what was there before.
-template <bool COH>
-__device__ __forceinline__ int32_t list_free(const int32_t* refs, int64_t pages, int32_t want, int32_t* list, int32_t* sh) {
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    auto is_free = [&](int64_t i, int64_t end) {
-        if (i >= end) return false;
-        if constexpr (COH) return __hip_atomic_load(refs + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0;
-        else return refs[i] == 0;
-    };
-    int64_t first, last;
-    plan_segment(pages, wave, first, last);
-    int32_t mine = 0;
-    for (int64_t i = first; i < last; i += kWave) mine += __popcll(__ballot(is_free(i + lane, last)));
-    int32_t total;
-    int32_t at = plan_prefix(mine, sh, total);
-    for (int64_t i = first; i < last && at < want; i += kWave) {
-        const bool free = is_free(i + lane, last);
-        const uint64_t mask = __ballot(free);
-        const int32_t r = at + __popcll(mask & ((uint64_t{1} << lane) - 1));
-        if (free && r < want) list[r] = static_cast<int32_t>(i + lane);
-        at += __popcll(mask);
+template <typename F>
+__device__ __forceinline__ int32_t list_free(PageMap& m, int64_t pages, int32_t want, int32_t* list, F&& used) {
+    int32_t found = 0;
+    for (int64_t first = 0; first < pages; first += kMapPages) {
+        const int n = static_cast<int>(min<int64_t>(kMapPages, pages - first));
+        const int32_t total = map_pages(m, first, pages, used);
+        if (found < want)
+            for (int i = threadIdx.x; i < n; i += kPlanThreads) {
+                const int32_t r = found + i - used_before(m, i);
+                if (!(m.words[i / 64] >> (i & 63) & 1) && r < want) list[r] = static_cast<int32_t>(first + i);
+            }
+        found += n - total;
     }
-    return total;
+    return found;
 }
 
 // need[] to exclusive offsets in place (kept in global memory), total returned.
@@ -273,7 +359,7 @@ bool plan_alone(int64_t batch, int64_t width, int64_t pages) {
 // the rows and references are its work too.
 template <bool ALONE>
 __global__ __launch_bounds__(kPlanThreads) void reserve_plan_kernel(PageReserve a) {
-    __shared__ int32_t sh[kPlanWaves];
+    __shared__ PageMap map;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     if constexpr (ALONE) {
         for (int64_t b = wave; b < a.batch; b += kPlanWaves) reserve_row(a, b);
@@ -281,10 +367,10 @@ __global__ __launch_bounds__(kPlanThreads) void reserve_plan_kernel(PageReserve 
             for (int64_t i = threadIdx.x; i < a.pages; i += kPlanThreads) a.refs[i] = a.refs_in[i];
         __syncthreads();
     }
-    const int32_t total = scan_needs(a.need, a.batch, sh);
+    const int32_t total = scan_needs(a.need, a.batch, map.sh);
     if (total == 0) return;
     const int32_t want = static_cast<int32_t>(min<int64_t>(total, a.pages));
-    const int32_t found = list_free<false>(a.refs, a.pages, want, a.list, sh);
+    const int32_t found = list_free(map, a.pages, want, a.list, [&](int64_t i) { return a.refs[i] != 0; });
     __syncthreads();  // the list is this workgroup's own: the barrier orders it
     for (int64_t b = wave; b < a.batch; b += kPlanWaves) {
         const int32_t at = a.need[b], end = a.need[b + 1];
@@ -360,89 +446,147 @@ __global__ __launch_bounds__(256) void fork_rows_kernel(PageFork a) {
     if (b < a.batch) fork_row(a, b);
 }
 
-// One workgroup: the open pages wanted take the lowest free pages; a sequence
-// that finds none is left empty.  ALONE: the rows and references are its work
-// too.
-template <bool ALONE>
-__global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(PageFork a) {
-    __shared__ int32_t sh[kPlanWaves];
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    if constexpr (ALONE) {
-        if (a.refs != a.refs_in) {
-            for (int64_t i = threadIdx.x; i < a.pages; i += kPlanThreads) a.refs[i] = a.refs_in[i];
-            __syncthreads();
-        }
-        for (int64_t b = wave; b < a.batch; b += kPlanWaves) fork_row(a, b);
-        __syncthreads();
+// A child for whose open page none is free: empty, its shared pages given back.
+__device__ __forceinline__ void fork_drop(const PageFork& a, int64_t b, int32_t* refs) {
+    int32_t* row = a.rows + b * a.width;
+    for (int64_t i = threadIdx.x & (kWave - 1); i < a.width; i += kWave) {
+        if (static_cast<uint32_t>(row[i]) < static_cast<uint32_t>(a.pages)) atomicSub(refs + row[i], 1);
+        row[i] = -1;
     }
-    const int32_t total = scan_needs(a.need, a.batch, sh);
-    if (threadIdx.x == 0) *a.moves = total;
-    if (total == 0) return;
-    const int32_t found = list_free<ALONE>(a.refs, a.pages, static_cast<int32_t>(min<int64_t>(total, a.pages)), a.list, sh);
-    if (threadIdx.x == 0 && found < total) *a.moves = found;
+    if ((threadIdx.x & (kWave - 1)) == 0) {
+        a.new_counts[b] = 0;
+        if (a.status) atomicOr(a.status, kStatusNoPage);
+    }
+}
+
+// One workgroup: the open pages wanted take the lowest free pages; a sequence
+// that finds none is left empty.
+__global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(PageFork a) {
+    __shared__ PageMap map;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int32_t total = scan_needs(a.need, a.batch, map.sh);
+    if (total == 0) {
+        if (threadIdx.x == 0) *a.moves = 0;
+        return;
+    }
+    const int32_t found = list_free(map, a.pages, static_cast<int32_t>(min<int64_t>(total, a.pages)), a.list,
+                                    [&](int64_t i) { return a.refs[i] != 0; });
+    if (threadIdx.x == 0) *a.moves = min(found, total);
     __syncthreads();
     for (int64_t b = wave; b < a.batch; b += kPlanWaves) {
         const int32_t at = a.need[b];
         if (a.need[b + 1] == at) continue;
-        int32_t* row = a.rows + b * a.width;
-        const int64_t full = a.new_counts[b] >> a.page_log2;
-        if (at < found) {
-            if (lane == 0) {
-                const int32_t page = a.list[at];
-                row[full] = page;
-                a.refs[page] = 1;
-                a.pairs[at] = make_int2(a.source[b], page);
-            }
-        } else {
-            for (int64_t i = lane; i < a.width; i += kWave) {
-                if (static_cast<uint32_t>(row[i]) < static_cast<uint32_t>(a.pages)) atomicSub(a.refs + row[i], 1);
-                row[i] = -1;
-            }
-            if (lane == 0) {
-                a.new_counts[b] = 0;
-                if (a.status) atomicOr(a.status, kStatusNoPage);
-            }
+        if (at >= found) {
+            fork_drop(a, b, a.refs);
+        } else if (lane == 0) {
+            const int32_t page = a.list[at];
+            a.rows[b * a.width + (a.new_counts[b] >> a.page_log2)] = page;
+            a.refs[page] = 1;
+            a.pairs[at] = make_int2(a.source[b], page);
         }
     }
+}
+
+// The whole plan of a small table by one workgroup, a thread a sequence and a
+// thread a table entry, the reference counts in LDS.
+constexpr int kForkPages = 8192;
+__global__ __launch_bounds__(kPlanThreads) void fork_alone_kernel(PageFork a) {
+    __shared__ PageMap map;
+    __shared__ int32_t s_refs[kForkPages], s_first[kPlanThreads], s_parent[kPlanThreads], s_kept[kPlanThreads];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    const int batch = static_cast<int>(a.batch), width = static_cast<int>(a.width), pages = static_cast<int>(a.pages);
+    const int p = tid < batch ? static_cast<int>(parent_of(a, tid)) : -1;
+    const int count = p >= 0 ? static_cast<int>(clamp_count(a.counts_in[p], a.width << a.page_log2)) : 0;
+    s_first[tid] = kPlanThreads;
+    for (int i = tid; i < pages; i += kPlanThreads) s_refs[i] = a.refs_in[i];
+    __syncthreads();
+    if (p >= 0) atomicMin(s_first + p, tid);
+    __syncthreads();
+    const bool first = p >= 0 && s_first[p] == tid;
+    const int full = count >> a.page_log2;
+    s_parent[tid] = p;
+    s_kept[tid] = p < 0 ? 0 : first ? width : full;
+    const bool open = p >= 0 && !first && (count & ((1 << a.page_log2) - 1)) != 0;
+    const int32_t source = open ? a.table_in[p * width + full] : -1;
+    const int need = static_cast<uint32_t>(source) < static_cast<uint32_t>(pages) ? 1 : 0;
+    if (tid < batch) {
+        a.new_counts[tid] = count;
+        if (a.status && p < 0 && a.parents[tid] != -1) atomicOr(a.status, kStatusBadParent);
+    }
+    __syncthreads();
+    for (int i = tid; i < batch * width; i += kPlanThreads) {
+        const int b = i / width, e = i - b * width;
+        const int32_t was = a.table_in[i], now = e < s_kept[b] ? a.table_in[s_parent[b] * width + e] : -1;
+        a.rows[i] = now;
+        if (was != now) {
+            if (static_cast<uint32_t>(was) < static_cast<uint32_t>(pages)) atomicSub(s_refs + was, 1);
+            if (static_cast<uint32_t>(now) < static_cast<uint32_t>(pages)) atomicAdd(s_refs + now, 1);
+        }
+    }
+    const int32_t incl = static_cast<int32_t>(wave_incl_scan(static_cast<uint32_t>(need), lane));
+    int32_t total;
+    const int32_t at = plan_prefix(__builtin_amdgcn_readlane(incl, kWave - 1), map.sh, total) + incl - need;
+    int32_t found = 0;
+    if (total > 0) {
+        found = list_free(map, pages, min(total, pages), a.list, [&](int64_t i) { return s_refs[i] != 0; });
+        __syncthreads();
+        if (need && at < found) {
+            const int32_t page = a.list[at];
+            a.rows[tid * width + full] = page;
+            s_refs[page] = 1;
+            a.pairs[at] = make_int2(source, page);
+        }
+        s_first[tid] = need && at >= found ? 1 : 0;  // (read as the parents' no more)
+        __syncthreads();
+        if (found < total)
+            for (int b = wave; b < batch; b += kPlanWaves)
+                if (s_first[b] != 0) fork_drop(a, b, s_refs);
+        __syncthreads();
+    }
+    if (tid == 0) *a.moves = min(found, total);
+    for (int i = tid; i < pages; i += kPlanThreads) a.refs[i] = s_refs[i];
 }
 
 // ---- compact --------------------------------------------------------------
 
 // One workgroup: n = the live pages; the live pages from n on, ascending, move
-// to the free ones before n, ascending (as many).
+// to the free ones before n, ascending (as many).  A live page from n on is the
+// (live pages before it - live pages before n)-th mover, a free page before n the
+// (its number - live pages before it)-th hole.
 __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(PageCompact a) {
-    __shared__ int32_t sh[kPlanWaves];
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    int64_t first, last;
-    plan_segment(a.pages, wave, first, last);
-    int32_t live = 0;
-    for (int64_t i = first; i < last; i += kWave)
-        live += __popcll(__ballot(i + lane < last && a.refs_in[i + lane] > 0));
-    int32_t n;
-    plan_prefix(live, sh, n);
-    int32_t holes = 0, movers = 0;
-    for (int64_t i = first; i < last; i += kWave) {
-        const bool in = i + lane < last, used = in && a.refs_in[i + lane] > 0;
-        holes += __popcll(__ballot(in && !used && i + lane < n));
-        movers += __popcll(__ballot(used && i + lane >= n));
-    }
-    int32_t moves, same;
-    int32_t hole_at = plan_prefix(holes, sh, moves), mover_at = plan_prefix(movers, sh, same);
-    int32_t* pair = reinterpret_cast<int32_t*>(a.pairs);  // (source, target) of move j at 2j, 2j + 1
-    for (int64_t i = first; i < last; i += kWave) {
-        const bool in = i + lane < last;
-        const int32_t refs = in ? a.refs_in[i + lane] : 0;
-        const bool hole = in && refs <= 0 && i + lane < n, mover = refs > 0 && i + lane >= n;
-        const uint64_t hm = __ballot(hole), mm = __ballot(mover), below = (uint64_t{1} << lane) - 1;
-        if (hole) pair[2 * (hole_at + __popcll(hm & below)) + 1] = static_cast<int32_t>(i + lane);
-        if (mover) pair[2 * (mover_at + __popcll(mm & below))] = static_cast<int32_t>(i + lane);
-        if (in) {
-            a.map[i + lane] = refs > 0 ? static_cast<int32_t>(i + lane) : -1;
-            if (a.refs != a.refs_in) a.refs[i + lane] = refs;
+    __shared__ PageMap map;
+    auto used = [&](int64_t i) { return a.refs_in[i] > 0; };
+    int64_t n = 0;
+    int32_t whole = 0;
+    for (int64_t first = 0; first < a.pages; first += kMapPages) n += whole = map_pages(map, first, a.pages, used);
+    // the live pages before n: those of the parts before n's, and what the map
+    // of its part says
+    int64_t below = 0;
+    if (a.pages <= kMapPages) {
+        below = n < a.pages ? used_before(map, static_cast<int>(n)) : n;
+    } else {
+        for (int64_t first = 0; first < n; first += kMapPages) {
+            const int32_t part = map_pages(map, first, a.pages, used);
+            below += n - first < kMapPages ? used_before(map, static_cast<int>(n - first)) : part;
         }
-        hole_at += __popcll(hm);
-        mover_at += __popcll(mm);
     }
+    int32_t* pair = reinterpret_cast<int32_t*>(a.pairs);  // (source, target) of move j at 2j, 2j + 1
+    int64_t before = 0;
+    for (int64_t first = 0; first < a.pages; first += kMapPages) {
+        const int32_t part = a.pages <= kMapPages ? whole : map_pages(map, first, a.pages, used);
+        const int size = static_cast<int>(min<int64_t>(kMapPages, a.pages - first));
+        for (int i = threadIdx.x; i < size; i += kPlanThreads) {
+            const int32_t refs = a.refs_in[first + i];
+            const bool live = refs > 0;
+            const int64_t page = first + i, rank = before + used_before(map, i);
+            if (!live && page < n) pair[2 * (page - rank) + 1] = static_cast<int32_t>(page);
+            if (live && page >= n) pair[2 * (rank - below)] = static_cast<int32_t>(page);
+            a.map[page] = live ? static_cast<int32_t>(page) : -1;
+            if (a.refs != a.refs_in) a.refs[page] = refs;
+        }
+        before += part;
+    }
+    const int32_t moves = static_cast<int32_t>(n - below);
     if (threadIdx.x == 0) *a.moves = moves;
     __syncthreads();
     for (int32_t j = threadIdx.x; j < moves; j += kPlanThreads) {
@@ -511,7 +655,8 @@ hipError_t copy_words(const void* src, void* dst, int64_t n, hipStream_t s) {
     }
 
 hipError_t launch_paged_write(const PagedWrite& a, const PagedView& c, int dtype, int dim_group, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>((a.rows + 15) / 16), static_cast<unsigned>(c.kv_heads),
+    const int per = 16 * (dtype == POPKV_DTYPE_F32 ? kWriteRows<float> : kWriteRows<bf16_t>);
+    const dim3 grid(static_cast<unsigned>((a.rows + per - 1) / per), static_cast<unsigned>(c.kv_heads),
                     static_cast<unsigned>(c.batch));
     POPKV_PAGED_T(paged_write_kernel)
     return hipGetLastError();
@@ -541,15 +686,15 @@ hipError_t launch_page_reserve(const PageReserve& a, hipStream_t s) {
 }
 
 hipError_t launch_page_fork(const PageFork& a, const PageMoves& m, hipStream_t s) {
-    if (plan_alone(a.batch, a.width, a.pages)) {
-        hipLaunchKernelGGL(fork_plan_kernel<true>, dim3(1), dim3(kPlanThreads), 0, s, a);
+    if (plan_alone(a.batch, a.width, a.pages) && a.batch <= kPlanThreads && a.pages <= kForkPages) {
+        hipLaunchKernelGGL(fork_alone_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
     } else {
         if (a.refs != a.refs_in) {
             const hipError_t e = copy_words(a.refs_in, a.refs, a.pages, s);
             if (e != hipSuccess) return e;
         }
         hipLaunchKernelGGL(fork_rows_kernel, dim3(static_cast<unsigned>((a.batch + 3) / 4)), dim3(256), 0, s, a);
-        hipLaunchKernelGGL(fork_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, s, a);
+        hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
     }
     hipLaunchKernelGGL(move_pages_kernel, dim3(blocks_for(a.batch * m.layers * m.parts, 1, 2048)), dim3(256), 0, s, m);
     return hipGetLastError();

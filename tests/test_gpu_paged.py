@@ -607,7 +607,7 @@ def moved(pool, moves):
 
 
 SHAPES = [(0, 1, 1, 32, 0), (1, 1, 4, 64, 2), (2, 5, 6, 32, 40), (3, 33, 9, 64, 7), (4, 130, 20, 128, 300),
-          (5, 7, 70, 32, 2000), (6, 1100, 2, 32, 500)]
+          (5, 7, 70, 32, 2000), (6, 1100, 2, 32, 500), (7, 40, 500, 32, 9000)]
 
 
 @pytest.mark.parametrize("in_place", (False, True))
@@ -689,6 +689,37 @@ def test_compact(seed, batch, width, page, spare, in_place):
     again, page_map = paged.compact_pages(cache, new)
     same_book(again, book)
     assert torch.equal(cache.codes, moved(codes, moves))
+
+
+@pytest.mark.parametrize("spare", (65530, 70001, 140000))
+def test_pools_of_several_parts(spare):
+    """Pools past the 65536 pages that a plan maps at once: pages reserved,
+    forked and compacted across the parts."""
+    cache, pages, book = random_pages(21, 12, 9, 32, spare, layers=1, kv_heads=1, group=64)
+    rng = np.random.default_rng(spare)
+    used = rng.random(cache.pages) < 0.5
+    extra = torch.from_numpy(used.astype(np.int32)).to(DEV)  # pages that others hold
+    pages.refs += extra
+    book.refs = pages.refs.tolist()
+    tokens = [int(x) for x in rng.integers(0, 100, 12)]
+    book.reserve(tokens)
+    pages = paged.reserve_pages(pages, torch.tensor(tokens, device=DEV))
+    same_book(pages, book)
+    # the lowest free pages lie past the first part
+    pages.refs[:66000] += 1
+    book.refs = pages.refs.tolist()
+    codes = cache.codes.clone()
+    parents = [0, 0, 0, 3, 3, -1, 6, 7, 8, 8, 8, 11]
+    codes = moved(codes, book.fork(parents))
+    pages = paged.fork_sequences(cache, pages, torch.tensor(parents, device=DEV))
+    same_book(pages, book)
+    assert torch.equal(cache.codes, codes)
+    pages.refs[:66000] -= 1
+    book.refs = pages.refs.tolist()
+    moves, where = book.compact()
+    pages, page_map = paged.compact_pages(cache, pages)
+    same_book(pages, book)
+    assert page_map.tolist() == where and torch.equal(cache.codes, moved(codes, moves))
 
 
 def test_compact_of_empty_and_full_pools():
