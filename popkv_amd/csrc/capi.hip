@@ -982,8 +982,8 @@ int popkv_paged_attention(const void* queries, int32_t dtype, const void* codes,
     if (q_heads <= 0 || q_heads > 65535 || q_heads % kv_heads != 0 || q_heads / kv_heads > 16)
         return fail(POPKV_ERR_UNSUPPORTED, "paged attention supports 1 to 16 query heads per KV head");
     if (max_tokens < 0 || max_tokens > (int64_t{1} << 30)) return fail(POPKV_ERR_TOKENS, "invalid token count");
-    if (batch * ceil_div(max_tokens, 32) > 0x7fffffff)
-        return fail(POPKV_ERR_UNSUPPORTED, "batch * max_tokens must stay below 2^36 tokens");
+    if (batch * (ceil_div(max_tokens, 32) + 32) > (int64_t{1} << 30))
+        return fail(POPKV_ERR_UNSUPPORTED, "batch * max_tokens must stay below 2^35 tokens");
     if (workspace_bytes < popkv_paged_attention_workspace_bytes(batch, q_heads, kv_heads, max_tokens))
         return fail(POPKV_ERR_WORKSPACE, "paged attention needs %zu workspace bytes",
                     popkv_paged_attention_workspace_bytes(batch, q_heads, kv_heads, max_tokens));

@@ -254,12 +254,21 @@ constexpr int kDenseWaves = 8;
 constexpr int kDenseThreads = kDenseWaves * kWave;
 constexpr int kDenseBlocks = 256;
 
+// What a further sequence costs a workgroup beside its tiles, in tiles: the
+// queries, the join of the waves, the state or output.  Sequences 0, 14 and 28
+// tiles apart: a ragged batch of five up to 20001, fp16 8 queries a KV head, 30.4,
+// 28.3 and 26.5 us; 64 up to 2000 42, 36.2 and 33.8; 16 up to 1000 20.2, 13.7 and
+// 14.6; 64 of one token 37, 11.5 and 11.4.
+constexpr int kSequenceCost = 24;
+
 // Workgroups of a KV head: one a CU in all, with a tile for each wave.
 int dense_workgroups(int64_t batch, int64_t kv_heads, int64_t max_tokens) {
     const int64_t target = kDenseBlocks / kv_heads < 1 ? 1 : kDenseBlocks / kv_heads;
-    const int64_t tiles = batch * ((max_tokens + kPageTile - 1) / kPageTile);
-    const int64_t most = (tiles + kDenseWaves - 1) / kDenseWaves;
-    return static_cast<int>(most < 1 ? 1 : most < target ? most : target);
+    const int64_t tiles = (max_tokens + kPageTile - 1) / kPageTile;
+    const int64_t most = (batch * ((tiles < 1 ? 1 : tiles) + kSequenceCost) + kDenseWaves - 1) / kDenseWaves;
+    const int64_t one = (tiles + kDenseWaves - 1) / kDenseWaves;  // (a sequence alone has no further one)
+    const int64_t n = batch == 1 ? one : most;
+    return static_cast<int>(n < 1 ? 1 : n < target ? n : target);
 }
 
 // A workgroup's part of a sequence: tokens [t0, t1) of sequence b, part s of n;
@@ -268,57 +277,78 @@ struct DenseShare {
     int b, s, n, first, t0, t1;
 };
 
-// The work of one KV head is the batch's tiles of 32 tokens laid end to end,
-// cut among the grid's workgroups by the real lengths, which are read on the
-// device: every workgroup takes as many tiles (at least one a wave), whether they
-// are part of one long sequence or several short ones, and calls f for each of
-// the sequences that it has some of.  (Splits of each sequence by itself left a
-// few workgroups more than fit at once, a second round: a ragged batch of five up
-// to 20001, 64 query heads over 8 KV heads fp16 35 us.)  An empty sequence
-// belongs to the workgroup at whose tiles it lies.  Workgroup w's state for
+// The work of one KV head is the batch's tiles of 32 tokens laid end to end
+// (one at least a sequence, kSequenceCost places apart), cut among the grid's
+// workgroups by the real lengths, which are read on the device: every workgroup
+// takes as many places (one a wave at least), whether they are part of one long
+// sequence or several short ones.  (Splits of each sequence by itself left a few
+// workgroups more than fit at once, a second round: a ragged batch of five up to
+// 20001, 64 query heads over 8 KV heads fp16 35 us.)  Workgroup w's state for
 // sequence b has place w + b: one of the two grows from a part to the next, so
-// places differ.  Each wave works this out by itself from the counts.  (The
-// entry refuses batches of 2^31 tiles and more.)
-template <typename F>
-__device__ __forceinline__ void dense_walk(const PagedView& c, int64_t max_tokens, int groups, F&& f) {
-    const int lane = threadIdx.x & (kWave - 1);
-    const int w = div_nonneg(blockIdx.x, c.kv_heads);
-    const int64_t most = min(c.width << c.page_log2, max_tokens);
-    auto count_of = [&](int b) { return b < c.batch ? static_cast<int>(clamp_count(c.counts[b], most)) : 0; };
-    auto tiles_of = [](int count) { return (count + kPageTile - 1) / kPageTile; };
-    auto scan = [&](int v) { return static_cast<int>(wave_incl_scan(static_cast<uint32_t>(v), lane)); };
-    const int count0 = count_of(lane), incl0 = scan(tiles_of(count0));
-    int total = __builtin_amdgcn_readlane(incl0, kWave - 1);
-    for (int b0 = kWave; b0 < c.batch; b0 += kWave)
-        total += __builtin_amdgcn_readlane(scan(tiles_of(count_of(b0 + lane))), kWave - 1);
-    const int per = max(div_nonneg(total + groups - 1, groups), kDenseWaves);
-    // (w * per may pass 2^31 only past the last tile)
-    const int r0 = static_cast<int>(min<int64_t>(static_cast<int64_t>(w) * per, total)), r1 = min(r0 + per, total);
-    if (w > 0 && r0 >= total) return;
-    const bool last = r1 >= total;
-    int base = 0;
-    for (int b0 = 0; b0 < c.batch && (last || base < r1); b0 += kWave) {
-        const int count = b0 == 0 ? count0 : count_of(b0 + lane);
-        const int tiles = tiles_of(count), incl = b0 == 0 ? incl0 : scan(tiles);
-        const int start = base + incl - tiles;
-        const bool here =
-            b0 + lane < c.batch && (tiles ? start < r1 && start + tiles > r0 : start >= r0 && (last || start < r1));
-        for (uint64_t mask = __ballot(here); mask; mask &= mask - 1) {
-            const int src = __ffsll(static_cast<unsigned long long>(mask)) - 1;
-            const int from = __builtin_amdgcn_readlane(start, src), to = from + __builtin_amdgcn_readlane(tiles, src);
-            DenseShare sh;
-            sh.b = b0 + src;
-            const int w0 = from >= r0 ? w : from / per, w1 = to <= r1 ? w : (to - 1) / per;
-            sh.s = w - w0;
-            sh.n = w1 - w0 + 1;
-            sh.first = w0 + sh.b;
-            sh.t0 = (max(from, r0) - from) * kPageTile;
-            sh.t1 = min(__builtin_amdgcn_readlane(count, src), (min(to, r1) - from) * kPageTile);
-            f(sh);
+// places differ.  Each wave works its parts out by itself from the counts.  (The
+// entry refuses batches of 2^30 places and more.)
+struct DenseWalk {
+    const PagedView& c;
+    const int64_t most;
+    const int lane, w;
+    int per, r0, r1, b0, base;
+    int count, tiles, start;  // lane i: sequence b0 + i
+    uint64_t mask;            // its sequences still to come, of the 64 from b0 on
+
+    __device__ __forceinline__ DenseWalk(const PagedView& view, int64_t max_tokens, int groups)
+        : c(view), most(min(view.width << view.page_log2, max_tokens)), lane(threadIdx.x & (kWave - 1)),
+          w(div_nonneg(blockIdx.x, view.kv_heads)), b0(0), base(0) {
+        load();
+        int total = __builtin_amdgcn_readlane(incl(), kWave - 1);
+        for (int b = kWave; b < c.batch; b += kWave) {
+            const int n = cost(b + lane, tiles_of(count_of(b + lane)));
+            total += __builtin_amdgcn_readlane(static_cast<int>(wave_incl_scan(static_cast<uint32_t>(n), lane)), kWave - 1);
         }
-        base += __builtin_amdgcn_readlane(incl, kWave - 1);
+        total -= kSequenceCost;
+        per = max(div_nonneg(total + groups - 1, groups), kDenseWaves);
+        r0 = static_cast<int>(min<int64_t>(static_cast<int64_t>(w) * per, int64_t{1} << 30));
+        r1 = r0 + per;
+        find();
     }
-}
+    __device__ __forceinline__ int count_of(int b) const {
+        return b < c.batch ? static_cast<int>(clamp_count(c.counts[b], most)) : 0;
+    }
+    static __device__ __forceinline__ int tiles_of(int n) { return max((n + kPageTile - 1) / kPageTile, 1); }
+    __device__ __forceinline__ int cost(int b, int n) const { return b < c.batch ? n + kSequenceCost : 0; }
+    __device__ __forceinline__ void load() {
+        count = count_of(b0 + lane);
+        tiles = tiles_of(count);
+    }
+    __device__ __forceinline__ int incl() const {
+        return static_cast<int>(wave_incl_scan(static_cast<uint32_t>(cost(b0 + lane, tiles)), lane));
+    }
+    __device__ __forceinline__ void find() {
+        const int n = incl();
+        start = base + n - cost(b0 + lane, tiles);
+        mask = __ballot(b0 + lane < c.batch && start < r1 && start + tiles > r0);
+        base += __builtin_amdgcn_readlane(n, kWave - 1);
+    }
+    // the next sequence that the workgroup has a part of
+    __device__ __forceinline__ bool next(DenseShare& sh) {
+        while (mask == 0) {
+            b0 += kWave;
+            if (b0 >= c.batch || base >= r1) return false;
+            load();
+            find();
+        }
+        const int src = __ffsll(static_cast<unsigned long long>(mask)) - 1;
+        mask &= mask - 1;
+        const int from = __builtin_amdgcn_readlane(start, src), to = from + __builtin_amdgcn_readlane(tiles, src);
+        sh.b = b0 + src;
+        const int w0 = from >= r0 ? w : from / per, w1 = to <= r1 ? w : (to - 1) / per;
+        sh.s = w - w0;
+        sh.n = w1 - w0 + 1;
+        sh.first = w0 + sh.b;
+        sh.t0 = (max(from, r0) - from) * kPageTile;
+        sh.t1 = min(__builtin_amdgcn_readlane(count, src), (min(to, r1) - from) * kPageTile);
+        return true;
+    }
+};
 
 // A row's logit with the current token, by one wave.
 template <typename T>
@@ -543,97 +573,15 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
     constexpr int WAVE_BYTES = STAGES * STAGE + TERMS * 16 * PP * 4;
     // a wave's two stages, then its weights on their way from the logits' lanes
     // to the product's: [term][head][token pair (t, 16 + t) at 4 (t % 4) + t / 4]
-    // (20 words a head: writes and reads meet different banks); once the tiles are done the waves' states meet in the same place
+    // (20 words a head: writes and reads meet different banks)
     __shared__ __align__(16) unsigned char s_mem[W * WAVE_BYTES];
     __shared__ float s_m[W][ROWS], s_l[W][ROWS];
-    static_assert(W * ROWS * PITCH * 4 <= W * WAVE_BYTES);
-    float (*s_acc)[ROWS][PITCH] = reinterpret_cast<float (*)[ROWS][PITCH]>(s_mem);
+    __shared__ __align__(16) float s_acc[W][ROWS][PITCH];
     const int h = blockIdx.x - div_nonneg(blockIdx.x, c.kv_heads) * c.kv_heads;
     const int group = a.q_heads / c.kv_heads;
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int col = lane & 15, grp = lane >> 4;
-    dense_walk(c, max_tokens, groups, [&](const DenseShare& sh) __attribute__((always_inline)) {
-    // the queries: row `col`, dims 32 s + 8 grp .. + 7 in step s, largest
-    // magnitude of a head in [1/2, 1)
-    uint32_t qa[HALVES][4][4], ql[LOWS][4];
-    float factor[4];  // of rows 4 grp + i
-    {
-        float q[4][8], top = 0.0f;
-        const int64_t row = static_cast<int64_t>(sh.b) * a.q_heads + static_cast<int64_t>(h) * group + min(col, group - 1);
-        const T* src = static_cast<const T*>(a.q) + row * 128 + 8 * grp;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) load8<T>(src + 32 * s, q[s]);
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (col >= group) q[s][i] = 0.0f;
-                top = fmaxf(top, fabsf(q[s][i]));
-            }
-        top = fmaxf(top, lane_xor<16>(top));
-        top = fmaxf(top, lane_xor<32>(top));
-        const int e = static_cast<int>((__float_as_uint(top) >> 23) & 0xffu) - 127;
-        const float mine = ldexpf(kScaleHigh, e + 1);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) factor[i] = __shfl(mine, 4 * grp + i);
-        float sum[4];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            sum[s] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                q[s][i] = ldexpf(q[s][i], -1 - e);
-                sum[s] += q[s][i];
-                if (i & 1) q[s][i] *= 0.0625f;
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t x = pack_half2(q[s][j], q[s][j + 4]);
-                if constexpr (HALVES == 2) {
-                    qa[0][s][j] = grp < 2 ? x : 0u;
-                    qa[1][s][j] = grp < 2 ? 0u : x;
-                } else {
-                    qa[0][s][j] = x;
-                }
-            }
-            sum[s] += lane_xor<16>(sum[s]);
-        }
-        // the low terms' product: lane group 0 holds the groups' sums of queries
-        // for low, lane group 1 minus their products with codes of zero for
-        // delta, each as (high, rest)
-        float qs[R];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const float other = lane_xor<32>(sum[s]);
-            if constexpr (R == 8) {
-                qs[2 * s] = grp < 2 ? sum[s] : other;
-                qs[2 * s + 1] = grp < 2 ? other : sum[s];
-            } else if constexpr (R == 4) {
-                qs[s] = sum[s] + other;
-            } else {
-                qs[s / 2] = s & 1 ? qs[s / 2] + (sum[s] + other) : sum[s] + other;
-            }
-        }
-        const uint32_t none[4] = {0x64006400u, 0x64006400u, 0x64006400u, 0x64006400u};
-#pragma unroll
-        for (int g = 0; g < 4 * LOWS; ++g) {
-            uint32_t x = 0;
-            if (g < R) {
-                f32x4_t z = {0.0f, 0.0f, 0.0f, 0.0f};
-                if constexpr (R == 2) z = mfma_f16(none, qa[0][2 * g % 4 + 1], mfma_f16(none, qa[0][2 * g % 4], z));
-                else z = mfma_f16(none, qa[g % HALVES][g / HALVES % 4], z);
-                // (rows of codes times columns of queries: every element of column `col` is head `col`'s)
-                const float term = grp == 0 ? qs[g % R] : -z[0];
-                const float high = static_cast<float>(static_cast<_Float16>(term));
-                x = pack_half2(high, term - high);
-            }
-            ql[g / 4][g % 4] = grp < 2 ? x : 0u;
-        }
-    }
-    const CodeBits bits;
-    const uint32_t low_or_delta = grp == 1 ? 0x03020302u : 0x01000100u;  // byte picks of a scale pair
-
     // A tile's codes and scales go from memory to LDS without passing through
     // registers, 1 KB an instruction, two tiles ahead of the one in work: lane
     // l's 16 bytes of load i are quarter (l % 8) ^ swz(token) of token 8 i + l /
@@ -645,8 +593,8 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
     };
     const int64_t per_page = static_cast<int64_t>(c.kv_heads) << c.page_log2, head_row = static_cast<int64_t>(h) << c.page_log2;
     const int in_page = (1 << c.page_log2) - 1;
-    const int first = sh.t0 + wave * kPageTile;
-    const int tiles = first < sh.t1 ? (sh.t1 - first + W * kPageTile - 1) / (W * kPageTile) : 0;
+    DenseShare sh;  // the part whose tiles are loaded
+    int first = 0, tiles = 0;
     unsigned char* const mine = s_mem + wave * WAVE_BYTES;
     const uint32_t lds = __builtin_amdgcn_readfirstlane(
         static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)mine)));
@@ -722,10 +670,102 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
     uint32_t* const s_p = reinterpret_cast<uint32_t*>(mine + STAGES * STAGE);
     const int pair = 4 * (col & 3) + (col >> 2);  // where the weights of tokens col and 16 + col go
 
+    const CodeBits bits;
+    const uint32_t low_or_delta = grp == 1 ? 0x03020302u : 0x01000100u;  // byte picks of a scale pair
+
+    // Starts a part: its first two tiles on their way, then its queries (row
+    // `col`, dims 32 s + 8 grp .. + 7 in step s).
+    Raw8<T> raw[4];
+    int left = 0, next = 0;
+    auto start_part = [&] {
+        first = sh.t0 + wave * kPageTile;
+        tiles = first < sh.t1 ? (sh.t1 - first + W * kPageTile - 1) / (W * kPageTile) : 0;
+        left = tiles > 0 ? issue(0, 0) : 0;
+        next = tiles > 1 ? issue(1, 1) : 0;
+        const int64_t row = static_cast<int64_t>(sh.b) * a.q_heads + static_cast<int64_t>(h) * group + min(col, group - 1);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) raw[s].load(static_cast<const T*>(a.q) + row * 128 + 8 * grp + 32 * s);
+    };
+
+    DenseWalk walk(c, max_tokens, groups);
+    while (walk.next(sh)) {
+    start_part();
     f32x4_t acc[8];
+    float ref[4], l[4];  // rows 4 grp + i: weights are 2^(logit - ref)
+    // the queries in fp16, the largest magnitude of a head in [1/2, 1)
+    uint32_t qa[HALVES][4][4], ql[LOWS][4];
+    float factor[4];  // of rows 4 grp + i
+    {
+        float q[4][8], top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                q[s][i] = col < group ? raw[s].get(i) : 0.0f;
+                top = fmaxf(top, fabsf(q[s][i]));
+            }
+        top = fmaxf(top, lane_xor<16>(top));
+        top = fmaxf(top, lane_xor<32>(top));
+        const int e = static_cast<int>((__float_as_uint(top) >> 23) & 0xffu) - 127;
+        const float mine = ldexpf(kScaleHigh, e + 1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) factor[i] = __shfl(mine, 4 * grp + i);
+        float sum[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            sum[s] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                q[s][i] = ldexpf(q[s][i], -1 - e);
+                sum[s] += q[s][i];
+                if (i & 1) q[s][i] *= 0.0625f;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t x = pack_half2(q[s][j], q[s][j + 4]);
+                if constexpr (HALVES == 2) {
+                    qa[0][s][j] = grp < 2 ? x : 0u;
+                    qa[1][s][j] = grp < 2 ? 0u : x;
+                } else {
+                    qa[0][s][j] = x;
+                }
+            }
+            sum[s] += lane_xor<16>(sum[s]);
+        }
+        // the low terms' product: lane group 0 holds the groups' sums of queries
+        // for low, lane group 1 minus their products with codes of zero for
+        // delta, each as (high, rest)
+        float qs[R];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const float other = lane_xor<32>(sum[s]);
+            if constexpr (R == 8) {
+                qs[2 * s] = grp < 2 ? sum[s] : other;
+                qs[2 * s + 1] = grp < 2 ? other : sum[s];
+            } else if constexpr (R == 4) {
+                qs[s] = sum[s] + other;
+            } else {
+                qs[s / 2] = s & 1 ? qs[s / 2] + (sum[s] + other) : sum[s] + other;
+            }
+        }
+        const uint32_t none[4] = {0x64006400u, 0x64006400u, 0x64006400u, 0x64006400u};
+#pragma unroll
+        for (int g = 0; g < 4 * LOWS; ++g) {
+            uint32_t x = 0;
+            if (g < R) {
+                f32x4_t z = {0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (R == 2) z = mfma_f16(none, qa[0][2 * g % 4 + 1], mfma_f16(none, qa[0][2 * g % 4], z));
+                else z = mfma_f16(none, qa[g % HALVES][g / HALVES % 4], z);
+                // (rows of codes times columns of queries: every element of column `col` is head `col`'s)
+                const float term = grp == 0 ? qs[g % R] : -z[0];
+                const float high = static_cast<float>(static_cast<_Float16>(term));
+                x = pack_half2(high, term - high);
+            }
+            ql[g / 4][g % 4] = grp < 2 ? x : 0u;
+        }
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    float ref[4], l[4];  // rows 4 grp + i: weights are 2^(logit - ref)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         ref[i] = kNone;
@@ -864,7 +904,6 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
         if (next) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LOADS) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
     };
-    int left = tiles > 0 ? issue(0, 0) : 0, next = tiles > 1 ? issue(1, 1) : 0;
 #pragma unroll 1
     for (int i = 0; i < tiles; ++i) {
         // the two waves of a SIMD go first in turn: left to itself the older one
@@ -881,10 +920,9 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
     }
 
     __builtin_amdgcn_s_setprio(0);
-    __syncthreads();  // every wave is done with its stages
-    // the waves' states meet in LDS, eight heads at a time
 #pragma unroll
     for (int i = 0; i < 4; ++i) l[i] = row_sum<16>(l[i]);
+    // the waves' states meet in LDS, eight heads at a time
     for (int r0 = 0; r0 < group; r0 += ROWS) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -904,7 +942,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
         __syncthreads();
     }
     dense_merge<T>(a, c, sh, h, group);
-    });
+    }
 }
 
 // VALU form (fp32), QC query heads of the group at a time.  A tile of 32
@@ -922,7 +960,8 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
     __shared__ float s_acc[W][QC][128];
     const int64_t per_page = static_cast<int64_t>(c.kv_heads) << c.page_log2;
     const int64_t head_row = static_cast<int64_t>(h) << c.page_log2;
-    dense_walk(c, max_tokens, groups, [&](const DenseShare& sh) __attribute__((always_inline)) {
+    DenseWalk walk(c, max_tokens, groups);
+    for (DenseShare sh; walk.next(sh);) {
     for (int j0 = 0; j0 < group; j0 += QC) {
         const int rows = min(QC, group - j0);
         float q[QC][16];
@@ -971,7 +1010,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
         __syncthreads();
     }
     dense_merge<T>(a, c, sh, h, group);
-    });
+    }
 }
 
 // ---- indexed ----------------------------------------------------------------
