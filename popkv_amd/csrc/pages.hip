@@ -262,6 +262,20 @@ __device__ __forceinline__ int32_t plan_prefix(int32_t v, int32_t* sh, int32_t& 
     return base;
 }
 
+// Copies `n` words by the whole workgroup.  (Loads come in batches before their
+// stores: the compiler cannot know that the two do not overlap.)
+__device__ __forceinline__ void plan_copy(const int32_t* src, int32_t* dst, int n) {
+    constexpr int AHEAD = 8;
+    for (int i0 = threadIdx.x; i0 < n; i0 += AHEAD * kPlanThreads) {
+        int32_t x[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) x[j] = i0 + j * kPlanThreads < n ? src[i0 + j * kPlanThreads] : 0;
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+            if (i0 + j * kPlanThreads < n) dst[i0 + j * kPlanThreads] = x[j];
+    }
+}
+
 // The used pages of a part of the pool as bits in LDS, with how many lie before
 // each word: any page's rank among the used or the free ones is a popcount
 // away.  A pool of more than kMapPages goes through it part by part.
@@ -345,28 +359,11 @@ __device__ __forceinline__ int32_t scan_needs(int32_t* need, int64_t batch, int3
     return base;
 }
 
-// Tables and pools up to which one workgroup does the whole plan: a launch
-// saved is worth more than the other CUs.  Reserve and fork, out of place, one
-// launch against two or three (us):
-constexpr int64_t kPlanAlone = 16384;
-
-bool plan_alone(int64_t batch, int64_t width, int64_t pages) {
-    return batch * width <= kPlanAlone && pages <= kPlanAlone;
-}
-
 // One workgroup: the missing entries of the sequences, in order, take the
-// lowest free pages; a sequence whose share does not fit gets none.  ALONE:
-// the rows and references are its work too.
-template <bool ALONE>
+// lowest free pages; a sequence whose share does not fit gets none.
 __global__ __launch_bounds__(kPlanThreads) void reserve_plan_kernel(PageReserve a) {
     __shared__ PageMap map;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    if constexpr (ALONE) {
-        for (int64_t b = wave; b < a.batch; b += kPlanWaves) reserve_row(a, b);
-        if (a.refs != a.refs_in)
-            for (int64_t i = threadIdx.x; i < a.pages; i += kPlanThreads) a.refs[i] = a.refs_in[i];
-        __syncthreads();
-    }
     const int32_t total = scan_needs(a.need, a.batch, map.sh);
     if (total == 0) return;
     const int32_t want = static_cast<int32_t>(min<int64_t>(total, a.pages));
@@ -394,6 +391,112 @@ __global__ __launch_bounds__(kPlanThreads) void reserve_plan_kernel(PageReserve 
             }
             r += __popcll(mask);
         }
+    }
+}
+
+// Tables and pools up to which one workgroup does the whole plan, a thread a
+// sequence, a table entry and a page: a launch or two saved are worth more than
+// the other CUs.  Reserve and fork, alone against in several launches (us, with
+// the pages moved): 64 sequences of 14 entries over 1031 pages 6.2 and 12.5, 9.2
+// and 14.0; 128 of 113 over 8100 18.1 and 20.7, 14.2 and 18.9; 8 of 1876 16.2 and
+// 15.5, 13.6 and 32.3; 512 of 26 19.2 and 47, 16.5 and 30.
+constexpr int64_t kPlanAlone = 16384;
+
+bool plan_alone(int64_t batch, int64_t width, int64_t pages) {
+    return batch <= kPlanThreads && batch * width <= kPlanAlone && pages <= kPlanAlone;
+}
+
+// i / width of an entry of such a table, inverse = 1 / width: (i + 1/2) / width
+// lies at least 1 / (2 width) from an integer, and its fp32 rounding is off by
+// less, i being below 2^14.
+__device__ __forceinline__ int row_of(int i, float inverse) {
+    return static_cast<int>((static_cast<float>(i) + 0.5f) * inverse);
+}
+
+// The r-th free page (r below how many there are) of a mapped pool.
+__device__ __forceinline__ int nth_free(const PageMap& m, int pages, int r) {
+    int lo = 0, hi = (pages + 63) / 64 - 1;  // the last word with at most r free pages before it
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (mid * 64 - m.before[mid] <= r) lo = mid;
+        else hi = mid - 1;
+    }
+    uint64_t free = ~m.words[lo];
+    int left = r - (lo * 64 - m.before[lo]), at = 0;
+#pragma unroll
+    for (int half = 32; half; half /= 2) {
+        const int n = __popcll(free & ((uint64_t{1} << half) - 1));
+        if (left >= n) {
+            left -= n;
+            at += half;
+            free >>= half;
+        }
+    }
+    return lo * 64 + at;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void reserve_alone_kernel(PageReserve a) {
+    __shared__ PageMap map;
+    __shared__ uint64_t s_missing[kPlanAlone / 64];
+    __shared__ int32_t s_before[kPlanAlone / 64], s_lo[kPlanThreads], s_hi[kPlanThreads], s_need[kPlanThreads];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1);
+    const int batch = static_cast<int>(a.batch), width = static_cast<int>(a.width), pages = static_cast<int>(a.pages);
+    const int entries = batch * width, words = (entries + 63) / 64;
+    const float inverse = 1.0f / static_cast<float>(width);
+    s_need[tid] = 0;
+    if (tid < batch) {
+        int64_t lo, hi;
+        bool fits;
+        reserve_range(a, tid, lo, hi, fits);
+        s_lo[tid] = static_cast<int32_t>(lo);
+        s_hi[tid] = static_cast<int32_t>(hi);
+        if (!fits && a.status) atomicOr(a.status, kStatusFull);
+        if (a.counts != a.counts_in) a.counts[tid] = a.counts_in[tid];
+    }
+    const int32_t used = map_pages(map, 0, pages, [&](int64_t i) { return a.refs_in[i] != 0; });
+    if (a.refs != a.refs_in) plan_copy(a.refs_in, a.refs, pages);
+    constexpr int AHEAD = 4;
+    for (int i0 = 0; i0 < entries; i0 += AHEAD * kPlanThreads) {
+        int32_t page[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int i = i0 + j * kPlanThreads + tid;
+            page[j] = i < entries ? a.table_in[i] : 0;
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int i = i0 + j * kPlanThreads + tid;
+            bool missing = false;
+            if (i < entries) {
+                const int b = row_of(i, inverse), e = i - b * width;
+                if (a.table != a.table_in) a.table[i] = page[j];
+                missing = page[j] < 0 && e >= s_lo[b] && e < s_hi[b];
+                if (missing) atomicAdd(s_need + b, 1);
+            }
+            const uint64_t bits = __ballot(missing);
+            if (lane == 0 && i / 64 < words) s_missing[i / 64] = bits;
+        }
+    }
+    __syncthreads();
+    // ranks: of the missing entries before each word, and of each sequence's last
+    auto scan = [&](int32_t v, int32_t& total) {
+        const int32_t incl = static_cast<int32_t>(wave_incl_scan(static_cast<uint32_t>(v), lane));
+        return plan_prefix(__builtin_amdgcn_readlane(incl, kWave - 1), map.sh, total) + incl;
+    };
+    int32_t total;
+    const int32_t n = tid < words ? __popcll(s_missing[tid]) : 0, incl = scan(n, total);
+    if (tid < words) s_before[tid] = incl - n;
+    if (total == 0) return;
+    const int32_t need = s_need[tid], end = scan(need, total), found = pages - used;
+    if (need > 0 && end > found && a.status) atomicOr(a.status, kStatusNoPage);
+    s_need[tid] = end;
+    __syncthreads();
+    for (int i = tid; i < entries; i += kPlanThreads) {
+        const uint64_t bits = s_missing[i / 64];
+        if (!(bits >> (i & 63) & 1) || s_need[row_of(i, inverse)] > found) continue;
+        const int page = nth_free(map, pages, s_before[i / 64] + __popcll(bits & ((uint64_t{1} << (i & 63)) - 1)));
+        a.table[i] = page;
+        a.refs[page] = 1;
     }
 }
 
@@ -495,10 +598,11 @@ __global__ __launch_bounds__(kPlanThreads) void fork_alone_kernel(PageFork a) {
     __shared__ int32_t s_refs[kForkPages], s_first[kPlanThreads], s_parent[kPlanThreads], s_kept[kPlanThreads];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
     const int batch = static_cast<int>(a.batch), width = static_cast<int>(a.width), pages = static_cast<int>(a.pages);
+    const float inverse = 1.0f / static_cast<float>(width);
     const int p = tid < batch ? static_cast<int>(parent_of(a, tid)) : -1;
     const int count = p >= 0 ? static_cast<int>(clamp_count(a.counts_in[p], a.width << a.page_log2)) : 0;
     s_first[tid] = kPlanThreads;
-    for (int i = tid; i < pages; i += kPlanThreads) s_refs[i] = a.refs_in[i];
+    plan_copy(a.refs_in, s_refs, pages);
     __syncthreads();
     if (p >= 0) atomicMin(s_first + p, tid);
     __syncthreads();
@@ -514,13 +618,27 @@ __global__ __launch_bounds__(kPlanThreads) void fork_alone_kernel(PageFork a) {
         if (a.status && p < 0 && a.parents[tid] != -1) atomicOr(a.status, kStatusBadParent);
     }
     __syncthreads();
-    for (int i = tid; i < batch * width; i += kPlanThreads) {
-        const int b = i / width, e = i - b * width;
-        const int32_t was = a.table_in[i], now = e < s_kept[b] ? a.table_in[s_parent[b] * width + e] : -1;
-        a.rows[i] = now;
-        if (was != now) {
-            if (static_cast<uint32_t>(was) < static_cast<uint32_t>(pages)) atomicSub(s_refs + was, 1);
-            if (static_cast<uint32_t>(now) < static_cast<uint32_t>(pages)) atomicAdd(s_refs + now, 1);
+    constexpr int AHEAD = 4;
+    for (int i0 = 0; i0 < batch * width; i0 += AHEAD * kPlanThreads) {
+        int32_t was[AHEAD], now[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int i = i0 + j * kPlanThreads + tid;
+            was[j] = now[j] = -1;
+            if (i < batch * width) {
+                const int b = row_of(i, inverse), e = i - b * width;
+                was[j] = a.table_in[i];
+                if (e < s_kept[b]) now[j] = a.table_in[s_parent[b] * width + e];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int i = i0 + j * kPlanThreads + tid;
+            if (i < batch * width) a.rows[i] = now[j];
+            if (was[j] != now[j]) {
+                if (static_cast<uint32_t>(was[j]) < static_cast<uint32_t>(pages)) atomicSub(s_refs + was[j], 1);
+                if (static_cast<uint32_t>(now[j]) < static_cast<uint32_t>(pages)) atomicAdd(s_refs + now[j], 1);
+            }
         }
     }
     const int32_t incl = static_cast<int32_t>(wave_incl_scan(static_cast<uint32_t>(need), lane));
@@ -544,7 +662,7 @@ __global__ __launch_bounds__(kPlanThreads) void fork_alone_kernel(PageFork a) {
         __syncthreads();
     }
     if (tid == 0) *a.moves = min(found, total);
-    for (int i = tid; i < pages; i += kPlanThreads) a.refs[i] = s_refs[i];
+    plan_copy(s_refs, a.refs, pages);
 }
 
 // ---- compact --------------------------------------------------------------
@@ -575,14 +693,23 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(PageCompact 
     for (int64_t first = 0; first < a.pages; first += kMapPages) {
         const int32_t part = a.pages <= kMapPages ? whole : map_pages(map, first, a.pages, used);
         const int size = static_cast<int>(min<int64_t>(kMapPages, a.pages - first));
-        for (int i = threadIdx.x; i < size; i += kPlanThreads) {
-            const int32_t refs = a.refs_in[first + i];
-            const bool live = refs > 0;
-            const int64_t page = first + i, rank = before + used_before(map, i);
-            if (!live && page < n) pair[2 * (page - rank) + 1] = static_cast<int32_t>(page);
-            if (live && page >= n) pair[2 * (rank - below)] = static_cast<int32_t>(page);
-            a.map[page] = live ? static_cast<int32_t>(page) : -1;
-            if (a.refs != a.refs_in) a.refs[page] = refs;
+        constexpr int AHEAD = 8;
+        for (int i0 = threadIdx.x; i0 < size; i0 += AHEAD * kPlanThreads) {
+            int32_t refs[AHEAD];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j)
+                refs[j] = i0 + j * kPlanThreads < size ? a.refs_in[first + i0 + j * kPlanThreads] : 0;
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const int i = i0 + j * kPlanThreads;
+                if (i >= size) break;
+                const bool live = refs[j] > 0;
+                const int64_t page = first + i, rank = before + used_before(map, i);
+                if (!live && page < n) pair[2 * (page - rank) + 1] = static_cast<int32_t>(page);
+                if (live && page >= n) pair[2 * (rank - below)] = static_cast<int32_t>(page);
+                a.map[page] = live ? static_cast<int32_t>(page) : -1;
+                if (a.refs != a.refs_in) a.refs[page] = refs[j];
+            }
         }
         before += part;
     }
@@ -673,7 +800,7 @@ hipError_t launch_paged_read(const PagedRead& a, const PagedView& c, int dtype, 
 
 hipError_t launch_page_reserve(const PageReserve& a, hipStream_t s) {
     if (plan_alone(a.batch, a.width, a.pages)) {
-        hipLaunchKernelGGL(reserve_plan_kernel<true>, dim3(1), dim3(kPlanThreads), 0, s, a);
+        hipLaunchKernelGGL(reserve_alone_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
         return hipGetLastError();
     }
     if (a.refs != a.refs_in) {
@@ -681,12 +808,12 @@ hipError_t launch_page_reserve(const PageReserve& a, hipStream_t s) {
         if (e != hipSuccess) return e;
     }
     hipLaunchKernelGGL(reserve_rows_kernel, dim3(static_cast<unsigned>((a.batch + 3) / 4)), dim3(256), 0, s, a);
-    hipLaunchKernelGGL(reserve_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, s, a);
+    hipLaunchKernelGGL(reserve_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
     return hipGetLastError();
 }
 
 hipError_t launch_page_fork(const PageFork& a, const PageMoves& m, hipStream_t s) {
-    if (plan_alone(a.batch, a.width, a.pages) && a.batch <= kPlanThreads && a.pages <= kForkPages) {
+    if (plan_alone(a.batch, a.width, a.pages) && a.pages <= kForkPages) {
         hipLaunchKernelGGL(fork_alone_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
     } else {
         if (a.refs != a.refs_in) {
