@@ -514,7 +514,8 @@ __device__ __forceinline__ void dense_merge(const PagedAttend& a, const PagedVie
 //                                    they are, each scale group by itself
 //   S = sum_g delta_g dot_g + sum_g low_g qsum_g   in fp32, the second sum by
 //                                    one more product (qsum in two fp16 terms)
-//   O[head, dim] += P . V            V as low + c delta in fp16
+//   O[head, dim] += P . V            V as low + c delta in fp16 (fp16 outputs:
+//                                    exactly, in three parts)
 // so keys enter the logits exactly: with the outlier channels that keys have,
 // their rounding to fp16 was four times fp16's own in the result.  (C layout:
 // lane l holds rows 4 (l / 16) .. + 3 of column l % 16; A and B: lane l holds
@@ -528,16 +529,20 @@ __device__ __forceinline__ void dense_merge(const PagedAttend& a, const PagedVie
 // Queries are scaled by a power of two per head (bf16 reaches past fp16, and
 // 1024 times a group's sum must not), and the weights are kept around 2^8, where fp16 keeps
 // 11 bits; fp16 outputs take a second term for the rest of each weight.
-// The same pairs as low + c * delta.
-__device__ __forceinline__ void dequantise_pairs(const CodeBits& k, uint32_t w, half2_t delta, half2_t low, uint32_t (&out)[4]) {
+// The same pairs as c, and as low + c * delta.
+__device__ __forceinline__ void code_pairs(const CodeBits& k, uint32_t w, half2_t (&out)[4]) {
     const half2_t k1024 = {1024.0f16, 1024.0f16}, k16th = {0.0625f16, 0.0625f16}, k64 = {-64.0f16, -64.0f16};
     uint32_t b[4];
     biased_pairs(k, w, b);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const half2_t c = i & 1 ? __builtin_elementwise_fma(as_half2(b[i]), k16th, k64) : as_half2(b[i]) - k1024;
-        out[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c, delta, low));
-    }
+    for (int i = 0; i < 4; ++i)
+        out[i] = i & 1 ? __builtin_elementwise_fma(as_half2(b[i]), k16th, k64) : as_half2(b[i]) - k1024;
+}
+__device__ __forceinline__ void dequantise_pairs(const CodeBits& k, uint32_t w, half2_t delta, half2_t low, uint32_t (&out)[4]) {
+    half2_t code[4];
+    code_pairs(k, w, code);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(code[i], delta, low));
 }
 
 __device__ __forceinline__ f32x4_t mfma_f16(const uint32_t (&a)[4], const uint32_t (&b)[4], f32x4_t c) {
@@ -690,7 +695,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
     DenseWalk walk(c, max_tokens, groups);
     while (walk.next(sh)) {
     start_part();
-    f32x4_t acc[8];
+    f32x4_t acc[8], low_acc = {0.0f, 0.0f, 0.0f, 0.0f};
     float ref[4], l[4];  // rows 4 grp + i: weights are 2^(logit - ref)
     // the queries in fp16, the largest magnitude of a head in [1/2, 1)
     uint32_t qa[HALVES][4][4], ql[LOWS][4];
@@ -847,6 +852,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
                 l[i] *= f;
 #pragma unroll
                 for (int d = 0; d < 8; ++d) acc[d][i] *= f;
+                if constexpr (TERMS == 2) low_acc[i] *= f;
                 ref[i] = to;
             }
             exponents();
@@ -876,23 +882,56 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
         }
         // a lane's eight dims 8 col .. + 7 of V: the low halves of the tokens'
         // dwords hold dims 0 .. 3, the high ones 4 .. 7
+        if constexpr (TERMS == 1) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            uint32_t vf[4][4];  // [dim][token pair]
+            for (int half = 0; half < 2; ++half) {
+                uint32_t vf[4][4];  // [dim][token pair]
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t v0 = x.v[2 * j], v1 = x.v[2 * j + 1];
-                uint32_t d[4];
-                dequantise_pairs(bits, half ? high_halves(v0, v1) : low_halves(v0, v1),
-                                 as_half2(high_halves(x.vs[2 * j], x.vs[2 * j + 1])),
-                                 as_half2(low_halves(x.vs[2 * j], x.vs[2 * j + 1])), d);
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t v0 = x.v[2 * j], v1 = x.v[2 * j + 1];
+                    uint32_t d[4];
+                    dequantise_pairs(bits, half ? high_halves(v0, v1) : low_halves(v0, v1),
+                                     as_half2(high_halves(x.vs[2 * j], x.vs[2 * j + 1])),
+                                     as_half2(low_halves(x.vs[2 * j], x.vs[2 * j + 1])), d);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) vf[i][j] = d[i];
+                    for (int i = 0; i < 4; ++i) vf[i][j] = d[i];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[4 * half + i] = mfma_f16(pa[0], vf[i], acc[4 * half + i]);
             }
+        } else {
+            // exactly: delta in two parts of at most seven and four bits, whose
+            // products with a code fit fp16, and the lows by themselves (the
+            // same sum for each of a lane's dims)
+            uint32_t lows[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int j = 0; j < 4; ++j) lows[j] = low_halves(x.vs[2 * j], x.vs[2 * j + 1]);
 #pragma unroll
-                for (int n = 0; n < TERMS; ++n) acc[4 * half + i] = mfma_f16(pa[n], vf[i], acc[4 * half + i]);
+            for (int n = 0; n < TERMS; ++n) low_acc = mfma_f16(pa[n], lows, low_acc);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t vh[4][4], vl[4][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t v0 = x.v[2 * j], v1 = x.v[2 * j + 1];
+                    const half2_t delta = as_half2(high_halves(x.vs[2 * j], x.vs[2 * j + 1]));
+                    const half2_t top7 = as_half2(__builtin_bit_cast(uint32_t, delta) & 0xfff0fff0u);
+                    half2_t code[4];
+                    code_pairs(bits, half ? high_halves(v0, v1) : low_halves(v0, v1), code);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        vh[i][j] = __builtin_bit_cast(uint32_t, code[i] * top7);
+                        vl[i][j] = __builtin_bit_cast(uint32_t, code[i] * (delta - top7));
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    f32x4_t& sum = acc[4 * half + i];
+                    sum = mfma_f16(pa[0], vh[i], sum);
+                    sum = mfma_f16(pa[TERMS - 1], vh[i], sum);
+                    sum = mfma_f16(pa[0], vl[i], sum);
+                }
+            }
         }
         // the next tile's weights overwrite s_p only after every lane has read
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -922,6 +961,9 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
     __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) l[i] = row_sum<16>(l[i]);
+    if constexpr (TERMS == 2)
+#pragma unroll
+        for (int d = 0; d < 8; ++d) acc[d] += low_acc;
     // the waves' states meet in LDS, eight heads at a time
     for (int r0 = 0; r0 < group; r0 += ROWS) {
 #pragma unroll

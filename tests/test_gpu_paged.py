@@ -390,6 +390,73 @@ def test_dense_attention_of_large_and_small_queries(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group", (16, 64))
+@pytest.mark.parametrize("scale", (1e-2, 1e-3, 1e-4))
+def test_attention_over_small_values(dtype, group, scale):
+    """Keys and values whose scales, and the parts they are split in, lie among
+    fp16's subnormals: the format's own values, no worse."""
+    gen = torch.Generator().manual_seed(30)
+    cache, table = make([900], 2, group=group)
+    k, v = fill(cache, table, 0, [900], gen, scale=scale)
+    table.advance(900)
+    q = torch.randn(1, 8, 128, generator=gen).to(dtype).to(DEV)
+    ck, cv = ((torch.randn(1, 2, 128, generator=gen) * scale).to(dtype).to(DEV) for _ in range(2))
+    want = attend(q, k, v, ck, cv, [900])
+    # the type's step (or a subnormal's), the fp32 work on values of this size,
+    # and for bf16 V and the weights in fp16: half a step of the largest value
+    # each, or half of fp16's least
+    bound = ULP[dtype] * want.abs() + FP32 * scale + (2.0 ** -24 if dtype == torch.float16 else 0)
+    if dtype == torch.bfloat16:
+        bound = bound + v.abs().max() * 2 * 2.0 ** -11 + 2.0 ** -25
+    err = (paged.paged_attention_step(q, cache, 0, table, ck, cv).cpu().double() - want).abs()
+    assert (err <= bound).all(), float((err / bound).max())
+    idx = torch.arange(901, device=DEV).expand(1, 8, 901).contiguous()
+    got = paged.paged_indexed_attention(q, cache, 0, table, ck, cv, idx, torch.arange(8, device=DEV) // 4)
+    bound = ULP[dtype] * want.abs() + FP32 * scale + (2.0 ** -24 if dtype == torch.float16 else 0)
+    assert ((got.cpu().double() - want).abs() <= bound).all()
+
+
+def test_strided_and_unaligned_operands():
+    """Queries, current rows, indices and rows to write as views, at odd offsets;
+    `out` given."""
+    gen = torch.Generator().manual_seed(31)
+    cache, table = make([100, 60], 2)
+    raw = torch.randn(2, 2, 100, 131, generator=gen).to(torch.bfloat16).to(DEV)
+    rows_k, rows_v = raw[..., 1:129], raw[..., 3:131]  # rows neither contiguous nor aligned
+    paged.write_tokens(cache, 0, table, rows_k, rows_v, tokens=torch.tensor([100, 60], device=DEV))
+    table.advance(torch.tensor([100, 60], device=DEV), bound=100)
+    k, v = dequantised(rows_k, 32), dequantised(rows_v, 32)
+    q = torch.randn(8, 2, 129, generator=gen).to(DEV).transpose(0, 1)[..., 1:]
+    c = torch.randn(2, 2, 2, 129, generator=gen).to(DEV)[..., 1:]
+    ck, cv = c[0], c[1]
+    out = torch.full((2, 8, 128), float("nan"), device=DEV)
+    want = attend(q, k, v, ck, cv, [100, 60])
+    assert paged.paged_attention_step(q, cache, 0, table, ck, cv, out=out) is out
+    assert ((out.cpu().double() - want).abs() <= ULP[torch.float32] * want.abs() + FP32).all()
+    idx = torch.arange(202, device=DEV).view(1, 1, 202).expand(2, 8, 202)[..., ::2]  # every second token
+    got = paged.paged_indexed_attention(q, cache, 0, table, ck, cv, idx, torch.arange(8) // 4, idx >= 0,
+                                        out=out.view(2, 8, 128))
+    want = attend(q, k, v, ck, cv, [100, 60], [[list(range(0, 101, 2))] * 8, [list(range(0, 61, 2))] * 8])
+    assert ((got.cpu().double() - want).abs() <= ULP[torch.float32] * want.abs() + FP32).all()
+
+
+@pytest.mark.parametrize("dtype", (torch.float16, torch.float32))
+def test_counts_past_the_launch_bound(dtype):
+    """A device count above max_tokens is taken as max_tokens, one past the
+    table as the table's capacity, a negative one as zero."""
+    gen = torch.Generator().manual_seed(32)
+    cache, table = make([96, 96, 96], 1, page=32)
+    k, v = fill(cache, table, 0, [96, 96, 96], gen)
+    table.counts.copy_(torch.tensor([90, 10 ** 12, -4]))
+    table.bound = 70
+    q, ck, cv = (torch.randn(3, n, 128, generator=gen).to(dtype).to(DEV) for n in (2, 1, 1))
+    for most, lengths in ((70, [70, 70, 0]), (96, [90, 96, 0])):
+        want = attend(q, k, v, ck, cv, lengths)
+        got = paged.paged_attention_step(q, cache, 0, table, ck, cv, max_tokens=most)
+        assert ((got.cpu().double() - want).abs() <= allowed(want, dtype, q, k, v, ck, cv)).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("index", (torch.int64, torch.int32))
 @pytest.mark.parametrize("lengths,selected,kv_heads,group", [([700, 33, 0], 1, 2, 4), ([700, 33, 0], 129, 2, 4),
                                                              ([1000], 900, 1, 3), ([64] * 5, 64, 3, 1),
