@@ -146,22 +146,23 @@ def allocate_paged_cache(layers: int, pages: int, kv_heads: int, *, page_tokens:
 def _check_table(pages: PageTable, what: str = "page table") -> tuple[int, int, int]:
     """Shapes and types of a page table (ValueError): (batch, width, pages)."""
     table, counts, refs = pages.table, pages.counts, pages.refs
-    shape, held = table.shape, refs.shape
-    if len(shape) != 2 or table.dtype is not torch.int32 or not table.is_contiguous() or not shape[0] or not shape[1]:
+    shape, batches, held = table.shape, counts.shape, refs.shape
+    if len(shape) != 2 or table.dtype is not torch.int32 or not table.is_contiguous() or not table.numel():
         raise ValueError(f"{what}: table must be a contiguous int32 [batch, width]")
-    if counts.shape != shape[:1] or counts.dtype is not torch.int64 or not counts.is_contiguous():
+    batch, width = shape
+    if len(batches) != 1 or batches[0] != batch or counts.dtype is not torch.int64 or not counts.is_contiguous():
         raise ValueError(f"{what}: counts must be a contiguous int64 [batch]")
-    if len(held) != 1 or refs.dtype is not torch.int32 or not refs.is_contiguous() or not held[0]:
+    if len(held) != 1 or refs.dtype is not torch.int32 or not held[0] or not refs.is_contiguous():
         raise ValueError(f"{what}: refs must be a contiguous int32 [pages]")
     if pages.page_tokens not in PAGE_TOKENS:
         raise ValueError(f"page_tokens must be one of {PAGE_TOKENS}")
-    return shape[0], shape[1], held[0]
+    return batch, width, held[0]
 
 
-def _check_cache(cache: PagedKVCache, pages: PageTable, layer: int = 0) -> tuple[tuple[int, int, int], tuple]:
-    """Shapes and types of a pool and its page table (ValueError):
-    (batch, width, KV heads), and the C entries' arguments for a layer, from
-    the codes to the batch."""
+def _check_cache(cache: PagedKVCache, pages: PageTable, layer: int = 0) -> tuple[int, int, int, tuple]:
+    """Shapes and types of a pool and its page table (ValueError): batch,
+    width, KV heads, and the C entries' arguments for a layer, from the codes
+    to the batch."""
     batch, width, count = _check_table(pages)
     codes, scales, g = cache.codes, cache.scales, cache.dim_group_size
     if g != 16 and g != 32 and g != 64:
@@ -169,7 +170,7 @@ def _check_cache(cache: PagedKVCache, pages: PageTable, layer: int = 0) -> tuple
     shape = codes.shape
     if len(shape) != 6 or codes.dtype is not torch.uint8 or shape[4] != 2 or shape[5] != 64 or not codes.is_contiguous():
         raise ValueError("codes must be a contiguous uint8 [layers, pages, KV heads, page tokens, 2, 64]")
-    layers, held, kv_heads, page_tokens = shape[:4]
+    layers, held, kv_heads, page_tokens, _, _ = shape
     want = (layers, held, kv_heads, page_tokens, 2, 128 // g, 2)
     if scales.shape != want or scales.dtype is not torch.float16 or not scales.is_contiguous():
         raise ValueError(f"scales must be a contiguous float16 {list(want)}")
@@ -178,9 +179,9 @@ def _check_cache(cache: PagedKVCache, pages: PageTable, layer: int = 0) -> tuple
     if not 0 <= layer < layers:
         raise ValueError(f"layer must be in [0, {layers})")
     rows = layer * held * kv_heads * page_tokens
-    return (batch, width, kv_heads), (codes.data_ptr() + rows * 128, scales.data_ptr() + rows * (1024 // g), held,
-                                      kv_heads, page_tokens, g, pages.table.data_ptr(), width, pages.counts.data_ptr(),
-                                      batch)
+    return batch, width, kv_heads, (codes.data_ptr() + rows * 128, scales.data_ptr() + rows * (1024 // g), held,
+                                    kv_heads, page_tokens, g, pages.table.data_ptr(), width, pages.counts.data_ptr(),
+                                    batch)
 
 
 def _check_status(status: torch.Tensor | None) -> None:
@@ -206,22 +207,23 @@ def _tokens(tokens: torch.Tensor, batch: int) -> torch.Tensor:
     return tokens.contiguous()
 
 
-def _rows4(x: torch.Tensor, batch: int, kv_heads: int, what: str) -> torch.Tensor:
-    """K or V rows as [B, KVH, rows, 128] with contiguous, 16-byte aligned
-    rows; a [B, KVH, 128] is one row."""
-    if x.ndim == 3:
-        x = x.unsqueeze(2)
+def _rows(x: torch.Tensor, batch: int, kv_heads: int, what: str) -> tuple[torch.Tensor, int, int, int, int]:
+    """K or V rows [B, KVH, rows, 128], or [B, KVH, 128] for one row, with
+    contiguous and 16-byte aligned rows (a copy where they are not): the
+    tensor, its row count and its strides."""
     shape = x.shape
-    if len(shape) != 4 or shape[0] != batch or shape[1] != kv_heads or shape[3] != 128:
+    n = len(shape)
+    if (n != 4 and n != 3) or shape[0] != batch or shape[1] != kv_heads or shape[-1] != 128:
         raise ValueError(f"{what} must be [{batch}, {kv_heads}, rows, 128] or [{batch}, {kv_heads}, 128]")
     if x.dtype not in _FLOATS:
         raise RuntimeError(f"{x.dtype} is not supported; expected fp32/fp16/bf16")
-    if x.data_ptr() % 16 or not x.is_contiguous():
-        unit = 16 // x.element_size()
-        strides = x.stride()
-        if strides[3] != 1 or x.data_ptr() % 16 or any(s % unit for s in strides[:3]):
-            x = _aligned(x)
-    return x
+    rows = shape[2] if n == 4 else 1
+    if not x.is_contiguous() or x.data_ptr() % 16:
+        strides, unit = x.stride(), 16 // x.element_size()
+        if strides[-1] == 1 and x.data_ptr() % 16 == 0 and not any(s % unit for s in strides[:-1]):
+            return x, rows, strides[0], strides[1], strides[2] if n == 4 else 128
+        x = _aligned(x)
+    return x, rows, kv_heads * rows * 128, rows * 128, 128
 
 
 def _new_table(pages: PageTable, out: PageTable | None) -> PageTable:
@@ -282,18 +284,18 @@ def write_tokens(cache: PagedKVCache, layer: int, pages: PageTable, k: torch.Ten
     ``tokens[b]`` (int64 [B] on the device; None: all rows).  The pages come
     from ``reserve_pages``; a row without one is not written and sets
     ``status`` (bit 4, or bit 1 past the table's end)."""
-    (batch, _, kv_heads), pool = _check_cache(cache, pages, layer)
+    batch, _, kv_heads, pool = _check_cache(cache, pages, layer)
     _check_status(status)
-    k = _rows4(k, batch, kv_heads, "new keys")
-    v = _rows4(v, batch, kv_heads, "new values")
-    if k.shape != v.shape or k.dtype != v.dtype:
+    k, rows, *k_strides = _rows(k, batch, kv_heads, "new keys")
+    v, v_rows, *v_strides = _rows(v, batch, kv_heads, "new values")
+    if rows != v_rows or k.dtype != v.dtype:
         raise ValueError("new keys and values must share shape and dtype")
     if tokens is not None:
         tokens = _tokens(tokens, batch)
     dev = _on_device(cache.codes, cache.scales, pages.table, pages.counts, k, v, tokens, status)
     with nat.on_device(dev):
-        nat.call("popkv_paged_write", k.data_ptr(), v.data_ptr(), nat.dtype_code(k), *k.stride()[:3], *v.stride()[:3],
-                 k.shape[2], nat.ptr(tokens), *pool, nat.ptr(status), nat.stream_of(dev))
+        nat.call("popkv_paged_write", k.data_ptr(), v.data_ptr(), nat.dtype_code(k), *k_strides, *v_strides, rows,
+                 nat.ptr(tokens), *pool, nat.ptr(status), nat.stream_of(dev))
 
 
 def read_tokens(cache: PagedKVCache, layer: int, pages: PageTable, *, dtype: torch.dtype = torch.bfloat16,
@@ -302,7 +304,7 @@ def read_tokens(cache: PagedKVCache, layer: int, pages: PageTable, *, dtype: tor
     """One layer's cached rows as K, V [B, KVH, rows, 128] (``rows``: default
     ``pages.bound``).  Rows past a sequence's count are zero in new tensors and
     left as they are in ``out``."""
-    (batch, _, kv_heads), pool = _check_cache(cache, pages, layer)
+    batch, _, kv_heads, pool = _check_cache(cache, pages, layer)
     if out is None:
         rows = pages.bound if rows is None else int(rows)
         if rows < 0:
@@ -364,7 +366,7 @@ def paged_attention_step(q: torch.Tensor, cache: PagedKVCache, layer: int, pages
     for the launch -- give the largest count a captured graph will see.  The
     workspace holds merge tickets and split states: share it only with this
     module's attention calls, ordered on one stream."""
-    (batch, width, kv_heads), pool = _check_cache(cache, pages, layer)
+    batch, width, kv_heads, pool = _check_cache(cache, pages, layer)
     q_heads, dtype = _step_operands(q, batch, kv_heads, k, v, out)
     if q_heads > 16 * kv_heads:
         raise ValueError("paged attention supports 1 to 16 query heads per KV head")
@@ -395,7 +397,7 @@ def paged_indexed_attention(q: torch.Tensor, cache: PagedKVCache, layer: int, pa
     ``valid_mask`` is False are left out, an index named twice counts twice,
     and a row with nothing left is zero.  head_to_kv: [QH] KV head indices.
     The workspace as for ``paged_attention_step``."""
-    (batch, _, kv_heads), pool = _check_cache(cache, pages, layer)
+    batch, _, kv_heads, pool = _check_cache(cache, pages, layer)
     q_heads, dtype = _step_operands(q, batch, kv_heads, k, v, out)
     shape = indices.shape
     if len(shape) != 3 or shape[0] != batch or shape[1] != q_heads or shape[2] < 1:
@@ -408,14 +410,15 @@ def paged_indexed_attention(q: torch.Tensor, cache: PagedKVCache, layer: int, pa
     qc, kc, vc = _aligned(q), _aligned(k), _aligned(v)
     idx = (indices if indices.dtype in _INDEX_CODES else indices.long()).contiguous()
     mask = None if valid_mask is None else valid_mask.to(torch.bool).contiguous().view(torch.uint8)
-    mapping = head_to_kv.to(device=dev, dtype=torch.int64).contiguous()
+    if head_to_kv.dtype is not torch.int64 or head_to_kv.device != dev or not head_to_kv.is_contiguous():
+        head_to_kv = head_to_kv.to(device=dev, dtype=torch.int64).contiguous()
     output = torch.empty_like(qc) if out is None else out
     selected = shape[2]
     nbytes = nat.lib().popkv_paged_indexed_attention_workspace_bytes(batch, q_heads, selected)
     ws = (workspace or LayerStepWorkspace()).get(nbytes, dev, batch * q_heads)
     with nat.on_device(dev):
         nat.call("popkv_paged_indexed_attention", qc.data_ptr(), dtype, *pool, kc.data_ptr(), vc.data_ptr(),
-                 idx.data_ptr(), _INDEX_CODES[idx.dtype], nat.ptr(mask), mapping.data_ptr(), q_heads, selected,
+                 idx.data_ptr(), _INDEX_CODES[idx.dtype], nat.ptr(mask), head_to_kv.data_ptr(), q_heads, selected,
                  output.data_ptr(), ws.data_ptr(), ws.numel(), nat.stream_of(dev))
     return output
 
@@ -431,7 +434,7 @@ def fork_sequences(cache: PagedKVCache, pages: PageTable, parents: torch.Tensor,
     sets ``status`` bit 4; a parent outside the batch empties the sequence and
     sets bit 8.  Returns a new page table, or writes ``out`` (which may be
     ``pages``); the old one must not be written through any more."""
-    (batch, width, kv_heads), pool = _check_cache(cache, pages)
+    batch, width, kv_heads, pool = _check_cache(cache, pages)
     _check_status(status)
     if parents.shape != (batch,) or parents.dtype is not torch.int64:
         raise ValueError(f"parents must be an int64 [{batch}] tensor")
@@ -455,7 +458,7 @@ def compact_pages(cache: PagedKVCache, pages: PageTable, *, out: PageTable | Non
     Returns the new page table (or ``out``, which may be ``pages``) and the
     int32 [pages] map of where each live page is now (-1: it was free), for
     whoever holds pages outside this table."""
-    (batch, width, kv_heads), pool = _check_cache(cache, pages)
+    batch, width, kv_heads, pool = _check_cache(cache, pages)
     new = _new_table(pages, out)
     dev = _on_device(cache.codes, cache.scales, pages.table, pages.counts, pages.refs, new.table, new.counts, new.refs)
     page_map = torch.empty_like(pages.refs)
