@@ -315,8 +315,8 @@ def read_tokens(cache: PagedKVCache, layer: int, pages: PageTable, *, dtype: tor
         v = torch.empty_like(k)
     else:
         k, v = out
-        if k.ndim != 4 or tuple(k.shape) != (batch, kv_heads, int(k.shape[2]), 128) != k.shape \
-                or v.dtype != k.dtype or not k.is_contiguous() or not v.is_contiguous():
+        if k.ndim != 4 or k.shape != (batch, kv_heads, k.shape[2], 128) or v.shape != k.shape or v.dtype != k.dtype \
+                or not k.is_contiguous() or not v.is_contiguous():
             raise ValueError(f"out must be two contiguous [{batch}, {kv_heads}, rows, 128] tensors")
         if rows is not None and rows != int(k.shape[2]):
             raise ValueError("rows must be out's row count")
@@ -342,8 +342,11 @@ def _step_operands(q: torch.Tensor, batch: int, kv_heads: int, k: torch.Tensor, 
     if v.shape != want:
         raise ValueError(f"current v must be [{batch}, {kv_heads}, 128]")
     dtype = q.dtype
-    if out is not None and (out.shape != shape or not out.is_contiguous()):
-        raise ValueError("out must be a contiguous tensor shaped like q")
+    if out is not None:
+        if out.shape != shape or not out.is_contiguous():
+            raise ValueError("out must be a contiguous tensor shaped like q")
+        if out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr()):  # (workgroups still read them)
+            raise ValueError("out must not be one of the operands")
     if k.dtype != dtype or v.dtype != dtype or (out is not None and out.dtype != dtype):
         raise RuntimeError("queries, current K/V and out must share a dtype")
     return q_heads, nat.dtype_code(q)

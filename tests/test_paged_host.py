@@ -108,6 +108,12 @@ def test_write_and_read_refusals():
         paged.read_tokens(cache, 0, t, out=(k, k.half()))
     with pytest.raises(ValueError, match="out"):
         paged.read_tokens(cache, 0, t, out=(k[:, :1], k[:, :1]))
+    for bad in (k[:, :, :4].contiguous(), k[:2], k[0]):
+        with pytest.raises(ValueError, match="out"):
+            paged.read_tokens(cache, 0, t, out=(k, bad))
+        if bad.shape != (3, 2, 4, 128):
+            with pytest.raises(ValueError, match="out"):
+                paged.read_tokens(cache, 0, t, out=(bad, bad))
     with pytest.raises(ValueError, match="row count"):
         paged.read_tokens(cache, 0, t, rows=4, out=(k, k))
 
@@ -135,6 +141,9 @@ def test_attention_refusals():
         dense(q, k, k, max_tokens=99)
     with pytest.raises(ValueError, match="out"):
         dense(q, k, k, out=q[:, :4])
+    for call in (lambda **kw: dense(q, k, k, **kw), lambda **kw: pick(idx, mapping, **kw)):
+        with pytest.raises(ValueError, match="one of the operands"):
+            call(out=q)
     with pytest.raises(RuntimeError, match="share a dtype"):
         dense(q, k.half(), k)
     with pytest.raises(RuntimeError, match="share a dtype"):
