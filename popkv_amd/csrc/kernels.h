@@ -251,7 +251,7 @@ hipError_t launch_attention_dense(const void* queries, int dtype, const void* pr
                                   int kv_heads, float* partials, uint32_t* tickets, const void* current_k,
                                   const void* current_v, void* output, hipStream_t stream);
 
-// ---- paged 4-bit K/V cache (pages.hip, paged_attention.hip) ----------------
+// ---- paged 4-bit K/V cache (pages.hip, paged_dense.hip, paged_indexed.hip) ---
 // One layer of the pool and the batch's page table: codes [pages, KVH, P, 2,
 // 64] bytes, scales [pages, KVH, P, 2, R] (low, delta) fp16 pairs, table
 // [batch, width] (page of every P = 2^page_log2 tokens; outside [0, pages):

@@ -1,5 +1,5 @@
 // Device pieces shared by the kernels of the paged 4-bit K/V cache
-// (pages.hip, paged_attention.hip): where a token's codes and scales lie.
+// (pages.hip, paged_dense.hip, paged_indexed.hip): where a token's codes and scales lie.
 //
 // One layer's pool: codes [pages, KVH, P, 2, 64] bytes -- a token's K row and
 // V row side by side, 128 bytes, one L2 line, so a gathered token costs one

@@ -1,0 +1,318 @@
+// Decode attention over selected tokens of the paged 4-bit K/V cache, the
+// current token among them or not.
+#include "paged_attention.h"
+
+namespace popkv {
+namespace {
+
+// An octet's state for one query head, fp32 or 16-bit queries.  16-bit: codes
+// as fp16 c - 8, dot products in packed pairs (v_dot2, fp32 sums),
+//   s = delta sum(q (c - 8)) + mid sum(q),  mid = low + 8 delta
+//   acc += (p delta) (c - 8),  the p mid apart
+// 76 instructions a token against 115 for values dequantised to fp32; taking
+// the middle of the codes keeps the two sums from cancelling.
+template <typename T>
+struct PickFold {
+    FoldState<1> st;
+    CodeBits bits;
+    uint32_t qh[8];
+    float qsum, factor, mid;
+    __device__ __forceinline__ void start(const T* src) {
+        st.clear();
+        mid = 0.0f;
+        float q[16], top = 0.0f;
+        load8<T>(src, q);
+        load8<T>(src + 8, q + 8);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(q[i]));
+        top = fmaxf(top, dpp_mov<0xB1>(top));
+        top = fmaxf(top, dpp_mov<0x4E>(top));
+        top = fmaxf(top, dpp_mov<0x141>(top));
+        // fp16 to the queries' precision: the head's largest magnitude in [2^8, 2^9)
+        const int e = static_cast<int>((__float_as_uint(top) >> 23) & 0xffu) - 127;
+        factor = ldexpf(kScaleHigh, e - 8);
+        qsum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            q[i] = ldexpf(q[i], 8 - e);
+            qsum += q[i];
+        }
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) qh[4 * w + j] = pack_half2(q[8 * w + j], q[8 * w + j + 4]);
+    }
+    static __device__ __forceinline__ void centred(const CodeBits& k, uint32_t w, half2_t (&out)[4]) {
+        const half2_t k1032 = {1032.0f16, 1032.0f16}, k16th = {0.0625f16, 0.0625f16}, k72 = {-72.0f16, -72.0f16};
+        uint32_t b[4];
+        biased_pairs(k, w, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            out[j] = j & 1 ? __builtin_elementwise_fma(as_half2(b[j]), k16th, k72) : as_half2(b[j]) - k1032;
+    }
+    __device__ __forceinline__ void fold(const Row4 (&r)[4], const bool (&live)[4]) {
+        float s[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            float dot = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                half2_t c[4];
+                centred(bits, w ? r[t].k.y : r[t].k.x, c);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) dot = __builtin_amdgcn_fdot2(as_half2(qh[4 * w + j]), c[j], dot, false);
+            }
+            const float low = f16_lo(r[t].ks), delta = f16_hi(r[t].ks);
+            const float x = row_sum<8>(fmaf(delta, dot, fmaf(8.0f, delta, low) * qsum)) * factor;
+            s[t] = live[t] ? x : -INFINITY;
+        }
+        const float mn = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), st.m[0]);
+        if (__ballot(mn != st.m[0]) != 0) {
+            const float f = mn == -INFINITY ? 1.0f : exp2_fast(st.m[0] - mn);
+            st.l[0] *= f;
+            mid *= f;
+#pragma unroll
+            for (int d = 0; d < 16; ++d) st.acc[0][d] *= f;
+            st.m[0] = mn;
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const float p = s[t] == -INFINITY ? 0.0f : exp2_fast(s[t] - mn);
+            const float low = f16_lo(r[t].vs), delta = f16_hi(r[t].vs);
+            st.l[0] += p;
+            mid = fmaf(p, fmaf(8.0f, delta, low), mid);
+            const float pd = p * delta;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                half2_t c[4];
+                centred(bits, w ? r[t].v.y : r[t].v.x, c);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    st.acc[0][8 * w + j] = fmaf(static_cast<float>(c[j][0]), pd, st.acc[0][8 * w + j]);
+                    st.acc[0][8 * w + j + 4] = fmaf(static_cast<float>(c[j][1]), pd, st.acc[0][8 * w + j + 4]);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void join() {
+#pragma unroll
+        for (int d = 0; d < 16; ++d) st.acc[0][d] += mid;
+        join_octets<1>(st);
+    }
+};
+template <>
+struct PickFold<float> {
+    FoldState<1> st;
+    float q[1][16];
+    __device__ __forceinline__ void start(const float* src) {
+        st.clear();
+        load8<float>(src, q[0]);
+        load8<float>(src + 8, q[0] + 8);
+    }
+    __device__ __forceinline__ void fold(const Row4 (&r)[4], const bool (&live)[4]) { fold4<1>(st, q, r, live); }
+    __device__ __forceinline__ void join() { join_octets<1>(st); }
+};
+
+constexpr int kPickWaves = 4;
+constexpr int kPickThreads = kPickWaves * kWave;
+constexpr int kPickRows = 8;                            // tokens an octet loads at once
+constexpr int kPickTile = kPickRows * kWave / 8;        // tokens of a wave's pass
+constexpr int kPickLeast = kPickWaves * kPickTile;
+constexpr int kPickBlocks = 512;
+constexpr int kPickState = kState + 1;                  // (m, l, acc[128], hits of the current token)
+
+// Output dim threadIdx.x (of waves 0 and 1) from the row's state and `hits`
+// times the current token; nothing at all gives zero.
+template <typename T>
+__device__ __forceinline__ void pick_finish(float m, float l, float x, float hits, const T* q, const T* ck, const T* cv,
+                                            T* out) {
+    const int lane = threadIdx.x & (kWave - 1), d = threadIdx.x;
+    if (hits > 0.0f) {
+        const float s = scaled_logit(wave_sum(fmaf(Elem<T>::load(q, lane), Elem<T>::load(ck, lane),
+                                                   Elem<T>::load(q, lane + 64) * Elem<T>::load(ck, lane + 64))));
+        const float mx = fmaxf(m, s);
+        const float f = state_weight(m, l, mx);
+        const float w = s == -INFINITY && mx != -INFINITY ? 0.0f : hits * exp2_fast(s - mx);
+        l = fmaf(l, f, w);
+        x = fmaf(x, f, w * Elem<T>::load(cv, d));
+    }
+    Elem<T>::store(out, d, l == 0.0f ? 0.0f : x / l);
+}
+
+// Merges a row's `n` states by the whole workgroup: the weights of 64 states at
+// a time by every wave alike, the sums by threads (dim, half of the states).
+template <typename T>
+__device__ __forceinline__ void pick_merge(const float* ps, int n, const T* q, const T* ck, const T* cv, T* out) {
+    constexpr int NF = 16;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int d = threadIdx.x & 127, half = threadIdx.x >> 7;
+    float m = -INFINITY, l = 0.0f, hits = 0.0f, a = 0.0f;
+    for (int s0 = 0; s0 < n; s0 += 2 * NF) {
+        const int k = min(2 * NF, n - s0);
+        const float* p = ps + static_cast<int64_t>(s0) * kPickState;
+        float x[NF], ms = -INFINITY, ls = 0.0f, hs = 0.0f;
+        if (lane < k) {
+            ms = ld_f32<true>(p + lane * kPickState);
+            ls = ld_f32<true>(p + lane * kPickState + 1);
+            hs = ld_f32<true>(p + lane * kPickState + kState);
+        }
+#pragma unroll
+        for (int j = 0; j < NF; ++j) x[j] = ld_f32<true>(p + min(2 * j + half, k - 1) * kPickState + 2 + d);
+        const float mx = fmaxf(m, wave_max(ms));
+        const float f = state_weight(m, l, mx), w = state_weight(ms, ls, mx);
+        l = fmaf(l, f, wave_sum(ls * w));
+        hits += wave_sum(hs);
+        a *= f;
+#pragma unroll
+        for (int j = 0; j < NF; ++j)
+            if (2 * j + half < k) a = fmaf(__shfl(w, 2 * j + half), x[j], a);
+        m = mx;
+    }
+    __shared__ float s_sum[128];
+    if (half == 1) s_sum[d] = a;
+    __syncthreads();
+    if (wave < 2) pick_finish<T>(m, l, a + s_sum[d], hits, q, ck, cv, out);
+}
+
+// One workgroup a (split of the selection, query head, sequence): every query
+// head gathers its own tokens.  The current token is counted, not read: the
+// merge folds it in as often as it was selected.
+template <typename T, int G, typename I>
+__global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend a, PagedIndexed ix, PagedView c,
+                                                                     int splits, int per) {
+    constexpr int R = 128 / G;
+    const int s = blockIdx.x, qh = blockIdx.y, b = blockIdx.z;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int oct = lane / 8, d0 = (lane % 8) * 16;
+    const int64_t row = static_cast<int64_t>(b) * a.q_heads + qh;
+    const int64_t kvh = ix.head_to_kv[qh];
+    const int h = static_cast<int>(kvh < 0 ? 0 : kvh >= c.kv_heads ? c.kv_heads - 1 : kvh);
+    const int64_t count = clamp_count(c.counts[b], c.width << c.page_log2);
+    PickFold<T> f;
+    f.start(static_cast<const T*>(a.q) + row * 128 + d0);
+    const I* idx = static_cast<const I*>(ix.indices) + row * ix.selected;
+    const uint8_t* valid = ix.valid ? ix.valid + row * ix.selected : nullptr;
+    const int32_t* table = c.table + b * c.width;
+    const int64_t e0 = static_cast<int64_t>(s) * per, e1 = min<int64_t>(e0 + per, ix.selected);
+    int hits = 0;
+    for (int64_t e = e0 + wave * kPickTile; e < e1; e += kPickLeast) {
+        Row4 r[2][4];
+        bool live[2][4];
+        int64_t tok[kPickRows];
+        int32_t page[kPickRows];
+#pragma unroll
+        for (int i = 0; i < kPickRows; ++i) {
+            const int64_t at = e + oct + 8 * i;
+            const bool in = at < e1 && (!valid || valid[at] != 0);
+            tok[i] = in ? static_cast<int64_t>(idx[at]) : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < kPickRows; ++i) {
+            hits += tok[i] == count ? 1 : 0;
+            page[i] = tok[i] >= 0 && tok[i] < count ? table[tok[i] >> c.page_log2] : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < kPickRows; ++i) {
+            Row4& x = r[i / 4][i % 4];
+            const bool there = static_cast<uint32_t>(page[i]) < static_cast<uint32_t>(c.pages);
+            live[i / 4][i % 4] = there;
+            x.k = x.v = make_uint2(0u, 0u);
+            x.ks = x.vs = 0u;
+            if (there) {
+                const int64_t at_row = ((static_cast<int64_t>(page[i]) * c.kv_heads + h) << c.page_log2) +
+                                       (tok[i] & ((1 << c.page_log2) - 1));
+                const char* code = c.codes + at_row * kCodeRow + d0 / 2;
+                const uint32_t* sc = c.scales + at_row * (2 * R) + d0 / G;
+                x.k = *reinterpret_cast<const uint2*>(code);
+                x.v = *reinterpret_cast<const uint2*>(code + 64);
+                x.ks = sc[0];
+                x.vs = sc[R];
+            }
+        }
+        f.fold(r[0], live[0]);
+        f.fold(r[1], live[1]);
+    }
+    f.join();
+    const float wave_hits = wave_sum(static_cast<float>(hits)) * 0.125f;  // the eight lanes of an octet count alike
+    __shared__ float s_m[kPickWaves], s_l[kPickWaves], s_hits[kPickWaves], s_acc[kPickWaves][128];
+    if (lane < 8) {
+#pragma unroll
+        for (int d = 0; d < 16; ++d) s_acc[wave][d0 + d] = f.st.acc[0][d];
+        if (lane == 0) {
+            s_m[wave] = f.st.m[0];
+            s_l[wave] = f.st.l[0];
+            s_hits[wave] = wave_hits;
+        }
+    }
+    __syncthreads();
+    float* mine = a.partials + (row * splits + s) * kPickState;
+    const int64_t kv = (static_cast<int64_t>(b) * c.kv_heads + h) * 128;
+    const T *q = static_cast<const T*>(a.q) + row * 128, *ck = static_cast<const T*>(a.cur_k) + kv,
+            *cv = static_cast<const T*>(a.cur_v) + kv;
+    T* out = static_cast<T*>(a.out) + row * 128;
+    if (wave < 2) {
+        float mx = -INFINITY, l = 0.0f, x = 0.0f, n = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kPickWaves; ++w) mx = fmaxf(mx, s_m[w]);
+#pragma unroll
+        for (int w = 0; w < kPickWaves; ++w) {
+            const float g = state_weight(s_m[w], s_l[w], mx);
+            x = fmaf(g, s_acc[w][threadIdx.x], x);
+            l = fmaf(g, s_l[w], l);
+            n += s_hits[w];
+        }
+        if (splits == 1) {
+            pick_finish<T>(mx, l, x, n, q, ck, cv, out);
+        } else {
+            st_f32<true>(mine + 2 + threadIdx.x, x);
+            if (threadIdx.x == 0) {
+                st_f32<true>(mine, mx);
+                st_f32<true>(mine + 1, l);
+                st_f32<true>(mine + kState, n);
+            }
+        }
+    }
+    if (splits == 1) return;
+    __shared__ uint32_t s_last;
+    if (!last_of(a.tickets + row, splits, &s_last)) return;
+    pick_merge<T>(a.partials + row * splits * kPickState, splits, q, ck, cv, out);
+}
+
+struct PickPlan {
+    int splits, per;
+};
+PickPlan pick_plan(int64_t rows, int64_t selected) {
+    int64_t want = kPickBlocks / rows;
+    const int64_t most = (selected + kPickLeast - 1) / kPickLeast;
+    if (want > most) want = most;
+    if (want < 1) want = 1;
+    const int64_t per = ((selected + want - 1) / want + kPickLeast - 1) / kPickLeast * kPickLeast;
+    return {static_cast<int>((selected + per - 1) / per), static_cast<int>(per)};
+}
+
+template <typename T, int G>
+hipError_t launch_indexed_t(const PagedAttend& a, const PagedIndexed& ix, const PagedView& c, hipStream_t stream) {
+    const PickPlan p = pick_plan(static_cast<int64_t>(c.batch) * a.q_heads, ix.selected);
+    const dim3 grid(static_cast<unsigned>(p.splits), static_cast<unsigned>(a.q_heads), static_cast<unsigned>(c.batch));
+    if (ix.index_dtype == POPKV_INDEX_I32)
+        hipLaunchKernelGGL((paged_indexed_kernel<T, G, int32_t>), grid, dim3(kPickThreads), 0, stream, a, ix, c,
+                           p.splits, p.per);
+    else
+        hipLaunchKernelGGL((paged_indexed_kernel<T, G, int64_t>), grid, dim3(kPickThreads), 0, stream, a, ix, c,
+                           p.splits, p.per);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t paged_indexed_splits(int64_t rows, int64_t selected) { return pick_plan(rows, selected).splits; }
+
+hipError_t launch_paged_indexed(const PagedAttend& a, const PagedIndexed& ix, const PagedView& c, int dtype,
+                                int dim_group, hipStream_t stream) {
+#define POPKV_CALL(T, G) launch_indexed_t<T, G>(a, ix, c, stream)
+    POPKV_PAGED_T(POPKV_CALL)
+#undef POPKV_CALL
+}
+
+}  // namespace popkv
