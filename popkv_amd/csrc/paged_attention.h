@@ -65,109 +65,14 @@ __device__ __forceinline__ void biased_pairs(const CodeBits& k, uint32_t w, uint
     out[3] = (x & k.odd) | k.bias;
 }
 
-// ---- the VALU fold ----------------------------------------------------------
-
-// Eight lanes a token, sixteen dims each (one scale group at G = 16, 32, 64).
-struct Row4 {
-    uint2 k, v;
-    uint32_t ks, vs;
-};
-
-template <int QC>
-struct FoldState {
-    float m[QC], l[QC], acc[QC][16];
-    __device__ __forceinline__ void clear() {
+// The pairs of biased_pairs as c - 8.
+__device__ __forceinline__ void centred_pairs(const CodeBits& k, uint32_t w, half2_t (&out)[4]) {
+    const half2_t k1032 = {1032.0f16, 1032.0f16}, k16th = {0.0625f16, 0.0625f16}, k72 = {-72.0f16, -72.0f16};
+    uint32_t b[4];
+    biased_pairs(k, w, b);
 #pragma unroll
-        for (int j = 0; j < QC; ++j) {
-            m[j] = -INFINITY;
-            l[j] = 0.0f;
-#pragma unroll
-            for (int d = 0; d < 16; ++d) acc[j][d] = 0.0f;
-        }
-    }
-};
-
-// This lane's sixteen values low + c * delta, rounded once to fp32.  (Sums of
-// codes with the scales applied after save an fma a value, but delta sum(q c)
-// and low sum(q) cancel: fp32 results were twice as far off.)
-__device__ __forceinline__ void values16(uint2 w, uint32_t scale, float (&x)[16]) {
-    codes8(w.x, x);
-    codes8(w.y, x + 8);
-    const float low = f16_lo(scale), delta = f16_hi(scale);
-#pragma unroll
-    for (int d = 0; d < 16; ++d) x[d] = fmaf(x[d], delta, low);
-}
-
-// Folds four tokens into the lane octet's state, in fp32.  Dead tokens have
-// zero scales (their values count with weight 0, so they must be finite).
-template <int QC>
-__device__ __forceinline__ void fold4(FoldState<QC>& st, const float (&q)[QC][16], const Row4 (&r)[4],
-                                      const bool (&live)[4]) {
-    float s[QC][4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        float k[16];
-        values16(r[t].k, r[t].ks, k);
-#pragma unroll
-        for (int j = 0; j < QC; ++j) {
-            float dot = 0.0f;
-#pragma unroll
-            for (int d = 0; d < 16; ++d) dot = fmaf(q[j][d], k[d], dot);
-            const float x = scaled_logit(row_sum<8>(dot));
-            s[j][t] = live[t] ? x : -INFINITY;
-        }
-    }
-    bool moved = false;
-    float alpha[QC];
-#pragma unroll
-    for (int j = 0; j < QC; ++j) {
-        const float mn = fmaxf(fmaxf(fmaxf(s[j][0], s[j][1]), fmaxf(s[j][2], s[j][3])), st.m[j]);
-        alpha[j] = mn == -INFINITY ? 1.0f : exp2_fast(st.m[j] - mn);
-        moved = moved || mn != st.m[j];
-        st.m[j] = mn;
-    }
-    if (__ballot(moved) != 0) {
-#pragma unroll
-        for (int j = 0; j < QC; ++j) {
-            st.l[j] *= alpha[j];
-#pragma unroll
-            for (int d = 0; d < 16; ++d) st.acc[j][d] *= alpha[j];
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        float v[16];
-        values16(r[t].v, r[t].vs, v);
-#pragma unroll
-        for (int j = 0; j < QC; ++j) {
-            const float p = s[j][t] == -INFINITY ? 0.0f : exp2_fast(s[j][t] - st.m[j]);
-            st.l[j] += p;
-#pragma unroll
-            for (int d = 0; d < 16; ++d) st.acc[j][d] = fmaf(p, v[d], st.acc[j][d]);
-        }
-    }
-}
-
-// The eight octets' states of a wave become one, in every octet.
-template <int QC>
-__device__ __forceinline__ void join_octets(FoldState<QC>& st) {
-#pragma unroll
-    for (int j = 0; j < QC; ++j) {
-        float mx = st.m[j];
-        mx = fmaxf(mx, lane_xor<8>(mx));
-        mx = fmaxf(mx, lane_xor<16>(mx));
-        mx = fmaxf(mx, lane_xor<32>(mx));
-        const float f = state_weight(st.m[j], st.l[j], mx);
-        auto sum = [](float v) {
-            v += lane_xor<8>(v);
-            v += lane_xor<16>(v);
-            return v + lane_xor<32>(v);
-        };
-        st.l[j] = sum(st.l[j] * f);
-#pragma unroll
-        for (int d = 0; d < 16; ++d) st.acc[j][d] = sum(st.acc[j][d] * f);
-        st.m[j] = mx;
-    }
+    for (int i = 0; i < 4; ++i)
+        out[i] = i & 1 ? __builtin_elementwise_fma(as_half2(b[i]), k16th, k72) : as_half2(b[i]) - k1032;
 }
 
 // ---- the merge --------------------------------------------------------------

@@ -349,16 +349,16 @@ __device__ __forceinline__ void exchange_quarters(uint32_t (&d)[4]) {
     d[3] = y[1];
 }
 
-// Matrix-core form (16-bit types), one workgroup a (share, KV head) for the
-// whole group: its query heads are the 16 rows of the products (those past the
-// group zero), so any group of 1 to 16 costs the same.  A wave takes tiles of
-// 32 tokens, two of 16 for the logits:
+// One workgroup a (share, KV head) for the whole group: its query heads are the
+// 16 rows of matrix products (those past the group zero), so any group of 1 to
+// 16 costs the same.  A wave takes tiles of 32 tokens, two of 16 for the logits:
 //   dot_g[head, token] = q . c       one 16 x 16 x 32 step per 32 dims, codes as
 //                                    they are, each scale group by itself
 //   S = sum_g delta_g dot_g + sum_g low_g qsum_g   in fp32, the second sum by
 //                                    one more product (qsum in two fp16 terms)
-//   O[head, dim] += P . V            V as low + c delta in fp16 (fp16 outputs:
-//                                    exactly, in three parts)
+//   O[head, dim] += P . V            V as low + c delta in fp16 (bf16 tensors), or
+//                                    exactly, in three parts: low, and c times
+//                                    delta's upper seven and lower four bits
 // so keys enter the logits exactly: with the outlier channels that keys have,
 // their rounding to fp16 was four times fp16's own in the result.  (C layout:
 // lane l holds rows 4 (l / 16) .. + 3 of column l % 16; A and B: lane l holds
@@ -367,18 +367,34 @@ __device__ __forceinline__ void exchange_quarters(uint32_t (&d)[4]) {
 // is 1024 + 16 c.  For the keys the queries of odd dims are divided by 16, and
 // what codes of zero would give, times delta, is taken off in that same extra
 // product, so a dword of eight costs five instructions; for the values a packed
-// subtraction and a packed fma follow (13).  A token's 16-byte quarters are exchanged among the four
-// lane groups (lane swaps), so that a step's 32 dims are one group's.
+// subtraction and a packed fma follow (13).  A token's 16-byte quarters are
+// exchanged among the four lane groups (lane swaps), so that a step's 32 dims
+// are one group's.
 // Queries are scaled by a power of two per head (bf16 reaches past fp16, and
-// 1024 times a group's sum must not), and the weights are kept around 2^8, where fp16 keeps
-// 11 bits; fp16 outputs take a second term for the rest of each weight.
+// 1024 times a group's sum must not), and the weights are kept around 2^8, where
+// fp16 keeps 11 bits; fp16 and fp32 take a second term for the rest of each
+// weight (22 bits).  fp32 takes two terms of the queries as well, and codes
+// c - 8 with low + 8 delta beside them, so that the two sums do not cancel: its
+// results are as far off as fp32 products of dequantised values, or less
+// (relative 1e-6 against 2e-6 at 20001 tokens).
+// 8 x 65536 tokens of 8 KV heads, 64-dim groups, 604 MB: bf16 116.7 us (5.2
+// TB/s, as fast as memory streams), fp32 168 (bound by the vector instructions
+// around the products: two terms and exact values are twice bf16's).  A ragged
+// batch of five up to 20001 with 64 query heads, 32-dim groups, 77 MB: fp16 28.4
+// (27.3 with values rounded to fp16), fp32 31.7 (94 by fp32 vector products).
 template <typename T, int G>
-__global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAttend a, PagedView c, int64_t max_tokens,
+__global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend a, PagedView c, int64_t max_tokens,
                                                                          int groups) {
     constexpr int R = 128 / G;
+    constexpr bool F32 = std::is_same_v<T, float>;
     constexpr int HALVES = R == 8 ? 2 : 1;        // groups of a 32-dim step
+    // Query registers: fp32 two terms; 16-bit types a set for each half of a step,
+    // zero in the other (31.3 us at 16-dim groups, a ragged fp16 batch, against 32.9
+    // with the codes masked; fp32 has no registers left for that and masks them).
+    constexpr int QSETS = F32 ? 2 : HALVES;
     constexpr int LOWS = R == 8 ? 2 : 1;          // products for the low terms (four groups each)
-    constexpr int TERMS = std::is_same_v<T, f16_t> ? 2 : 1;
+    constexpr int TERMS = std::is_same_v<T, bf16_t> ? 1 : 2;
+    constexpr int QTOP = F32 ? 5 : 0;             // queries lie below 2^QTOP
     constexpr float kBase = 8.0f, kTop = 15.0f;   // weights start at 2^8 and may grow to 2^15
     constexpr float kNone = -3e38f;               // no weight yet
     constexpr int W = kDenseWaves, ROWS = 8, PITCH = 132;
@@ -488,6 +504,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
     const int pair = 4 * (col & 3) + (col >> 2);  // where the weights of tokens col and 16 + col go
 
     const CodeBits bits;
+    const uint32_t half_mask[2] = {grp < 2 ? ~0u : 0u, grp < 2 ? 0u : ~0u};  // (fp32 at 16-dim groups)
     const uint32_t low_or_delta = grp == 1 ? 0x03020302u : 0x01000100u;  // byte picks of a scale pair
 
     // Starts a part: its first two tiles on their way, then its queries (row
@@ -511,7 +528,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
         f32x4_t acc[8], low_acc = {0.0f, 0.0f, 0.0f, 0.0f};
         float ref[4], l[4];  // rows 4 grp + i: weights are 2^(logit - ref)
         // the queries in fp16, the largest magnitude of a head in [1/2, 1)
-        uint32_t qa[HALVES][4][4], ql[LOWS][4];
+        uint32_t qa[QSETS][4][4], ql[LOWS][4];
         float factor[4];  // of rows 4 grp + i
         {
             float q[4][8], top = 0.0f;
@@ -525,7 +542,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
             top = fmaxf(top, lane_xor<16>(top));
             top = fmaxf(top, lane_xor<32>(top));
             const int e = static_cast<int>((__float_as_uint(top) >> 23) & 0xffu) - 127;
-            const float mine = ldexpf(kScaleHigh, e + 1);
+            const float mine = ldexpf(kScaleHigh, e + 1 - QTOP);
 #pragma unroll
             for (int i = 0; i < 4; ++i) factor[i] = __shfl(mine, 4 * grp + i);
             float sum[4];
@@ -534,14 +551,18 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
                 sum[s] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    q[s][i] = ldexpf(q[s][i], -1 - e);
+                    q[s][i] = ldexpf(q[s][i], QTOP - 1 - e);
                     sum[s] += q[s][i];
-                    if (i & 1) q[s][i] *= 0.0625f;
+                    if (!F32 && (i & 1)) q[s][i] *= 0.0625f;
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t x = pack_half2(q[s][j], q[s][j + 4]);
-                    if constexpr (HALVES == 2) {
+                    if constexpr (F32) {
+                        qa[0][s][j] = x;
+                        qa[1][s][j] = pack_half2(q[s][j] - static_cast<float>(as_half2(x)[0]),
+                                                 q[s][j + 4] - static_cast<float>(as_half2(x)[1]));
+                    } else if constexpr (HALVES == 2) {
                         qa[0][s][j] = grp < 2 ? x : 0u;
                         qa[1][s][j] = grp < 2 ? 0u : x;
                     } else {
@@ -551,8 +572,8 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
                 sum[s] += lane_xor<16>(sum[s]);
             }
             // the low terms' product: lane group 0 holds the groups' sums of queries
-            // for low, lane group 1 minus their products with codes of zero for
-            // delta, each as (high, rest)
+            // for low, lane group 1 minus their products with codes of zero (fp32:
+            // of c = -8) for delta, each as (high, rest)
             float qs[R];
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
@@ -572,7 +593,8 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
                 uint32_t x = 0;
                 if (g < R) {
                     f32x4_t z = {0.0f, 0.0f, 0.0f, 0.0f};
-                    if constexpr (R == 2) z = mfma_f16(none, qa[0][2 * g % 4 + 1], mfma_f16(none, qa[0][2 * g % 4], z));
+                    if constexpr (F32) z[0] = -8.0f * qs[g % R];
+                    else if constexpr (R == 2) z = mfma_f16(none, qa[0][2 * g % 4 + 1], mfma_f16(none, qa[0][2 * g % 4], z));
                     else z = mfma_f16(none, qa[g % HALVES][g / HALVES % 4], z);
                     // (rows of codes times columns of queries: every element of column `col` is head `col`'s)
                     const float term = grp == 0 ? qs[g % R] : -z[0];
@@ -608,6 +630,22 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
 #pragma unroll
                 for (int st = 0; st < 4; ++st) {
                     uint32_t cb[4];
+                    if constexpr (F32) {
+                        half2_t code[4];
+                        centred_pairs(bits, w[st], code);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) cb[i] = __builtin_bit_cast(uint32_t, code[i]);
+#pragma unroll
+                        for (int n = 0; n < HALVES; ++n) {
+                            f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+                            if (R == 2 && (st & 1)) sum = dot[st / 2];
+                            uint32_t x[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) x[i] = HALVES == 2 ? cb[i] & half_mask[n] : cb[i];
+                            dot[R == 2 ? st / 2 : HALVES * st + n] = mfma_f16(qa[0][st], x, mfma_f16(qa[1][st], x, sum));
+                        }
+                        continue;
+                    }
                     biased_pairs(bits, w[st], cb);
                     if constexpr (R == 2) {
                         dot[st / 2] = mfma_f16(qa[0][st], cb, st & 1 ? dot[st / 2] : f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
@@ -639,7 +677,10 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) e[i][u] = fmaf(s[u][i], factor[i], -ref[i]);
+                    for (int u = 0; u < 2; ++u) {
+                        e[i][u] = fmaf(s[u][i], factor[i], -ref[i]);
+                        if constexpr (F32) e[i][u] = fmaf(s[u][i] * factor[i], kScaleLow / kScaleHigh, e[i][u]);
+                    }
                 if (!whole) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -723,6 +764,15 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
                 for (int j = 0; j < 4; ++j) lows[j] = low_halves(x.vs[2 * j], x.vs[2 * j + 1]);
 #pragma unroll
                 for (int n = 0; n < TERMS; ++n) low_acc = mfma_f16(pa[n], lows, low_acc);
+                if constexpr (F32) {
+                    uint32_t eights[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        eights[j] = __builtin_bit_cast(
+                            uint32_t, as_half2(high_halves(x.vs[2 * j], x.vs[2 * j + 1])) * half2_t{8.0f16, 8.0f16});
+#pragma unroll
+                    for (int n = 0; n < TERMS; ++n) low_acc = mfma_f16(pa[n], eights, low_acc);
+                }
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     uint32_t vh[4][4], vl[4][4];
@@ -732,7 +782,8 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
                         const half2_t delta = as_half2(high_halves(x.vs[2 * j], x.vs[2 * j + 1]));
                         const half2_t top7 = as_half2(__builtin_bit_cast(uint32_t, delta) & 0xfff0fff0u);
                         half2_t code[4];
-                        code_pairs(bits, half ? high_halves(v0, v1) : low_halves(v0, v1), code);
+                        if constexpr (F32) centred_pairs(bits, half ? high_halves(v0, v1) : low_halves(v0, v1), code);
+                        else code_pairs(bits, half ? high_halves(v0, v1) : low_halves(v0, v1), code);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             vh[i][j] = __builtin_bit_cast(uint32_t, code[i] * top7);
@@ -745,6 +796,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
                         sum = mfma_f16(pa[0], vh[i], sum);
                         sum = mfma_f16(pa[TERMS - 1], vh[i], sum);
                         sum = mfma_f16(pa[0], vl[i], sum);
+                        if constexpr (F32) sum = mfma_f16(pa[1], vl[i], sum);
                     }
                 }
             }
@@ -802,90 +854,11 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_mfma_kernel(PagedAt
     }
 }
 
-// VALU form (fp32), QC query heads of the group at a time.  A tile of 32
-// tokens lies in one page: its table entry is one scalar.
-template <typename T, int G, int QC>
-__global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend a, PagedView c, int64_t max_tokens,
-                                                                    int groups) {
-    constexpr int R = 128 / G, W = kDenseWaves;
-    const int h = blockIdx.x - div_nonneg(blockIdx.x, c.kv_heads) * c.kv_heads;
-    const int group = a.q_heads / c.kv_heads;
-    const int lane = threadIdx.x & (kWave - 1);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int oct = lane / 8, d0 = (lane % 8) * 16;
-    __shared__ float s_m[W][QC], s_l[W][QC];
-    __shared__ float s_acc[W][QC][128];
-    const int64_t per_page = static_cast<int64_t>(c.kv_heads) << c.page_log2;
-    const int64_t head_row = static_cast<int64_t>(h) << c.page_log2;
-    DenseWalk walk(c, max_tokens, groups);
-    for (DenseShare sh; walk.next(sh);) {
-        for (int j0 = 0; j0 < group; j0 += QC) {
-            const int rows = min(QC, group - j0);
-            float q[QC][16];
-#pragma unroll
-            for (int j = 0; j < QC; ++j) {
-                const int64_t row =
-                    static_cast<int64_t>(sh.b) * a.q_heads + static_cast<int64_t>(h) * group + j0 + min(j, rows - 1);
-                load8<T>(static_cast<const T*>(a.q) + row * 128 + d0, q[j]);
-                load8<T>(static_cast<const T*>(a.q) + row * 128 + d0 + 8, q[j] + 8);
-            }
-            FoldState<QC> st;
-            st.clear();
-            for (int64_t t = sh.t0 + wave * kPageTile; t < sh.t1; t += W * kPageTile) {
-                const int32_t page = c.table[sh.b * c.width + (t >> c.page_log2)];
-                if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(c.pages)) continue;  // uniform
-                const int64_t row0 = page * per_page + head_row + (t & ((1 << c.page_log2) - 1));
-                const int left = static_cast<int>(min<int64_t>(kPageTile, sh.t1 - t));
-                Row4 r[4];
-                bool live[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int tok = oct + 8 * i;
-                    live[i] = tok < left;
-                    const char* code = c.codes + (row0 + tok) * kCodeRow + d0 / 2;
-                    const uint32_t* sc = c.scales + (row0 + tok) * (2 * R) + d0 / G;
-                    r[i].k = *reinterpret_cast<const uint2*>(code);
-                    r[i].v = *reinterpret_cast<const uint2*>(code + 64);
-                    r[i].ks = sc[0];
-                    r[i].vs = live[i] ? sc[R] : 0u;  // what lies behind the last token may be anything
-                }
-                fold4<QC>(st, q, r, live);
-            }
-            join_octets<QC>(st);
-            if (lane < 8) {
-#pragma unroll
-                for (int j = 0; j < QC; ++j) {
-#pragma unroll
-                    for (int d = 0; d < 16; ++d) s_acc[wave][j][d0 + d] = st.acc[j][d];
-                    if (lane == 0) {
-                        s_m[wave][j] = st.m[j];
-                        s_l[wave][j] = st.l[j];
-                    }
-                }
-            }
-            __syncthreads();
-            emit_rows<T, QC, 128>(a, c, sh, h, group, j0, s_m, s_l, s_acc);
-            __syncthreads();
-        }
-        dense_merge<T>(a, c, sh, h, group);
-    }
-}
-
 template <typename T, int G>
 hipError_t launch_dense_t(const PagedAttend& a, const PagedView& c, int64_t max_tokens, hipStream_t stream) {
-    const int group = a.q_heads / c.kv_heads;
     const int per_head = dense_workgroups(c.batch, c.kv_heads, max_tokens);
-    const dim3 grid(static_cast<unsigned>(per_head * c.kv_heads));
-#define POPKV_DENSE(...) \
-    hipLaunchKernelGGL((__VA_ARGS__), grid, dim3(kDenseThreads), 0, stream, a, c, max_tokens, per_head)
-    if constexpr (sizeof(T) == 2) {
-        POPKV_DENSE(paged_dense_mfma_kernel<T, G>);
-    } else {
-        if (group == 1) POPKV_DENSE(paged_dense_kernel<T, G, 1>);
-        else if (group == 2) POPKV_DENSE(paged_dense_kernel<T, G, 2>);
-        else POPKV_DENSE(paged_dense_kernel<T, G, 4>);
-    }
-#undef POPKV_DENSE
+    hipLaunchKernelGGL((paged_dense_kernel<T, G>), dim3(static_cast<unsigned>(per_head * c.kv_heads)),
+                       dim3(kDenseThreads), 0, stream, a, c, max_tokens, per_head);
     return hipGetLastError();
 }
 

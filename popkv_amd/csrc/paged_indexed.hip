@@ -5,15 +5,61 @@
 namespace popkv {
 namespace {
 
-// An octet's state for one query head, fp32 or 16-bit queries.  16-bit: codes
-// as fp16 c - 8, dot products in packed pairs (v_dot2, fp32 sums),
+// Eight lanes a token, sixteen dims each (one scale group at G = 16, 32, 64).
+struct Row4 {
+    uint2 k, v;
+    uint32_t ks, vs;
+};
+
+// An octet's state for one query head, its lane's sixteen dims.
+struct FoldState {
+    float m, l, acc[16];
+    __device__ __forceinline__ void clear() {
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 16; ++d) acc[d] = 0.0f;
+    }
+    // the maximum of four more logits; the state follows it
+    __device__ __forceinline__ bool raise(const float (&s)[4], float& by) {
+        const float mn = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), m);
+        if (__ballot(mn != m) == 0) return false;
+        by = mn == -INFINITY ? 1.0f : exp2_fast(m - mn);
+        l *= by;
+#pragma unroll
+        for (int d = 0; d < 16; ++d) acc[d] *= by;
+        m = mn;
+        return true;
+    }
+    // the eight octets' states of a wave become one, in every octet
+    __device__ __forceinline__ void join() {
+        float mx = m;
+        mx = fmaxf(mx, lane_xor<8>(mx));
+        mx = fmaxf(mx, lane_xor<16>(mx));
+        mx = fmaxf(mx, lane_xor<32>(mx));
+        const float f = state_weight(m, l, mx);
+        auto sum = [](float v) {
+            v += lane_xor<8>(v);
+            v += lane_xor<16>(v);
+            return v + lane_xor<32>(v);
+        };
+        l = sum(l * f);
+#pragma unroll
+        for (int d = 0; d < 16; ++d) acc[d] = sum(acc[d] * f);
+        m = mx;
+    }
+};
+
+// An octet's fold of four tokens for 16-bit and, below, fp32 queries; dead
+// tokens have zero scales (their values count with weight 0).  16-bit: codes as
+// fp16 c - 8, dot products in packed pairs (v_dot2, fp32 sums),
 //   s = delta sum(q (c - 8)) + mid sum(q),  mid = low + 8 delta
 //   acc += (p delta) (c - 8),  the p mid apart
 // 76 instructions a token against 115 for values dequantised to fp32; taking
 // the middle of the codes keeps the two sums from cancelling.
 template <typename T>
 struct PickFold {
-    FoldState<1> st;
+    FoldState st;
     CodeBits bits;
     uint32_t qh[8];
     float qsum, factor, mid;
@@ -42,14 +88,6 @@ struct PickFold {
 #pragma unroll
             for (int j = 0; j < 4; ++j) qh[4 * w + j] = pack_half2(q[8 * w + j], q[8 * w + j + 4]);
     }
-    static __device__ __forceinline__ void centred(const CodeBits& k, uint32_t w, half2_t (&out)[4]) {
-        const half2_t k1032 = {1032.0f16, 1032.0f16}, k16th = {0.0625f16, 0.0625f16}, k72 = {-72.0f16, -72.0f16};
-        uint32_t b[4];
-        biased_pairs(k, w, b);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            out[j] = j & 1 ? __builtin_elementwise_fma(as_half2(b[j]), k16th, k72) : as_half2(b[j]) - k1032;
-    }
     __device__ __forceinline__ void fold(const Row4 (&r)[4], const bool (&live)[4]) {
         float s[4];
 #pragma unroll
@@ -58,7 +96,7 @@ struct PickFold {
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 half2_t c[4];
-                centred(bits, w ? r[t].k.y : r[t].k.x, c);
+                centred_pairs(bits, w ? r[t].k.y : r[t].k.x, c);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) dot = __builtin_amdgcn_fdot2(as_half2(qh[4 * w + j]), c[j], dot, false);
             }
@@ -66,51 +104,76 @@ struct PickFold {
             const float x = row_sum<8>(fmaf(delta, dot, fmaf(8.0f, delta, low) * qsum)) * factor;
             s[t] = live[t] ? x : -INFINITY;
         }
-        const float mn = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), st.m[0]);
-        if (__ballot(mn != st.m[0]) != 0) {
-            const float f = mn == -INFINITY ? 1.0f : exp2_fast(st.m[0] - mn);
-            st.l[0] *= f;
-            mid *= f;
-#pragma unroll
-            for (int d = 0; d < 16; ++d) st.acc[0][d] *= f;
-            st.m[0] = mn;
-        }
+        float by;
+        if (st.raise(s, by)) mid *= by;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            const float p = s[t] == -INFINITY ? 0.0f : exp2_fast(s[t] - mn);
+            const float p = s[t] == -INFINITY ? 0.0f : exp2_fast(s[t] - st.m);
             const float low = f16_lo(r[t].vs), delta = f16_hi(r[t].vs);
-            st.l[0] += p;
+            st.l += p;
             mid = fmaf(p, fmaf(8.0f, delta, low), mid);
             const float pd = p * delta;
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 half2_t c[4];
-                centred(bits, w ? r[t].v.y : r[t].v.x, c);
+                centred_pairs(bits, w ? r[t].v.y : r[t].v.x, c);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    st.acc[0][8 * w + j] = fmaf(static_cast<float>(c[j][0]), pd, st.acc[0][8 * w + j]);
-                    st.acc[0][8 * w + j + 4] = fmaf(static_cast<float>(c[j][1]), pd, st.acc[0][8 * w + j + 4]);
+                    st.acc[8 * w + j] = fmaf(static_cast<float>(c[j][0]), pd, st.acc[8 * w + j]);
+                    st.acc[8 * w + j + 4] = fmaf(static_cast<float>(c[j][1]), pd, st.acc[8 * w + j + 4]);
                 }
             }
         }
     }
     __device__ __forceinline__ void join() {
 #pragma unroll
-        for (int d = 0; d < 16; ++d) st.acc[0][d] += mid;
-        join_octets<1>(st);
+        for (int d = 0; d < 16; ++d) st.acc[d] += mid;
+        st.join();
     }
 };
+// fp32: values low + c * delta, rounded once to fp32.  (Sums of codes with the
+// scales applied after save an fma a value, but delta sum(q c) and low sum(q)
+// cancel: results were twice as far off.)
 template <>
 struct PickFold<float> {
-    FoldState<1> st;
-    float q[1][16];
+    FoldState st;
+    float q[16];
     __device__ __forceinline__ void start(const float* src) {
         st.clear();
-        load8<float>(src, q[0]);
-        load8<float>(src + 8, q[0] + 8);
+        load8<float>(src, q);
+        load8<float>(src + 8, q + 8);
     }
-    __device__ __forceinline__ void fold(const Row4 (&r)[4], const bool (&live)[4]) { fold4<1>(st, q, r, live); }
-    __device__ __forceinline__ void join() { join_octets<1>(st); }
+    static __device__ __forceinline__ void values16(uint2 w, uint32_t scale, float (&x)[16]) {
+        codes8(w.x, x);
+        codes8(w.y, x + 8);
+        const float low = f16_lo(scale), delta = f16_hi(scale);
+#pragma unroll
+        for (int d = 0; d < 16; ++d) x[d] = fmaf(x[d], delta, low);
+    }
+    __device__ __forceinline__ void fold(const Row4 (&r)[4], const bool (&live)[4]) {
+        float s[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            float k[16], dot = 0.0f;
+            values16(r[t].k, r[t].ks, k);
+#pragma unroll
+            for (int d = 0; d < 16; ++d) dot = fmaf(q[d], k[d], dot);
+            const float x = scaled_logit(row_sum<8>(dot));
+            s[t] = live[t] ? x : -INFINITY;
+        }
+        float by;
+        st.raise(s, by);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            float v[16];
+            values16(r[t].v, r[t].vs, v);
+            const float p = s[t] == -INFINITY ? 0.0f : exp2_fast(s[t] - st.m);
+            st.l += p;
+#pragma unroll
+            for (int d = 0; d < 16; ++d) st.acc[d] = fmaf(p, v[d], st.acc[d]);
+        }
+    }
+    __device__ __forceinline__ void join() { st.join(); }
 };
 
 constexpr int kPickWaves = 4;
@@ -238,10 +301,10 @@ __global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend
     __shared__ float s_m[kPickWaves], s_l[kPickWaves], s_hits[kPickWaves], s_acc[kPickWaves][128];
     if (lane < 8) {
 #pragma unroll
-        for (int d = 0; d < 16; ++d) s_acc[wave][d0 + d] = f.st.acc[0][d];
+        for (int d = 0; d < 16; ++d) s_acc[wave][d0 + d] = f.st.acc[d];
         if (lane == 0) {
-            s_m[wave] = f.st.m[0];
-            s_l[wave] = f.st.l[0];
+            s_m[wave] = f.st.m;
+            s_l[wave] = f.st.l;
             s_hits[wave] = wave_hits;
         }
     }
