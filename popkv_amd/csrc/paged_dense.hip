@@ -77,7 +77,8 @@ constexpr int kDenseBlocks = 256;
 // 14.6; 64 of one token 37, 11.5 and 11.4.
 constexpr int kSequenceCost = 24;
 
-// Workgroups of a KV head: one a CU in all, with a tile for each wave.
+// Workgroups of a KV head: one a CU in all, with a tile for each wave (with two
+// 4095 tokens of 8 KV heads take 13.7 us instead of 12.3).
 int dense_workgroups(int64_t batch, int64_t kv_heads, int64_t max_tokens) {
     const int64_t target = kDenseBlocks / kv_heads < 1 ? 1 : kDenseBlocks / kv_heads;
     const int64_t tiles = (max_tokens + kPageTile - 1) / kPageTile;
@@ -274,8 +275,11 @@ __device__ __forceinline__ void merge_rows(const float* ps, int64_t stride, int 
 // The last workgroup of a (sequence, KV head) in several parts merges them.
 // More than kOneLevel merge in two levels, as one workgroup's reading of them is
 // what takes the time: the last workgroup of every kSet leaves the set's state
-// in the place of its first, and the last of those merges the sets'.  Tickets of
-// a (sequence, KV head): kTickets, the sets' from 1 on.
+// in the place of its first, and the last of those merges the sets' (157 parts,
+// 40000 tokens of one KV head with 8 query heads: 17.4 us against 23.9 in one
+// level; up to 32 parts one level is faster, 14.4 us against 17.7 at 16000
+// tokens of 8 KV heads).  Tickets of a (sequence, KV head): kPagedTickets, the
+// sets' from 1 on.
 constexpr int kOneLevel = 32, kSet = 16;
 static_assert(kDenseBlocks / kSet + 1 <= kPagedTickets);
 

@@ -181,6 +181,10 @@ constexpr int kPickThreads = kPickWaves * kWave;
 constexpr int kPickRows = 8;                            // tokens an octet loads at once
 constexpr int kPickTile = kPickRows * kWave / 8;        // tokens of a wave's pass
 constexpr int kPickLeast = kPickWaves * kPickTile;
+// Workgroups in all, two a CU where the selections are long enough for a pass of
+// the workgroup each: four sequences of 2048 of 32767 tokens, 32 heads, 17.3 us
+// (one a CU 20 to 22, four the same), two of them 11.6 (12.3); one of 4096 13.1
+// (10.6 to 12.4, four 13.1); 64 heads of 1500 10.9 (11.9).
 constexpr int kPickBlocks = 512;
 constexpr int kPickState = kState + 1;                  // (m, l, acc[128], hits of the current token)
 
@@ -238,8 +242,13 @@ __device__ __forceinline__ void pick_merge(const float* ps, int n, const T* q, c
 }
 
 // One workgroup a (split of the selection, query head, sequence): every query
-// head gathers its own tokens.  The current token is counted, not read: the
-// merge folds it in as often as it was selected.
+// head gathers its own tokens, a line of codes and one of scales each, eight of
+// them on their way in an octet (four: 19.1 us against 13.5, with fp32 products),
+// the next eight indices behind them.  The current token is counted, not read:
+// the merge folds it in as often as it was selected.  Bound by its chain of
+// reads (index, page table entry, token) and the hand-off of the splits: 4096 of
+// 32767 tokens for each of 32 heads, bf16, 64-dim groups, 20 MB: 13 us (1.5
+// TB/s); 256 of them, without a hand-off, 6.4.
 template <typename T, int G, typename I>
 __global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend a, PagedIndexed ix, PagedView c,
                                                                      int splits, int per) {
@@ -259,17 +268,20 @@ __global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend
     const int32_t* table = c.table + b * c.width;
     const int64_t e0 = static_cast<int64_t>(s) * per, e1 = min<int64_t>(e0 + per, ix.selected);
     int hits = 0;
-    for (int64_t e = e0 + wave * kPickTile; e < e1; e += kPickLeast) {
-        Row4 r[2][4];
-        bool live[2][4];
-        int64_t tok[kPickRows];
-        int32_t page[kPickRows];
+    I tok[kPickRows];
+    auto pick = [&](int64_t e) {
 #pragma unroll
         for (int i = 0; i < kPickRows; ++i) {
             const int64_t at = e + oct + 8 * i;
             const bool in = at < e1 && (!valid || valid[at] != 0);
-            tok[i] = in ? static_cast<int64_t>(idx[at]) : -1;
+            tok[i] = in ? idx[at] : I{-1};
         }
+    };
+    pick(e0 + wave * kPickTile);
+    for (int64_t e = e0 + wave * kPickTile; e < e1; e += kPickLeast) {
+        Row4 r[2][4];
+        bool live[2][4];
+        int32_t page[kPickRows];
 #pragma unroll
         for (int i = 0; i < kPickRows; ++i) {
             hits += tok[i] == count ? 1 : 0;
@@ -293,6 +305,7 @@ __global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend
                 x.vs = sc[R];
             }
         }
+        pick(e + kPickLeast);  // the next pass's, on their way while this one's rows are
         f.fold(r[0], live[0]);
         f.fold(r[1], live[1]);
     }
