@@ -43,6 +43,7 @@ steps, as for ``batch.append_batched``.  Implementation limits: head_dim 128;
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
@@ -192,13 +193,18 @@ def _check_status(status: torch.Tensor | None) -> None:
 def _on_device(first: torch.Tensor, *tensors: torch.Tensor | None) -> torch.device:
     """Every operand on the first one's CUDA device (RuntimeError, as
     elsewhere in the package)."""
-    dev = first.device
-    if not first.is_cuda:
+    index = first.get_device()
+    if index < 0:
         raise RuntimeError("the paged cache must be on a CUDA device")
     for t in tensors:
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"every operand must be on the paged cache's device {dev}, got {t.device}")
-    return dev
+        if t is not None and t.get_device() != index:
+            raise RuntimeError(f"every operand must be on the paged cache's device {first.device}, got {t.device}")
+    return first.device
+
+
+@lru_cache(maxsize=4096)
+def _workspace_bytes(call: str, *sizes: int) -> int:
+    return getattr(nat.lib(), call + "_workspace_bytes")(*sizes)
 
 
 def _tokens(tokens: torch.Tensor, batch: int) -> torch.Tensor:
@@ -267,7 +273,7 @@ def reserve_pages(pages: PageTable, tokens: int | torch.Tensor = 1, *, bound: in
             raise ValueError("tokens must not be negative")
     new = _new_table(pages, out)
     dev = _on_device(pages.table, pages.counts, pages.refs, tokens, status, new.table, new.counts, new.refs)
-    nbytes = nat.lib().popkv_page_reserve_workspace_bytes(batch, count)
+    nbytes = _workspace_bytes("popkv_page_reserve", batch, count)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with nat.on_device(dev):
         nat.call("popkv_page_reserve", pages.table.data_ptr(), pages.counts.data_ptr(), pages.refs.data_ptr(),
@@ -333,7 +339,7 @@ def _step_operands(q: torch.Tensor, batch: int, kv_heads: int, k: torch.Tensor, 
     shape = q.shape
     if len(shape) != 3 or shape[0] != batch or shape[2] != 128:
         raise ValueError(f"q must be [{batch}, query heads, 128]")
-    q_heads = shape[1]
+    _, q_heads, _ = shape
     if q_heads <= 0 or q_heads % kv_heads != 0:
         raise ValueError("query heads must be a positive multiple of the KV heads")
     want = (batch, kv_heads, 128)
@@ -354,7 +360,8 @@ def _step_operands(q: torch.Tensor, batch: int, kv_heads: int, k: torch.Tensor, 
 
 def _aligned(x: torch.Tensor) -> torch.Tensor:
     """x contiguous and 16-byte aligned."""
-    x = x.contiguous()
+    if not x.is_contiguous():
+        return x.contiguous()  # (an allocation of its own)
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
@@ -378,12 +385,12 @@ def paged_attention_step(q: torch.Tensor, cache: PagedKVCache, layer: int, pages
         raise ValueError("max_tokens must cover the page table's bound")
     most = min(most, width * pages.page_tokens)
     dev = _on_device(cache.codes, cache.scales, pages.table, pages.counts, q, k, v, out)
-    qc, kc, vc = _aligned(q), _aligned(k), _aligned(v)
-    output = torch.empty_like(qc) if out is None else out
-    nbytes = nat.lib().popkv_paged_attention_workspace_bytes(batch, q_heads, kv_heads, most)
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    output = torch.empty_like(q) if out is None else out
+    nbytes = _workspace_bytes("popkv_paged_attention", batch, q_heads, kv_heads, most)
     ws = (workspace or LayerStepWorkspace()).get(nbytes, dev, batch * kv_heads)
     with nat.on_device(dev):
-        nat.call("popkv_paged_attention", qc.data_ptr(), dtype, *pool, most, kc.data_ptr(), vc.data_ptr(), q_heads,
+        nat.call("popkv_paged_attention", q.data_ptr(), dtype, *pool, most, k.data_ptr(), v.data_ptr(), q_heads,
                  output.data_ptr(), ws.data_ptr(), ws.numel(), nat.stream_of(dev))
     return output
 
@@ -410,17 +417,17 @@ def paged_indexed_attention(q: torch.Tensor, cache: PagedKVCache, layer: int, pa
     if head_to_kv.ndim != 1 or head_to_kv.shape[0] != q_heads:
         raise ValueError(f"head_to_kv must be a vector of {q_heads} KV head indices")
     dev = _on_device(cache.codes, cache.scales, pages.table, pages.counts, q, k, v, out, indices, valid_mask)
-    qc, kc, vc = _aligned(q), _aligned(k), _aligned(v)
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
     idx = (indices if indices.dtype in _INDEX_CODES else indices.long()).contiguous()
     mask = None if valid_mask is None else valid_mask.to(torch.bool).contiguous().view(torch.uint8)
     if head_to_kv.dtype is not torch.int64 or head_to_kv.device != dev or not head_to_kv.is_contiguous():
         head_to_kv = head_to_kv.to(device=dev, dtype=torch.int64).contiguous()
-    output = torch.empty_like(qc) if out is None else out
+    output = torch.empty_like(q) if out is None else out
     selected = shape[2]
-    nbytes = nat.lib().popkv_paged_indexed_attention_workspace_bytes(batch, q_heads, selected)
+    nbytes = _workspace_bytes("popkv_paged_indexed_attention", batch, q_heads, selected)
     ws = (workspace or LayerStepWorkspace()).get(nbytes, dev, batch * q_heads)
     with nat.on_device(dev):
-        nat.call("popkv_paged_indexed_attention", qc.data_ptr(), dtype, *pool, kc.data_ptr(), vc.data_ptr(),
+        nat.call("popkv_paged_indexed_attention", q.data_ptr(), dtype, *pool, k.data_ptr(), v.data_ptr(),
                  idx.data_ptr(), _INDEX_CODES[idx.dtype], nat.ptr(mask), head_to_kv.data_ptr(), q_heads, selected,
                  output.data_ptr(), ws.data_ptr(), ws.numel(), nat.stream_of(dev))
     return output
@@ -445,7 +452,7 @@ def fork_sequences(cache: PagedKVCache, pages: PageTable, parents: torch.Tensor,
     dev = _on_device(cache.codes, cache.scales, pages.table, pages.counts, pages.refs, parents, status, new.table,
                      new.counts, new.refs)
     parents = parents.contiguous()
-    nbytes = nat.lib().popkv_page_fork_workspace_bytes(batch, width)
+    nbytes = _workspace_bytes("popkv_page_fork", batch, width)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with nat.on_device(dev):
         nat.call("popkv_page_fork", pool[0], pool[1], cache.codes.shape[0], pool[2], kv_heads, pool[4], pool[5], pool[6],
@@ -465,7 +472,7 @@ def compact_pages(cache: PagedKVCache, pages: PageTable, *, out: PageTable | Non
     new = _new_table(pages, out)
     dev = _on_device(cache.codes, cache.scales, pages.table, pages.counts, pages.refs, new.table, new.counts, new.refs)
     page_map = torch.empty_like(pages.refs)
-    nbytes = nat.lib().popkv_page_compact_workspace_bytes(pool[2])
+    nbytes = _workspace_bytes("popkv_page_compact", pool[2])
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with nat.on_device(dev):
         nat.call("popkv_page_compact", pool[0], pool[1], cache.codes.shape[0], pool[2], kv_heads, pool[4], pool[5],
