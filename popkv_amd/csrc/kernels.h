@@ -348,7 +348,7 @@ hipError_t launch_page_compact(const PageCompact& a, const PageMoves& m, hipStre
 
 // Decode attention over the pages (head_dim 128): q, out [batch, QH, 128],
 // current k / v [batch, KVH, 128].  tickets (kPagedTickets for each of batch *
-// KVH, or of batch * QH indexed): zero on entry, left zero.
+// KVH, or one for each of batch * QH indexed): zero on entry, left zero.
 constexpr int kPagedTickets = 32;
 struct PagedAttend {
     const void *q, *cur_k, *cur_v;

@@ -185,6 +185,12 @@ def _check_cache(cache: PagedKVCache, pages: PageTable, layer: int = 0) -> tuple
                                     batch)
 
 
+def _ticket_rows(nbytes: int) -> int:
+    """The zero region of an attention workspace in LayerStepWorkspace's KiB: the
+    same for every call that has at most the C entries' 2^18 bytes of tickets."""
+    return 256 if nbytes <= 1 << 18 else -(-nbytes // 1024)
+
+
 def _check_status(status: torch.Tensor | None) -> None:
     if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
         raise ValueError("status must be an int32 tensor of at least one element")
@@ -375,7 +381,9 @@ def paged_attention_step(q: torch.Tensor, cache: PagedKVCache, layer: int, pages
     head.  ``max_tokens`` (default ``pages.bound``) bounds the device counts
     for the launch -- give the largest count a captured graph will see.  The
     workspace holds merge tickets and split states: share it only with this
-    module's attention calls, ordered on one stream."""
+    module's attention calls, ordered on one stream.  It grows with the calls; a
+    captured graph goes on using the buffer that it was captured with, so let
+    the largest call come first, or keep a workspace for each graph."""
     batch, width, kv_heads, pool = _check_cache(cache, pages, layer)
     q_heads, dtype = _step_operands(q, batch, kv_heads, k, v, out)
     if q_heads > 16 * kv_heads:
@@ -388,7 +396,7 @@ def paged_attention_step(q: torch.Tensor, cache: PagedKVCache, layer: int, pages
     q, k, v = _aligned(q), _aligned(k), _aligned(v)
     output = torch.empty_like(q) if out is None else out
     nbytes = _workspace_bytes("popkv_paged_attention", batch, q_heads, kv_heads, most)
-    ws = (workspace or LayerStepWorkspace()).get(nbytes, dev, batch * kv_heads)
+    ws = (workspace or LayerStepWorkspace()).get(nbytes, dev, _ticket_rows(batch * kv_heads * 128))
     with nat.on_device(dev):
         nat.call("popkv_paged_attention", q.data_ptr(), dtype, *pool, most, k.data_ptr(), v.data_ptr(), q_heads,
                  output.data_ptr(), ws.data_ptr(), ws.numel(), nat.stream_of(dev))
@@ -425,7 +433,7 @@ def paged_indexed_attention(q: torch.Tensor, cache: PagedKVCache, layer: int, pa
     output = torch.empty_like(q) if out is None else out
     selected = shape[2]
     nbytes = _workspace_bytes("popkv_paged_indexed_attention", batch, q_heads, selected)
-    ws = (workspace or LayerStepWorkspace()).get(nbytes, dev, batch * q_heads)
+    ws = (workspace or LayerStepWorkspace()).get(nbytes, dev, _ticket_rows(batch * q_heads * 4))
     with nat.on_device(dev):
         nat.call("popkv_paged_indexed_attention", q.data_ptr(), dtype, *pool, k.data_ptr(), v.data_ptr(),
                  idx.data_ptr(), _INDEX_CODES[idx.dtype], nat.ptr(mask), head_to_kv.data_ptr(), q_heads, selected,

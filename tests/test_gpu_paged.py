@@ -960,6 +960,50 @@ def test_a_captured_decode_step():
     assert torch.equal(cache.codes, other.codes)
 
 
+def test_captured_calls_of_different_rows_share_a_workspace():
+    """Graphs of dense and indexed calls with 2, 8 and 24 rows, captured on one
+    workspace one after the other and replayed in turns: each finds its tickets
+    zero whatever states the others left.  Equal bits with a workspace alone."""
+    gen = torch.Generator().manual_seed(41)
+    calls = []
+    for lengths, kv_heads, group in (([20000], 2, 4), ([9000, 700, 5000], 2, 4)):
+        cache, table = make(lengths, kv_heads, max_tokens=max(lengths) + 1)
+        fill(cache, table, 0, lengths, gen)
+        table.advance(torch.tensor(lengths, device=DEV), bound=max(lengths))
+        batch, qh = len(lengths), kv_heads * group
+        q, ck, cv = (torch.randn(batch, n, 128, generator=gen).to(DEV) for n in (qh, kv_heads, kv_heads))
+        idx = torch.randint(0, 700, (batch, qh, 3000), generator=gen).to(DEV)
+        mapping = torch.arange(qh, device=DEV) // group
+        calls.append(lambda out, ws, a=(q, cache, 0, table, ck, cv): paged.paged_attention_step(*a, workspace=ws, out=out))
+        calls.append(lambda out, ws, a=(q, cache, 0, table, ck, cv, idx, mapping):
+                     paged.paged_indexed_attention(*a, workspace=ws, out=out))
+    shapes = [(1, 8, 128)] * 2 + [(3, 8, 128)] * 2
+    want = [torch.empty(s, device=DEV) for s in shapes]
+    out = [torch.empty(s, device=DEV) for s in shapes]
+    ws = popkv.LayerStepWorkspace()
+    for call, x, y in zip(calls, want, out):
+        call(x, popkv.LayerStepWorkspace())
+    for call, y in list(zip(calls, out)) * 2:  # the workspace takes its size
+        call(y, ws)
+    buffer = ws.buffer
+    graphs = []
+    for call, y in zip(calls, out):
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            call(y, ws)
+    assert ws.buffer is buffer
+    for i in (0, 3, 1, 2, 0, 1, 3, 2, 2, 0, 3, 1, 0):
+        out[i].fill_(float("nan"))
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[i], want[i]), i
+        j = (i + 1) % 4
+        out[j].fill_(float("nan"))
+        calls[j](out[j], ws)  # and eager calls between the replays
+        assert torch.equal(out[j], want[j]), j
+
+
 def test_two_streams_at_once():
     """Two batches on two streams, each with its own workspace."""
     gen = torch.Generator().manual_seed(15)
