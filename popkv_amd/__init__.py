@@ -11,8 +11,15 @@ Hand-written gfx950 HIP kernels behind a C ABI (``include/popkv_hip.h``,
 * ``popkv_amd.popkv``           RetrievalConfig, PopKVCache, build/append,
                                 the per-layer retrieval step (reference popkv.py)
 * ``popkv_amd.decode_runtime``  DecodeEventPool (reference decode_runtime.py)
+
+and beside it, without a counterpart in the reference,
+
+* ``popkv_amd.batch``           decode of sequences of different lengths
+* ``popkv_amd.paged``           a paged 4-bit K/V cache for batched decode: write,
+                                attention, forks, compaction
+* ``popkv_amd.wire``            packed caches as bytes
 """
 from __future__ import annotations
 
-__all__ = ["popkv_cuda", "sparse_kernels", "topk", "popkv", "decode_runtime", "workloads"]
+__all__ = ["popkv_cuda", "sparse_kernels", "topk", "popkv", "decode_runtime", "batch", "paged", "wire", "workloads"]
 __version__ = "0.1.0"
