@@ -19,10 +19,14 @@ __device__ __forceinline__ void fold_states(const float* ps, int64_t stride, int
             ls = ld_f32<true>(ps + (s0 + lane) * stride + 1);
         }
 #pragma unroll
-        for (int j = 0; j < NF; ++j) {
-            const float* p = ps + (s0 + min(j, k - 1)) * stride + 2;
-            x0[j] = ld_f32<true>(p + lane);
-            x1[j] = ld_f32<true>(p + lane + 64);
+        for (int j0 = 0; j0 < NF; j0 += 8) {
+            if (j0 >= k) break;
+#pragma unroll
+            for (int j = j0; j < j0 + 8; ++j) {
+                const float* p = ps + (s0 + min(j, k - 1)) * stride + 2;
+                x0[j] = ld_f32<true>(p + lane);
+                x1[j] = ld_f32<true>(p + lane + 64);
+            }
         }
         const float mx = fmaxf(m, wave_max(ms));
         const float w = state_weight(ms, ls, mx);
@@ -50,17 +54,29 @@ __device__ __forceinline__ float current_logit(const T* q, const T* ck) {
                                       Elem<T>::load(q, lane + 64) * Elem<T>::load(ck, lane + 64))));
 }
 
-// A row's output from its merged state and the current token (NaN logits stay).
+// A row's query and its current token, lanes as in fold_states.
 template <typename T>
-__device__ __forceinline__ void finish_row(float m, float l, float a0, float a1, const T* q, const T* ck, const T* cv,
-                                           T* out) {
-    const int lane = threadIdx.x & (kWave - 1);
-    const float s = current_logit(q, ck), mx = fmaxf(m, s);
-    const float f = state_weight(m, l, mx), w = s == -INFINITY && mx != -INFINITY ? 0.0f : exp2_fast(s - mx);
-    l = fmaf(l, f, w);
-    Elem<T>::store(out, lane, fmaf(a0, f, w * Elem<T>::load(cv, lane)) / l);
-    Elem<T>::store(out, lane + 64, fmaf(a1, f, w * Elem<T>::load(cv, lane + 64)) / l);
-}
+struct CurrentRow {
+    float q0, q1, k0, k1, v0, v1;
+    __device__ __forceinline__ void load(const T* q, const T* ck, const T* cv) {
+        const int lane = threadIdx.x & (kWave - 1);
+        q0 = Elem<T>::load(q, lane);
+        q1 = Elem<T>::load(q, lane + 64);
+        k0 = Elem<T>::load(ck, lane);
+        k1 = Elem<T>::load(ck, lane + 64);
+        v0 = Elem<T>::load(cv, lane);
+        v1 = Elem<T>::load(cv, lane + 64);
+    }
+    // the row's output from its merged state and the current token (NaN logits stay)
+    __device__ __forceinline__ void finish(float m, float l, float a0, float a1, T* out) const {
+        const int lane = threadIdx.x & (kWave - 1);
+        const float s = scaled_logit(wave_sum(fmaf(q0, k0, q1 * k1))), mx = fmaxf(m, s);
+        const float f = state_weight(m, l, mx), w = s == -INFINITY && mx != -INFINITY ? 0.0f : exp2_fast(s - mx);
+        l = fmaf(l, f, w);
+        Elem<T>::store(out, lane, fmaf(a0, f, w * v0) / l);
+        Elem<T>::store(out, lane + 64, fmaf(a1, f, w * v1) / l);
+    }
+};
 
 // Workgroups of eight waves, one a CU.  (Four waves three times a CU, with as
 // many bytes again on their way, were slower, 137 against 116 us at 8 x 64K and
@@ -228,6 +244,13 @@ __device__ __forceinline__ void emit_rows(const PagedAttend& a, const PagedView&
 }
 static_assert(kDenseWaves == 8, "a row's waves are eight neighbouring lanes");
 
+// Waves a row in the merge of a group's `n` states.
+__device__ __forceinline__ int merge_share(int n, int group) {
+    int share = 1;
+    while (share * 2 * group <= kDenseWaves && share * 2 <= n) share *= 2;
+    return share;
+}
+
 // Merges `n` states of each of the group's rows, `stride` floats apart: a row
 // takes a wave, or several waves' shares of its states where the group has fewer
 // rows than the workgroup waves.  done(r, m, l, a0, a1) by the wave that has row
@@ -238,8 +261,7 @@ __device__ __forceinline__ void merge_rows(const float* ps, int64_t stride, int 
     __shared__ float s_part[W][kState];
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    int share = 1;  // waves a row
-    while (share * 2 * group <= W && share * 2 <= n) share *= 2;
+    const int share = merge_share(n, group);
     const int at_once = W / share;
     for (int r0 = 0; r0 < group; r0 += at_once) {
         const int r = r0 + wave / share, part = wave % share;
@@ -309,12 +331,20 @@ __device__ __forceinline__ void dense_merge(const PagedAttend& a, const PagedVie
         n = (n + kSet - 1) / kSet;
         step = kSet;
     }
+    // the current token of the wave's first row on its way with the ticket
+    CurrentRow<T> cur;
+    const int64_t row0 = static_cast<int64_t>(sh.b) * a.q_heads + static_cast<int64_t>(h) * group;
+    const int64_t kv = (static_cast<int64_t>(sh.b) * c.kv_heads + h) * 128;
+    auto load = [&](int r) {
+        cur.load(static_cast<const T*>(a.q) + (row0 + r) * 128, static_cast<const T*>(a.cur_k) + kv,
+                 static_cast<const T*>(a.cur_v) + kv);
+    };
+    const int first = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) / merge_share(n, group);
+    load(min(first, group - 1));
     if (!last_of(tickets, n, &s_last)) return;
     merge_rows(ps, step * stride, n, group, [&](int r, float m, float l, float a0, float a1) {
-        const int64_t row = static_cast<int64_t>(sh.b) * a.q_heads + static_cast<int64_t>(h) * group + r;
-        const int64_t kv = (static_cast<int64_t>(sh.b) * c.kv_heads + h) * 128;
-        finish_row<T>(m, l, a0, a1, static_cast<const T*>(a.q) + row * 128, static_cast<const T*>(a.cur_k) + kv,
-                      static_cast<const T*>(a.cur_v) + kv, static_cast<T*>(a.out) + row * 128);
+        if (r != first) load(r);
+        cur.finish(m, l, a0, a1, static_cast<T*>(a.out) + (row0 + r) * 128);
     });
 }
 

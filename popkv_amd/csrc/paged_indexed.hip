@@ -188,28 +188,37 @@ constexpr int kPickLeast = kPickWaves * kPickTile;
 constexpr int kPickBlocks = 512;
 constexpr int kPickState = kState + 1;                  // (m, l, acc[128], hits of the current token)
 
-// Output dim threadIdx.x (of waves 0 and 1) from the row's state and `hits`
-// times the current token; nothing at all gives zero.
+// A row's query and its current token, for output dim threadIdx.x of waves 0
+// and 1.
 template <typename T>
-__device__ __forceinline__ void pick_finish(float m, float l, float x, float hits, const T* q, const T* ck, const T* cv,
-                                            T* out) {
-    const int lane = threadIdx.x & (kWave - 1), d = threadIdx.x;
-    if (hits > 0.0f) {
-        const float s = scaled_logit(wave_sum(fmaf(Elem<T>::load(q, lane), Elem<T>::load(ck, lane),
-                                                   Elem<T>::load(q, lane + 64) * Elem<T>::load(ck, lane + 64))));
-        const float mx = fmaxf(m, s);
-        const float f = state_weight(m, l, mx);
-        const float w = s == -INFINITY && mx != -INFINITY ? 0.0f : hits * exp2_fast(s - mx);
-        l = fmaf(l, f, w);
-        x = fmaf(x, f, w * Elem<T>::load(cv, d));
+struct CurrentDim {
+    float q0, q1, k0, k1, v;
+    __device__ __forceinline__ void load(const T* q, const T* ck, const T* cv) {
+        const int lane = threadIdx.x & (kWave - 1);
+        q0 = Elem<T>::load(q, lane);
+        q1 = Elem<T>::load(q, lane + 64);
+        k0 = Elem<T>::load(ck, lane);
+        k1 = Elem<T>::load(ck, lane + 64);
+        v = Elem<T>::load(cv, threadIdx.x & 127);
     }
-    Elem<T>::store(out, d, l == 0.0f ? 0.0f : x / l);
-}
+    // the output from the row's state and `hits` times the current token;
+    // nothing at all gives zero
+    __device__ __forceinline__ void finish(float m, float l, float x, float hits, T* out) const {
+        if (hits > 0.0f) {
+            const float s = scaled_logit(wave_sum(fmaf(q0, k0, q1 * k1))), mx = fmaxf(m, s);
+            const float f = state_weight(m, l, mx);
+            const float w = s == -INFINITY && mx != -INFINITY ? 0.0f : hits * exp2_fast(s - mx);
+            l = fmaf(l, f, w);
+            x = fmaf(x, f, w * v);
+        }
+        Elem<T>::store(out, threadIdx.x, l == 0.0f ? 0.0f : x / l);
+    }
+};
 
 // Merges a row's `n` states by the whole workgroup: the weights of 64 states at
 // a time by every wave alike, the sums by threads (dim, half of the states).
 template <typename T>
-__device__ __forceinline__ void pick_merge(const float* ps, int n, const T* q, const T* ck, const T* cv, T* out) {
+__device__ __forceinline__ void pick_merge(const float* ps, int n, const CurrentDim<T>& cur, T* out) {
     constexpr int NF = 16;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int d = threadIdx.x & 127, half = threadIdx.x >> 7;
@@ -224,7 +233,11 @@ __device__ __forceinline__ void pick_merge(const float* ps, int n, const T* q, c
             hs = ld_f32<true>(p + lane * kPickState + kState);
         }
 #pragma unroll
-        for (int j = 0; j < NF; ++j) x[j] = ld_f32<true>(p + min(2 * j + half, k - 1) * kPickState + 2 + d);
+        for (int j0 = 0; j0 < NF; j0 += 4) {
+            if (2 * j0 >= k) break;
+#pragma unroll
+            for (int j = j0; j < j0 + 4; ++j) x[j] = ld_f32<true>(p + min(2 * j + half, k - 1) * kPickState + 2 + d);
+        }
         const float mx = fmaxf(m, wave_max(ms));
         const float f = state_weight(m, l, mx), w = state_weight(ms, ls, mx);
         l = fmaf(l, f, wave_sum(ls * w));
@@ -238,7 +251,7 @@ __device__ __forceinline__ void pick_merge(const float* ps, int n, const T* q, c
     __shared__ float s_sum[128];
     if (half == 1) s_sum[d] = a;
     __syncthreads();
-    if (wave < 2) pick_finish<T>(m, l, a + s_sum[d], hits, q, ck, cv, out);
+    if (wave < 2) cur.finish(m, l, a + s_sum[d], hits, out);
 }
 
 // One workgroup a (split of the selection, query head, sequence): every query
@@ -309,6 +322,10 @@ __global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend
         f.fold(r[0], live[0]);
         f.fold(r[1], live[1]);
     }
+    const int64_t kv = (static_cast<int64_t>(b) * c.kv_heads + h) * 128;
+    CurrentDim<T> cur;  // on its way while the wave's octets join
+    cur.load(static_cast<const T*>(a.q) + row * 128, static_cast<const T*>(a.cur_k) + kv,
+             static_cast<const T*>(a.cur_v) + kv);
     f.join();
     const float wave_hits = wave_sum(static_cast<float>(hits)) * 0.125f;  // the eight lanes of an octet count alike
     __shared__ float s_m[kPickWaves], s_l[kPickWaves], s_hits[kPickWaves], s_acc[kPickWaves][128];
@@ -323,9 +340,6 @@ __global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend
     }
     __syncthreads();
     float* mine = a.partials + (row * splits + s) * kPickState;
-    const int64_t kv = (static_cast<int64_t>(b) * c.kv_heads + h) * 128;
-    const T *q = static_cast<const T*>(a.q) + row * 128, *ck = static_cast<const T*>(a.cur_k) + kv,
-            *cv = static_cast<const T*>(a.cur_v) + kv;
     T* out = static_cast<T*>(a.out) + row * 128;
     if (wave < 2) {
         float mx = -INFINITY, l = 0.0f, x = 0.0f, n = 0.0f;
@@ -339,7 +353,7 @@ __global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend
             n += s_hits[w];
         }
         if (splits == 1) {
-            pick_finish<T>(mx, l, x, n, q, ck, cv, out);
+            cur.finish(mx, l, x, n, out);
         } else {
             st_f32<true>(mine + 2 + threadIdx.x, x);
             if (threadIdx.x == 0) {
@@ -352,7 +366,7 @@ __global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend
     if (splits == 1) return;
     __shared__ uint32_t s_last;
     if (!last_of(a.tickets + row, splits, &s_last)) return;
-    pick_merge<T>(a.partials + row * splits * kPickState, splits, q, ck, cv, out);
+    pick_merge<T>(a.partials + row * splits * kPickState, splits, cur, out);
 }
 
 struct PickPlan {
