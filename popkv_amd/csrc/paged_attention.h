@@ -77,6 +77,40 @@ __device__ __forceinline__ void centred_pairs(const CodeBits& k, uint32_t w, hal
 
 // ---- the merge --------------------------------------------------------------
 
+// Two neighbouring floats of a state (8-byte aligned), as ld_f32<true> and
+// st_f32<true>.
+__device__ __forceinline__ float2 ld_pair(const float* p) {
+    uint64_t* at = reinterpret_cast<uint64_t*>(const_cast<float*>(p));
+    return __builtin_bit_cast(float2, __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+__device__ __forceinline__ void st_pair(float* p, float x, float y) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, make_float2(x, y)),
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Two neighbouring elements.
+template <typename T>
+__device__ __forceinline__ float2 load2(const T* p) {
+    if constexpr (sizeof(T) == 4) {
+        return *reinterpret_cast<const float2*>(p);
+    } else {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+        if constexpr (Elem<T>::kDtype == POPKV_DTYPE_F16) return make_float2(f16_lo(w), f16_hi(w));
+        else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store2(T* p, float x, float y) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float2*>(p) = make_float2(x, y);
+    } else {
+        uint32_t w;
+        if constexpr (Elem<T>::kDtype == POPKV_DTYPE_F16) w = f16_rne(x) | static_cast<uint32_t>(f16_rne(y)) << 16;
+        else w = bf16_rne(x) | static_cast<uint32_t>(bf16_rne(y)) << 16;
+        *reinterpret_cast<uint32_t*>(p) = w;
+    }
+}
+
 // Whether this workgroup is the last of `n` to come here (the states before it
 // are acknowledged; the ticket goes back to zero).
 __device__ __forceinline__ bool last_of(uint32_t* ticket, uint32_t n, uint32_t* s_last) {

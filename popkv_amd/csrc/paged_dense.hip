@@ -5,76 +5,56 @@
 namespace popkv {
 namespace {
 
-// Adds `n` states, `stride` floats apart, to a wave's running (m, l, a0, a1);
-// a lane owns dims lane and lane + 64.
-__device__ __forceinline__ void fold_states(const float* ps, int64_t stride, int n, float& m, float& l, float& a0,
-                                            float& a1) {
+// Adds `n` states, `stride` floats apart, to a wave's running (m, l, a); a lane
+// owns dims 2 lane and 2 lane + 1.
+__device__ __forceinline__ void fold_states(const float* ps, int64_t stride, int n, float& m, float& l, float2& a) {
     constexpr int NF = 32;
     const int lane = threadIdx.x & (kWave - 1);
     for (int s0 = 0; s0 < n; s0 += NF) {
-        float ms = -INFINITY, ls = 0.0f, x0[NF], x1[NF];
+        float2 state = make_float2(-INFINITY, 0.0f), x[NF];
         const int k = min(NF, n - s0);
-        if (lane < k) {
-            ms = ld_f32<true>(ps + (s0 + lane) * stride);
-            ls = ld_f32<true>(ps + (s0 + lane) * stride + 1);
-        }
+        if (lane < k) state = ld_pair(ps + (s0 + lane) * stride);
 #pragma unroll
         for (int j0 = 0; j0 < NF; j0 += 8) {
             if (j0 >= k) break;
 #pragma unroll
-            for (int j = j0; j < j0 + 8; ++j) {
-                const float* p = ps + (s0 + min(j, k - 1)) * stride + 2;
-                x0[j] = ld_f32<true>(p + lane);
-                x1[j] = ld_f32<true>(p + lane + 64);
-            }
+            for (int j = j0; j < j0 + 8; ++j) x[j] = ld_pair(ps + (s0 + min(j, k - 1)) * stride + 2 + 2 * lane);
         }
-        const float mx = fmaxf(m, wave_max(ms));
-        const float w = state_weight(ms, ls, mx);
+        const float mx = fmaxf(m, wave_max(state.x));
+        const float w = state_weight(state.x, state.y, mx);
         const float f = state_weight(m, l, mx);
-        l = fmaf(l, f, wave_sum(ls * w));
-        a0 *= f;
-        a1 *= f;
+        l = fmaf(l, f, wave_sum(state.y * w));
+        a.x *= f;
+        a.y *= f;
 #pragma unroll
         for (int j = 0; j < NF; ++j) {
             if (j < k) {
                 const float wj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), j));
-                a0 = fmaf(wj, x0[j], a0);
-                a1 = fmaf(wj, x1[j], a1);
+                a.x = fmaf(wj, x[j].x, a.x);
+                a.y = fmaf(wj, x[j].y, a.y);
             }
         }
         m = mx;
     }
 }
 
-// A row's logit with the current token, by one wave.
-template <typename T>
-__device__ __forceinline__ float current_logit(const T* q, const T* ck) {
-    const int lane = threadIdx.x & (kWave - 1);
-    return scaled_logit(wave_sum(fmaf(Elem<T>::load(q, lane), Elem<T>::load(ck, lane),
-                                      Elem<T>::load(q, lane + 64) * Elem<T>::load(ck, lane + 64))));
-}
-
 // A row's query and its current token, lanes as in fold_states.
 template <typename T>
 struct CurrentRow {
-    float q0, q1, k0, k1, v0, v1;
-    __device__ __forceinline__ void load(const T* q, const T* ck, const T* cv) {
-        const int lane = threadIdx.x & (kWave - 1);
-        q0 = Elem<T>::load(q, lane);
-        q1 = Elem<T>::load(q, lane + 64);
-        k0 = Elem<T>::load(ck, lane);
-        k1 = Elem<T>::load(ck, lane + 64);
-        v0 = Elem<T>::load(cv, lane);
-        v1 = Elem<T>::load(cv, lane + 64);
+    float2 q, k, v;
+    __device__ __forceinline__ void load(const T* q_row, const T* k_row, const T* v_row) {
+        const int d = 2 * (threadIdx.x & (kWave - 1));
+        q = load2<T>(q_row + d);
+        k = load2<T>(k_row + d);
+        v = load2<T>(v_row + d);
     }
+    __device__ __forceinline__ float logit() const { return scaled_logit(wave_sum(fmaf(q.x, k.x, q.y * k.y))); }
     // the row's output from its merged state and the current token (NaN logits stay)
-    __device__ __forceinline__ void finish(float m, float l, float a0, float a1, T* out) const {
-        const int lane = threadIdx.x & (kWave - 1);
-        const float s = scaled_logit(wave_sum(fmaf(q0, k0, q1 * k1))), mx = fmaxf(m, s);
+    __device__ __forceinline__ void finish(float m, float l, float2 a, T* out) const {
+        const float s = logit(), mx = fmaxf(m, s);
         const float f = state_weight(m, l, mx), w = s == -INFINITY && mx != -INFINITY ? 0.0f : exp2_fast(s - mx);
         l = fmaf(l, f, w);
-        Elem<T>::store(out, lane, fmaf(a0, f, w * v0) / l);
-        Elem<T>::store(out, lane + 64, fmaf(a1, f, w * v1) / l);
+        store2<T>(out + 2 * (threadIdx.x & (kWave - 1)), fmaf(a.x, f, w * v.x) / l, fmaf(a.y, f, w * v.y) / l);
     }
 };
 
@@ -191,16 +171,18 @@ __device__ __forceinline__ void emit_rows(const PagedAttend& a, const PagedView&
                                           int group, int r0, const float (*s_m)[ROWS], const float (*s_l)[ROWS],
                                           const float (*s_acc)[ROWS][PITCH]) {
     constexpr int W = kDenseWaves;
+    static_assert(ROWS <= W);
     __shared__ float s_cur[ROWS];
     const int rows = min(ROWS, group - r0);
     const int64_t kv = (static_cast<int64_t>(sh.b) * c.kv_heads + h) * 128;
     const int64_t row0 = static_cast<int64_t>(sh.b) * a.q_heads + static_cast<int64_t>(h) * group + r0;
+    CurrentRow<T> cur;  // of the wave's own row, where the outputs are written here
+    const int lane = threadIdx.x & (kWave - 1), own = threadIdx.x / kWave;
     if (sh.n == 1) {
-        for (int r = threadIdx.x / kWave; r < rows; r += W) {
-            const float x = current_logit(static_cast<const T*>(a.q) + (row0 + r) * 128,
-                                          static_cast<const T*>(a.cur_k) + kv);
-            if ((threadIdx.x & (kWave - 1)) == 0) s_cur[r] = x;
-        }
+        const T* q = static_cast<const T*>(a.q) + (row0 + min(own, rows - 1)) * 128;
+        cur.load(q, static_cast<const T*>(a.cur_k) + kv, static_cast<const T*>(a.cur_v) + kv);
+        const float x = cur.logit();
+        if (lane == 0 && own < rows) s_cur[own] = x;
         __syncthreads();
     }
     // a row's maximum and the factors of its waves, once
@@ -223,26 +205,25 @@ __device__ __forceinline__ void emit_rows(const PagedAttend& a, const PagedView&
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < rows * 128; i += W * kWave) {
-        const int j = i / 128, d = i % 128;
-        float x = 0.0f;
+    if (own >= rows) return;
+    float2 x = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int w = 0; w < W; ++w) x = fmaf(s_f[j][w], s_acc[w][j][d], x);
-        if (sh.n == 1) {
-            x = fmaf(s_f[j][W + 2], Elem<T>::load(static_cast<const T*>(a.cur_v) + kv, d), x);
-            Elem<T>::store(static_cast<T*>(a.out) + (row0 + j) * 128, d, x / s_f[j][W + 1]);
-        } else {
-            float* p = a.partials +
-                       ((static_cast<int64_t>(sh.first + sh.s) * c.kv_heads + h) * group + r0 + j) * kState;
-            st_f32<true>(p + 2 + d, x);
-            if (d == 0) {
-                st_f32<true>(p, s_f[j][W]);
-                st_f32<true>(p + 1, s_f[j][W + 1]);
-            }
-        }
+    for (int w = 0; w < W; ++w) {
+        const float2 y = *reinterpret_cast<const float2*>(&s_acc[w][own][2 * lane]);
+        x.x = fmaf(s_f[own][w], y.x, x.x);
+        x.y = fmaf(s_f[own][w], y.y, x.y);
+    }
+    if (sh.n == 1) {
+        const float l = s_f[own][W + 1], w = s_f[own][W + 2];
+        store2<T>(static_cast<T*>(a.out) + (row0 + own) * 128 + 2 * lane, fmaf(w, cur.v.x, x.x) / l,
+                  fmaf(w, cur.v.y, x.y) / l);
+    } else {
+        float* p = a.partials + ((static_cast<int64_t>(sh.first + sh.s) * c.kv_heads + h) * group + r0 + own) * kState;
+        st_pair(p + 2 + 2 * lane, x.x, x.y);
+        if (lane == 0) st_pair(p, s_f[own][W], s_f[own][W + 1]);
     }
 }
-static_assert(kDenseWaves == 8, "a row's waves are eight neighbouring lanes");
+static_assert(kDenseWaves == 8, "a row's waves are eight neighbouring lanes, a wave for each of eight rows");
 
 // Waves a row in the merge of a group's `n` states.
 __device__ __forceinline__ int merge_share(int n, int group) {
@@ -253,22 +234,23 @@ __device__ __forceinline__ int merge_share(int n, int group) {
 
 // Merges `n` states of each of the group's rows, `stride` floats apart: a row
 // takes a wave, or several waves' shares of its states where the group has fewer
-// rows than the workgroup waves.  done(r, m, l, a0, a1) by the wave that has row
-// r's state.
+// rows than the workgroup waves.  done(r, m, l, a) by the wave that has row r's
+// state.
 template <typename F>
 __device__ __forceinline__ void merge_rows(const float* ps, int64_t stride, int n, int group, F&& done) {
     constexpr int W = kDenseWaves;
-    __shared__ float s_part[W][kState];
+    __shared__ __align__(8) float s_part[W][kState];
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int share = merge_share(n, group);
     const int at_once = W / share;
     for (int r0 = 0; r0 < group; r0 += at_once) {
         const int r = r0 + wave / share, part = wave % share;
-        float m = -INFINITY, l = 0.0f, a0 = 0.0f, a1 = 0.0f;
+        float m = -INFINITY, l = 0.0f;
+        float2 a = make_float2(0.0f, 0.0f);
         if (r < group) {
             const int s0 = n * part / share, s1 = n * (part + 1) / share;
-            fold_states(ps + s0 * stride + static_cast<int64_t>(r) * kState, stride, s1 - s0, m, l, a0, a1);
+            fold_states(ps + s0 * stride + static_cast<int64_t>(r) * kState, stride, s1 - s0, m, l, a);
         }
         if (share > 1) {
             __syncthreads();
@@ -276,21 +258,20 @@ __device__ __forceinline__ void merge_rows(const float* ps, int64_t stride, int 
                 s_part[wave][0] = m;
                 s_part[wave][1] = l;
             }
-            s_part[wave][2 + lane] = a0;
-            s_part[wave][66 + lane] = a1;
+            *reinterpret_cast<float2*>(&s_part[wave][2 + 2 * lane]) = a;
             __syncthreads();
             if (part == 0 && r < group) {
                 for (int w = 1; w < share; ++w) {
                     const float m2 = s_part[wave + w][0], l2 = s_part[wave + w][1], mx = fmaxf(m, m2);
                     const float f = state_weight(m, l, mx), g = state_weight(m2, l2, mx);
                     l = fmaf(l, f, l2 * g);
-                    a0 = fmaf(a0, f, s_part[wave + w][2 + lane] * g);
-                    a1 = fmaf(a1, f, s_part[wave + w][66 + lane] * g);
+                    a.x = fmaf(a.x, f, s_part[wave + w][2 + 2 * lane] * g);
+                    a.y = fmaf(a.y, f, s_part[wave + w][3 + 2 * lane] * g);
                     m = mx;
                 }
             }
         }
-        if (part == 0 && r < group) done(r, m, l, a0, a1);
+        if (part == 0 && r < group) done(r, m, l, a);
     }
 }
 
@@ -319,14 +300,10 @@ __device__ __forceinline__ void dense_merge(const PagedAttend& a, const PagedVie
         const int set = sh.s / kSet, in_set = min(kSet, n - set * kSet);
         float* dst = ps + set * kSet * stride;
         if (!last_of(tickets + 1 + set, in_set, &s_last)) return;
-        merge_rows(dst, stride, in_set, group, [&](int r, float m, float l, float a0, float a1) {
+        merge_rows(dst, stride, in_set, group, [&](int r, float m, float l, float2 a) {
             float* p = dst + static_cast<int64_t>(r) * kState;
-            if (lane == 0) {
-                st_f32<true>(p, m);
-                st_f32<true>(p + 1, l);
-            }
-            st_f32<true>(p + 2 + lane, a0);
-            st_f32<true>(p + 66 + lane, a1);
+            if (lane == 0) st_pair(p, m, l);
+            st_pair(p + 2 + 2 * lane, a.x, a.y);
         });
         n = (n + kSet - 1) / kSet;
         step = kSet;
@@ -342,9 +319,9 @@ __device__ __forceinline__ void dense_merge(const PagedAttend& a, const PagedVie
     const int first = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) / merge_share(n, group);
     load(min(first, group - 1));
     if (!last_of(tickets, n, &s_last)) return;
-    merge_rows(ps, step * stride, n, group, [&](int r, float m, float l, float a0, float a1) {
+    merge_rows(ps, step * stride, n, group, [&](int r, float m, float l, float2 acc) {
         if (r != first) load(r);
-        cur.finish(m, l, a0, a1, static_cast<T*>(a.out) + (row0 + r) * 128);
+        cur.finish(m, l, acc, static_cast<T*>(a.out) + (row0 + r) * 128);
     });
 }
 
