@@ -67,14 +67,14 @@ constexpr int kDenseThreads = kDenseWaves * kWave;
 constexpr int kDenseBlocks = 256;
 
 // What a further sequence costs a workgroup beside its tiles, in tiles: the
-// queries, the join of the waves, the state or output.  Sequences 0, 14 and 28
-// tiles apart: a ragged batch of five up to 20001, fp16 8 queries a KV head, 30.4,
-// 28.3 and 26.5 us; 64 up to 2000 42, 36.2 and 33.8; 16 up to 1000 20.2, 13.7 and
-// 14.6; 64 of one token 37, 11.5 and 11.4.
+// queries, the join of the waves, the state or output.  Sequences 0, 14, 24 and 30
+// tiles apart: a ragged batch of five up to 20001, fp16 8 queries a KV head, 31.2,
+// 28.2, 26.6 and 27.0 us; 64 up to 2000 41.0, 34.5, 32.6 and 32.2; 16 up to 1000
+// 19.0, 12.5, 12.8 and 13.6; 64 of one token 34, 11.0, 11.0 and 10.8.
 constexpr int kSequenceCost = 24;
 
 // Workgroups of a KV head: one a CU in all, with a tile for each wave (with two
-// 4095 tokens of 8 KV heads take 13.7 us instead of 12.3).
+// 4095 tokens of 8 KV heads take 12.4 us instead of 10.9).
 int dense_workgroups(int64_t batch, int64_t kv_heads, int64_t max_tokens) {
     const int64_t target = kDenseBlocks / kv_heads < 1 ? 1 : kDenseBlocks / kv_heads;
     const int64_t tiles = (max_tokens + kPageTile - 1) / kPageTile;
@@ -279,8 +279,8 @@ __device__ __forceinline__ void merge_rows(const float* ps, int64_t stride, int 
 // More than kOneLevel merge in two levels, as one workgroup's reading of them is
 // what takes the time: the last workgroup of every kSet leaves the set's state
 // in the place of its first, and the last of those merges the sets' (157 parts,
-// 40000 tokens of one KV head with 8 query heads: 17.4 us against 23.9 in one
-// level; up to 32 parts one level is faster, 14.4 us against 17.7 at 16000
+// 40000 tokens of one KV head with 8 query heads: 15.6 us against 22.1 in one
+// level; up to 32 parts one level is faster, 13.1 us against 15.7 at 16000
 // tokens of 8 KV heads).  Tickets of a (sequence, KV head): kPagedTickets, the
 // sets' from 1 on.
 constexpr int kOneLevel = 32, kSet = 16;
@@ -388,11 +388,14 @@ __device__ __forceinline__ void exchange_quarters(uint32_t (&d)[4]) {
 // c - 8 with low + 8 delta beside them, so that the two sums do not cancel: its
 // results are as far off as fp32 products of dequantised values, or less
 // (relative 1e-6 against 2e-6 at 20001 tokens).
-// 8 x 65536 tokens of 8 KV heads, 64-dim groups, 604 MB: bf16 116.7 us (5.2
-// TB/s, as fast as memory streams), fp32 168 (bound by the vector instructions
-// around the products: two terms and exact values are twice bf16's).  A ragged
-// batch of five up to 20001 with 64 query heads, 32-dim groups, 77 MB: fp16 28.4
-// (27.3 with values rounded to fp16), fp32 31.7 (94 by fp32 vector products).
+// 8 x 65536 tokens of 8 KV heads, 64-dim groups, 604 MB: bf16 114 us (5.3 TB/s,
+// as fast as memory streams), fp32 154 (bound by the vector instructions around
+// the products: two terms and exact values are twice bf16's).  A ragged batch of
+// five up to 20001 with 64 query heads, 32-dim groups, 77 MB: fp16 26.6 (a
+// twenty-fifth less with values rounded to fp16), fp32 30.7 (94 by fp32 vector
+// products).  4095 tokens, 5 MB, 10.9: a chain of reads, one tile a wave, the
+// hand-off.  Queries' elements below 2^-30 (16-bit types 2^-21) of the head's
+// largest are rounded away.
 template <typename T, int G>
 __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend a, PagedView c, int64_t max_tokens,
                                                                          int groups) {
