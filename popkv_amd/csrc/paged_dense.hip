@@ -394,8 +394,9 @@ __device__ __forceinline__ void exchange_quarters(uint32_t (&d)[4]) {
 // five up to 20001 with 64 query heads, 32-dim groups, 77 MB: fp16 26.6 (a
 // twenty-fifth less with values rounded to fp16), fp32 30.7 (94 by fp32 vector
 // products).  4095 tokens, 5 MB, 10.9: a chain of reads, one tile a wave, the
-// hand-off.  Queries' elements below 2^-30 (16-bit types 2^-21) of the head's
-// largest are rounded away.
+// hand-off.  (What the queries' fp16 terms round: 16-bit queries are exact down to
+// 2^-9 of the head's largest and off by at most 2^-20 of it below; fp32 ones by
+// 2^-24 of themselves or 2^-29 of the largest.)
 template <typename T, int G>
 __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend a, PagedView c, int64_t max_tokens,
                                                                          int groups) {

@@ -274,7 +274,7 @@ def reserve_pages(pages: PageTable, tokens: int | torch.Tensor = 1, *, bound: in
     if isinstance(tokens, torch.Tensor):
         tokens = _tokens(tokens, batch)
     else:
-        each, tokens = int(tokens), None
+        each, tokens = min(int(tokens), pages.capacity + 1), None  # (more than fit are as good as one more)
         if each < 0:
             raise ValueError("tokens must not be negative")
     new = _new_table(pages, out)
