@@ -78,25 +78,6 @@ template <> __device__ __forceinline__ void load8<float>(const float* p, float v
     v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
 
-// Eight consecutive elements to a 16-byte aligned address.
-template <typename T> __device__ __forceinline__ void store8(T* p, const float v[8]);
-template <> __device__ __forceinline__ void store8<bf16_t>(bf16_t* p, const float v[8]) {
-    uint32_t u[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = bf16_rne(v[2 * i]) | (static_cast<uint32_t>(bf16_rne(v[2 * i + 1])) << 16);
-    *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
-}
-template <> __device__ __forceinline__ void store8<f16_t>(f16_t* p, const float v[8]) {
-    uint32_t u[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = f16_rne(v[2 * i]) | (static_cast<uint32_t>(f16_rne(v[2 * i + 1])) << 16);
-    *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
-}
-template <> __device__ __forceinline__ void store8<float>(float* p, const float v[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
-
 // ---- representative reduction trees ---------------------------------------
 // The production packers reduce one representative group's 32 (or 16) lane
 // contributions with a halving tree: a_i = z_i + z_{i+16}, then +8, +4, +2, +1.

@@ -101,14 +101,8 @@ __device__ __forceinline__ float2 load2(const T* p) {
 }
 template <typename T>
 __device__ __forceinline__ void store2(T* p, float x, float y) {
-    if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float2*>(p) = make_float2(x, y);
-    } else {
-        uint32_t w;
-        if constexpr (Elem<T>::kDtype == POPKV_DTYPE_F16) w = f16_rne(x) | static_cast<uint32_t>(f16_rne(y)) << 16;
-        else w = bf16_rne(x) | static_cast<uint32_t>(bf16_rne(y)) << 16;
-        *reinterpret_cast<uint32_t*>(p) = w;
-    }
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(p) = make_float2(x, y);
+    else *reinterpret_cast<uint32_t*>(p) = pack2<T>(x, y);
 }
 
 // Whether this workgroup is the last of `n` to come here (the states before it

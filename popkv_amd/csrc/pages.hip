@@ -20,6 +20,14 @@ constexpr float kScaleLimit = 57344.0f;
 template <typename T>
 struct Eight {
     Raw8<T> raw;
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (sizeof(T) == 4) {
+            raw.a = __builtin_bit_cast(float4, load_once(p));
+            raw.b = __builtin_bit_cast(float4, load_once(p + 4));
+        } else {
+            raw.u = __builtin_bit_cast(uint4, load_once(p));
+        }
+    }
     // the largest magnitude's bits: at least kNotFinite for infinity and NaN
     static constexpr uint32_t kNotFinite = Elem<T>::kDtype == POPKV_DTYPE_F32 ? 0x7f800000u
                                            : Elem<T>::kDtype == POPKV_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
@@ -134,8 +142,8 @@ __global__ __launch_bounds__(256) void paged_write_kernel(PagedWrite a, PagedVie
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
         const int64_t t = min(t0 + 16 * i, most - 1), pos = count + t;  // (rows past the last repeat it)
-        x[i][0].raw.load(k + t * a.k_ts);
-        x[i][1].raw.load(v + t * a.v_ts);
+        x[i][0].load(k + t * a.k_ts);
+        x[i][1].load(v + t * a.v_ts);
         page[i] = pos < limit ? c.table[b * c.width + (pos >> c.page_log2)] : -1;
     }
 #pragma unroll
@@ -165,13 +173,17 @@ __global__ __launch_bounds__(256) void paged_write_kernel(PagedWrite a, PagedVie
 // ---- read -----------------------------------------------------------------
 
 // The inverse: rows [0, count) of every sequence as K/V rows of T; rows past a
-// count are cleared when `fill`, else left as they are.  Sixteen lanes a row;
-// bound by the rows written: 32768 tokens of 8 heads bf16 29 us (153 MB, 5.3
-// TB/s); fp32, a ragged batch of five up to 4701, 193 MB written, 33 (5.9).
+// count are cleared when `fill`, else left as they are.  Sixteen lanes a row,
+// each two pieces of 16 bytes: of 16-bit rows its eight dims of K and of V, of
+// fp32 rows four dims in either half, so that a store instruction fills whole
+// lines (32 bytes a lane instead left half of each line for the next one).
+// Bound by the rows written, which pass the caches by: a prompt of 32767 tokens
+// of 8 heads bf16, 64-dim groups, written and read back in turn with others,
+// 71.3 us against 80.5 with plain loads and stores; fp32 rows of 268 MB 45.6
+// against 73.1 (5.9 TB/s; 32 bytes a lane past the caches are slower than either).
 template <typename T, int G>
 __global__ __launch_bounds__(256) void paged_read_kernel(PagedRead a, PagedView c) {
-    constexpr int R = 128 / G;
-    const int lane = threadIdx.x & (kWave - 1);
+    constexpr int R = 128 / G, DIMS = 16 / sizeof(T), PIECES = sizeof(T) / 2;
     const int64_t t = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16;
     const int h = blockIdx.y, b = blockIdx.z;
     if (t >= a.rows) return;
@@ -179,22 +191,37 @@ __global__ __launch_bounds__(256) void paged_read_kernel(PagedRead a, PagedView 
     const int32_t page = t < count ? c.table[b * c.width + (t >> c.page_log2)] : -1;
     const bool live = static_cast<uint32_t>(page) < static_cast<uint32_t>(c.pages);
     if (!live && !a.fill && t >= count) return;
-    const int d = (lane & 15) * 8;
     const int64_t row =
         (((live ? static_cast<int64_t>(page) : 0) * c.kv_heads + h) << c.page_log2) + (t & ((1 << c.page_log2) - 1));
-    const uint32_t* codes = reinterpret_cast<const uint32_t*>(c.codes + row * kCodeRow);
+    const char* codes = c.codes + row * kCodeRow;
     const uint32_t* scales = c.scales + row * (2 * R);
     T* dst[2] = {static_cast<T*>(a.k), static_cast<T*>(a.v)};
-    const int64_t at = ((static_cast<int64_t>(b) * c.kv_heads + h) * a.rows + t) * 128 + d;
+    const int64_t at = ((static_cast<int64_t>(b) * c.kv_heads + h) * a.rows + t) * 128;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-        float x[8];
-        const uint32_t s = scales[R * w + d / G];
-        codes8(codes[16 * w + (lane & 15)], x);
-        const float low = f16_lo(s), delta = f16_hi(s);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = live ? fmaf(x[i], delta, low) : 0.0f;
-        store8<T>(dst[w] + at, x);
+        for (int piece = 0; piece < PIECES; ++piece) {
+            const int d = 128 / PIECES * piece + DIMS * (threadIdx.x & 15);
+            float x[DIMS];
+            const uint32_t s = scales[R * w + d / G];
+            const float low = f16_lo(s), delta = f16_hi(s);
+            if constexpr (sizeof(T) == 4) {
+                const uint32_t code = *reinterpret_cast<const uint16_t*>(codes + 64 * w + d / 2);
+#pragma unroll
+                for (int i = 0; i < DIMS; ++i) x[i] = static_cast<float>(code >> (4 * i) & 15u);
+            } else {
+                codes8(*reinterpret_cast<const uint32_t*>(codes + 64 * w + d / 2), x);
+            }
+#pragma unroll
+            for (int i = 0; i < DIMS; ++i) x[i] = live ? fmaf(x[i], delta, low) : 0.0f;
+            u32x4 out;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (sizeof(T) == 4) out[i] = __float_as_uint(x[i]);
+                else out[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+            }
+            store_once(dst[w] + at + d, out);
+        }
     }
 }
 
@@ -729,9 +756,12 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(PageCompact 
 
 // ---- the pages of a plan, and its table -----------------------------------
 
-// Copies the plan's pages in every layer, and lays the new table down in the
-// first workgroups.  Sources are live pages and targets pages nothing else
-// holds, so no workgroup reads what another writes.
+// Copies the plan's pages in every layer, 16 KB a workgroup at a time, and lays
+// the new table down in the first workgroups.  Sources are live pages and
+// targets pages nothing else holds, so no workgroup reads what another writes.
+// Bound by the copy: half of 640 pages of 16 layers, 206 MB read and written, 84
+// us with the plan (91 through the caches, a load at a time); units of 4 or 64 KB
+// cost a fork of 28 pages 3 and 2 us.
 __global__ __launch_bounds__(256) void move_pages_kernel(PageMoves m) {
     const int64_t step = int64_t{256} * gridDim.x, me = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     for (int64_t i = me; i < m.entries; i += step) {
@@ -751,10 +781,17 @@ __global__ __launch_bounds__(256) void move_pages_kernel(PageMoves m) {
         const int64_t off = (codes ? part : part - m.code_parts) * kMoveBytes;
         char* pool = codes ? m.codes : m.scales;
         const int64_t base = layer * m.pages * bytes + off;
-        const uint4* src = reinterpret_cast<const uint4*>(pool + base + pair.x * bytes);
-        uint4* dst = reinterpret_cast<uint4*>(pool + base + pair.y * bytes);
-        const int64_t n = min<int64_t>(kMoveBytes, bytes - off) / 16;
-        for (int64_t i = threadIdx.x; i < n; i += 256) dst[i] = src[i];
+        const u32x4* src = reinterpret_cast<const u32x4*>(pool + base + pair.x * bytes) + threadIdx.x;
+        u32x4* dst = reinterpret_cast<u32x4*>(pool + base + pair.y * bytes) + threadIdx.x;
+        const int n = static_cast<int>(min<int64_t>(kMoveBytes, bytes - off) / 16) - threadIdx.x;
+        constexpr int LOADS = kMoveBytes / (256 * 16);  // a thread's, all on their way before the first store
+        u32x4 x[LOADS];
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j)
+            if (256 * j < n) x[j] = load_once(src + 256 * j);
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j)
+            if (256 * j < n) store_once(dst + 256 * j, x[j]);
     }
 }
 
