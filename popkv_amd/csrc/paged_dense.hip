@@ -388,7 +388,7 @@ __device__ __forceinline__ void exchange_quarters(uint32_t (&d)[4]) {
 // c - 8 with low + 8 delta beside them, so that the two sums do not cancel: its
 // results are as far off as fp32 products of dequantised values, or less
 // (relative 1e-6 against 2e-6 at 20001 tokens).
-// 8 x 65536 tokens of 8 KV heads, 64-dim groups, 604 MB: bf16 114 us (5.3 TB/s,
+// 8 x 65536 tokens of 8 KV heads, 64-dim groups, 604 MB: bf16 108 us (5.6 TB/s,
 // as fast as memory streams), fp32 154 (bound by the vector instructions around
 // the products: two terms and exact values are twice bf16's).  A ragged batch of
 // five up to 20001 with 64 query heads, 32-dim groups, 77 MB: fp16 26.6 (a
@@ -433,6 +433,8 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
     // l's 16 bytes of load i are quarter (l % 8) ^ swz(token) of token 8 i + l /
     // 8, so that the reads below (16 tokens' equal quarters; four tokens' 64
     // bytes of V) meet 64 different banks.  swz(t) = 4 (t / 2 % 2) + t / 4 % 4.
+    // Codes pass the caches by (131071 tokens 33.9 us against 37.9, 4095 and a ragged
+    // batch whose pages stay in the last-level cache 1 % slower).
     struct Tile {
         uint4 k[2];
         uint32_t ks[2][R], v[8], vs[8];
@@ -466,10 +468,10 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
             "s_waitcnt lgkmcnt(0)\n\t"
             "s_mov_b32 m0, %0\n\t"
             "s_nop 1\n\t"
-            "global_load_lds_dwordx4 %1, %3\n\t"
-            "global_load_lds_dwordx4 %2, %3 offset:1024\n\t"
-            "global_load_lds_dwordx4 %1, %3 offset:2048\n\t"
-            "global_load_lds_dwordx4 %2, %3 offset:3072\n\t"
+            "global_load_lds_dwordx4 %1, %3 nt\n\t"
+            "global_load_lds_dwordx4 %2, %3 offset:1024 nt\n\t"
+            "global_load_lds_dwordx4 %1, %3 offset:2048 nt\n\t"
+            "global_load_lds_dwordx4 %2, %3 offset:3072 nt\n\t"
             "s_mov_b32 m0, %4\n\t"
             "s_nop 1\n\t"
             "global_load_lds_dwordx4 %5, %6"
