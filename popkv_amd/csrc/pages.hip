@@ -761,7 +761,9 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(PageCompact 
 // targets pages nothing else holds, so no workgroup reads what another writes.
 // Bound by the copy: half of 640 pages of 16 layers, 206 MB read and written, 84
 // us with the plan (91 through the caches, a load at a time); units of 4 or 64 KB
-// cost a fork of 28 pages 3 and 2 us.
+// cost a fork of 28 pages 3 and 2 us.  ONCE: pages pass the caches by, as a
+// compaction's do; a fork's few stay there (34 MB 8 us, 14 past the caches).
+template <bool ONCE>
 __global__ __launch_bounds__(256) void move_pages_kernel(PageMoves m) {
     const int64_t step = int64_t{256} * gridDim.x, me = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     for (int64_t i = me; i < m.entries; i += step) {
@@ -788,10 +790,13 @@ __global__ __launch_bounds__(256) void move_pages_kernel(PageMoves m) {
         u32x4 x[LOADS];
 #pragma unroll
         for (int j = 0; j < LOADS; ++j)
-            if (256 * j < n) x[j] = load_once(src + 256 * j);
+            if (256 * j < n) x[j] = ONCE ? load_once(src + 256 * j) : src[256 * j];
 #pragma unroll
         for (int j = 0; j < LOADS; ++j)
-            if (256 * j < n) store_once(dst + 256 * j, x[j]);
+            if (256 * j < n) {
+                if constexpr (ONCE) store_once(dst + 256 * j, x[j]);
+                else dst[256 * j] = x[j];
+            }
     }
 }
 
@@ -863,14 +868,15 @@ hipError_t launch_page_fork(const PageFork& a, const PageMoves& m, hipStream_t s
         hipLaunchKernelGGL(fork_rows_kernel, dim3(static_cast<unsigned>((a.batch + 3) / 4)), dim3(256), 0, s, a);
         hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
     }
-    hipLaunchKernelGGL(move_pages_kernel, dim3(blocks_for(a.batch * m.layers * m.parts, 1, 2048)), dim3(256), 0, s, m);
+    const unsigned grid = blocks_for(a.batch * m.layers * m.parts, 1, 2048);
+    hipLaunchKernelGGL(move_pages_kernel<false>, dim3(grid), dim3(256), 0, s, m);
     return hipGetLastError();
 }
 
 hipError_t launch_page_compact(const PageCompact& a, const PageMoves& m, hipStream_t s) {
     hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
     const unsigned grid = blocks_for(a.pages / 2 * m.layers * m.parts, 1, 2048);
-    hipLaunchKernelGGL(move_pages_kernel, dim3(grid), dim3(256), 0, s, m);
+    hipLaunchKernelGGL(move_pages_kernel<true>, dim3(grid), dim3(256), 0, s, m);
     return hipGetLastError();
 }
 
