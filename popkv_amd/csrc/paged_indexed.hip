@@ -176,16 +176,9 @@ struct PickFold<float> {
     __device__ __forceinline__ void join() { st.join(); }
 };
 
-constexpr int kPickWaves = 4;
-constexpr int kPickThreads = kPickWaves * kWave;
 constexpr int kPickRows = 8;                            // tokens an octet loads at once
 constexpr int kPickTile = kPickRows * kWave / 8;        // tokens of a wave's pass
-constexpr int kPickLeast = kPickWaves * kPickTile;
-// Workgroups in all, two a CU where the selections are long enough for a pass of
-// the workgroup each: four sequences of 2048 of 32767 tokens, 32 heads, 17.3 us
-// (one a CU 20 to 22, four the same), two of them 11.6 (12.3); one of 4096 13.1
-// (10.6 to 12.4, four 13.1); 64 heads of 1500 10.9 (11.9).
-constexpr int kPickBlocks = 512;
+constexpr int kPickBlocks = 256;                        // workgroups in all, one a CU
 constexpr int kPickState = kState + 1;                  // (m, l, acc[128], hits of the current token)
 
 // A row's query and its current token, for output dim threadIdx.x of waves 0
@@ -215,16 +208,16 @@ struct CurrentDim {
     }
 };
 
-// Merges a row's `n` states by the whole workgroup: the weights of 64 states at
-// a time by every wave alike, the sums by threads (dim, half of the states).
-template <typename T>
+// Merges a row's `n` states by the whole workgroup: the weights of 32 states at
+// a time by every wave alike, the sums by threads (dim, part of the states).
+template <typename T, int W>
 __device__ __forceinline__ void pick_merge(const float* ps, int n, const CurrentDim<T>& cur, T* out) {
-    constexpr int NF = 16;
+    constexpr int PARTS = W * kWave / 128, BURST = 32, NF = BURST / PARTS;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int d = threadIdx.x & 127, half = threadIdx.x >> 7;
+    const int d = threadIdx.x & 127, part = threadIdx.x >> 7;
     float m = -INFINITY, l = 0.0f, hits = 0.0f, a = 0.0f;
-    for (int s0 = 0; s0 < n; s0 += 2 * NF) {
-        const int k = min(2 * NF, n - s0);
+    for (int s0 = 0; s0 < n; s0 += BURST) {
+        const int k = min(BURST, n - s0);
         const float* p = ps + static_cast<int64_t>(s0) * kPickState;
         float x[NF], ms = -INFINITY, ls = 0.0f, hs = 0.0f;
         if (lane < k) {
@@ -234,9 +227,9 @@ __device__ __forceinline__ void pick_merge(const float* ps, int n, const Current
         }
 #pragma unroll
         for (int j0 = 0; j0 < NF; j0 += 4) {
-            if (2 * j0 >= k) break;
+            if (PARTS * j0 >= k) break;
 #pragma unroll
-            for (int j = j0; j < j0 + 4; ++j) x[j] = ld_f32<true>(p + min(2 * j + half, k - 1) * kPickState + 2 + d);
+            for (int j = j0; j < j0 + 4; ++j) x[j] = ld_f32<true>(p + min(PARTS * j + part, k - 1) * kPickState + 2 + d);
         }
         const float mx = fmaxf(m, wave_max(ms));
         const float f = state_weight(m, l, mx), w = state_weight(ms, ls, mx);
@@ -245,13 +238,18 @@ __device__ __forceinline__ void pick_merge(const float* ps, int n, const Current
         a *= f;
 #pragma unroll
         for (int j = 0; j < NF; ++j)
-            if (2 * j + half < k) a = fmaf(__shfl(w, 2 * j + half), x[j], a);
+            if (PARTS * j + part < k) a = fmaf(__shfl(w, PARTS * j + part), x[j], a);
         m = mx;
     }
-    __shared__ float s_sum[128];
-    if (half == 1) s_sum[d] = a;
+    __shared__ float s_sum[PARTS][128];
+    s_sum[part][d] = a;
     __syncthreads();
-    if (wave < 2) cur.finish(m, l, a + s_sum[d], hits, out);
+    if (wave < 2) {
+        float x = a;
+#pragma unroll
+        for (int i = 1; i < PARTS; ++i) x += s_sum[i][d];
+        cur.finish(m, l, x, hits, out);
+    }
 }
 
 // One workgroup a (split of the selection, query head, sequence): every query
@@ -260,10 +258,10 @@ __device__ __forceinline__ void pick_merge(const float* ps, int n, const Current
 // the next eight indices behind them.  The current token is counted, not read:
 // the merge folds it in as often as it was selected.  Bound by its chain of
 // reads (index, page table entry, token) and the hand-off of the splits: 4096 of
-// 32767 tokens for each of 32 heads, bf16, 64-dim groups, 20 MB: 13 us (1.5
+// 32767 tokens for each of 32 heads, bf16, 64-dim groups, 20 MB: 11.4 us (1.8
 // TB/s); 256 of them, without a hand-off, 6.4.
-template <typename T, int G, typename I>
-__global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend a, PagedIndexed ix, PagedView c,
+template <typename T, int G, typename I, int W>
+__global__ __launch_bounds__(W * kWave) void paged_indexed_kernel(PagedAttend a, PagedIndexed ix, PagedView c,
                                                                      int splits, int per) {
     constexpr int R = 128 / G;
     const int s = blockIdx.x, qh = blockIdx.y, b = blockIdx.z;
@@ -291,7 +289,7 @@ __global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend
         }
     };
     pick(e0 + wave * kPickTile);
-    for (int64_t e = e0 + wave * kPickTile; e < e1; e += kPickLeast) {
+    for (int64_t e = e0 + wave * kPickTile; e < e1; e += W * kPickTile) {
         Row4 r[2][4];
         bool live[2][4];
         int32_t page[kPickRows];
@@ -318,7 +316,7 @@ __global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend
                 x.vs = sc[R];
             }
         }
-        pick(e + kPickLeast);  // the next pass's, on their way while this one's rows are
+        pick(e + W * kPickTile);  // the next pass's, on their way while this one's rows are
         f.fold(r[0], live[0]);
         f.fold(r[1], live[1]);
     }
@@ -328,7 +326,7 @@ __global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend
              static_cast<const T*>(a.cur_v) + kv);
     f.join();
     const float wave_hits = wave_sum(static_cast<float>(hits)) * 0.125f;  // the eight lanes of an octet count alike
-    __shared__ float s_m[kPickWaves], s_l[kPickWaves], s_hits[kPickWaves], s_acc[kPickWaves][128];
+    __shared__ float s_m[W], s_l[W], s_hits[W], s_acc[W][128];
     if (lane < 8) {
 #pragma unroll
         for (int d = 0; d < 16; ++d) s_acc[wave][d0 + d] = f.st.acc[d];
@@ -344,9 +342,9 @@ __global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend
     if (wave < 2) {
         float mx = -INFINITY, l = 0.0f, x = 0.0f, n = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kPickWaves; ++w) mx = fmaxf(mx, s_m[w]);
+        for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_m[w]);
 #pragma unroll
-        for (int w = 0; w < kPickWaves; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float g = state_weight(s_m[w], s_l[w], mx);
             x = fmaf(g, s_acc[w][threadIdx.x], x);
             l = fmaf(g, s_l[w], l);
@@ -366,31 +364,45 @@ __global__ __launch_bounds__(kPickThreads) void paged_indexed_kernel(PagedAttend
     if (splits == 1) return;
     __shared__ uint32_t s_last;
     if (!last_of(a.tickets + row, splits, &s_last)) return;
-    pick_merge<T>(a.partials + row * splits * kPickState, splits, cur, out);
+    pick_merge<T, W>(a.partials + row * splits * kPickState, splits, cur, out);
 }
 
+// Waves a workgroup, and the splits of a row's selection into `per` tokens each.
+// Four waves where that leaves no more than a pass to each of one workgroup a CU
+// (more CUs share the gathers: 1024 of 32767 tokens for 32 heads 8.7 us, by eight
+// 10.2; 1001 for 48 rows fp32 9.2 and 11.4) and where there are more rows than
+// CUs (several workgroups on each: 512 rows of 1000 24.4 and 27.4); else eight, a
+// workgroup a CU and half as many states (4096 for 32 heads 11.4, by four 13.1;
+// 256 rows of 1024 14.9 and 17.2, of 500 9.0 and 11.4; four sequences of 2048 for
+// 32 heads 16.9 and 17.1).
 struct PickPlan {
-    int splits, per;
+    int waves, splits, per;
 };
 PickPlan pick_plan(int64_t rows, int64_t selected) {
+    const int64_t passes = rows * ((selected + 4 * kPickTile - 1) / (4 * kPickTile));
+    const int waves = rows <= kPickBlocks && passes > kPickBlocks ? 8 : 4;
+    const int64_t least = waves * kPickTile, most = (selected + least - 1) / least;
     int64_t want = kPickBlocks / rows;
-    const int64_t most = (selected + kPickLeast - 1) / kPickLeast;
     if (want > most) want = most;
     if (want < 1) want = 1;
-    const int64_t per = ((selected + want - 1) / want + kPickLeast - 1) / kPickLeast * kPickLeast;
-    return {static_cast<int>((selected + per - 1) / per), static_cast<int>(per)};
+    const int64_t per = ((selected + want - 1) / want + least - 1) / least * least;
+    return {waves, static_cast<int>((selected + per - 1) / per), static_cast<int>(per)};
 }
 
 template <typename T, int G>
 hipError_t launch_indexed_t(const PagedAttend& a, const PagedIndexed& ix, const PagedView& c, hipStream_t stream) {
     const PickPlan p = pick_plan(static_cast<int64_t>(c.batch) * a.q_heads, ix.selected);
     const dim3 grid(static_cast<unsigned>(p.splits), static_cast<unsigned>(a.q_heads), static_cast<unsigned>(c.batch));
-    if (ix.index_dtype == POPKV_INDEX_I32)
-        hipLaunchKernelGGL((paged_indexed_kernel<T, G, int32_t>), grid, dim3(kPickThreads), 0, stream, a, ix, c,
-                           p.splits, p.per);
-    else
-        hipLaunchKernelGGL((paged_indexed_kernel<T, G, int64_t>), grid, dim3(kPickThreads), 0, stream, a, ix, c,
-                           p.splits, p.per);
+#define POPKV_PICK(I, W) \
+    hipLaunchKernelGGL((paged_indexed_kernel<T, G, I, W>), grid, dim3(W * kWave), 0, stream, a, ix, c, p.splits, p.per)
+    if (ix.index_dtype == POPKV_INDEX_I32) {
+        if (p.waves == 8) POPKV_PICK(int32_t, 8);
+        else POPKV_PICK(int32_t, 4);
+    } else {
+        if (p.waves == 8) POPKV_PICK(int64_t, 8);
+        else POPKV_PICK(int64_t, 4);
+    }
+#undef POPKV_PICK
     return hipGetLastError();
 }
 

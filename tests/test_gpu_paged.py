@@ -460,7 +460,8 @@ def test_counts_past_the_launch_bound(dtype):
 @pytest.mark.parametrize("index", (torch.int64, torch.int32))
 @pytest.mark.parametrize("lengths,selected,kv_heads,group", [([700, 33, 0], 1, 2, 4), ([700, 33, 0], 129, 2, 4),
                                                              ([1000], 900, 1, 3), ([64] * 5, 64, 3, 1),
-                                                             ([5000, 4000], 2500, 2, 8)])
+                                                             ([5000, 4000], 2500, 2, 8),
+                                                             ([300, 0, 90, 400, 33] * 2, 400, 4, 4)])
 def test_indexed_attention(dtype, index, lengths, selected, kv_heads, group):
     """Selections with padding, masked entries, repeats, the current token
     never, once and twice, numbers outside the sequence, and rows that keep
