@@ -114,8 +114,8 @@ struct DenseWalk {
         load();
         int total = __builtin_amdgcn_readlane(incl(), kWave - 1);
         for (int b = kWave; b < c.batch; b += kWave) {
-            const uint32_t n = wave_incl_scan(static_cast<uint32_t>(cost(b + lane, tiles_of(count_of(b + lane)))), lane);
-            total += __builtin_amdgcn_readlane(static_cast<int>(n), kWave - 1);
+            const uint32_t n = static_cast<uint32_t>(cost(b + lane, tiles_of(count_of(b + lane))));
+            total += __builtin_amdgcn_readlane(static_cast<int>(wave_incl_scan(n, lane)), kWave - 1);
         }
         total -= kSequenceCost;
         per = max(div_nonneg(total + groups - 1, groups), kDenseWaves);
@@ -544,7 +544,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
         start_part();
         f32x4_t acc[8], low_acc = {0.0f, 0.0f, 0.0f, 0.0f};
         float ref[4], l[4];  // rows 4 grp + i: weights are 2^(logit - ref)
-        // the queries in fp16, the largest magnitude of a head in [1/2, 1)
+        // the queries in fp16, the largest magnitude of a head in [1/2, 1) 2^QTOP
         uint32_t qa[QSETS][4][4], ql[LOWS][4];
         float factor[4];  // of rows 4 grp + i
         {
@@ -611,7 +611,8 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
                 if (g < R) {
                     f32x4_t z = {0.0f, 0.0f, 0.0f, 0.0f};
                     if constexpr (F32) z[0] = -8.0f * qs[g % R];
-                    else if constexpr (R == 2) z = mfma_f16(none, qa[0][2 * g % 4 + 1], mfma_f16(none, qa[0][2 * g % 4], z));
+                    else if constexpr (R == 2)
+                        z = mfma_f16(none, qa[0][2 * g % 4 + 1], mfma_f16(none, qa[0][2 * g % 4], z));
                     else z = mfma_f16(none, qa[g % HALVES][g / HALVES % 4], z);
                     // (rows of codes times columns of queries: every element of column `col` is head `col`'s)
                     const float term = grp == 0 ? qs[g % R] : -z[0];
@@ -659,7 +660,8 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
                             uint32_t x[4];
 #pragma unroll
                             for (int i = 0; i < 4; ++i) x[i] = HALVES == 2 ? cb[i] & half_mask[n] : cb[i];
-                            dot[R == 2 ? st / 2 : HALVES * st + n] = mfma_f16(qa[0][st], x, mfma_f16(qa[1][st], x, sum));
+                            sum = mfma_f16(qa[0][st], x, mfma_f16(qa[1][st], x, sum));
+                            dot[R == 2 ? st / 2 : HALVES * st + n] = sum;
                         }
                         continue;
                     }

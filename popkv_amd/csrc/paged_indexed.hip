@@ -229,7 +229,8 @@ __device__ __forceinline__ void pick_merge(const float* ps, int n, const Current
         for (int j0 = 0; j0 < NF; j0 += 4) {
             if (PARTS * j0 >= k) break;
 #pragma unroll
-            for (int j = j0; j < j0 + 4; ++j) x[j] = ld_f32<true>(p + min(PARTS * j + part, k - 1) * kPickState + 2 + d);
+            for (int j = j0; j < j0 + 4; ++j)
+                x[j] = ld_f32<true>(p + min(PARTS * j + part, k - 1) * kPickState + 2 + d);
         }
         const float mx = fmaxf(m, wave_max(ms));
         const float f = state_weight(m, l, mx), w = state_weight(ms, ls, mx);

@@ -169,7 +169,8 @@ def _check_cache(cache: PagedKVCache, pages: PageTable, layer: int = 0) -> tuple
     if g != 16 and g != 32 and g != 64:
         raise ValueError("dim_group_size must be one of 16, 32, 64")
     shape = codes.shape
-    if len(shape) != 6 or codes.dtype is not torch.uint8 or shape[4] != 2 or shape[5] != 64 or not codes.is_contiguous():
+    if len(shape) != 6 or codes.dtype is not torch.uint8 or shape[4] != 2 or shape[5] != 64 \
+            or not codes.is_contiguous():
         raise ValueError("codes must be a contiguous uint8 [layers, pages, KV heads, page tokens, 2, 64]")
     layers, held, kv_heads, page_tokens, _, _ = shape
     want = (layers, held, kv_heads, page_tokens, 2, 128 // g, 2)
@@ -463,9 +464,10 @@ def fork_sequences(cache: PagedKVCache, pages: PageTable, parents: torch.Tensor,
     nbytes = _workspace_bytes("popkv_page_fork", batch, width)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with nat.on_device(dev):
-        nat.call("popkv_page_fork", pool[0], pool[1], cache.codes.shape[0], pool[2], kv_heads, pool[4], pool[5], pool[6],
-                 pool[8], pages.refs.data_ptr(), new.table.data_ptr(), new.counts.data_ptr(), new.refs.data_ptr(), width,
-                 batch, parents.data_ptr(), nat.ptr(status), ws.data_ptr(), nbytes, nat.stream_of(dev))
+        nat.call("popkv_page_fork", pool[0], pool[1], cache.codes.shape[0], pool[2], kv_heads, pool[4], pool[5],
+                 pool[6], pool[8], pages.refs.data_ptr(), new.table.data_ptr(), new.counts.data_ptr(),
+                 new.refs.data_ptr(), width, batch, parents.data_ptr(), nat.ptr(status), ws.data_ptr(), nbytes,
+                 nat.stream_of(dev))
     return new
 
 
