@@ -115,58 +115,45 @@ __device__ __forceinline__ void quantise8(const Eight<T>& in, uint32_t& code, ui
     code = bad ? 0u : static_cast<uint32_t>(even) | (static_cast<uint32_t>(odd) << 16);
 }
 
-// Sixteen lanes a row (eight dims each), NT rows of K and V a lane, all loaded
-// before the first is encoded: the K and the V row of a token make one 128-byte
-// line of codes.  Bound by the stream of the rows, 2 * 128 * sizeof(T) bytes
-// read and 128 + 8R written per token and head: 32767 tokens of 8 heads bf16,
-// 64-dim groups, 172 MB in 33.5 us (5.1 TB/s); with one row a lane and the codes
-// by way of fp64 divisions and fp32 reciprocals by division 41.1, four rows 34.6,
-// eight 40.6.
-template <typename T>
-constexpr int kWriteRows = sizeof(T) == 4 ? 1 : 2;
+// Sixteen lanes a row, eight dims of its K and of its V each: the K and the V
+// row of a token make one 128-byte line of codes.  Bound by the stream of the
+// rows, 2 * 128 * sizeof(T) bytes read, which pass the caches by, and 128 + 8R
+// written per token and head: 32768 tokens of 8 heads bf16, 64-dim groups, 172 MB
+// in 35 us (4.9 TB/s), fp32 with 32-dim groups 310 MB in 61 (5.1); two rows a lane
+// 35 and 61, at 8192 tokens 13.2 and 16.8 against 12.0 and 16.3.
 template <typename T, int G>
 __global__ __launch_bounds__(256) void paged_write_kernel(PagedWrite a, PagedView c) {
-    constexpr int R = 128 / G, NT = kWriteRows<T>;
+    constexpr int R = 128 / G;
     const int lane16 = threadIdx.x & 15;
-    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (16 * NT) + threadIdx.x / 16;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16;
     const int h = blockIdx.y, b = blockIdx.z;
     const int64_t most = a.tokens ? clamp_count(a.tokens[b], a.rows) : a.rows;
-    if (static_cast<int64_t>(blockIdx.x) * (16 * NT) >= most) return;
+    if (static_cast<int64_t>(blockIdx.x) * 16 >= most) return;
     const int64_t limit = c.width << c.page_log2;
-    const int64_t count = clamp_count(c.counts[b], limit);
+    const int64_t pos = clamp_count(c.counts[b], limit) + t;
     const int d = lane16 * 8;
-    const T* k = static_cast<const T*>(a.k) + b * a.k_bs + h * a.k_hs + d;
-    const T* v = static_cast<const T*>(a.v) + b * a.v_bs + h * a.v_hs + d;
-    Eight<T> x[NT][2];
-    int32_t page[NT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        const int64_t t = min(t0 + 16 * i, most - 1), pos = count + t;  // (rows past the last repeat it)
-        x[i][0].load(k + t * a.k_ts);
-        x[i][1].load(v + t * a.v_ts);
-        page[i] = pos < limit ? c.table[b * c.width + (pos >> c.page_log2)] : -1;
-    }
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        const int64_t t = t0 + 16 * i, pos = count + t;
-        const bool live = t < most, there = static_cast<uint32_t>(page[i]) < static_cast<uint32_t>(c.pages);
-        uint32_t code[2], scale[2];
-        quantise8<T, G / 8>(x[i][0], code[0], scale[0]);
-        quantise8<T, G / 8>(x[i][1], code[1], scale[1]);
-        if (live && there) {
-            const int64_t row =
-                ((static_cast<int64_t>(page[i]) * c.kv_heads + h) << c.page_log2) + (pos & ((1 << c.page_log2) - 1));
-            uint32_t* codes = reinterpret_cast<uint32_t*>(c.codes + row * kCodeRow);
-            uint32_t* scales = c.scales + row * (2 * R);
-            codes[lane16] = code[0];
-            codes[16 + lane16] = code[1];
-            if (d % G == 0) {
-                scales[d / G] = scale[0];
-                scales[R + d / G] = scale[1];
-            }
-        } else if (live && a.status && lane16 == 0 && h == 0) {
-            atomicOr(a.status, pos < limit ? kStatusNoPage : kStatusFull);
+    const int64_t from = min(t, most - 1);  // (rows past the last repeat it)
+    Eight<T> k, v;
+    k.load(static_cast<const T*>(a.k) + b * a.k_bs + h * a.k_hs + from * a.k_ts + d);
+    v.load(static_cast<const T*>(a.v) + b * a.v_bs + h * a.v_hs + from * a.v_ts + d);
+    const int32_t page = pos < limit ? c.table[b * c.width + (pos >> c.page_log2)] : -1;
+    uint32_t code[2], scale[2];
+    quantise8<T, G / 8>(k, code[0], scale[0]);
+    quantise8<T, G / 8>(v, code[1], scale[1]);
+    if (t >= most) return;
+    if (static_cast<uint32_t>(page) < static_cast<uint32_t>(c.pages)) {
+        const int64_t row =
+            ((static_cast<int64_t>(page) * c.kv_heads + h) << c.page_log2) + (pos & ((1 << c.page_log2) - 1));
+        uint32_t* codes = reinterpret_cast<uint32_t*>(c.codes + row * kCodeRow);
+        uint32_t* scales = c.scales + row * (2 * R);
+        codes[lane16] = code[0];
+        codes[16 + lane16] = code[1];
+        if (d % G == 0) {
+            scales[d / G] = scale[0];
+            scales[R + d / G] = scale[1];
         }
+    } else if (a.status && lane16 == 0 && h == 0) {
+        atomicOr(a.status, pos < limit ? kStatusNoPage : kStatusFull);
     }
 }
 
@@ -827,8 +814,7 @@ hipError_t copy_words(const void* src, void* dst, int64_t n, hipStream_t s) {
     }
 
 hipError_t launch_paged_write(const PagedWrite& a, const PagedView& c, int dtype, int dim_group, hipStream_t stream) {
-    const int per = 16 * (dtype == POPKV_DTYPE_F32 ? kWriteRows<float> : kWriteRows<bf16_t>);
-    const dim3 grid(static_cast<unsigned>((a.rows + per - 1) / per), static_cast<unsigned>(c.kv_heads),
+    const dim3 grid(static_cast<unsigned>((a.rows + 15) / 16), static_cast<unsigned>(c.kv_heads),
                     static_cast<unsigned>(c.batch));
     POPKV_PAGED_T(paged_write_kernel)
     return hipGetLastError();
