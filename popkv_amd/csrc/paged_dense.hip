@@ -368,8 +368,8 @@ __device__ __forceinline__ void exchange_quarters(uint32_t (&d)[4]) {
 //   S = sum_g delta_g dot_g + sum_g low_g qsum_g   in fp32, the second sum by
 //                                    one more product (qsum in two fp16 terms)
 //   O[head, dim] += P . V            V as low + c delta in fp16 (bf16 tensors), or
-//                                    exactly, in three parts: low, and c times
-//                                    delta's upper seven and lower four bits
+//                                    exactly, in parts: low, 8 delta, and c - 8
+//                                    times delta's upper seven and lower four bits
 // so keys enter the logits exactly: with the outlier channels that keys have,
 // their rounding to fp16 was four times fp16's own in the result.  (C layout:
 // lane l holds rows 4 (l / 16) .. + 3 of column l % 16; A and B: lane l holds
@@ -775,23 +775,22 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
                     for (int i = 0; i < 4; ++i) acc[4 * half + i] = mfma_f16(pa[0], vf[i], acc[4 * half + i]);
                 }
             } else {
-                // exactly: delta in two parts of at most seven and four bits, whose
-                // products with a code fit fp16, and the lows by themselves (the
-                // same sum for each of a lane's dims)
+                // exactly: codes as c - 8, times delta in two parts of at most seven
+                // and four bits (products that fp16 holds, as deltas reach 7646 and
+                // 15 times one may pass fp16's largest number), and low and 8 delta
+                // by themselves (the same sums for each of a lane's dims)
                 uint32_t lows[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) lows[j] = low_halves(x.vs[2 * j], x.vs[2 * j + 1]);
 #pragma unroll
                 for (int n = 0; n < TERMS; ++n) low_acc = mfma_f16(pa[n], lows, low_acc);
-                if constexpr (F32) {
-                    uint32_t eights[4];
+                uint32_t eights[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        eights[j] = __builtin_bit_cast(
-                            uint32_t, as_half2(high_halves(x.vs[2 * j], x.vs[2 * j + 1])) * half2_t{8.0f16, 8.0f16});
+                for (int j = 0; j < 4; ++j)
+                    eights[j] = __builtin_bit_cast(
+                        uint32_t, as_half2(high_halves(x.vs[2 * j], x.vs[2 * j + 1])) * half2_t{8.0f16, 8.0f16});
 #pragma unroll
-                    for (int n = 0; n < TERMS; ++n) low_acc = mfma_f16(pa[n], eights, low_acc);
-                }
+                for (int n = 0; n < TERMS; ++n) low_acc = mfma_f16(pa[n], eights, low_acc);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     uint32_t vh[4][4], vl[4][4];
@@ -801,8 +800,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
                         const half2_t delta = as_half2(high_halves(x.vs[2 * j], x.vs[2 * j + 1]));
                         const half2_t top7 = as_half2(__builtin_bit_cast(uint32_t, delta) & 0xfff0fff0u);
                         half2_t code[4];
-                        if constexpr (F32) centred_pairs(bits, half ? high_halves(v0, v1) : low_halves(v0, v1), code);
-                        else code_pairs(bits, half ? high_halves(v0, v1) : low_halves(v0, v1), code);
+                        centred_pairs(bits, half ? high_halves(v0, v1) : low_halves(v0, v1), code);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             vh[i][j] = __builtin_bit_cast(uint32_t, code[i] * top7);

@@ -1049,3 +1049,49 @@ def test_a_retrieval_step_over_the_pages():
     want = attend(q[None], dequantised(keys, 32)[None], dequantised(vals, 32)[None], ck[None], cv[None], [tokens],
                   [[row.tolist() for row in idx.cpu()]])
     assert ((got.cpu().double() - want).abs() <= ULP[torch.bfloat16] * want.abs() + FP32).all()
+
+
+# ---------------------------------------------------------------- wide value groups
+
+def wide_values(limit, dtype, gen, tokens, every):
+    """V rows [1, 2, tokens, 128]; every `every`-th token's groups span +-limit."""
+    v = torch.randn(1, 2, tokens, 128, generator=gen)
+    wide = (torch.rand(1, 2, tokens, 128, generator=gen) * 2 - 1) * limit
+    wide[..., 0::16], wide[..., 1::16] = -limit, limit
+    far = torch.arange(tokens) % every == every - 1
+    return torch.where(far[:, None], wide, v).to(dtype), far
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group", (16, 32, 64))
+@pytest.mark.parametrize("limit", (34000.0, 57344.0))
+@pytest.mark.parametrize("weights", ("all", "none"))
+def test_attention_over_wide_value_groups(dtype, group, limit, weights):
+    """Value groups up to the format's whole range (15 delta past fp16's largest
+    number), in tokens that count like any other and in tokens whose weight is
+    2^-40 and less, which change nothing."""
+    gen = torch.Generator().manual_seed(50 + group)
+    cache, table = make([300], 2, group=group)
+    v, far = wide_values(limit, dtype, gen, 300, 1 if weights == "all" else 9)
+    base = torch.randn(128, generator=gen)
+    k = torch.randn(1, 2, 300, 128, generator=gen)
+    if weights == "none":  # logits below -30
+        k[:, :, far] = -4 * base
+    k = k.to(dtype)
+    paged.write_tokens(cache, 0, table, k.to(DEV), v.to(DEV))
+    table.advance(300)
+    k, v = dequantised(k, group), dequantised(v, group)
+    q = (base + 0.1 * torch.randn(1, 8, 128, generator=gen)).to(dtype).to(DEV)
+    ck, cv = (torch.randn(1, 2, 128, generator=gen).to(dtype).to(DEV) for _ in range(2))
+    want = attend(q, k, v, ck, cv, [300])
+    # the output's rounding; the fp32 work (FP32 is that of values up to about
+    # 5); the wide tokens' own weights, below 2^-40 of 57344 each; and for the
+    # dense bf16 form V and the weights in fp16, half a step of the largest each
+    top = v.abs().max() if weights == "all" else v[:, :, ~far].abs().max()
+    bound = ULP[dtype] * want.abs() + FP32 * top / 5 + 300 * 57344 * 2.0 ** -40
+    half = bound + (2 * 2.0 ** -11 * top if dtype == torch.bfloat16 else 0)
+    got = paged.paged_attention_step(q, cache, 0, table, ck, cv).cpu().double()
+    assert ((got - want).abs() <= half).all(), float((got - want).abs().max())
+    idx = torch.arange(301, device=DEV).expand(1, 8, 301).contiguous()
+    got = paged.paged_indexed_attention(q, cache, 0, table, ck, cv, idx, torch.arange(8, device=DEV) // 4)
+    assert ((got.cpu().double() - want).abs() <= bound).all(), float((got.cpu().double() - want).abs().max())
