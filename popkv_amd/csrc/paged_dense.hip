@@ -363,40 +363,46 @@ __device__ __forceinline__ void exchange_quarters(uint32_t (&d)[4]) {
 // One workgroup a (share, KV head) for the whole group: its query heads are the
 // 16 rows of matrix products (those past the group zero), so any group of 1 to
 // 16 costs the same.  A wave takes tiles of 32 tokens, two of 16 for the logits:
-//   dot_g[head, token] = q . c       one 16 x 16 x 32 step per 32 dims, codes as
-//                                    they are, each scale group by itself
-//   S = sum_g delta_g dot_g + sum_g low_g qsum_g   in fp32, the second sum by
-//                                    one more product (qsum in two fp16 terms)
+//   dot_g[head, token] = q . (c - 8)   one 16 x 16 x 32 step per 32 dims, each
+//                                    scale group by itself
+//   S = sum_g delta_g dot_g + sum_g (low_g + 8 delta_g) qsum_g   in fp32, the
+//                                    second sum by one more product (qsum in two
+//                                    fp16 terms)
 //   O[head, dim] += P . V            V as low + c delta in fp16 (bf16 tensors), or
 //                                    exactly, in parts: low, 8 delta, and c - 8
 //                                    times delta's upper seven and lower four bits
-// so keys enter the logits exactly: with the outlier channels that keys have,
-// their rounding to fp16 was four times fp16's own in the result.  (C layout:
-// lane l holds rows 4 (l / 16) .. + 3 of column l % 16; A and B: lane l holds
-// k-elements 8 (l / 16) .. + 7 of row / column l % 16.)
+// so keys enter the logits unrounded: with the outlier channels that keys have,
+// their rounding to fp16 was four times fp16's own in the result.  Codes are taken
+// from their middle because the two sums must not cancel more than the keys do:
+// with 1024 + c, the bits as they come, sum(q) a thousandfold went through the
+// fp32 sums, and results of queries of one sign were 1.5 to 2.6 times as far off
+// as fp16's own rounding (now 1.00 of it; 5 % of bf16's time at 8 x 65535, 4 of
+// fp16's).  (C layout: lane l holds rows 4 (l / 16) .. + 3 of column l % 16; A and
+// B: lane l holds k-elements 8 (l / 16) .. + 7 of row / column l % 16.)
 // A code becomes fp16 by its bits: 0x6400 | c is 1024 + c, and 0x6400 | 16 c
-// is 1024 + 16 c.  For the keys the queries of odd dims are divided by 16, and
-// what codes of zero would give, times delta, is taken off in that same extra
-// product, so a dword of eight costs five instructions; for the values a packed
-// subtraction and a packed fma follow (13).  A token's 16-byte quarters are
-// exchanged among the four lane groups (lane swaps), so that a step's 32 dims
-// are one group's.
-// Queries are scaled by a power of two per head (bf16 reaches past fp16, and
-// 1024 times a group's sum must not), and the weights are kept around 2^8, where
-// fp16 keeps 11 bits; fp16 and fp32 take a second term for the rest of each
-// weight (22 bits).  fp32 takes two terms of the queries as well, and codes
-// c - 8 with low + 8 delta beside them, so that the two sums do not cancel: its
-// results are as far off as fp32 products of dequantised values, or less
-// (relative 1e-6 against 2e-6 at 20001 tokens).
-// 8 x 65536 tokens of 8 KV heads, 64-dim groups, 604 MB: bf16 108 us (5.6 TB/s,
-// as fast as memory streams), fp32 154 (bound by the vector instructions around
-// the products: two terms and exact values are twice bf16's).  A ragged batch of
-// five up to 20001 with 64 query heads, 32-dim groups, 77 MB: fp16 26.6 (a
-// twenty-fifth less with values rounded to fp16), fp32 30.7 (94 by fp32 vector
-// products).  4095 tokens, 5 MB, 10.9: a chain of reads, one tile a wave, the
-// hand-off.  (What the queries' fp16 terms round: 16-bit queries are exact down to
-// 2^-9 of the head's largest and off by at most 2^-20 of it below; fp32 ones by
-// 2^-24 of themselves or 2^-29 of the largest.)
+// is 1024 + 16 c; a packed subtraction, or an fma by 1/16, leaves c - 8 (nine
+// instructions a dword of eight).  A token's 16-byte quarters are exchanged among
+// the four lane groups (lane swaps), so that a step's 32 dims are one group's.
+// What is held in fewer bits than fp32:
+//   queries: scaled by a power of two per head, 16-bit ones exact down to 2^-18
+//     (fp16) and 2^-21 (bf16) of the head's largest, fp32 ones two terms, off by at
+//     most 2^-23 of themselves; below that any by 2^-29 of the largest.
+//   weights: kept around 2^8, where fp16 keeps 11 bits, a second term for the
+//     rest (22 bits) with fp16 and fp32 tensors.  bf16 ones have no such term and V
+//     rounded to fp16: each off by at most half a step, 2^-11 of it, an eighth of
+//     what the result's own rounding may be.  Both exact, as for fp16, 8 x 65535
+//     took 140 us against 112 and the ragged batch 27.9 against 24.1, for a norm of
+//     the error of 1.634e-3 of the result's instead of 1.652e-3.
+// fp32 results are as far off as fp32 products of dequantised values, or less,
+// where queries have no mean (relative 1.0e-6 against 2.1e-6 at 20001 tokens), and
+// two to three times as far where they have one sign (3.1e-6 against 2.0e-6, at
+// 64-dim groups 5.2e-6 and 1.7e-6): the two sums of S then cancel.
+// 8 x 65536 tokens of 8 KV heads, 64-dim groups, 604 MB: bf16 112 us (5.4 TB/s;
+// such a stream is read in 97 by itself), fp16 138, fp32 154: bound by the vector
+// instructions around the products.  A ragged batch of five up to 20001 with 64
+// query heads, 32-dim groups, 77 MB: bf16 24.1, fp16 27.8, fp32 30 (94 by fp32
+// vector products).  4095 tokens, 5 MB, 10.9: a chain of reads, one tile a wave,
+// the hand-off.
 template <typename T, int G>
 __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend a, PagedView c, int64_t max_tokens,
                                                                          int groups) {
@@ -409,7 +415,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
     constexpr int QSETS = F32 ? 2 : HALVES;
     constexpr int LOWS = R == 8 ? 2 : 1;          // products for the low terms (four groups each)
     constexpr int TERMS = std::is_same_v<T, bf16_t> ? 1 : 2;
-    constexpr int QTOP = F32 ? 5 : 0;             // queries lie below 2^QTOP
+    constexpr int QTOP = 5;                       // queries lie below 2^QTOP
     constexpr float kBase = 8.0f, kTop = 15.0f;   // weights start at 2^8 and may grow to 2^15
     constexpr float kNone = -3e38f;               // no weight yet
     constexpr int W = kDenseWaves, ROWS = 8, PITCH = 132;
@@ -570,7 +576,6 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
                 for (int i = 0; i < 8; ++i) {
                     q[s][i] = ldexpf(q[s][i], QTOP - 1 - e);
                     sum[s] += q[s][i];
-                    if (!F32 && (i & 1)) q[s][i] *= 0.0625f;
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -589,8 +594,8 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
                 sum[s] += lane_xor<16>(sum[s]);
             }
             // the low terms' product: lane group 0 holds the groups' sums of queries
-            // for low, lane group 1 minus their products with codes of zero (fp32:
-            // of c = -8) for delta, each as (high, rest)
+            // for low, lane group 1 eight times them for delta (what codes lack in c
+            // - 8), each as (high, rest)
             float qs[R];
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
@@ -604,18 +609,11 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
                     qs[s / 2] = s & 1 ? qs[s / 2] + (sum[s] + other) : sum[s] + other;
                 }
             }
-            const uint32_t none[4] = {0x64006400u, 0x64006400u, 0x64006400u, 0x64006400u};
 #pragma unroll
             for (int g = 0; g < 4 * LOWS; ++g) {
                 uint32_t x = 0;
                 if (g < R) {
-                    f32x4_t z = {0.0f, 0.0f, 0.0f, 0.0f};
-                    if constexpr (F32) z[0] = -8.0f * qs[g % R];
-                    else if constexpr (R == 2)
-                        z = mfma_f16(none, qa[0][2 * g % 4 + 1], mfma_f16(none, qa[0][2 * g % 4], z));
-                    else z = mfma_f16(none, qa[g % HALVES][g / HALVES % 4], z);
-                    // (rows of codes times columns of queries: every element of column `col` is head `col`'s)
-                    const float term = grp == 0 ? qs[g % R] : -z[0];
+                    const float term = grp == 0 ? qs[g % R] : 8.0f * qs[g % R];
                     const float high = static_cast<float>(static_cast<_Float16>(term));
                     x = pack_half2(high, term - high);
                 }
@@ -648,30 +646,23 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
 #pragma unroll
                 for (int st = 0; st < 4; ++st) {
                     uint32_t cb[4];
-                    if constexpr (F32) {
-                        half2_t code[4];
-                        centred_pairs(bits, w[st], code);
+                    half2_t code[4];
+                    centred_pairs(bits, w[st], code);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) cb[i] = __builtin_bit_cast(uint32_t, code[i]);
+                    for (int i = 0; i < 4; ++i) cb[i] = __builtin_bit_cast(uint32_t, code[i]);
 #pragma unroll
-                        for (int n = 0; n < HALVES; ++n) {
-                            f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
-                            if (R == 2 && (st & 1)) sum = dot[st / 2];
+                    for (int n = 0; n < HALVES; ++n) {
+                        f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+                        if (R == 2 && (st & 1)) sum = dot[st / 2];
+                        if constexpr (F32) {
                             uint32_t x[4];
 #pragma unroll
                             for (int i = 0; i < 4; ++i) x[i] = HALVES == 2 ? cb[i] & half_mask[n] : cb[i];
                             sum = mfma_f16(qa[0][st], x, mfma_f16(qa[1][st], x, sum));
-                            dot[R == 2 ? st / 2 : HALVES * st + n] = sum;
+                        } else {
+                            sum = mfma_f16(qa[n][st], cb, sum);
                         }
-                        continue;
-                    }
-                    biased_pairs(bits, w[st], cb);
-                    if constexpr (R == 2) {
-                        dot[st / 2] = mfma_f16(qa[0][st], cb, st & 1 ? dot[st / 2] : f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
-                    } else {
-#pragma unroll
-                        for (int n = 0; n < HALVES; ++n)
-                            dot[HALVES * st + n] = mfma_f16(qa[n][st], cb, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
+                        dot[R == 2 ? st / 2 : HALVES * st + n] = sum;
                     }
                 }
 #pragma unroll

@@ -1095,3 +1095,70 @@ def test_attention_over_wide_value_groups(dtype, group, limit, weights):
     idx = torch.arange(301, device=DEV).expand(1, 8, 301).contiguous()
     got = paged.paged_indexed_attention(q, cache, 0, table, ck, cv, idx, torch.arange(8, device=DEV) // 4)
     assert ((got.cpu().double() - want).abs() <= bound).all(), float((got.cpu().double() - want).abs().max())
+
+
+# ---------------------------------------------------------------- what the logits may lose
+
+def outlier_rows(shape, gen):
+    """K rows with four channels per KV head ten times as large."""
+    x = torch.randn(shape, generator=gen)
+    for h in range(shape[1]):
+        x[:, h, :, torch.randperm(128, generator=gen)[:4]] *= 10
+    return x
+
+
+def logit_steps(q, k, group, kv_heads, n):
+    """Of the dense kernel's sums for a logit, over the magnitudes that pass
+    through them: [B, QH, n], in logits.  S = sum_g (low + 8 delta) qsum + sum_g
+    delta (q . (c - 8))."""
+    code, low, delta = (torch.from_numpy(t.astype(np.float64)) for t in quantise(k[:, :, :n].double().numpy(), group))
+    per = q.shape[1] // kv_heads
+    q = q.cpu().double()
+    out = torch.zeros(q.shape[0], q.shape[1], n, dtype=torch.float64)
+    for h in range(q.shape[1]):
+        g = h // per
+        part = q[:, h].unflatten(-1, (-1, group))  # [B, R, G]
+        apart = torch.einsum("brg,bnrg->bnr", part.abs(), (code[:, g].unflatten(-1, (-1, group)) - 8).abs())
+        first = ((low[:, g].abs() + 8 * delta[:, g]) * part.sum(-1).abs()[:, None]).sum(-1)
+        out[:, h] = first + (delta[:, g] * apart).sum(-1)
+    return out / math.sqrt(128)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group", (16, 32, 64))
+@pytest.mark.parametrize("kind", ("mean", "sign"))
+def test_dense_logits_keep_what_fp32_sums_keep(dtype, group, kind):
+    """Queries that do not average out over keys with outlier channels: the
+    results' distance from float64 is that of the type's own rounding and of a
+    few fp32 roundings of what the sums hold, in the norm."""
+    gen = torch.Generator().manual_seed(60 + group)
+    tokens = 3001
+    cache, table = make([tokens], 2, group=group)
+    k, v = outlier_rows((1, 2, tokens, 128), gen), torch.randn(1, 2, tokens, 128, generator=gen)
+    paged.write_tokens(cache, 0, table, k.to(DEV), v.to(DEV))
+    table.advance(tokens)
+    q = torch.randn(1, 32, 128, generator=gen) * 1.5
+    q = (q + 1.5 if kind == "mean" else q.abs()).to(dtype).to(DEV)
+    ck, cv = (torch.randn(1, 2, 128, generator=gen).to(dtype).to(DEV) for _ in range(2))
+    keys, vals = dequantised(k, group), dequantised(v, group)
+    want = attend(q, keys, vals, ck, cv, [tokens])
+    got = paged.paged_attention_step(q, cache, 0, table, ck, cv).cpu().double()
+    # a logit's error: a step of fp32 (2^-23) of all that its sums hold, and of
+    # the logit itself for its scaling and its exponential
+    steps = logit_steps(q, k, group, 2, tokens)
+    work = torch.zeros_like(want)
+    for h in range(32):
+        g = h // 16
+        rows = torch.cat([keys[0, g], ck[0, g, None].cpu().double()])
+        logit = rows @ q[0, h].cpu().double() / math.sqrt(128)
+        p = torch.softmax(logit, 0)[:tokens]
+        e = 2.0 ** -23 * (steps[0, h] + 2 * logit[:tokens].abs() + 8)
+        if dtype == torch.bfloat16:  # V and the weights in fp16: half a step each, uniform
+            e = torch.sqrt(e * e + 2 * (2.0 ** -11) ** 2 / 3)
+        # errors of different tokens are independent: they add in the square
+        work[0, h] = torch.sqrt(((p * e) ** 2) @ (vals[0, g].abs() + want[0, h].abs()) ** 2)
+    rounding = (want.to(dtype).double() - want).norm()
+    allowed_norm = torch.sqrt(rounding ** 2 + work.norm() ** 2)
+    # (of 4096 elements, the cross term of rounding and work is within four of
+    # its deviations, 4 / sqrt(4096))
+    assert (got - want).norm() <= (1 + 4 / 64) * allowed_norm, float((got - want).norm() / allowed_norm)
