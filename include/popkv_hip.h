@@ -393,7 +393,8 @@ int popkv_dense_attention(const void* queries, int32_t dtype,
  * 128 contiguous; 16-byte aligned) of one layer into the pages: row t of
  * sequence b at position counts[b] + t, for t < tokens[b] (device, NULL: every
  * row).  codes / scales: that layer's.  The pages must be there
- * (popkv_page_reserve); a row without one writes nothing and sets status. */
+ * (popkv_page_reserve); a row without one writes nothing and sets status.  Here
+ * and in the read rows may be 0, and k and v then be anything. */
 int popkv_paged_write(const void* k, const void* v, int32_t dtype, int64_t k_batch_stride, int64_t k_head_stride,
                       int64_t k_token_stride, int64_t v_batch_stride, int64_t v_head_stride, int64_t v_token_stride,
                       int64_t rows, const int64_t* tokens, void* codes, void* scales, int64_t pages, int64_t kv_heads,

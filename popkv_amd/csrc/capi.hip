@@ -931,10 +931,10 @@ int popkv_paged_write(const void* k, const void* v, int32_t dtype, int64_t k_bat
     int st = check_pool(codes, scales, pages, kv_heads, page_tokens, dim_group_size);
     if (st) return st;
     if ((st = check_table(table, counts, width, batch))) return st;
-    if (!k || !v) return fail(POPKV_ERR_INVALID, "null pointer");
     if (!valid_dtype(dtype)) return fail(POPKV_ERR_INVALID, "keys and values must be fp32/fp16/bf16");
     if (rows < 0 || rows > (int64_t{1} << 30)) return fail(POPKV_ERR_INVALID, "bad row count");
-    if (rows == 0) return POPKV_OK;
+    if (rows == 0) return POPKV_OK;  // (before the pointers: an empty tensor has none)
+    if (!k || !v) return fail(POPKV_ERR_INVALID, "null pointer");
     const int64_t es = static_cast<int64_t>(elem_size(dtype));
     const int64_t strides[] = {k_batch_stride, k_head_stride, k_token_stride, v_batch_stride, v_head_stride,
                                v_token_stride};
@@ -955,11 +955,11 @@ int popkv_paged_read(void* k, void* v, int32_t dtype, int64_t rows, int32_t fill
     int st = check_pool(codes, scales, pages, kv_heads, page_tokens, dim_group_size);
     if (st) return st;
     if ((st = check_table(table, counts, width, batch))) return st;
-    if (!k || !v) return fail(POPKV_ERR_INVALID, "null pointer");
     if (!valid_dtype(dtype)) return fail(POPKV_ERR_INVALID, "keys and values must be fp32/fp16/bf16");
     if (rows < 0 || rows > (int64_t{1} << 30)) return fail(POPKV_ERR_INVALID, "bad row count");
+    if (rows == 0) return POPKV_OK;  // (before the pointers: an empty tensor has none)
+    if (!k || !v) return fail(POPKV_ERR_INVALID, "null pointer");
     if (!aligned16(k) || !aligned16(v)) return fail(POPKV_ERR_UNSUPPORTED, "rows read from pages need 16-byte alignment");
-    if (rows == 0) return POPKV_OK;
     const popkv::PagedRead a{k, v, rows, fill};
     return launched(popkv::launch_paged_read(a, paged_view(const_cast<void*>(codes), const_cast<void*>(scales), pages,
                                                            kv_heads, page_tokens, table, width, counts, batch),

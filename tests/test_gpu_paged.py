@@ -1162,3 +1162,18 @@ def test_dense_logits_keep_what_fp32_sums_keep(dtype, group, kind):
     # (of 4096 elements, the cross term of rounding and work is within four of
     # its deviations, 4 / sqrt(4096))
     assert (got - want).norm() <= (1 + 4 / 64) * allowed_norm, float((got - want).norm() / allowed_norm)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_no_rows(dtype):
+    """No rows to write, and the rows of a table that holds none yet."""
+    cache, table = make([64, 64], 3)
+    before = cache.codes.clone()
+    none = torch.empty(2, 3, 0, 128, dtype=dtype, device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    paged.write_tokens(cache, 0, table, none, none, status=status)
+    paged.write_tokens(cache, 0, table, none, none, tokens=torch.tensor([3, 0], device=DEV), status=status)
+    assert int(status) == 0 and torch.equal(cache.codes, before)
+    for k, v in (paged.read_tokens(cache, 0, table, dtype=dtype), paged.read_tokens(cache, 0, table, dtype=dtype, rows=0),
+                 paged.read_tokens(cache, 0, table, out=(none, none.clone()))):
+        assert tuple(k.shape) == tuple(v.shape) == (2, 3, 0, 128) and k.dtype == v.dtype == dtype

@@ -287,3 +287,18 @@ def test_c_page_call_refusals():
         refused(name, args, "layer count", layers=0)
         refused(name, args, "or none of them", refs_out=P)
         refused(name, args, "workspace bytes", bytes=args["bytes"] - 1)
+
+
+def test_c_no_rows_are_no_work():
+    """An empty tensor has no address: a call without rows is done, whatever
+    its row pointers, and still refuses a bad pool, table, type or row count."""
+    write = dict(k=None, v=None, dtype=2, kb=0, kh=0, kt=128, vb=0, vh=0, vt=128, rows=0, tokens=None, **POOL, **TABLE,
+                 status=None, stream=None)
+    read = dict(k=None, v=None, dtype=2, rows=0, fill=1, **POOL, **TABLE, stream=None)
+    for name, args in (("popkv_paged_write", write), ("popkv_paged_read", read)):
+        _native.call(name, *args.values())
+        _native.call(name, *{**args, "k": P + 2, "v": P + 4}.values())
+        pool_and_table_refusals(name, args)
+        refused(name, args, "fp32/fp16/bf16", dtype=3)
+        refused(name, args, "row count", rows=-1)
+        refused(name, args, "null pointer", rows=1)
