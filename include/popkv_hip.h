@@ -415,8 +415,8 @@ int popkv_paged_read(void* k, void* v, int32_t dtype, int64_t rows, int32_t fill
  * query heads per KV head.  max_tokens (host) bounds every count and sizes the
  * launch; a larger count is taken as max_tokens.  Tokens without a page are
  * left out.  Workspace: popkv_paged_attention_workspace_bytes() bytes, 16-byte
- * aligned, whose first max(2^18, batch * KVH * 128) bytes (the merge tickets) are
- * zero on entry and left zero.  One launch. */
+ * aligned, whose first 2^18 bytes (the merge tickets) are zero on entry and left
+ * zero.  One launch. */
 size_t popkv_paged_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t max_tokens);
 int popkv_paged_attention(const void* queries, int32_t dtype, const void* codes, const void* scales, int64_t pages,
                           int64_t kv_heads, int32_t page_tokens, int32_t dim_group_size, const int32_t* table,
@@ -428,10 +428,9 @@ int popkv_paged_attention(const void* queries, int32_t dtype, const void* codes,
  * index equal to counts[b] is the current token; one outside [0, counts[b]]
  * (-1 pads a short row) or with valid_mask 0 is left out, one named twice
  * counts twice, and a row with nothing left is zero.  head_to_kv [QH] int64
- * (entries are clamped to [0, KVH)).  Workspace as above, its first max(2^18,
- * batch * QH * 4) bytes zero.  Calls of both kinds and any shapes may share a
- * workspace, ordered on one stream; where their zero regions differ (batch * KVH
- * above 2048, batch * QH above 65536) it is cleared in between. */
+ * (entries are clamped to [0, KVH)).  Workspace as above.  Calls of both kinds
+ * and any shapes, captured ones too, may share a workspace, ordered on one stream,
+ * without clearing it in between. */
 size_t popkv_paged_indexed_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t selected);
 int popkv_paged_indexed_attention(const void* queries, int32_t dtype, const void* codes, const void* scales,
                                   int64_t pages, int64_t kv_heads, int32_t page_tokens, int32_t dim_group_size,

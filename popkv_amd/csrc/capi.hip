@@ -910,15 +910,6 @@ void carve_compact(Carve& c, popkv::PageCompact& a) {
     a.moves = c.take<int32_t>(1);
 }
 
-// The merge tickets at the start of the attention workspaces.  The states of a
-// call begin behind kTicketBytes however few tickets it has, so that calls of
-// any shapes (captured ones too) share a workspace without clearing it.
-constexpr size_t kTicketBytes = 256 << 10;
-size_t attend_tickets(int64_t tickets) {
-    const size_t bytes = align_up(static_cast<size_t>(tickets) * 4);
-    return bytes < kTicketBytes ? kTicketBytes : bytes;
-}
-
 }  // namespace
 
 extern "C" {
@@ -969,7 +960,7 @@ int popkv_paged_read(void* k, void* v, int32_t dtype, int64_t rows, int32_t fill
 
 size_t popkv_paged_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t max_tokens) {
     if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || max_tokens < 0) return 0;
-    return attend_tickets(batch * kv_heads * popkv::kPagedTickets) +
+    return popkv::kPagedTicketBytes +
            align_up(static_cast<size_t>(popkv::paged_dense_items(batch, kv_heads, max_tokens) * q_heads * (128 + 2)) * 4);
 }
 
@@ -995,7 +986,7 @@ int popkv_paged_attention(const void* queries, int32_t dtype, const void* codes,
         return fail(POPKV_ERR_UNSUPPORTED, "paged attention tensors need 16-byte alignment");
     char* ws = static_cast<char*>(workspace);
     const popkv::PagedAttend a{queries, current_k, current_v, output, static_cast<int>(q_heads),
-                               reinterpret_cast<float*>(ws + attend_tickets(batch * kv_heads * popkv::kPagedTickets)),
+                               reinterpret_cast<float*>(ws + popkv::kPagedTicketBytes),
                                reinterpret_cast<uint32_t*>(ws)};
     return launched(popkv::launch_paged_dense(a, paged_view(const_cast<void*>(codes), const_cast<void*>(scales), pages,
                                                             kv_heads, page_tokens, table, width, counts, batch),
@@ -1006,7 +997,7 @@ int popkv_paged_attention(const void* queries, int32_t dtype, const void* codes,
 size_t popkv_paged_indexed_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t selected) {
     if (batch <= 0 || q_heads <= 0 || selected <= 0) return 0;
     const int64_t rows = batch * q_heads;
-    return attend_tickets(rows) +
+    return popkv::kPagedTicketBytes +
            align_up(static_cast<size_t>(rows * popkv::paged_indexed_splits(rows, selected) * (128 + 3)) * 4);
 }
 
@@ -1034,7 +1025,7 @@ int popkv_paged_indexed_attention(const void* queries, int32_t dtype, const void
         return fail(POPKV_ERR_UNSUPPORTED, "paged attention tensors need 16-byte alignment");
     char* ws = static_cast<char*>(workspace);
     const popkv::PagedAttend a{queries, current_k, current_v, output, static_cast<int>(q_heads),
-                               reinterpret_cast<float*>(ws + attend_tickets(batch * q_heads)),
+                               reinterpret_cast<float*>(ws + popkv::kPagedTicketBytes),
                                reinterpret_cast<uint32_t*>(ws)};
     const popkv::PagedIndexed ix{indices, index_dtype, valid_mask, head_to_kv, selected};
     return launched(popkv::launch_paged_indexed(a, ix, paged_view(const_cast<void*>(codes), const_cast<void*>(scales),

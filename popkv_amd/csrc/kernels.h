@@ -347,9 +347,10 @@ struct PageCompact {
 hipError_t launch_page_compact(const PageCompact& a, const PageMoves& m, hipStream_t stream);
 
 // Decode attention over the pages (head_dim 128): q, out [batch, QH, 128],
-// current k / v [batch, KVH, 128].  tickets (kPagedTickets for each of batch *
-// KVH, or one for each of batch * QH indexed): zero on entry, left zero.
-constexpr int kPagedTickets = 32;
+// current k / v [batch, KVH, 128].  tickets: kPagedTicketBytes, zero on entry,
+// left zero.  Only rows in several parts have any, of which there are fewer than
+// workgroups in a launch, so these bytes are enough for every batch.
+constexpr int64_t kPagedTicketBytes = int64_t{1} << 18;
 struct PagedAttend {
     const void *q, *cur_k, *cur_v;
     void* out;

@@ -281,10 +281,13 @@ __device__ __forceinline__ void merge_rows(const float* ps, int64_t stride, int 
 // in the place of its first, and the last of those merges the sets' (157 parts,
 // 40000 tokens of one KV head with 8 query heads: 15.6 us against 22.1 in one
 // level; up to 32 parts one level is faster, 13.1 us against 15.7 at 16000
-// tokens of 8 KV heads).  Tickets of a (sequence, KV head): kPagedTickets, the
-// sets' from 1 on.
-constexpr int kOneLevel = 32, kSet = 16;
-static_assert(kDenseBlocks / kSet + 1 <= kPagedTickets);
+// tokens of 8 KV heads).  A (sequence, KV head) in several parts has kTickets
+// tickets, the sets' from 1 on, in the place of the workgroup of its first part: no
+// other goes on past that workgroup's end.  (A KV head has several workgroups only
+// where they all are kDenseBlocks at most.)
+constexpr int kOneLevel = 32, kSet = 16, kTickets = 32;
+static_assert(kDenseBlocks / kSet + 1 <= kTickets);
+static_assert(int64_t{kDenseBlocks} * kTickets * 4 <= kPagedTicketBytes);
 
 template <typename T>
 __device__ __forceinline__ void dense_merge(const PagedAttend& a, const PagedView& c, const DenseShare& sh, int h,
@@ -292,7 +295,7 @@ __device__ __forceinline__ void dense_merge(const PagedAttend& a, const PagedVie
     __shared__ uint32_t s_last;
     if (sh.n == 1) return;
     const int lane = threadIdx.x & (kWave - 1);
-    uint32_t* tickets = a.tickets + (static_cast<int64_t>(sh.b) * c.kv_heads + h) * kPagedTickets;
+    uint32_t* tickets = a.tickets + (static_cast<int64_t>(sh.first - sh.b) * c.kv_heads + h) * kTickets;
     const int64_t stride = static_cast<int64_t>(c.kv_heads) * group * kState;
     float* ps = a.partials + (static_cast<int64_t>(sh.first) * c.kv_heads + h) * group * kState;
     int n = sh.n, step = 1;

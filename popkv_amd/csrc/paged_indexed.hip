@@ -179,6 +179,7 @@ struct PickFold<float> {
 constexpr int kPickRows = 8;                            // tokens an octet loads at once
 constexpr int kPickTile = kPickRows * kWave / 8;        // tokens of a wave's pass
 constexpr int kPickBlocks = 256;                        // workgroups in all, one a CU
+static_assert(int64_t{kPickBlocks} / 2 * 4 <= kPagedTicketBytes);  // (more rows than half of them have one split each)
 constexpr int kPickState = kState + 1;                  // (m, l, acc[128], hits of the current token)
 
 // A row's query and its current token, for output dim threadIdx.x of waves 0

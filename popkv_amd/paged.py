@@ -53,6 +53,7 @@ from .popkv import LayerStepWorkspace
 PAGE_TOKENS = (32, 64, 128, 256)
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 _INDEX_CODES = {torch.int64: nat.INDEX_I64, torch.int32: nat.INDEX_I32}
+_TICKET_KIB = 256  # the zero region of an attention workspace, of any call
 
 
 @dataclass
@@ -184,12 +185,6 @@ def _check_cache(cache: PagedKVCache, pages: PageTable, layer: int = 0) -> tuple
     return batch, width, kv_heads, (codes.data_ptr() + rows * 128, scales.data_ptr() + rows * (1024 // g), held,
                                     kv_heads, page_tokens, g, pages.table.data_ptr(), width, pages.counts.data_ptr(),
                                     batch)
-
-
-def _ticket_rows(nbytes: int) -> int:
-    """The zero region of an attention workspace in LayerStepWorkspace's KiB: the
-    same for every call that has at most the C entries' 2^18 bytes of tickets."""
-    return 256 if nbytes <= 1 << 18 else -(-nbytes // 1024)
 
 
 def _check_status(status: torch.Tensor | None) -> None:
@@ -397,7 +392,7 @@ def paged_attention_step(q: torch.Tensor, cache: PagedKVCache, layer: int, pages
     q, k, v = _aligned(q), _aligned(k), _aligned(v)
     output = torch.empty_like(q) if out is None else out
     nbytes = _workspace_bytes("popkv_paged_attention", batch, q_heads, kv_heads, most)
-    ws = (workspace or LayerStepWorkspace()).get(nbytes, dev, _ticket_rows(batch * kv_heads * 128))
+    ws = (workspace or LayerStepWorkspace()).get(nbytes, dev, _TICKET_KIB)
     with nat.on_device(dev):
         nat.call("popkv_paged_attention", q.data_ptr(), dtype, *pool, most, k.data_ptr(), v.data_ptr(), q_heads,
                  output.data_ptr(), ws.data_ptr(), ws.numel(), nat.stream_of(dev))
@@ -434,7 +429,7 @@ def paged_indexed_attention(q: torch.Tensor, cache: PagedKVCache, layer: int, pa
     output = torch.empty_like(q) if out is None else out
     selected = shape[2]
     nbytes = _workspace_bytes("popkv_paged_indexed_attention", batch, q_heads, selected)
-    ws = (workspace or LayerStepWorkspace()).get(nbytes, dev, _ticket_rows(batch * q_heads * 4))
+    ws = (workspace or LayerStepWorkspace()).get(nbytes, dev, _TICKET_KIB)
     with nat.on_device(dev):
         nat.call("popkv_paged_indexed_attention", q.data_ptr(), dtype, *pool, k.data_ptr(), v.data_ptr(),
                  idx.data_ptr(), _INDEX_CODES[idx.dtype], nat.ptr(mask), head_to_kv.data_ptr(), q_heads, selected,

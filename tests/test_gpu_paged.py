@@ -1177,3 +1177,40 @@ def test_no_rows(dtype):
     for k, v in (paged.read_tokens(cache, 0, table, dtype=dtype), paged.read_tokens(cache, 0, table, dtype=dtype, rows=0),
                  paged.read_tokens(cache, 0, table, out=(none, none.clone()))):
         assert tuple(k.shape) == tuple(v.shape) == (2, 3, 0, 128) and k.dtype == v.dtype == dtype
+
+
+@pytest.mark.parametrize("batch", (256, 257, 264))
+def test_captured_calls_of_many_rows_share_a_workspace(batch):
+    """2048 rows (sequences times KV heads), 2056 and 2112, the last sequences in
+    several parts, captured once; a call of few rows leaves its states in the
+    workspace between the replays."""
+    gen = torch.Generator().manual_seed(70)
+    lengths = [i % 3 for i in range(batch - 3)] + [20000, 0, 30000]
+
+    def case(lengths, kv_heads):
+        cache, table = make(lengths, kv_heads, page=32, max_tokens=max(lengths) + 1, poison=False)
+        cache.codes.random_(0, 256)
+        cache.scales.uniform_(-1, 1)
+        table.advance(torch.tensor(lengths, device=DEV), bound=max(lengths))
+        q, ck, cv = (torch.randn(len(lengths), kv_heads, 128, generator=gen).to(DEV) for _ in range(3))
+        return lambda out, ws: paged.paged_attention_step(q, cache, 0, table, ck, cv, workspace=ws, out=out)
+
+    many, few = case(lengths, 8), case([20000], 8)
+    want, out, small = (torch.empty(n, 8, 128, device=DEV) for n in (batch, batch, 1))
+    many(want, popkv.LayerStepWorkspace())
+    ws = popkv.LayerStepWorkspace()
+    many(out, ws)
+    buffer = ws.buffer
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        many(out, ws)
+    for _ in range(3):
+        few(small, ws)
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert ws.buffer is buffer and torch.equal(out, want)
+    few(small, ws)
+    many(out, ws)  # and without a graph
+    assert torch.equal(out, want)
