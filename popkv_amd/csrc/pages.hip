@@ -222,7 +222,10 @@ __global__ __launch_bounds__(256) void copy_words_kernel(const uint32_t* src, ui
 
 // The entries of sequence b that `new_tokens` more tokens need: [lo, hi).
 // Entries before the next token's page are never touched (a program may have
-// dropped them).
+// dropped them); of the others, one outside the pool is no page and is missing.
+__device__ __forceinline__ bool is_missing(const PageReserve& a, int32_t page) {
+    return static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages);
+}
 __device__ __forceinline__ void reserve_range(const PageReserve& a, int64_t b, int64_t& lo, int64_t& hi, bool& fits) {
     const int64_t limit = a.width << a.page_log2;
     const int64_t n = clamp_count(a.counts_in[b], limit);
@@ -242,7 +245,7 @@ __device__ __forceinline__ void reserve_row(const PageReserve& a, int64_t b) {
     reserve_range(a, b, lo, hi, fits);
     const int32_t* row = a.table_in + b * a.width;
     int32_t need = 0;
-    for (int64_t i = lo + lane; i < hi; i += kWave) need += row[i] < 0 ? 1 : 0;
+    for (int64_t i = lo + lane; i < hi; i += kWave) need += is_missing(a, row[i]) ? 1 : 0;
     need = static_cast<int32_t>(wave_incl_scan(static_cast<uint32_t>(need), lane));
     if (lane == kWave - 1) {
         a.need[b] = need;
@@ -399,7 +402,7 @@ __global__ __launch_bounds__(kPlanThreads) void reserve_plan_kernel(PageReserve 
         int32_t* row = a.table + b * a.width;
         int32_t r = at;
         for (int64_t i = lo; i < hi; i += kWave) {
-            const bool missing = i + lane < hi && row[i + lane] < 0;
+            const bool missing = i + lane < hi && is_missing(a, row[i + lane]);
             const uint64_t mask = __ballot(missing);
             if (missing) {
                 const int32_t page = a.list[r + __popcll(mask & ((uint64_t{1} << lane) - 1))];
@@ -487,7 +490,7 @@ __global__ __launch_bounds__(kPlanThreads) void reserve_alone_kernel(PageReserve
             if (i < entries) {
                 const int b = row_of(i, inverse), e = i - b * width;
                 if (a.table != a.table_in) a.table[i] = page[j];
-                missing = page[j] < 0 && e >= s_lo[b] && e < s_hi[b];
+                missing = is_missing(a, page[j]) && e >= s_lo[b] && e < s_hi[b];
                 if (missing) atomicAdd(s_need + b, 1);
             }
             const uint64_t bits = __ballot(missing);

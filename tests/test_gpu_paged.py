@@ -1214,3 +1214,32 @@ def test_captured_calls_of_many_rows_share_a_workspace(batch):
     few(small, ws)
     many(out, ws)  # and without a graph
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("in_place", (False, True))
+@pytest.mark.parametrize("seed,batch,width,page,spare", SHAPES)
+def test_reserve_where_an_entry_is_no_page(seed, batch, width, page, spare, in_place):
+    """An entry outside the pool is no page, as -1 is: a reservation fills it."""
+    cache, pages, book = random_pages(seed, batch, width, page, spare)
+    rng = np.random.default_rng(seed + 3)
+    outside = [cache.pages, cache.pages + 7, 2 ** 31 - 1, -1, -5, -2 ** 31]
+    for b in range(batch):  # from the next token's page on: nothing holds what lies there but the row itself
+        for i in range(book.counts[b] // page, width):
+            if book.table[b][i] < 0 or rng.random() < 0.3:
+                if book.table[b][i] >= 0:
+                    book.refs[book.table[b][i]] -= 1
+                pages.table[b, i] = outside[int(rng.integers(len(outside)))]
+                book.table[b][i] = -1
+    pages.refs.copy_(torch.tensor(book.refs, dtype=torch.int32))
+    left = pages.table.cpu()
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    many = [int(x) for x in rng.integers(0, width * page, batch)]
+    for tokens in ([1] * batch, many):
+        book.reserve(tokens)
+        pages = paged.reserve_pages(pages, torch.tensor(tokens, device=DEV), status=status,
+                                    out=pages if in_place else None)
+        got, want = pages.table.cpu(), torch.tensor(book.table)
+        # what no token asked for is left as it was
+        assert torch.equal(got, torch.where(want < 0, left, want.int()))
+        assert pages.refs.tolist() == book.refs and pages.counts.tolist() == book.counts
+        assert int(status) == book.status
