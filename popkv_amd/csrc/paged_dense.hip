@@ -472,24 +472,32 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
         const int64_t row = (there ? e : 0) * per_page + head_row + (t & in_page);
         const char* code = c.codes + row * kCodeRow;
         const char* sc = reinterpret_cast<const char*>(c.scales) + row * ROWB;
-        // (the wave has read what the stage held; the loads write LDS behind the compiler's back)
-        asm volatile(
-            "s_waitcnt lgkmcnt(0)\n\t"
-            "s_mov_b32 m0, %0\n\t"
-            "s_nop 1\n\t"
-            "global_load_lds_dwordx4 %1, %3 nt\n\t"
-            "global_load_lds_dwordx4 %2, %3 offset:1024 nt\n\t"
-            "global_load_lds_dwordx4 %1, %3 offset:2048 nt\n\t"
-            "global_load_lds_dwordx4 %2, %3 offset:3072 nt\n\t"
-            "s_mov_b32 m0, %4\n\t"
-            "s_nop 1\n\t"
-            "global_load_lds_dwordx4 %5, %6"
-            :
-            : "s"(lds + stage * STAGE), "v"(even), "v"(odd), "s"(code), "s"(lds + stage * STAGE + 4096), "v"(flat),
-              "s"(sc)
-            : "memory");
-        if constexpr (SLOADS == 2)
-            asm volatile("global_load_lds_dwordx4 %0, %1 offset:1024" : : "v"(flat), "s"(sc) : "memory");
+        // (the wave has read what the stage held; the loads write LDS behind the
+        // compiler's back.  All of a tile's in one statement, which leaves m0, where
+        // the LDS address stands, as it found it: the compiler takes no notice of m0
+        // between statements.)
+        uint32_t m0;
+#define POPKV_TILE_LOADS(LAST)                                                                                      \
+    asm volatile(                                                                                                   \
+        "s_waitcnt lgkmcnt(0)\n\t"                                                                                  \
+        "s_mov_b32 %0, m0\n\t"                                                                                      \
+        "s_mov_b32 m0, %1\n\t"                                                                                      \
+        "s_nop 1\n\t"                                                                                               \
+        "global_load_lds_dwordx4 %2, %4 nt\n\t"                                                                     \
+        "global_load_lds_dwordx4 %3, %4 offset:1024 nt\n\t"                                                         \
+        "global_load_lds_dwordx4 %2, %4 offset:2048 nt\n\t"                                                         \
+        "global_load_lds_dwordx4 %3, %4 offset:3072 nt\n\t"                                                         \
+        "s_mov_b32 m0, %5\n\t"                                                                                      \
+        "s_nop 1\n\t"                                                                                               \
+        "global_load_lds_dwordx4 %6, %7\n\t" LAST                                                                   \
+        "s_mov_b32 m0, %0"                                                                                          \
+        : "=&s"(m0)                                                                                                 \
+        : "s"(lds + stage * STAGE), "v"(even), "v"(odd), "s"(code), "s"(lds + stage * STAGE + 4096), "v"(flat),     \
+          "s"(sc)                                                                                                   \
+        : "memory")
+        if constexpr (SLOADS == 2) POPKV_TILE_LOADS("global_load_lds_dwordx4 %6, %7 offset:1024\n\t");
+        else POPKV_TILE_LOADS("");
+#undef POPKV_TILE_LOADS
         return there ? min(kPageTile, sh.t1 - t) : 0;
     };
     // lane addresses in a stage: K of token col (+ 16), V dword col of tokens
