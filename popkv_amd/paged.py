@@ -245,10 +245,12 @@ def _new_table(pages: PageTable, out: PageTable | None) -> PageTable:
     if out.table.shape != pages.table.shape or out.refs.shape != pages.refs.shape \
             or out.page_tokens != pages.page_tokens:
         raise ValueError("out must have the page table's shape")
-    same = [a.data_ptr() == b.data_ptr() for a, b in ((out.table, pages.table), (out.counts, pages.counts),
-                                                      (out.refs, pages.refs))]
+    both = ((out.table, pages.table), (out.counts, pages.counts), (out.refs, pages.refs))
+    same = [a.data_ptr() == b.data_ptr() for a, b in both]
     if any(same) and not all(same):
         raise ValueError("out shares some of the page table's tensors: share all of them or none")
+    if not any(same) and any(_overlap(a, b) for a, b in both):
+        raise ValueError("out's tensors must not overlap the page table's")
     out.bound = pages.bound
     return out
 
@@ -311,7 +313,7 @@ def read_tokens(cache: PagedKVCache, layer: int, pages: PageTable, *, dtype: tor
                 ) -> tuple[torch.Tensor, torch.Tensor]:
     """One layer's cached rows as K, V [B, KVH, rows, 128] (``rows``: default
     ``pages.bound``).  Rows past a sequence's count are zero in new tensors and
-    left as they are in ``out``."""
+    left as they are in ``out`` (two tensors that share no memory)."""
     batch, _, kv_heads, pool = _check_cache(cache, pages, layer)
     if out is None:
         rows = pages.bound if rows is None else int(rows)
@@ -328,6 +330,8 @@ def read_tokens(cache: PagedKVCache, layer: int, pages: PageTable, *, dtype: tor
             raise ValueError(f"out must be two contiguous [{batch}, {kv_heads}, rows, 128] tensors")
         if rows is not None and rows != int(k.shape[2]):
             raise ValueError("rows must be out's row count")
+        if _overlap(k, v):
+            raise ValueError("out's two tensors must not overlap")
     dev = _on_device(cache.codes, cache.scales, pages.table, pages.counts, k, v)
     with nat.on_device(dev):
         nat.call("popkv_paged_read", k.data_ptr(), v.data_ptr(), nat.dtype_code(k), k.shape[2],
@@ -353,11 +357,21 @@ def _step_operands(q: torch.Tensor, batch: int, kv_heads: int, k: torch.Tensor, 
     if out is not None:
         if out.shape != shape or not out.is_contiguous():
             raise ValueError("out must be a contiguous tensor shaped like q")
-        if out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr()):  # (workgroups still read them)
-            raise ValueError("out must not be one of the operands")
+        if _overlap(out, q) or _overlap(out, k) or _overlap(out, v):  # (workgroups still read them)
+            raise ValueError("out must not be one of the operands, nor overlap one")
     if k.dtype != dtype or v.dtype != dtype or (out is not None and out.dtype != dtype):
         raise RuntimeError("queries, current K/V and out must share a dtype")
     return q_heads, nat.dtype_code(q)
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether contiguous `a` shares bytes with b (one with other strides is
+    read through a copy: only its own first element counts)."""
+    first, second = a.data_ptr(), b.data_ptr()
+    if first == second:
+        return a.numel() > 0 and b.numel() > 0
+    return b.is_contiguous() and first < second + b.numel() * b.element_size() \
+        and second < first + a.numel() * a.element_size()
 
 
 def _aligned(x: torch.Tensor) -> torch.Tensor:
@@ -379,7 +393,8 @@ def paged_attention_step(q: torch.Tensor, cache: PagedKVCache, layer: int, pages
     workspace holds merge tickets and split states: share it only with this
     module's attention calls, ordered on one stream.  It grows with the calls; a
     captured graph goes on using the buffer that it was captured with, so let
-    the largest call come first, or keep a workspace for each graph."""
+    the largest call come first, or keep a workspace for each graph.  ``out``
+    shares no memory with the operands."""
     batch, width, kv_heads, pool = _check_cache(cache, pages, layer)
     q_heads, dtype = _step_operands(q, batch, kv_heads, k, v, out)
     if q_heads > 16 * kv_heads:
@@ -410,7 +425,7 @@ def paged_indexed_attention(q: torch.Tensor, cache: PagedKVCache, layer: int, pa
     pad short rows).  Indices outside [0, counts[b]] and entries whose
     ``valid_mask`` is False are left out, an index named twice counts twice,
     and a row with nothing left is zero.  head_to_kv: [QH] KV head indices.
-    The workspace as for ``paged_attention_step``."""
+    The workspace and ``out`` as for ``paged_attention_step``."""
     batch, _, kv_heads, pool = _check_cache(cache, pages, layer)
     q_heads, dtype = _step_operands(q, batch, kv_heads, k, v, out)
     shape = indices.shape

@@ -302,3 +302,58 @@ def test_c_no_rows_are_no_work():
         refused(name, args, "fp32/fp16/bf16", dtype=3)
         refused(name, args, "row count", rows=-1)
         refused(name, args, "null pointer", rows=1)
+
+
+def test_outputs_that_overlap_operands():
+    """Workgroups read the operands while others write: an output that shares
+    memory with one is refused wherever in it that begins."""
+    cache = pool()
+    t = table(cache)
+    t.bound = 100
+    idx, mapping = torch.zeros(3, 8, 4, dtype=torch.int64), torch.zeros(8, dtype=torch.int64)
+    flat = torch.zeros(9 * 8 * 128)
+    rows = lambda first, heads: flat[first * 128:(first + 3 * heads) * 128].view(3, heads, 128)  # noqa: E731
+    q, k, v = rows(0, 8), rows(24, 2), rows(30, 2)
+    for first in (1, 23, 24, 27, 29, 30, 35):
+        for call in (lambda out: paged.paged_attention_step(q, cache, 0, t, k, v, out=out),
+                     lambda out: paged.paged_indexed_attention(q, cache, 0, t, k, v, idx, mapping, out=out)):
+            with pytest.raises(ValueError, match="one of the operands"):
+                call(rows(first, 8))
+    for call in (lambda out: paged.paged_attention_step(q, cache, 0, t, k, v, out=out),
+                 lambda out: paged.paged_indexed_attention(q, cache, 0, t, k, v, idx, mapping, out=out)):
+        with pytest.raises(RuntimeError, match="CUDA device"):  # behind the last of them
+            call(rows(36, 8))
+    x = torch.zeros(2 * 3 * 2 * 5 * 128 + 128)
+    part = lambda first: x[first:first + 3 * 2 * 5 * 128].view(3, 2, 5, 128)  # noqa: E731
+    for second in (0, 128, 3 * 2 * 5 * 128 - 128):
+        for out in ((part(0), part(second)), (part(second), part(0))):
+            with pytest.raises(ValueError, match="overlap"):
+                paged.read_tokens(cache, 0, t, out=out)
+    with pytest.raises(RuntimeError, match="CUDA device"):
+        paged.read_tokens(cache, 0, t, out=(part(0), part(3 * 2 * 5 * 128)))
+    none = torch.zeros(3, 2, 0, 128)
+    with pytest.raises(RuntimeError, match="CUDA device"):  # no rows: nothing to overlap
+        paged.read_tokens(cache, 0, t, out=(none, none))
+
+
+def test_output_tables_that_overlap_the_input():
+    """An output table of its own shares no memory with the input's, not even a
+    part of a tensor."""
+    cache = pool()
+    raw = (torch.full((4, 4), -1, dtype=torch.int32), torch.zeros(4, dtype=torch.int64), torch.zeros(8, dtype=torch.int32))
+    at = lambda i, j, n: paged.PageTable(raw[0][i:i + 3], raw[1][j:j + 3], raw[2][n:n + 6], 64)  # noqa: E731
+    pages = at(0, 0, 0)
+    apart = table(cache)
+    for table_at, counts_at, refs_at in ((1, None, None), (None, 1, None), (None, None, 2), (1, 1, 1)):
+        other = at(table_at or 0, counts_at or 0, refs_at or 0)
+        out = paged.PageTable(apart.table if table_at is None else other.table,
+                              apart.counts if counts_at is None else other.counts,
+                              apart.refs if refs_at is None else other.refs, 64)
+        for call in (lambda: paged.reserve_pages(pages, out=out),
+                     lambda: paged.fork_sequences(cache, pages, torch.arange(3), out=out),
+                     lambda: paged.compact_pages(cache, pages, out=out)):
+            with pytest.raises(ValueError, match="overlap"):
+                call()
+    for out in (at(0, 0, 0), apart):  # in place by another name, and apart
+        with pytest.raises(RuntimeError, match="CUDA device"):
+            paged.reserve_pages(pages, out=out)
