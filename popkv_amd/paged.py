@@ -235,7 +235,8 @@ def _rows(x: torch.Tensor, batch: int, kv_heads: int, what: str) -> tuple[torch.
 
 
 def _new_table(pages: PageTable, out: PageTable | None) -> PageTable:
-    """The table a call writes: `out`, or a new one."""
+    """The table a call writes: `out`, whose bound follows once the call is
+    made, or a new one."""
     if out is pages:
         return pages
     if out is None:
@@ -251,7 +252,6 @@ def _new_table(pages: PageTable, out: PageTable | None) -> PageTable:
         raise ValueError("out shares some of the page table's tensors: share all of them or none")
     if not any(same) and any(_overlap(a, b) for a, b in both):
         raise ValueError("out's tensors must not overlap the page table's")
-    out.bound = pages.bound
     return out
 
 
@@ -283,6 +283,7 @@ def reserve_pages(pages: PageTable, tokens: int | torch.Tensor = 1, *, bound: in
         nat.call("popkv_page_reserve", pages.table.data_ptr(), pages.counts.data_ptr(), pages.refs.data_ptr(),
                  new.table.data_ptr(), new.counts.data_ptr(), new.refs.data_ptr(), width, batch, count,
                  pages.page_tokens, nat.ptr(tokens), each, nat.ptr(status), ws.data_ptr(), nbytes, nat.stream_of(dev))
+    new.bound = pages.bound
     return new
 
 
@@ -478,6 +479,7 @@ def fork_sequences(cache: PagedKVCache, pages: PageTable, parents: torch.Tensor,
                  pool[6], pool[8], pages.refs.data_ptr(), new.table.data_ptr(), new.counts.data_ptr(),
                  new.refs.data_ptr(), width, batch, parents.data_ptr(), nat.ptr(status), ws.data_ptr(), nbytes,
                  nat.stream_of(dev))
+    new.bound = pages.bound
     return new
 
 
@@ -498,4 +500,5 @@ def compact_pages(cache: PagedKVCache, pages: PageTable, *, out: PageTable | Non
         nat.call("popkv_page_compact", pool[0], pool[1], cache.codes.shape[0], pool[2], kv_heads, pool[4], pool[5],
                  pool[6], pool[8], pages.refs.data_ptr(), new.table.data_ptr(), new.counts.data_ptr(),
                  new.refs.data_ptr(), width, batch, page_map.data_ptr(), ws.data_ptr(), nbytes, nat.stream_of(dev))
+    new.bound = pages.bound
     return new, page_map

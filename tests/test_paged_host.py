@@ -357,3 +357,15 @@ def test_output_tables_that_overlap_the_input():
     for out in (at(0, 0, 0), apart):  # in place by another name, and apart
         with pytest.raises(RuntimeError, match="CUDA device"):
             paged.reserve_pages(pages, out=out)
+
+
+def test_a_refused_call_leaves_its_output_as_it_was():
+    cache = pool()
+    pages, out = table(cache), table(cache)
+    pages.bound, out.bound = 100, 7
+    for call in (lambda: paged.reserve_pages(pages, out=out),
+                 lambda: paged.fork_sequences(cache, pages, torch.arange(3), out=out),
+                 lambda: paged.compact_pages(cache, pages, out=out)):
+        with pytest.raises(RuntimeError, match="CUDA device"):
+            call()
+        assert out.bound == 7
