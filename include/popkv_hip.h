@@ -460,7 +460,8 @@ int popkv_page_reserve(const int32_t* table_in, const int64_t* counts_in, const 
  * status).  Full pages are shared.  The open page, and pages reserved behind
  * it, stay with the parent's lowest child; every other child gets a copy of
  * the open page in all `layers` (codes / scales: the whole pool).  A child for
- * whose copy the pool has no page is left empty and sets status. */
+ * whose copy the pool has no page is left empty and sets status.  The input
+ * table is spent: pages that ended sequences gave back may hold such copies. */
 size_t popkv_page_fork_workspace_bytes(int64_t batch, int64_t width);
 int popkv_page_fork(void* codes, void* scales, int64_t layers, int64_t pages, int64_t kv_heads, int32_t page_tokens,
                     int32_t dim_group_size, const int32_t* table_in, const int64_t* counts_in, const int32_t* refs_in,

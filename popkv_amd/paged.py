@@ -88,8 +88,11 @@ class PageTable:
     """``table`` int32 [B, width] (the page of every ``page_tokens`` tokens,
     -1 where there is none), ``counts`` int64 [B] cached tokens, ``refs`` int32
     [pages] (0: free), and ``bound``, the most tokens any sequence holds as far
-    as the host knows (it sizes launches; the counts themselves stay on the
-    device)."""
+    as the host knows (the counts themselves stay on the device).  It sizes
+    launches, and the dense attention leaves out what lies past it; ``advance``
+    raises it and no call lowers it.  A program that knows better sets it: higher
+    after replays of a captured step, which move the counts alone, lower once its
+    long sequences have ended."""
     table: torch.Tensor
     counts: torch.Tensor
     refs: torch.Tensor
@@ -117,7 +120,9 @@ class PageTable:
 
     def advance(self, tokens: int | torch.Tensor = 1, *, bound: int | None = None) -> None:
         """Every sequence gained ``tokens`` tokens (an int64 [B] on the device
-        for different numbers, with the new ``bound``)."""
+        for different numbers, with the new ``bound``).  Negative numbers take
+        tokens back, but not into a page that a fork shares: what is written
+        there next would be every holder's."""
         if isinstance(tokens, torch.Tensor):
             if bound is None:
                 raise ValueError("give the new bound with tokens on the device")
@@ -463,7 +468,8 @@ def fork_sequences(cache: PagedKVCache, pages: PageTable, parents: torch.Tensor,
     lowest child.  A child for whose copy no page is free is left empty and
     sets ``status`` bit 4; a parent outside the batch empties the sequence and
     sets bit 8.  Returns a new page table, or writes ``out`` (which may be
-    ``pages``); the old one must not be written through any more."""
+    ``pages``); the old one is spent: pages that its ended sequences gave back
+    may hold other tokens already."""
     batch, width, kv_heads, pool = _check_cache(cache, pages)
     _check_status(status)
     if parents.shape != (batch,) or parents.dtype is not torch.int64:
@@ -489,7 +495,7 @@ def compact_pages(cache: PagedKVCache, pages: PageTable, *, out: PageTable | Non
     layer: those at n or later move, in order, to the free places before n.
     Returns the new page table (or ``out``, which may be ``pages``) and the
     int32 [pages] map of where each live page is now (-1: it was free), for
-    whoever holds pages outside this table."""
+    whoever holds pages outside this table; the old table is spent."""
     batch, width, kv_heads, pool = _check_cache(cache, pages)
     new = _new_table(pages, out)
     dev = _on_device(cache.codes, cache.scales, pages.table, pages.counts, pages.refs, new.table, new.counts, new.refs)

@@ -1243,3 +1243,40 @@ def test_reserve_where_an_entry_is_no_page(seed, batch, width, page, spare, in_p
         assert torch.equal(got, torch.where(want < 0, left, want.int()))
         assert pages.refs.tolist() == book.refs and pages.counts.tolist() == book.counts
         assert int(status) == book.status
+
+
+def test_the_bound_is_the_programs():
+    """Replays move the counts and not the host's bound: eager calls see the
+    new tokens once the program has set it, and it may lower it as well."""
+    gen = torch.Generator().manual_seed(80)
+    cache, table = make([64, 30], 2, page=32, max_tokens=96)
+    rows = torch.randn(2, 2, 64, 128, generator=gen).to(DEV)
+    step = torch.zeros(2, 2, 1, 128, device=DEV)
+
+    def call():
+        paged.write_tokens(cache, 0, table, step, step)
+        table.advance()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # (compiles nothing: the first use of the kernels outside the capture)
+        paged.write_tokens(cache, 0, table, step, step)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    table.bound = 0
+    for t in range(30):
+        step.copy_(rows[:, :, t:t + 1])
+        graph.replay()
+    assert table.counts.tolist() == [30, 30] and table.bound == 0
+    table.bound = 30
+    want = dequantised(rows[:, :, :30], 32)
+    for x in paged.read_tokens(cache, 0, table, dtype=torch.float32):
+        assert torch.equal(x.cpu(), want.float())
+    q, ck, cv = (torch.randn(2, 2, 128, generator=gen).to(DEV) for _ in range(3))
+    for most, lengths in ((30, [30, 30]), (12, [12, 12])):
+        table.bound = most
+        want = attend(q, dequantised(rows, 32), dequantised(rows, 32), ck, cv, lengths)
+        got = paged.paged_attention_step(q, cache, 0, table, ck, cv)
+        assert ((got.cpu().double() - want).abs() <= ULP[torch.float32] * want.abs() + FP32).all()
