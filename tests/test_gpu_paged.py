@@ -1280,3 +1280,82 @@ def test_the_bound_is_the_programs():
         want = attend(q, dequantised(rows, 32), dequantised(rows, 32), ck, cv, lengths)
         got = paged.paged_attention_step(q, cache, 0, table, ck, cv)
         assert ((got.cpu().double() - want).abs() <= ULP[torch.float32] * want.abs() + FP32).all()
+
+
+# ---------------------------------------------------------------- bounds that a wrong sum breaks
+
+def near(want, dtype, q, k, v, ck, cv, group, lengths):
+    """Largest error per element of the dense kernel on K, V rows (as written):
+    a logit's sums pass at most sixteen fp32 steps (2^-23) of the magnitudes they
+    hold, its scaling and exponential four of itself and sixteen of one; the sums
+    over the tokens 64 steps of what they hold (|low| + 16 delta); bf16 V and
+    weights half an fp16 step each, and no weight is off by more than 2^-33 of the
+    largest; then the result's own rounding."""
+    kv_heads = ck.shape[1]
+    per = q.shape[1] // kv_heads
+    bound = torch.zeros_like(want)
+    for b, n in enumerate(lengths):
+        steps = logit_steps(q[b:b + 1], k[b:b + 1], group, kv_heads, n)[0]
+        for g in range(kv_heads):
+            keys = torch.cat([dequantised(k[b, g, :n], group), ck[b, g, None].cpu().double()])
+            vals = torch.cat([dequantised(v[b, g, :n], group), cv[b, g, None].cpu().double()]).abs()
+            _, low, delta = quantise(v[b, g, :n].double().numpy(), group)
+            held = np.repeat(np.abs(low.astype(np.float64)) + 16 * delta.astype(np.float64), group, -1)
+            held = torch.cat([torch.from_numpy(held.reshape(n, 128)), vals[n:]])
+            for h in range(g * per, g * per + per):
+                logit = keys @ q[b, h].cpu().double() / math.sqrt(128)
+                p = torch.softmax(logit, 0)
+                e = 2.0 ** -23 * (16 * torch.cat([steps[h], logit[n:].abs()]) + 4 * logit.abs() + 16)
+                bound[b, h] = (p * e) @ (vals + want[b, h].abs()) + 64 * 2.0 ** -23 * (p @ held)
+                if dtype == torch.bfloat16:
+                    bound[b, h] += 2 * 2.0 ** -11 * (p @ vals) + n * 2.0 ** -33 * vals.max()
+    half = torch.finfo(dtype).eps / 2
+    return half * (want.abs() + bound) + bound
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group", (16, 32, 64))
+@pytest.mark.parametrize("kv_heads,per,lengths", [(1, 16, [8200]), (2, 3, [20011]), (1, 8, [66000]), (1, 1, [65569]),
+                                                  (4, 1, [4097, 33, 1, 1500]), (3, 2, [300] * 9)])
+def test_dense_attention_to_its_bound(dtype, group, kv_heads, per, lengths):
+    """Long sequences, merges in two levels and ragged batches against bounds
+    that neither zeros nor half of the tokens would pass."""
+    gen = torch.Generator().manual_seed(90 + group + per)
+    cache, table = make(lengths, kv_heads, group=group, max_tokens=max(lengths) + 1)
+    batch = len(lengths)
+    k, v = (torch.randn(batch, kv_heads, max(lengths), 128, generator=gen) for _ in range(2))
+    count = torch.tensor(lengths, device=DEV)
+    paged.write_tokens(cache, 0, table, k.to(DEV), v.to(DEV), tokens=count)
+    table.advance(count, bound=max(lengths))
+    q = (torch.randn(batch, kv_heads * per, 128, generator=gen) * 2).to(dtype).to(DEV)
+    ck, cv = (torch.randn(batch, kv_heads, 128, generator=gen).to(dtype).to(DEV) for _ in range(2))
+    keys, vals = dequantised(k, group), dequantised(v, group)
+    want = attend(q, keys, vals, ck, cv, lengths)
+    bound = near(want, dtype, q, k, v, ck, cv, group, lengths)
+    got = paged.paged_attention_step(q, cache, 0, table, ck, cv).cpu().double()
+    assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())
+    half = attend(q, keys, vals, ck, cv, [n // 2 for n in lengths])
+    for wrong in (torch.zeros_like(want), half):
+        assert ((wrong - want).abs() > bound).double().mean() > 0.9
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group", (16, 32, 64))
+@pytest.mark.parametrize("first,last", [(0, 1), (96, 700), (0, 700)])
+def test_attention_keeps_nan_values(dtype, group, first, last):
+    """NaN values in live rows of one KV head: NaN in the dims of their scale
+    group for that KV head's queries, none elsewhere."""
+    gen = torch.Generator().manual_seed(first + last + group)
+    cache, table = make([700], 2, group=group)
+    k, v = (torch.randn(1, 2, 700, 128, generator=gen) for _ in range(2))
+    v[0, 1, first:last, 70] = float("nan")
+    paged.write_tokens(cache, 0, table, k.to(DEV), v.to(DEV))
+    table.advance(700)
+    q = torch.randn(1, 8, 128, generator=gen).to(dtype).to(DEV)
+    ck, cv = (torch.randn(1, 2, 128, generator=gen).to(dtype).to(DEV) for _ in range(2))
+    idx = torch.arange(701, device=DEV).expand(1, 8, 701).contiguous()
+    want = torch.zeros(8, 128, dtype=torch.bool)
+    want[4:, 70 // group * group:(70 // group + 1) * group] = True
+    for got in (paged.paged_attention_step(q, cache, 0, table, ck, cv),
+                paged.paged_indexed_attention(q, cache, 0, table, ck, cv, idx, torch.arange(8, device=DEV) // 4)):
+        assert torch.equal(got[0].isnan().cpu(), want)
