@@ -68,9 +68,9 @@ constexpr int kDenseBlocks = 256;
 
 // What a further sequence costs a workgroup beside its tiles, in tiles: the
 // queries, the join of the waves, the state or output.  Sequences 0, 14, 24 and 30
-// tiles apart: a ragged batch of five up to 20001, fp16 8 queries a KV head, 31.2,
-// 28.2, 26.6 and 27.0 us; 64 up to 2000 41.0, 34.5, 32.6 and 32.2; 16 up to 1000
-// 19.0, 12.5, 12.8 and 13.6; 64 of one token 34, 11.0, 11.0 and 10.8.
+// tiles apart: a ragged batch of five up to 20001, fp16 8 queries a KV head, 32.5,
+// 29.0, 28.0 and 27.8 us; 64 up to 2000 42.0, 35.5, 33.6 and 33.2; 16 up to 1000
+// 19.9, 13.1, 13.5 and 14.5; 64 of one token 34.7, 11.0, 11.0 and 10.8.
 constexpr int kSequenceCost = 24;
 
 // Workgroups of a KV head: one a CU in all, with a tile for each wave (with two
@@ -280,7 +280,7 @@ __device__ __forceinline__ void merge_rows(const float* ps, int64_t stride, int 
 // what takes the time: the last workgroup of every kSet leaves the set's state
 // in the place of its first, and the last of those merges the sets' (157 parts,
 // 40000 tokens of one KV head with 8 query heads: 15.6 us against 22.1 in one
-// level; up to 32 parts one level is faster, 13.1 us against 15.7 at 16000
+// level; up to 32 parts one level is faster, 13.7 us against 15.7 at 16000
 // tokens of 8 KV heads).  A (sequence, KV head) in several parts has kTickets
 // tickets, the sets' from 1 on, in the place of the workgroup of its first part: no
 // other goes on past that workgroup's end.  (A KV head has several workgroups only
@@ -376,12 +376,13 @@ __device__ __forceinline__ void exchange_quarters(uint32_t (&d)[4]) {
 //                                    times delta's upper seven and lower four bits
 // so keys enter the logits unrounded: with the outlier channels that keys have,
 // their rounding to fp16 was four times fp16's own in the result.  Codes are taken
-// from their middle because the two sums must not cancel more than the keys do:
-// with 1024 + c, the bits as they come, sum(q) a thousandfold went through the
-// fp32 sums, and results of queries of one sign were 1.5 to 2.6 times as far off
-// as fp16's own rounding (now 1.00 of it; 5 % of bf16's time at 8 x 65535, 4 of
-// fp16's).  (C layout: lane l holds rows 4 (l / 16) .. + 3 of column l % 16; A and
-// B: lane l holds k-elements 8 (l / 16) .. + 7 of row / column l % 16.)
+// from their middle so that the two sums cancel little: with 1024 + c, the bits as
+// they come, sum(q) a thousandfold went through the fp32 sums, and fp16 results of
+// queries of one sign were 1.5 to 2.6 times as far off as their own rounding (now
+// 1.00 of it, for 5 % of the time at 8 x 65535; sums that start at minus the
+// thousandfold cost nothing and were still 1.8 times as far off).  (C layout: lane
+// l holds rows 4 (l / 16) .. + 3 of column l % 16; A and B: lane l holds k-elements
+// 8 (l / 16) .. + 7 of row / column l % 16.)
 // A code becomes fp16 by its bits: 0x6400 | c is 1024 + c, and 0x6400 | 16 c
 // is 1024 + 16 c; a packed subtraction, or an fma by 1/16, leaves c - 8 (nine
 // instructions a dword of eight).  A token's 16-byte quarters are exchanged among
@@ -400,12 +401,13 @@ __device__ __forceinline__ void exchange_quarters(uint32_t (&d)[4]) {
 // where queries have no mean (relative 1.0e-6 against 2.1e-6 at 20001 tokens), and
 // two to three times as far where they have one sign (3.1e-6 against 2.0e-6, at
 // 64-dim groups 5.2e-6 and 1.7e-6): the two sums of S then cancel.
-// 8 x 65536 tokens of 8 KV heads, 64-dim groups, 604 MB: bf16 112 us (5.4 TB/s;
-// such a stream is read in 97 by itself), fp16 138, fp32 154: bound by the vector
-// instructions around the products.  A ragged batch of five up to 20001 with 64
-// query heads, 32-dim groups, 77 MB: bf16 24.1, fp16 27.8, fp32 30 (94 by fp32
-// vector products).  4095 tokens, 5 MB, 10.9: a chain of reads, one tile a wave,
-// the hand-off.
+// 8 x 65536 tokens of 8 KV heads, 64-dim groups, 604 MB: bf16 112 to 118 us with
+// the card (5.4 to 5.1 TB/s, where a plain read of as many bytes takes 86 us), fp16
+// 138 to 145, fp32 154: bound by the vector instructions around the products, 325 a
+// tile beside 18 matrix instructions in bf16.  A ragged batch of five up to 20001
+// with 64 query heads, 32-dim groups, 77 MB: bf16 24.1, fp16 27.8, fp32 30 (94 by
+// fp32 vector products).  4095 tokens, 5 MB, 10.9: a chain of reads, one tile a
+// wave, the hand-off.
 template <typename T, int G>
 __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend a, PagedView c, int64_t max_tokens,
                                                                          int groups) {
@@ -413,7 +415,7 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
     constexpr bool F32 = std::is_same_v<T, float>;
     constexpr int HALVES = R == 8 ? 2 : 1;        // groups of a 32-dim step
     // Query registers: fp32 two terms; 16-bit types a set for each half of a step,
-    // zero in the other (31.3 us at 16-dim groups, a ragged fp16 batch, against 32.9
+    // zero in the other (31.2 us at 16-dim groups, a ragged fp16 batch, against 32.7
     // with the codes masked; fp32 has no registers left for that and masks them).
     constexpr int QSETS = F32 ? 2 : HALVES;
     constexpr int LOWS = R == 8 ? 2 : 1;          // products for the low terms (four groups each)
@@ -442,8 +444,9 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
     // l's 16 bytes of load i are quarter (l % 8) ^ swz(token) of token 8 i + l /
     // 8, so that the reads below (16 tokens' equal quarters; four tokens' 64
     // bytes of V) meet 64 different banks.  swz(t) = 4 (t / 2 % 2) + t / 4 % 4.
-    // Codes pass the caches by (131071 tokens 33.9 us against 37.9, 4095 and a ragged
-    // batch whose pages stay in the last-level cache 1 % slower).
+    // Codes pass the caches by (8 x 65535 tokens 112.8 us against 118.0; what stays
+    // in the last-level cache from call to call, 131071 and 4095 tokens and a ragged
+    // batch, 0 to 3 % slower).
     struct Tile {
         uint4 k[2];
         uint32_t ks[2][R], v[8], vs[8];
@@ -832,7 +835,8 @@ __global__ __launch_bounds__(kDenseThreads) void paged_dense_kernel(PagedAttend 
 #pragma unroll 1
         for (int i = 0; i < tiles; ++i) {
             // the two waves of a SIMD go first in turn: left to itself the older one
-            // ends early and leaves the other alone (131071 tokens: 20 and 28 us)
+            // ends early and leaves the other alone (131071 tokens: 20 and 28 us; the
+            // launch at 8 x 65535 112.8 us, without turns 117.1)
             if (((i ^ (wave >> 2)) & 1) != 0) __builtin_amdgcn_s_setprio(1);
             else __builtin_amdgcn_s_setprio(0);
             Tile x;

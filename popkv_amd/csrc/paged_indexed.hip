@@ -260,7 +260,7 @@ __device__ __forceinline__ void pick_merge(const float* ps, int n, const Current
 // the next eight indices behind them.  The current token is counted, not read:
 // the merge folds it in as often as it was selected.  Bound by its chain of
 // reads (index, page table entry, token) and the hand-off of the splits: 4096 of
-// 32767 tokens for each of 32 heads, bf16, 64-dim groups, 20 MB: 11.4 us (1.8
+// 32767 tokens for each of 32 heads, bf16, 64-dim groups, 20 MB: 11.9 us (1.7
 // TB/s); 256 of them, without a hand-off, 6.4.
 template <typename T, int G, typename I, int W>
 __global__ __launch_bounds__(W * kWave) void paged_indexed_kernel(PagedAttend a, PagedIndexed ix, PagedView c,
@@ -374,7 +374,7 @@ __global__ __launch_bounds__(W * kWave) void paged_indexed_kernel(PagedAttend a,
 // (more CUs share the gathers: 1024 of 32767 tokens for 32 heads 8.7 us, by eight
 // 10.2; 1001 for 48 rows fp32 9.2 and 11.4) and where there are more rows than
 // CUs (several workgroups on each: 512 rows of 1000 24.4 and 27.4); else eight, a
-// workgroup a CU and half as many states (4096 for 32 heads 11.4, by four 13.1;
+// workgroup a CU and half as many states (4096 for 32 heads 11.9, by four 13.1;
 // 256 rows of 1024 14.9 and 17.2, of 500 9.0 and 11.4; four sequences of 2048 for
 // 32 heads 16.9 and 17.1).
 struct PickPlan {

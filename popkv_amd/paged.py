@@ -38,7 +38,9 @@ A page that a sequence still fills is its alone; full pages may be shared.
 of its work: 1 a page table row is full, 4 no free page is left (or a token's
 page is missing), 8 a fork's parent lies outside the batch.  Poll it after
 steps, as for ``batch.append_batched``.  Implementation limits: head_dim 128;
-1 to 16 query heads per KV head in the dense attention.
+1 to 16 query heads per KV head in the dense attention; one query token a
+sequence.  The retrieval's packed planes are not part of the pages: forks and
+compactions leave them as they are.
 """
 from __future__ import annotations
 
@@ -426,8 +428,9 @@ def paged_indexed_attention(q: torch.Tensor, cache: PagedKVCache, layer: int, pa
                             out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention over selected tokens, the sparse layers' counterpart of
     ``paged_attention_step``: indices [B, QH, selected] (int64 or int32), the
-    current token named by ``counts[b]``, as a retrieval step returns them
-    (``batch.popkv_layer_step_batched(return_indices=True)``, whose -1 entries
+    current token named by ``counts[b]``, as a retrieval returns them
+    (``topk.select_with_current``, or, over its own 16-bit caches,
+    ``batch.popkv_layer_step_batched(return_indices=True)``, whose -1 entries
     pad short rows).  Indices outside [0, counts[b]] and entries whose
     ``valid_mask`` is False are left out, an index named twice counts twice,
     and a row with nothing left is zero.  head_to_kv: [QH] KV head indices.
