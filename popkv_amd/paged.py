@@ -92,7 +92,7 @@ class PageTable:
     [pages] (0: free), and ``bound``, the most tokens any sequence holds as far
     as the host knows (the counts themselves stay on the device).  It sizes
     launches, and the dense attention leaves out what lies past it; ``advance``
-    raises it and no call lowers it.  A program that knows better sets it: higher
+    moves it and no other call does.  A program that knows better sets it: higher
     after replays of a captured step, which move the counts alone, lower once its
     long sequences have ended."""
     table: torch.Tensor

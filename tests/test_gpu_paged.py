@@ -1359,3 +1359,33 @@ def test_attention_keeps_nan_values(dtype, group, first, last):
     for got in (paged.paged_attention_step(q, cache, 0, table, ck, cv),
                 paged.paged_indexed_attention(q, cache, 0, table, ck, cv, idx, torch.arange(8, device=DEV) // 4)):
         assert torch.equal(got[0].isnan().cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_small_queries_beside_a_large_one(dtype):
+    """A head's largest query element is 2^14 times the others, and the keys
+    make up for it: no query element loses bits to the largest."""
+    gen = torch.Generator().manual_seed(95)
+    group, tokens = 16, 400
+    cache, table = make([tokens], 2, group=group)
+    k, v = torch.randn(1, 2, tokens, 128, generator=gen) * 6e3, torch.randn(1, 2, tokens, 128, generator=gen)
+    k[..., :group] = 0  # (the large element's group)
+    paged.write_tokens(cache, 0, table, k.to(DEV), v.to(DEV))
+    table.advance(tokens)
+    q = torch.randn(1, 8, 128, generator=gen) * 1e-3
+    q[..., 0] = 16.0
+    q = q.to(dtype).to(DEV)
+    ck = torch.zeros(1, 2, 128, dtype=dtype, device=DEV)
+    cv = torch.randn(1, 2, 128, generator=gen).to(dtype).to(DEV)
+    keys, vals = dequantised(k, group), dequantised(v, group)
+    want = attend(q, keys, vals, ck, cv, [tokens])
+    bound = near(want, dtype, q, k, v, ck, cv, group, [tokens])
+    # and each element off by at most 2^-29 of the largest, in the products with c - 8
+    code, _, delta = quantise(k.double().numpy(), group)
+    size = torch.from_numpy(np.abs(code.astype(np.float64) - 8) * np.repeat(delta.astype(np.float64), group, -1)).sum(-1)
+    for h in range(8):
+        p = torch.softmax(torch.cat([keys[0, h // 4] @ q[0, h].cpu().double() / math.sqrt(128), torch.zeros(1)]), 0)
+        e = 2.0 ** -29 * 16 * size[0, h // 4] / math.sqrt(128)
+        bound[0, h] += (p[:tokens] * e) @ (vals[0, h // 4].abs() + want[0, h].abs())
+    got = paged.paged_attention_step(q, cache, 0, table, ck, cv).cpu().double()
+    assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())
