@@ -1389,3 +1389,41 @@ def test_small_queries_beside_a_large_one(dtype):
         bound[0, h] += (p[:tokens] * e) @ (vals[0, h // 4].abs() + want[0, h].abs())
     got = paged.paged_attention_step(q, cache, 0, table, ck, cv).cpu().double()
     assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kv_heads,per", [(64, 2), (100, 1), (129, 1), (300, 2)])
+def test_attention_of_many_kv_heads(dtype, kv_heads, per):
+    """As many KV heads as leave each four workgroups, two, or one, and more of
+    them than the card has places for at once; 256-token pages, int32 indices."""
+    lengths = [2100, 0, 300]
+    gen = torch.Generator().manual_seed(kv_heads)
+    cache, table = make(lengths, kv_heads, group=64, page=256, max_tokens=2101)
+    k, v = (torch.randn(3, kv_heads, 2100, 128, generator=torch.Generator(device=DEV).manual_seed(kv_heads + i),
+                        device=DEV) for i in range(2))
+    count = torch.tensor(lengths, device=DEV)
+    paged.write_tokens(cache, 0, table, k, v, tokens=count)
+    table.advance(count, bound=2100)
+    rows, vals = paged.read_tokens(cache, 0, table, dtype=torch.float32)  # (bit for bit the format's: tested above)
+    q = torch.randn(3, kv_heads * per, 128, generator=gen).to(dtype).to(DEV)
+    ck, cv = (torch.randn(3, kv_heads, 128, generator=gen).to(dtype).to(DEV) for _ in range(2))
+    rows = torch.cat([rows, torch.zeros_like(rows[:, :, :1])], 2).double()
+    vals = torch.cat([vals, torch.zeros_like(vals[:, :, :1])], 2).double()
+    for b, n in enumerate(lengths):
+        rows[b, :, n], vals[b, :, n] = ck[b].double(), cv[b].double()
+    want = torch.zeros(q.shape, dtype=torch.float64, device=DEV)
+    for b, n in enumerate(lengths):
+        for h in range(kv_heads):
+            s = torch.softmax(q[b, h * per:(h + 1) * per].double() @ rows[b, h, :n + 1].t().contiguous() / math.sqrt(128), 1)
+            want[b, h * per:(h + 1) * per] = s @ vals[b, h, :n + 1]
+    # fp32 work, and for the dense bf16 form V and the weights in fp16 of the largest value
+    bound = torch.finfo(dtype).eps / 2 * (want.abs() + FP32) + FP32
+    half = bound + (2 * 2.0 ** -11 * float(vals.abs().max()) if dtype == torch.bfloat16 else 0)
+    ws = popkv.LayerStepWorkspace()
+    for _ in range(2):
+        got = paged.paged_attention_step(q, cache, 0, table, ck, cv, workspace=ws)
+        assert ((got.double() - want).abs() <= half).all(), float((got.double() - want).abs().max())
+    idx = torch.arange(2101, device=DEV, dtype=torch.int32).expand(3, kv_heads * per, 2101).contiguous()
+    got = paged.paged_indexed_attention(q, cache, 0, table, ck, cv, idx, torch.arange(kv_heads * per, device=DEV) // per,
+                                        workspace=ws)
+    assert ((got.double() - want).abs() <= bound).all(), float((got.double() - want).abs().max())
