@@ -440,6 +440,34 @@ int popkv_paged_indexed_attention(const void* queries, int32_t dtype, const void
                                   int64_t q_heads, int64_t selected, void* output, void* workspace,
                                   size_t workspace_bytes, void* stream);
 
+/* Attention of a chunk of new tokens of one layer: row t of sequence b, t <
+ * tokens[b] (int64 [batch], device; NULL: all `rows`), attends over b's cached
+ * tokens and the chunk's tokens 0 .. t, which are not cached yet: output[b, i, t] =
+ * softmax(q . [K; k] / sqrt(128)) . [V; v].  queries, output [batch, QH, rows, 128],
+ * k, v [batch, KVH, rows, 128], each with element strides of batch, head and row and
+ * contiguous rows, 16-byte aligned; query head i on KV head i / (QH / KVH), any
+ * number of query heads per KV head.  Output rows past tokens[b] are cleared with
+ * fill, else left as they are.  max_tokens bounds the counts as in
+ * popkv_paged_attention; tokens without a page are left out.  rows may be 0.
+ * weights (float32 [batch, KVH, weight_stride], NULL: none): the attention weights
+ * of every token, summed over the rows and the query heads of its KV head, are added
+ * at the token's place, a chunk's token t at counts[b] + t (places past
+ * weight_stride are left out).  Workspace: popkv_paged_chunk_attention_workspace_bytes()
+ * bytes (with weights != 0 for calls that gather them), 16-byte aligned; its first
+ * 2^18 bytes are not written, the others' content does not matter. */
+size_t popkv_paged_chunk_attention_workspace_bytes(int32_t dtype, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                                   int64_t rows, int64_t max_tokens, int32_t weights);
+int popkv_paged_chunk_attention(const void* queries, int32_t dtype, int64_t q_batch_stride, int64_t q_head_stride,
+                                int64_t q_row_stride, const void* k, int64_t k_batch_stride, int64_t k_head_stride,
+                                int64_t k_row_stride, const void* v, int64_t v_batch_stride, int64_t v_head_stride,
+                                int64_t v_row_stride, int64_t rows, const int64_t* tokens, const void* codes,
+                                const void* scales, int64_t pages, int64_t kv_heads, int32_t page_tokens,
+                                int32_t dim_group_size, const int32_t* table, int64_t width, const int64_t* counts,
+                                int64_t batch, int64_t max_tokens, int64_t q_heads, void* output,
+                                int64_t out_batch_stride, int64_t out_head_stride, int64_t out_row_stride, int32_t fill,
+                                float* weights, int64_t weight_stride, void* workspace, size_t workspace_bytes,
+                                void* stream);
+
 /* Page bookkeeping.  Each call reads a page table (table_in, counts_in,
  * refs_in) and writes another, or the same one (all three outputs the inputs,
  * or none of them).  Pages are taken lowest first.  The workspace's content
@@ -477,6 +505,26 @@ int popkv_page_compact(void* codes, void* scales, int64_t layers, int64_t pages,
                        int32_t dim_group_size, const int32_t* table_in, const int64_t* counts_in,
                        const int32_t* refs_in, int32_t* table, int64_t* counts, int32_t* refs, int64_t width,
                        int64_t batch, int32_t* page_map, void* workspace, size_t workspace_bytes, void* stream);
+
+/* evict: sequences of more than keeps[b] tokens (int64 [batch], device, held in
+ * [0, keep]; NULL: keep) are cut to as many, in every layer and KV head by itself:
+ * the last min(recent, keeps[b]) of them and, of the others, those of the largest
+ * weights (float32 [layers, batch, KVH, weight_stride], weight_stride >= width *
+ * page_tokens; NaN the largest, ties to the lowest place).  The kept tokens move to places
+ * 0 .. keeps[b] - 1 in their order, their weights with them to `weights` (which may
+ * be weights_in), zero behind; kept int32 [layers, batch, KVH, keep] says where each
+ * was (-1 past keeps[b], and for sequences that are not cut).  Pages behind are given
+ * back, ones reserved ahead too.  A page of the front that has further holders is not
+ * written: a free one takes its place.  A sequence for which the pool has none, or one
+ * of whose tokens' pages is missing, stays as it was and sets status.  The input table is
+ * spent. */
+size_t popkv_page_evict_workspace_bytes(int64_t batch, int64_t width, int64_t pages);
+int popkv_page_evict(void* codes, void* scales, int64_t layers, int64_t pages, int64_t kv_heads, int32_t page_tokens,
+                     int32_t dim_group_size, const int32_t* table_in, const int64_t* counts_in, const int32_t* refs_in,
+                     int32_t* table, int64_t* counts, int32_t* refs, int64_t width, int64_t batch,
+                     const float* weights_in, float* weights, int64_t weight_stride, const int64_t* keeps, int64_t keep,
+                     int64_t recent, int32_t* kept, int32_t* status, void* workspace, size_t workspace_bytes,
+                     void* stream);
 
 #ifdef __cplusplus
 }

@@ -84,6 +84,11 @@ _SIGNATURES = {
     "popkv_paged_indexed_attention": (ctypes.c_int, [_vp, _c_i32, _vp, _vp, _c_i64, _c_i64, _c_i32, _c_i32, _vp, _c_i64,
                                                      _vp, _c_i64, _vp, _vp, _vp, _c_i32, _vp, _vp, _c_i64, _c_i64, _vp,
                                                      _vp, _c_size, _vp]),
+    "popkv_paged_chunk_attention_workspace_bytes": (_c_size, [_c_i32, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i32]),
+    "popkv_paged_chunk_attention": (ctypes.c_int, [_vp, _c_i32, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp,
+                                                   _c_i64, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64, _c_i32,
+                                                   _c_i32, _vp, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64,
+                                                   _c_i64, _c_i32, _vp, _c_i64, _vp, _c_size, _vp]),
     "popkv_page_reserve_workspace_bytes": (_c_size, [_c_i64, _c_i64]),
     "popkv_page_reserve": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i32, _vp, _c_i64, _vp,
                                           _vp, _c_size, _vp]),
@@ -93,6 +98,10 @@ _SIGNATURES = {
     "popkv_page_compact_workspace_bytes": (_c_size, [_c_i64]),
     "popkv_page_compact": (ctypes.c_int, [_vp, _vp, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _vp, _vp, _vp, _vp, _vp, _vp,
                                           _c_i64, _c_i64, _vp, _vp, _c_size, _vp]),
+    "popkv_page_evict_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64]),
+    "popkv_page_evict": (ctypes.c_int, [_vp, _vp, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _vp, _vp, _vp, _vp, _vp, _vp,
+                                        _c_i64, _c_i64, _vp, _vp, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _vp, _c_size,
+                                        _vp]),
 }
 
 

@@ -910,6 +910,25 @@ void carve_compact(Carve& c, popkv::PageCompact& a) {
     a.moves = c.take<int32_t>(1);
 }
 
+void carve_evict(Carve& c, popkv::PageEvict& a) {
+    a.old = c.take<int32_t>(a.batch * a.width);
+    a.need = c.take<int32_t>(a.batch + 1);
+    a.list = c.take<int32_t>(a.pages);
+    a.held = c.take<int32_t>(a.batch);
+    a.cut = c.take<int32_t>(a.batch);
+}
+// Behind the merge tickets of the other paged attention calls, which may share the workspace.
+void carve_chunk(Carve& c, popkv::PagedChunk& a, int32_t dtype, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                 int64_t rows, int64_t max_tokens, bool weights) {
+    (void)max_tokens;
+    if (!weights) return;
+    a.row_tiles = popkv::paged_chunk_row_tiles(rows, q_heads / kv_heads);
+    const int64_t tiles = batch * kv_heads * a.row_tiles;
+    a.queries = c.take<uint4>(tiles * popkv::paged_chunk_stored(dtype) * 512);
+    a.factors = c.take<float>(tiles * 32);
+    a.lse = c.take<float>(tiles * 32);
+}
+
 }  // namespace
 
 extern "C" {
@@ -1035,6 +1054,80 @@ int popkv_paged_indexed_attention(const void* queries, int32_t dtype, const void
                     "popkv_paged_indexed_attention");
 }
 
+size_t popkv_paged_chunk_attention_workspace_bytes(int32_t dtype, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                                   int64_t rows, int64_t max_tokens, int32_t weights) {
+    if (!valid_dtype(dtype) || batch <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || rows <= 0 ||
+        max_tokens < 0)
+        return 0;
+    Carve c{nullptr};
+    popkv::PagedChunk a{};
+    carve_chunk(c, a, dtype, batch, q_heads, kv_heads, rows, max_tokens, weights != 0);
+    return popkv::kPagedTicketBytes + c.off;
+}
+
+int popkv_paged_chunk_attention(const void* queries, int32_t dtype, int64_t q_batch_stride, int64_t q_head_stride,
+                                int64_t q_row_stride, const void* k, int64_t k_batch_stride, int64_t k_head_stride,
+                                int64_t k_row_stride, const void* v, int64_t v_batch_stride, int64_t v_head_stride,
+                                int64_t v_row_stride, int64_t rows, const int64_t* tokens, const void* codes,
+                                const void* scales, int64_t pages, int64_t kv_heads, int32_t page_tokens,
+                                int32_t dim_group_size, const int32_t* table, int64_t width, const int64_t* counts,
+                                int64_t batch, int64_t max_tokens, int64_t q_heads, void* output,
+                                int64_t out_batch_stride, int64_t out_head_stride, int64_t out_row_stride, int32_t fill,
+                                float* weights, int64_t weight_stride, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+    int st = check_pool(codes, scales, pages, kv_heads, page_tokens, dim_group_size);
+    if (st) return st;
+    if ((st = check_table(table, counts, width, batch))) return st;
+    if (!valid_dtype(dtype)) return fail(POPKV_ERR_INVALID, "tensors must be fp32/fp16/bf16");
+    if (q_heads <= 0 || q_heads > 65535 || q_heads % kv_heads != 0)
+        return fail(POPKV_ERR_INVALID, "query heads must be a positive multiple of the KV heads");
+    if (max_tokens < 0 || max_tokens > (int64_t{1} << 30)) return fail(POPKV_ERR_TOKENS, "invalid token count");
+    if (rows < 0 || rows * q_heads > (int64_t{1} << 30)) return fail(POPKV_ERR_INVALID, "bad row count");
+    if (rows == 0) return POPKV_OK;  // (before the pointers: an empty tensor has none)
+    if (!queries || !k || !v || !output || !workspace) return fail(POPKV_ERR_INVALID, "null pointer");
+    if (weights && weight_stride <= 0) return fail(POPKV_ERR_INVALID, "bad weight stride");
+    const int64_t es = static_cast<int64_t>(elem_size(dtype));
+    const int64_t strides[] = {q_batch_stride, q_head_stride, q_row_stride, k_batch_stride,   k_head_stride,   k_row_stride,
+                               v_batch_stride, v_head_stride, v_row_stride, out_batch_stride, out_head_stride, out_row_stride};
+    for (int64_t x : strides)
+        if (x < 0 || (x * es) % 16) return fail(POPKV_ERR_UNSUPPORTED, "chunk attention rows need 16-byte alignment");
+    if (!aligned16(queries) || !aligned16(k) || !aligned16(v) || !aligned16(output) || !aligned16(workspace))
+        return fail(POPKV_ERR_UNSUPPORTED, "chunk attention tensors need 16-byte alignment");
+    if (reinterpret_cast<uintptr_t>(weights) % 4) return fail(POPKV_ERR_UNSUPPORTED, "weights need 4-byte alignment");
+    const size_t need = popkv_paged_chunk_attention_workspace_bytes(dtype, batch, q_heads, kv_heads, rows, max_tokens,
+                                                                    weights != nullptr);
+    if (workspace_bytes < need) return fail(POPKV_ERR_WORKSPACE, "chunk attention needs %zu workspace bytes", need);
+    popkv::PagedChunk a{};
+    a.q = queries;
+    a.k = k;
+    a.v = v;
+    a.out = output;
+    a.q_bs = q_batch_stride;
+    a.q_hs = q_head_stride;
+    a.q_ts = q_row_stride;
+    a.k_bs = k_batch_stride;
+    a.k_hs = k_head_stride;
+    a.k_ts = k_row_stride;
+    a.v_bs = v_batch_stride;
+    a.v_hs = v_head_stride;
+    a.v_ts = v_row_stride;
+    a.o_bs = out_batch_stride;
+    a.o_hs = out_head_stride;
+    a.o_ts = out_row_stride;
+    a.rows = rows;
+    a.tokens = tokens;
+    a.q_heads = static_cast<int>(q_heads);
+    a.fill = fill;
+    a.weights = weights;
+    a.weight_stride = weight_stride;
+    Carve c{static_cast<char*>(workspace) + popkv::kPagedTicketBytes};
+    carve_chunk(c, a, dtype, batch, q_heads, kv_heads, rows, max_tokens, weights != nullptr);
+    return launched(popkv::launch_paged_chunk(a, paged_view(const_cast<void*>(codes), const_cast<void*>(scales), pages,
+                                                            kv_heads, page_tokens, table, width, counts, batch),
+                                              max_tokens, dtype, dim_group_size, as_stream(stream)),
+                    "popkv_paged_chunk_attention");
+}
+
 size_t popkv_page_reserve_workspace_bytes(int64_t batch, int64_t pages) {
     if (batch <= 0 || pages <= 0) return 0;
     Carve c{nullptr};
@@ -1145,6 +1238,69 @@ int popkv_page_compact(void* codes, void* scales, int64_t layers, int64_t pages,
     m.counts = counts == counts_in ? nullptr : counts;
     m.batch = batch;
     return launched(popkv::launch_page_compact(a, m, as_stream(stream)), "popkv_page_compact");
+}
+
+size_t popkv_page_evict_workspace_bytes(int64_t batch, int64_t width, int64_t pages) {
+    if (batch <= 0 || width <= 0 || pages <= 0) return 0;
+    Carve c{nullptr};
+    popkv::PageEvict a{};
+    a.batch = batch;
+    a.width = width;
+    a.pages = pages;
+    carve_evict(c, a);
+    return c.off;
+}
+
+int popkv_page_evict(void* codes, void* scales, int64_t layers, int64_t pages, int64_t kv_heads, int32_t page_tokens,
+                     int32_t dim_group_size, const int32_t* table_in, const int64_t* counts_in, const int32_t* refs_in,
+                     int32_t* table, int64_t* counts, int32_t* refs, int64_t width, int64_t batch,
+                     const float* weights_in, float* weights, int64_t weight_stride, const int64_t* keeps, int64_t keep,
+                     int64_t recent, int32_t* kept, int32_t* status, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+    int st = check_pool(codes, scales, pages, kv_heads, page_tokens, dim_group_size);
+    if (st) return st;
+    if ((st = check_table(table_in, counts_in, width, batch))) return st;
+    if (keep < 0 || recent < 0) return fail(POPKV_ERR_INVALID, "bad token count");
+    if (!refs_in || !table || !counts || !refs || !weights_in || !weights || (!kept && keep > 0) || !workspace)
+        return fail(POPKV_ERR_INVALID, "null pointer");
+    if (layers <= 0 || layers > 65535) return fail(POPKV_ERR_INVALID, "bad layer count");
+    if (layers * batch * kv_heads > 0x7fffffff) return fail(POPKV_ERR_UNSUPPORTED, "too many sequences and heads");
+    if (weight_stride < width * page_tokens) return fail(POPKV_ERR_INVALID, "weights must cover the page table");
+    if (width * page_tokens > (int64_t{1} << 30)) return fail(POPKV_ERR_UNSUPPORTED, "a page table row is too long");
+    if (keep > width * page_tokens) return fail(POPKV_ERR_INVALID, "keep must fit the page table");
+    if ((table == table_in) != (counts == counts_in) || (table == table_in) != (refs == refs_in))
+        return fail(POPKV_ERR_INVALID, "the outputs are the inputs or none of them");
+    if (workspace_bytes < popkv_page_evict_workspace_bytes(batch, width, pages))
+        return fail(POPKV_ERR_WORKSPACE, "page evict needs %zu workspace bytes",
+                    popkv_page_evict_workspace_bytes(batch, width, pages));
+    if (!aligned16(workspace)) return fail(POPKV_ERR_UNSUPPORTED, "the workspace needs 16-byte alignment");
+    popkv::PageEvict a{};
+    a.table_in = table_in;
+    a.counts_in = counts_in;
+    a.refs_in = refs_in;
+    a.table = table;
+    a.counts = counts;
+    a.refs = refs;
+    a.codes = static_cast<char*>(codes);
+    a.scales = static_cast<uint32_t*>(scales);
+    a.layers = layers;
+    a.batch = batch;
+    a.width = width;
+    a.pages = pages;
+    a.kv_heads = static_cast<int>(kv_heads);
+    a.page_log2 = log2_of(page_tokens);
+    a.scale_words = 2 * (128 / dim_group_size);
+    a.weights_in = weights_in;
+    a.weights = weights;
+    a.weight_stride = weight_stride;
+    a.keeps = keeps;
+    a.keep = keep;
+    a.recent = recent;
+    a.kept = kept;
+    a.status = status;
+    Carve c{static_cast<char*>(workspace)};
+    carve_evict(c, a);
+    return launched(popkv::launch_page_evict(a, as_stream(stream)), "popkv_page_evict");
 }
 
 }  // extern "C"

@@ -346,6 +346,32 @@ struct PageCompact {
 };
 hipError_t launch_page_compact(const PageCompact& a, const PageMoves& m, hipStream_t stream);
 
+// Sequences of more than keeps[b] (null: `keep`; at most `keep`) tokens cut to as
+// many: per layer and KV head the last `recent` ones and those of the largest
+// weights, in their order.  weights [layers, batch, KVH, weight_stride], kept
+// [layers, batch, KVH, keep] the tokens' old places (-1: sequence as it was).
+// Workspace: old batch * width, need batch + 1, list pages, held batch, cut batch.
+struct PageEvict {
+    const int32_t* table_in;
+    const int64_t* counts_in;
+    const int32_t* refs_in;
+    int32_t* table;
+    int64_t* counts;
+    int32_t* refs;
+    char* codes;
+    uint32_t* scales;
+    int64_t layers, batch, width, pages;
+    int kv_heads, page_log2, scale_words;
+    const float* weights_in;
+    float* weights;
+    int64_t weight_stride;
+    const int64_t* keeps;
+    int64_t keep, recent;
+    int32_t *kept, *status;
+    int32_t *old, *need, *list, *held, *cut;  // old, held: the table and counts as they were; cut: tokens kept, -1: all
+};
+hipError_t launch_page_evict(const PageEvict& a, hipStream_t stream);
+
 // Decode attention over the pages (head_dim 128): q, out [batch, QH, 128],
 // current k / v [batch, KVH, 128].  tickets: kPagedTicketBytes, zero on entry,
 // left zero.  Only rows in several parts have any, of which there are fewer than
@@ -375,5 +401,29 @@ struct PagedIndexed {
 int64_t paged_indexed_splits(int64_t rows, int64_t selected);
 hipError_t launch_paged_indexed(const PagedAttend& a, const PagedIndexed& ix, const PagedView& c, int dtype,
                                 int dim_group, hipStream_t stream);
+
+// Attention of tokens[b] (null: `rows`) new tokens a sequence (head_dim 128): q,
+// out [batch, QH, rows, 128], k / v [batch, KVH, rows, 128], strides in elements,
+// rows contiguous.  Rows past tokens[b] of out are cleared with fill, else left.
+// weights [batch, KVH, weight_stride] (null: none): every token's attention
+// weight over the rows of its KV head's query heads, added.
+struct PagedChunk {
+    const void *q, *k, *v;
+    void* out;
+    int64_t q_bs, q_hs, q_ts, k_bs, k_hs, k_ts, v_bs, v_hs, v_ts, o_bs, o_hs, o_ts, rows;
+    const int64_t* tokens;
+    int q_heads, fill;
+    float* weights;
+    int64_t weight_stride;
+    // with weights, for every (sequence, KV head) row_tiles times 32 rows: the
+    // query operands (paged_chunk_stored(dtype) * 8 KB a tile), factors and sums
+    int64_t row_tiles;
+    uint4* queries;
+    float *factors, *lse;
+};
+int64_t paged_chunk_stored(int dtype);
+int64_t paged_chunk_row_tiles(int64_t rows, int64_t group);
+hipError_t launch_paged_chunk(const PagedChunk& a, const PagedView& c, int64_t max_tokens, int dtype, int dim_group,
+                              hipStream_t stream);
 
 }  // namespace popkv

@@ -20,8 +20,13 @@ popkv.py:105-111).
     attention (``popkv.dense_attention_step``) and the sparse layers' attention
     over selected tokens (``sparse_kernels.indexed_attention_split``), for a
     batch, reading the pages;
-  * ``read_tokens``: the cached rows back in a float dtype, for a prefill that
-    extends a cached prefix;
+  * ``paged_chunk_attention``: several new tokens a sequence at once, over the
+    cached tokens and, causally, each other: a prompt behind a cached prefix, a
+    prompt's next part, proposed tokens to verify; it can gather every token's
+    attention weight (``allocate_token_weights``) as it goes;
+  * ``evict_tokens``: sequences cut, in every layer and KV head by itself, to their
+    most recent tokens and those that gathered the largest weights;
+  * ``read_tokens``: the cached rows back in a float dtype;
   * ``fork_sequences``: beams, several answers to one prompt, sequences that
     end; ``compact_pages``: the live pages to the front of the pool.
 
@@ -33,14 +38,20 @@ A decode step of a batch:
         write_tokens(cache, layer, pages, k, v)
     pages.advance()
 
+A prompt, or a part of one, is the same with ``paged_chunk_attention``, ``tokens``
+of every sequence reserved, written and advanced; a bounded cache gives that call
+``weights=w[layer]`` (one token is a chunk too) and calls
+``evict_tokens(cache, pages, w, keep, out=pages, weights_out=w)`` once the
+sequences have grown past ``keep`` by some.
+
 A page that a sequence still fills is its alone; full pages may be shared.
 ``status`` (int32, on the device) collects bits where a call could not do all
 of its work: 1 a page table row is full, 4 no free page is left (or a token's
 page is missing), 8 a fork's parent lies outside the batch.  Poll it after
 steps, as for ``batch.append_batched``.  Implementation limits: head_dim 128;
-1 to 16 query heads per KV head in the dense attention; one query token a
-sequence.  The retrieval's packed planes are not part of the pages: forks and
-compactions leave them as they are.
+1 to 16 query heads per KV head in ``paged_attention_step``.  The retrieval's
+packed planes are not part of the pages: forks and compactions leave them as they
+are; ``evict_tokens`` says which tokens it kept.
 """
 from __future__ import annotations
 
@@ -459,6 +470,165 @@ def paged_indexed_attention(q: torch.Tensor, cache: PagedKVCache, layer: int, pa
                  idx.data_ptr(), _INDEX_CODES[idx.dtype], nat.ptr(mask), head_to_kv.data_ptr(), q_heads, selected,
                  output.data_ptr(), ws.data_ptr(), ws.numel(), nat.stream_of(dev))
     return output
+
+
+def allocate_token_weights(cache: PagedKVCache, pages: PageTable) -> torch.Tensor:
+    """What tokens have gathered, nothing yet: float32 [layers, B, KVH,
+    ``pages.capacity``] for ``paged_chunk_attention`` and ``evict_tokens``.  After
+    ``fork_sequences`` the children's are ``weights[:, parents]``."""
+    return torch.zeros((cache.layers, pages.batch, cache.kv_heads, pages.capacity), dtype=torch.float32,
+                       device=cache.codes.device)
+
+
+def _span(x: torch.Tensor) -> tuple[int, int]:
+    """The addresses from x's first byte to behind its last."""
+    last = sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
+    return x.data_ptr(), x.data_ptr() + (last + 1) * x.element_size()
+
+
+def _chunk_out(q: torch.Tensor, out: torch.Tensor | None, operands: tuple[torch.Tensor, ...]) -> torch.Tensor:
+    """The tensor a chunk's rows go to: `out`, its rows contiguous, aligned, apart
+    from each other and from the operands; or a new one laid out like q."""
+    if out is None:
+        out = torch.empty_like(q)  # (q's order of dimensions, where it has no gaps)
+        return out if out.stride(3) == 1 else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out.shape != q.shape:
+        raise ValueError("out must be shaped like q")
+    if out.dtype != q.dtype:
+        raise RuntimeError("queries, new K/V and out must share a dtype")
+    if not out.numel():
+        return out
+    reach = 1
+    for stride, n in sorted((s, n) for s, n in zip(out.stride(), out.shape) if n > 1):
+        if stride < reach:
+            raise ValueError("out's rows must not overlap")
+        reach = stride * (n - 1) + reach
+    unit = 16 // out.element_size()
+    if out.stride(3) != 1 or out.data_ptr() % 16 or any(s % unit for s, n in zip(out.stride()[:3], out.shape) if n > 1):
+        raise ValueError("out's rows must be contiguous and 16-byte aligned")
+    first, last = _span(out)
+    for x in operands:
+        if x.numel():
+            a, b = _span(x)
+            if first < b and a < last:  # (workgroups still read them)
+                raise ValueError("out must not be one of the operands, nor overlap one")
+    return out
+
+
+def paged_chunk_attention(q: torch.Tensor, cache: PagedKVCache, layer: int, pages: PageTable, k: torch.Tensor,
+                          v: torch.Tensor, *, tokens: torch.Tensor | None = None,
+                          weights: torch.Tensor | None = None, max_tokens: int | None = None,
+                          workspace: LayerStepWorkspace | None = None,
+                          out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a chunk of new tokens of one layer: q [B, QH, rows, 128], their
+    k/v [B, KVH, rows, 128], not cached yet (any strides with contiguous rows) ->
+    [B, QH, rows, 128].  Row t of sequence b, t < ``tokens[b]`` (int64 [B] on the
+    device; None: all rows), attends over b's cached tokens and the chunk's tokens 0
+    .. t; query head h reads KV head h // (QH / KVH).  Rows past ``tokens[b]`` are
+    zero in a new tensor and left as they are in ``out``.  ``write_tokens`` and
+    ``advance`` with the same ``tokens`` follow.
+
+    ``weights`` (contiguous float32 [B, KVH, ``pages.capacity``], a layer of
+    ``allocate_token_weights``): every token's attention weight, summed over the rows
+    and the query heads of its KV head, is added to its place, token t of the chunk at
+    ``counts[b] + t``.
+
+    ``max_tokens`` and ``workspace`` as for ``paged_attention_step``; ``out`` shares
+    no memory with the operands."""
+    batch, width, kv_heads, pool = _check_cache(cache, pages, layer)
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != batch or shape[3] != 128:
+        raise ValueError(f"q must be [{batch}, query heads, rows, 128]")
+    _, q_heads, rows, _ = shape
+    if q_heads <= 0 or q_heads % kv_heads != 0:
+        raise ValueError("query heads must be a positive multiple of the KV heads")
+    want = (batch, kv_heads, rows, 128)
+    if k.shape != want or v.shape != want:
+        raise ValueError(f"new k and v must be {list(want)}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise RuntimeError("queries, new K/V and out must share a dtype")
+    dtype = nat.dtype_code(q)
+    if tokens is not None:
+        tokens = _tokens(tokens, batch)
+    most = pages.bound if max_tokens is None else int(max_tokens)
+    if most < pages.bound:
+        raise ValueError("max_tokens must cover the page table's bound")
+    capacity = width * pages.page_tokens
+    most = min(most, capacity)
+    if weights is not None:
+        if weights.shape != (batch, kv_heads, capacity) or weights.dtype is not torch.float32 \
+                or not weights.is_contiguous():
+            raise ValueError(f"weights must be a contiguous float32 [{batch}, {kv_heads}, {capacity}]")
+        if any(_overlap(weights, x) for x in (q, k, v)) or (out is not None and _overlap(weights, out)):
+            raise ValueError("weights must not overlap another operand")
+    output = _chunk_out(q, out, (q, k, v))
+    dev = _on_device(cache.codes, cache.scales, pages.table, pages.counts, q, k, v, tokens, weights, out)
+    if rows == 0:
+        return output
+    q, _, *q_strides = _rows(q, batch, q_heads, "q")
+    k, _, *k_strides = _rows(k, batch, kv_heads, "new keys")
+    v, _, *v_strides = _rows(v, batch, kv_heads, "new values")
+    nbytes = _workspace_bytes("popkv_paged_chunk_attention", dtype, batch, q_heads, kv_heads, rows, most,
+                              0 if weights is None else 1)
+    ws = (workspace or LayerStepWorkspace()).get(nbytes, dev, _TICKET_KIB)
+    o_strides = [s if n > 1 else 0 for s, n in zip(output.stride()[:3], shape)]
+    with nat.on_device(dev):
+        nat.call("popkv_paged_chunk_attention", q.data_ptr(), dtype, *q_strides, k.data_ptr(), *k_strides, v.data_ptr(),
+                 *v_strides, rows, nat.ptr(tokens), *pool, most, q_heads, output.data_ptr(), *o_strides,
+                 1 if out is None else 0, nat.ptr(weights), capacity, ws.data_ptr(), ws.numel(), nat.stream_of(dev))
+    return output
+
+
+def evict_tokens(cache: PagedKVCache, pages: PageTable, weights: torch.Tensor, keep: int, *, recent: int = 0,
+                 keeps: torch.Tensor | None = None, status: torch.Tensor | None = None,
+                 out: PageTable | None = None, weights_out: torch.Tensor | None = None
+                 ) -> tuple[PageTable, torch.Tensor, torch.Tensor]:
+    """Sequences of more than ``keep`` tokens are cut to ``keep`` (``keeps``, int64 [B]
+    on the device: to that many each, ``keep`` at most).  Every layer and KV head
+    keeps the last ``recent`` tokens and, of the others, those of the largest
+    ``weights`` (float32 [layers, B, KVH, ``pages.capacity``]; NaN is the largest, of
+    equal ones the first is kept), in their order at the front of the sequence; the
+    pages behind are given back, reserved ones too.  A page of the front that a fork
+    shares is not written: a free one takes its place.  A sequence for which none is
+    free, or one of whose tokens' pages is missing, stays as it was and sets
+    ``status`` bit 4.
+
+    Returns the new page table (or ``out``, which may be ``pages``), the kept tokens'
+    weights, zero behind them (or ``weights_out``, which may be ``weights``), and where
+    each kept token was, int32 [layers, B, KVH, keep] (-1 past a sequence's share and
+    for sequences that were not cut), for whoever holds more about the tokens.  The
+    bound stays: once no ``status`` is set, it may be lowered to ``keep``.  The old
+    table is spent."""
+    batch, width, kv_heads, pool = _check_cache(cache, pages)
+    _check_status(status)
+    capacity = width * pages.page_tokens
+    want = (cache.codes.shape[0], batch, kv_heads, capacity)
+    for x in (weights, weights_out):
+        if x is not None and (x.shape != want or x.dtype is not torch.float32 or not x.is_contiguous()):
+            raise ValueError(f"weights must be a contiguous float32 {list(want)}")
+    keep, recent = min(int(keep), capacity), min(int(recent), capacity)
+    if keep < 0 or recent < 0:
+        raise ValueError("keep and recent must not be negative")
+    if keeps is not None and (keeps.shape != (batch,) or keeps.dtype is not torch.int64):
+        raise ValueError(f"keeps must be an int64 [{batch}] tensor")
+    if weights_out is not None and weights_out.data_ptr() != weights.data_ptr() and _overlap(weights_out, weights):
+        raise ValueError("weights_out must be weights or not overlap them")
+    new = _new_table(pages, out)
+    dev = _on_device(cache.codes, cache.scales, pages.table, pages.counts, pages.refs, weights, weights_out, keeps, status,
+                     new.table, new.counts, new.refs)
+    moved = torch.empty_like(weights) if weights_out is None else weights_out
+    kept = torch.empty((*want[:3], keep), dtype=torch.int32, device=dev)
+    if keeps is not None:
+        keeps = keeps.contiguous()
+    nbytes = _workspace_bytes("popkv_page_evict", batch, width, pool[2])
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with nat.on_device(dev):
+        nat.call("popkv_page_evict", pool[0], pool[1], want[0], pool[2], kv_heads, pool[4], pool[5], pool[6], pool[8],
+                 pages.refs.data_ptr(), new.table.data_ptr(), new.counts.data_ptr(), new.refs.data_ptr(), width, batch,
+                 weights.data_ptr(), moved.data_ptr(), capacity, nat.ptr(keeps), keep, recent, kept.data_ptr(),
+                 nat.ptr(status), ws.data_ptr(), nbytes, nat.stream_of(dev))
+    new.bound = pages.bound
+    return new, moved, kept
 
 
 def fork_sequences(cache: PagedKVCache, pages: PageTable, parents: torch.Tensor, *,
