@@ -20,7 +20,8 @@ CSRC = PKG / "csrc"
 LIB_DIR = PKG / "_lib"
 LIB_PATH = LIB_DIR / "libpopkv_hip.so"
 SOURCES = ("pack.hip", "score.hip", "select.hip", "attention.hip", "dense.hip", "pages.hip", "paged_dense.hip",
-           "paged_indexed.hip", "paged_chunk.hip", "page_evict.hip", "capi.hip")
+           "paged_indexed.hip", "paged_chunk.hip", "paged_chunk_bf16.hip",
+           "paged_chunk_f16.hip", "paged_chunk_f32.hip", "page_evict.hip", "capi.hip")
 ARCH = os.environ.get("POPKV_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [

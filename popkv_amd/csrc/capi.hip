@@ -920,11 +920,17 @@ void carve_evict(Carve& c, popkv::PageEvict& a) {
 // Behind the merge tickets of the other paged attention calls, which may share the workspace.
 void carve_chunk(Carve& c, popkv::PagedChunk& a, int32_t dtype, int64_t batch, int64_t q_heads, int64_t kv_heads,
                  int64_t rows, int64_t max_tokens, bool weights) {
-    (void)max_tokens;
+    const popkv::ChunkPlan p = popkv::paged_chunk_plan(dtype, batch, q_heads, kv_heads, rows, max_tokens);
+    a.shape = a.row_waves = p.shape;
+    a.groups = p.groups;
+    a.least = p.least;
+    a.item_cost = p.item_cost;
+    a.row_blocks = p.row_blocks;
+    a.parts = c.take<int2>(batch * p.row_blocks);
+    a.partials = c.take<float>(p.states);
     if (!weights) return;
-    a.row_tiles = popkv::paged_chunk_row_tiles(rows, q_heads / kv_heads);
-    const int64_t tiles = batch * kv_heads * a.row_tiles;
-    a.queries = c.take<uint4>(tiles * popkv::paged_chunk_stored(dtype) * 512);
+    const int64_t tiles = batch * kv_heads * p.row_blocks * p.shape;
+    a.queries = c.take<uint4>(tiles * p.stored * 512);
     a.factors = c.take<float>(tiles * 32);
     a.lse = c.take<float>(tiles * 32);
 }
@@ -1086,6 +1092,8 @@ int popkv_paged_chunk_attention(const void* queries, int32_t dtype, int64_t q_ba
     if (rows == 0) return POPKV_OK;  // (before the pointers: an empty tensor has none)
     if (!queries || !k || !v || !output || !workspace) return fail(POPKV_ERR_INVALID, "null pointer");
     if (weights && weight_stride <= 0) return fail(POPKV_ERR_INVALID, "bad weight stride");
+    if (popkv::paged_chunk_plan(dtype, batch, q_heads, kv_heads, rows, max_tokens).places > (int64_t{1} << 30))
+        return fail(POPKV_ERR_UNSUPPORTED, "too many rows and tokens for one call");
     const int64_t es = static_cast<int64_t>(elem_size(dtype));
     const int64_t strides[] = {q_batch_stride, q_head_stride, q_row_stride, k_batch_stride,   k_head_stride,   k_row_stride,
                                v_batch_stride, v_head_stride, v_row_stride, out_batch_stride, out_head_stride, out_row_stride};

@@ -415,14 +415,24 @@ struct PagedChunk {
     int q_heads, fill;
     float* weights;
     int64_t weight_stride;
-    // with weights, for every (sequence, KV head) row_tiles times 32 rows: the
-    // query operands (paged_chunk_stored(dtype) * 8 KB a tile), factors and sums
-    int64_t row_tiles;
+    // of the plan; parts [batch, row_blocks]: first workgroup and number of parts
+    int shape, row_waves, groups, least, item_cost;
+    int64_t row_blocks;
+    int2* parts;
+    float* partials;
+    // with weights, for every (sequence, KV head) row_blocks * row_waves times 32
+    // rows: the query operands (plan.stored * 8 KB a tile), factors and sums
     uint4* queries;
     float *factors, *lse;
 };
-int64_t paged_chunk_stored(int dtype);
-int64_t paged_chunk_row_tiles(int64_t rows, int64_t group);
+// How a call is cut: waves of 32 rows a workgroup (shape), blocks of so many rows a
+// sequence, workgroups a KV head, the fewest tiles of tokens of one, what a block costs
+// beside its tiles, floats of partial states, stored operands of 32 rows.
+struct ChunkPlan {
+    int shape, groups, least, item_cost, stored;
+    int64_t row_blocks, states, places;
+};
+ChunkPlan paged_chunk_plan(int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t rows, int64_t max_tokens);
 hipError_t launch_paged_chunk(const PagedChunk& a, const PagedView& c, int64_t max_tokens, int dtype, int dim_group,
                               hipStream_t stream);
 

@@ -75,6 +75,23 @@ __device__ __forceinline__ void centred_pairs(const CodeBits& k, uint32_t w, hal
         out[i] = i & 1 ? __builtin_elementwise_fma(as_half2(b[i]), k16th, k72) : as_half2(b[i]) - k1032;
 }
 
+// The pairs of biased_pairs as c, and as low + c * delta.
+__device__ __forceinline__ void code_pairs(const CodeBits& k, uint32_t w, half2_t (&out)[4]) {
+    const half2_t k1024 = {1024.0f16, 1024.0f16}, k16th = {0.0625f16, 0.0625f16}, k64 = {-64.0f16, -64.0f16};
+    uint32_t b[4];
+    biased_pairs(k, w, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        out[i] = i & 1 ? __builtin_elementwise_fma(as_half2(b[i]), k16th, k64) : as_half2(b[i]) - k1024;
+}
+__device__ __forceinline__ void dequantise_pairs(const CodeBits& k, uint32_t w, half2_t delta, half2_t low,
+                                                 uint32_t (&out)[4]) {
+    half2_t code[4];
+    code_pairs(k, w, code);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(code[i], delta, low));
+}
+
 // ---- the merge --------------------------------------------------------------
 
 // Two neighbouring floats of a state (8-byte aligned), as ld_f32<true> and

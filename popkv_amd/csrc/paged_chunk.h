@@ -1,0 +1,1133 @@
+// Kernels of the chunk attention over the paged 4-bit K/V cache, instantiated for
+// each element type by a source of its own (paged_chunk_*.hip).
+#pragma once
+
+#include "paged_attention.h"
+
+namespace popkv {
+namespace {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+
+constexpr int kFrag = 1024;                   // bytes of one operand of a 32 x 32 x 16 product
+
+__device__ __forceinline__ f32x16_t mfma_h(const uint4& a, const uint4& b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0,
+                                                  0);
+}
+__device__ __forceinline__ f32x16_t mfma_b(const uint4& a, const uint4& b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
+                                                   0, 0);
+}
+
+// x as bf16 terms: the first `n` of x = b0 + b1 + b2 (b1, b2 zero where x is not finite).
+template <int N>
+__device__ __forceinline__ void bf16_terms(float x, uint32_t (&t)[N]) {
+    t[0] = bf16_rne(x);
+    float rest = x - bits_bf16(t[0]);
+    if ((t[0] & 0x7f80u) == 0x7f80u) rest = 0.0f;
+#pragma unroll
+    for (int i = 1; i < N; ++i) {
+        t[i] = bf16_rne(rest);
+        rest -= bits_bf16(t[i]);
+    }
+}
+
+// Whether one of eight elements is an infinity or NaN.
+template <typename T>
+__device__ __forceinline__ bool odd_values(const Raw8<T>& x) {
+    bool odd = false;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) odd = odd || (__float_as_uint(x.get(i)) & 0x7f800000u) == 0x7f800000u;
+    } else {
+        constexpr uint32_t kTop = Elem<T>::kDtype == POPKV_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        u16x2 m = __builtin_bit_cast(u16x2, x.u.x & 0x7fff7fffu);
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x.u.y & 0x7fff7fffu));
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x.u.z & 0x7fff7fffu));
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x.u.w & 0x7fff7fffu));
+        odd = max(m[0], m[1]) >= kTop;
+    }
+    return odd;
+}
+__device__ __forceinline__ bool is_odd(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+template <typename T>
+__device__ __forceinline__ void clear_odd(Raw8<T>& x) {
+    if constexpr (sizeof(T) == 4) {
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = is_odd(x.get(i)) ? 0.0f : x.get(i);
+        x.a = make_float4(y[0], y[1], y[2], y[3]);
+        x.b = make_float4(y[4], y[5], y[6], y[7]);
+    } else {
+        auto word = [&](uint32_t w, int i) {
+            return (is_odd(x.get(i)) ? 0u : w & 0xffffu) | (is_odd(x.get(i + 1)) ? 0u : w & 0xffff0000u);
+        };
+        x.u = make_uint4(word(x.u.x, 0), word(x.u.y, 2), word(x.u.z, 4), word(x.u.w, 6));
+    }
+}
+
+// What the kernel holds of each element type.  EXACT: cached keys enter the logits
+// unrounded (else in fp16).
+template <typename T, bool EXACT>
+struct ChunkTypes {
+    static constexpr bool F32 = std::is_same_v<T, float>;
+    static constexpr bool F16 = std::is_same_v<T, f16_t>;
+    static constexpr int QT = F32 ? 2 : 1;         // fp16 terms of the queries
+    static constexpr int KT = EXACT ? 2 : 1;       // of the cached keys
+    static constexpr int VT = F32 || F16 ? 2 : 1;  // of the cached values and their weights
+    static constexpr int NT = F32 ? 3 : 1;         // planes of the new tokens (fp32: bf16 terms)
+    static constexpr int PT = F32 ? 3 : 2;         // terms of the weights on new tokens
+    static constexpr int QPLANES = F32 ? 3 : 1;
+    static constexpr int STORED = QT + QPLANES;    // query operands kept for the second pass
+    static constexpr int PLANES = KT + VT > 2 * NT ? KT + VT : 2 * NT;
+};
+
+// Where lane l's sixteen bytes of value operand i of four lie in its KB: writers
+// of one instruction (16 dwords of codes) meet different banks, readers too.
+__device__ __forceinline__ int value_slot(int l, int i) { return (l ^ (i | ((l >> 4 & 1) << 3))) * 16; }
+
+// A workgroup's shape: WR waves of 32 rows (a row is a token and a head of the
+// group, heads innermost) times WT waves that share a tile's tokens.
+template <int WR_, int WT_>
+struct ChunkShape {
+    static constexpr int WR = WR_, WT = WT_, W = WR * WT, THREADS = W * kWave;
+    static constexpr int ROWS = 32 * WR;
+    static constexpr int TILE = WT == 4 ? 128 : 64, SUB = TILE / 32;  // tokens of a tile
+    static constexpr int UNITS = 4 * TILE;                            // quarters of keys, or dwords of four tokens' values
+    static constexpr bool ROLES = THREADS >= 2 * UNITS;               // half of the threads stage keys, half values
+    static constexpr int PER = ROLES ? 1 : UNITS / THREADS;
+    static constexpr int STATE = WR * (32 * 128 + 64);                // floats of a part's state
+};
+
+// Sequence b's chunk: its new tokens, cached tokens, and per tile of rows j the
+// tiles of both.
+struct ChunkSizes {
+    int rows, count;
+    __device__ __forceinline__ ChunkSizes(const PagedChunk& a, const PagedView& c, int64_t max_tokens, int b)
+        : rows(static_cast<int>(a.tokens ? clamp_count(a.tokens[b], a.rows) : a.rows)),
+          count(static_cast<int>(clamp_count(c.counts[b], min(c.width << c.page_log2, max_tokens)))) {}
+};
+
+struct ChunkPart {
+    int b, j, x0, x1, s, n, first;
+};
+
+// The work of one KV head is the batch's tiles of rows laid end to end, each as long
+// as its tiles of tokens, cut among the grid's workgroups by the real lengths, which
+// are read on the device.  Workgroup w's state of a tile of rows that goes on from
+// the workgroup before has place 2 w, of one that begins in it 2 w + 1.  Each wave
+// works its parts out by itself.
+template <typename S>
+struct ChunkWalk {
+    const PagedChunk& a;
+    const PagedView& c;
+    const int64_t most;
+    const int lane, w, items, group;
+    int per, r0, r1, i0, base;
+    int start, tiles;  // lane i: item i0 + i
+    uint64_t mask;
+
+    __device__ __forceinline__ ChunkWalk(const PagedChunk& a_, const PagedView& c_, int64_t max_tokens, int w_, int groups)
+        : a(a_), c(c_), most(max_tokens), lane(threadIdx.x & (kWave - 1)), w(w_),
+          items(c.batch * static_cast<int>(a.row_blocks)), group(a.q_heads / c.kv_heads), i0(0), base(0) {
+        int total = 0;
+        for (int i = 0; i < items; i += kWave)
+            total += __builtin_amdgcn_readlane(static_cast<int>(wave_incl_scan(static_cast<uint32_t>(cost(length(i + lane))), lane)),
+                                               kWave - 1);
+        per = max((total + groups - 1) / groups, a.least);
+        r0 = static_cast<int>(min<int64_t>(static_cast<int64_t>(w) * per, int64_t{1} << 30));
+        r1 = r0 + per;
+        find();
+    }
+    __device__ __forceinline__ int length(int i) const {
+        if (i >= items) return 0;
+        const int b = i / static_cast<int>(a.row_blocks), j = i - b * static_cast<int>(a.row_blocks);
+        const ChunkSizes z(a, c, most, b);
+        if (static_cast<int64_t>(j) * S::ROWS >= static_cast<int64_t>(z.rows) * group) return 0;
+        const int seen = static_cast<int>(min<int64_t>((static_cast<int64_t>(j + 1) * S::ROWS - 1) / group + 1, z.rows));
+        return (z.count + S::TILE - 1) / S::TILE + (seen + S::TILE - 1) / S::TILE;
+    }
+    __device__ __forceinline__ int cost(int n) const { return n > 0 ? n + a.item_cost : 0; }
+    __device__ __forceinline__ void find() {
+        tiles = length(i0 + lane);
+        const int n = static_cast<int>(wave_incl_scan(static_cast<uint32_t>(cost(tiles)), lane));
+        start = base + n - cost(tiles);
+        mask = __ballot(tiles > 0 && start < r1 && start + tiles > r0);
+        base += __builtin_amdgcn_readlane(n, kWave - 1);
+    }
+    __device__ __forceinline__ bool next(ChunkPart& p) {
+        while (mask == 0) {
+            i0 += kWave;
+            if (i0 >= items || base >= r1) return false;
+            find();
+        }
+        const int src = __ffsll(static_cast<unsigned long long>(mask)) - 1;
+        mask &= mask - 1;
+        const int from = __builtin_amdgcn_readlane(start, src), to = from + __builtin_amdgcn_readlane(tiles, src);
+        const int item = i0 + src;
+        p.b = item / static_cast<int>(a.row_blocks);
+        p.j = item - p.b * static_cast<int>(a.row_blocks);
+        const int w0 = from >= r0 ? w : from / per, w1 = to <= r1 ? w : (to - 1) / per;
+        p.s = w - w0;
+        p.n = w1 - w0 + 1;
+        p.first = w0;
+        p.x0 = max(from, r0) - from;
+        p.x1 = min(to, r1) - from;
+        return true;
+    }
+};
+
+// Sixteen neighbouring values of a row, times f.
+template <typename T>
+__device__ __forceinline__ void store16(T* p, const f32x16_t& x, float f) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 16; j += 4)
+            *reinterpret_cast<float4*>(p + j) = make_float4(x[j] * f, x[j + 1] * f, x[j + 2] * f, x[j + 3] * f);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; j += 8)
+            *reinterpret_cast<uint4*>(p + j) =
+                make_uint4(pack2<T>(x[j] * f, x[j + 1] * f), pack2<T>(x[j + 2] * f, x[j + 3] * f),
+                           pack2<T>(x[j + 4] * f, x[j + 5] * f), pack2<T>(x[j + 6] * f, x[j + 7] * f));
+    }
+}
+
+template <typename T, int G, bool EXACT, typename S>
+__global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, PagedView c, int64_t max_tokens, int groups) {
+    using C = ChunkTypes<T, EXACT>;
+    constexpr int R = 128 / G;
+    constexpr int LOWS = R == 8 ? 2 : 1;
+    constexpr int QTOP = 5;
+    constexpr float kBase = 8.0f, kNone = -3e38f, kFull = 65504.0f;
+    constexpr int PLANE = S::SUB * 8 * kFrag, BUF = C::PLANES * PLANE;
+    constexpr int BUFS = 2 * BUF <= 140 * 1024 ? 2 : 1;
+    static_assert(BUF <= 150 * 1024);
+    static_assert(S::WT == 1 || BUFS * BUF >= S::W / 2 * 16384 + 4096);
+    __shared__ __align__(16) unsigned char s_mem[BUFS * BUF];
+    __shared__ __align__(16) uint32_t s_scale[BUFS][EXACT ? S::TILE : 1][R];
+    __shared__ float s_bias[BUFS][S::TILE];
+    __shared__ int s_ragged[BUFS][S::W], s_odd_keys[BUFS][S::W];
+
+    const int h = blockIdx.x - div_nonneg(blockIdx.x, c.kv_heads) * c.kv_heads;
+    const int w_id = div_nonneg(blockIdx.x, c.kv_heads);
+    const int tid = threadIdx.x, lane = tid & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int wr = wave % S::WR, wt = wave / S::WR;
+    const int col = lane & 31, half = lane >> 5;
+    const int group = a.q_heads / c.kv_heads;
+
+    // rows behind a sequence's last one
+    if (a.fill && a.tokens)
+        for (int64_t i = blockIdx.x; i < static_cast<int64_t>(c.batch) * a.q_heads; i += gridDim.x) {
+            const int64_t b = i / a.q_heads;
+            T* const out = static_cast<T*>(a.out) + b * a.o_bs + (i - b * a.q_heads) * a.o_hs;
+            constexpr int V = 128 * sizeof(T) / 16;
+            for (int64_t k = clamp_count(a.tokens[b], a.rows) * V + tid; k < a.rows * V; k += S::THREADS)
+                reinterpret_cast<uint4*>(out + k / V * a.o_ts)[k % V] = make_uint4(0u, 0u, 0u, 0u);
+        }
+
+    // a thread's part of a tile: a quarter of a token's key, a dword of four tokens'
+    // values, which share a page
+    constexpr int VALUES_FROM = S::ROLES ? S::UNITS : 0;
+    const bool keys = !S::ROLES || wave < S::UNITS / kWave, vals = !S::ROLES || wave >= S::UNITS / kWave;
+    const int64_t per_page = static_cast<int64_t>(c.kv_heads) << c.page_log2;
+    const int64_t head_row = static_cast<int64_t>(h) << c.page_log2;
+    const int in_page = (1 << c.page_log2) - 1;
+    const CodeBits bits;
+    auto value_at = [&](unsigned char* base, int unit, int e) {  // dim e of the dword, the quad's eight bytes
+        const int dw = unit % 16, quad = unit / 16, u = quad / 8, s = quad % 8 / 4, r = quad % 4;
+        const int i = dw % 8 / 2, m = 8 * (2 * (dw % 2) + e / 4) + 4 * (dw / 8) + e % 4;
+        return reinterpret_cast<uint2*>(base + ((u * 2 + s) * 4 + i) * kFrag + value_slot((r & 1) * 32 + m, i) + 8 * (r >> 1));
+    };
+    auto key_at = [&](unsigned char* base, int unit, int e) {  // eight dims 32 quarter + 8 e
+        const int token = unit / 4, quarter = unit % 4;
+        return reinterpret_cast<uint4*>(base + (token / 32 * 8 + 4 * (quarter & 1) + e) * kFrag +
+                                        (quarter / 2 * 32 + token % 32) * 16);
+    };
+    auto ld16 = [&](const unsigned char* p) { return *reinterpret_cast<const uint4*>(p); };
+
+    ChunkWalk<S> walk(a, c, max_tokens, w_id, groups);
+    ChunkPart part;
+    while (walk.next(part)) {
+        const int b = part.b;
+        const ChunkSizes z(a, c, max_tokens, b);
+        const int rows = z.rows, count = z.count;
+        const int cached_tiles = (count + S::TILE - 1) / S::TILE;
+        const int64_t all = static_cast<int64_t>(rows) * group, row0 = static_cast<int64_t>(part.j) * S::ROWS;
+        const int64_t row = min<int64_t>(row0 + 32 * wr + col, all - 1);
+        const bool live_row = row0 + 32 * wr + col < all;
+        const int t_row = static_cast<int>(row / group);
+        const int head = h * group + static_cast<int>(row - static_cast<int64_t>(t_row) * group);
+        const T* const q_row = static_cast<const T*>(a.q) + b * a.q_bs + head * a.q_hs + static_cast<int64_t>(t_row) * a.q_ts + 64 * half;
+        // what the second pass reads of these rows: the query operands of both kinds of
+        // tokens, their factors, their sums
+        const int64_t row_tile = (static_cast<int64_t>(b) * c.kv_heads + h) * a.row_blocks * S::WR + part.j * S::WR + wr;
+        const bool store_rows = a.weights && part.s == 0 && wt == 0 && row0 + 32 * wr < all;
+
+        f32x16_t acc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
+        float ref = kNone, l = 0.0f;
+        uint4 q[C::QPLANES][8];
+
+        // Weights 2^(logit - ref) of 32 tokens from their products: lane's own row,
+        // tokens 8 (i / 4) + 4 half + i % 4.  They are kept below fp16's largest number:
+        // ref moves where one would pass it, and starts so that the first tile's largest
+        // is 2^kBase.
+        auto weights = [&](const f32x16_t& s, float f, float (&p)[16]) {
+            float sum = 0.0f;
+            auto exps = [&] {
+                sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) p[i] = exp2_fast(fmaf(s[i], f, -ref));
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sum += p[i];
+            };
+            exps();
+            if (__ballot(!(sum < kFull)) != 0) {
+                float mx = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i] * f);
+                mx = fmaxf(mx, lane_xor<32>(mx));
+                const float to = fmaxf(mx - kBase, ref), g = exp2_fast(ref - to);
+                l *= g;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) acc[i][j] *= g;
+                ref = to;
+                exps();
+            }
+            l += sum;
+        };
+
+        __syncthreads();  // nothing reads the last part's LDS any more
+        // ---- cached tokens
+        if (part.x0 < cached_tiles) {
+            uint4 ql[LOWS];
+            float factor;
+            {
+                Raw8<T> raw[8];
+#pragma unroll
+                for (int s = 0; s < 8; ++s) raw[s].load(q_row + 8 * s);
+                float top = 0.0f;
+#pragma unroll
+                for (int s = 0; s < 8; ++s)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(raw[s].get(i)));
+                top = fmaxf(top, lane_xor<32>(top));
+                const int e = static_cast<int>((__float_as_uint(top) >> 23) & 0xffu) - 127;
+                factor = ldexpf(kScaleHigh, e + 1 - QTOP);
+                float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // of this half's scale groups
+#pragma unroll
+                for (int s = 0; s < 8; ++s) {
+                    float x[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        x[i] = ldexpf(raw[s].get(i), QTOP - 1 - e);
+                        sums[8 * s / G] += x[i];
+                    }
+                    uint32_t w[4], rest[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        w[j] = pack_half2(x[j], x[j + 4]);
+                        rest[j] = pack_half2(x[j] - static_cast<float>(as_half2(w[j])[0]),
+                                             x[j + 4] - static_cast<float>(as_half2(w[j])[1]));
+                    }
+                    q[0][s] = make_uint4(w[0], w[1], w[2], w[3]);
+                    if constexpr (C::QT == 2) q[1][s] = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+                }
+                if constexpr (EXACT) {
+                    // sums of the queries, for the scales' low and 8 delta (what codes lack in c - 8)
+                    float qs[8];
+#pragma unroll
+                    for (int g = 0; g < 8; ++g) qs[g] = 0.0f;
+#pragma unroll
+                    for (int g = 0; g < R / 2; ++g) {
+                        const float other = lane_xor<32>(sums[g]);
+                        qs[g] = half == 0 ? sums[g] : other;
+                        qs[R / 2 + g] = half == 0 ? other : sums[g];
+                    }
+#pragma unroll
+                    for (int n = 0; n < LOWS; ++n) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            const float term = half == 0 ? qs[4 * n + g] : 8.0f * qs[4 * n + g];
+                            const float high = static_cast<float>(static_cast<_Float16>(term));
+                            w[g] = pack_half2(high, term - high);
+                        }
+                        ql[n] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                if (store_rows) {
+                    if (half == 0) a.factors[row_tile * 32 + col] = factor;
+#pragma unroll
+                    for (int n = 0; n < C::QT; ++n)
+#pragma unroll
+                        for (int s = 0; s < 8; ++s) a.queries[((row_tile * C::STORED + n) * 8 + s) * kWave + lane] = q[n][s];
+                }
+            }
+            uint4 xk[S::PER];
+            uint32_t xks[S::PER][2], xv[S::PER][4], xvs[S::PER][4];
+            bool key_there[S::PER];
+            auto load = [&](int tile) {
+#pragma unroll
+                for (int p = 0; p < S::PER; ++p) {
+                    const int unit = tid - (vals && S::ROLES ? VALUES_FROM : 0) + p * S::THREADS;
+                    const int t = tile * S::TILE + unit / 16 * 4;  // the quad of both
+                    int32_t e = -1;
+                    if (t < count) e = c.table[b * c.width + (t >> c.page_log2)];
+                    const bool there = static_cast<uint32_t>(e) < static_cast<uint32_t>(c.pages);
+                    const int64_t at = (there ? e : 0) * per_page + head_row + (t & in_page);
+                    if (keys) {
+                        const int quarter = unit % 4, k = unit / 4 % 4;
+                        xk[p] = *reinterpret_cast<const uint4*>(c.codes + (at + k) * kCodeRow + 16 * quarter);
+                        const uint32_t* sc = c.scales + (at + k) * (2 * R);
+                        key_there[p] = there && t + k < count;
+                        if constexpr (R == 8) {
+                            xks[p][0] = sc[2 * quarter];
+                            xks[p][1] = sc[2 * quarter + 1];
+                        } else {
+                            xks[p][0] = sc[R == 4 ? quarter : quarter / 2];
+                        }
+                        if (!key_there[p]) xks[p][0] = xks[p][1] = 0u;
+                    }
+                    if (vals) {
+                        const int dw = unit % 16;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            xv[p][j] = *reinterpret_cast<const uint32_t*>(c.codes + (at + j) * kCodeRow + 64 + 4 * dw);
+                            xvs[p][j] = c.scales[(at + j) * (2 * R) + R + 8 * dw / G];
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (!there || t + j >= count) xvs[p][j] = 0u;
+                    }
+                }
+            };
+            auto stage = [&](int buf) {
+                unsigned char* const s_k = s_mem + buf * BUF;
+                unsigned char* const s_v = s_k + C::KT * PLANE;
+                bool some = false;
+#pragma unroll
+                for (int p = 0; p < S::PER; ++p) {
+                    const int unit = tid - (vals && S::ROLES ? VALUES_FROM : 0) + p * S::THREADS;
+                    if (keys) {
+                        const int token = unit / 4, quarter = unit % 4;
+                        const uint32_t w[4] = {xk[p].x, xk[p].y, xk[p].z, xk[p].w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t sc = xks[p][R == 8 ? e / 2 : 0];
+                            const half2_t delta = as_half2(high_halves(sc, sc));
+                            if constexpr (EXACT) {
+                                const half2_t top7 = as_half2(__builtin_bit_cast(uint32_t, delta) & 0xfff0fff0u);
+                                const half2_t low4 = delta - top7;
+                                half2_t code[4];
+                                centred_pairs(bits, w[e], code);
+                                uint32_t hi[4], lo[4];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    hi[i] = __builtin_bit_cast(uint32_t, code[i] * top7);
+                                    lo[i] = __builtin_bit_cast(uint32_t, code[i] * low4);
+                                }
+                                *key_at(s_k, unit, e) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                                *key_at(s_k + PLANE, unit, e) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                            } else {
+                                uint32_t x[4];
+                                dequantise_pairs(bits, w[e], delta, as_half2(low_halves(sc, sc)), x);
+                                *key_at(s_k, unit, e) = make_uint4(x[0], x[1], x[2], x[3]);
+                            }
+                        }
+                        if constexpr (EXACT) {
+                            if constexpr (R == 8) {
+                                s_scale[buf][token][2 * quarter] = xks[p][0];
+                                s_scale[buf][token][2 * quarter + 1] = xks[p][1];
+                            } else if (R == 4 || quarter % 2 == 0) {
+                                s_scale[buf][token][R == 4 ? quarter : quarter / 2] = xks[p][0];
+                            }
+                        }
+                        if (quarter == 0) s_bias[buf][token] = key_there[p] ? 0.0f : 1.0f;
+                        some = some || !key_there[p];
+                    }
+                    if (vals) {
+                        uint32_t out[8][2], low[8][2];  // [dim][token pair]
+#pragma unroll
+                        for (int t2 = 0; t2 < 2; ++t2) {
+                            const uint32_t v0 = xv[p][2 * t2], v1 = xv[p][2 * t2 + 1];
+                            const half2_t delta = as_half2(high_halves(xvs[p][2 * t2], xvs[p][2 * t2 + 1]));
+                            const half2_t base = as_half2(low_halves(xvs[p][2 * t2], xvs[p][2 * t2 + 1]));
+#pragma unroll
+                            for (int hw = 0; hw < 2; ++hw) {
+                                const uint32_t w = hw ? high_halves(v0, v1) : low_halves(v0, v1);
+                                if constexpr (C::VT == 1) {
+                                    uint32_t x[4];
+                                    dequantise_pairs(bits, w, delta, base, x);
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) out[4 * hw + i][t2] = x[i];
+                                } else {
+                                    // low + code * delta to 22 bits
+                                    half2_t code[4];
+                                    code_pairs(bits, w, code);
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+                                        float y[2], rest[2];
+#pragma unroll
+                                        for (int k = 0; k < 2; ++k) {
+                                            y[k] = fmaf(static_cast<float>(code[i][k]), static_cast<float>(delta[k]),
+                                                        static_cast<float>(base[k]));
+                                            rest[k] = y[k] - static_cast<float>(static_cast<_Float16>(y[k]));
+                                        }
+                                        out[4 * hw + i][t2] = pack_half2(y[0], y[1]);
+                                        low[4 * hw + i][t2] = pack_half2(rest[0], rest[1]);
+                                    }
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            *value_at(s_v, unit, e) = make_uint2(out[e][0], out[e][1]);
+                            if constexpr (C::VT == 2) *value_at(s_v + PLANE, unit, e) = make_uint2(low[e][0], low[e][1]);
+                        }
+                    }
+                }
+                const bool any = __ballot(some) != 0;
+                if (lane == 0) s_ragged[buf][wave] = any ? 1 : 0;
+            };
+            auto fold = [&](int buf) {
+                const unsigned char* const s_k = s_mem + buf * BUF;
+                const unsigned char* const s_v = s_k + C::KT * PLANE;
+                int flags = 0;
+#pragma unroll
+                for (int i = 0; i < S::W; ++i) flags |= s_ragged[buf][i];
+                const bool ragged = __builtin_amdgcn_readfirstlane(flags) != 0;
+#pragma unroll
+                for (int uu = 0; uu < S::SUB / S::WT; ++uu) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    const int u = uu * S::WT + wt;
+                    f32x16_t s;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+                    if constexpr (EXACT) {
+                        const uint32_t pick = half == 0 ? 0x01000100u : 0x03020302u;
+#pragma unroll
+                        for (int n = 0; n < LOWS; ++n) {
+                            uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                            for (int g = 0; g < 4 && g < R; ++g) {
+                                const uint32_t sc = s_scale[buf][32 * u + col][4 * n + g];
+                                w[g] = __builtin_amdgcn_perm(sc, sc, pick);
+                            }
+                            s = mfma_h(make_uint4(w[0], w[1], w[2], w[3]), ql[n], s);
+                        }
+                    }
+#pragma unroll
+                    for (int st = 0; st < 8; ++st)
+#pragma unroll
+                        for (int kt = 0; kt < C::KT; ++kt) {
+                            const uint4 k = ld16(s_k + kt * PLANE + (u * 8 + st) * kFrag + lane * 16);
+#pragma unroll
+                            for (int qt = C::QT - 1; qt >= 0; --qt) s = mfma_h(k, q[qt][st], s);
+                        }
+                    if (ragged) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            s[i] = s_bias[buf][32 * u + 8 * (i / 4) + 4 * half + i % 4] != 0.0f ? -INFINITY : s[i];
+                    }
+                    float p[16];
+                    weights(s, factor, p);
+#pragma unroll
+                    for (int st = 0; st < 2; ++st) {
+                        uint32_t w[4], rest[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float p0 = p[8 * st + 2 * j], p1 = p[8 * st + 2 * j + 1];
+                            w[j] = pack_half2(p0, p1);
+                            if constexpr (C::VT == 2)
+                                rest[j] = pack_half2(p0 - static_cast<float>(as_half2(w[j])[0]),
+                                                     p1 - static_cast<float>(as_half2(w[j])[1]));
+                        }
+                        const uint4 ph = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const unsigned char* at = s_v + ((u * 2 + st) * 4 + i) * kFrag + value_slot(lane, i);
+                            const uint4 v = ld16(at);
+                            acc[i] = mfma_h(v, ph, acc[i]);
+                            if constexpr (C::VT == 2) {
+                                acc[i] = mfma_h(v, make_uint4(rest[0], rest[1], rest[2], rest[3]), acc[i]);
+                                acc[i] = mfma_h(ld16(at + PLANE), ph, acc[i]);
+                            }
+                        }
+                    }
+                }
+            };
+            const int x1 = min(part.x1, cached_tiles);
+            load(part.x0);
+            if constexpr (BUFS == 2) {
+                stage(0);
+                if (part.x0 + 1 < x1) load(part.x0 + 1);
+                __syncthreads();
+                for (int x = part.x0; x < x1; ++x) {
+                    const int buf = (x - part.x0) & 1;
+                    fold(buf);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (x + 1 < x1) stage(buf ^ 1);
+                    if (x + 2 < x1) load(x + 2);
+                    __syncthreads();
+                }
+            } else {
+                for (int x = part.x0; x < x1; ++x) {
+                    stage(0);
+                    if (x + 1 < x1) load(x + 1);
+                    __syncthreads();
+                    fold(0);
+                    __syncthreads();
+                }
+            }
+        }
+
+        // ---- the new tokens, in their own type (fp32: three bf16 terms)
+        if (store_rows || part.x1 > cached_tiles) {
+            Raw8<T> raw[8];
+#pragma unroll
+            for (int s = 0; s < 8; ++s) raw[s].load(q_row + 8 * s);
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                if constexpr (C::F32) {
+                    uint32_t t[8][3];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) bf16_terms<3>(raw[s].get(i), t[i]);
+#pragma unroll
+                    for (int n = 0; n < 3; ++n)
+                        q[n][s] = make_uint4(t[0][n] | t[1][n] << 16, t[2][n] | t[3][n] << 16, t[4][n] | t[5][n] << 16,
+                                             t[6][n] | t[7][n] << 16);
+                } else {
+                    q[0][s] = raw[s].u;
+                }
+            }
+            if (store_rows) {
+#pragma unroll
+                for (int n = 0; n < C::QPLANES; ++n)
+#pragma unroll
+                    for (int s = 0; s < 8; ++s) a.queries[((row_tile * C::STORED + C::QT + n) * 8 + s) * kWave + lane] = q[n][s];
+            }
+        }
+        if (part.x1 > cached_tiles) {
+            const T* const k_head = static_cast<const T*>(a.k) + b * a.k_bs + h * a.k_hs;
+            const T* const v_head = static_cast<const T*>(a.v) + b * a.v_bs + h * a.v_hs;
+            auto mfma_t = [&](const uint4& x, const uint4& y, f32x16_t z) {
+                if constexpr (C::F16) return mfma_h(x, y, z);
+                else return mfma_b(x, y, z);
+            };
+            Raw8<T> nk[S::PER][4], nv[S::PER][4];
+            auto load = [&](int tile) {
+#pragma unroll
+                for (int p = 0; p < S::PER; ++p) {
+                    const int unit = tid - (vals && S::ROLES ? VALUES_FROM : 0) + p * S::THREADS;
+                    if (keys) {
+                        const int t = tile * S::TILE + unit / 4;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            nk[p][e].load(k_head + static_cast<int64_t>(min(t, rows - 1)) * a.k_ts + 32 * (unit % 4) + 8 * e);
+                            if (t >= rows) nk[p][e].zero();
+                        }
+                    }
+                    if (vals) {
+                        const int t = tile * S::TILE + unit / 16 * 4;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            nv[p][j].load(v_head + static_cast<int64_t>(min(t + j, rows - 1)) * a.v_ts + 8 * (unit % 16));
+                            if (t + j >= rows) nv[p][j].zero();
+                        }
+                    }
+                }
+            };
+            auto stage = [&](int buf) {
+                unsigned char* const s_k = s_mem + buf * BUF;
+                unsigned char* const s_v = s_k + C::NT * PLANE;
+                bool odd = false, odd_key = false;
+#pragma unroll
+                for (int p = 0; p < S::PER; ++p) {
+                    const int unit = tid - (vals && S::ROLES ? VALUES_FROM : 0) + p * S::THREADS;
+                    if (keys) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if constexpr (C::F32) {
+                                odd_key = odd_key || odd_values<T>(nk[p][e]);
+                                uint32_t t[8][3];
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) bf16_terms<3>(nk[p][e].get(i), t[i]);
+#pragma unroll
+                                for (int n = 0; n < 3; ++n)
+                                    *key_at(s_k + n * PLANE, unit, e) = make_uint4(t[0][n] | t[1][n] << 16, t[2][n] | t[3][n] << 16,
+                                                                                   t[4][n] | t[5][n] << 16, t[6][n] | t[7][n] << 16);
+                            } else {
+                                *key_at(s_k, unit, e) = nk[p][e].u;
+                            }
+                        }
+                    }
+                    if (vals) {
+                        bool mine = false;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) mine = mine || odd_values<T>(nv[p][j]);
+                        odd = odd || mine;
+                        if (__ballot(mine) != 0) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) clear_odd<T>(nv[p][j]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            if constexpr (C::F32) {
+                                uint32_t t[4][3];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) bf16_terms<3>(nv[p][j].get(e), t[j]);
+#pragma unroll
+                                for (int n = 0; n < 3; ++n)
+                                    *value_at(s_v + n * PLANE, unit, e) = make_uint2(t[0][n] | t[1][n] << 16, t[2][n] | t[3][n] << 16);
+                            } else {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const uint4& x = nv[p][j].u;
+                                    w[j] = e < 2 ? x.x : e < 4 ? x.y : e < 6 ? x.z : x.w;
+                                }
+                                *value_at(s_v, unit, e) = e & 1 ? make_uint2(high_halves(w[0], w[1]), high_halves(w[2], w[3]))
+                                                                : make_uint2(low_halves(w[0], w[1]), low_halves(w[2], w[3]));
+                            }
+                        }
+                    }
+                }
+                const bool any = __ballot(odd) != 0, any_key = __ballot(odd_key) != 0;
+                if (lane == 0) {
+                    s_ragged[buf][wave] = any ? 1 : 0;
+                    s_odd_keys[buf][wave] = any_key ? 1 : 0;
+                }
+            };
+            // Infinite and NaN values: times a weight of zero they would reach rows that do
+            // not see their token, so the products take them as zero, and their dims of the
+            // rows that do see it get them here.
+            auto add_odd = [&](int first) {
+#pragma unroll 1
+                for (int t = first; t < min(first + 32, rows); ++t) {
+                    const T* v_row = v_head + static_cast<int64_t>(t) * a.v_ts + 64 * half;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        Raw8<T> v;
+                        v.load(v_row + 8 * i);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            acc[i / 2][8 * (i & 1) + j] += t <= t_row && is_odd(v.get(j)) ? v.get(j) : 0.0f;
+                    }
+                }
+            };
+            // Logits of fp32 keys with an infinite element: its product with the lower
+            // terms of a query is no part of the sum.
+            auto odd_logits = [&](int first, f32x16_t& s) {
+#pragma unroll 1
+                for (int t = 0; t < min(32, rows - first); ++t) {
+                    const T* k_row = k_head + static_cast<int64_t>(first + t) * a.k_ts + 64 * half;
+                    float dot = 0.0f;
+                    bool odd = false;
+#pragma unroll 1
+                    for (int i = 0; i < 8; ++i) {
+                        Raw8<T> k, x;
+                        k.load(k_row + 8 * i);
+                        x.load(q_row + 8 * i);
+                        odd = odd || odd_values<T>(k);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) dot = fmaf(x.get(j), k.get(j), dot);
+                    }
+                    if (__ballot(odd) == 0) continue;
+                    dot += lane_xor<32>(dot);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] = 8 * (i / 4) + 4 * half + i % 4 == t ? dot : s[i];
+                }
+            };
+            auto fold = [&](int tile, int buf) {
+                const unsigned char* const s_k = s_mem + buf * BUF;
+                const unsigned char* const s_v = s_k + C::NT * PLANE;
+                int flags = 0, key_flags = 0;
+#pragma unroll
+                for (int i = 0; i < S::W; ++i) {
+                    flags |= s_ragged[buf][i];
+                    if constexpr (C::F32) key_flags |= s_odd_keys[buf][i];
+                }
+#pragma unroll
+                for (int uu = 0; uu < S::SUB / S::WT; ++uu) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    const int u = uu * S::WT + wt;
+                    f32x16_t s;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+                    for (int st = 0; st < 8; ++st) {
+                        uint4 k[C::NT];
+#pragma unroll
+                        for (int n = 0; n < C::NT; ++n) k[n] = ld16(s_k + n * PLANE + (u * 8 + st) * kFrag + lane * 16);
+                        // the smallest products first
+#pragma unroll
+                        for (int n = C::NT - 1; n >= 0; --n)
+#pragma unroll
+                            for (int m = n; m >= 0; --m) s = mfma_t(k[m], q[n - m][st], s);
+                    }
+                    const int first = tile * S::TILE + 32 * u, t0 = first + 4 * half;
+                    if constexpr (C::F32)
+                        if (__builtin_amdgcn_readfirstlane(key_flags) != 0) odd_logits(first, s);
+                    // (tokens behind the chunk's last are ahead of every row)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] = t0 + 8 * (i / 4) + i % 4 <= t_row ? s[i] : -INFINITY;
+                    float p[16];
+                    weights(s, kScaleHigh, p);
+#pragma unroll
+                    for (int st = 0; st < 2; ++st) {
+                        uint4 pw[C::PT];
+                        uint32_t t[8][C::PT];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float y = p[8 * st + j];
+                            if constexpr (C::F16) {
+                                const _Float16 high = static_cast<_Float16>(y), low = static_cast<_Float16>(y - static_cast<float>(high));
+                                t[j][0] = __builtin_bit_cast(uint16_t, high);
+                                t[j][1] = __builtin_bit_cast(uint16_t, low);
+                            } else {
+                                bf16_terms<C::PT>(y, t[j]);
+                            }
+                        }
+#pragma unroll
+                        for (int n = 0; n < C::PT; ++n)
+                            pw[n] = make_uint4(t[0][n] | t[1][n] << 16, t[2][n] | t[3][n] << 16, t[4][n] | t[5][n] << 16,
+                                               t[6][n] | t[7][n] << 16);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const unsigned char* at = s_v + ((u * 2 + st) * 4 + i) * kFrag + value_slot(lane, i);
+#pragma unroll
+                            for (int n = 0; n < C::NT; ++n) {
+                                const uint4 v = ld16(at + n * PLANE);
+#pragma unroll
+                                for (int m = 0; m < C::PT; ++m)
+                                    if (n + m < 3) acc[i] = mfma_t(v, pw[m], acc[i]);
+                            }
+                        }
+                    }
+                    if (__builtin_amdgcn_readfirstlane(flags) != 0) add_odd(first);
+                }
+            };
+            const int x0 = max(part.x0 - cached_tiles, 0), x1 = part.x1 - cached_tiles;
+            load(x0);
+            if constexpr (BUFS == 2) {
+                stage(0);
+                if (x0 + 1 < x1) load(x0 + 1);
+                __syncthreads();
+                for (int x = x0; x < x1; ++x) {
+                    const int buf = (x - x0) & 1;
+                    fold(x, buf);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (x + 1 < x1) stage(buf ^ 1);
+                    if (x + 2 < x1) load(x + 2);
+                    __syncthreads();
+                }
+            } else {
+                for (int x = x0; x < x1; ++x) {
+                    stage(0);
+                    if (x + 1 < x1) load(x + 1);
+                    __syncthreads();
+                    fold(x, 0);
+                    __syncthreads();
+                }
+            }
+        }
+
+        l += lane_xor<32>(l);
+        // waves that shared the tokens: their states to the first of them, by halves
+        if constexpr (S::WT > 1) {
+#pragma unroll
+            for (int n = S::WT / 2; n >= 1; n /= 2) {
+                float* const at = reinterpret_cast<float*>(s_mem) + ((wt % n) * S::WR + wr) * 4096;
+                float* const ml = reinterpret_cast<float*>(s_mem) + S::W / 2 * 4096 + ((wt % n) * S::WR + wr) * 64;
+                if (wt >= n && wt < 2 * n) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        *reinterpret_cast<float4*>(at + (i * kWave + lane) * 4) =
+                            make_float4(acc[i / 4][4 * (i % 4)], acc[i / 4][4 * (i % 4) + 1], acc[i / 4][4 * (i % 4) + 2],
+                                        acc[i / 4][4 * (i % 4) + 3]);
+                    if (half == 0) {
+                        ml[col] = ref;
+                        ml[32 + col] = l;
+                    }
+                }
+                __syncthreads();
+                if (wt < n) {
+                    const float m2 = ml[col], l2 = ml[32 + col], mx = fmaxf(ref, m2);
+                    const float f = exp2_fast(ref - mx), g = exp2_fast(m2 - mx);
+                    l = fmaf(l, f, l2 * g);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float4 y = *reinterpret_cast<const float4*>(at + (i * kWave + lane) * 4);
+                        f32x16_t& x = acc[i / 4];
+                        const int j = 4 * (i % 4);
+                        x[j] = fmaf(x[j], f, y.x * g);
+                        x[j + 1] = fmaf(x[j + 1], f, y.y * g);
+                        x[j + 2] = fmaf(x[j + 2], f, y.z * g);
+                        x[j + 3] = fmaf(x[j + 3], f, y.w * g);
+                    }
+                    ref = mx;
+                }
+                __syncthreads();
+            }
+            if (wt > 0) continue;
+        }
+        if (part.n == 1) {
+            if (live_row) {
+                T* const out = static_cast<T*>(a.out) + b * a.o_bs + head * a.o_hs + static_cast<int64_t>(t_row) * a.o_ts + 64 * half;
+                const float f = 1.0f / l;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) store16<T>(out + 16 * i, acc[i], f);
+            }
+            // (rows past the last one weigh nothing)
+            if (store_rows && half == 0) a.lse[row_tile * 32 + col] = live_row ? ref + __log2f(l) : INFINITY;
+        } else {
+            float* const state = a.partials + ((2 * static_cast<int64_t>(w_id) + (part.s == 0 ? 1 : 0)) * c.kv_heads + h) * S::STATE +
+                                 wr * (4096 + 64);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                *reinterpret_cast<float4*>(state + (i * kWave + lane) * 4) = make_float4(
+                    acc[i / 4][4 * (i % 4)], acc[i / 4][4 * (i % 4) + 1], acc[i / 4][4 * (i % 4) + 2], acc[i / 4][4 * (i % 4) + 3]);
+            if (half == 0) {
+                state[4096 + col] = ref;
+                state[4096 + 32 + col] = l;
+            }
+        }
+        if (h == 0 && part.s == 0 && tid == 0) a.parts[b * a.row_blocks + part.j] = make_int2(part.first, part.n);
+    }
+}
+
+// Tiles of rows in several parts: a wave for 16 of each half's 64 dims.
+template <typename T, typename S>
+__global__ __launch_bounds__(256) void chunk_merge_kernel(PagedChunk a, PagedView c, int64_t max_tokens) {
+    const int h = blockIdx.y, b = blockIdx.z;
+    const int j = blockIdx.x / S::WR, wr = blockIdx.x % S::WR;
+    const int lane = threadIdx.x & (kWave - 1), col = lane & 31, half = lane >> 5;
+    const int i = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int group = a.q_heads / c.kv_heads;
+    const ChunkSizes z(a, c, max_tokens, b);
+    const int64_t all = static_cast<int64_t>(z.rows) * group, row = static_cast<int64_t>(j) * S::ROWS + 32 * wr + col;
+    if (row - col >= all) return;
+    const int2 parts = a.parts[b * a.row_blocks + j];
+    if (parts.y <= 1) return;
+    auto state = [&](int s) {
+        const int64_t place = 2 * static_cast<int64_t>(parts.x + s) + (s == 0 ? 1 : 0);
+        return a.partials + (place * c.kv_heads + h) * S::STATE + wr * (4096 + 64);
+    };
+    float m = -INFINITY, l = 0.0f;
+    for (int s = 0; s < parts.y; ++s) m = fmaxf(m, state(s)[4096 + col]);
+    f32x16_t acc;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) acc[k] = 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < parts.y; ++s) {
+        const float* p = state(s);
+        const float f = exp2_fast(p[4096 + col] - m);
+        l = fmaf(f, p[4096 + 32 + col], l);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float4 y = *reinterpret_cast<const float4*>(p + ((4 * i + k) * kWave + lane) * 4);
+            acc[4 * k] = fmaf(f, y.x, acc[4 * k]);
+            acc[4 * k + 1] = fmaf(f, y.y, acc[4 * k + 1]);
+            acc[4 * k + 2] = fmaf(f, y.z, acc[4 * k + 2]);
+            acc[4 * k + 3] = fmaf(f, y.w, acc[4 * k + 3]);
+        }
+    }
+    if (row < all) {
+        const int t_row = static_cast<int>(row / group);
+        const int head = h * group + static_cast<int>(row - static_cast<int64_t>(t_row) * group);
+        store16<T>(static_cast<T*>(a.out) + b * a.o_bs + head * a.o_hs + static_cast<int64_t>(t_row) * a.o_ts + 64 * half + 16 * i,
+                   acc, 1.0f / l);
+    }
+    if (a.weights && i == 0 && half == 0) {
+        const int64_t row_tile = (static_cast<int64_t>(b) * c.kv_heads + h) * a.row_blocks * S::WR + j * S::WR + wr;
+        a.lse[row_tile * 32 + col] = row < all ? m + __log2f(l) : INFINITY;
+    }
+}
+
+// The attention weights of 32 tokens of a KV head a wave, from the logits once
+// more and the rows' sums: keys stay in registers as two fp16 terms (fp32's 22
+// bits), every row's operands pass once.
+template <typename T, int G>
+__global__ __launch_bounds__(256) void chunk_weights_kernel(PagedChunk a, PagedView c, int64_t max_tokens) {
+    using C = ChunkTypes<T, true>;
+    constexpr int R = 128 / G;
+    const int b = blockIdx.z, h = blockIdx.y;
+    const int lane = threadIdx.x & (kWave - 1), col = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int group = a.q_heads / c.kv_heads;
+    const int rows = static_cast<int>(a.tokens ? clamp_count(a.tokens[b], a.rows) : a.rows);
+    const int count = static_cast<int>(clamp_count(c.counts[b], min(c.width << c.page_log2, max_tokens)));
+    const int cached_tiles = (count + 31) / 32, tile = blockIdx.x * 4 + wave;
+    const bool cached = tile < cached_tiles;
+    const int t0 = 32 * (cached ? tile : tile - cached_tiles);
+    if (rows == 0 || (!cached && t0 >= rows)) return;
+    const int64_t all = static_cast<int64_t>(rows) * group;
+    const int64_t base = (static_cast<int64_t>(b) * c.kv_heads + h) * (a.row_blocks * a.row_waves);
+    const int token = t0 + col;
+    uint4 k[C::F32 ? 3 : 2][8];
+    bool there = true, odd = false;
+    if (cached) {
+        const int32_t e = token < count ? c.table[b * c.width + (token >> c.page_log2)] : -1;
+        there = static_cast<uint32_t>(e) < static_cast<uint32_t>(c.pages);
+        const int64_t at = (there ? e : 0) * (static_cast<int64_t>(c.kv_heads) << c.page_log2) +
+                           (static_cast<int64_t>(h) << c.page_log2) + (token & ((1 << c.page_log2) - 1));
+        const uint4* codes = reinterpret_cast<const uint4*>(c.codes + at * kCodeRow + 32 * half);
+        const uint4 w0 = codes[0], w1 = codes[1];
+        const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            const uint32_t sc = c.scales[at * (2 * R) + (64 * half + 8 * s) / G];
+            float code[8], x[8], y[8];
+            codes8(w[s], code);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = fmaf(code[i], f16_hi(sc), f16_lo(sc));
+                y[i] = x[i] - static_cast<float>(static_cast<_Float16>(x[i]));
+            }
+            k[0][s] = make_uint4(pack_half2(x[0], x[4]), pack_half2(x[1], x[5]), pack_half2(x[2], x[6]), pack_half2(x[3], x[7]));
+            k[1][s] = make_uint4(pack_half2(y[0], y[4]), pack_half2(y[1], y[5]), pack_half2(y[2], y[6]), pack_half2(y[3], y[7]));
+        }
+    } else {
+        const T* k_row = static_cast<const T*>(a.k) + b * a.k_bs + h * a.k_hs + static_cast<int64_t>(min(token, rows - 1)) * a.k_ts;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            Raw8<T> raw;
+            raw.load(k_row + 64 * half + 8 * s);
+            if constexpr (C::F32) {
+                odd = odd || odd_values<T>(raw);
+                uint32_t t[8][3];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) bf16_terms<3>(raw.get(i), t[i]);
+#pragma unroll
+                for (int n = 0; n < 3; ++n)
+                    k[n][s] = make_uint4(t[0][n] | t[1][n] << 16, t[2][n] | t[3][n] << 16, t[4][n] | t[5][n] << 16,
+                                         t[6][n] | t[7][n] << 16);
+            } else {
+                k[0][s] = raw.u;
+            }
+        }
+    }
+    // (the parts of an infinite fp32 key's products are no sum: its logit is minus
+    // infinity or makes the row NaN)
+    if constexpr (C::F32) odd = odd || lane_xor<32>(odd ? 1.0f : 0.0f) != 0.0f;
+    float sum = 0.0f;
+    const int64_t first_row = cached ? 0 : static_cast<int64_t>(t0) * group;
+    const int64_t own_first = cached ? 0 : static_cast<int64_t>(token) * group;  // the first row that sees the token
+    for (int64_t r0 = first_row / 32 * 32; r0 < all; r0 += 32) {
+        const uint4* q = a.queries + (base + r0 / 32) * (C::STORED * 8 * kWave) + lane;
+        f32x16_t s;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+        if (cached) {
+#pragma unroll
+            for (int st = 0; st < 8; ++st)
+#pragma unroll
+                for (int qt = C::QT - 1; qt >= 0; --qt) {
+                    const uint4 x = q[(qt * 8 + st) * kWave];
+                    s = mfma_h(x, k[1][st], s);
+                    s = mfma_h(x, k[0][st], s);
+                }
+        } else {
+#pragma unroll
+            for (int st = 0; st < 8; ++st) {
+                uint4 x[C::QPLANES];
+#pragma unroll
+                for (int n = 0; n < C::QPLANES; ++n) x[n] = q[((C::QT + n) * 8 + st) * kWave];
+#pragma unroll
+                for (int n = C::QPLANES - 1; n >= 0; --n)
+#pragma unroll
+                    for (int m = n; m >= 0; --m) {
+                        if constexpr (C::F16) s = mfma_h(x[m], k[n - m][st], s);
+                        else s = mfma_b(x[m], k[n - m][st], s);
+                    }
+            }
+        }
+        const float4* lse = reinterpret_cast<const float4*>(a.lse + (base * 32 + r0) + 4 * half);
+        const float4* factors = reinterpret_cast<const float4*>(a.factors + (base * 32 + r0) + 4 * half);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 off = lse[2 * i];
+            float4 f = make_float4(kScaleHigh, kScaleHigh, kScaleHigh, kScaleHigh);
+            if (cached) f = factors[2 * i];
+            const int64_t r = r0 + 8 * i + 4 * half;
+            if constexpr (C::F32)
+                if (odd)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[4 * i + j] = -INFINITY;
+            sum += r >= own_first ? exp2_fast(fmaf(s[4 * i], f.x, -off.x)) : 0.0f;
+            sum += r + 1 >= own_first ? exp2_fast(fmaf(s[4 * i + 1], f.y, -off.y)) : 0.0f;
+            sum += r + 2 >= own_first ? exp2_fast(fmaf(s[4 * i + 2], f.z, -off.z)) : 0.0f;
+            sum += r + 3 >= own_first ? exp2_fast(fmaf(s[4 * i + 3], f.w, -off.w)) : 0.0f;
+        }
+    }
+    sum += lane_xor<32>(sum);
+    const int64_t at = cached ? token : static_cast<int64_t>(count) + token;
+    if (half == 0 && there && (cached || token < rows) && at < a.weight_stride)
+        a.weights[(static_cast<int64_t>(b) * c.kv_heads + h) * a.weight_stride + at] += sum;
+}
+
+template <typename T, int G, bool EXACT, typename S>
+hipError_t launch_chunk_s(const PagedChunk& a, const PagedView& c, int64_t max_tokens, hipStream_t stream) {
+    hipLaunchKernelGGL((paged_chunk_kernel<T, G, EXACT, S>), dim3(static_cast<unsigned>(a.groups * c.kv_heads)),
+                       dim3(S::THREADS), 0, stream, a, c, max_tokens, a.groups);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && a.groups > 1) {
+        hipLaunchKernelGGL((chunk_merge_kernel<T, S>), dim3(static_cast<unsigned>(a.row_blocks * S::WR), c.kv_heads, c.batch),
+                           dim3(256), 0, stream, a, c, max_tokens);
+        e = hipGetLastError();
+    }
+    return e;
+}
+
+template <typename T, int G, bool EXACT>
+hipError_t launch_chunk_e(const PagedChunk& a, const PagedView& c, int64_t max_tokens, hipStream_t stream) {
+    switch (a.shape) {
+        case 1:
+            if constexpr (!std::is_same_v<T, float>)
+                return launch_chunk_s<T, G, EXACT, ChunkShape<1, 4>>(a, c, max_tokens, stream);
+        case 2: return launch_chunk_s<T, G, EXACT, ChunkShape<2, 2>>(a, c, max_tokens, stream);
+        case 8:
+            if constexpr (!std::is_same_v<T, float>)
+                return launch_chunk_s<T, G, EXACT, ChunkShape<8, 1>>(a, c, max_tokens, stream);
+        default: return launch_chunk_s<T, G, EXACT, ChunkShape<4, 1>>(a, c, max_tokens, stream);
+    }
+}
+
+template <typename T, int G>
+hipError_t launch_chunk_t(const PagedChunk& a, const PagedView& c, int64_t max_tokens, hipStream_t stream) {
+    hipError_t e;
+    if constexpr (std::is_same_v<T, bf16_t>) {
+        e = a.weights ? launch_chunk_e<T, G, true>(a, c, max_tokens, stream)
+                      : launch_chunk_e<T, G, false>(a, c, max_tokens, stream);
+    } else {
+        e = launch_chunk_e<T, G, true>(a, c, max_tokens, stream);
+    }
+    if (e != hipSuccess || !a.weights) return e;
+    const int64_t most = min(max_tokens, c.width << c.page_log2);
+    const unsigned blocks = static_cast<unsigned>(((most + 31) / 32 + (a.rows + 31) / 32 + 3) / 4);
+    hipLaunchKernelGGL((chunk_weights_kernel<T, G>), dim3(blocks, c.kv_heads, c.batch), dim3(256), 0, stream, a, c, max_tokens);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_chunk(const PagedChunk& a, const PagedView& c, int64_t max_tokens, int dim_group, hipStream_t stream) {
+    switch (dim_group) {
+        case 16: return launch_chunk_t<T, 16>(a, c, max_tokens, stream);
+        case 32: return launch_chunk_t<T, 32>(a, c, max_tokens, stream);
+        default: return launch_chunk_t<T, 64>(a, c, max_tokens, stream);
+    }
+}
+
+}  // namespace
+}  // namespace popkv

@@ -1,0 +1,11 @@
+// The chunk attention's kernels in bf16.
+#include "paged_chunk.h"
+
+namespace popkv {
+
+hipError_t launch_paged_chunk_bf16(const PagedChunk& a, const PagedView& c, int64_t max_tokens, int dim_group,
+                                 hipStream_t stream) {
+    return launch_chunk<bf16_t>(a, c, max_tokens, dim_group, stream);
+}
+
+}  // namespace popkv
