@@ -21,17 +21,28 @@ __device__ __forceinline__ f32x16_t mfma_b(const uint4& a, const uint4& b, f32x1
                                                    0, 0);
 }
 
-// x as bf16 terms: the first `n` of x = b0 + b1 + b2 (b1, b2 zero where x is not finite).
+// Two floats as N pairs of bf16 terms that add up to them (the lower ones zero
+// where a float is not finite).
+typedef __bf16 bf16x2_raw __attribute__((ext_vector_type(2)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 template <int N>
-__device__ __forceinline__ void bf16_terms(float x, uint32_t (&t)[N]) {
-    t[0] = bf16_rne(x);
-    float rest = x - bits_bf16(t[0]);
-    if ((t[0] & 0x7f80u) == 0x7f80u) rest = 0.0f;
+__device__ __forceinline__ void bf16_terms(float x, float y, uint32_t (&t)[N]) {
+    t[0] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{x, y}), bf16x2_raw));
 #pragma unroll
     for (int i = 1; i < N; ++i) {
-        t[i] = bf16_rne(rest);
-        rest -= bits_bf16(t[i]);
+        x = i == 1 && (t[0] & 0x7f80u) == 0x7f80u ? 0.0f : x - __uint_as_float(t[i - 1] << 16);
+        y = i == 1 && (t[0] & 0x7f800000u) == 0x7f800000u ? 0.0f : y - __uint_as_float(t[i - 1] & 0xffff0000u);
+        t[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{x, y}), bf16x2_raw));
     }
+}
+// Eight elements of an operand.
+template <int N, typename F>
+__device__ __forceinline__ void bf16_operand(F&& x, uint4 (&q)[N]) {
+    uint32_t t[4][N];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bf16_terms<N>(x(2 * j), x(2 * j + 1), t[j]);
+#pragma unroll
+    for (int n = 0; n < N; ++n) q[n] = make_uint4(t[0][n], t[1][n], t[2][n], t[3][n]);
 }
 
 // Whether one of eight elements is an infinity or NaN.
@@ -307,6 +318,19 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
             l += sum;
         };
 
+        // eight of them as an operand, in two fp16 terms
+        auto half_terms = [&](const float (&p)[16], int first, uint4& high, uint4& low) {
+            uint32_t w[4], rest[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float p0 = p[first + 2 * j], p1 = p[first + 2 * j + 1];
+                w[j] = pack_half2(p0, p1);
+                rest[j] = pack_half2(p0 - static_cast<float>(as_half2(w[j])[0]), p1 - static_cast<float>(as_half2(w[j])[1]));
+            }
+            high = make_uint4(w[0], w[1], w[2], w[3]);
+            low = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+        };
+
         __syncthreads();  // nothing reads the last part's LDS any more
         // ---- cached tokens
         if (part.x0 < cached_tiles) {
@@ -377,13 +401,22 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
             uint4 xk[S::PER];
             uint32_t xks[S::PER][2], xv[S::PER][4], xvs[S::PER][4];
             bool key_there[S::PER];
-            auto load = [&](int tile) {
+            // (a tile's page entries are on their way while the one before is loaded)
+            int32_t entry[S::PER];
+            auto find = [&](int tile) {
 #pragma unroll
                 for (int p = 0; p < S::PER; ++p) {
                     const int unit = tid - (vals && S::ROLES ? VALUES_FROM : 0) + p * S::THREADS;
                     const int t = tile * S::TILE + unit / 16 * 4;  // the quad of both
-                    int32_t e = -1;
-                    if (t < count) e = c.table[b * c.width + (t >> c.page_log2)];
+                    entry[p] = t < count ? c.table[b * c.width + (t >> c.page_log2)] : -1;
+                }
+            };
+            auto load = [&](int tile) {
+#pragma unroll
+                for (int p = 0; p < S::PER; ++p) {
+                    const int unit = tid - (vals && S::ROLES ? VALUES_FROM : 0) + p * S::THREADS;
+                    const int t = tile * S::TILE + unit / 16 * 4;
+                    const int32_t e = entry[p];
                     const bool there = static_cast<uint32_t>(e) < static_cast<uint32_t>(c.pages);
                     const int64_t at = (there ? e : 0) * per_page + head_row + (t & in_page);
                     if (keys) {
@@ -544,23 +577,15 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                     weights(s, factor, p);
 #pragma unroll
                     for (int st = 0; st < 2; ++st) {
-                        uint32_t w[4], rest[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float p0 = p[8 * st + 2 * j], p1 = p[8 * st + 2 * j + 1];
-                            w[j] = pack_half2(p0, p1);
-                            if constexpr (C::VT == 2)
-                                rest[j] = pack_half2(p0 - static_cast<float>(as_half2(w[j])[0]),
-                                                     p1 - static_cast<float>(as_half2(w[j])[1]));
-                        }
-                        const uint4 ph = make_uint4(w[0], w[1], w[2], w[3]);
+                        uint4 ph, pl;
+                        half_terms(p, 8 * st, ph, pl);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const unsigned char* at = s_v + ((u * 2 + st) * 4 + i) * kFrag + value_slot(lane, i);
                             const uint4 v = ld16(at);
                             acc[i] = mfma_h(v, ph, acc[i]);
                             if constexpr (C::VT == 2) {
-                                acc[i] = mfma_h(v, make_uint4(rest[0], rest[1], rest[2], rest[3]), acc[i]);
+                                acc[i] = mfma_h(v, pl, acc[i]);
                                 acc[i] = mfma_h(ld16(at + PLANE), ph, acc[i]);
                             }
                         }
@@ -568,10 +593,13 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                 }
             };
             const int x1 = min(part.x1, cached_tiles);
+            find(part.x0);
             load(part.x0);
+            find(part.x0 + 1);
             if constexpr (BUFS == 2) {
                 stage(0);
                 if (part.x0 + 1 < x1) load(part.x0 + 1);
+                find(part.x0 + 2);
                 __syncthreads();
                 for (int x = part.x0; x < x1; ++x) {
                     const int buf = (x - part.x0) & 1;
@@ -579,12 +607,14 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                     __builtin_amdgcn_sched_barrier(0);
                     if (x + 1 < x1) stage(buf ^ 1);
                     if (x + 2 < x1) load(x + 2);
+                    find(x + 3);
                     __syncthreads();
                 }
             } else {
                 for (int x = part.x0; x < x1; ++x) {
                     stage(0);
                     if (x + 1 < x1) load(x + 1);
+                    find(x + 2);
                     __syncthreads();
                     fold(0);
                     __syncthreads();
@@ -600,13 +630,10 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
 #pragma unroll
             for (int s = 0; s < 8; ++s) {
                 if constexpr (C::F32) {
-                    uint32_t t[8][3];
+                    uint4 t[3];
+                    bf16_operand<3>([&](int i) { return raw[s].get(i); }, t);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) bf16_terms<3>(raw[s].get(i), t[i]);
-#pragma unroll
-                    for (int n = 0; n < 3; ++n)
-                        q[n][s] = make_uint4(t[0][n] | t[1][n] << 16, t[2][n] | t[3][n] << 16, t[4][n] | t[5][n] << 16,
-                                             t[6][n] | t[7][n] << 16);
+                    for (int n = 0; n < 3; ++n) q[n][s] = t[n];
                 } else {
                     q[0][s] = raw[s].u;
                 }
@@ -660,13 +687,10 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                         for (int e = 0; e < 4; ++e) {
                             if constexpr (C::F32) {
                                 odd_key = odd_key || odd_values<T>(nk[p][e]);
-                                uint32_t t[8][3];
+                                uint4 t[3];
+                                bf16_operand<3>([&](int i) { return nk[p][e].get(i); }, t);
 #pragma unroll
-                                for (int i = 0; i < 8; ++i) bf16_terms<3>(nk[p][e].get(i), t[i]);
-#pragma unroll
-                                for (int n = 0; n < 3; ++n)
-                                    *key_at(s_k + n * PLANE, unit, e) = make_uint4(t[0][n] | t[1][n] << 16, t[2][n] | t[3][n] << 16,
-                                                                                   t[4][n] | t[5][n] << 16, t[6][n] | t[7][n] << 16);
+                                for (int n = 0; n < 3; ++n) *key_at(s_k + n * PLANE, unit, e) = t[n];
                             } else {
                                 *key_at(s_k, unit, e) = nk[p][e].u;
                             }
@@ -684,12 +708,11 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             if constexpr (C::F32) {
-                                uint32_t t[4][3];
+                                uint32_t t[2][3];
+                                bf16_terms<3>(nv[p][0].get(e), nv[p][1].get(e), t[0]);
+                                bf16_terms<3>(nv[p][2].get(e), nv[p][3].get(e), t[1]);
 #pragma unroll
-                                for (int j = 0; j < 4; ++j) bf16_terms<3>(nv[p][j].get(e), t[j]);
-#pragma unroll
-                                for (int n = 0; n < 3; ++n)
-                                    *value_at(s_v + n * PLANE, unit, e) = make_uint2(t[0][n] | t[1][n] << 16, t[2][n] | t[3][n] << 16);
+                                for (int n = 0; n < 3; ++n) *value_at(s_v + n * PLANE, unit, e) = make_uint2(t[0][n], t[1][n]);
                             } else {
                                 uint32_t w[4];
 #pragma unroll
@@ -749,6 +772,7 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                     for (int i = 0; i < 16; ++i) s[i] = 8 * (i / 4) + 4 * half + i % 4 == t ? dot : s[i];
                 }
             };
+            int t_first = 0, t_last = 0;
             auto fold = [&](int tile, int buf) {
                 const unsigned char* const s_k = s_mem + buf * BUF;
                 const unsigned char* const s_v = s_k + C::NT * PLANE;
@@ -762,6 +786,7 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                 for (int uu = 0; uu < S::SUB / S::WT; ++uu) {
                     __builtin_amdgcn_sched_barrier(0);
                     const int u = uu * S::WT + wt;
+                    if (tile * S::TILE + 32 * u > t_last) continue;
                     f32x16_t s;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[i] = 0.0f;
@@ -780,6 +805,7 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                     if constexpr (C::F32)
                         if (__builtin_amdgcn_readfirstlane(key_flags) != 0) odd_logits(first, s);
                     // (tokens behind the chunk's last are ahead of every row)
+                    if (first + 31 > t_first)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[i] = t0 + 8 * (i / 4) + i % 4 <= t_row ? s[i] : -INFINITY;
                     float p[16];
@@ -787,22 +813,8 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
 #pragma unroll
                     for (int st = 0; st < 2; ++st) {
                         uint4 pw[C::PT];
-                        uint32_t t[8][C::PT];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float y = p[8 * st + j];
-                            if constexpr (C::F16) {
-                                const _Float16 high = static_cast<_Float16>(y), low = static_cast<_Float16>(y - static_cast<float>(high));
-                                t[j][0] = __builtin_bit_cast(uint16_t, high);
-                                t[j][1] = __builtin_bit_cast(uint16_t, low);
-                            } else {
-                                bf16_terms<C::PT>(y, t[j]);
-                            }
-                        }
-#pragma unroll
-                        for (int n = 0; n < C::PT; ++n)
-                            pw[n] = make_uint4(t[0][n] | t[1][n] << 16, t[2][n] | t[3][n] << 16, t[4][n] | t[5][n] << 16,
-                                               t[6][n] | t[7][n] << 16);
+                        if constexpr (C::F16) half_terms(p, 8 * st, pw[0], pw[1]);
+                        else bf16_operand<C::PT>([&](int j) { return p[8 * st + j]; }, pw);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const unsigned char* at = s_v + ((u * 2 + st) * 4 + i) * kFrag + value_slot(lane, i);
@@ -819,6 +831,9 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                 }
             };
             const int x0 = max(part.x0 - cached_tiles, 0), x1 = part.x1 - cached_tiles;
+            // (of the wave's rows)
+            t_first = __builtin_amdgcn_readfirstlane(t_row);
+            t_last = __builtin_amdgcn_readlane(t_row, 31);
             load(x0);
             if constexpr (BUFS == 2) {
                 stage(0);
@@ -1006,13 +1021,10 @@ __global__ __launch_bounds__(256) void chunk_weights_kernel(PagedChunk a, PagedV
             raw.load(k_row + 64 * half + 8 * s);
             if constexpr (C::F32) {
                 odd = odd || odd_values<T>(raw);
-                uint32_t t[8][3];
+                uint4 t[3];
+                bf16_operand<3>([&](int i) { return raw.get(i); }, t);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) bf16_terms<3>(raw.get(i), t[i]);
-#pragma unroll
-                for (int n = 0; n < 3; ++n)
-                    k[n][s] = make_uint4(t[0][n] | t[1][n] << 16, t[2][n] | t[3][n] << 16, t[4][n] | t[5][n] << 16,
-                                         t[6][n] | t[7][n] << 16);
+                for (int n = 0; n < 3; ++n) k[n][s] = t[n];
             } else {
                 k[0][s] = raw.u;
             }
