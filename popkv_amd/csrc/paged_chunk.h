@@ -191,6 +191,84 @@ struct ChunkWalk {
     }
 };
 
+// Weights of 32 tokens as operands of two products of 16 tokens each, in N terms of a
+// type (QK, PV: the products of an operand beside them).  SUM: their sum is the rounded ones' (two a step).
+template <int N, bool SUM_, int QK_>
+struct HalfWeights {
+    static constexpr bool SUM = SUM_;
+    static constexpr int QK = QK_, PV = N;
+    uint4 at[N][2];
+    __device__ __forceinline__ void pack(const float (&p)[16]) {
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+            uint32_t w[4], rest[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float p0 = p[8 * st + 2 * j], p1 = p[8 * st + 2 * j + 1];
+                w[j] = pack_half2(p0, p1);
+                rest[j] = pack_half2(p0 - static_cast<float>(as_half2(w[j])[0]), p1 - static_cast<float>(as_half2(w[j])[1]));
+            }
+            at[0][st] = make_uint4(w[0], w[1], w[2], w[3]);
+            if constexpr (N == 2) at[1][st] = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+        }
+    }
+    // of the first terms
+    __device__ __forceinline__ float sum() const {
+        const half2_t one = {1.0f16, 1.0f16};
+        float x = 0.0f;
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+            x = __builtin_amdgcn_fdot2(as_half2(at[0][st].x), one, x, false);
+            x = __builtin_amdgcn_fdot2(as_half2(at[0][st].y), one, x, false);
+            x = __builtin_amdgcn_fdot2(as_half2(at[0][st].z), one, x, false);
+            x = __builtin_amdgcn_fdot2(as_half2(at[0][st].w), one, x, false);
+        }
+        return x;
+    }
+};
+template <int N, int QK_>
+struct Bf16Weights {
+    static constexpr bool SUM = false;
+    static constexpr int QK = QK_, PV = N;
+    uint4 at[N][2];
+    __device__ __forceinline__ void pack(const float (&p)[16]) {
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+            uint4 t[N];
+            bf16_operand<N>([&](int j) { return p[8 * st + j]; }, t);
+#pragma unroll
+            for (int n = 0; n < N; ++n) at[n][st] = t[n];
+        }
+    }
+};
+
+// Eight operands of products, four of them read ahead: products(at, product) calls
+// product(i, operand) with the sixteen bytes at(i), i = 0 .. 7.
+template <typename A, typename F>
+__device__ __forceinline__ void products(A&& at, F&& product) {
+    uint4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const uint4*>(at(i));
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        product(i, x[i % 4]);
+        if (i < 4) x[i] = *reinterpret_cast<const uint4*>(at(i + 4));
+    }
+}
+// For the scheduler, of such products and other work: M products an operand, V vector
+// instructions and E exponentials behind each.
+template <int M, int V, int E>
+__device__ __forceinline__ void interleave() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, V, 0);
+        if (E) __builtin_amdgcn_sched_group_barrier(0x400, E, 0);
+        if (i < 4) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+}
+
 // Sixteen neighbouring values of a row, times f.
 template <typename T>
 __device__ __forceinline__ void store16(T* p, const f32x16_t& x, float f) {
@@ -208,17 +286,17 @@ __device__ __forceinline__ void store16(T* p, const f32x16_t& x, float f) {
 }
 
 template <typename T, int G, bool EXACT, typename S>
-__global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, PagedView c, int64_t max_tokens, int groups) {
+__global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_chunk_kernel(PagedChunk a, PagedView c, int64_t max_tokens, int groups) {
     using C = ChunkTypes<T, EXACT>;
     constexpr int R = 128 / G;
     constexpr int LOWS = R == 8 ? 2 : 1;
     constexpr int QTOP = 5;
     constexpr float kBase = 8.0f, kNone = -3e38f, kFull = 65504.0f;
     constexpr int PLANE = S::SUB * 8 * kFrag, BUF = C::PLANES * PLANE;
-    constexpr int BUFS = 2 * BUF <= 140 * 1024 ? 2 : 1;
+    constexpr int BUFS = S::WR == 8 && 2 * BUF <= 140 * 1024 ? 2 : 1;
     static_assert(BUF <= 150 * 1024);
-    static_assert(S::WT == 1 || BUFS * BUF >= S::W / 2 * 16384 + 4096);
-    __shared__ __align__(16) unsigned char s_mem[BUFS * BUF];
+    constexpr int JOIN = S::WT == 1 ? 0 : S::W / 2 * (16384 + 256);  // half of the waves' states
+    __shared__ __align__(16) unsigned char s_mem[BUFS * BUF > JOIN ? BUFS * BUF : JOIN];
     __shared__ __align__(16) uint32_t s_scale[BUFS][EXACT ? S::TILE : 1][R];
     __shared__ float s_bias[BUFS][S::TILE];
     __shared__ int s_ragged[BUFS][S::W], s_odd_keys[BUFS][S::W];
@@ -249,10 +327,14 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
     const int64_t head_row = static_cast<int64_t>(h) << c.page_log2;
     const int in_page = (1 << c.page_log2) - 1;
     const CodeBits bits;
-    auto value_at = [&](unsigned char* base, int unit, int e) {  // dim e of the dword, the quad's eight bytes
+    // where dim 0 of a unit's dword goes, its quad's eight bytes; dim e at value_dim(, e)
+    auto value_at = [&](int unit) {
         const int dw = unit % 16, quad = unit / 16, u = quad / 8, s = quad % 8 / 4, r = quad % 4;
-        const int i = dw % 8 / 2, m = 8 * (2 * (dw % 2) + e / 4) + 4 * (dw / 8) + e % 4;
-        return reinterpret_cast<uint2*>(base + ((u * 2 + s) * 4 + i) * kFrag + value_slot((r & 1) * 32 + m, i) + 8 * (r >> 1));
+        const int i = dw % 8 / 2, m = 16 * (dw % 2) + 4 * (dw / 8);
+        return ((u * 2 + s) * 4 + i) * kFrag + value_slot((r & 1) * 32 + m, i) + 8 * (r >> 1);
+    };
+    auto value_dim = [&](unsigned char* base, int at, int e) {
+        return reinterpret_cast<uint2*>(base + (at ^ ((e % 4) * 16 | e / 4 * 128)));
     };
     auto key_at = [&](unsigned char* base, int unit, int e) {  // eight dims 32 quarter + 8 e
         const int token = unit / 4, quarter = unit % 4;
@@ -287,20 +369,24 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
         float ref = kNone, l = 0.0f;
         uint4 q[C::QPLANES][8];
 
-        // Weights 2^(logit - ref) of 32 tokens from their products: lane's own row,
-        // tokens 8 (i / 4) + 4 half + i % 4.  They are kept below fp16's largest number:
-        // ref moves where one would pass it, and starts so that the first tile's largest
-        // is 2^kBase.
-        auto weights = [&](const f32x16_t& s, float f, float (&p)[16]) {
-            float sum = 0.0f;
-            auto exps = [&] {
-                sum = 0.0f;
+        // Weights 2^(logit - ref) of 32 tokens from their products, as operands of the
+        // second product: lane's own row, tokens 8 (i / 4) + 4 half + i % 4; and their
+        // sum.  They are kept below fp16's largest number: ref moves where one would
+        // pass it, and starts so that the first tile's largest is 2^kBase.
+        auto soft = [&](const f32x16_t& s, float f, auto& out) {
+            float p[16], sum = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) p[i] = exp2_fast(fmaf(s[i], f, -ref));
+            for (int i = 0; i < 16; ++i) p[i] = exp2_fast(fmaf(s[i], f, -ref));
+            out.pack(p);
+            if constexpr (std::decay_t<decltype(out)>::SUM) {
+                sum = out.sum();
+            } else {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sum += p[i];
-            };
-            exps();
+            }
+            return sum;
+        };
+        auto settle = [&](const f32x16_t& s, float f, auto& out, float sum) {
             if (__ballot(!(sum < kFull)) != 0) {
                 float mx = -INFINITY;
 #pragma unroll
@@ -313,22 +399,33 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
 #pragma unroll
                     for (int j = 0; j < 16; ++j) acc[i][j] *= g;
                 ref = to;
-                exps();
+                sum = soft(s, f, out);
             }
             l += sum;
         };
-
-        // eight of them as an operand, in two fp16 terms
-        auto half_terms = [&](const float (&p)[16], int first, uint4& high, uint4& low) {
-            uint32_t w[4], rest[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float p0 = p[first + 2 * j], p1 = p[first + 2 * j + 1];
-                w[j] = pack_half2(p0, p1);
-                rest[j] = pack_half2(p0 - static_cast<float>(as_half2(w[j])[0]), p1 - static_cast<float>(as_half2(w[j])[1]));
+        // A wave's one or two 32-token parts of a tile: the vector work of one beside the
+        // matrix products of the other, `tail` beside the last.
+        auto fold_tile = [&](auto weights_of, bool second, float f, auto&& qk, auto&& mask, auto&& pv, auto&& tail) {
+            decltype(weights_of) p0, p1;
+            f32x16_t s0 = qk(wt);
+            mask(wt, s0);
+            if (S::SUB / S::WT == 2 && second) {
+                constexpr int u1 = S::SUB / S::WT == 2 ? 1 : 0;
+                f32x16_t s1 = qk(u1);
+                const float sum0 = soft(s0, f, p0);
+                interleave<std::decay_t<decltype(p0)>::QK, 4, 2>();
+                settle(s0, f, p0, sum0);
+                mask(u1, s1);
+                pv(wt, p0);
+                const float sum1 = soft(s1, f, p1);
+                interleave<std::decay_t<decltype(p0)>::PV, 4, 2>();
+                settle(s1, f, p1, sum1);
+                pv(u1, p1);
+            } else {
+                settle(s0, f, p0, soft(s0, f, p0));
+                pv(wt, p0);
             }
-            high = make_uint4(w[0], w[1], w[2], w[3]);
-            low = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+            tail();
         };
 
         __syncthreads();  // nothing reads the last part's LDS any more
@@ -398,8 +495,9 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                         for (int s = 0; s < 8; ++s) a.queries[((row_tile * C::STORED + n) * 8 + s) * kWave + lane] = q[n][s];
                 }
             }
-            uint4 xk[S::PER];
-            uint32_t xks[S::PER][2], xv[S::PER][4], xvs[S::PER][4];
+            // codes and scales on their way (with roles, of keys or of values)
+            constexpr int SETS = S::ROLES ? 1 : 2, VALS = SETS - 1;
+            uint32_t x[S::PER][SETS][4], xs[S::PER][SETS][4];
             bool key_there[S::PER];
             // (a tile's page entries are on their way while the one before is loaded)
             int32_t entry[S::PER];
@@ -421,27 +519,31 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                     const int64_t at = (there ? e : 0) * per_page + head_row + (t & in_page);
                     if (keys) {
                         const int quarter = unit % 4, k = unit / 4 % 4;
-                        xk[p] = *reinterpret_cast<const uint4*>(c.codes + (at + k) * kCodeRow + 16 * quarter);
+                        const uint4 w = *reinterpret_cast<const uint4*>(c.codes + (at + k) * kCodeRow + 16 * quarter);
+                        x[p][0][0] = w.x;
+                        x[p][0][1] = w.y;
+                        x[p][0][2] = w.z;
+                        x[p][0][3] = w.w;
                         const uint32_t* sc = c.scales + (at + k) * (2 * R);
                         key_there[p] = there && t + k < count;
                         if constexpr (R == 8) {
-                            xks[p][0] = sc[2 * quarter];
-                            xks[p][1] = sc[2 * quarter + 1];
+                            xs[p][0][0] = sc[2 * quarter];
+                            xs[p][0][1] = sc[2 * quarter + 1];
                         } else {
-                            xks[p][0] = sc[R == 4 ? quarter : quarter / 2];
+                            xs[p][0][0] = sc[R == 4 ? quarter : quarter / 2];
                         }
-                        if (!key_there[p]) xks[p][0] = xks[p][1] = 0u;
+                        if (!key_there[p]) xs[p][0][0] = xs[p][0][1] = 0u;
                     }
                     if (vals) {
                         const int dw = unit % 16;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            xv[p][j] = *reinterpret_cast<const uint32_t*>(c.codes + (at + j) * kCodeRow + 64 + 4 * dw);
-                            xvs[p][j] = c.scales[(at + j) * (2 * R) + R + 8 * dw / G];
+                            x[p][VALS][j] = *reinterpret_cast<const uint32_t*>(c.codes + (at + j) * kCodeRow + 64 + 4 * dw);
+                            xs[p][VALS][j] = c.scales[(at + j) * (2 * R) + R + 8 * dw / G];
                         }
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            if (!there || t + j >= count) xvs[p][j] = 0u;
+                            if (!there || t + j >= count) xs[p][VALS][j] = 0u;
                     }
                 }
             };
@@ -454,10 +556,10 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                     const int unit = tid - (vals && S::ROLES ? VALUES_FROM : 0) + p * S::THREADS;
                     if (keys) {
                         const int token = unit / 4, quarter = unit % 4;
-                        const uint32_t w[4] = {xk[p].x, xk[p].y, xk[p].z, xk[p].w};
+                        const uint32_t (&w)[4] = x[p][0];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const uint32_t sc = xks[p][R == 8 ? e / 2 : 0];
+                            const uint32_t sc = xs[p][0][R == 8 ? e / 2 : 0];
                             const half2_t delta = as_half2(high_halves(sc, sc));
                             if constexpr (EXACT) {
                                 const half2_t top7 = as_half2(__builtin_bit_cast(uint32_t, delta) & 0xfff0fff0u);
@@ -480,22 +582,24 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                         }
                         if constexpr (EXACT) {
                             if constexpr (R == 8) {
-                                s_scale[buf][token][2 * quarter] = xks[p][0];
-                                s_scale[buf][token][2 * quarter + 1] = xks[p][1];
+                                s_scale[buf][token][2 * quarter] = xs[p][0][0];
+                                s_scale[buf][token][2 * quarter + 1] = xs[p][0][1];
                             } else if (R == 4 || quarter % 2 == 0) {
-                                s_scale[buf][token][R == 4 ? quarter : quarter / 2] = xks[p][0];
+                                s_scale[buf][token][R == 4 ? quarter : quarter / 2] = xs[p][0][0];
                             }
                         }
                         if (quarter == 0) s_bias[buf][token] = key_there[p] ? 0.0f : 1.0f;
                         some = some || !key_there[p];
                     }
                     if (vals) {
+                        int place = value_at(unit);
+                        asm volatile("" : "+v"(place));  // (its eight forms need no registers between tiles)
                         uint32_t out[8][2], low[8][2];  // [dim][token pair]
 #pragma unroll
                         for (int t2 = 0; t2 < 2; ++t2) {
-                            const uint32_t v0 = xv[p][2 * t2], v1 = xv[p][2 * t2 + 1];
-                            const half2_t delta = as_half2(high_halves(xvs[p][2 * t2], xvs[p][2 * t2 + 1]));
-                            const half2_t base = as_half2(low_halves(xvs[p][2 * t2], xvs[p][2 * t2 + 1]));
+                            const uint32_t v0 = x[p][VALS][2 * t2], v1 = x[p][VALS][2 * t2 + 1];
+                            const half2_t delta = as_half2(high_halves(xs[p][VALS][2 * t2], xs[p][VALS][2 * t2 + 1]));
+                            const half2_t base = as_half2(low_halves(xs[p][VALS][2 * t2], xs[p][VALS][2 * t2 + 1]));
 #pragma unroll
                             for (int hw = 0; hw < 2; ++hw) {
                                 const uint32_t w = hw ? high_halves(v0, v1) : low_halves(v0, v1);
@@ -525,25 +629,22 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                         }
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            *value_at(s_v, unit, e) = make_uint2(out[e][0], out[e][1]);
-                            if constexpr (C::VT == 2) *value_at(s_v + PLANE, unit, e) = make_uint2(low[e][0], low[e][1]);
+                            *value_dim(s_v, place, e) = make_uint2(out[e][0], out[e][1]);
+                            if constexpr (C::VT == 2) *value_dim(s_v + PLANE, place, e) = make_uint2(low[e][0], low[e][1]);
                         }
                     }
                 }
                 const bool any = __ballot(some) != 0;
                 if (lane == 0) s_ragged[buf][wave] = any ? 1 : 0;
             };
-            auto fold = [&](int buf) {
+            auto fold = [&](int buf, auto&& tail) {
                 const unsigned char* const s_k = s_mem + buf * BUF;
                 const unsigned char* const s_v = s_k + C::KT * PLANE;
                 int flags = 0;
 #pragma unroll
                 for (int i = 0; i < S::W; ++i) flags |= s_ragged[buf][i];
                 const bool ragged = __builtin_amdgcn_readfirstlane(flags) != 0;
-#pragma unroll
-                for (int uu = 0; uu < S::SUB / S::WT; ++uu) {
-                    __builtin_amdgcn_sched_barrier(0);
-                    const int u = uu * S::WT + wt;
+                auto qk = [&](int u) {
                     f32x16_t s;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[i] = 0.0f;
@@ -561,36 +662,32 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                         }
                     }
 #pragma unroll
-                    for (int st = 0; st < 8; ++st)
+                    for (int kt = C::KT - 1; kt >= 0; --kt)
+                        products([&](int st) { return s_k + kt * PLANE + (u * 8 + st) * kFrag + lane * 16; },
+                                 [&](int st, const uint4& k) {
 #pragma unroll
-                        for (int kt = 0; kt < C::KT; ++kt) {
-                            const uint4 k = ld16(s_k + kt * PLANE + (u * 8 + st) * kFrag + lane * 16);
-#pragma unroll
-                            for (int qt = C::QT - 1; qt >= 0; --qt) s = mfma_h(k, q[qt][st], s);
-                        }
+                                     for (int qt = C::QT - 1; qt >= 0; --qt) s = mfma_h(k, q[qt][st], s);
+                                 });
+                    return s;
+                };
+                auto mask = [&](int u, f32x16_t& s) {
                     if (ragged) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
                             s[i] = s_bias[buf][32 * u + 8 * (i / 4) + 4 * half + i % 4] != 0.0f ? -INFINITY : s[i];
                     }
-                    float p[16];
-                    weights(s, factor, p);
+                };
+                auto pv = [&](int u, const HalfWeights<C::VT, !EXACT, C::QT>& p) {
 #pragma unroll
-                    for (int st = 0; st < 2; ++st) {
-                        uint4 ph, pl;
-                        half_terms(p, 8 * st, ph, pl);
+                    for (int vt = 0; vt < C::VT; ++vt)
+                        products(
+                            [&](int n) { return s_v + vt * PLANE + (u * 8 + n) * kFrag + value_slot(lane, n % 4); },
+                            [&](int n, const uint4& v) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const unsigned char* at = s_v + ((u * 2 + st) * 4 + i) * kFrag + value_slot(lane, i);
-                            const uint4 v = ld16(at);
-                            acc[i] = mfma_h(v, ph, acc[i]);
-                            if constexpr (C::VT == 2) {
-                                acc[i] = mfma_h(v, pl, acc[i]);
-                                acc[i] = mfma_h(ld16(at + PLANE), ph, acc[i]);
-                            }
-                        }
-                    }
-                }
+                                for (int pt = 0; pt < C::VT - vt; ++pt) acc[n % 4] = mfma_h(v, p.at[pt][n / 4], acc[n % 4]);
+                            });
+                };
+                fold_tile(HalfWeights<C::VT, !EXACT, C::QT>{}, true, factor, qk, mask, pv, tail);
             };
             const int x1 = min(part.x1, cached_tiles);
             find(part.x0);
@@ -598,16 +695,17 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
             find(part.x0 + 1);
             if constexpr (BUFS == 2) {
                 stage(0);
-                if (part.x0 + 1 < x1) load(part.x0 + 1);
+                load(part.x0 + 1);
                 find(part.x0 + 2);
                 __syncthreads();
                 for (int x = part.x0; x < x1; ++x) {
                     const int buf = (x - part.x0) & 1;
-                    fold(buf);
-                    __builtin_amdgcn_sched_barrier(0);
-                    if (x + 1 < x1) stage(buf ^ 1);
-                    if (x + 2 < x1) load(x + 2);
-                    find(x + 3);
+                    // (behind the part's last tile: what nothing reads)
+                    fold(buf, [&] {
+                        stage(buf ^ 1);
+                        load(x + 2);
+                        find(x + 3);
+                    });
                     __syncthreads();
                 }
             } else {
@@ -616,7 +714,7 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                     if (x + 1 < x1) load(x + 1);
                     find(x + 2);
                     __syncthreads();
-                    fold(0);
+                    fold(0, [] {});
                     __syncthreads();
                 }
             }
@@ -697,6 +795,8 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                         }
                     }
                     if (vals) {
+                        int place = value_at(unit);
+                        asm volatile("" : "+v"(place));
                         bool mine = false;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) mine = mine || odd_values<T>(nv[p][j]);
@@ -712,7 +812,7 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                                 bf16_terms<3>(nv[p][0].get(e), nv[p][1].get(e), t[0]);
                                 bf16_terms<3>(nv[p][2].get(e), nv[p][3].get(e), t[1]);
 #pragma unroll
-                                for (int n = 0; n < 3; ++n) *value_at(s_v + n * PLANE, unit, e) = make_uint2(t[0][n], t[1][n]);
+                                for (int n = 0; n < 3; ++n) *value_dim(s_v + n * PLANE, place, e) = make_uint2(t[0][n], t[1][n]);
                             } else {
                                 uint32_t w[4];
 #pragma unroll
@@ -720,7 +820,7 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                                     const uint4& x = nv[p][j].u;
                                     w[j] = e < 2 ? x.x : e < 4 ? x.y : e < 6 ? x.z : x.w;
                                 }
-                                *value_at(s_v, unit, e) = e & 1 ? make_uint2(high_halves(w[0], w[1]), high_halves(w[2], w[3]))
+                                *value_dim(s_v, place, e) = e & 1 ? make_uint2(high_halves(w[0], w[1]), high_halves(w[2], w[3]))
                                                                 : make_uint2(low_halves(w[0], w[1]), low_halves(w[2], w[3]));
                             }
                         }
@@ -772,8 +872,10 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                     for (int i = 0; i < 16; ++i) s[i] = 8 * (i / 4) + 4 * half + i % 4 == t ? dot : s[i];
                 }
             };
-            int t_first = 0, t_last = 0;
-            auto fold = [&](int tile, int buf) {
+            // (of the wave's rows)
+            const int t_first = __builtin_amdgcn_readfirstlane(t_row), t_last = __builtin_amdgcn_readlane(t_row, 31);
+            using Weights = std::conditional_t<C::F16, HalfWeights<C::PT, false, 1>, Bf16Weights<C::PT, 1>>;
+            auto fold = [&](int tile, int buf, auto&& tail) {
                 const unsigned char* const s_k = s_mem + buf * BUF;
                 const unsigned char* const s_v = s_k + C::NT * PLANE;
                 int flags = 0, key_flags = 0;
@@ -782,69 +884,57 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                     flags |= s_ragged[buf][i];
                     if constexpr (C::F32) key_flags |= s_odd_keys[buf][i];
                 }
-#pragma unroll
-                for (int uu = 0; uu < S::SUB / S::WT; ++uu) {
-                    __builtin_amdgcn_sched_barrier(0);
-                    const int u = uu * S::WT + wt;
-                    if (tile * S::TILE + 32 * u > t_last) continue;
+                const bool odd = __builtin_amdgcn_readfirstlane(flags) != 0, odd_keys = __builtin_amdgcn_readfirstlane(key_flags) != 0;
+                auto qk = [&](int u) {
                     f32x16_t s;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
-                    for (int st = 0; st < 8; ++st) {
-                        uint4 k[C::NT];
+                    for (int n = C::NT - 1; n >= 0; --n)
+                        products([&](int st) { return s_k + n * PLANE + (u * 8 + st) * kFrag + lane * 16; },
+                                 [&](int st, const uint4& k) {
 #pragma unroll
-                        for (int n = 0; n < C::NT; ++n) k[n] = ld16(s_k + n * PLANE + (u * 8 + st) * kFrag + lane * 16);
-                        // the smallest products first
-#pragma unroll
-                        for (int n = C::NT - 1; n >= 0; --n)
-#pragma unroll
-                            for (int m = n; m >= 0; --m) s = mfma_t(k[m], q[n - m][st], s);
-                    }
+                                     for (int m = C::NT - 1 - n; m >= 0; --m) s = mfma_t(k, q[m][st], s);
+                                 });
+                    return s;
+                };
+                auto mask = [&](int u, f32x16_t& s) {
                     const int first = tile * S::TILE + 32 * u, t0 = first + 4 * half;
                     if constexpr (C::F32)
-                        if (__builtin_amdgcn_readfirstlane(key_flags) != 0) odd_logits(first, s);
+                        if (odd_keys) odd_logits(first, s);
                     // (tokens behind the chunk's last are ahead of every row)
-                    if (first + 31 > t_first)
+                    if (first + 31 > t_first) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) s[i] = t0 + 8 * (i / 4) + i % 4 <= t_row ? s[i] : -INFINITY;
-                    float p[16];
-                    weights(s, kScaleHigh, p);
-#pragma unroll
-                    for (int st = 0; st < 2; ++st) {
-                        uint4 pw[C::PT];
-                        if constexpr (C::F16) half_terms(p, 8 * st, pw[0], pw[1]);
-                        else bf16_operand<C::PT>([&](int j) { return p[8 * st + j]; }, pw);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const unsigned char* at = s_v + ((u * 2 + st) * 4 + i) * kFrag + value_slot(lane, i);
-#pragma unroll
-                            for (int n = 0; n < C::NT; ++n) {
-                                const uint4 v = ld16(at + n * PLANE);
-#pragma unroll
-                                for (int m = 0; m < C::PT; ++m)
-                                    if (n + m < 3) acc[i] = mfma_t(v, pw[m], acc[i]);
-                            }
-                        }
+                        for (int i = 0; i < 16; ++i) s[i] = t0 + 8 * (i / 4) + i % 4 <= t_row ? s[i] : -INFINITY;
                     }
-                    if (__builtin_amdgcn_readfirstlane(flags) != 0) add_odd(first);
-                }
+                };
+                auto pv = [&](int u, const Weights& p) {
+#pragma unroll
+                    for (int n = 0; n < C::NT; ++n)
+                        products(
+                            [&](int k) { return s_v + n * PLANE + (u * 8 + k) * kFrag + value_slot(lane, k % 4); },
+                            [&](int k, const uint4& v) {
+#pragma unroll
+                                for (int m = 0; m < C::PT - n; ++m) acc[k % 4] = mfma_t(v, p.at[m][k / 4], acc[k % 4]);
+                            });
+                    if (odd) add_odd(tile * S::TILE + 32 * u);
+                };
+                // (a wave's rows may lie before all of a part of the tile)
+                if (tile * S::TILE + 32 * wt > t_last) tail();
+                else fold_tile(Weights{}, tile * S::TILE + 32 <= t_last, kScaleHigh, qk, mask, pv, tail);
             };
             const int x0 = max(part.x0 - cached_tiles, 0), x1 = part.x1 - cached_tiles;
-            // (of the wave's rows)
-            t_first = __builtin_amdgcn_readfirstlane(t_row);
-            t_last = __builtin_amdgcn_readlane(t_row, 31);
             load(x0);
             if constexpr (BUFS == 2) {
                 stage(0);
-                if (x0 + 1 < x1) load(x0 + 1);
+                load(x0 + 1);
                 __syncthreads();
                 for (int x = x0; x < x1; ++x) {
                     const int buf = (x - x0) & 1;
-                    fold(x, buf);
-                    __builtin_amdgcn_sched_barrier(0);
-                    if (x + 1 < x1) stage(buf ^ 1);
-                    if (x + 2 < x1) load(x + 2);
+                    fold(x, buf, [&] {
+                        stage(buf ^ 1);
+                        load(x + 2);
+                    });
                     __syncthreads();
                 }
             } else {
@@ -852,7 +942,7 @@ __global__ __launch_bounds__(S::THREADS) void paged_chunk_kernel(PagedChunk a, P
                     stage(0);
                     if (x + 1 < x1) load(x + 1);
                     __syncthreads();
-                    fold(x, 0);
+                    fold(x, 0, [] {});
                     __syncthreads();
                 }
             }
