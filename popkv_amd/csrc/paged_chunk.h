@@ -498,7 +498,7 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
             // codes and scales on their way (with roles, of keys or of values)
             constexpr int SETS = S::ROLES ? 1 : 2, VALS = SETS - 1;
             uint32_t x[S::PER][SETS][4], xs[S::PER][SETS][4];
-            bool key_there[S::PER];
+            int left[S::PER];  // of a quad's four tokens, those that are there
             // (a tile's page entries are on their way while the one before is loaded)
             int32_t entry[S::PER];
             auto find = [&](int tile) {
@@ -514,46 +514,58 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                 for (int p = 0; p < S::PER; ++p) {
                     const int unit = tid - (vals && S::ROLES ? VALUES_FROM : 0) + p * S::THREADS;
                     const int t = tile * S::TILE + unit / 16 * 4;
-                    const int32_t e = entry[p];
-                    const bool there = static_cast<uint32_t>(e) < static_cast<uint32_t>(c.pages);
-                    const int64_t at = (there ? e : 0) * per_page + head_row + (t & in_page);
+                    const bool there = static_cast<uint32_t>(entry[p]) < static_cast<uint32_t>(c.pages);
+                    const int64_t at = (there ? entry[p] : 0) * per_page + head_row + (t & in_page);
+                    const char* const code = c.codes + at * kCodeRow;
+                    const uint32_t* const sc = c.scales + at * (2 * R);
+                    left[p] = there ? count - t : 0;
                     if (keys) {
                         const int quarter = unit % 4, k = unit / 4 % 4;
-                        const uint4 w = *reinterpret_cast<const uint4*>(c.codes + (at + k) * kCodeRow + 16 * quarter);
+                        const uint4 w = *reinterpret_cast<const uint4*>(code + k * kCodeRow + 16 * quarter);
                         x[p][0][0] = w.x;
                         x[p][0][1] = w.y;
                         x[p][0][2] = w.z;
                         x[p][0][3] = w.w;
-                        const uint32_t* sc = c.scales + (at + k) * (2 * R);
-                        key_there[p] = there && t + k < count;
                         if constexpr (R == 8) {
-                            xs[p][0][0] = sc[2 * quarter];
-                            xs[p][0][1] = sc[2 * quarter + 1];
+                            xs[p][0][0] = sc[k * 2 * R + 2 * quarter];
+                            xs[p][0][1] = sc[k * 2 * R + 2 * quarter + 1];
                         } else {
-                            xs[p][0][0] = sc[R == 4 ? quarter : quarter / 2];
+                            xs[p][0][0] = sc[k * 2 * R + (R == 4 ? quarter : quarter / 2)];
                         }
-                        if (!key_there[p]) xs[p][0][0] = xs[p][0][1] = 0u;
                     }
                     if (vals) {
                         const int dw = unit % 16;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            x[p][VALS][j] = *reinterpret_cast<const uint32_t*>(c.codes + (at + j) * kCodeRow + 64 + 4 * dw);
-                            xs[p][VALS][j] = c.scales[(at + j) * (2 * R) + R + 8 * dw / G];
+                            x[p][VALS][j] = *reinterpret_cast<const uint32_t*>(code + 4 * dw + (j * kCodeRow + 64));
+                            xs[p][VALS][j] = sc[8 * dw / G + (j * 2 * R + R)];
                         }
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (!there || t + j >= count) xs[p][VALS][j] = 0u;
                     }
                 }
             };
             auto stage = [&](int buf) {
                 unsigned char* const s_k = s_mem + buf * BUF;
                 unsigned char* const s_v = s_k + C::KT * PLANE;
-                bool some = false;
+                bool any = false;
 #pragma unroll
                 for (int p = 0; p < S::PER; ++p) {
                     const int unit = tid - (vals && S::ROLES ? VALUES_FROM : 0) + p * S::THREADS;
+                    if (__ballot(left[p] < 4) != 0) {
+                        // what lies behind the last token, or in no page, may be anything
+                        any = true;
+                        if (keys) {
+                            const bool there = unit / 4 % 4 < left[p];
+                            if (!there) xs[p][0][0] = xs[p][0][1] = 0u;
+                            if (unit % 4 == 0) s_bias[buf][unit / 4] = there ? 0.0f : 1.0f;
+                        }
+                        if (vals) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                if (j >= left[p]) xs[p][VALS][j] = 0u;
+                        }
+                    } else if (keys && unit % 4 == 0) {
+                        s_bias[buf][unit / 4] = 0.0f;
+                    }
                     if (keys) {
                         const int token = unit / 4, quarter = unit % 4;
                         const uint32_t (&w)[4] = x[p][0];
@@ -588,8 +600,6 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                                 s_scale[buf][token][R == 4 ? quarter : quarter / 2] = xs[p][0][0];
                             }
                         }
-                        if (quarter == 0) s_bias[buf][token] = key_there[p] ? 0.0f : 1.0f;
-                        some = some || !key_there[p];
                     }
                     if (vals) {
                         int place = value_at(unit);
@@ -634,7 +644,6 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                         }
                     }
                 }
-                const bool any = __ballot(some) != 0;
                 if (lane == 0) s_ragged[buf][wave] = any ? 1 : 0;
             };
             auto fold = [&](int buf, auto&& tail) {
@@ -760,7 +769,6 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             nk[p][e].load(k_head + static_cast<int64_t>(min(t, rows - 1)) * a.k_ts + 32 * (unit % 4) + 8 * e);
-                            if (t >= rows) nk[p][e].zero();
                         }
                     }
                     if (vals) {
@@ -768,18 +776,28 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             nv[p][j].load(v_head + static_cast<int64_t>(min(t + j, rows - 1)) * a.v_ts + 8 * (unit % 16));
-                            if (t + j >= rows) nv[p][j].zero();
                         }
                     }
                 }
             };
-            auto stage = [&](int buf) {
+            auto stage = [&](int tile, int buf) {
                 unsigned char* const s_k = s_mem + buf * BUF;
                 unsigned char* const s_v = s_k + C::NT * PLANE;
                 bool odd = false, odd_key = false;
 #pragma unroll
                 for (int p = 0; p < S::PER; ++p) {
                     const int unit = tid - (vals && S::ROLES ? VALUES_FROM : 0) + p * S::THREADS;
+                    if ((tile + 1) * S::TILE > rows) {  // what lies behind the chunk's last token may be anything
+                        if (keys && tile * S::TILE + unit / 4 >= rows) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) nk[p][e].zero();
+                        }
+                        if (vals) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                if (tile * S::TILE + unit / 16 * 4 + j >= rows) nv[p][j].zero();
+                        }
+                    }
                     if (keys) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
@@ -926,20 +944,20 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
             const int x0 = max(part.x0 - cached_tiles, 0), x1 = part.x1 - cached_tiles;
             load(x0);
             if constexpr (BUFS == 2) {
-                stage(0);
+                stage(x0, 0);
                 load(x0 + 1);
                 __syncthreads();
                 for (int x = x0; x < x1; ++x) {
                     const int buf = (x - x0) & 1;
                     fold(x, buf, [&] {
-                        stage(buf ^ 1);
+                        stage(x + 1, buf ^ 1);
                         load(x + 2);
                     });
                     __syncthreads();
                 }
             } else {
                 for (int x = x0; x < x1; ++x) {
-                    stage(0);
+                    stage(x, 0);
                     if (x + 1 < x1) load(x + 1);
                     __syncthreads();
                     fold(x, 0, [] {});
