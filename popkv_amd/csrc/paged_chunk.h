@@ -90,7 +90,7 @@ struct ChunkTypes {
     static constexpr int KT = EXACT ? 2 : 1;       // of the cached keys
     static constexpr int VT = F32 || F16 ? 2 : 1;  // of the cached values and their weights
     static constexpr int NT = F32 ? 3 : 1;         // planes of the new tokens (fp32: bf16 terms)
-    static constexpr int PT = F32 ? 3 : 2;         // terms of the weights on new tokens
+    static constexpr int PT = F32 ? 3 : F16 ? 2 : 1;  // terms of the weights on new tokens
     static constexpr int QPLANES = F32 ? 3 : 1;
     static constexpr int STORED = QT + QPLANES;    // query operands kept for the second pass
     static constexpr int PLANES = KT + VT > 2 * NT ? KT + VT : 2 * NT;
@@ -123,7 +123,7 @@ struct ChunkSizes {
 };
 
 struct ChunkPart {
-    int b, j, x0, x1, s, n, first;
+    int b, j, rows, count, x0, x1, s, n, first;
 };
 
 // The work of one KV head is the batch's tiles of rows laid end to end, each as long
@@ -136,52 +136,65 @@ struct ChunkWalk {
     const PagedChunk& a;
     const PagedView& c;
     const int64_t most;
-    const int lane, w, items, group;
+    const int lane, w, items, blocks, group;
+    int4* const held;  // entry i: item i0 + i's rows, count, tiles and start (in LDS: no registers between parts)
     int per, r0, r1, i0, base;
-    int start, tiles;  // lane i: item i0 + i
     uint64_t mask;
+    struct Item {
+        int rows, count, tiles;
+    };
 
-    __device__ __forceinline__ ChunkWalk(const PagedChunk& a_, const PagedView& c_, int64_t max_tokens, int w_, int groups)
+    __device__ __forceinline__ ChunkWalk(const PagedChunk& a_, const PagedView& c_, int64_t max_tokens, int w_, int groups,
+                                         int4* held_)
         : a(a_), c(c_), most(max_tokens), lane(threadIdx.x & (kWave - 1)), w(w_),
-          items(c.batch * static_cast<int>(a.row_blocks)), group(a.q_heads / c.kv_heads), i0(0), base(0) {
+          items(c.batch * static_cast<int>(a.row_blocks)), blocks(static_cast<int>(a.row_blocks)),
+          group(div_nonneg(a.q_heads, c.kv_heads)), held(held_), i0(0), base(0) {
         int total = 0;
-        for (int i = 0; i < items; i += kWave)
-            total += __builtin_amdgcn_readlane(static_cast<int>(wave_incl_scan(static_cast<uint32_t>(cost(length(i + lane))), lane)),
-                                               kWave - 1);
-        per = max((total + groups - 1) / groups, a.least);
+        Item x{};
+        for (int i = (items - 1) & ~(kWave - 1); i >= 0; i -= kWave) {  // (the first ones stay)
+            x = load(i);
+            total += __builtin_amdgcn_readlane(incl(x), kWave - 1);
+        }
+        per = max(div_nonneg(total + groups - 1, groups), a.least);
         r0 = static_cast<int>(min<int64_t>(static_cast<int64_t>(w) * per, int64_t{1} << 30));
         r1 = r0 + per;
-        find();
+        find(x);
     }
-    __device__ __forceinline__ int length(int i) const {
-        if (i >= items) return 0;
-        const int b = i / static_cast<int>(a.row_blocks), j = i - b * static_cast<int>(a.row_blocks);
+    __device__ __forceinline__ Item load(int first) const {
+        const int i = first + lane, b = min(blocks == 1 ? i : i / blocks, c.batch - 1), j = i - b * blocks;
         const ChunkSizes z(a, c, most, b);
-        if (static_cast<int64_t>(j) * S::ROWS >= static_cast<int64_t>(z.rows) * group) return 0;
-        const int seen = static_cast<int>(min<int64_t>((static_cast<int64_t>(j + 1) * S::ROWS - 1) / group + 1, z.rows));
-        return (z.count + S::TILE - 1) / S::TILE + (seen + S::TILE - 1) / S::TILE;
+        const int all = z.rows * group;  // (the entry holds rows * heads below 2^30)
+        const int seen = min(((j + 1) * S::ROWS - 1) / group + 1, z.rows);
+        const int tiles = (z.count + S::TILE - 1) / S::TILE + (seen + S::TILE - 1) / S::TILE;
+        return {z.rows, z.count, i < items && j * S::ROWS < all ? tiles : 0};
     }
-    __device__ __forceinline__ int cost(int n) const { return n > 0 ? n + a.item_cost : 0; }
-    __device__ __forceinline__ void find() {
-        tiles = length(i0 + lane);
-        const int n = static_cast<int>(wave_incl_scan(static_cast<uint32_t>(cost(tiles)), lane));
-        start = base + n - cost(tiles);
-        mask = __ballot(tiles > 0 && start < r1 && start + tiles > r0);
+    __device__ __forceinline__ int cost(const Item& x) const { return x.tiles > 0 ? x.tiles + a.item_cost : 0; }
+    __device__ __forceinline__ int incl(const Item& x) const {
+        return static_cast<int>(wave_incl_scan(static_cast<uint32_t>(cost(x)), lane));
+    }
+    // (every wave of the workgroup writes the same; all are past reading the last)
+    __device__ __forceinline__ void find(const Item& x) {
+        const int n = incl(x), start = base + n - cost(x);
+        mask = __ballot(x.tiles > 0 && start < r1 && start + x.tiles > r0);
+        held[lane] = make_int4(x.rows, x.count, x.tiles, start);
         base += __builtin_amdgcn_readlane(n, kWave - 1);
     }
     __device__ __forceinline__ bool next(ChunkPart& p) {
         while (mask == 0) {
             i0 += kWave;
             if (i0 >= items || base >= r1) return false;
-            find();
+            __syncthreads();
+            find(load(i0));
         }
         const int src = __ffsll(static_cast<unsigned long long>(mask)) - 1;
         mask &= mask - 1;
-        const int from = __builtin_amdgcn_readlane(start, src), to = from + __builtin_amdgcn_readlane(tiles, src);
-        const int item = i0 + src;
-        p.b = item / static_cast<int>(a.row_blocks);
-        p.j = item - p.b * static_cast<int>(a.row_blocks);
-        const int w0 = from >= r0 ? w : from / per, w1 = to <= r1 ? w : (to - 1) / per;
+        const int4 x = held[src];
+        const int from = __builtin_amdgcn_readfirstlane(x.w), to = from + __builtin_amdgcn_readfirstlane(x.z);
+        p.b = div_nonneg(i0 + src, blocks);
+        p.j = i0 + src - p.b * blocks;
+        p.rows = __builtin_amdgcn_readfirstlane(x.x);
+        p.count = __builtin_amdgcn_readfirstlane(x.y);
+        const int w0 = from >= r0 ? w : div_nonneg(from, per), w1 = to <= r1 ? w : div_nonneg(to - 1, per);
         p.s = w - w0;
         p.n = w1 - w0 + 1;
         p.first = w0;
@@ -226,9 +239,9 @@ struct HalfWeights {
         return x;
     }
 };
-template <int N, int QK_>
+template <int N, bool SUM_, int QK_>
 struct Bf16Weights {
-    static constexpr bool SUM = false;
+    static constexpr bool SUM = SUM_;
     static constexpr int QK = QK_, PV = N;
     uint4 at[N][2];
     __device__ __forceinline__ void pack(const float (&p)[16]) {
@@ -239,6 +252,18 @@ struct Bf16Weights {
 #pragma unroll
             for (int n = 0; n < N; ++n) at[n][st] = t[n];
         }
+    }
+    __device__ __forceinline__ float sum() const {
+        const bf16x2_t one = __builtin_bit_cast(bf16x2_t, 0x3f803f80u);
+        float x = 0.0f;
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+            x = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, at[0][st].x), one, x, false);
+            x = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, at[0][st].y), one, x, false);
+            x = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, at[0][st].z), one, x, false);
+            x = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, at[0][st].w), one, x, false);
+        }
+        return x;
     }
 };
 
@@ -295,7 +320,7 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
     constexpr int PLANE = S::SUB * 8 * kFrag, BUF = C::PLANES * PLANE;
     constexpr int BUFS = S::WR == 8 && 2 * BUF <= 140 * 1024 ? 2 : 1;
     static_assert(BUF <= 150 * 1024);
-    constexpr int JOIN = S::WT == 1 ? 0 : S::W / 2 * (16384 + 256);  // half of the waves' states
+    constexpr int JOIN = S::WT == 1 ? 0 : S::W * (16384 + 256);  // the waves' states
     __shared__ __align__(16) unsigned char s_mem[BUFS * BUF > JOIN ? BUFS * BUF : JOIN];
     __shared__ __align__(16) uint32_t s_scale[BUFS][EXACT ? S::TILE : 1][R];
     __shared__ float s_bias[BUFS][S::TILE];
@@ -307,7 +332,7 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int wr = wave % S::WR, wt = wave / S::WR;
     const int col = lane & 31, half = lane >> 5;
-    const int group = a.q_heads / c.kv_heads;
+    const int group = div_nonneg(a.q_heads, c.kv_heads);
 
     // rows behind a sequence's last one
     if (a.fill && a.tokens)
@@ -343,19 +368,29 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
     };
     auto ld16 = [&](const unsigned char* p) { return *reinterpret_cast<const uint4*>(p); };
 
-    ChunkWalk<S> walk(a, c, max_tokens, w_id, groups);
+    __shared__ int4 s_items[kWave];
+    ChunkWalk<S> walk(a, c, max_tokens, w_id, groups, s_items);
     ChunkPart part;
     while (walk.next(part)) {
         const int b = part.b;
-        const ChunkSizes z(a, c, max_tokens, b);
-        const int rows = z.rows, count = z.count;
+        const int rows = part.rows, count = part.count;
         const int cached_tiles = (count + S::TILE - 1) / S::TILE;
-        const int64_t all = static_cast<int64_t>(rows) * group, row0 = static_cast<int64_t>(part.j) * S::ROWS;
-        const int64_t row = min<int64_t>(row0 + 32 * wr + col, all - 1);
-        const bool live_row = row0 + 32 * wr + col < all;
-        const int t_row = static_cast<int>(row / group);
-        const int head = h * group + static_cast<int>(row - static_cast<int64_t>(t_row) * group);
-        const T* const q_row = static_cast<const T*>(a.q) + b * a.q_bs + head * a.q_hs + static_cast<int64_t>(t_row) * a.q_ts + 64 * half;
+        const int all = rows * group, row0 = part.j * S::ROWS;  // (below 2^30)
+        // (a lane's row, worked out where it is needed: registers between are dear)
+        struct Row {
+            int t, head;
+            bool live;
+        };
+        auto own_row = [&] {
+            int k = col;
+            asm volatile("" : "+v"(k));
+            const int row = min(row0 + 32 * wr + k, all - 1);
+            const int t = (group & (group - 1)) == 0 ? row >> __builtin_ctz(group) : row / group;
+            return Row{t, h * group + row - t * group, row0 + 32 * wr + k < all};
+        };
+        auto query = [&](const Row& r) {
+            return static_cast<const T*>(a.q) + b * a.q_bs + r.head * a.q_hs + static_cast<int64_t>(r.t) * a.q_ts + 64 * half;
+        };
         // what the second pass reads of these rows: the query operands of both kinds of
         // tokens, their factors, their sums
         const int64_t row_tile = (static_cast<int64_t>(b) * c.kv_heads + h) * a.row_blocks * S::WR + part.j * S::WR + wr;
@@ -431,12 +466,64 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
         __syncthreads();  // nothing reads the last part's LDS any more
         // ---- cached tokens
         if (part.x0 < cached_tiles) {
+            // codes and scales on their way (with roles, of keys or of values)
+            constexpr int SETS = S::ROLES ? 1 : 2, VALS = SETS - 1;
+            uint32_t x[S::PER][SETS][4], xs[S::PER][SETS][4];
+            int left[S::PER];  // of a quad's four tokens, those that are there
+            // (a tile's page entries are on their way while the one before is loaded)
+            int32_t entry[S::PER];
+            auto find = [&](int tile) {
+#pragma unroll
+                for (int p = 0; p < S::PER; ++p) {
+                    const int unit = tid - (vals && S::ROLES ? VALUES_FROM : 0) + p * S::THREADS;
+                    const int t = tile * S::TILE + unit / 16 * 4;  // the quad of both
+                    entry[p] = t < count ? c.table[b * c.width + (t >> c.page_log2)] : -1;
+                }
+            };
+            auto load = [&](int tile) {
+#pragma unroll
+                for (int p = 0; p < S::PER; ++p) {
+                    const int unit = tid - (vals && S::ROLES ? VALUES_FROM : 0) + p * S::THREADS;
+                    const int t = tile * S::TILE + unit / 16 * 4;
+                    const bool there = static_cast<uint32_t>(entry[p]) < static_cast<uint32_t>(c.pages);
+                    const int64_t at = (there ? entry[p] : 0) * per_page + head_row + (t & in_page);
+                    const char* const code = c.codes + at * kCodeRow;
+                    const uint32_t* const sc = c.scales + at * (2 * R);
+                    left[p] = there ? count - t : 0;
+                    if (keys) {
+                        const int quarter = unit % 4, k = unit / 4 % 4;
+                        const uint4 w = *reinterpret_cast<const uint4*>(code + k * kCodeRow + 16 * quarter);
+                        x[p][0][0] = w.x;
+                        x[p][0][1] = w.y;
+                        x[p][0][2] = w.z;
+                        x[p][0][3] = w.w;
+                        if constexpr (R == 8) {
+                            xs[p][0][0] = sc[k * 2 * R + 2 * quarter];
+                            xs[p][0][1] = sc[k * 2 * R + 2 * quarter + 1];
+                        } else {
+                            xs[p][0][0] = sc[k * 2 * R + (R == 4 ? quarter : quarter / 2)];
+                        }
+                    }
+                    if (vals) {
+                        const int dw = unit % 16;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            x[p][VALS][j] = *reinterpret_cast<const uint32_t*>(code + 4 * dw + (j * kCodeRow + 64));
+                            xs[p][VALS][j] = sc[8 * dw / G + (j * 2 * R + R)];
+                        }
+                    }
+                }
+            };
             uint4 ql[LOWS];
             float factor;
             {
+                find(part.x0);
                 Raw8<T> raw[8];
+                const T* const q_row = query(own_row());
 #pragma unroll
                 for (int s = 0; s < 8; ++s) raw[s].load(q_row + 8 * s);
+                load(part.x0);
+                find(part.x0 + 1);
                 float top = 0.0f;
 #pragma unroll
                 for (int s = 0; s < 8; ++s)
@@ -495,54 +582,6 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                         for (int s = 0; s < 8; ++s) a.queries[((row_tile * C::STORED + n) * 8 + s) * kWave + lane] = q[n][s];
                 }
             }
-            // codes and scales on their way (with roles, of keys or of values)
-            constexpr int SETS = S::ROLES ? 1 : 2, VALS = SETS - 1;
-            uint32_t x[S::PER][SETS][4], xs[S::PER][SETS][4];
-            int left[S::PER];  // of a quad's four tokens, those that are there
-            // (a tile's page entries are on their way while the one before is loaded)
-            int32_t entry[S::PER];
-            auto find = [&](int tile) {
-#pragma unroll
-                for (int p = 0; p < S::PER; ++p) {
-                    const int unit = tid - (vals && S::ROLES ? VALUES_FROM : 0) + p * S::THREADS;
-                    const int t = tile * S::TILE + unit / 16 * 4;  // the quad of both
-                    entry[p] = t < count ? c.table[b * c.width + (t >> c.page_log2)] : -1;
-                }
-            };
-            auto load = [&](int tile) {
-#pragma unroll
-                for (int p = 0; p < S::PER; ++p) {
-                    const int unit = tid - (vals && S::ROLES ? VALUES_FROM : 0) + p * S::THREADS;
-                    const int t = tile * S::TILE + unit / 16 * 4;
-                    const bool there = static_cast<uint32_t>(entry[p]) < static_cast<uint32_t>(c.pages);
-                    const int64_t at = (there ? entry[p] : 0) * per_page + head_row + (t & in_page);
-                    const char* const code = c.codes + at * kCodeRow;
-                    const uint32_t* const sc = c.scales + at * (2 * R);
-                    left[p] = there ? count - t : 0;
-                    if (keys) {
-                        const int quarter = unit % 4, k = unit / 4 % 4;
-                        const uint4 w = *reinterpret_cast<const uint4*>(code + k * kCodeRow + 16 * quarter);
-                        x[p][0][0] = w.x;
-                        x[p][0][1] = w.y;
-                        x[p][0][2] = w.z;
-                        x[p][0][3] = w.w;
-                        if constexpr (R == 8) {
-                            xs[p][0][0] = sc[k * 2 * R + 2 * quarter];
-                            xs[p][0][1] = sc[k * 2 * R + 2 * quarter + 1];
-                        } else {
-                            xs[p][0][0] = sc[k * 2 * R + (R == 4 ? quarter : quarter / 2)];
-                        }
-                    }
-                    if (vals) {
-                        const int dw = unit % 16;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            x[p][VALS][j] = *reinterpret_cast<const uint32_t*>(code + 4 * dw + (j * kCodeRow + 64));
-                            xs[p][VALS][j] = sc[8 * dw / G + (j * 2 * R + R)];
-                        }
-                    }
-                }
-            };
             auto stage = [&](int buf) {
                 unsigned char* const s_k = s_mem + buf * BUF;
                 unsigned char* const s_v = s_k + C::KT * PLANE;
@@ -699,9 +738,6 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                 fold_tile(HalfWeights<C::VT, !EXACT, C::QT>{}, true, factor, qk, mask, pv, tail);
             };
             const int x1 = min(part.x1, cached_tiles);
-            find(part.x0);
-            load(part.x0);
-            find(part.x0 + 1);
             if constexpr (BUFS == 2) {
                 stage(0);
                 load(part.x0 + 1);
@@ -732,6 +768,7 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
         // ---- the new tokens, in their own type (fp32: three bf16 terms)
         if (store_rows || part.x1 > cached_tiles) {
             Raw8<T> raw[8];
+            const T* const q_row = query(own_row());
 #pragma unroll
             for (int s = 0; s < 8; ++s) raw[s].load(q_row + 8 * s);
 #pragma unroll
@@ -753,13 +790,15 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
             }
         }
         if (part.x1 > cached_tiles) {
+            const int t_row = own_row().t;
             const T* const k_head = static_cast<const T*>(a.k) + b * a.k_bs + h * a.k_hs;
             const T* const v_head = static_cast<const T*>(a.v) + b * a.v_bs + h * a.v_hs;
             auto mfma_t = [&](const uint4& x, const uint4& y, f32x16_t z) {
                 if constexpr (C::F16) return mfma_h(x, y, z);
                 else return mfma_b(x, y, z);
             };
-            Raw8<T> nk[S::PER][4], nv[S::PER][4];
+            constexpr int SETS = S::ROLES ? 1 : 2, VALS = SETS - 1;
+            Raw8<T> x[S::PER][SETS][4];
             auto load = [&](int tile) {
 #pragma unroll
                 for (int p = 0; p < S::PER; ++p) {
@@ -768,14 +807,14 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                         const int t = tile * S::TILE + unit / 4;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            nk[p][e].load(k_head + static_cast<int64_t>(min(t, rows - 1)) * a.k_ts + 32 * (unit % 4) + 8 * e);
+                            x[p][0][e].load(k_head + static_cast<int64_t>(min(t, rows - 1)) * a.k_ts + 32 * (unit % 4) + 8 * e);
                         }
                     }
                     if (vals) {
                         const int t = tile * S::TILE + unit / 16 * 4;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            nv[p][j].load(v_head + static_cast<int64_t>(min(t + j, rows - 1)) * a.v_ts + 8 * (unit % 16));
+                            x[p][VALS][j].load(v_head + static_cast<int64_t>(min(t + j, rows - 1)) * a.v_ts + 8 * (unit % 16));
                         }
                     }
                 }
@@ -790,25 +829,25 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                     if ((tile + 1) * S::TILE > rows) {  // what lies behind the chunk's last token may be anything
                         if (keys && tile * S::TILE + unit / 4 >= rows) {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) nk[p][e].zero();
+                            for (int e = 0; e < 4; ++e) x[p][0][e].zero();
                         }
                         if (vals) {
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-                                if (tile * S::TILE + unit / 16 * 4 + j >= rows) nv[p][j].zero();
+                                if (tile * S::TILE + unit / 16 * 4 + j >= rows) x[p][VALS][j].zero();
                         }
                     }
                     if (keys) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             if constexpr (C::F32) {
-                                odd_key = odd_key || odd_values<T>(nk[p][e]);
+                                odd_key = odd_key || odd_values<T>(x[p][0][e]);
                                 uint4 t[3];
-                                bf16_operand<3>([&](int i) { return nk[p][e].get(i); }, t);
+                                bf16_operand<3>([&](int i) { return x[p][0][e].get(i); }, t);
 #pragma unroll
                                 for (int n = 0; n < 3; ++n) *key_at(s_k + n * PLANE, unit, e) = t[n];
                             } else {
-                                *key_at(s_k, unit, e) = nk[p][e].u;
+                                *key_at(s_k, unit, e) = x[p][0][e].u;
                             }
                         }
                     }
@@ -817,26 +856,26 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                         asm volatile("" : "+v"(place));
                         bool mine = false;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) mine = mine || odd_values<T>(nv[p][j]);
+                        for (int j = 0; j < 4; ++j) mine = mine || odd_values<T>(x[p][VALS][j]);
                         odd = odd || mine;
                         if (__ballot(mine) != 0) {
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) clear_odd<T>(nv[p][j]);
+                            for (int j = 0; j < 4; ++j) clear_odd<T>(x[p][VALS][j]);
                         }
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             if constexpr (C::F32) {
                                 uint32_t t[2][3];
-                                bf16_terms<3>(nv[p][0].get(e), nv[p][1].get(e), t[0]);
-                                bf16_terms<3>(nv[p][2].get(e), nv[p][3].get(e), t[1]);
+                                bf16_terms<3>(x[p][VALS][0].get(e), x[p][VALS][1].get(e), t[0]);
+                                bf16_terms<3>(x[p][VALS][2].get(e), x[p][VALS][3].get(e), t[1]);
 #pragma unroll
                                 for (int n = 0; n < 3; ++n) *value_dim(s_v + n * PLANE, place, e) = make_uint2(t[0][n], t[1][n]);
                             } else {
                                 uint32_t w[4];
 #pragma unroll
                                 for (int j = 0; j < 4; ++j) {
-                                    const uint4& x = nv[p][j].u;
-                                    w[j] = e < 2 ? x.x : e < 4 ? x.y : e < 6 ? x.z : x.w;
+                                    const uint4& y = x[p][VALS][j].u;
+                                    w[j] = e < 2 ? y.x : e < 4 ? y.y : e < 6 ? y.z : y.w;
                                 }
                                 *value_dim(s_v, place, e) = e & 1 ? make_uint2(high_halves(w[0], w[1]), high_halves(w[2], w[3]))
                                                                 : make_uint2(low_halves(w[0], w[1]), low_halves(w[2], w[3]));
@@ -855,7 +894,7 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
             // rows that do see it get them here.
             auto add_odd = [&](int first) {
 #pragma unroll 1
-                for (int t = first; t < min(first + 32, rows); ++t) {
+                for (int t = first; t < min(first + S::TILE / S::WT, rows); ++t) {
                     const T* v_row = v_head + static_cast<int64_t>(t) * a.v_ts + 64 * half;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -873,6 +912,7 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
 #pragma unroll 1
                 for (int t = 0; t < min(32, rows - first); ++t) {
                     const T* k_row = k_head + static_cast<int64_t>(first + t) * a.k_ts + 64 * half;
+                    const T* const q_row = query(own_row());
                     float dot = 0.0f;
                     bool odd = false;
 #pragma unroll 1
@@ -892,7 +932,7 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
             };
             // (of the wave's rows)
             const int t_first = __builtin_amdgcn_readfirstlane(t_row), t_last = __builtin_amdgcn_readlane(t_row, 31);
-            using Weights = std::conditional_t<C::F16, HalfWeights<C::PT, false, 1>, Bf16Weights<C::PT, 1>>;
+            using Weights = std::conditional_t<C::F16, HalfWeights<C::PT, false, 1>, Bf16Weights<C::PT, C::PT == 1 && !EXACT, 1>>;
             auto fold = [&](int tile, int buf, auto&& tail) {
                 const unsigned char* const s_k = s_mem + buf * BUF;
                 const unsigned char* const s_v = s_k + C::NT * PLANE;
@@ -935,11 +975,11 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
 #pragma unroll
                                 for (int m = 0; m < C::PT - n; ++m) acc[k % 4] = mfma_t(v, p.at[m][k / 4], acc[k % 4]);
                             });
-                    if (odd) add_odd(tile * S::TILE + 32 * u);
                 };
                 // (a wave's rows may lie before all of a part of the tile)
                 if (tile * S::TILE + 32 * wt > t_last) tail();
                 else fold_tile(Weights{}, tile * S::TILE + 32 <= t_last, kScaleHigh, qk, mask, pv, tail);
+                if (odd) add_odd(tile * S::TILE + 32 * wt);
             };
             const int x0 = max(part.x0 - cached_tiles, 0), x1 = part.x1 - cached_tiles;
             load(x0);
@@ -967,61 +1007,71 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
         }
 
         l += lane_xor<32>(l);
-        // waves that shared the tokens: their states to the first of them, by halves
+        // Waves that shared the tokens: each takes D of the four tiles of dims from all of
+        // them.
+        constexpr int D = 4 / S::WT;
         if constexpr (S::WT > 1) {
+            float* const states = reinterpret_cast<float*>(s_mem);
+            float* const sums = states + S::W * 4096;
 #pragma unroll
-            for (int n = S::WT / 2; n >= 1; n /= 2) {
-                float* const at = reinterpret_cast<float*>(s_mem) + ((wt % n) * S::WR + wr) * 4096;
-                float* const ml = reinterpret_cast<float*>(s_mem) + S::W / 2 * 4096 + ((wt % n) * S::WR + wr) * 64;
-                if (wt >= n && wt < 2 * n) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        *reinterpret_cast<float4*>(at + (i * kWave + lane) * 4) =
-                            make_float4(acc[i / 4][4 * (i % 4)], acc[i / 4][4 * (i % 4) + 1], acc[i / 4][4 * (i % 4) + 2],
-                                        acc[i / 4][4 * (i % 4) + 3]);
-                    if (half == 0) {
-                        ml[col] = ref;
-                        ml[32 + col] = l;
-                    }
-                }
-                __syncthreads();
-                if (wt < n) {
-                    const float m2 = ml[col], l2 = ml[32 + col], mx = fmaxf(ref, m2);
-                    const float f = exp2_fast(ref - mx), g = exp2_fast(m2 - mx);
-                    l = fmaf(l, f, l2 * g);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float4 y = *reinterpret_cast<const float4*>(at + (i * kWave + lane) * 4);
-                        f32x16_t& x = acc[i / 4];
-                        const int j = 4 * (i % 4);
-                        x[j] = fmaf(x[j], f, y.x * g);
-                        x[j + 1] = fmaf(x[j + 1], f, y.y * g);
-                        x[j + 2] = fmaf(x[j + 2], f, y.z * g);
-                        x[j + 3] = fmaf(x[j + 3], f, y.w * g);
-                    }
-                    ref = mx;
-                }
-                __syncthreads();
+            for (int i = 0; i < 16; ++i)
+                *reinterpret_cast<float4*>(states + (wave * 16 + i) * 256 + lane * 4) =
+                    make_float4(acc[i / 4][4 * (i % 4)], acc[i / 4][4 * (i % 4) + 1], acc[i / 4][4 * (i % 4) + 2],
+                                acc[i / 4][4 * (i % 4) + 3]);
+            if (half == 0) {
+                sums[wave * 64 + col] = ref;
+                sums[wave * 64 + 32 + col] = l;
             }
-            if (wt > 0) continue;
+            __syncthreads();
+            float f[S::WT];
+#pragma unroll
+            for (int n = 0; n < S::WT; ++n) f[n] = sums[(n * S::WR + wr) * 64 + col];
+            ref = f[0];
+#pragma unroll
+            for (int n = 1; n < S::WT; ++n) ref = fmaxf(ref, f[n]);
+            l = 0.0f;
+#pragma unroll
+            for (int n = 0; n < S::WT; ++n) {
+                f[n] = exp2_fast(f[n] - ref);
+                l = fmaf(f[n], sums[(n * S::WR + wr) * 64 + 32 + col], l);
+            }
+#pragma unroll
+            for (int i = 0; i < 4 * D; ++i) {
+                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int n = 0; n < S::WT; ++n) {
+                    const float4 y = *reinterpret_cast<const float4*>(states + ((n * S::WR + wr) * 16 + wt * 4 * D + i) * 256 + lane * 4);
+                    x.x = fmaf(f[n], y.x, x.x);
+                    x.y = fmaf(f[n], y.y, x.y);
+                    x.z = fmaf(f[n], y.z, x.z);
+                    x.w = fmaf(f[n], y.w, x.w);
+                }
+                const int j = 4 * (i % 4);
+                acc[i / 4][j] = x.x;
+                acc[i / 4][j + 1] = x.y;
+                acc[i / 4][j + 2] = x.z;
+                acc[i / 4][j + 3] = x.w;
+            }
         }
         if (part.n == 1) {
-            if (live_row) {
-                T* const out = static_cast<T*>(a.out) + b * a.o_bs + head * a.o_hs + static_cast<int64_t>(t_row) * a.o_ts + 64 * half;
+            const Row r = own_row();
+            if (r.live) {
+                T* const out = static_cast<T*>(a.out) + b * a.o_bs + r.head * a.o_hs + static_cast<int64_t>(r.t) * a.o_ts +
+                               64 * half + 16 * D * wt;
                 const float f = 1.0f / l;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) store16<T>(out + 16 * i, acc[i], f);
+                for (int i = 0; i < D; ++i) store16<T>(out + 16 * i, acc[i], f);
             }
             // (rows past the last one weigh nothing)
-            if (store_rows && half == 0) a.lse[row_tile * 32 + col] = live_row ? ref + __log2f(l) : INFINITY;
+            if (store_rows && half == 0) a.lse[row_tile * 32 + col] = r.live ? ref + __log2f(l) : INFINITY;
         } else {
             float* const state = a.partials + ((2 * static_cast<int64_t>(w_id) + (part.s == 0 ? 1 : 0)) * c.kv_heads + h) * S::STATE +
                                  wr * (4096 + 64);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                *reinterpret_cast<float4*>(state + (i * kWave + lane) * 4) = make_float4(
+            for (int i = 0; i < 4 * D; ++i)
+                *reinterpret_cast<float4*>(state + ((4 * D * wt + i) * kWave + lane) * 4) = make_float4(
                     acc[i / 4][4 * (i % 4)], acc[i / 4][4 * (i % 4) + 1], acc[i / 4][4 * (i % 4) + 2], acc[i / 4][4 * (i % 4) + 3]);
-            if (half == 0) {
+            if (half == 0 && wt == 0) {
                 state[4096 + col] = ref;
                 state[4096 + 32 + col] = l;
             }
@@ -1048,6 +1098,7 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(PagedChunk a, PagedVie
         return a.partials + (place * c.kv_heads + h) * S::STATE + wr * (4096 + 64);
     };
     float m = -INFINITY, l = 0.0f;
+#pragma unroll 8
     for (int s = 0; s < parts.y; ++s) m = fmaxf(m, state(s)[4096 + col]);
     f32x16_t acc;
 #pragma unroll
