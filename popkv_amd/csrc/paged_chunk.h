@@ -366,6 +366,11 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
         return reinterpret_cast<uint4*>(base + (token / 32 * 8 + 4 * (quarter & 1) + e) * kFrag +
                                         (quarter / 2 * 32 + token % 32) * 16);
     };
+    auto new_key_at = [&](unsigned char* base, int unit, int e) {  // eight dims 8 quarter + 32 e (four threads 64 bytes)
+        const int token = unit / 4, quarter = unit % 4;
+        return reinterpret_cast<uint4*>(base + (token / 32 * 8 + 4 * (e & 1) + quarter) * kFrag +
+                                        (e / 2 * 32 + token % 32) * 16);
+    };
     auto ld16 = [&](const unsigned char* p) { return *reinterpret_cast<const uint4*>(p); };
 
     __shared__ int4 s_items[kWave];
@@ -439,28 +444,26 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
             l += sum;
         };
         // A wave's one or two 32-token parts of a tile: the vector work of one beside the
-        // matrix products of the other, `tail` beside the last.
-        auto fold_tile = [&](auto weights_of, bool second, float f, auto&& qk, auto&& mask, auto&& pv, auto&& tail) {
+        // matrix products of the other.
+        auto fold_tile = [&](auto weights_of, float f, auto&& qk, auto&& mask, auto&& pv) {
             decltype(weights_of) p0, p1;
             f32x16_t s0 = qk(wt);
             mask(wt, s0);
-            if (S::SUB / S::WT == 2 && second) {
-                constexpr int u1 = S::SUB / S::WT == 2 ? 1 : 0;
-                f32x16_t s1 = qk(u1);
+            if constexpr (S::SUB / S::WT == 2) {
+                f32x16_t s1 = qk(1);
                 const float sum0 = soft(s0, f, p0);
                 interleave<std::decay_t<decltype(p0)>::QK, 4, 2>();
                 settle(s0, f, p0, sum0);
-                mask(u1, s1);
-                pv(wt, p0);
+                mask(1, s1);
+                pv(0, p0);
                 const float sum1 = soft(s1, f, p1);
                 interleave<std::decay_t<decltype(p0)>::PV, 4, 2>();
                 settle(s1, f, p1, sum1);
-                pv(u1, p1);
+                pv(1, p1);
             } else {
                 settle(s0, f, p0, soft(s0, f, p0));
                 pv(wt, p0);
             }
-            tail();
         };
 
         __syncthreads();  // nothing reads the last part's LDS any more
@@ -685,7 +688,7 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                 }
                 if (lane == 0) s_ragged[buf][wave] = any ? 1 : 0;
             };
-            auto fold = [&](int buf, auto&& tail) {
+            auto fold = [&](int buf) {
                 const unsigned char* const s_k = s_mem + buf * BUF;
                 const unsigned char* const s_v = s_k + C::KT * PLANE;
                 int flags = 0;
@@ -735,7 +738,7 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                                 for (int pt = 0; pt < C::VT - vt; ++pt) acc[n % 4] = mfma_h(v, p.at[pt][n / 4], acc[n % 4]);
                             });
                 };
-                fold_tile(HalfWeights<C::VT, !EXACT, C::QT>{}, true, factor, qk, mask, pv, tail);
+                fold_tile(HalfWeights<C::VT, !EXACT, C::QT>{}, factor, qk, mask, pv);
             };
             const int x1 = min(part.x1, cached_tiles);
             if constexpr (BUFS == 2) {
@@ -746,11 +749,10 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                 for (int x = part.x0; x < x1; ++x) {
                     const int buf = (x - part.x0) & 1;
                     // (behind the part's last tile: what nothing reads)
-                    fold(buf, [&] {
-                        stage(buf ^ 1);
-                        load(x + 2);
-                        find(x + 3);
-                    });
+                    fold(buf);
+                    stage(buf ^ 1);
+                    load(x + 2);
+                    find(x + 3);
                     __syncthreads();
                 }
             } else {
@@ -759,7 +761,7 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                     if (x + 1 < x1) load(x + 1);
                     find(x + 2);
                     __syncthreads();
-                    fold(0, [] {});
+                    fold(0);
                     __syncthreads();
                 }
             }
@@ -807,7 +809,7 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                         const int t = tile * S::TILE + unit / 4;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            x[p][0][e].load(k_head + static_cast<int64_t>(min(t, rows - 1)) * a.k_ts + 32 * (unit % 4) + 8 * e);
+                            x[p][0][e].load(k_head + static_cast<int64_t>(min(t, rows - 1)) * a.k_ts + 8 * (unit % 4) + 32 * e);
                         }
                     }
                     if (vals) {
@@ -845,9 +847,9 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                                 uint4 t[3];
                                 bf16_operand<3>([&](int i) { return x[p][0][e].get(i); }, t);
 #pragma unroll
-                                for (int n = 0; n < 3; ++n) *key_at(s_k + n * PLANE, unit, e) = t[n];
+                                for (int n = 0; n < 3; ++n) *new_key_at(s_k + n * PLANE, unit, e) = t[n];
                             } else {
-                                *key_at(s_k, unit, e) = x[p][0][e].u;
+                                *new_key_at(s_k, unit, e) = x[p][0][e].u;
                             }
                         }
                     }
@@ -892,9 +894,9 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
             // Infinite and NaN values: times a weight of zero they would reach rows that do
             // not see their token, so the products take them as zero, and their dims of the
             // rows that do see it get them here.
-            auto add_odd = [&](int first) {
+            auto add_odd = [&](int first, int last) {
 #pragma unroll 1
-                for (int t = first; t < min(first + S::TILE / S::WT, rows); ++t) {
+                for (int t = first; t < min(last, rows); ++t) {
                     const T* v_row = v_head + static_cast<int64_t>(t) * a.v_ts + 64 * half;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -933,7 +935,8 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
             // (of the wave's rows)
             const int t_first = __builtin_amdgcn_readfirstlane(t_row), t_last = __builtin_amdgcn_readlane(t_row, 31);
             using Weights = std::conditional_t<C::F16, HalfWeights<C::PT, false, 1>, Bf16Weights<C::PT, C::PT == 1 && !EXACT, 1>>;
-            auto fold = [&](int tile, int buf, auto&& tail) {
+            bool odd = false;
+            auto fold = [&](int tile, int buf) {
                 const unsigned char* const s_k = s_mem + buf * BUF;
                 const unsigned char* const s_v = s_k + C::NT * PLANE;
                 int flags = 0, key_flags = 0;
@@ -942,7 +945,8 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                     flags |= s_ragged[buf][i];
                     if constexpr (C::F32) key_flags |= s_odd_keys[buf][i];
                 }
-                const bool odd = __builtin_amdgcn_readfirstlane(flags) != 0, odd_keys = __builtin_amdgcn_readfirstlane(key_flags) != 0;
+                odd = odd || __builtin_amdgcn_readfirstlane(flags) != 0;
+                const bool odd_keys = __builtin_amdgcn_readfirstlane(key_flags) != 0;
                 auto qk = [&](int u) {
                     f32x16_t s;
 #pragma unroll
@@ -976,10 +980,8 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                                 for (int m = 0; m < C::PT - n; ++m) acc[k % 4] = mfma_t(v, p.at[m][k / 4], acc[k % 4]);
                             });
                 };
-                // (a wave's rows may lie before all of a part of the tile)
-                if (tile * S::TILE + 32 * wt > t_last) tail();
-                else fold_tile(Weights{}, tile * S::TILE + 32 <= t_last, kScaleHigh, qk, mask, pv, tail);
-                if (odd) add_odd(tile * S::TILE + 32 * wt);
+                // (a wave's rows may lie before its part of the tile)
+                if (tile * S::TILE + 32 * wt <= t_last) fold_tile(Weights{}, kScaleHigh, qk, mask, pv);
             };
             const int x0 = max(part.x0 - cached_tiles, 0), x1 = part.x1 - cached_tiles;
             load(x0);
@@ -989,10 +991,9 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                 __syncthreads();
                 for (int x = x0; x < x1; ++x) {
                     const int buf = (x - x0) & 1;
-                    fold(x, buf, [&] {
-                        stage(x + 1, buf ^ 1);
-                        load(x + 2);
-                    });
+                    fold(x, buf);
+                    stage(x + 1, buf ^ 1);
+                    load(x + 2);
                     __syncthreads();
                 }
             } else {
@@ -1000,10 +1001,12 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                     stage(x, 0);
                     if (x + 1 < x1) load(x + 1);
                     __syncthreads();
-                    fold(x, 0, [] {});
+                    fold(x, 0);
                     __syncthreads();
                 }
             }
+            // (by one of the waves that share a tile's tokens)
+            if (odd && wt == 0) add_odd(x0 * S::TILE, x1 * S::TILE);
         }
 
         l += lane_xor<32>(l);
