@@ -453,8 +453,9 @@ int popkv_paged_indexed_attention(const void* queries, int32_t dtype, const void
  * of every token, summed over the rows and the query heads of its KV head, are added
  * at the token's place, a chunk's token t at counts[b] + t (places past
  * weight_stride are left out).  Workspace: popkv_paged_chunk_attention_workspace_bytes()
- * bytes (with weights != 0 for calls that gather them), 16-byte aligned; its first
- * 2^18 bytes are not written, the others' content does not matter. */
+ * bytes (with weights != 0 for calls that gather them), 16-byte aligned, its first
+ * 2^18 bytes zero on entry and left zero, as for popkv_paged_attention, which does
+ * the work of a chunk of one token. */
 size_t popkv_paged_chunk_attention_workspace_bytes(int32_t dtype, int64_t batch, int64_t q_heads, int64_t kv_heads,
                                                    int64_t rows, int64_t max_tokens, int32_t weights);
 int popkv_paged_chunk_attention(const void* queries, int32_t dtype, int64_t q_batch_stride, int64_t q_head_stride,

@@ -88,7 +88,8 @@ struct ChunkTypes {
     static constexpr bool F16 = std::is_same_v<T, f16_t>;
     static constexpr int QT = F32 ? 2 : 1;         // fp16 terms of the queries
     static constexpr int KT = EXACT ? 2 : 1;       // of the cached keys
-    static constexpr int VT = F32 || F16 ? 2 : 1;  // of the cached values and their weights
+    static constexpr int VT = F32 ? 2 : 1;         // of the cached values
+    static constexpr int CT = F32 || F16 ? 2 : 1;  // of their weights
     static constexpr int NT = F32 ? 3 : 1;         // planes of the new tokens (fp32: bf16 terms)
     static constexpr int PT = F32 ? 3 : F16 ? 2 : 1;  // terms of the weights on new tokens
     static constexpr int QPLANES = F32 ? 3 : 1;
@@ -728,17 +729,17 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                             s[i] = s_bias[buf][32 * u + 8 * (i / 4) + 4 * half + i % 4] != 0.0f ? -INFINITY : s[i];
                     }
                 };
-                auto pv = [&](int u, const HalfWeights<C::VT, !EXACT, C::QT>& p) {
+                auto pv = [&](int u, const HalfWeights<C::CT, C::CT == 1 && !EXACT, C::QT>& p) {
 #pragma unroll
                     for (int vt = 0; vt < C::VT; ++vt)
                         products(
                             [&](int n) { return s_v + vt * PLANE + (u * 8 + n) * kFrag + value_slot(lane, n % 4); },
                             [&](int n, const uint4& v) {
 #pragma unroll
-                                for (int pt = 0; pt < C::VT - vt; ++pt) acc[n % 4] = mfma_h(v, p.at[pt][n / 4], acc[n % 4]);
+                                for (int pt = 0; pt < C::CT - vt; ++pt) acc[n % 4] = mfma_h(v, p.at[pt][n / 4], acc[n % 4]);
                             });
                 };
-                fold_tile(HalfWeights<C::VT, !EXACT, C::QT>{}, factor, qk, mask, pv);
+                fold_tile(HalfWeights<C::CT, C::CT == 1 && !EXACT, C::QT>{}, factor, qk, mask, pv);
             };
             const int x1 = min(part.x1, cached_tiles);
             if constexpr (BUFS == 2) {

@@ -45,15 +45,16 @@ def attend(q, k, v, nk, nv, lengths, new):
 
 def allowed(want, dtype, v, nv):
     """Largest error per element: the output's rounding (half a step) and the fp32 work;
-    for bf16 tensors the roundings, half a step each of at most the largest value, of
-    cached values (fp16, 2^-11) and of the weights, fp16 on cached tokens and bf16 (2^-8)
-    on new ones, twice as the sum that they are divided by is the rounded ones'."""
+    for 16-bit tensors the rounding of cached values to fp16, half a step (2^-11) of at
+    most the largest value; for bf16 ones those of the weights too, fp16 on cached tokens
+    and bf16 (2^-8) on new ones, twice as the sum that they are divided by is the rounded
+    ones'."""
     bound = torch.finfo(dtype).eps / 2 * want.abs() + FP32
-    if dtype != torch.bfloat16:
+    if dtype == torch.float32:
         return bound
     group = want.shape[1] // nv.shape[1]
     top = torch.cat([v, nv.cpu().double()], 2).abs().amax((2, 3)).repeat_interleave(group, 1)[..., None, None]
-    return bound + top * (3 * 2.0 ** -11 + 2 * 2.0 ** -8)
+    return bound + top * (2.0 ** -11 if dtype == torch.float16 else 3 * 2.0 ** -11 + 2 * 2.0 ** -8)
 
 
 def setup(lengths, new, kv_heads, group, dtype, *, dims=32, page=64, seed=0, spread=2.0, layers=1):
