@@ -421,10 +421,11 @@ struct PagedChunk {
     int2* parts;
     float* partials;
     // with weights, for every (sequence, KV head) row_blocks * row_waves times 32
-    // rows: the query operands (plan.stored * 8 KB a tile), factors and sums
+    // rows: the query operands (plan.stored KB a tile), factors and sums
     uint4* queries;
     float *factors, *lse;
 };
+constexpr int kChunkStored16 = 18, kChunkStored32 = 42;  // KB of stored operands of 32 rows
 // How a call is cut: waves of 32 rows a workgroup (shape), blocks of so many rows a
 // sequence, workgroups a KV head, the fewest tiles of tokens of one, what a block costs
 // beside its tiles, floats of partial states, stored operands of 32 rows.

@@ -93,9 +93,14 @@ struct ChunkTypes {
     static constexpr int NT = F32 ? 3 : 1;         // planes of the new tokens (fp32: bf16 terms)
     static constexpr int PT = F32 ? 3 : F16 ? 2 : 1;  // terms of the weights on new tokens
     static constexpr int QPLANES = F32 ? 3 : 1;
-    static constexpr int STORED = QT + QPLANES;    // query operands kept for the second pass
+    // query operands kept for the second pass: for cached tokens, for new ones, the low
+    // terms' (of 1 KB, eight a plane)
+    static constexpr int STORED = 8 * (QT + QPLANES) + 2;
     static constexpr int PLANES = KT + VT > 2 * NT ? KT + VT : 2 * NT;
 };
+
+static_assert(ChunkTypes<float, true>::STORED == kChunkStored32 && ChunkTypes<bf16_t, true>::STORED == kChunkStored16 &&
+              ChunkTypes<f16_t, true>::STORED == kChunkStored16);
 
 // Where lane l's sixteen bytes of value operand i of four lie in its KB: writers
 // of one instruction (16 dwords of codes) meet different banks, readers too.
@@ -583,7 +588,11 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
 #pragma unroll
                     for (int n = 0; n < C::QT; ++n)
 #pragma unroll
-                        for (int s = 0; s < 8; ++s) a.queries[((row_tile * C::STORED + n) * 8 + s) * kWave + lane] = q[n][s];
+                        for (int s = 0; s < 8; ++s) a.queries[(row_tile * C::STORED + 8 * n + s) * kWave + lane] = q[n][s];
+                    if constexpr (EXACT)
+#pragma unroll
+                        for (int n = 0; n < LOWS; ++n)
+                            a.queries[(row_tile * C::STORED + 8 * (C::QT + C::QPLANES) + n) * kWave + lane] = ql[n];
                 }
             }
             auto stage = [&](int buf) {
@@ -789,7 +798,8 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
 #pragma unroll
                 for (int n = 0; n < C::QPLANES; ++n)
 #pragma unroll
-                    for (int s = 0; s < 8; ++s) a.queries[((row_tile * C::STORED + C::QT + n) * 8 + s) * kWave + lane] = q[n][s];
+                    for (int s = 0; s < 8; ++s)
+                        a.queries[(row_tile * C::STORED + 8 * (C::QT + n) + s) * kWave + lane] = q[n][s];
             }
         }
         if (part.x1 > cached_tiles) {
@@ -1101,25 +1111,42 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(PagedChunk a, PagedVie
         const int64_t place = 2 * static_cast<int64_t>(parts.x + s) + (s == 0 ? 1 : 0);
         return a.partials + (place * c.kv_heads + h) * S::STATE + wr * (4096 + 64);
     };
+    constexpr int AHEAD = 4;  // parts on their way at once
     float m = -INFINITY, l = 0.0f;
-#pragma unroll 8
-    for (int s = 0; s < parts.y; ++s) m = fmaxf(m, state(s)[4096 + col]);
     f32x16_t acc;
 #pragma unroll
     for (int k = 0; k < 16; ++k) acc[k] = 0.0f;
-#pragma unroll 4
-    for (int s = 0; s < parts.y; ++s) {
-        const float* p = state(s);
-        const float f = exp2_fast(p[4096 + col] - m);
-        l = fmaf(f, p[4096 + 32 + col], l);
+    for (int s0 = 0; s0 < parts.y; s0 += AHEAD) {
+        float4 y[AHEAD][4];
+        float pm[AHEAD], pl[AHEAD], mx = m;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float4 y = *reinterpret_cast<const float4*>(p + ((4 * i + k) * kWave + lane) * 4);
-            acc[4 * k] = fmaf(f, y.x, acc[4 * k]);
-            acc[4 * k + 1] = fmaf(f, y.y, acc[4 * k + 1]);
-            acc[4 * k + 2] = fmaf(f, y.z, acc[4 * k + 2]);
-            acc[4 * k + 3] = fmaf(f, y.w, acc[4 * k + 3]);
+        for (int n = 0; n < AHEAD; ++n) {
+            const float* p = state(min(s0 + n, parts.y - 1));
+            pm[n] = p[4096 + col];
+            pl[n] = p[4096 + 32 + col];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[n][k] = *reinterpret_cast<const float4*>(p + ((4 * i + k) * kWave + lane) * 4);
         }
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) mx = fmaxf(mx, pm[n]);
+        const float g = m == -INFINITY ? 0.0f : exp2_fast(m - mx);
+        l *= g;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) acc[k] *= g;
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) {
+            if (s0 + n >= parts.y) break;
+            const float f = exp2_fast(pm[n] - mx);
+            l = fmaf(f, pl[n], l);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                acc[4 * k] = fmaf(f, y[n][k].x, acc[4 * k]);
+                acc[4 * k + 1] = fmaf(f, y[n][k].y, acc[4 * k + 1]);
+                acc[4 * k + 2] = fmaf(f, y[n][k].z, acc[4 * k + 2]);
+                acc[4 * k + 3] = fmaf(f, y[n][k].w, acc[4 * k + 3]);
+            }
+        }
+        m = mx;
     }
     if (row < all) {
         const int t_row = static_cast<int>(row / group);
@@ -1133,123 +1160,188 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(PagedChunk a, PagedVie
     }
 }
 
-// The attention weights of 32 tokens of a KV head a wave, from the logits once
-// more and the rows' sums: keys stay in registers as two fp16 terms (fp32's 22
-// bits), every row's operands pass once.
-template <typename T, int G>
-__global__ __launch_bounds__(256) void chunk_weights_kernel(PagedChunk a, PagedView c, int64_t max_tokens) {
+// The attention weights of N times 32 tokens of a KV head a wave, from the logits once
+// more and the rows' sums: keys stay in registers, as the first pass has them, and
+// every row's operands pass once.  Rows stand in the products' rows, so that a token's
+// weights lie in one lane's registers and that of the other half.
+template <typename T, int G, int N>
+__global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void chunk_weights_kernel(PagedChunk a, PagedView c,
+                                                                                     int64_t max_tokens) {
     using C = ChunkTypes<T, true>;
-    constexpr int R = 128 / G;
+    constexpr int R = 128 / G, LOWS = R == 8 ? 2 : 1, SPAN = 32 * N;
     const int b = blockIdx.z, h = blockIdx.y;
     const int lane = threadIdx.x & (kWave - 1), col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int group = a.q_heads / c.kv_heads;
-    const int rows = static_cast<int>(a.tokens ? clamp_count(a.tokens[b], a.rows) : a.rows);
-    const int count = static_cast<int>(clamp_count(c.counts[b], min(c.width << c.page_log2, max_tokens)));
-    const int cached_tiles = (count + 31) / 32, tile = blockIdx.x * 4 + wave;
-    const bool cached = tile < cached_tiles;
-    const int t0 = 32 * (cached ? tile : tile - cached_tiles);
+    const int group = div_nonneg(a.q_heads, c.kv_heads);
+    const ChunkSizes z(a, c, max_tokens, b);
+    const int rows = z.rows, count = z.count;
+    const int cached_spans = (count + SPAN - 1) / SPAN, span = blockIdx.x * 4 + wave;
+    const bool cached = span < cached_spans;
+    const int t0 = SPAN * (cached ? span : span - cached_spans);
     if (rows == 0 || (!cached && t0 >= rows)) return;
-    const int64_t all = static_cast<int64_t>(rows) * group;
+    const int all = rows * group;
     const int64_t base = (static_cast<int64_t>(b) * c.kv_heads + h) * (a.row_blocks * a.row_waves);
-    const int token = t0 + col;
-    uint4 k[C::F32 ? 3 : 2][8];
-    bool there = true, odd = false;
-    if (cached) {
-        const int32_t e = token < count ? c.table[b * c.width + (token >> c.page_log2)] : -1;
-        there = static_cast<uint32_t>(e) < static_cast<uint32_t>(c.pages);
-        const int64_t at = (there ? e : 0) * (static_cast<int64_t>(c.kv_heads) << c.page_log2) +
-                           (static_cast<int64_t>(h) << c.page_log2) + (token & ((1 << c.page_log2) - 1));
-        const uint4* codes = reinterpret_cast<const uint4*>(c.codes + at * kCodeRow + 32 * half);
-        const uint4 w0 = codes[0], w1 = codes[1];
-        const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+    float sum[N];
+    bool there[N];
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            const uint32_t sc = c.scales[at * (2 * R) + (64 * half + 8 * s) / G];
-            float code[8], x[8], y[8];
-            codes8(w[s], code);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = fmaf(code[i], f16_hi(sc), f16_lo(sc));
-                y[i] = x[i] - static_cast<float>(static_cast<_Float16>(x[i]));
-            }
-            k[0][s] = make_uint4(pack_half2(x[0], x[4]), pack_half2(x[1], x[5]), pack_half2(x[2], x[6]), pack_half2(x[3], x[7]));
-            k[1][s] = make_uint4(pack_half2(y[0], y[4]), pack_half2(y[1], y[5]), pack_half2(y[2], y[6]), pack_half2(y[3], y[7]));
-        }
-    } else {
-        const T* k_row = static_cast<const T*>(a.k) + b * a.k_bs + h * a.k_hs + static_cast<int64_t>(min(token, rows - 1)) * a.k_ts;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            Raw8<T> raw;
-            raw.load(k_row + 64 * half + 8 * s);
-            if constexpr (C::F32) {
-                odd = odd || odd_values<T>(raw);
-                uint4 t[3];
-                bf16_operand<3>([&](int i) { return raw.get(i); }, t);
-#pragma unroll
-                for (int n = 0; n < 3; ++n) k[n][s] = t[n];
-            } else {
-                k[0][s] = raw.u;
-            }
-        }
-    }
-    // (the parts of an infinite fp32 key's products are no sum: its logit is minus
-    // infinity or makes the row NaN)
-    if constexpr (C::F32) odd = odd || lane_xor<32>(odd ? 1.0f : 0.0f) != 0.0f;
-    float sum = 0.0f;
-    const int64_t first_row = cached ? 0 : static_cast<int64_t>(t0) * group;
-    const int64_t own_first = cached ? 0 : static_cast<int64_t>(token) * group;  // the first row that sees the token
-    for (int64_t r0 = first_row / 32 * 32; r0 < all; r0 += 32) {
-        const uint4* q = a.queries + (base + r0 / 32) * (C::STORED * 8 * kWave) + lane;
-        f32x16_t s;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = 0.0f;
-        if (cached) {
-#pragma unroll
-            for (int st = 0; st < 8; ++st)
-#pragma unroll
-                for (int qt = C::QT - 1; qt >= 0; --qt) {
-                    const uint4 x = q[(qt * 8 + st) * kWave];
-                    s = mfma_h(x, k[1][st], s);
-                    s = mfma_h(x, k[0][st], s);
-                }
-        } else {
-#pragma unroll
-            for (int st = 0; st < 8; ++st) {
-                uint4 x[C::QPLANES];
-#pragma unroll
-                for (int n = 0; n < C::QPLANES; ++n) x[n] = q[((C::QT + n) * 8 + st) * kWave];
-#pragma unroll
-                for (int n = C::QPLANES - 1; n >= 0; --n)
-#pragma unroll
-                    for (int m = n; m >= 0; --m) {
-                        if constexpr (C::F16) s = mfma_h(x[m], k[n - m][st], s);
-                        else s = mfma_b(x[m], k[n - m][st], s);
-                    }
-            }
-        }
+    for (int n = 0; n < N; ++n) sum[n] = 0.0f;
+    // a tile of 32 rows: its logits' products by `logits`, what weighs by `seen`
+    auto tile = [&](int r0, auto&& logits, auto&& seen, bool scaled) {
         const float4* lse = reinterpret_cast<const float4*>(a.lse + (base * 32 + r0) + 4 * half);
         const float4* factors = reinterpret_cast<const float4*>(a.factors + (base * 32 + r0) + 4 * half);
+        float4 off[4], f[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float4 off = lse[2 * i];
-            float4 f = make_float4(kScaleHigh, kScaleHigh, kScaleHigh, kScaleHigh);
-            if (cached) f = factors[2 * i];
-            const int64_t r = r0 + 8 * i + 4 * half;
-            if constexpr (C::F32)
-                if (odd)
+            off[i] = lse[2 * i];
+            f[i] = scaled ? factors[2 * i] : make_float4(kScaleHigh, kScaleHigh, kScaleHigh, kScaleHigh);
+        }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) s[4 * i + j] = -INFINITY;
-            sum += r >= own_first ? exp2_fast(fmaf(s[4 * i], f.x, -off.x)) : 0.0f;
-            sum += r + 1 >= own_first ? exp2_fast(fmaf(s[4 * i + 1], f.y, -off.y)) : 0.0f;
-            sum += r + 2 >= own_first ? exp2_fast(fmaf(s[4 * i + 2], f.z, -off.z)) : 0.0f;
-            sum += r + 3 >= own_first ? exp2_fast(fmaf(s[4 * i + 3], f.w, -off.w)) : 0.0f;
+        for (int n = 0; n < N; ++n) {
+            const f32x16_t s = logits(n);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = r0 + 8 * i + 4 * half;
+                sum[n] += seen(n, r, exp2_fast(fmaf(s[4 * i], f[i].x, -off[i].x)), off[i].x);
+                sum[n] += seen(n, r + 1, exp2_fast(fmaf(s[4 * i + 1], f[i].y, -off[i].y)), off[i].y);
+                sum[n] += seen(n, r + 2, exp2_fast(fmaf(s[4 * i + 2], f[i].z, -off[i].z)), off[i].z);
+                sum[n] += seen(n, r + 3, exp2_fast(fmaf(s[4 * i + 3], f[i].w, -off[i].w)), off[i].w);
+            }
+        }
+    };
+    const uint4* const queries = a.queries + base * (C::STORED * kWave) + lane;
+    if (cached) {
+        const CodeBits bits;
+        uint4 k[N][2][8], low[N][LOWS];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int token = t0 + 32 * n + col;
+            const int32_t e = token < count ? c.table[b * c.width + (token >> c.page_log2)] : -1;
+            there[n] = static_cast<uint32_t>(e) < static_cast<uint32_t>(c.pages);
+            const int64_t at = (there[n] ? e : 0) * (static_cast<int64_t>(c.kv_heads) << c.page_log2) +
+                               (static_cast<int64_t>(h) << c.page_log2) + (token & ((1 << c.page_log2) - 1));
+            const uint4* codes = reinterpret_cast<const uint4*>(c.codes + at * kCodeRow + 32 * half);
+            const uint4 w0 = codes[0], w1 = codes[1];
+            const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+            uint32_t sc[R];
+#pragma unroll
+            for (int g = 0; g < R; ++g) sc[g] = c.scales[at * (2 * R) + g];
+            const uint32_t pick = half == 0 ? 0x01000100u : 0x03020302u;
+#pragma unroll
+            for (int m = 0; m < LOWS; ++m) {
+                uint32_t x[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int g = 0; g < 4 && g < R; ++g) x[g] = __builtin_amdgcn_perm(sc[4 * m + g], sc[4 * m + g], pick);
+                low[n][m] = make_uint4(x[0], x[1], x[2], x[3]);
+            }
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                const uint32_t own = half == 0 ? sc[8 * s / G] : sc[R / 2 + 8 * s / G];
+                const half2_t delta = as_half2(high_halves(own, own));
+                const half2_t top7 = as_half2(__builtin_bit_cast(uint32_t, delta) & 0xfff0fff0u), low4 = delta - top7;
+                half2_t code[4];
+                centred_pairs(bits, w[s], code);
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    hi[i] = __builtin_bit_cast(uint32_t, code[i] * top7);
+                    lo[i] = __builtin_bit_cast(uint32_t, code[i] * low4);
+                }
+                k[n][0][s] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                k[n][1][s] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+        }
+        for (int r0 = 0; r0 < all; r0 += 32) {
+            const uint4* q = queries + r0 / 32 * static_cast<int64_t>(C::STORED * kWave);
+            uint4 x[C::QT][8], ql[LOWS];
+#pragma unroll
+            for (int n = 0; n < LOWS; ++n) ql[n] = q[(8 * (C::QT + C::QPLANES) + n) * kWave];
+#pragma unroll
+            for (int n = 0; n < C::QT; ++n)
+#pragma unroll
+                for (int s = 0; s < 8; ++s) x[n][s] = q[(8 * n + s) * kWave];
+            tile(
+                r0,
+                [&](int n) {
+                    f32x16_t s;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+                    for (int m = 0; m < LOWS; ++m) s = mfma_h(ql[m], low[n][m], s);
+#pragma unroll
+                    for (int st = 0; st < 8; ++st)
+#pragma unroll
+                        for (int kt = 1; kt >= 0; --kt)
+#pragma unroll
+                            for (int qt = C::QT - 1; qt >= 0; --qt) s = mfma_h(x[qt][st], k[n][kt][st], s);
+                    return s;
+                },
+                [&](int, int, float p, float) { return p; }, true);
+        }
+    } else {
+        uint4 k[N][C::NT][8];
+        bool odd[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int token = t0 + 32 * n + col;
+            there[n] = token < rows;
+            odd[n] = false;
+            const T* k_row = static_cast<const T*>(a.k) + b * a.k_bs + h * a.k_hs + static_cast<int64_t>(min(token, rows - 1)) * a.k_ts;
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                Raw8<T> raw;
+                raw.load(k_row + 64 * half + 8 * s);
+                if constexpr (C::F32) {
+                    odd[n] = odd[n] || odd_values<T>(raw);
+                    uint4 t[3];
+                    bf16_operand<3>([&](int i) { return raw.get(i); }, t);
+#pragma unroll
+                    for (int m = 0; m < 3; ++m) k[n][m][s] = t[m];
+                } else {
+                    k[n][0][s] = raw.u;
+                }
+            }
+            // (the parts of an infinite fp32 key's products are no sum: its logit is minus
+            // infinity or makes the row NaN)
+            if constexpr (C::F32) odd[n] = odd[n] || lane_xor<32>(odd[n] ? 1.0f : 0.0f) != 0.0f;
+        }
+        for (int r0 = t0 * group / 32 * 32; r0 < all; r0 += 32) {
+            const uint4* q = queries + r0 / 32 * static_cast<int64_t>(C::STORED * kWave) + 8 * C::QT * kWave;
+            uint4 x[C::QPLANES][8];
+#pragma unroll
+            for (int n = 0; n < C::QPLANES; ++n)
+#pragma unroll
+                for (int s = 0; s < 8; ++s) x[n][s] = q[(8 * n + s) * kWave];
+            tile(
+                r0,
+                [&](int n) {
+                    f32x16_t s;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+                    for (int m = C::NT - 1; m >= 0; --m)
+#pragma unroll
+                        for (int j = C::NT - 1 - m; j >= 0; --j)
+#pragma unroll
+                            for (int st = 0; st < 8; ++st) {
+                                if constexpr (C::F16) s = mfma_h(x[j][st], k[n][m][st], s);
+                                else s = mfma_b(x[j][st], k[n][m][st], s);
+                            }
+                    return s;
+                },
+                [&](int n, int r, float p, float off) {
+                    if (C::F32 && odd[n]) p = off == off ? 0.0f : off;
+                    return r >= (t0 + 32 * n + col) * group ? p : 0.0f;
+                },
+                false);
         }
     }
-    sum += lane_xor<32>(sum);
-    const int64_t at = cached ? token : static_cast<int64_t>(count) + token;
-    if (half == 0 && there && (cached || token < rows) && at < a.weight_stride)
-        a.weights[(static_cast<int64_t>(b) * c.kv_heads + h) * a.weight_stride + at] += sum;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const float x = sum[n] + lane_xor<32>(sum[n]);
+        const int64_t at = static_cast<int64_t>(cached ? 0 : count) + t0 + 32 * n + col;
+        if (half == 0 && there[n] && at < a.weight_stride)
+            a.weights[(static_cast<int64_t>(b) * c.kv_heads + h) * a.weight_stride + at] += x;
+    }
 }
 
 template <typename T, int G, bool EXACT, typename S>
@@ -1290,9 +1382,15 @@ hipError_t launch_chunk_t(const PagedChunk& a, const PagedView& c, int64_t max_t
     }
     if (e != hipSuccess || !a.weights) return e;
     const int64_t most = min(max_tokens, c.width << c.page_log2);
-    const unsigned blocks = static_cast<unsigned>(((most + 31) / 32 + (a.rows + 31) / 32 + 3) / 4);
-    hipLaunchKernelGGL((chunk_weights_kernel<T, G>), dim3(blocks, c.kv_heads, c.batch), dim3(256), 0, stream, a, c, max_tokens);
-    return hipGetLastError();
+    auto launch = [&](auto kernel, int64_t span) {
+        const unsigned blocks = static_cast<unsigned>(((most + span - 1) / span + (a.rows + span - 1) / span + 3) / 4);
+        hipLaunchKernelGGL(kernel, dim3(blocks, c.kv_heads, c.batch), dim3(256), 0, stream, a, c, max_tokens);
+        return hipGetLastError();
+    };
+    // two parts a wave where many rows pass, one where keys are most of the work
+    if constexpr (!std::is_same_v<T, float>)
+        if (a.rows * (a.q_heads / c.kv_heads) > 128) return launch(chunk_weights_kernel<T, G, 2>, 64);
+    return launch(chunk_weights_kernel<T, G, 1>, 32);
 }
 
 template <typename T>

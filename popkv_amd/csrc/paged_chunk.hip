@@ -33,7 +33,7 @@ ChunkPlan paged_chunk_plan(int dtype, int64_t batch, int64_t q_heads, int64_t kv
     const int64_t most = ceil_of(batch * p.row_blocks * tiles, p.least);
     p.groups = static_cast<int>(most < target ? most : target);
     p.states = p.groups > 1 ? 2 * static_cast<int64_t>(p.groups) * kv_heads * p.shape * (32 * 128 + 64) : 0;
-    p.stored = dtype == POPKV_DTYPE_F32 ? 5 : 2;
+    p.stored = f32 ? kChunkStored32 : kChunkStored16;
     p.places = batch * p.row_blocks * tiles;
     return p;
 }
