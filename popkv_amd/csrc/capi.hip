@@ -920,7 +920,7 @@ void carve_evict(Carve& c, popkv::PageEvict& a) {
 // Behind the merge tickets of the other paged attention calls, which may share the workspace.
 void carve_chunk(Carve& c, popkv::PagedChunk& a, int32_t dtype, int64_t batch, int64_t q_heads, int64_t kv_heads,
                  int64_t rows, int64_t max_tokens, bool weights) {
-    const popkv::ChunkPlan p = popkv::paged_chunk_plan(dtype, batch, q_heads, kv_heads, rows, max_tokens);
+    const popkv::ChunkPlan p = popkv::paged_chunk_plan(dtype, batch, q_heads, kv_heads, rows, max_tokens, weights);
     a.shape = a.row_waves = p.shape;
     a.groups = p.groups;
     a.least = p.least;
@@ -1095,7 +1095,7 @@ int popkv_paged_chunk_attention(const void* queries, int32_t dtype, int64_t q_ba
     if (rows == 0) return POPKV_OK;  // (before the pointers: an empty tensor has none)
     if (!queries || !k || !v || !output || !workspace) return fail(POPKV_ERR_INVALID, "null pointer");
     if (weights && weight_stride <= 0) return fail(POPKV_ERR_INVALID, "bad weight stride");
-    if (popkv::paged_chunk_plan(dtype, batch, q_heads, kv_heads, rows, max_tokens).places > (int64_t{1} << 30))
+    if (popkv::paged_chunk_plan(dtype, batch, q_heads, kv_heads, rows, max_tokens, weights != nullptr).places > (int64_t{1} << 30))
         return fail(POPKV_ERR_UNSUPPORTED, "too many rows and tokens for one call");
     const int64_t es = static_cast<int64_t>(elem_size(dtype));
     const int64_t strides[] = {q_batch_stride, q_head_stride, q_row_stride, k_batch_stride,   k_head_stride,   k_row_stride,

@@ -433,7 +433,8 @@ struct ChunkPlan {
     int shape, groups, least, item_cost, stored;
     int64_t row_blocks, states, places;
 };
-ChunkPlan paged_chunk_plan(int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t rows, int64_t max_tokens);
+ChunkPlan paged_chunk_plan(int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t rows, int64_t max_tokens,
+                           bool weights);
 hipError_t launch_paged_chunk(const PagedChunk& a, const PagedView& c, int64_t max_tokens, int dtype, int dim_group,
                               hipStream_t stream);
 

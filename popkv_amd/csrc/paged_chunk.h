@@ -210,6 +210,14 @@ struct ChunkWalk {
     }
 };
 
+// The lane's number, worked out where it stands: for rare paths in loops that have no
+// register left to keep it in.
+__device__ __forceinline__ int fresh_lane() {
+    uint32_t all = ~0u;
+    asm volatile("" : "+s"(all));
+    return static_cast<int>(__builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0u)));
+}
+
 // Weights of 32 tokens as operands of two products of 16 tokens each, in N terms of a
 // type (QK, PV: the products of an operand beside them).  SUM: their sum is the rounded ones' (two a step).
 template <int N, bool SUM_, int QK_>
@@ -606,17 +614,19 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                         // what lies behind the last token, or in no page, may be anything
                         any = true;
                         if (keys) {
-                            const bool there = unit / 4 % 4 < left[p];
+                            const int rare = (wave * kWave + fresh_lane() + p * S::THREADS);
+                            const bool there = rare / 4 % 4 < left[p];
                             if (!there) xs[p][0][0] = xs[p][0][1] = 0u;
-                            if (unit % 4 == 0) s_bias[buf][unit / 4] = there ? 0.0f : 1.0f;
+                            if (rare % 4 == 0) s_bias[buf][rare / 4] = there ? 0.0f : 1.0f;
                         }
                         if (vals) {
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
                                 if (j >= left[p]) xs[p][VALS][j] = 0u;
                         }
-                    } else if (keys && unit % 4 == 0) {
-                        s_bias[buf][unit / 4] = 0.0f;
+                    } else if (keys) {
+                        const int rare = (wave * kWave + fresh_lane() + p * S::THREADS);
+                        if (rare % 4 == 0) s_bias[buf][rare / 4] = 0.0f;
                     }
                     if (keys) {
                         const int token = unit / 4, quarter = unit % 4;
@@ -733,12 +743,12 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                 };
                 auto mask = [&](int u, f32x16_t& s) {
                     if (ragged) {
+                        const float* const bias = &s_bias[buf][32 * u + fresh_lane() / 32 * 4];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            s[i] = s_bias[buf][32 * u + 8 * (i / 4) + 4 * half + i % 4] != 0.0f ? -INFINITY : s[i];
+                        for (int i = 0; i < 16; ++i) s[i] = bias[8 * (i / 4) + i % 4] != 0.0f ? -INFINITY : s[i];
                     }
                 };
-                auto pv = [&](int u, const HalfWeights<C::CT, C::CT == 1 && !EXACT, C::QT>& p) {
+                auto pv = [&](int u, const HalfWeights<C::CT, C::CT == 1 && !EXACT, C::QT * C::KT>& p) {
 #pragma unroll
                     for (int vt = 0; vt < C::VT; ++vt)
                         products(
@@ -748,7 +758,7 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                                 for (int pt = 0; pt < C::CT - vt; ++pt) acc[n % 4] = mfma_h(v, p.at[pt][n / 4], acc[n % 4]);
                             });
                 };
-                fold_tile(HalfWeights<C::CT, C::CT == 1 && !EXACT, C::QT>{}, factor, qk, mask, pv);
+                fold_tile(HalfWeights<C::CT, C::CT == 1 && !EXACT, C::QT * C::KT>{}, factor, qk, mask, pv);
             };
             const int x1 = min(part.x1, cached_tiles);
             if constexpr (BUFS == 2) {
@@ -1111,12 +1121,13 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(PagedChunk a, PagedVie
         const int64_t place = 2 * static_cast<int64_t>(parts.x + s) + (s == 0 ? 1 : 0);
         return a.partials + (place * c.kv_heads + h) * S::STATE + wr * (4096 + 64);
     };
-    constexpr int AHEAD = 4;  // parts on their way at once
     float m = -INFINITY, l = 0.0f;
     f32x16_t acc;
 #pragma unroll
     for (int k = 0; k < 16; ++k) acc[k] = 0.0f;
-    for (int s0 = 0; s0 < parts.y; s0 += AHEAD) {
+    // (parts on their way at once: four, eight where there are more)
+    auto fold = [&](auto ahead, int s0) {
+        constexpr int AHEAD = decltype(ahead)::value;
         float4 y[AHEAD][4];
         float pm[AHEAD], pl[AHEAD], mx = m;
 #pragma unroll
@@ -1147,7 +1158,11 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(PagedChunk a, PagedVie
             }
         }
         m = mx;
-    }
+    };
+    if (parts.y <= 4)
+        fold(std::integral_constant<int, 4>{}, 0);
+    else
+        for (int s0 = 0; s0 < parts.y; s0 += 8) fold(std::integral_constant<int, 8>{}, s0);
     if (row < all) {
         const int t_row = static_cast<int>(row / group);
         const int head = h * group + static_cast<int>(row - static_cast<int64_t>(t_row) * group);

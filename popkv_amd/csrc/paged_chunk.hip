@@ -19,7 +19,8 @@ int64_t ceil_of(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace
 
-ChunkPlan paged_chunk_plan(int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t rows, int64_t max_tokens) {
+ChunkPlan paged_chunk_plan(int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t rows, int64_t max_tokens,
+                           bool weights) {
     ChunkPlan p{};
     const int64_t all = rows * (q_heads / kv_heads);
     const bool f32 = dtype == POPKV_DTYPE_F32;
@@ -27,7 +28,7 @@ ChunkPlan paged_chunk_plan(int dtype, int64_t batch, int64_t q_heads, int64_t kv
     p.row_blocks = ceil_of(all, 32 * p.shape);
     p.least = 4;
     p.item_cost = 2;
-    const int tile = p.shape == 1 ? 128 : 64, at_once = p.shape == 8 || f32 ? 1 : 2;
+    const int tile = p.shape == 1 ? 128 : 64, at_once = p.shape == 8 || f32 || (p.shape == 1 && (weights || dtype != POPKV_DTYPE_BF16)) ? 1 : 2;
     const int64_t tiles = ceil_of(max_tokens, tile) + ceil_of(rows, tile) + p.item_cost;
     const int64_t target = ceil_of(kChunkCus * at_once, kv_heads);
     const int64_t most = ceil_of(batch * p.row_blocks * tiles, p.least);
