@@ -12,9 +12,7 @@ constexpr int32_t kFresh = -2;  // an entry whose page another sequence holds to
 
 // Sequence b by one wave: whether it is cut, its old row kept, its new one with
 // the fresh pages still to come, which are counted.
-__global__ __launch_bounds__(256) void evict_rows_kernel(PageEvict a) {
-    const int64_t b = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
-    if (b >= a.batch) return;
+__device__ __forceinline__ void evict_row(const PageEvict& a, int64_t b) {
     const int lane = threadIdx.x & (kWave - 1);
     const int64_t page = int64_t{1} << a.page_log2;
     const int64_t n = clamp_count(a.counts_in[b], a.width << a.page_log2);
@@ -50,10 +48,14 @@ __global__ __launch_bounds__(256) void evict_rows_kernel(PageEvict a) {
     }
 }
 
-// One workgroup: fresh pages handed out, lowest first, sequences in order; one
+__global__ __launch_bounds__(256) void evict_rows_kernel(PageEvict a) {
+    const int64_t b = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
+    if (b < a.batch) evict_row(a, b);
+}
+
+// Fresh pages handed out by one workgroup, lowest first, sequences in order; one
 // whose share does not fit stays as it was.
-__global__ __launch_bounds__(kPlanThreads) void evict_plan_kernel(PageEvict a) {
-    __shared__ PageMap map;
+__device__ __forceinline__ void evict_plan(const PageEvict& a, PageMap& map) {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int32_t total = scan_needs(a.need, a.batch, map.sh);
     int32_t found = 0;
@@ -92,6 +94,20 @@ __global__ __launch_bounds__(kPlanThreads) void evict_plan_kernel(PageEvict a) {
         }
         if (lane == 0) a.counts[b] = cut >= 0 ? cut : a.counts_in[b];
     }
+}
+
+__global__ __launch_bounds__(kPlanThreads) void evict_plan_kernel(PageEvict a) {
+    __shared__ PageMap map;
+    evict_plan(a, map);
+}
+
+// The whole plan of a small table.
+__global__ __launch_bounds__(kPlanThreads) void evict_alone_kernel(PageEvict a) {
+    __shared__ PageMap map;
+    if (a.refs != a.refs_in) plan_copy(a.refs_in, a.refs, static_cast<int>(a.pages));
+    for (int64_t b = threadIdx.x / kWave; b < a.batch; b += kPlanWaves) evict_row(a, b);
+    __syncthreads();
+    evict_plan(a, map);
 }
 
 // Order of weights: NaN above all, -0 as 0.
@@ -221,9 +237,9 @@ __global__ __launch_bounds__(kEvictThreads) void evict_move_kernel(PageEvict a) 
                 dst[p] = row_of(to, j);
                 if (part == 7) w[p] = w_in[i];
                 if (src[p] != dst[p]) {
-                    codes[p] = *reinterpret_cast<const u32x4*>(a.codes + src[p] * kCodeRow + 16 * part);
+                    codes[p] = load_once(a.codes + src[p] * kCodeRow + 16 * part);
                     if (4 * part < a.scale_words)
-                        scales[p] = *reinterpret_cast<const u32x4*>(a.scales + src[p] * a.scale_words + 4 * part);
+                        scales[p] = load_once(a.scales + src[p] * a.scale_words + 4 * part);
                 }
             }
         }
@@ -236,9 +252,9 @@ __global__ __launch_bounds__(kEvictThreads) void evict_move_kernel(PageEvict a) 
             if (j < k) {
                 if (part == 7) w_out[j] = w[p];
                 if (src[p] != dst[p]) {
-                    *reinterpret_cast<u32x4*>(a.codes + dst[p] * kCodeRow + 16 * part) = codes[p];
+                    store_once(a.codes + dst[p] * kCodeRow + 16 * part, codes[p]);
                     if (4 * part < a.scale_words)
-                        *reinterpret_cast<u32x4*>(a.scales + dst[p] * a.scale_words + 4 * part) = scales[p];
+                        store_once(a.scales + dst[p] * a.scale_words + 4 * part, scales[p]);
                 }
             }
         }
@@ -250,12 +266,16 @@ __global__ __launch_bounds__(kEvictThreads) void evict_move_kernel(PageEvict a) 
 }  // namespace
 
 hipError_t launch_page_evict(const PageEvict& a, hipStream_t s) {
-    if (a.refs != a.refs_in) {
-        const hipError_t e = copy_words(a.refs_in, a.refs, a.pages, s);
-        if (e != hipSuccess) return e;
+    if (plan_alone(a.batch, a.width, a.pages)) {
+        hipLaunchKernelGGL(evict_alone_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
+    } else {
+        if (a.refs != a.refs_in) {
+            const hipError_t e = copy_words(a.refs_in, a.refs, a.pages, s);
+            if (e != hipSuccess) return e;
+        }
+        hipLaunchKernelGGL(evict_rows_kernel, dim3(static_cast<unsigned>((a.batch + 3) / 4)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(evict_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
     }
-    hipLaunchKernelGGL(evict_rows_kernel, dim3(static_cast<unsigned>((a.batch + 3) / 4)), dim3(256), 0, s, a);
-    hipLaunchKernelGGL(evict_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
     hipLaunchKernelGGL(evict_move_kernel, dim3(static_cast<unsigned>(a.layers * a.batch * a.kv_heads)),
                        dim3(kEvictThreads), 0, s, a);
     return hipGetLastError();

@@ -141,5 +141,17 @@ __device__ __forceinline__ int32_t scan_needs(int32_t* need, int64_t batch, int3
     return base;
 }
 
+// Tables and pools up to which one workgroup does the whole plan, a thread a
+// sequence, a table entry and a page: a launch or two saved are worth more than
+// the other CUs.  Reserve and fork, alone against in several launches (us, with
+// the pages moved): 64 sequences of 14 entries over 1031 pages 6.2 and 12.5, 9.2
+// and 14.0; 128 of 113 over 8100 18.1 and 20.7, 14.2 and 18.9; 8 of 1876 16.2 and
+// 15.5, 13.6 and 32.3; 512 of 26 19.2 and 47, 16.5 and 30.
+constexpr int64_t kPlanAlone = 16384;
+
+bool plan_alone(int64_t batch, int64_t width, int64_t pages) {
+    return batch <= kPlanThreads && batch * width <= kPlanAlone && pages <= kPlanAlone;
+}
+
 }  // namespace
 }  // namespace popkv
