@@ -1210,9 +1210,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void chunk_weights_k
             off[i] = lse[2 * i];
             f[i] = scaled ? factors[2 * i] : make_float4(kScaleHigh, kScaleHigh, kScaleHigh, kScaleHigh);
         }
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const f32x16_t s = logits(n);
+        auto add = [&](int n, const f32x16_t& s) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = r0 + 8 * i + 4 * half;
@@ -1221,7 +1219,22 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void chunk_weights_k
                 sum[n] += seen(n, r + 2, exp2_fast(fmaf(s[4 * i + 2], f[i].z, -off[i].z)), off[i].z);
                 sum[n] += seen(n, r + 3, exp2_fast(fmaf(s[4 * i + 3], f[i].w, -off[i].w)), off[i].w);
             }
+        };
+        f32x16_t s = logits(0);
+#pragma unroll
+        for (int n = 1; n < N; ++n) {
+            __builtin_amdgcn_sched_barrier(0);
+            const f32x16_t next = logits(n);
+            add(n - 1, s);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {  // (a product, and a weight beside it)
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
+            }
+            s = next;
         }
+        add(N - 1, s);
     };
     const uint4* const queries = a.queries + base * (C::STORED * kWave) + lane;
     if (cached) {
