@@ -932,7 +932,7 @@ void carve_chunk(Carve& c, popkv::PagedChunk& a, int32_t dtype, int64_t batch, i
     const int64_t tiles = batch * kv_heads * p.row_blocks * p.shape;
     a.queries = c.take<uint4>(tiles * p.stored * 64);
     a.factors = c.take<float>(tiles * 32);
-    a.lse = c.take<float>(tiles * 32);
+    a.sums = c.take<float2>(tiles * 32);
 }
 
 }  // namespace

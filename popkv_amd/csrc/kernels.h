@@ -423,7 +423,8 @@ struct PagedChunk {
     // with weights, for every (sequence, KV head) row_blocks * row_waves times 32
     // rows: the query operands (plan.stored KB a tile), factors and sums
     uint4* queries;
-    float *factors, *lse;
+    float* factors;
+    float2* sums;
 };
 constexpr int kChunkStored16 = 18, kChunkStored32 = 42;  // KB of stored operands of 32 rows
 // How a call is cut: waves of 32 rows a workgroup (shape), blocks of so many rows a

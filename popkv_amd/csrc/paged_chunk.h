@@ -308,6 +308,13 @@ __device__ __forceinline__ void interleave() {
     }
 }
 
+// What a row's weights are 2^(logit - x) y with: its largest weights' logits less x lie
+// about zero, where a float's step is small.  (Rows past the last one weigh nothing.)
+constexpr float kBase = 8.0f;  // weights start at 2^kBase
+__device__ __forceinline__ float2 row_sums(float ref, float l, bool live) {
+    return live ? make_float2(ref + kBase, exp2_fast(kBase) / l) : make_float2(INFINITY, 0.0f);
+}
+
 // Sixteen neighbouring values of a row, times f.
 template <typename T>
 __device__ __forceinline__ void store16(T* p, const f32x16_t& x, float f) {
@@ -330,7 +337,7 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
     constexpr int R = 128 / G;
     constexpr int LOWS = R == 8 ? 2 : 1;
     constexpr int QTOP = 5;
-    constexpr float kBase = 8.0f, kNone = -3e38f, kFull = 65504.0f;
+    constexpr float kNone = -3e38f, kFull = 65504.0f;
     constexpr int PLANE = S::SUB * 8 * kFrag, BUF = C::PLANES * PLANE;
     constexpr int BUFS = S::WR == 8 && 2 * BUF <= 140 * 1024 ? 2 : 1;
     static_assert(BUF <= 150 * 1024);
@@ -420,7 +427,7 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
-        float ref = kNone, l = 0.0f;
+        float ref = kNone, l = 0.0f, lost = 0.0f;
         uint4 q[C::QPLANES][8];
 
         // Weights 2^(logit - ref) of 32 tokens from their products, as operands of the
@@ -448,6 +455,7 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                 mx = fmaxf(mx, lane_xor<32>(mx));
                 const float to = fmaxf(mx - kBase, ref), g = exp2_fast(ref - to);
                 l *= g;
+                lost *= g;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -455,7 +463,13 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                 ref = to;
                 sum = soft(s, f, out);
             }
-            l += sum;
+            if constexpr (EXACT) {  // (what a tile's sum loses goes to the next)
+                const float some = sum - lost, all_of = l + some;
+                lost = (all_of - l) - some;
+                l = all_of;
+            } else {
+                l += sum;
+            }
         };
         // A wave's one or two 32-token parts of a tile: the vector work of one beside the
         // matrix products of the other.
@@ -1087,7 +1101,7 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                 for (int i = 0; i < D; ++i) store16<T>(out + 16 * i, acc[i], f);
             }
             // (rows past the last one weigh nothing)
-            if (store_rows && half == 0) a.lse[row_tile * 32 + col] = r.live ? ref + __log2f(l) : INFINITY;
+            if (store_rows && half == 0) a.sums[row_tile * 32 + col] = row_sums(ref, l, r.live);
         } else {
             float* const state = a.partials + ((2 * static_cast<int64_t>(w_id) + (part.s == 0 ? 1 : 0)) * c.kv_heads + h) * S::STATE +
                                  wr * (4096 + 64);
@@ -1171,7 +1185,7 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(PagedChunk a, PagedVie
     }
     if (a.weights && i == 0 && half == 0) {
         const int64_t row_tile = (static_cast<int64_t>(b) * c.kv_heads + h) * a.row_blocks * S::WR + j * S::WR + wr;
-        a.lse[row_tile * 32 + col] = row < all ? m + __log2f(l) : INFINITY;
+        a.sums[row_tile * 32 + col] = row_sums(m, l, row < all);
     }
 }
 
@@ -1196,29 +1210,34 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void chunk_weights_k
     if (rows == 0 || (!cached && t0 >= rows)) return;
     const int all = rows * group;
     const int64_t base = (static_cast<int64_t>(b) * c.kv_heads + h) * (a.row_blocks * a.row_waves);
-    float sum[N];
+    float sum[N], lost[N];  // (thousands of rows: what a tile's sum loses goes to the next)
     bool there[N];
 #pragma unroll
-    for (int n = 0; n < N; ++n) sum[n] = 0.0f;
-    // a tile of 32 rows: its logits' products by `logits`, what weighs by `seen`
-    auto tile = [&](int r0, auto&& logits, auto&& seen, bool scaled) {
-        const float4* lse = reinterpret_cast<const float4*>(a.lse + (base * 32 + r0) + 4 * half);
+    for (int n = 0; n < N; ++n) sum[n] = lost[n] = 0.0f;
+    // a tile of 32 rows: its logits' products by `logits`, a row's weight added by `add_one`
+    auto tile = [&](int r0, auto&& logits, auto&& add_one, bool scaled) {
+        const float4* sums = reinterpret_cast<const float4*>(a.sums + (base * 32 + r0) + 4 * half);
         const float4* factors = reinterpret_cast<const float4*>(a.factors + (base * 32 + r0) + 4 * half);
-        float4 off[4], f[4];
+        float4 f[4], x[4][2];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            off[i] = lse[2 * i];
+            x[i][0] = sums[4 * i];
+            x[i][1] = sums[4 * i + 1];
             f[i] = scaled ? factors[2 * i] : make_float4(kScaleHigh, kScaleHigh, kScaleHigh, kScaleHigh);
         }
         auto add = [&](int n, const f32x16_t& s) {
+            float some = -lost[n];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = r0 + 8 * i + 4 * half;
-                sum[n] += seen(n, r, exp2_fast(fmaf(s[4 * i], f[i].x, -off[i].x)), off[i].x);
-                sum[n] += seen(n, r + 1, exp2_fast(fmaf(s[4 * i + 1], f[i].y, -off[i].y)), off[i].y);
-                sum[n] += seen(n, r + 2, exp2_fast(fmaf(s[4 * i + 2], f[i].z, -off[i].z)), off[i].z);
-                sum[n] += seen(n, r + 3, exp2_fast(fmaf(s[4 * i + 3], f[i].w, -off[i].w)), off[i].w);
+                some = add_one(some, n, r, exp2_fast(fmaf(s[4 * i], f[i].x, -x[i][0].x)), x[i][0].y);
+                some = add_one(some, n, r + 1, exp2_fast(fmaf(s[4 * i + 1], f[i].y, -x[i][0].z)), x[i][0].w);
+                some = add_one(some, n, r + 2, exp2_fast(fmaf(s[4 * i + 2], f[i].z, -x[i][1].x)), x[i][1].y);
+                some = add_one(some, n, r + 3, exp2_fast(fmaf(s[4 * i + 3], f[i].w, -x[i][1].z)), x[i][1].w);
             }
+            const float all_of = sum[n] + some;
+            lost[n] = (all_of - sum[n]) - some;
+            sum[n] = all_of;
         };
         f32x16_t s = logits(0);
 #pragma unroll
@@ -1296,14 +1315,15 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void chunk_weights_k
 #pragma unroll
                     for (int m = 0; m < LOWS; ++m) s = mfma_h(ql[m], low[n][m], s);
 #pragma unroll
-                    for (int st = 0; st < 8; ++st)
+                    // (the small products first: the sums round less)
+                    for (int kt = 1; kt >= 0; --kt)
 #pragma unroll
-                        for (int kt = 1; kt >= 0; --kt)
+                        for (int qt = C::QT - 1; qt >= 0; --qt)
 #pragma unroll
-                            for (int qt = C::QT - 1; qt >= 0; --qt) s = mfma_h(x[qt][st], k[n][kt][st], s);
+                            for (int st = 0; st < 8; ++st) s = mfma_h(x[qt][st], k[n][kt][st], s);
                     return s;
                 },
-                [&](int, int, float p, float) { return p; }, true);
+                [&](float some, int, int, float p, float g) { return fmaf(p, g, some); }, true);
         }
     } else {
         uint4 k[N][C::NT][8];
@@ -1356,9 +1376,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void chunk_weights_k
                             }
                     return s;
                 },
-                [&](int n, int r, float p, float off) {
-                    if (C::F32 && odd[n]) p = off == off ? 0.0f : off;
-                    return r >= (t0 + 32 * n + col) * group ? p : 0.0f;
+                [&](float some, int n, int r, float p, float g) {
+                    p *= g;
+                    if (C::F32 && odd[n]) p = g == g ? 0.0f : g;
+                    return some + (r >= (t0 + 32 * n + col) * group ? p : 0.0f);
                 },
                 false);
         }
