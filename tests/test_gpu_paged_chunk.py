@@ -286,6 +286,36 @@ def test_large_batches():
     assert ((got.cpu().double() - want).abs() <= allowed(want, torch.bfloat16, v, nv)).all()
 
 
+@pytest.mark.parametrize("kv_heads", (1, 300))
+def test_many_heads_and_long_chunks(kv_heads):
+    """More KV heads than CUs; a chunk of many tiles of rows in one group."""
+    lengths, new = ([90], [3]) if kv_heads == 300 else ([700], [1100])
+    cache, table, k, v, q, nk, nv = setup(lengths, new, kv_heads, 2, torch.bfloat16, page=32, seed=15)
+    want, gathered = attend(q, k, v, nk, nv, lengths, new)
+    w = torch.zeros((1, kv_heads, table.capacity), device=DEV)
+    for weights in (None, w):
+        got = paged.paged_chunk_attention(q, cache, 0, table, nk, nv, weights=weights)
+        assert ((got.cpu().double() - want).abs() <= allowed(want, torch.bfloat16, v, nv)).all()
+    total = lengths[0] + new[0]
+    assert ((w[:, :, :total].cpu().double() - gathered).abs() <= FP32 * (gathered + 0.01)).all()
+
+
+def test_weights_on_average_as_exact_as_float32():
+    """The norm of the weights' error beside that of plain float32 sums of dequantised
+    rows: one rounding more of each logit, and of each sum, at most."""
+    lengths, new = [2000], [64]
+    cache, table, k, v, q, nk, nv = setup(lengths, new, 2, 4, torch.bfloat16, seed=16)
+    _, gathered = attend(q, k, v, nk, nv, lengths, new)
+    w = torch.zeros((1, 2, table.capacity), device=DEV)
+    paged.paged_chunk_attention(q, cache, 0, table, nk, nv, weights=w)
+    keys = torch.cat((k[0, :, :2000], nk[0].cpu().double()), 1).float()
+    logits = q[0].cpu().float().reshape(2, 4 * 64, 128) @ keys.transpose(1, 2) / math.sqrt(128)
+    ahead = torch.arange(2064)[None] > 2000 + torch.arange(64)[:, None]
+    p = torch.softmax(logits.unflatten(1, (4, 64)).masked_fill(ahead, -math.inf), 3).sum((1, 2))
+    plain = (p.double() - gathered[0]).norm()
+    assert (w[0, :, :2064].cpu().double() - gathered[0]).norm() <= 2 * plain
+
+
 def test_no_rows():
     cache, table, _, _, q, nk, nv = setup([5], [1], 1, 1, torch.bfloat16)
     got = paged.paged_chunk_attention(q[:, :, :0], cache, 0, table, nk[:, :, :0], nv[:, :, :0])
@@ -452,6 +482,28 @@ def test_evict_pages_that_forks_share():
     status = torch.zeros(1, dtype=torch.int32, device=DEV)
     check_evict(cache, table, w, 150, 20, cut=(2,), status=status)
     assert int(status) == 4
+
+
+def test_evict_from_a_large_pool():
+    """Pools and tables past what one workgroup plans."""
+    cache, table, w = filled_pool([200 + i % 90 for i in range(40)], 1, page=32, layers=1, spare=17_000, seed=11)
+    for b in range(1, 40, 3):
+        held = table.table[b, :2].long()
+        table.refs[held] -= 1
+        table.table[b, :2] = table.table[b - 1, :2]
+        table.refs[table.table[b - 1, :2].long()] += 1
+    check_evict(cache, table, w.clone(), 230, 16)
+    check_evict(cache, table, w.clone(), 100, 16, out=table)
+
+
+def test_evict_to_nothing_and_reuse():
+    """Everything given back, and the pages taken again."""
+    cache, table, w = filled_pool([100, 40], 2, page=32, spare=0, seed=12)
+    new = check_evict(cache, table, w, 0, 5, out=table, weights_out=w)
+    assert not new.refs.any() and (new.table == -1).all() and not w.any()
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    paged.reserve_pages(new, 40, status=status, out=new)
+    assert int(status) == 0 and (new.table >= 0).sum() == 4
 
 
 def test_evict_missing_pages_and_counts_outside():
