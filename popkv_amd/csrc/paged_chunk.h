@@ -13,12 +13,12 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 constexpr int kFrag = 1024;                   // bytes of one operand of a 32 x 32 x 16 product
 
 __device__ __forceinline__ f32x16_t mfma_h(const uint4& a, const uint4& b, f32x16_t c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0,
-                                                  0);
+    const half8_t x = __builtin_bit_cast(half8_t, a), y = __builtin_bit_cast(half8_t, b);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
 }
 __device__ __forceinline__ f32x16_t mfma_b(const uint4& a, const uint4& b, f32x16_t c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
-                                                   0, 0);
+    const bf16x8_t x = __builtin_bit_cast(bf16x8_t, a), y = __builtin_bit_cast(bf16x8_t, b);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
 }
 
 // Two floats as N pairs of bf16 terms that add up to them (the lower ones zero
@@ -113,7 +113,7 @@ struct ChunkShape {
     static constexpr int WR = WR_, WT = WT_, W = WR * WT, THREADS = W * kWave;
     static constexpr int ROWS = 32 * WR;
     static constexpr int TILE = WT == 4 ? 128 : 64, SUB = TILE / 32;  // tokens of a tile
-    static constexpr int UNITS = 4 * TILE;                            // quarters of keys, or dwords of four tokens' values
+    static constexpr int UNITS = 4 * TILE;              // quarters of keys, or dwords of four tokens' values
     static constexpr bool ROLES = THREADS >= 2 * UNITS;               // half of the threads stage keys, half values
     static constexpr int PER = ROLES ? 1 : UNITS / THREADS;
     static constexpr int STATE = WR * (32 * 128 + 64);                // floats of a part's state
@@ -219,7 +219,8 @@ __device__ __forceinline__ int fresh_lane() {
 }
 
 // Weights of 32 tokens as operands of two products of 16 tokens each, in N terms of a
-// type (QK, PV: the products of an operand beside them).  SUM: their sum is the rounded ones' (two a step).
+// type (QK, PV: the products of an operand beside them).  SUM: their sum is the rounded
+// ones' (two a step).
 template <int N, bool SUM_, int QK_>
 struct HalfWeights {
     static constexpr bool SUM = SUM_;
@@ -233,7 +234,8 @@ struct HalfWeights {
             for (int j = 0; j < 4; ++j) {
                 const float p0 = p[8 * st + 2 * j], p1 = p[8 * st + 2 * j + 1];
                 w[j] = pack_half2(p0, p1);
-                rest[j] = pack_half2(p0 - static_cast<float>(as_half2(w[j])[0]), p1 - static_cast<float>(as_half2(w[j])[1]));
+                rest[j] = pack_half2(p0 - static_cast<float>(as_half2(w[j])[0]),
+                                     p1 - static_cast<float>(as_half2(w[j])[1]));
             }
             at[0][st] = make_uint4(w[0], w[1], w[2], w[3]);
             if constexpr (N == 2) at[1][st] = make_uint4(rest[0], rest[1], rest[2], rest[3]);
@@ -331,8 +333,43 @@ __device__ __forceinline__ void store16(T* p, const f32x16_t& x, float f) {
     }
 }
 
+// One pass over the tokens with each row's running reference and sum.  A workgroup has
+// a block of rows of one (sequence, KV head) and goes through its part's tiles: first
+// cached ones, dequantised once a workgroup into operands of the matrix instructions,
+// then the chunk's own.  Products stand transposed,
+//   S[token, row] = K q    P = 2^(S f - ref)    O[dim, row] += V P
+// so that a lane holds one row's logits of 16 tokens, which are, in their order, what
+// the second product takes from it: weights never leave the lane, and which token is
+// which place of an operand is settled where values are staged.  (C layout of 32 x 32
+// products: lane l holds column l % 32, rows 8 (i / 4) + 4 (l / 32) + i % 4; A and B:
+// lane l holds elements 8 (l / 32) .. + 7 of row / column l % 32.)
+// Cached keys: in fp16, low + c delta rounded once, for bf16 rows; EXACT, for fp16 and
+// fp32 rows and wherever weights are gathered, as (c - 8) times delta's upper seven and
+// lower four bits, which fp16 holds, and low and 8 delta by the queries' sums.
+// What is held in fewer bits than fp32, half a step each, and why:
+//   queries of cached tokens: scaled by a power of two a row, 16-bit ones exact down to
+//     2^-18 of the row's largest, fp32 ones two terms;
+//   keys of bf16 rows, 2^-11: exact ones are another plane and 17 products instead of 8;
+//   values, 2^-11, with 16-bit rows: fp32 ones are two terms;
+//   weights: bf16 rows fp16 on cached tokens and bf16 on new ones; fp16 rows two fp16
+//     terms; fp32 rows two fp16 and three bf16 terms.
+// Error of the results against 64 bits, norm over norm, beside plain float32 products of
+// dequantised rows: bf16 1.90e-3 and 1.66e-3 (its own rounding), fp16 2.7e-4 and 2.1e-4
+// (with values and weights in two terms each 2.1e-4, for 20 % of the time), fp32 1.2e-6
+// and 1.4e-6.
+// Eight waves of 32 rows, one workgroup a CU, where a sequence has the rows: dequantised
+// tiles are shared by 256 rows, two waves a SIMD, tiles staged one ahead into the other
+// half of LDS and their codes loaded two ahead, page entries three.  The vector work of
+// 32 tokens (16 exponentials a lane among it) stands beside the products of the next 32,
+// operands read four ahead: 2048 rows of 4 heads behind 30719 tokens 1295 us against
+// 1393 with one after the other.  Values masked where they are staged and not where they are
+// loaded (1210 against 1295): nothing waits for a load.  Bound by the vector
+// instructions, 270 a wave and tile of 64 tokens beside 32 products: 1.2 ms, 900 TFLOP/s,
+// where a product of 8192 reaches 1190 to 1280.
+// Fewer rows: waves share a tile's tokens instead (WT), and join by dims in LDS.
 template <typename T, int G, bool EXACT, typename S>
-__global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_chunk_kernel(PagedChunk a, PagedView c, int64_t max_tokens, int groups) {
+__global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 || (EXACT && S::WT == 4) ? 1 : 2)) void paged_chunk_kernel(
+    PagedChunk a, PagedView c, int64_t max_tokens, int groups) {
     using C = ChunkTypes<T, EXACT>;
     constexpr int R = 128 / G;
     constexpr int LOWS = R == 8 ? 2 : 1;
@@ -392,7 +429,6 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
         return reinterpret_cast<uint4*>(base + (token / 32 * 8 + 4 * (e & 1) + quarter) * kFrag +
                                         (e / 2 * 32 + token % 32) * 16);
     };
-    auto ld16 = [&](const unsigned char* p) { return *reinterpret_cast<const uint4*>(p); };
 
     __shared__ int4 s_items[kWave];
     ChunkWalk<S> walk(a, c, max_tokens, w_id, groups, s_items);
@@ -415,7 +451,8 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
             return Row{t, h * group + row - t * group, row0 + 32 * wr + k < all};
         };
         auto query = [&](const Row& r) {
-            return static_cast<const T*>(a.q) + b * a.q_bs + r.head * a.q_hs + static_cast<int64_t>(r.t) * a.q_ts + 64 * half;
+            return static_cast<const T*>(a.q) + b * a.q_bs + r.head * a.q_hs + static_cast<int64_t>(r.t) * a.q_ts +
+                   64 * half;
         };
         // what the second pass reads of these rows: the query operands of both kinds of
         // tokens, their factors, their sums
@@ -969,7 +1006,8 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
             };
             // (of the wave's rows)
             const int t_first = __builtin_amdgcn_readfirstlane(t_row), t_last = __builtin_amdgcn_readlane(t_row, 31);
-            using Weights = std::conditional_t<C::F16, HalfWeights<C::PT, false, 1>, Bf16Weights<C::PT, C::PT == 1 && !EXACT, 1>>;
+            using Weights = std::conditional_t<C::F16, HalfWeights<C::PT, false, 1>,
+                                               Bf16Weights<C::PT, C::PT == 1 && !EXACT, 1>>;
             bool odd = false;
             auto fold = [&](int tile, int buf) {
                 const unsigned char* const s_k = s_mem + buf * BUF;
@@ -1078,7 +1116,8 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
                 float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (int n = 0; n < S::WT; ++n) {
-                    const float4 y = *reinterpret_cast<const float4*>(states + ((n * S::WR + wr) * 16 + wt * 4 * D + i) * 256 + lane * 4);
+                    const float4 y = *reinterpret_cast<const float4*>(
+                        states + ((n * S::WR + wr) * 16 + wt * 4 * D + i) * 256 + lane * 4);
                     x.x = fmaf(f[n], y.x, x.x);
                     x.y = fmaf(f[n], y.y, x.y);
                     x.z = fmaf(f[n], y.z, x.z);
@@ -1103,12 +1142,13 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
             // (rows past the last one weigh nothing)
             if (store_rows && half == 0) a.sums[row_tile * 32 + col] = row_sums(ref, l, r.live);
         } else {
-            float* const state = a.partials + ((2 * static_cast<int64_t>(w_id) + (part.s == 0 ? 1 : 0)) * c.kv_heads + h) * S::STATE +
-                                 wr * (4096 + 64);
+            const int64_t place = 2 * static_cast<int64_t>(w_id) + (part.s == 0 ? 1 : 0);
+            float* const state = a.partials + (place * c.kv_heads + h) * S::STATE + wr * (4096 + 64);
 #pragma unroll
             for (int i = 0; i < 4 * D; ++i)
                 *reinterpret_cast<float4*>(state + ((4 * D * wt + i) * kWave + lane) * 4) = make_float4(
-                    acc[i / 4][4 * (i % 4)], acc[i / 4][4 * (i % 4) + 1], acc[i / 4][4 * (i % 4) + 2], acc[i / 4][4 * (i % 4) + 3]);
+                    acc[i / 4][4 * (i % 4)], acc[i / 4][4 * (i % 4) + 1], acc[i / 4][4 * (i % 4) + 2],
+                    acc[i / 4][4 * (i % 4) + 3]);
             if (half == 0 && wt == 0) {
                 state[4096 + col] = ref;
                 state[4096 + 32 + col] = l;
@@ -1118,7 +1158,10 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 ? 1 : 2)) void paged_ch
     }
 }
 
-// Tiles of rows in several parts: a wave for 16 of each half's 64 dims.
+// Blocks of rows in several parts: a wave for 16 of each half's 64 dims of 32 rows.  A
+// launch of its own: the parts' states are up to 34 MB, which one workgroup a block
+// would read too slowly.  Bound by its chain of reads (sizes, part, states), 5 us, and for
+// 256 parts of 256 rows by the states, 17 us.
 template <typename T, typename S>
 __global__ __launch_bounds__(256) void chunk_merge_kernel(PagedChunk a, PagedView c, int64_t max_tokens) {
     const int h = blockIdx.y, b = blockIdx.z;
@@ -1180,8 +1223,8 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(PagedChunk a, PagedVie
     if (row < all) {
         const int t_row = static_cast<int>(row / group);
         const int head = h * group + static_cast<int>(row - static_cast<int64_t>(t_row) * group);
-        store16<T>(static_cast<T*>(a.out) + b * a.o_bs + head * a.o_hs + static_cast<int64_t>(t_row) * a.o_ts + 64 * half + 16 * i,
-                   acc, 1.0f / l);
+        T* const out = static_cast<T*>(a.out) + b * a.o_bs + head * a.o_hs + static_cast<int64_t>(t_row) * a.o_ts;
+        store16<T>(out + 64 * half + 16 * i, acc, 1.0f / l);
     }
     if (a.weights && i == 0 && half == 0) {
         const int64_t row_tile = (static_cast<int64_t>(b) * c.kv_heads + h) * a.row_blocks * S::WR + j * S::WR + wr;
@@ -1192,7 +1235,12 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(PagedChunk a, PagedVie
 // The attention weights of N times 32 tokens of a KV head a wave, from the logits once
 // more and the rows' sums: keys stay in registers, as the first pass has them, and
 // every row's operands pass once.  Rows stand in the products' rows, so that a token's
-// weights lie in one lane's registers and that of the other half.
+// weights lie in one lane's registers and that of the other half: no atomics, and equal
+// bits from call to call.  Bound by the matrix instructions and the exponentials beside
+// them: 4092 rows of each of two fp16 sequences up to 9023 tokens, 249 us (282 without
+// the products of one part beside the weights of the other; operands through LDS for four
+// waves, in the place of each wave's own reads, 328); 16 decode steps up to 4200
+// tokens by the keys' dequantisation, 18 us.
 template <typename T, int G, int N>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void chunk_weights_kernel(PagedChunk a, PagedView c,
                                                                                      int64_t max_tokens) {
@@ -1333,7 +1381,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void chunk_weights_k
             const int token = t0 + 32 * n + col;
             there[n] = token < rows;
             odd[n] = false;
-            const T* k_row = static_cast<const T*>(a.k) + b * a.k_bs + h * a.k_hs + static_cast<int64_t>(min(token, rows - 1)) * a.k_ts;
+            const T* k_row =
+                static_cast<const T*>(a.k) + b * a.k_bs + h * a.k_hs + static_cast<int64_t>(min(token, rows - 1)) * a.k_ts;
 #pragma unroll
             for (int s = 0; s < 8; ++s) {
                 Raw8<T> raw;

@@ -15,22 +15,31 @@ hipError_t launch_paged_chunk_f32(const PagedChunk& a, const PagedView& c, int64
 namespace {
 
 constexpr int kChunkCus = 256;
+// Fewest tiles of a workgroup, and what a block of rows costs beside its tiles: its
+// queries, first reads, state or output.
+constexpr int kLeastTiles = 4, kBlockCost = 2;
 int64_t ceil_of(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace
 
+// As many rows a workgroup as there are, up to 256 (fp32 128: two terms of everything
+// fill its registers), which share a tile's dequantisation.  Two workgroups a CU where
+// their LDS allows it (eight verifications of 6 tokens behind up to 8201 38 us, with one a
+// CU 40), and no more than fit at once (the first pass of 16 decode steps with weights,
+// whose LDS holds one, 41 us, in two rounds 51).
 ChunkPlan paged_chunk_plan(int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t rows, int64_t max_tokens,
                            bool weights) {
     ChunkPlan p{};
-    const int64_t all = rows * (q_heads / kv_heads);
     const bool f32 = dtype == POPKV_DTYPE_F32;
+    const int64_t all = rows * (q_heads / kv_heads);
     p.shape = all <= 32 && !f32 ? 1 : all <= 64 ? 2 : all <= 128 || f32 ? 4 : 8;
     p.row_blocks = ceil_of(all, 32 * p.shape);
-    p.least = 4;
-    p.item_cost = 2;
-    const int tile = p.shape == 1 ? 128 : 64, at_once = p.shape == 8 || f32 || (p.shape == 1 && (weights || dtype != POPKV_DTYPE_BF16)) ? 1 : 2;
+    p.least = kLeastTiles;
+    p.item_cost = kBlockCost;
+    const bool alone = p.shape == 8 || f32 || (p.shape == 1 && (weights || dtype != POPKV_DTYPE_BF16));
+    const int64_t tile = p.shape == 1 ? 128 : 64;
     const int64_t tiles = ceil_of(max_tokens, tile) + ceil_of(rows, tile) + p.item_cost;
-    const int64_t target = ceil_of(kChunkCus * at_once, kv_heads);
+    const int64_t target = ceil_of(kChunkCus * (alone ? 1 : 2), kv_heads);
     const int64_t most = ceil_of(batch * p.row_blocks * tiles, p.least);
     p.groups = static_cast<int>(most < target ? most : target);
     p.states = p.groups > 1 ? 2 * static_cast<int64_t>(p.groups) * kv_heads * p.shape * (32 * 128 + 64) : 0;

@@ -475,7 +475,7 @@ def paged_indexed_attention(q: torch.Tensor, cache: PagedKVCache, layer: int, pa
 def allocate_token_weights(cache: PagedKVCache, pages: PageTable) -> torch.Tensor:
     """What tokens have gathered, nothing yet: float32 [layers, B, KVH,
     ``pages.capacity``] for ``paged_chunk_attention`` and ``evict_tokens``.  After
-    ``fork_sequences`` the children's are ``weights[:, parents]``."""
+    ``fork_sequences`` the children's are ``weights[:, parents]`` (zero for -1)."""
     return torch.zeros((cache.layers, pages.batch, cache.kv_heads, pages.capacity), dtype=torch.float32,
                        device=cache.codes.device)
 
@@ -531,7 +531,8 @@ def paged_chunk_attention(q: torch.Tensor, cache: PagedKVCache, layer: int, page
     ``weights`` (contiguous float32 [B, KVH, ``pages.capacity``], a layer of
     ``allocate_token_weights``): every token's attention weight, summed over the rows
     and the query heads of its KV head, is added to its place, token t of the chunk at
-    ``counts[b] + t``.
+    ``counts[b] + t``.  What tokens that are taken back (``advance`` of a negative number)
+    gathered stays at their places: clear those.
 
     ``max_tokens`` and ``workspace`` as for ``paged_attention_step``; ``out`` shares
     no memory with the operands."""
@@ -614,8 +615,8 @@ def evict_tokens(cache: PagedKVCache, pages: PageTable, weights: torch.Tensor, k
     if weights_out is not None and weights_out.data_ptr() != weights.data_ptr() and _overlap(weights_out, weights):
         raise ValueError("weights_out must be weights or not overlap them")
     new = _new_table(pages, out)
-    dev = _on_device(cache.codes, cache.scales, pages.table, pages.counts, pages.refs, weights, weights_out, keeps, status,
-                     new.table, new.counts, new.refs)
+    dev = _on_device(cache.codes, cache.scales, pages.table, pages.counts, pages.refs, weights, weights_out, keeps,
+                     status, new.table, new.counts, new.refs)
     moved = torch.empty_like(weights) if weights_out is None else weights_out
     kept = torch.empty((*want[:3], keep), dtype=torch.int32, device=dev)
     if keeps is not None:
