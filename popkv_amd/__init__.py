@@ -16,7 +16,8 @@ and beside it, without a counterpart in the reference,
 
 * ``popkv_amd.batch``           decode of sequences of different lengths
 * ``popkv_amd.paged``           a paged 4-bit K/V cache for batched decode: write,
-                                attention, forks, compaction
+                                attention (a token or a chunk a sequence), forks,
+                                compaction, eviction
 * ``popkv_amd.wire``            packed caches as bytes
 """
 from __future__ import annotations

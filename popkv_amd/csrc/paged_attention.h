@@ -1,5 +1,6 @@
 // Device pieces shared by the attention kernels of the paged 4-bit K/V cache
-// (paged_dense.hip, paged_indexed.hip).  Both split a row's tokens among
+// (paged_dense.hip, paged_indexed.hip; paged_chunk.h takes the scale and the
+// codes).  The first two split a row's tokens among
 // workgroups that each leave an online-softmax state (m, l, acc[128]), base-2
 // exponents; the last workgroup of a row merges them in the same launch (the
 // hand-off rule stands in attention_common.h).  The current token's K/V, not

@@ -1237,10 +1237,10 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(PagedChunk a, PagedVie
 // every row's operands pass once.  Rows stand in the products' rows, so that a token's
 // weights lie in one lane's registers and that of the other half: no atomics, and equal
 // bits from call to call.  Bound by the matrix instructions and the exponentials beside
-// them: 4092 rows of each of two fp16 sequences up to 9023 tokens, 249 us (282 without
-// the products of one part beside the weights of the other; operands through LDS for four
-// waves, in the place of each wave's own reads, 328); 16 decode steps up to 4200
-// tokens by the keys' dequantisation, 18 us.
+// them: up to 4092 rows of each of two fp16 sequences up to 9023 tokens, 294 us (with sums
+// not compensated 249, then 282 without the products of one part beside the weights of the
+// other, and 328 with operands through LDS for four waves in the place of each wave's own
+// reads); 16 decode steps up to 4200 tokens by the keys' dequantisation, 19 us.
 template <typename T, int G, int N>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void chunk_weights_kernel(PagedChunk a, PagedView c,
                                                                                      int64_t max_tokens) {
