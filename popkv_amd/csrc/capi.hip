@@ -1091,7 +1091,8 @@ int popkv_paged_chunk_attention(const void* queries, int32_t dtype, int64_t q_ba
     if (q_heads <= 0 || q_heads > 65535 || q_heads % kv_heads != 0)
         return fail(POPKV_ERR_INVALID, "query heads must be a positive multiple of the KV heads");
     if (max_tokens < 0 || max_tokens > (int64_t{1} << 30)) return fail(POPKV_ERR_TOKENS, "invalid token count");
-    if (rows < 0 || rows * q_heads > (int64_t{1} << 30)) return fail(POPKV_ERR_INVALID, "bad row count");
+    // (a merge has 256 threads for 32 rows of a KV head, a grid fewer than 2^32 a dimension)
+    if (rows < 0 || rows * q_heads > (int64_t{1} << 28)) return fail(POPKV_ERR_INVALID, "bad row count");
     if (rows == 0) return POPKV_OK;  // (before the pointers: an empty tensor has none)
     if (!queries || !k || !v || !output || !workspace) return fail(POPKV_ERR_INVALID, "null pointer");
     if (weights && weight_stride <= 0) return fail(POPKV_ERR_INVALID, "bad weight stride");
@@ -1285,7 +1286,9 @@ int popkv_page_evict(void* codes, void* scales, int64_t layers, int64_t pages, i
     if (!refs_in || !table || !counts || !refs || !weights_in || !weights || (!kept && keep > 0) || !workspace)
         return fail(POPKV_ERR_INVALID, "null pointer");
     if (layers <= 0 || layers > 65535) return fail(POPKV_ERR_INVALID, "bad layer count");
-    if (layers * batch * kv_heads > 0x7fffffff) return fail(POPKV_ERR_UNSUPPORTED, "too many sequences and heads");
+    // (1024 threads for each, and a grid fewer than 2^32 a dimension: refused before the table is changed)
+    if (batch * kv_heads >= int64_t{1} << 22 || layers * batch * kv_heads > 0x7fffffff)
+        return fail(POPKV_ERR_UNSUPPORTED, "too many sequences and heads");
     if (weight_stride < width * page_tokens) return fail(POPKV_ERR_INVALID, "weights must cover the page table");
     if (width * page_tokens > (int64_t{1} << 30)) return fail(POPKV_ERR_UNSUPPORTED, "a page table row is too long");
     if (keep > width * page_tokens) return fail(POPKV_ERR_INVALID, "keep must fit the page table");

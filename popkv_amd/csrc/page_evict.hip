@@ -132,9 +132,9 @@ __global__ __launch_bounds__(kEvictThreads) void evict_move_kernel(PageEvict a) 
     __shared__ uint32_t s_pick[2];
     __shared__ uint32_t s_above[kEvictWaves], s_equal[kEvictWaves];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    const int64_t item = blockIdx.x;
-    const int h = static_cast<int>(item % a.kv_heads);
-    const int64_t b = item / a.kv_heads % a.batch, layer = item / a.kv_heads / a.batch;
+    const int64_t layer = blockIdx.y, item = layer * gridDim.x + blockIdx.x;
+    const int h = static_cast<int>(blockIdx.x) % a.kv_heads;
+    const int64_t b = static_cast<int>(blockIdx.x) / a.kv_heads;
     const float* w_in = a.weights_in + item * a.weight_stride;
     float* w_out = a.weights + item * a.weight_stride;
     int32_t* kept = a.kept + item * a.keep;
@@ -280,7 +280,7 @@ hipError_t launch_page_evict(const PageEvict& a, hipStream_t s) {
         hipLaunchKernelGGL(evict_rows_kernel, dim3(static_cast<unsigned>((a.batch + 3) / 4)), dim3(256), 0, s, a);
         hipLaunchKernelGGL(evict_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
     }
-    hipLaunchKernelGGL(evict_move_kernel, dim3(static_cast<unsigned>(a.layers * a.batch * a.kv_heads)),
+    hipLaunchKernelGGL(evict_move_kernel, dim3(static_cast<unsigned>(a.batch * a.kv_heads), static_cast<unsigned>(a.layers)),
                        dim3(kEvictThreads), 0, s, a);
     return hipGetLastError();
 }

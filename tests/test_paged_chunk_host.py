@@ -153,6 +153,7 @@ def test_c_chunk_refusals():
     refused(name, args, "token count", most=-1)
     for rows in (-1, 1 << 29):
         refused(name, args, "row count", rows=rows)
+    refused(name, args, "row count", rows=(1 << 25) + 1)
     refused(name, args, "workspace bytes", bytes=need - 1)
     # an empty chunk is done, whatever its pointers
     _native.call(name, *{**args, "rows": 0, "q": None, "out": None, "ws": None}.values())
@@ -177,6 +178,8 @@ def test_c_evict_refusals():
     refused(name, args, "fit the page table", keep=257)
     refused(name, args, "or none of them", refs_out=P)
     refused(name, args, "too many", layers=65535, batch=65535, width=1)
+    # a launch of so many heads would fail once the table is already the new one
+    refused(name, args, "too many", layers=1, batch=32768, kv_heads=128, width=1)
     refused(name, args, "workspace bytes", bytes=need - 1)
     refused(name, args, "16-byte", ws=P + 8)
     assert lib.popkv_page_evict_workspace_bytes(0, 4, 4) == 0
