@@ -333,6 +333,30 @@ __device__ __forceinline__ void store16(T* p, const f32x16_t& x, float f) {
     }
 }
 
+// 4 N of them.
+template <typename T, int N>
+__device__ __forceinline__ void store4s(T* p, const float4 (&x)[N], float f) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            *reinterpret_cast<float4*>(p + 4 * k) = make_float4(x[k].x * f, x[k].y * f, x[k].z * f, x[k].w * f);
+    } else {
+        uint32_t w[2 * N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            w[2 * k] = pack2<T>(x[k].x * f, x[k].y * f);
+            w[2 * k + 1] = pack2<T>(x[k].z * f, x[k].w * f);
+        }
+        if constexpr (N == 1) {
+            *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 2 * N; k += 4)
+                *reinterpret_cast<uint4*>(p + 2 * k) = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+        }
+    }
+}
+
 // One pass over the tokens with each row's running reference and sum.  A workgroup has
 // a block of rows of one (sequence, KV head) and goes through its part's tiles: first
 // cached ones, dequantised once a workgroup into operands of the matrix instructions,
@@ -1158,14 +1182,19 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 || (EXACT && S::WT == 4
     }
 }
 
-// Blocks of rows in several parts: a wave for 16 of each half's 64 dims of 32 rows.  A
+// Blocks of rows in several parts: a wave for 4 N of each half's 64 dims of 32 rows.  A
 // launch of its own: the parts' states are up to 34 MB, which one workgroup a block
 // would read too slowly.  Bound by its chain of reads (sizes, part, states), 5 us, and for
-// 256 parts of 256 rows by the states, 17 us.
-template <typename T, typename S>
+// 256 parts of 256 rows by the states, 14 us.  Few tiles of rows have many parts each: then
+// a wave has 4 dims and 16 parts on their way (64 tiles of 8 to 13 parts 9.5 us, with 16
+// dims 11.4; of 32 parts 14.2 and 17.7; 288 tiles 6.2 both ways).
+constexpr int kFewTiles = 256;
+template <typename T, typename S, int N>
 __global__ __launch_bounds__(256) void chunk_merge_kernel(PagedChunk a, PagedView c, int64_t max_tokens) {
+    constexpr int PIECES = 4 / N;
     const int h = blockIdx.y, b = blockIdx.z;
-    const int j = blockIdx.x / S::WR, wr = blockIdx.x % S::WR;
+    const int piece = blockIdx.x % PIECES, block = blockIdx.x / PIECES;
+    const int j = block / S::WR, wr = block % S::WR;
     const int lane = threadIdx.x & (kWave - 1), col = lane & 31, half = lane >> 5;
     const int i = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int group = a.q_heads / c.kv_heads;
@@ -1179,13 +1208,13 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(PagedChunk a, PagedVie
         return a.partials + (place * c.kv_heads + h) * S::STATE + wr * (4096 + 64);
     };
     float m = -INFINITY, l = 0.0f;
-    f32x16_t acc;
+    float4 acc[N];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) acc[k] = 0.0f;
-    // (parts on their way at once: four, eight where there are more)
+    for (int k = 0; k < N; ++k) acc[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    // (parts on their way at once: four, where there are more eight of 16 dims or 16 of 4)
     auto fold = [&](auto ahead, int s0) {
         constexpr int AHEAD = decltype(ahead)::value;
-        float4 y[AHEAD][4];
+        float4 y[AHEAD][N];
         float pm[AHEAD], pl[AHEAD], mx = m;
 #pragma unroll
         for (int n = 0; n < AHEAD; ++n) {
@@ -1193,40 +1222,42 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(PagedChunk a, PagedVie
             pm[n] = p[4096 + col];
             pl[n] = p[4096 + 32 + col];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) y[n][k] = *reinterpret_cast<const float4*>(p + ((4 * i + k) * kWave + lane) * 4);
+            for (int k = 0; k < N; ++k)
+                y[n][k] = *reinterpret_cast<const float4*>(p + ((4 * i + N * piece + k) * kWave + lane) * 4);
         }
 #pragma unroll
         for (int n = 0; n < AHEAD; ++n) mx = fmaxf(mx, pm[n]);
         const float g = m == -INFINITY ? 0.0f : exp2_fast(m - mx);
         l *= g;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) acc[k] *= g;
+        for (int k = 0; k < N; ++k) acc[k] = make_float4(acc[k].x * g, acc[k].y * g, acc[k].z * g, acc[k].w * g);
 #pragma unroll
         for (int n = 0; n < AHEAD; ++n) {
             if (s0 + n >= parts.y) break;
             const float f = exp2_fast(pm[n] - mx);
             l = fmaf(f, pl[n], l);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                acc[4 * k] = fmaf(f, y[n][k].x, acc[4 * k]);
-                acc[4 * k + 1] = fmaf(f, y[n][k].y, acc[4 * k + 1]);
-                acc[4 * k + 2] = fmaf(f, y[n][k].z, acc[4 * k + 2]);
-                acc[4 * k + 3] = fmaf(f, y[n][k].w, acc[4 * k + 3]);
+            for (int k = 0; k < N; ++k) {
+                acc[k].x = fmaf(f, y[n][k].x, acc[k].x);
+                acc[k].y = fmaf(f, y[n][k].y, acc[k].y);
+                acc[k].z = fmaf(f, y[n][k].z, acc[k].z);
+                acc[k].w = fmaf(f, y[n][k].w, acc[k].w);
             }
         }
         m = mx;
     };
+    constexpr int MOST = N == 4 ? 8 : 16;
     if (parts.y <= 4)
         fold(std::integral_constant<int, 4>{}, 0);
     else
-        for (int s0 = 0; s0 < parts.y; s0 += 8) fold(std::integral_constant<int, 8>{}, s0);
+        for (int s0 = 0; s0 < parts.y; s0 += MOST) fold(std::integral_constant<int, MOST>{}, s0);
     if (row < all) {
         const int t_row = static_cast<int>(row / group);
         const int head = h * group + static_cast<int>(row - static_cast<int64_t>(t_row) * group);
         T* const out = static_cast<T*>(a.out) + b * a.o_bs + head * a.o_hs + static_cast<int64_t>(t_row) * a.o_ts;
-        store16<T>(out + 64 * half + 16 * i, acc, 1.0f / l);
+        store4s<T, N>(out + 64 * half + 16 * i + 4 * N * piece, acc, 1.0f / l);
     }
-    if (a.weights && i == 0 && half == 0) {
+    if (a.weights && i == 0 && half == 0 && piece == 0) {
         const int64_t row_tile = (static_cast<int64_t>(b) * c.kv_heads + h) * a.row_blocks * S::WR + j * S::WR + wr;
         a.sums[row_tile * 32 + col] = row_sums(m, l, row < all);
     }
@@ -1448,9 +1479,14 @@ hipError_t launch_chunk_s(const PagedChunk& a, const PagedView& c, int64_t max_t
                        dim3(S::THREADS), 0, stream, a, c, max_tokens, a.groups);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.groups > 1) {
-        hipLaunchKernelGGL((chunk_merge_kernel<T, S>), dim3(static_cast<unsigned>(a.row_blocks * S::WR), c.kv_heads, c.batch),
-                           dim3(256), 0, stream, a, c, max_tokens);
-        e = hipGetLastError();
+        const int64_t tiles = a.row_blocks * S::WR;
+        auto launch = [&](auto kernel, int64_t pieces) {
+            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles * pieces), c.kv_heads, c.batch), dim3(256), 0,
+                               stream, a, c, max_tokens);
+            return hipGetLastError();
+        };
+        e = tiles * c.kv_heads * c.batch <= kFewTiles ? launch(chunk_merge_kernel<T, S, 1>, 4)
+                                                      : launch(chunk_merge_kernel<T, S, 4>, 1);
     }
     return e;
 }
