@@ -1464,10 +1464,12 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void chunk_weights_k
                 false);
         }
     }
+    // (new tokens stand behind all cached ones, those past max_tokens among them)
+    const int64_t first = cached ? 0 : clamp_count(c.counts[b], c.width << c.page_log2);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         const float x = sum[n] + lane_xor<32>(sum[n]);
-        const int64_t at = static_cast<int64_t>(cached ? 0 : count) + t0 + 32 * n + col;
+        const int64_t at = first + t0 + 32 * n + col;
         if (half == 0 && there[n] && at < a.weight_stride)
             a.weights[(static_cast<int64_t>(b) * c.kv_heads + h) * a.weight_stride + at] += x;
     }
