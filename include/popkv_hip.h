@@ -516,9 +516,10 @@ int popkv_page_compact(void* codes, void* scales, int64_t layers, int64_t pages,
  * be weights_in), zero behind; kept int32 [layers, batch, KVH, keep] says where each
  * was (-1 past keeps[b], and for sequences that are not cut).  Pages behind are given
  * back, ones reserved ahead too.  A page of the front that has further holders is not
- * written: a free one takes its place.  A sequence for which the pool has none, or one
- * of whose tokens' pages is missing, stays as it was and sets status.  The input table is
- * spent. */
+ * written: a free one takes its place, lowest first, sequences in order.  Free are the
+ * pages that were free before the call, not those that it gives back.  A sequence that
+ * needs more than are left, or one of whose tokens' pages is missing, stays as it was
+ * and sets status; those behind it go on.  The input table is spent. */
 size_t popkv_page_evict_workspace_bytes(int64_t batch, int64_t width, int64_t pages);
 int popkv_page_evict(void* codes, void* scales, int64_t layers, int64_t pages, int64_t kv_heads, int32_t page_tokens,
                      int32_t dim_group_size, const int32_t* table_in, const int64_t* counts_in, const int32_t* refs_in,

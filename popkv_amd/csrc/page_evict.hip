@@ -53,8 +53,27 @@ __global__ __launch_bounds__(256) void evict_rows_kernel(PageEvict a) {
     if (b < a.batch) evict_row(a, b);
 }
 
+// Where there are fewer free pages than are needed: need[] (offsets that
+// scan_needs made) to offsets of the shares that still fit, in order, -1 for those
+// that do not.  By one wave, 64 sequences at a time.
+__device__ __forceinline__ void fit_needs(int32_t* need, int64_t batch, int32_t found, int lane) {
+    int32_t at = 0;
+    for (int64_t b0 = 0; b0 < batch; b0 += kWave) {
+        const int64_t b = b0 + lane;
+        const int32_t n = b < batch ? need[b + 1] - need[b] : 0;
+        int32_t mine = 0;
+        for (int i = 0; i < kWave; ++i) {
+            const int32_t x = __builtin_amdgcn_readlane(n, i);
+            const bool fits = x <= found - at;
+            if (i == lane) mine = fits ? at : -1;
+            at += fits ? x : 0;
+        }
+        if (b < batch) need[b] = mine;  // (the next 64 read theirs and those behind)
+    }
+}
+
 // Fresh pages handed out by one workgroup, lowest first, sequences in order; one
-// whose share does not fit stays as it was.
+// whose share does not fit in what is left stays as it was, and the next ones go on.
 __device__ __forceinline__ void evict_plan(const PageEvict& a, PageMap& map) {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int32_t total = scan_needs(a.need, a.batch, map.sh);
@@ -62,13 +81,14 @@ __device__ __forceinline__ void evict_plan(const PageEvict& a, PageMap& map) {
     if (total > 0)
         found = list_free(map, a.pages, static_cast<int32_t>(min<int64_t>(total, a.pages)), a.list,
                           [&](int64_t i) { return a.refs[i] != 0; });
+    if (total > found && wave == 0) fit_needs(a.need, a.batch, found, lane);
     __syncthreads();
     for (int64_t b = wave; b < a.batch; b += kPlanWaves) {
-        const int32_t at = a.need[b], end = a.need[b + 1];
+        const int32_t at = a.need[b];
         int32_t* row = a.table + b * a.width;
         const int32_t* old = a.old + b * a.width;
         int32_t cut = a.cut[b];
-        if (end > at && end > found) {
+        if (at < 0) {
             for (int64_t i = lane; i < a.width; i += kWave) row[i] = old[i];
             if (lane == 0) {
                 a.cut[b] = -1;

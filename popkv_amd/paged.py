@@ -590,9 +590,10 @@ def evict_tokens(cache: PagedKVCache, pages: PageTable, weights: torch.Tensor, k
     ``weights`` (float32 [layers, B, KVH, ``pages.capacity``]; NaN is the largest, of
     equal ones the first is kept), in their order at the front of the sequence; the
     pages behind are given back, reserved ones too.  A page of the front that a fork
-    shares is not written: a free one takes its place.  A sequence for which none is
-    free, or one of whose tokens' pages is missing, stays as it was and sets
-    ``status`` bit 4.
+    shares is not written: a free one takes its place.  Free are the pages that were
+    free before the call; those that it gives back serve the next one.  A sequence that
+    needs more than are left (the ones behind it go on), or one of whose tokens' pages
+    is missing, stays as it was and sets ``status`` bit 4.
 
     Returns the new page table (or ``out``, which may be ``pages``), the kept tokens'
     weights, zero behind them (or ``weights_out``, which may be ``weights``), and where

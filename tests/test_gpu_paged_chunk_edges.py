@@ -8,7 +8,7 @@ import torch
 
 from popkv_amd import paged
 
-from test_gpu_paged_chunk import DEV, DTYPES, FP32, allowed, attend, setup
+from test_gpu_paged_chunk import DEV, DTYPES, FP32, allowed, attend, check_evict, filled_pool, setup
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +37,39 @@ def test_weights_of_new_tokens_behind_a_bound_that_cuts(dtype):
     w.fill_(0.25)
     paged.paged_chunk_attention(q, cache, 0, table, nk, nv, tokens=torch.tensor(new, device=DEV), weights=w)
     assert (w[:, :, 40:] == 0.25).all()
+
+
+@pytest.mark.parametrize("batch,large", [(5, False), (5, True), (150, False), (150, True)])
+def test_evict_passes_over_shares_that_do_not_fit(batch, large):
+    """A sequence that needs more free pages than are left stays whole, and those behind it
+    still take theirs; in one workgroup's plan and in several launches'."""
+    left, cut = 4 if batch == 5 else 151, []  # (the last of 151 fits past the first 64 sequences)
+    cache, table, w = filled_pool([320 if batch == 5 else 130] * batch, 1, page=32, layers=1,
+                                  spare=17_000 if large else left, seed=32)
+    table.refs[torch.nonzero(table.refs == 0)[left:, 0]] = 3  # held elsewhere
+    shared = [5, 2, 0, 4, 1] if batch == 5 else [(7 * b) % 5 for b in range(batch)]
+    for b, n in enumerate(shared):
+        table.refs[table.table[b, :n].long()] = 2  # held elsewhere too
+    keep = 150 if batch == 5 else 100
+    stay = -(-keep // 32)
+    for b, n in enumerate(shared):
+        if min(n, stay) <= left:
+            left -= min(n, stay)
+            cut.append(b)
+    assert 0 < len(cut) < batch
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    check_evict(cache, table, w, keep, 20, cut=cut, status=status)
+    assert int(status) == 4
+
+
+def test_pages_given_back_serve_the_next_call():
+    """Free pages are those that were free before the call: what it gives back itself
+    lets a second call cut the sequences that the first had to leave."""
+    cache, table, w = filled_pool([320, 320], 2, page=32, spare=0, seed=33)
+    table.refs[table.table[0, :2].long()] = 2
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    check_evict(cache, table, w, 150, 20, cut=(1,), out=table, weights_out=w, status=status)
+    assert int(status) == 4
+    status.zero_()
+    check_evict(cache, table, w, 150, 20, cut=(0,), out=table, weights_out=w, status=status)
+    assert int(status) == 0 and table.counts.tolist() == [150, 150]
