@@ -21,17 +21,23 @@ __device__ __forceinline__ f32x16_t mfma_b(const uint4& a, const uint4& b, f32x1
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
 }
 
-// Two floats as N pairs of bf16 terms that add up to them (the lower ones zero
-// where a float is not finite).
+// Two floats as N pairs of bf16 terms that add up to them.  Of several terms the first
+// is held in bf16's range, which the largest floats round past; infinities and NaN then
+// stand in the others.
 typedef __bf16 bf16x2_raw __attribute__((ext_vector_type(2)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 template <int N>
 __device__ __forceinline__ void bf16_terms(float x, float y, uint32_t (&t)[N]) {
-    t[0] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{x, y}), bf16x2_raw));
+    f32x2_t held = {x, y};
+    if constexpr (N > 1) {
+        constexpr float kTop = 0x1.fep127f;
+        held = f32x2_t{__builtin_amdgcn_fmed3f(x, -kTop, kTop), __builtin_amdgcn_fmed3f(y, -kTop, kTop)};
+    }
+    t[0] = __builtin_bit_cast(uint32_t, __builtin_convertvector(held, bf16x2_raw));
 #pragma unroll
     for (int i = 1; i < N; ++i) {
-        x = i == 1 && (t[0] & 0x7f80u) == 0x7f80u ? 0.0f : x - __uint_as_float(t[i - 1] << 16);
-        y = i == 1 && (t[0] & 0x7f800000u) == 0x7f800000u ? 0.0f : y - __uint_as_float(t[i - 1] & 0xffff0000u);
+        x -= __uint_as_float(t[i - 1] << 16);
+        y -= __uint_as_float(t[i - 1] & 0xffff0000u);
         t[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{x, y}), bf16x2_raw));
     }
 }

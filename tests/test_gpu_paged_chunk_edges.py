@@ -3,11 +3,14 @@ behind the counts, elements at the end of a type's range, the norm of the errors
 token both ways, shares of free pages that do not fit, proposals that are rejected."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
 from popkv_amd import paged
 
+from test_gpu_paged import make
 from test_gpu_paged_chunk import DEV, DTYPES, FP32, allowed, attend, check_evict, filled_pool, setup
 
 pytestmark = pytest.mark.gpu
@@ -37,6 +40,35 @@ def test_weights_of_new_tokens_behind_a_bound_that_cuts(dtype):
     w.fill_(0.25)
     paged.paged_chunk_attention(q, cache, 0, table, nk, nv, tokens=torch.tensor(new, device=DEV), weights=w)
     assert (w[:, :, 40:] == 0.25).all()
+
+
+def test_float32_elements_near_the_largest():
+    """Finite elements that bf16 would round to infinity: a value that a row does not see
+    does not reach it, one of small weight adds what it is worth, and a key's product with
+    a small query element is a logit like any other."""
+    gen = torch.Generator().manual_seed(31)
+    big = torch.finfo(torch.float32).max
+    base = torch.randn(128, generator=gen)
+    cache, table = make([0], 1, max_tokens=64)
+    for rows, group in ((40, 1), (9, 2), (90, 4)):  # waves that share tokens, and that do not
+        q = base + 0.1 * torch.randn(1, group, rows, 128, generator=gen)
+        nk, nv = (torch.randn(1, 1, rows, 128, generator=gen) for _ in range(2))
+        nk[0, 0, 5] = -4 * base  # weights of e^-40 and less
+        nv[0, 0, 5, 3], nv[0, 0, 5, 70], nv[0, 0, 5, 100] = big, -big, 3.397e38
+        want, _ = attend(q, torch.zeros(1, 1, 0, 128, dtype=torch.float64), torch.zeros(1, 1, 0, 128, dtype=torch.float64),
+                         nk, nv, [0], [rows])
+        got = paged.paged_chunk_attention(q.to(DEV), cache, 0, table, nk.to(DEV), nv.to(DEV)).cpu().double()
+        # a weight's own error: 24 steps of sums up to 512, times 1 / sqrt(128)
+        assert ((got - want).abs() <= FP32 + 24 * 2.0 ** -14 / math.sqrt(128) * want.abs()).all()
+        assert got[:, :, :5].abs().max() < 10
+        nv = torch.randn(1, 1, rows, 128, generator=gen)
+        q[..., 0], nk[0, 0, 2, 0], nk[0, 0, 3, 0] = 2.0 ** -126, big, -big
+        want, _ = attend(q, torch.zeros(1, 1, 0, 128, dtype=torch.float64), torch.zeros(1, 1, 0, 128, dtype=torch.float64),
+                         nk, nv, [0], [rows])
+        w = torch.zeros(1, 1, table.capacity, device=DEV)
+        got = paged.paged_chunk_attention(q.to(DEV), cache, 0, table, nk.to(DEV), nv.to(DEV), weights=w).cpu().double()
+        assert ((got - want).abs() <= FP32 * 4).all()
+        assert w.isfinite().all()
 
 
 @pytest.mark.parametrize("batch,large", [(5, False), (5, True), (150, False), (150, True)])
