@@ -452,7 +452,8 @@ int popkv_paged_indexed_attention(const void* queries, int32_t dtype, const void
  * weights (float32 [batch, KVH, weight_stride], NULL: none): the attention weights
  * of every token, summed over the rows and the query heads of its KV head, are added
  * at the token's place, a chunk's token t at counts[b] + t (places past
- * weight_stride are left out).  Workspace: popkv_paged_chunk_attention_workspace_bytes()
+ * weight_stride are left out); rows of tokens that are not going to be kept add to the
+ * sums of those they see, so leave them out of tokens.  Workspace: popkv_paged_chunk_attention_workspace_bytes()
  * bytes (with weights != 0 for calls that gather them), 16-byte aligned, its first
  * 2^18 bytes zero on entry and left zero, as for popkv_paged_attention, which does
  * the work of a chunk of one token. */

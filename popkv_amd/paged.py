@@ -42,7 +42,10 @@ A prompt, or a part of one, is the same with ``paged_chunk_attention``, ``tokens
 of every sequence reserved, written and advanced; a bounded cache gives that call
 ``weights=w[layer]`` (one token is a chunk too) and calls
 ``evict_tokens(cache, pages, w, keep, out=pages, weights_out=w)`` once the
-sequences have grown past ``keep`` by some.
+sequences have grown past ``keep`` by some.  Proposed tokens are verified without
+``weights``, as many as were accepted advanced over, and before that gathered by a
+second call with ``tokens`` of them: a row adds to every token that it sees, also if
+its own token is rejected.
 
 A page that a sequence still fills is its alone; full pages may be shared.
 ``status`` (int32, on the device) collects bits where a call could not do all
@@ -531,8 +534,10 @@ def paged_chunk_attention(q: torch.Tensor, cache: PagedKVCache, layer: int, page
     ``weights`` (contiguous float32 [B, KVH, ``pages.capacity``], a layer of
     ``allocate_token_weights``): every token's attention weight, summed over the rows
     and the query heads of its KV head, is added to its place, token t of the chunk at
-    ``counts[b] + t``.  What tokens that are taken back (``advance`` of a negative number)
-    gathered stays at their places: clear those.
+    ``counts[b] + t``.  Every row counts that ``tokens`` holds, so give the accepted ones of
+    proposals alone.  What tokens that are taken back later (``advance`` of a negative
+    number) gathered stays at their places, which have to be cleared, and what their rows
+    added to older tokens stays in those sums.
 
     ``max_tokens`` and ``workspace`` as for ``paged_attention_step``; ``out`` shares
     no memory with the operands."""

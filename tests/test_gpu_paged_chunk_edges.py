@@ -8,9 +8,9 @@ import math
 import pytest
 import torch
 
-from popkv_amd import paged
+from popkv_amd import paged, popkv
 
-from test_gpu_paged import make
+from test_gpu_paged import dequantised, make
 from test_gpu_paged_chunk import DEV, DTYPES, FP32, allowed, attend, check_evict, filled_pool, setup
 
 pytestmark = pytest.mark.gpu
@@ -105,3 +105,43 @@ def test_pages_given_back_serve_the_next_call():
     status.zero_()
     check_evict(cache, table, w, 150, 20, cut=(0,), out=table, weights_out=w, status=status)
     assert int(status) == 0 and table.counts.tolist() == [150, 150]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_proposed_tokens_of_which_some_are_accepted(dtype):
+    """Proposals verified without gathering, then the accepted ones' weights gathered before
+    they are advanced over: the sums are those of the rows that stay, whatever was
+    proposed beside them, and the next round's tokens begin at zero."""
+    kvh, group, page = 2, 2, 32
+    cache = paged.allocate_paged_cache(1, 40, kvh, page_tokens=page, dim_group_size=32, device=DEV)
+    table = paged.PageTable.create(2, 256, cache)
+    w = paged.allocate_token_weights(cache, table)
+    ws, status = popkv.LayerStepWorkspace(), torch.zeros(1, dtype=torch.int32, device=DEV)
+    gen = torch.Generator().manual_seed(34)
+    held = [[torch.zeros(kvh, 0, 128, dtype=torch.float64) for _ in range(2)] for _ in range(2)]  # [b][k, v]
+    sums = [torch.zeros(kvh, 0, dtype=torch.float64) for _ in range(2)]
+    for proposed, accepted in (([40, 33], [40, 33]), ([6, 6], [2, 6]), ([6, 4], [1, 1]), ([6, 6], [6, 3])):
+        most = max(proposed)
+        bound = table.bound + most
+        piece = torch.tensor(proposed, device=DEV)
+        q, k, v = (torch.randn(2, h, most, 128, generator=gen).to(dtype).to(DEV) for h in (kvh * group, kvh, kvh))
+        paged.reserve_pages(table, piece, bound=bound, status=status, out=table)
+        out = paged.paged_chunk_attention(q, cache, 0, table, k, v, tokens=piece, workspace=ws)
+        paged.write_tokens(cache, 0, table, k, v, tokens=piece, status=status)
+        took = torch.tensor(accepted, device=DEV)
+        paged.paged_chunk_attention(q, cache, 0, table, k, v, tokens=took, weights=w[0], workspace=ws)
+        table.advance(took, bound=bound)
+        kq, vq = dequantised(k, 32), dequantised(v, 32)
+        for b, m in enumerate(accepted):
+            ck, cv = held[b]
+            n = ck.shape[1]
+            want, _ = attend(q[b:b + 1], ck[None], cv[None], k[b:b + 1], v[b:b + 1], [n], [proposed[b]])
+            _, add = attend(q[b:b + 1], ck[None], cv[None], k[b:b + 1], v[b:b + 1], [n], [m])
+            bound_b = allowed(want, dtype, cv[None], v[b:b + 1])
+            assert ((out[b:b + 1].cpu().double() - want).abs() <= bound_b).all()
+            sums[b] = torch.cat((sums[b], torch.zeros(kvh, m)), 1) + add[0, :, :n + m]
+            held[b] = [torch.cat((ck, kq[b, :, :m]), 1), torch.cat((cv, vq[b, :, :m]), 1)]
+            have = w[0, b].cpu().double()
+            assert ((have[:, :n + m] - sums[b]).abs() <= 2 * FP32 * (1 + sums[b])).all()
+            assert not have[:, n + m:].any()
+    assert int(status) == 0 and table.counts.tolist() == [x[0].shape[1] for x in held]
