@@ -456,7 +456,9 @@ int popkv_paged_indexed_attention(const void* queries, int32_t dtype, const void
  * sums of those they see, so leave them out of tokens.  Workspace: popkv_paged_chunk_attention_workspace_bytes()
  * bytes (with weights != 0 for calls that gather them), 16-byte aligned, its first
  * 2^18 bytes zero on entry and left zero, as for popkv_paged_attention, which does
- * the work of a chunk of one token. */
+ * the work of a chunk of one token.  With weights a bf16 result has other bits than
+ * without: cached keys then enter unrounded, else in fp16.  New values beyond 2^90 may
+ * leave the range of the fp32 sums. */
 size_t popkv_paged_chunk_attention_workspace_bytes(int32_t dtype, int64_t batch, int64_t q_heads, int64_t kv_heads,
                                                    int64_t rows, int64_t max_tokens, int32_t weights);
 int popkv_paged_chunk_attention(const void* queries, int32_t dtype, int64_t q_batch_stride, int64_t q_head_stride,

@@ -384,19 +384,28 @@ __device__ __forceinline__ void store4s(T* p, const float4 (&x)[N], float f) {
 //   weights: bf16 rows fp16 on cached tokens and bf16 on new ones; fp16 rows two fp16
 //     terms; fp32 rows two fp16 and three bf16 terms.
 // Error of the results against 64 bits, norm over norm, beside plain float32 products of
-// dequantised rows: bf16 1.90e-3 and 1.66e-3 (its own rounding), fp16 2.7e-4 and 2.1e-4
-// (with values and weights in two terms each 2.1e-4, for 20 % of the time), fp32 1.2e-6
-// and 1.4e-6.
+// dequantised rows: bf16 1.64e-3 to 1.72e-3 over cached tokens, 1.78e-3 to 2.06e-3 over new
+// ones (1.66e-3, its own rounding), fp16 2.7e-4 to 2.9e-4 and 2.0e-4 (2.1e-4; with cached
+// values in two terms too, for 20 % of the time), fp32 1.2e-6 at most (1.4e-6).  A bf16
+// row's result has other bits where weights are gathered, its keys then being exact.
+// Sums are fp32 of weights up to 2^16: they hold values up to about 2^90.
 // Eight waves of 32 rows, one workgroup a CU, where a sequence has the rows: dequantised
 // tiles are shared by 256 rows, two waves a SIMD, tiles staged one ahead into the other
 // half of LDS and their codes loaded two ahead, page entries three.  The vector work of
 // 32 tokens (16 exponentials a lane among it) stands beside the products of the next 32,
 // operands read four ahead: 2048 rows of 4 heads behind 30719 tokens 1295 us against
 // 1393 with one after the other.  Values masked where they are staged and not where they are
-// loaded (1210 against 1295): nothing waits for a load.  Bound by the vector
-// instructions, 270 a wave and tile of 64 tokens beside 32 products: 1.2 ms, 900 TFLOP/s,
-// where a product of 8192 reaches 1190 to 1280.
-// Fewer rows: waves share a tile's tokens instead (WT), and join by dims in LDS.
+// loaded (1210 against 1295): nothing waits for a load.  1.2 ms, 900 TFLOP/s, where a
+// product of 8192 reaches 1190 to 1280.  Bound by how far the vector instructions, about
+// 250 a wave and tile of 64 tokens, stand beside its 32 matrix ones with two waves a SIMD:
+// of a pass's 2.76M cycles the vector unit is active for 1.24M (the matrix instructions'
+// issue among them) and the matrix unit for 1.02M, and waves wait for 35 % of their time.
+// All 256 registers are taken: the eight-wave kernels spill 48 to 69 more (188 to 264 bytes
+// of scratch a lane), most outside the loops over tiles; the exact form reads some back
+// inside them.
+// Fewer rows: waves share a tile's tokens instead (WT), and join by dims in LDS.  (The
+// 32-row bf16 form spills 8 registers, the others none; fp32 rows and the exact 32-row form
+// take 350 to 440, one wave a SIMD.)
 template <typename T, int G, bool EXACT, typename S>
 __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 || (EXACT && S::WT == 4) ? 1 : 2)) void paged_chunk_kernel(
     PagedChunk a, PagedView c, int64_t max_tokens, int groups) {
@@ -1189,8 +1198,8 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 || (EXACT && S::WT == 4
 }
 
 // Blocks of rows in several parts: a wave for 4 N of each half's 64 dims of 32 rows.  A
-// launch of its own: the parts' states are up to 34 MB, which one workgroup a block
-// would read too slowly.  Bound by its chain of reads (sizes, part, states), 5 us, and for
+// launch of its own: the parts' states are up to 68 MB (34 MB where each workgroup has
+// one, 133 KB), which one workgroup a block would read too slowly.  Bound by its chain of reads (sizes, part, states), 5 us, and for
 // 256 parts of 256 rows by the states, 14 us.  Few tiles of rows have many parts each: then
 // a wave has 4 dims and 16 parts on their way (64 tiles of 8 to 13 parts 9.5 us, with 16
 // dims 11.4; of 32 parts 14.2 and 17.7; 288 tiles 6.2 both ways).
@@ -1529,7 +1538,10 @@ hipError_t launch_chunk_t(const PagedChunk& a, const PagedView& c, int64_t max_t
         hipLaunchKernelGGL(kernel, dim3(blocks, c.kv_heads, c.batch), dim3(256), 0, stream, a, c, max_tokens);
         return hipGetLastError();
     };
-    // two parts a wave where many rows pass, one where keys are most of the work
+    // Two parts a wave where many rows pass, one where keys are most of the work (us of a
+    // call with one and two: 132 rows behind 32703 tokens 120 and 113, 256 139 and 128, 512
+    // 244 and 215; 16 sequences of 32 rows behind 4200 92.7 and 93.6, 32 rows behind 32703 64
+    // both ways.  Two are ahead below 128 rows too: 64 rows 79.5 and 77.7, 128 99.5 and 94.3.)
     if constexpr (!std::is_same_v<T, float>)
         if (a.rows * (a.q_heads / c.kv_heads) > 128) return launch(chunk_weights_kernel<T, G, 2>, 64);
     return launch(chunk_weights_kernel<T, G, 1>, 32);

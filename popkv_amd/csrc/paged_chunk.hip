@@ -16,7 +16,12 @@ namespace {
 
 constexpr int kChunkCus = 256;
 // Fewest tiles of a workgroup, and what a block of rows costs beside its tiles: its
-// queries, first reads, state or output.
+// queries, first reads, state or output.  us by the fewest tiles, 1, 2, 4, 8: a
+// verification of 6 tokens behind 2000 19.7, 18.0, 21.0, 27.9, eight of up to 8201 33.8,
+// 33.9, 33.6, 39.4, small ragged fp32 chunks 40.5, 40.5, 44.2, 57.0; longer calls the same.
+// By the cost, 0, 1, 2, 4, 8: the eight verifications 36.9, 34.8, 33.7, 34.0, 33.7, 16
+// decode steps with weights 69.4, 63.7, 62.6, 65.3, 70.6, 64 verifications behind up to 900
+// 41.0, 37.4, 37.7, 40.2, 40.1, six ragged fp16 prompts 668, 641, 594, 539, 545.
 constexpr int kLeastTiles = 4, kBlockCost = 2;
 int64_t ceil_of(int64_t a, int64_t b) { return (a + b - 1) / b; }
 

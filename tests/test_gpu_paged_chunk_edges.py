@@ -230,7 +230,7 @@ def test_pages_given_back_serve_the_next_call():
 def test_proposed_tokens_of_which_some_are_accepted(dtype):
     """Proposals verified without gathering, then the accepted ones' weights gathered before
     they are advanced over: the sums are those of the rows that stay, whatever was
-    proposed beside them, and the next round's tokens begin at zero."""
+    proposed beside them, and the next proposals' places begin at zero."""
     kvh, group, page = 2, 2, 32
     cache = paged.allocate_paged_cache(1, 40, kvh, page_tokens=page, dim_group_size=32, device=DEV)
     table = paged.PageTable.create(2, 256, cache)
