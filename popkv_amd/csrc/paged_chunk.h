@@ -386,8 +386,8 @@ __device__ __forceinline__ void store4s(T* p, const float4 (&x)[N], float f) {
 // Error of the results against 64 bits, norm over norm, beside plain float32 products of
 // dequantised rows: bf16 1.64e-3 to 1.72e-3 over cached tokens, 1.78e-3 to 2.06e-3 over new
 // ones (1.66e-3, its own rounding), fp16 2.7e-4 to 2.9e-4 and 2.0e-4 (2.1e-4; with cached
-// values in two terms too, for 20 % of the time), fp32 1.2e-6 at most (1.4e-6).  A bf16
-// row's result has other bits where weights are gathered, its keys then being exact.
+// values in two terms too, for 20 % of the time), fp32 2e-7 to 2.4e-6 with the logits'
+// size (1.1e-6 to 2.7e-6 where keys have outlier channels).  A bf16 row's result has other bits where weights are gathered, its keys then being exact.
 // Sums are fp32 of weights up to 2^16: they hold values up to about 2^90.
 // Eight waves of 32 rows, one workgroup a CU, where a sequence has the rows: dequantised
 // tiles are shared by 256 rows, two waves a SIMD, tiles staged one ahead into the other
