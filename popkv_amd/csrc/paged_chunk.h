@@ -387,7 +387,8 @@ __device__ __forceinline__ void store4s(T* p, const float4 (&x)[N], float f) {
 // dequantised rows: bf16 1.64e-3 to 1.72e-3 over cached tokens, 1.78e-3 to 2.06e-3 over new
 // ones (1.66e-3, its own rounding), fp16 2.7e-4 to 2.9e-4 and 2.0e-4 (2.1e-4; with cached
 // values in two terms too, for 20 % of the time), fp32 2e-7 to 2.4e-6 with the logits'
-// size (1.1e-6 to 2.7e-6 where keys have outlier channels).  A bf16 row's result has other bits where weights are gathered, its keys then being exact.
+// size (1.1e-6 to 2.7e-6 where keys have outlier channels).  A bf16 row's result has
+// other bits where weights are gathered, its keys then being exact.
 // Sums are fp32 of weights up to 2^16: they hold values up to about 2^90.
 // Eight waves of 32 rows, one workgroup a CU, where a sequence has the rows: dequantised
 // tiles are shared by 256 rows, two waves a SIMD, tiles staged one ahead into the other
@@ -1199,8 +1200,9 @@ __global__ __launch_bounds__(S::THREADS, (sizeof(T) == 4 || (EXACT && S::WT == 4
 
 // Blocks of rows in several parts: a wave for 4 N of each half's 64 dims of 32 rows.  A
 // launch of its own: the parts' states are up to 68 MB (34 MB where each workgroup has
-// one, 133 KB), which one workgroup a block would read too slowly.  Bound by its chain of reads (sizes, part, states), 5 us, and for
-// 256 parts of 256 rows by the states, 14 us.  Few tiles of rows have many parts each: then
+// one, 133 KB), which one workgroup a block would read too slowly.  Bound by its chain of
+// reads (sizes, part, states), 5 us, and for 256 parts of 256 rows by the states, 14 us.
+// Few tiles of rows have many parts each: then
 // a wave has 4 dims and 16 parts on their way (64 tiles of 8 to 13 parts 9.5 us, with 16
 // dims 11.4; of 32 parts 14.2 and 17.7; 288 tiles 6.2 both ways).
 constexpr int kFewTiles = 256;

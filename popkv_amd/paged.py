@@ -544,9 +544,9 @@ def paged_chunk_attention(q: torch.Tensor, cache: PagedKVCache, layer: int, page
     (fp16 on cached tokens, bf16 on new ones) and, without ``weights``, cached keys, so that
     with ``weights`` a bf16 result has other bits.  The error's norm against float64: bf16
     1.6e-3 to 2.1e-3 (its own rounding 1.66e-3), fp16 2.0e-4 to 2.9e-4 (2.1e-4), float32 2e-7
-    to 2.5e-6 with the logits' size, as plain float32 products.  New values beyond 2^90 may leave the range of the float32 sums.  One token of
-    every sequence laid out as a decode step's, without ``tokens`` and ``weights``, is
-    ``paged_attention_step``, to the bit.
+    to 2.5e-6 with the logits' size, as plain float32 products.  New values beyond 2^90 may
+    leave the range of the float32 sums.  One token of every sequence laid out as a decode
+    step's, without ``tokens`` and ``weights``, is ``paged_attention_step``, to the bit.
 
     ``max_tokens`` and ``workspace`` as for ``paged_attention_step``.  The workspace takes up
     to 70 MB of partial states, and with ``weights`` 18 KB (float32 42 KB) more for every 32
